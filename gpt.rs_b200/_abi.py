@@ -160,6 +160,36 @@ class LatentAttention(ctypes.Structure):
                                      "lat_head_stride", "out_head_stride")] + [("page_bytes", ctypes.c_int64)]
 
 
+class QkRotation(ctypes.Structure):
+    """gptrs_qk_rotation."""
+    _fields_ = [(n, ctypes.c_int) for n in ("q_heads", "kv_heads", "dim", "rot_half", "pairs", "axes")] + [("eps", ctypes.c_float)] + \
+        [(n, ctypes.c_void_p) for n in ("d_q_gain", "d_k_gain", "d_cos", "d_sin")] + [("positions", ctypes.c_int64), ("d_axis_positions", ctypes.c_void_p),
+                                                                                      ("axis_stride", ctypes.c_int64), ("d_pair_axis", ctypes.c_void_p)]
+
+
+class Kv8Cache(ctypes.Structure):
+    """gptrs_kv8_cache."""
+    _fields_ = [(n, ctypes.c_int) for n in ("q_heads", "kv_heads", "dim", "window")] + [("scale", ctypes.c_float), ("tile_tokens", ctypes.c_int)] + \
+        [(n, ctypes.c_int64) for n in ("block_bytes", "page_bytes", "open_bytes")]
+
+
+class Kv8AppendStep(ctypes.Structure):
+    """gptrs_kv8_append_step."""
+    _fields_ = [("rotation", ctypes.c_void_p), ("d_qkv", ctypes.c_void_p), ("ld", ctypes.c_int64)] + \
+        [(n, ctypes.c_void_p) for n in ("d_positions", "d_slot", "d_run_first", "d_run_last", "d_page_table")] + \
+        [("max_pages", ctypes.c_int64), ("d_pool", ctypes.c_void_p), ("n_pages", ctypes.c_int64), ("d_open", ctypes.c_void_p), ("n_slots", ctypes.c_int64),
+         ("d_q", ctypes.c_void_p), ("d_status", ctypes.c_void_p), ("rows", ctypes.c_int64)]
+
+
+class Kv8AttentionStep(ctypes.Structure):
+    """gptrs_kv8_attention_step."""
+    _fields_ = [("d_q", ctypes.c_void_p), ("ldq", ctypes.c_int64), ("d_pool", ctypes.c_void_p), ("n_pages", ctypes.c_int64), ("d_open", ctypes.c_void_p),
+                ("n_slots", ctypes.c_int64), ("d_page_table", ctypes.c_void_p), ("max_pages", ctypes.c_int64)] + \
+        [(n, ctypes.c_void_p) for n in ("d_slot", "d_ctx_len", "d_length", "d_tile_row", "d_tile_rows")] + \
+        [("n_tiles", ctypes.c_int64), ("max_ctx_len", ctypes.c_int64), ("splits", ctypes.c_int), ("d_out", ctypes.c_void_p), ("d_scratch", ctypes.c_void_p),
+         ("scratch_bytes", ctypes.c_size_t), ("d_status", ctypes.c_void_p), ("rows", ctypes.c_int64)]
+
+
 def prototypes(header_text: str | None = None) -> dict[str, tuple[str, list[str]]]:
     """Returns {name: (return type, [parameter declarations])} for every exported function."""
     text = header_text if header_text is not None else HEADER.read_text()

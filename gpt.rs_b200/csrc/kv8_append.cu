@@ -1,0 +1,368 @@
+// Append to the 8-bit cache (norm and rotation of queries and keys on the way), and reading tokens back.
+//
+// gptrs_cuda_kv8_append: a CTA takes a tile of consecutive rows x one kv head with its query heads. A group of dim / 8 lanes works on a
+// head's row at a time (four rotated pairs per lane). Queries and the tile's angles are read once. Blocks are written whole: the CTA with the row
+// that completes a block reads the keys and values of its 16 tokens (again, where they lie in front of the tile; from the open rows, where they
+// came with an earlier call), takes the largest magnitude over the CTA, and puts the bytes in order in shared memory. What a run does to a
+// slot's open rows is done by one CTA per kv head, the one with the run's first row: first the block that the run continues is read and
+// written, then the rows of the run's last two blocks are stored, so that no other CTA reads what this one overwrites.
+#include "kv8_cache.cuh"
+#include "qk_rotate.cuh"
+
+namespace gptrs {
+namespace {
+
+constexpr int kThreads = 128;
+
+struct AppendParams {
+    QkRotation r;
+    int rotates;
+    const __nv_bfloat16* qkv;
+    long long ld;
+    const int *positions, *slot, *run_first, *run_last, *table;
+    long long max_pages, n_pages, n_slots;
+    unsigned char* pool;
+    __nv_bfloat16* open;
+    __nv_bfloat16* q;
+    int* status;
+    int rows, q_heads, kv_heads, group, tile_rows;
+};
+
+template <int kDim>
+struct Appender {
+    static constexpr int kLanes = kDim / 8;                  // of a head's row
+    static constexpr int kGroups = kThreads / kLanes;        // rows at a time
+    static constexpr int kPer = kKv8Tokens / kGroups;        // tokens of a block per lane group
+    const AppendParams& p;
+    int lane, in_group, ca, cb, head;                        // lane group, lane in it, first channels of its two runs
+
+    __device__ Appender(const AppendParams& params, int kv_head) : p(params), head(kv_head) {
+        lane = threadIdx.x / kLanes;
+        in_group = threadIdx.x % kLanes;
+        pair_channels<4>(p.r, 4 * in_group, &ca, &cb);
+    }
+    // norm and rotation of a query's or key's row in registers; all lanes of the warp call it
+    __device__ void turn(const float* gain, float (&a)[4], float (&b)[4], const float (&c)[4], const float (&s)[4]) const {
+        if (gain) {
+            const float rms = rsqrtf(lane_group_sum(square_sum(a, b), kLanes) / kDim + p.r.eps);
+            times_gain(gain, ca, cb, rms, a, b);
+        }
+        if (4 * in_group < p.r.rot_half) rotate_pairs(!p.r.neighbours, a, b, c, s);
+    }
+    __device__ void angles(int row, float (&c)[4], float (&s)[4]) const {
+        if (p.rotates) pair_angles<4>(p.r, row, p.positions[row], 4 * in_group, p.status, c, s);
+    }
+    // key (which 0) or value (1) of a row of the call, rounded to bf16; live: of this lane group (the others only take part in the sum)
+    __device__ void fetch(int row, int which, bool live, float (&a)[4], float (&b)[4]) const {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a[k] = b[k] = 0.f;
+        if (live) {
+            const __nv_bfloat16* src = p.qkv + row * p.ld + (long long)(p.q_heads + which * p.kv_heads + head) * kDim;
+            load_vec(src + ca, a);
+            load_vec(src + cb, b);
+        }
+        if (which == 0 && p.rotates) {
+            float c[4] = {}, s[4] = {};
+            if (live) angles(row, c, s);
+            turn(p.r.k_gain, a, b, c, s);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            a[k] = __bfloat162float(__float2bfloat16_rn(a[k]));
+            b[k] = __bfloat162float(__float2bfloat16_rn(b[k]));
+        }
+    }
+};
+
+// |x| as an ordered whole number that keeps infinities and NaN above all finite values
+__device__ __forceinline__ uint32_t magnitude(const float (&a)[4], const float (&b)[4], uint32_t m) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = max(m, max(__float_as_uint(a[k]) & 0x7fffffffu, __float_as_uint(b[k]) & 0x7fffffffu));
+    return m;
+}
+
+template <int kDim>
+__global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams p) {
+    using A = Appender<kDim>;
+    __shared__ __align__(16) unsigned char bytes[32 * kDim + 16];
+    __shared__ uint32_t largest[2][kThreads / 32];
+
+    pdl_launch_dependents();
+    pdl_wait();
+    const int kv_head = blockIdx.y, tid = threadIdx.x;
+    const int row0 = blockIdx.x * p.tile_rows, row_end = min(row0 + p.tile_rows, p.rows);
+    A w(p, kv_head);
+
+    // ---- queries: a lane group takes a row's heads one after the other (tiles) or the groups share the heads (few rows) -----------------
+    const int by_head = p.tile_rows < A::kGroups;
+    const int row_step = by_head ? 1 : A::kGroups, head_step = by_head ? A::kGroups : 1;
+    for (int r0 = row0; r0 < row_end; r0 += row_step) {
+        const int row = by_head ? r0 : r0 + w.lane;
+        const bool live_row = row < row_end && p.slot[row < row_end ? row : row0] >= 0;
+        float c[4] = {}, s[4] = {};
+        if (live_row) w.angles(row, c, s);
+        for (int h0 = 0; h0 < p.group; h0 += head_step) {
+            const int h = by_head ? h0 + w.lane : h0;
+            const bool live = live_row && h < p.group;
+            float a[4] = {}, b[4] = {};
+            if (live) {
+                const __nv_bfloat16* src = p.qkv + row * p.ld + (long long)(kv_head * p.group + h) * kDim;
+                load_vec(src + w.ca, a);
+                load_vec(src + w.cb, b);
+            }
+            if (p.rotates) w.turn(p.r.q_gain, a, b, c, s);
+            if (live) {
+                __nv_bfloat16* dst = p.q + ((long long)row * p.q_heads + kv_head * p.group + h) * kDim;
+                store_vec(dst + w.ca, a);
+                store_vec(dst + w.cb, b);
+            }
+        }
+    }
+
+    // ---- keys and values ----------------------------------------------------------------------------------------------------------------
+    // The block that row `last` completes, of whose tokens those from `first` on came with this call. All threads of the CTA.
+    auto write_block = [&](int last, int first, int slot, int position) {
+        const int block = position / kKv8Tokens;
+        const __nv_bfloat16* const old = p.open + (long long)slot * kv8_open_elems(p.kv_heads, kDim);
+        float x[2][A::kPer][2][4];
+        uint32_t m[2] = {0, 0};
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int j = 0; j < A::kPer; ++j) {
+                const int token = w.lane + j * A::kGroups, row = last - (kKv8Tokens - 1) + token;
+                w.fetch(max(row, 0), which, row >= first, x[which][j][0], x[which][j][1]);
+                if (row < first) {
+                    const __nv_bfloat16* src = old + kv8_open_at(block, p.kv_heads, kv_head, which, kDim) + token * kDim;
+                    load_vec(src + w.ca, x[which][j][0]);
+                    load_vec(src + w.cb, x[which][j][1]);
+                }
+                m[which] = magnitude(x[which][j][0], x[which][j][1], m[which]);
+            }
+        const int page = block < p.max_pages ? kv8_page(p.table, slot, p.max_pages, block, p.n_pages, p.status) : -1;
+        if (block >= p.max_pages && tid == 0) atomicExch(p.status, 2);
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            m[which] = __reduce_max_sync(0xffffffffu, m[which]);
+            if ((tid & 31) == 0) largest[which][tid >> 5] = m[which];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            uint32_t all = 0;
+#pragma unroll
+            for (int i = 0; i < kThreads / 32; ++i) all = max(all, largest[which][i]);
+            const bool finite = all < 0x7f800000u;
+            const float scale = finite ? fmaxf(__fdiv_rn(__uint_as_float(all), 127.f), kKv8MinScale) : __uint_as_float(0x7fc00000u);
+#pragma unroll
+            for (int j = 0; j < A::kPer; ++j) {
+                const int token = w.lane + j * A::kGroups;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int ch = half ? w.cb : w.ca;
+                    uint32_t u[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) u[k] = finite ? (uint32_t)(__float2int_rn(__fdiv_rn(x[which][j][half][k], scale)) + 128) : 128u;
+                    if (which == 0) {
+                        *reinterpret_cast<uint32_t*>(bytes + kv8_key_at(token, ch)) = u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24;
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) bytes[kv8_value_at(token, ch + k, kDim)] = (unsigned char)u[k];
+                    }
+                }
+            }
+            if (tid == 0) reinterpret_cast<float*>(bytes + 32 * kDim)[which] = scale;
+        }
+        if (tid < 2) reinterpret_cast<float*>(bytes + 32 * kDim)[2 + tid] = 0.f;
+        __syncthreads();
+        if (page >= 0) {
+            uint4* dst = reinterpret_cast<uint4*>(p.pool + ((long long)page * p.kv_heads + kv_head) * kv8_block_bytes(kDim));
+            for (int i = tid; i < 2 * kDim + 1; i += kThreads) dst[i] = reinterpret_cast<const uint4*>(bytes)[i];
+        }
+        __syncthreads();   // `bytes` and `largest` may be written again, and the open rows too
+    };
+
+    for (int row = row0; row < row_end; ++row) {
+        const int slot = p.slot[row], position = p.positions[row], first = p.run_first[row], last = p.run_last[row];
+        if (slot < 0) continue;
+        if (slot >= p.n_slots || first < 0 || first > row || last < row || last >= p.rows || position < row - first || position > 0x7fffffff - kKv8Tokens - (last - row)) {
+            if (tid == 0) atomicExch(p.status, 2);
+            continue;
+        }
+        const int to_end = kKv8Tokens - 1 - position % kKv8Tokens;         // rows until the block of this one is complete
+        const bool continued = (position - (row - first)) % kKv8Tokens != 0;   // the run's first block holds tokens of an earlier call
+        const bool in_first = row - first < kKv8Tokens && (position - (row - first)) / kKv8Tokens == position / kKv8Tokens;
+        if (to_end == 0 && !(continued && in_first)) write_block(row, first, slot, position);
+        if (row != first) continue;
+        if (continued && row + to_end <= last) write_block(row + to_end, first, slot, position);
+        // the rows of the run's last two blocks stay as they are
+        const int end = position + (last - row);
+        const int keep = max(position, (end / kKv8Tokens - 1) * kKv8Tokens);
+        __nv_bfloat16* const open = p.open + (long long)slot * kv8_open_elems(p.kv_heads, kDim);
+        for (int q0 = keep; q0 <= end; q0 += A::kGroups) {
+            const int at = q0 + w.lane;
+            const bool live = at <= end;
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                float a[4], b[4];
+                w.fetch(live ? row + (at - position) : row, which, live, a, b);
+                if (live) {
+                    __nv_bfloat16* dst = open + kv8_open_at(at / kKv8Tokens, p.kv_heads, kv_head, which, kDim) + at % kKv8Tokens * kDim;
+                    store_vec(dst + w.ca, a);
+                    store_vec(dst + w.cb, b);
+                }
+            }
+        }
+    }
+}
+
+struct GatherParams {
+    const unsigned char* pool;
+    const __nv_bfloat16* open;
+    const int *table, *slot, *positions, *length;
+    long long max_pages, n_pages, n_slots;
+    void *k, *v;
+    int* status;
+    int rows, kv_heads;
+};
+// eight channels of a token per thread; the CTAs of neighbouring tokens read the same lines
+template <int kDim, typename T>
+__global__ void __launch_bounds__(kThreads) kv8_gather_kernel(const GatherParams p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const long long item = (long long)blockIdx.x * kThreads + threadIdx.x;
+    const int per_row = p.kv_heads * (kDim / 8);
+    const long long row = item / per_row;
+    if (row >= p.rows) return;
+    const int head = (int)(item % per_row) / (kDim / 8), d0 = (int)(item % (kDim / 8)) * 8;
+    const int slot = p.slot[row], position = p.positions[row];
+    float k[8] = {}, v[8] = {};
+    bool found = slot >= 0 && slot < p.n_slots && position >= 0 && position < p.length[slot >= 0 && slot < p.n_slots ? slot : 0];
+    if (found) {
+        const int block = position / kKv8Tokens, token = position % kKv8Tokens;
+        if (block < p.length[slot] / kKv8Tokens) {
+            const int page = block < p.max_pages ? kv8_page(p.table, slot, p.max_pages, block, p.n_pages, p.status) : -1;
+            found = page >= 0;
+            if (found) {
+                const unsigned char* b = p.pool + ((long long)page * p.kv_heads + head) * kv8_block_bytes(kDim);
+                const float2 scale = *reinterpret_cast<const float2*>(b + 32 * kDim);
+                const uint2 kb = *reinterpret_cast<const uint2*>(b + kv8_key_at(token, d0));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    k[i] = (float)((int)(((i < 4 ? kb.x : kb.y) >> (8 * (i & 3))) & 255) - 128) * scale.x;
+                    v[i] = (float)((int)b[kv8_value_at(token, d0 + i, kDim)] - 128) * scale.y;
+                }
+            }
+        } else {
+            const __nv_bfloat16* src = p.open + (long long)slot * kv8_open_elems(p.kv_heads, kDim) + kv8_open_at(block, p.kv_heads, head, 0, kDim) + token * kDim + d0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { k[i] = __bfloat162float(src[i]); v[i] = __bfloat162float(src[kKv8Tokens * kDim + i]); }
+        }
+    }
+    if (!found) atomicExch(p.status, 2);
+    const long long at = (row * p.kv_heads + head) * kDim + d0;
+    float (*const kk)[4] = reinterpret_cast<float(*)[4]>(k), (*const vv)[4] = reinterpret_cast<float(*)[4]>(v);
+    store_vec(static_cast<T*>(p.k) + at, kk[0]);
+    store_vec(static_cast<T*>(p.k) + at + 4, kk[1]);
+    store_vec(static_cast<T*>(p.v) + at, vv[0]);
+    store_vec(static_cast<T*>(p.v) + at + 4, vv[1]);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+
+int kv8_check(const gptrs_kv8_cache* c) {
+    GPTRS_REQUIRE(c, "null pointer");
+    gptrs_kv8_cache want = *c;
+    const int rc = gptrs_cuda_kv8_layout(&want);
+    if (rc) return rc;
+    GPTRS_REQUIRE(c->block_bytes == want.block_bytes && c->page_bytes == want.page_bytes && c->tile_tokens == want.tile_tokens, "call gptrs_cuda_kv8_layout first");
+    return GPTRS_OK;
+}
+
+}  // namespace gptrs
+
+using namespace gptrs;
+
+extern "C" {
+
+int gptrs_cuda_kv8_layout(gptrs_kv8_cache* c) {
+    GPTRS_REQUIRE(c, "null pointer");
+    GPTRS_REQUIRE(c->q_heads > 0 && c->kv_heads > 0 && c->q_heads % c->kv_heads == 0 && c->kv_heads <= 65535, "bad head counts");
+    GPTRS_REQUIRE(c->window >= 0, "bad window");
+    if (c->dim != 64 && c->dim != 128) return fail(GPTRS_UNIMPLEMENTED, "the 8-bit cache takes heads of 64 and 128 channels");
+    const int group = c->q_heads / c->kv_heads;
+    if (group > 64) return fail(GPTRS_UNIMPLEMENTED, "the 8-bit cache takes up to 64 query heads per kv head");
+    if (!(c->scale > 0.f)) {
+        GPTRS_REQUIRE(c->scale == 0.f, "the scale of the scores is positive, or 0 for 1 / sqrt(dim)");
+        c->scale = 1.f / sqrtf((float)c->dim);
+    }
+    c->tile_tokens = 2 * (128 / group);
+    c->block_bytes = kv8_block_bytes(c->dim);
+    c->page_bytes = c->block_bytes * c->kv_heads;
+    c->open_bytes = 2 * kv8_open_elems(c->kv_heads, c->dim);
+    return GPTRS_OK;
+}
+
+int gptrs_cuda_kv8_append(const gptrs_kv8_cache* c, const gptrs_kv8_append_step* s, void* stream) {
+    const int rc = kv8_check(c);
+    if (rc) return rc;
+    GPTRS_REQUIRE(s && s->d_qkv && s->d_positions && s->d_slot && s->d_run_first && s->d_run_last && s->d_page_table && s->d_pool && s->d_open && s->d_q && s->d_status,
+                  "null pointer");
+    GPTRS_REQUIRE(s->rows >= 0 && s->rows <= 0x3fffffff, "bad row count");
+    GPTRS_REQUIRE(s->max_pages >= 1 && s->n_pages >= 1 && s->n_slots >= 1, "empty cache");
+    AppendParams p = {};
+    const int64_t width = (int64_t)(c->q_heads + 2 * c->kv_heads) * c->dim;
+    p.ld = s->ld ? s->ld : width;
+    GPTRS_REQUIRE(p.ld >= width && p.ld % 8 == 0, "rows overlap, or do not start at multiples of 16 bytes");
+    GPTRS_REQUIRE(aligned16(s->d_qkv) && aligned16(s->d_pool) && aligned16(s->d_open) && aligned16(s->d_q), "pointers must be 16-byte aligned");
+    if (s->rotation) {
+        const int rr = qk_rotation_of(*s->rotation, s->rows, &p.r);
+        if (rr) return rr;
+        GPTRS_REQUIRE(p.r.q_heads == c->q_heads && p.r.kv_heads == c->kv_heads && p.r.dim == c->dim, "the rotation is of other heads");
+        if (p.r.rot_half % 4) return fail(GPTRS_UNIMPLEMENTED, "the append takes rotations of a multiple of 4 pairs");
+        GPTRS_REQUIRE(aligned16(p.r.cos) && aligned16(p.r.sin) && aligned16(p.r.q_gain) && aligned16(p.r.k_gain), "tables and gains must be 16-byte aligned");
+        p.rotates = 1;
+    } else {
+        p.r.dim = c->dim;
+    }
+    if (s->rows == 0) return GPTRS_OK;
+    p.qkv = static_cast<const __nv_bfloat16*>(s->d_qkv);
+    p.positions = s->d_positions; p.slot = s->d_slot; p.run_first = s->d_run_first; p.run_last = s->d_run_last; p.table = s->d_page_table;
+    p.max_pages = s->max_pages; p.n_pages = s->n_pages; p.n_slots = s->n_slots;
+    p.pool = static_cast<unsigned char*>(s->d_pool);
+    p.open = static_cast<__nv_bfloat16*>(s->d_open);
+    p.q = static_cast<__nv_bfloat16*>(s->d_q);
+    p.status = s->d_status;
+    p.rows = (int)s->rows; p.q_heads = c->q_heads; p.kv_heads = c->kv_heads; p.group = c->q_heads / c->kv_heads;
+    p.tile_rows = s->rows <= 256 ? 1 : kKv8Tokens;
+    const dim3 grid((unsigned)ceil_div(s->rows, p.tile_rows), (unsigned)c->kv_heads);
+    if (c->dim == 64) return launch_kernel(kv8_append_kernel<64>, grid, dim3(kThreads), 0, as_stream(stream), 1, p);
+    return launch_kernel(kv8_append_kernel<128>, grid, dim3(kThreads), 0, as_stream(stream), 1, p);
+}
+
+int gptrs_cuda_kv8_gather(const gptrs_kv8_cache* c, const void* d_pool, int64_t n_pages, const void* d_open, int64_t n_slots, const int32_t* d_page_table,
+                          int64_t max_pages, const int32_t* d_slot, const int32_t* d_positions, const int32_t* d_length, int dtype, void* d_k,
+                          void* d_v, int32_t* d_status, int64_t rows, void* stream) {
+    const int rc = kv8_check(c);
+    if (rc) return rc;
+    GPTRS_REQUIRE(d_pool && d_open && d_page_table && d_slot && d_positions && d_length && d_k && d_v && d_status, "null pointer");
+    GPTRS_REQUIRE(dtype == GPTRS_BF16 || dtype == GPTRS_F32, "keys and values come back in bf16 or f32");
+    GPTRS_REQUIRE(rows >= 0 && rows <= 0x3fffffff, "bad row count");
+    GPTRS_REQUIRE(max_pages >= 1 && n_pages >= 1 && n_slots >= 1, "empty cache");
+    GPTRS_REQUIRE(aligned16(d_pool) && aligned16(d_open) && aligned16(d_k) && aligned16(d_v), "pointers must be 16-byte aligned");
+    if (rows == 0) return GPTRS_OK;
+    GatherParams p = {static_cast<const unsigned char*>(d_pool), static_cast<const __nv_bfloat16*>(d_open), d_page_table, d_slot, d_positions, d_length,
+                      (long long)max_pages, (long long)n_pages, (long long)n_slots, d_k, d_v, d_status, (int)rows, c->kv_heads};
+    const int64_t ctas = (rows * c->kv_heads * (c->dim / 8) + kThreads - 1) / kThreads;
+    GPTRS_REQUIRE(ctas <= 0x7fffffff, "grid too large");
+    const dim3 grid((unsigned)ctas), block(kThreads);
+    if (c->dim == 64)
+        return dtype == GPTRS_F32 ? launch_kernel(kv8_gather_kernel<64, float>, grid, block, 0, as_stream(stream), 1, p)
+                                  : launch_kernel(kv8_gather_kernel<64, __nv_bfloat16>, grid, block, 0, as_stream(stream), 1, p);
+    return dtype == GPTRS_F32 ? launch_kernel(kv8_gather_kernel<128, float>, grid, block, 0, as_stream(stream), 1, p)
+                              : launch_kernel(kv8_gather_kernel<128, __nv_bfloat16>, grid, block, 0, as_stream(stream), 1, p);
+}
+
+}  // extern "C"

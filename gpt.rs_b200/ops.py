@@ -683,3 +683,230 @@ def gated_pairs_f32(gate_up, n, gate=GATE_SILU):
     out = torch.empty((gate_up.shape[0], n), device=gate_up.device)
     check(lib().gptrs_cuda_gated_pairs_f32(_ptr(gate_up), _ptr(out), gate_up.shape[0], n, gate, _stream()))
     return out
+
+
+# ---- norms and rotation of queries and keys, 8-bit paged cache ----------------------------------------------------------------
+# The calls below are objects: made once with their buffers, as a serving loop has them, and called every step on the current stream.
+PAIRS_HALVES, PAIRS_NEIGHBOURS = 0, 1
+
+
+class _Step:
+    """A prepared call: keeps its tensors alive and checks that they are on the current device."""
+
+    def _hold(self, **tensors):
+        self._tensors = {k: t for k, t in tensors.items() if t is not None}
+        devices = {t.device for t in self._tensors.values()}
+        if len(devices) != 1 or next(iter(devices)).type != "cuda":
+            raise ValueError(f"expected CUDA tensors of one device, got {sorted(map(str, devices))}")
+        self._device = next(iter(devices)).index
+
+    def _run(self, fn, *args):
+        if torch.cuda.current_device() != self._device:
+            raise ValueError(f"the tensors are on cuda:{self._device}, the current device is cuda:{torch.cuda.current_device()}")
+        status = fn(*args, _stream())
+        if status:
+            check(status)
+
+
+def _need(t, name, dtype, *shape):
+    """t is of that dtype and shape (None: any size) and contiguous."""
+    if t.dtype != dtype or t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)) or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor {list(shape)}, got {t.dtype} {list(t.shape)}")
+    return t
+
+
+def _rows_of(t, name, width, dtypes):
+    """A matrix whose rows lie a stride apart: (pointer, stride)."""
+    if t.dtype not in dtypes or t.dim() != 2 or t.shape[1] != width or t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width):
+        raise ValueError(f"{name}: expected rows of {width} values, got {t.dtype} {list(t.shape)} with strides {t.stride()}")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else width
+
+
+class QkRotation:
+    """Norms of queries and keys per head and their rotation (gptrs_qk_rotation): tables cos / sin f32 [positions][pairs] or None for no
+    rotation; gains f32 [dim] or None for no norms; positions on several axes as axis_positions int32 [axes][rows] with the axis of every pair in
+    pair_axis uint8 [pairs]."""
+
+    def __init__(self, q_heads, kv_heads, dim, cos=None, sin=None, q_gain=None, k_gain=None, eps=1e-6, neighbours=False, axis_positions=None, pair_axis=None):
+        r = self.struct = _abi.QkRotation(q_heads, kv_heads, dim)
+        self.rows = None
+        r.pairs, r.eps = PAIRS_NEIGHBOURS if neighbours else PAIRS_HALVES, eps
+        if cos is not None:
+            _need(cos, "cos", torch.float32, None, None)
+            _need(sin, "sin", torch.float32, *cos.shape)
+            r.rot_half, r.positions, r.d_cos, r.d_sin = cos.shape[1], cos.shape[0], cos.data_ptr(), sin.data_ptr()
+        if q_gain is not None:
+            r.d_q_gain = _need(q_gain, "q_gain", torch.float32, dim).data_ptr()
+        if k_gain is not None:
+            r.d_k_gain = _need(k_gain, "k_gain", torch.float32, dim).data_ptr()
+        if axis_positions is not None:
+            _need(axis_positions, "axis_positions", torch.int32, None, None)
+            r.axes, self.rows = axis_positions.shape
+            r.d_axis_positions, r.axis_stride = axis_positions.data_ptr(), self.rows
+        if pair_axis is not None:
+            r.d_pair_axis = _need(pair_axis, "pair_axis", torch.uint8, r.rot_half).data_ptr()
+        self.tensors = dict(cos=cos, sin=sin, q_gain=q_gain, k_gain=k_gain, axis_positions=axis_positions, pair_axis=pair_axis)
+
+    def check_rows(self, rows):
+        if self.rows is not None and self.rows < rows:
+            raise ValueError(f"axis_positions has {self.rows} rows, the call {rows}")
+
+
+class QkNormRope(_Step):
+    """gptrs_cuda_qk_norm_rope on rows [queries | keys | values] (f32 or bf16); call it to get `out` (qkv itself: in place)."""
+
+    def __init__(self, rotation, qkv, positions, out=None, status=None):
+        r = rotation.struct
+        self.rotation, self.rows = rotation, qkv.shape[0]
+        rotation.check_rows(self.rows)
+        width = (r.q_heads + 2 * r.kv_heads) * r.dim
+        self.out = torch.empty((self.rows, width), dtype=qkv.dtype, device=qkv.device) if out is None else out
+        self.status = _status(qkv.device, status)
+        src, ld_in = _rows_of(qkv, "qkv", width, (torch.float32, torch.bfloat16))
+        dst, ld_out = _rows_of(self.out, "out", width, (qkv.dtype,))
+        if self.out.shape[0] != self.rows:
+            raise ValueError("out has another number of rows")
+        positions = None if positions is None else _need(positions, "positions", torch.int32, self.rows)
+        self._hold(qkv=qkv, out=self.out, positions=positions, status=self.status, **rotation.tensors)
+        self._args = (ctypes.byref(r), src, _dt(qkv), ld_in, None if positions is None else positions.data_ptr(), dst, ld_out, self.status.data_ptr(), self.rows)
+        self._fn = lib().gptrs_cuda_qk_norm_rope
+
+    def __call__(self):
+        self._run(self._fn, *self._args)
+        return self.out
+
+
+def qk_norm_rope(rotation, qkv, positions, out=None, status=None):
+    return QkNormRope(rotation, qkv, positions, out, status)()
+
+
+def kv8_layout(q_heads, kv_heads, dim, window=0, scale=0.0):
+    a = _abi.Kv8Cache(q_heads, kv_heads, dim, window, scale)
+    check(lib().gptrs_cuda_kv8_layout(ctypes.byref(a)))
+    return a
+
+
+def new_kv8_pool(a, n_pages, device):
+    return torch.zeros((n_pages, a.kv_heads, a.block_bytes), dtype=torch.uint8, device=device)
+
+
+def new_kv8_open(a, n_slots, device):
+    """The rows of blocks that are not complete yet."""
+    return torch.zeros((n_slots, 2, a.kv_heads, 2, 16, a.dim), dtype=torch.bfloat16, device=device)
+
+
+def _kv8_cache(a, page_table, pool, open_rows):
+    _need(pool, "pool", torch.uint8, None, a.kv_heads, a.block_bytes)
+    _need(open_rows, "open_rows", torch.bfloat16, None, 2, a.kv_heads, 2, 16, a.dim)
+    _need(page_table, "page_table", torch.int32, open_rows.shape[0], None)
+    return pool.shape[0], open_rows.shape[0]
+
+
+class Kv8Append(_Step):
+    """gptrs_cuda_kv8_append: rows bf16 [T][queries | keys | values] of runs of consecutive positions -> queries [T][heads][dim], keys and
+    values into the cache. rotation None: queries and keys as they are."""
+
+    def __init__(self, a, rotation, qkv, positions, slot, run_first, run_last, page_table, pool, open_rows, q=None, status=None):
+        self.a, self.rotation, rows = a, rotation, qkv.shape[0]
+        s = self.step = _abi.Kv8AppendStep()
+        s.n_pages, s.n_slots = _kv8_cache(a, page_table, pool, open_rows)
+        self.q = torch.empty((rows, a.q_heads, a.dim), dtype=torch.bfloat16, device=qkv.device) if q is None else _need(q, "q", torch.bfloat16, rows, a.q_heads, a.dim)
+        self.status = _status(qkv.device, status)
+        s.d_qkv, s.ld = _rows_of(qkv, "qkv", (a.q_heads + 2 * a.kv_heads) * a.dim, (torch.bfloat16,))
+        s.d_positions, s.d_slot, s.d_run_first, s.d_run_last = (_need(t, n, torch.int32, rows).data_ptr() for n, t in
+                                                                (("positions", positions), ("slot", slot), ("run_first", run_first), ("run_last", run_last)))
+        s.d_page_table, s.max_pages, s.d_pool, s.d_open = page_table.data_ptr(), page_table.shape[1], pool.data_ptr(), open_rows.data_ptr()
+        s.d_q, s.d_status, s.rows = self.q.data_ptr(), self.status.data_ptr(), rows
+        if rotation is not None:
+            rotation.check_rows(rows)
+            s.rotation = ctypes.addressof(rotation.struct)
+        self._hold(qkv=qkv, positions=positions, slot=slot, run_first=run_first, run_last=run_last, page_table=page_table, pool=pool, open_rows=open_rows, q=self.q,
+                   status=self.status, **(rotation.tensors if rotation is not None else {}))
+        self._args = (ctypes.byref(a), ctypes.byref(s))
+        self._fn = lib().gptrs_cuda_kv8_append
+
+    def __call__(self):
+        self._run(self._fn, *self._args)
+        return self.q
+
+
+def kv8_append(*args, **kw):
+    return Kv8Append(*args, **kw)()
+
+
+class Kv8Gather(_Step):
+    """gptrs_cuda_kv8_gather: keys and values [T][kv heads][dim] of the tokens (slot[t], positions[t]); lengths [slots]."""
+
+    def __init__(self, a, pool, open_rows, page_table, slot, positions, lengths, dtype=torch.bfloat16, status=None):
+        n_pages, n_slots = _kv8_cache(a, page_table, pool, open_rows)
+        rows = slot.shape[0]
+        self.a = a
+        self.k, self.v = (torch.empty((rows, a.kv_heads, a.dim), dtype=dtype, device=pool.device) for _ in range(2))
+        self.status = _status(pool.device, status)
+        _need(slot, "slot", torch.int32, rows)
+        _need(positions, "positions", torch.int32, rows)
+        _need(lengths, "lengths", torch.int32, n_slots)
+        self._hold(pool=pool, open_rows=open_rows, page_table=page_table, slot=slot, positions=positions, lengths=lengths, k=self.k, v=self.v, status=self.status)
+        self._args = (ctypes.byref(a), pool.data_ptr(), n_pages, open_rows.data_ptr(), n_slots, page_table.data_ptr(), page_table.shape[1], slot.data_ptr(),
+                      positions.data_ptr(), lengths.data_ptr(), _dt(self.k), self.k.data_ptr(), self.v.data_ptr(), self.status.data_ptr(), rows)
+        self._fn = lib().gptrs_cuda_kv8_gather
+
+    def __call__(self):
+        self._run(self._fn, *self._args)
+        return self.k, self.v
+
+
+def kv8_gather(*args, **kw):
+    return Kv8Gather(*args, **kw)()
+
+
+def kv8_tiles(a, counts, device):
+    """Tiles of rows that come sequence by sequence, counts[i] of the i-th: (first rows, row counts)."""
+    first, n, row = [], [], 0
+    for count in counts:
+        for at in range(0, count, a.tile_tokens):
+            first.append(row + at)
+            n.append(min(a.tile_tokens, count - at))
+        row += count
+    return torch.tensor(first, dtype=torch.int32, device=device), torch.tensor(n, dtype=torch.int32, device=device)
+
+
+class Kv8Attention(_Step):
+    """gptrs_cuda_kv8_attention: q [T][heads][dim] (rows may lie a stride apart) -> out [T][heads * dim]. lengths [slots]: tokens that the
+    cache holds. `tiles` (kv8_tiles): rows of prompts; None: every row by itself."""
+
+    def __init__(self, a, q, pool, open_rows, page_table, slot, ctx_len, lengths, max_ctx_len, tiles=None, splits=None, out=None, status=None):
+        rows = q.shape[0]
+        self.a = a
+        s = self.step = _abi.Kv8AttentionStep()
+        s.n_pages, s.n_slots = _kv8_cache(a, page_table, pool, open_rows)
+        if q.dtype != torch.bfloat16 or q.shape[1:] != (a.q_heads, a.dim) or q.stride(2) != 1 or q.stride(1) != a.dim or (rows > 1 and q.stride(0) < a.q_heads * a.dim):
+            raise ValueError(f"q: expected bf16 [rows][{a.q_heads}][{a.dim}], got {q.dtype} {list(q.shape)} with strides {q.stride()}")
+        self.out = torch.empty((rows, a.q_heads * a.dim), dtype=torch.bfloat16, device=q.device) if out is None else _need(out, "out", torch.bfloat16, rows, a.q_heads * a.dim)
+        self.status = _status(q.device, status)
+        s.d_q, s.ldq = q.data_ptr(), q.stride(0) if rows > 1 else a.q_heads * a.dim
+        s.d_pool, s.d_open, s.d_page_table, s.max_pages = pool.data_ptr(), open_rows.data_ptr(), page_table.data_ptr(), page_table.shape[1]
+        s.d_slot, s.d_ctx_len = _need(slot, "slot", torch.int32, rows).data_ptr(), _need(ctx_len, "ctx_len", torch.int32, rows).data_ptr()
+        s.d_length = _need(lengths, "lengths", torch.int32, s.n_slots).data_ptr()
+        tile_row = tile_rows = None
+        if tiles is not None:
+            tile_row, tile_rows = _need(tiles[0], "tiles[0]", torch.int32, None), _need(tiles[1], "tiles[1]", torch.int32, tiles[0].shape[0])
+            s.d_tile_row, s.d_tile_rows, s.n_tiles = tile_row.data_ptr(), tile_rows.data_ptr(), tile_row.shape[0]
+        s.max_ctx_len = max_ctx_len
+        s.splits = lib().gptrs_cuda_kv8_splits(ctypes.byref(a), rows, s.n_tiles, max_ctx_len) if splits is None else splits
+        s.scratch_bytes = lib().gptrs_cuda_kv8_scratch_bytes(ctypes.byref(a), rows, s.n_tiles, s.splits)
+        scratch = torch.empty(s.scratch_bytes, dtype=torch.uint8, device=q.device) if s.scratch_bytes else None
+        s.d_scratch = None if scratch is None else scratch.data_ptr()
+        s.d_out, s.d_status, s.rows = self.out.data_ptr(), self.status.data_ptr(), rows
+        self._hold(q=q, pool=pool, open_rows=open_rows, page_table=page_table, slot=slot, ctx_len=ctx_len, lengths=lengths, tile_row=tile_row, tile_rows=tile_rows,
+                   scratch=scratch, out=self.out, status=self.status)
+        self._args = (ctypes.byref(a), ctypes.byref(s))
+        self._fn = lib().gptrs_cuda_kv8_attention
+
+    def __call__(self):
+        self._run(self._fn, *self._args)
+        return self.out
+
+
+def kv8_attention(*args, **kw):
+    return Kv8Attention(*args, **kw)()

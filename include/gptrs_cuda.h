@@ -700,6 +700,117 @@ int gptrs_cuda_kv_gather(const void* d_kv_pool, const int32_t* d_page_row, int64
                          int64_t head_dim, void* d_k_out, void* d_v_out, void* stream);
 
 /* ==============================================================================================
+ * Norms of queries and keys per head and their rotation in one pass, with positions on several axes (no counterpart in gpt.rs, which
+ * rotates by one position per token, ops/functional/rotary.rs). Rows are [queries | keys | values], q_heads + 2 kv_heads heads of dim values.
+ *     x <- x / sqrt(mean(x^2) + eps) gain                       (queries and keys; without gains x stays)
+ *     (a, b) <- (a cos - b sin, b cos + a sin)                   (rot_half pairs of channels; the channels behind them stay)
+ * cos and sin of pair i are row `position` of the tables, column i, position being the row's position on the axis of the pair: time for text,
+ * time, height and width for images and video.
+ * ============================================================================================ */
+enum { GPTRS_PAIRS_HALVES = 0, GPTRS_PAIRS_NEIGHBOURS = 1 };   /* pair i: channels (i, i + rot_half); (2 i, 2 i + 1) */
+typedef struct {
+    int q_heads, kv_heads, dim;
+    int rot_half;                      /* rotated pairs (0 = none) */
+    int pairs;                         /* GPTRS_PAIRS_* */
+    int axes;                          /* 0 or 1 = the rows' own positions unless d_axis_positions is given */
+    float eps;
+    const float *d_q_gain, *d_k_gain;  /* [dim], both or none */
+    const float *d_cos, *d_sin;        /* [positions][rot_half] */
+    int64_t positions;
+    const int32_t* d_axis_positions;   /* [axes][rows], axis_stride apart (0 = rows) */
+    int64_t axis_stride;
+    const uint8_t* d_pair_axis;        /* [rot_half]: axis of every pair; NULL: all on the first one */
+} gptrs_qk_rotation;
+/* qkv rows (f32 or bf16, ld_in apart, 0 = packed) -> the same rows with queries and keys normed and rotated, rounded once. d_out may be
+ * d_qkv with the same stride; otherwise the values are copied. dim even, at most 512. A position outside the tables or an axis that does
+ * not exist sets *d_status = 2 and turns by position 0. */
+int gptrs_cuda_qk_norm_rope(const gptrs_qk_rotation* r, const void* d_qkv, int dtype, int64_t ld_in, const int32_t* d_positions, void* d_out,
+                            int64_t ld_out, int32_t* d_status, int64_t rows, void* stream);
+
+/* ==============================================================================================
+ * Paged KV cache in 8 bits with a scale per block of tokens and head, and the attention that reads it (no counterpart in gpt.rs; half the
+ * bytes of the bf16 cache above). Pages hold 16 tokens and are addressed through page_table[slot][page index] in the same way. A page
+ * holds per kv head a block of block_bytes = 32 dim + 16: 16 dim bytes of keys, 16 dim bytes of values, the keys' and the values' scale (f32),
+ * 8 bytes of zeros. A byte u stands for (u - 128) scale; scale = max(largest |x| of the block's 16 dim keys or values / 127, 2^-60) and
+ * u - 128 = x / scale rounded to the nearest whole number (ties to even). If a key (value) of the block is not finite its scale is NaN. Order of
+ * the bytes (a thread of the attention reads 16 of them at a time and finds the operands of its matrix instructions):
+ *     keys    [dim / 32][token % 8][dim % 32 / 8][token / 8][dim % 8]
+ *     values  [dim / 32][dim % 8][token % 8 / 2][dim % 32 / 8][token / 8][token % 2]
+ * A block is written once, when its last token arrives. Until then its tokens are bf16 rows in the slot's part of `open`,
+ *     open[slot][block % 2][kv head][key, value][token % 16][dim],
+ * so that nothing is quantised twice and the cache does not depend on how tokens were cut into calls. A sequence may be taken back: to the first
+ * position of any block, or into the block of its last token or the one in front of it, whose rows stay there (until a later block, two
+ * further on, takes their place: one taken back to an earlier block and no further than that has that block's rows only).
+ * length[slot] = tokens appended to the slot; blocks below length / 16 are read from the pages, the last one from the open rows.
+ * bf16 activations, dim 64 or 128, any number of query heads per kv head up to 64. Waits inside the kernels are bounded.
+ * ============================================================================================ */
+typedef struct {
+    int q_heads, kv_heads, dim;
+    int window;                        /* position i sees i - window + 1 .. i; 0: all of 0 .. i */
+    float scale;                       /* of the scores; 0 = 1 / sqrt(dim) */
+    /* filled in by gptrs_cuda_kv8_layout: */
+    int tile_tokens;                   /* most rows of a tile of gptrs_cuda_kv8_attention */
+    int64_t block_bytes, page_bytes, open_bytes;   /* of a (page, kv head), of a page, of a slot's open rows */
+} gptrs_kv8_cache;
+int gptrs_cuda_kv8_layout(gptrs_kv8_cache* c);
+/* Projection rows [queries | keys | values] (bf16) -> normed and rotated queries in d_q [rows][q_heads][dim], keys (normed, rotated, rounded
+ * to bf16) and values into the cache. Rows come in runs of consecutive positions of one sequence, one run per slot and call; run_first and
+ * run_last give the first and the last row of the run of every row. Rows with a negative slot are padding: nothing of them is read or written.
+ * rotation NULL: queries and keys as they are. A block whose page_table entry is negative is not kept. *d_status = 2: a slot, position, page
+ * or run out of range (the keys and values of that row or block are left out). */
+typedef struct {
+    const gptrs_qk_rotation* rotation; /* rot_half a multiple of 4 */
+    const void* d_qkv;
+    int64_t ld;                        /* 0 = packed */
+    const int32_t *d_positions, *d_slot, *d_run_first, *d_run_last;
+    const int32_t* d_page_table;
+    int64_t max_pages;
+    void* d_pool;
+    int64_t n_pages;
+    void* d_open;
+    int64_t n_slots;
+    void* d_q;
+    int32_t* d_status;
+    int64_t rows;
+} gptrs_kv8_append_step;
+int gptrs_cuda_kv8_append(const gptrs_kv8_cache* c, const gptrs_kv8_append_step* s, void* stream);
+/* Tokens (d_slot[i], d_positions[i]) of the cache -> keys and values [rows][kv_heads][dim], rounded to dtype (GPTRS_BF16 or GPTRS_F32). A
+ * token that the cache does not hold gives zeros, and 2 in *d_status. */
+int gptrs_cuda_kv8_gather(const gptrs_kv8_cache* c, const void* d_pool, int64_t n_pages, const void* d_open, int64_t n_slots, const int32_t* d_page_table,
+                          int64_t max_pages, const int32_t* d_slot, const int32_t* d_positions, const int32_t* d_length, int dtype, void* d_k,
+                          void* d_v, int32_t* d_status, int64_t rows, void* stream);
+/* out [rows][q_heads][dim] (bf16) = softmax over the visible keys . values; row t belongs to slot[t] and sees the last `window` of its first
+ * ctx_len[t] tokens (the cache as it is behind the append). A row that sees nothing gives zeros, one with a negative slot is left as it was.
+ * n_tiles = 0: every row by itself (single tokens of many sequences); else tile i is the rows tile_row[i] .. + tile_rows[i], at most tile_tokens
+ * rows of one sequence at consecutive positions (prompts, chunks of prompts). The keys of a row or tile are read in at most `splits` parts
+ * (gptrs_cuda_kv8_splits; scratch: gptrs_cuda_kv8_scratch_bytes). max_ctx_len bounds ctx_len. *d_status = 2: a length, slot or
+ * page out of range, 3: a bounded wait ran out. */
+typedef struct {
+    const void* d_q;                   /* [rows][q_heads][dim], rows ldq apart (0 = packed) */
+    int64_t ldq;
+    const void* d_pool;
+    int64_t n_pages;
+    const void* d_open;
+    int64_t n_slots;
+    const int32_t* d_page_table;
+    int64_t max_pages;
+    const int32_t *d_slot, *d_ctx_len;
+    const int32_t* d_length;           /* [n_slots] */
+    const int32_t *d_tile_row, *d_tile_rows;
+    int64_t n_tiles;
+    int64_t max_ctx_len;
+    int splits;
+    void* d_out;
+    void* d_scratch;                   /* 16-byte aligned */
+    size_t scratch_bytes;
+    int32_t* d_status;
+    int64_t rows;
+} gptrs_kv8_attention_step;
+int gptrs_cuda_kv8_splits(const gptrs_kv8_cache* c, int64_t rows, int64_t n_tiles, int64_t max_ctx_len);
+size_t gptrs_cuda_kv8_scratch_bytes(const gptrs_kv8_cache* c, int64_t rows, int64_t n_tiles, int splits);
+int gptrs_cuda_kv8_attention(const gptrs_kv8_cache* c, const gptrs_kv8_attention_step* s, void* stream);
+
+/* ==============================================================================================
  * Row-wise functionals.
  * ============================================================================================ */
 /* hidden[T][D] (f32) += delta (optional, f32 or bf16), then rms_norm
