@@ -12,7 +12,7 @@
 // several splits of a row go through scratch and a second kernel.
 #include <algorithm>
 
-#include "kv8_cache.cuh"
+#include "kv8_attention.cuh"
 
 namespace gptrs {
 namespace {
@@ -20,33 +20,8 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kCols = 8;    // query heads of a CTA
 
-struct AttnParams {
-    const __nv_bfloat16* q;
-    long long ldq;
-    const unsigned char* pool;
-    const __nv_bfloat16* open;
-    const int *table, *slot, *ctx_len, *length;
-    __nv_bfloat16* out;
-    float *part_o, *part_ml;      // [row][head][split][dim], [row][head][split][2]
-    int* status;
-    long long n_pages, max_pages;
-    int n_slots, rows, q_heads, kv_heads, group, window, max_len, splits, chunk_blocks;
-    float scale_log2;
-};
-
-struct Span { int slot, begin, end, length; };   // visible tokens [begin, end) of a row, and what its sequence has
-__device__ __forceinline__ Span span_of(const AttnParams& p, int row) {
-    Span s = {p.slot[row], 0, 0, 0};
-    if (s.slot < 0) return s;
-    if (s.slot >= p.n_slots) { atomicExch(p.status, 2); s.slot = 0; return s; }
-    s.length = p.length[s.slot];
-    s.end = p.ctx_len[row];
-    if (s.end < 0 || s.end > p.max_len || s.end > s.length) { atomicExch(p.status, 2); s.end = max(0, min(min(s.end, p.max_len), s.length)); }
-    s.begin = p.window > 0 ? max(0, s.end - p.window) : 0;
-    return s;
-}
 // A row's blocks in parts of equal size, at most chunk_blocks each.
-__device__ __forceinline__ void parts_of(const AttnParams& p, const Span& s, int* first, int* blocks, int* parts, int* per) {
+__device__ __forceinline__ void parts_of(const Kv8Attention& p, const Kv8Span& s, int* first, int* blocks, int* parts, int* per) {
     *first = s.begin / kKv8Tokens;
     *blocks = s.end > s.begin ? (s.end - 1) / kKv8Tokens + 1 - *first : 0;
     *parts = (*blocks + p.chunk_blocks - 1) / p.chunk_blocks;
@@ -55,7 +30,7 @@ __device__ __forceinline__ void parts_of(const AttnParams& p, const Span& s, int
 }
 
 template <int kDim>
-__global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(const Kv8Attention p) {
     constexpr int kC = kDim / 32;      // chunks of 32 channels
     __shared__ float o_part[kWarps][kCols][kDim + 1];
     __shared__ float ml_part[kWarps][kCols][2];
@@ -66,7 +41,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(const AttnPa
     const int kv_head = blockIdx.y / eights, head0 = kv_head * p.group + (blockIdx.y % eights) * kCols;
     const int cols = min(kCols, p.group - (int)(blockIdx.y % eights) * kCols);
     const int row = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const Span span = span_of(p, row);
+    const Kv8Span span = kv8_span(p, row);
     if (span.slot < 0) return;
     int first, blocks, parts, per;
     parts_of(p, span, &first, &blocks, &parts, &per);
@@ -262,14 +237,14 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(const AttnPa
 
 // The parts of a row's head, added up in their order.
 template <int kDim>
-__global__ void __launch_bounds__(kDim / 2) kv8_merge_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kDim / 2) kv8_merge_kernel(const Kv8Attention p) {
     pdl_launch_dependents();
     pdl_wait();
     const int row = blockIdx.y, d = threadIdx.x * 2;
-    const Span span = span_of(p, row);
+    const Kv8Span span = kv8_span(p, row);
     if (span.slot < 0) return;
-    int first, blocks, parts, per;
-    parts_of(p, span, &first, &blocks, &parts, &per);
+    int first, blocks, parts = p.splits, per;
+    if (p.n_tiles == 0) parts_of(p, span, &first, &blocks, &parts, &per);   // of a tile every part has its sum
     if (parts <= 1) return;
     const long long at = (long long)row * p.q_heads + blockIdx.x;
     const float* ml = p.part_ml + 2 * at * p.splits;
@@ -278,6 +253,7 @@ __global__ void __launch_bounds__(kDim / 2) kv8_merge_kernel(const AttnParams p)
     const float ref = top == -INFINITY ? 0.f : top;
     for (int i = 0; i < parts; ++i) {
         const float f = ml[2 * i] == -INFINITY ? ml[2 * i + 1] : kv8_exp2(ml[2 * i] - ref);   // no maximum: nothing (0) or nothing but NaN
+        if (ml[2 * i] == -INFINITY && f == 0.f) continue;                                             // and its part of the output is not there
         const float2 v = *reinterpret_cast<const float2*>(p.part_o + (at * p.splits + i) * kDim + d);
         l += ml[2 * i + 1] * f;
         x += v.x * f;
@@ -290,9 +266,10 @@ __global__ void __launch_bounds__(kDim / 2) kv8_merge_kernel(const AttnParams p)
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <int kDim>
-int launch_attention(const AttnParams& p, cudaStream_t st) {
+int launch_attention(const Kv8Attention& p, cudaStream_t st) {
     const int eights = (p.group + kCols - 1) / kCols;
-    const int rc = launch_kernel(kv8_attention_kernel<kDim>, dim3((unsigned)p.splits, (unsigned)(p.kv_heads * eights), (unsigned)p.rows), dim3(kWarps * 32), 0, st, 1, p);
+    const int rc = p.n_tiles ? kv8_prompt_attention(p, kDim, st)
+                             : launch_kernel(kv8_attention_kernel<kDim>, dim3((unsigned)p.splits, (unsigned)(p.kv_heads * eights), (unsigned)p.rows), dim3(kWarps * 32), 0, st, 1, p);
     if (rc || p.splits == 1) return rc;
     return launch_kernel(kv8_merge_kernel<kDim>, dim3((unsigned)p.q_heads, (unsigned)p.rows), dim3(kDim / 2), 0, st, 1, p);
 }
@@ -306,6 +283,11 @@ extern "C" {
 
 int gptrs_cuda_kv8_splits(const gptrs_kv8_cache* c, int64_t rows, int64_t n_tiles, int64_t max_ctx_len) {
     if (!c || rows < 1 || c->kv_heads < 1) return 1;
+    if (n_tiles > 0) {
+        // a CTA per tile and kv head has an SM to itself: parts only where many SMs would have nothing, of 512 keys at least
+        const int64_t ctas = n_tiles * c->kv_heads, keys = c->window > 0 ? std::min<int64_t>(max_ctx_len, c->window + c->tile_tokens) : max_ctx_len;
+        return rows > 65535 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(sm_count() / ctas, keys / 512));
+    }
     const int64_t seen = c->window > 0 ? std::min<int64_t>(max_ctx_len, c->window + kKv8Tokens) : max_ctx_len;
     const int64_t blocks = (seen + kKv8Tokens - 1) / kKv8Tokens;
     const int64_t ctas = rows * c->kv_heads;
@@ -323,14 +305,14 @@ int gptrs_cuda_kv8_attention(const gptrs_kv8_cache* c, const gptrs_kv8_attention
     const int rc = kv8_check(c);
     if (rc) return rc;
     GPTRS_REQUIRE(s && s->d_q && s->d_pool && s->d_open && s->d_page_table && s->d_slot && s->d_ctx_len && s->d_length && s->d_out && s->d_status, "null pointer");
-    GPTRS_REQUIRE(s->rows >= 0 && s->rows <= 0x3fffffff && s->n_tiles >= 0, "bad row count");
+    GPTRS_REQUIRE(s->rows >= 0 && s->rows <= 0x3fffffff && s->n_tiles >= 0 && s->n_tiles <= 65535, "bad row count");
     GPTRS_REQUIRE(s->n_tiles == 0 || (s->d_tile_row && s->d_tile_rows), "tiles are missing");
     GPTRS_REQUIRE(s->max_pages >= 1 && s->max_pages * kKv8Tokens < ((int64_t)1 << 31) && s->n_pages >= 1 && s->n_slots >= 1 && s->n_slots <= 0x7fffffff, "bad cache sizes");
     GPTRS_REQUIRE(s->max_ctx_len >= 0 && s->max_ctx_len < ((int64_t)1 << 31), "bad max_ctx_len");
     GPTRS_REQUIRE(s->splits >= 1 && s->splits <= 65535, "bad number of splits");
     GPTRS_REQUIRE(aligned16(s->d_q) && aligned16(s->d_pool) && aligned16(s->d_open) && aligned16(s->d_out) && aligned16(s->d_scratch), "pointers must be 16-byte aligned");
     const int64_t width = (int64_t)c->q_heads * c->dim;
-    AttnParams p = {};
+    Kv8Attention p = {};
     p.ldq = s->ldq ? s->ldq : width;
     GPTRS_REQUIRE(p.ldq >= width && p.ldq % 8 == 0, "rows of queries overlap, or do not start at multiples of 16 bytes");
     GPTRS_REQUIRE(s->splits == 1 || (s->d_scratch && s->scratch_bytes >= gptrs_cuda_kv8_scratch_bytes(c, s->rows, s->n_tiles, s->splits)), "scratch is too small");
@@ -351,10 +333,13 @@ int gptrs_cuda_kv8_attention(const gptrs_kv8_cache* c, const gptrs_kv8_attention
     p.chunk_blocks = std::max(1, ceil_div(seen, s->splits));
     p.part_o = static_cast<float*>(s->d_scratch);
     p.part_ml = p.part_o + (size_t)p.rows * p.q_heads * p.splits * c->dim;
-    // grid.z holds 65535 rows: longer lists go in several launches over their own part of the scratch
-    for (int64_t row = 0; row < s->rows; row += 65535) {
-        AttnParams part = p;
-        part.rows = (int)std::min<int64_t>(65535, s->rows - row);
+    p.tile_row = s->d_tile_row; p.tile_rows = s->d_tile_rows; p.n_tiles = (int)s->n_tiles;
+    // a grid's last dimension holds 65535 rows: longer lists go in several launches over their own part of the scratch
+    const int64_t most = s->n_tiles && s->splits == 1 ? s->rows : 65535;
+    GPTRS_REQUIRE(s->n_tiles == 0 || s->rows <= most, "tiles of more than 65535 rows are not split along the keys");
+    for (int64_t row = 0; row < s->rows; row += most) {
+        Kv8Attention part = p;
+        part.rows = (int)std::min<int64_t>(most, s->rows - row);
         part.q += row * p.ldq; part.slot += row; part.ctx_len += row;
         part.out += row * width;
         part.part_o += row * p.q_heads * p.splits * c->dim;

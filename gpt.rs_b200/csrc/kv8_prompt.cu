@@ -1,0 +1,571 @@
+// Attention over the 8-bit cache for tiles of rows of one sequence (prompts), on the tcgen05 tensor cores.
+//
+// The formula of kv8_attention.cu: t = (s_K scale log2 e) q . a + log2 s_V, w = 2^(t - M), out = sum w b / sum (w / s_V). Whole numbers of 8 bits
+// become f16 in shared memory (exact), the scales of a block of 16 keys meet the scores of its 16 columns, so the matrix products see no scale.
+//
+// One CTA (one per SM) takes the rows of a tile x the query heads of one kv head, as two row tiles of 128 (row = token x group + head), and walks
+// the visible keys in blocks of 128 (8 pages):
+//   S_i[128 x 128] = Q_i . K^T     both operands f16 in shared memory (K-major, 128-byte swizzle), accumulator in tensor memory
+//   softmax                        warps 4 i .. 4 i + 3, a thread per row: running maximum with a lazy rescale (the weights stay below 2^8), weights
+//                                  rounded to f16 and written over the last 64 columns of S_i
+//   O_i[128 x dim] += P_i . V      A = P_i from tensor memory, B = V^T in shared memory (keys contiguous), accumulator in tensor memory
+// Warp 8 issues every product; warps 9 - 12 widen the pages, two of a block each: bytes from global memory to registers ahead of time, f16 into the
+// stage when the products that read it are complete. A thread of theirs takes the 16 bytes that the row kernel's lane would; which 16
+// is chosen so that eight (K) or sixteen (V) threads store to different banks. The order of the keys inside a page is the cache's
+// (pairs 0, 1, 8, 9, 2, 3, ...): P's columns are written in the same order.
+// The score registers: 64 columns at a time, first for the maximum, then again for the weights (columns 64 .. stay in registers between the two),
+// so that 416 threads fit their 152 registers.
+// Every wait is bounded: on a timeout code 3 goes to the status word and every role leaves its loop.
+#include "kv8_attention.cuh"
+#include "umma_common.cuh"
+
+namespace gptrs {
+
+void prefill_tc_fault(int* starve, uint32_t* wait_limit);   // the test switch of paged_prefill_tc.cu
+
+namespace {
+
+constexpr int kRows = 128;                 // of a row tile = lanes of tensor memory
+constexpr int kTiles = 2;
+constexpr int kSoftmaxThreads = kTiles * kRows;
+constexpr int kMmaWarp = kSoftmaxThreads / 32;
+constexpr int kLoadWarps = 4;
+constexpr int kThreads = kSoftmaxThreads + 32 + kLoadWarps * 32;
+constexpr int kKeys = 128;                 // of a block
+constexpr int kPages = kKeys / kKv8Tokens;
+constexpr int kHalfBytes = 128 * 128;      // 128 rows x 64 f16
+constexpr uint32_t kTmemCols = 512;        // S_0, S_1, O_0, O_1
+constexpr uint32_t kOCol = 256, kPCol = 64;
+constexpr float kRescaleStep = 8.f;
+constexpr int kScaleSlots = 4;             // blocks whose scales may be in use at a time are three at most
+
+struct PromptParams {
+    Kv8Attention a;
+    int starve;
+    uint32_t wait_limit;
+};
+
+__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) { umma_bf16(d, a, b, idesc, accumulate); }
+
+__device__ __forceinline__ void tmem_ld_32_async(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ void st_shared_v2(uint32_t addr, uint32_t a, uint32_t b) {
+    asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(addr), "r"(a), "r"(b) : "memory");
+}
+__device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
+    const uint4 v = ld_shared_v4(addr);
+    return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
+
+template <int kDim>
+constexpr size_t prompt_smem() { return (size_t)(kTiles + 2) * kRows * kDim * 2 + 2 * (size_t)kDim * kKeys * 2 + 1024; }
+
+template <int kDim>
+__global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_constant__ PromptParams params) {
+    const Kv8Attention& p = params.a;
+    constexpr int kQBytes = kRows * kDim * 2, kKBytes = kKeys * kDim * 2, kVHalf = kDim * 128;   // a half of V^T: 64 keys
+    constexpr int kC = kDim / 32;
+    constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(kRows >> 4) << 24);                       // f32 accumulator, f16 operands, M = 128
+    constexpr uint32_t kIdescS = kIdesc | ((uint32_t)(kKeys >> 3) << 17), kIdescO = kIdesc | ((uint32_t)(kDim >> 3) << 17);
+
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[kTiles], p_full[kTiles], o_full[kTiles], drained;
+    __shared__ uint32_t tmem_holder;
+    __shared__ int s_begin[kSoftmaxThreads / 32], s_end[kSoftmaxThreads / 32];
+    __shared__ __align__(16) float scales[kScaleSlots][kPages][4];   // s_K scale log2 e, log2 s_V, 1 / s_V
+
+    const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sQ = smem, sK = sQ + kTiles * kQBytes, sV = sK + 2 * kKBytes;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const bool is_softmax = tid < kSoftmaxThreads;
+    const int ti = is_softmax ? tid >> 7 : 0, row = tid & (kRows - 1);
+    const int group = p.group, tq = kRows / group;
+    const int kv_head = blockIdx.x, tile = (int)gridDim.y - 1 - (int)blockIdx.y;   // the longest contexts come last in a chunk: start them first
+
+    pdl_wait();
+    const int row0 = p.tile_row[tile], n_rows = p.tile_rows[tile];
+    if (row0 < 0 || n_rows < 0 || n_rows > kTiles * tq || row0 > p.rows - n_rows) {
+        if (tid == 0) atomicExch(p.status, 2);
+        return;
+    }
+    if (n_rows == 0) return;
+    const int slot = p.slot[row0];
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) { mbar_init(&k_full[i], kLoadWarps); mbar_init(&v_full[i], kLoadWarps); mbar_init(&k_empty[i], 1); mbar_init(&v_empty[i], 1); }
+        for (int i = 0; i < kTiles; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], kRows); mbar_init(&o_full[i], 1); }
+        mbar_init(&drained, 1);
+        mbar_fence_init();
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_holder)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_holder;
+    pdl_launch_dependents();   // every CTA of this grid holds its tensor memory (or has left)
+
+    // ---- a softmax thread's row ------------------------------------------------------------------------------------------------------------
+    const int in_tile = ti * tq + row / group, my_row = row0 + in_tile, my_head = kv_head * group + row % group;
+    bool live = is_softmax && row < tq * group && in_tile < n_rows;   // the output of this row is this thread's
+    int begin = 0, end = 0;
+    float q_scale = 0.f;
+    if (is_softmax) {
+        if (live) {
+            const Kv8Span s = kv8_span(p, my_row);
+            live = s.slot >= 0 && s.slot == slot;
+            if (s.slot >= 0 && s.slot != slot) atomicExch(p.status, 2);   // a tile is of one sequence
+            if (live) { begin = s.begin; end = s.end; }
+        }
+        const int warp_begin = __reduce_min_sync(0xffffffffu, end > begin ? begin : 0x7fffffff), warp_end = __reduce_max_sync(0xffffffffu, end > begin ? end : 0);
+        if (lane == 0) { s_begin[warp] = warp_begin; s_end[warp] = warp_end; }
+        // ---- its query: f16 with a power of two in front (kv8_cache.cuh) -> shared memory --------------------------------------------------------
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + (live ? my_row : row0) * p.ldq + (long long)my_head * kDim);
+        uint4 v[kDim / 8];
+        uint32_t big = 0;
+#pragma unroll
+        for (int c = 0; c < kDim / 8; ++c) {
+            v[c] = live ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+            big = __vmaxu2(big, __vmaxu2(abs_bits_max2(v[c].x, v[c].y), abs_bits_max2(v[c].z, v[c].w)));
+        }
+        const int e = pow2_exponent(widest_half(big));
+        const float factor = e == 128 ? 0.f : pow2(-e);
+        q_scale = e == 128 ? __uint_as_float(0x7fc00000u) : pow2(e);
+        const uint32_t dst = sQ + ti * kQBytes + row * 128;
+#pragma unroll
+        for (int c = 0; c < kDim / 8; ++c)
+            st_shared_v4(dst + (c >> 3) * kHalfBytes + (((c & 7) ^ (row & 7)) << 4), bf16x2_to_f16x2(v[c].x, factor), bf16x2_to_f16x2(v[c].y, factor),
+                         bf16x2_to_f16x2(v[c].z, factor), bf16x2_to_f16x2(v[c].w, factor));
+        fence_proxy_async();
+    }
+    __syncthreads();
+    // keys of this CTA: [first_key, last_key) of the tile, whole blocks of the split's share; nb_t[i] of them for row tile i
+    int tile_end[kTiles], first_key = 0x7fffffff, last_key = 0;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+        tile_end[i] = max(max(s_end[4 * i], s_end[4 * i + 1]), max(s_end[4 * i + 2], s_end[4 * i + 3]));
+        last_key = max(last_key, tile_end[i]);
+        first_key = min(first_key, min(min(s_begin[4 * i], s_begin[4 * i + 1]), min(s_begin[4 * i + 2], s_begin[4 * i + 3])));
+    }
+    int n_blocks = 0, nb_t[kTiles] = {0, 0};
+    if (last_key > 0) {
+        first_key = first_key / kKv8Tokens * kKv8Tokens;
+        const int all = (last_key - first_key + kKeys - 1) / kKeys;
+        const int per = (all + p.splits - 1) / p.splits, skip = min((int)blockIdx.z * per, all);
+        n_blocks = min(per, all - skip);
+        first_key += skip * kKeys;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) nb_t[i] = min(n_blocks, max(0, (tile_end[i] - first_key + kKeys - 1) / kKeys));
+    }
+    bool failed = false;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {   // whole warp
+        if (!failed && !mbar_wait_parked(smem_u32(bar), parity, params.wait_limit)) failed = true;
+        failed = __any_sync(0xffffffffu, failed);
+        return !failed;
+    };
+
+    if (warp > kMmaWarp) {
+        // ================= warps 9 - 12: pages 2 w, 2 w + 1 of every block ===================================================================
+        const int w = warp - kMmaWarp - 1;
+        const int length = p.length[slot < 0 ? 0 : slot];
+        const int end_block = (last_key + kKv8Tokens - 1) / kKv8Tokens;         // of the sequence's blocks of 16 tokens
+        const int kg = lane >> 3, kc = (lane >> 2) & 1, t = lane & 3;           // K: token, chunk of 32 channels, eight channels
+        const int vg = 2 * ((lane & 15) >> 2) + (lane >> 4);                    // V: channel, four tokens
+        enum { kNone, kClosed, kOpen };
+        struct Page { const unsigned char* at; int block, kind; };
+        auto find = [&](int kb, int j) {
+            Page pg = {nullptr, first_key / kKv8Tokens + kb * kPages + 2 * w + j, kNone};
+            if (pg.block >= end_block) return pg;
+            if ((pg.block + 1) * kKv8Tokens > length) { pg.kind = kOpen; return pg; }
+            const int page = kv8_page(p.table, slot, p.max_pages, pg.block, p.n_pages, p.status);
+            if (page < 0) { atomicExch(p.status, 2); return pg; }
+            pg.at = p.pool + ((long long)page * p.kv_heads + kv_head) * kv8_block_bytes(kDim);
+            pg.kind = kClosed;
+            return pg;
+        };
+        auto open_rows = [&](int block, int is_value) {
+            return p.open + (long long)slot * kv8_open_elems(p.kv_heads, kDim) + kv8_open_at(block, p.kv_heads, kv_head, is_value, kDim);
+        };
+        uint4 kb_[2][kC], vb_[2][kC];
+        float2 sc[2];
+        auto load_k = [&](const Page (&pg)[2]) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                if (pg[j].kind != kClosed) continue;
+                sc[j] = __ldg(reinterpret_cast<const float2*>(pg[j].at + 32 * kDim));
+#pragma unroll
+                for (int i = 0; i < kC; ++i)   // two channel chunks and tokens kg, kg + 4 of them
+                    kb_[j][i] = __ldg(reinterpret_cast<const uint4*>(pg[j].at + ((i >> 1) * 2 + kc) * 512 + ((kg + 4 * (i & 1)) * 4 + t) * 16));
+            }
+        };
+        auto load_v = [&](const Page (&pg)[2]) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                if (pg[j].kind != kClosed) continue;
+#pragma unroll
+                for (int i = 0; i < kC; ++i) vb_[j][i] = __ldg(reinterpret_cast<const uint4*>(pg[j].at + 16 * kDim + i * 512 + (vg * 4 + t) * 16));
+            }
+        };
+        auto store_k = [&](const Page& pg, int j, int kb, uint32_t base) {
+            float k_scale = 0.f, v_scale = 1.f;
+            const int page = 2 * w + j;
+            auto at = [&](int i, int r) {   // 16 bytes of token g + 8 r
+                const int g = kg + 4 * (i & 1), key = page * kKv8Tokens + g + 8 * r;
+                return base + (i >> 1) * kHalfBytes + key * 128 + (((4 * kc + t) ^ (key & 7)) << 4);
+            };
+            if (pg.kind == kClosed) {
+                k_scale = sc[j].x; v_scale = sc[j].y;
+#pragma unroll
+                for (int i = 0; i < kC; ++i) {
+                    uint32_t x[8];
+                    kv8_widen(kb_[j][i].x, &x[0], &x[1]); kv8_widen(kb_[j][i].y, &x[2], &x[3]);
+                    kv8_widen(kb_[j][i].z, &x[4], &x[5]); kv8_widen(kb_[j][i].w, &x[6], &x[7]);
+                    st_shared_v4(at(i, 0), x[0], x[1], x[2], x[3]);
+                    st_shared_v4(at(i, 1), x[4], x[5], x[6], x[7]);
+                }
+            } else {
+                // the rows of the block that is not complete, or nothing: zeros
+                const int have = pg.kind == kOpen ? length - pg.block * kKv8Tokens : 0;
+                const __nv_bfloat16* src = pg.kind == kOpen ? open_rows(pg.block, 0) : nullptr;
+                uint4 x[kC][2];
+                uint32_t big = 0, big_v = 0;
+#pragma unroll
+                for (int i = 0; i < kC; ++i)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const int token = kg + 4 * (i & 1) + 8 * r, d = ((i >> 1) * 2 + kc) * 32 + 8 * t;
+                        x[i][r] = token < have ? *reinterpret_cast<const uint4*>(src + token * kDim + d) : make_uint4(0, 0, 0, 0);
+                        const uint4 y = token < have ? *reinterpret_cast<const uint4*>(src + kKv8Tokens * kDim + token * kDim + d) : make_uint4(0, 0, 0, 0);
+                        big = __vmaxu2(big, __vmaxu2(abs_bits_max2(x[i][r].x, x[i][r].y), abs_bits_max2(x[i][r].z, x[i][r].w)));
+                        big_v = __vmaxu2(big_v, __vmaxu2(abs_bits_max2(y.x, y.y), abs_bits_max2(y.z, y.w)));
+                    }
+                const int e = pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big))), ev = pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big_v)));
+                const float factor = e == 128 ? 0.f : pow2(-e);
+                if (pg.kind == kOpen) {
+                    k_scale = e == 128 ? __uint_as_float(0x7fc00000u) : pow2(e);
+                    v_scale = ev == 128 ? __uint_as_float(0x7fc00000u) : pow2(ev);
+                }
+#pragma unroll
+                for (int i = 0; i < kC; ++i)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                        st_shared_v4(at(i, r), bf16x2_to_f16x2(x[i][r].x, factor), bf16x2_to_f16x2(x[i][r].y, factor), bf16x2_to_f16x2(x[i][r].z, factor),
+                                     bf16x2_to_f16x2(x[i][r].w, factor));
+            }
+            if (lane == 0) {
+                // a value scale that is not a number makes the weights none where the key is seen, and nothing else
+                float* s = scales[kb % kScaleSlots][page];
+                s[0] = k_scale * p.scale_log2;
+                s[1] = __log2f(v_scale);
+                s[2] = v_scale == v_scale ? __fdividef(1.f, v_scale) : 1.f;
+            }
+        };
+        auto store_v = [&](const Page& pg, int j, uint32_t base) {
+            const int page = 2 * w + j;
+            auto at = [&](int d) {   // four keys of channel d (d % 8 = vg)
+                return base + (page >> 2) * kVHalf + d * 128 + (((2 * (page & 3) + (t >> 1)) ^ (d & 7)) << 4) + (t & 1) * 8;
+            };
+            if (pg.kind == kClosed) {
+#pragma unroll
+                for (int i = 0; i < kC; ++i) {
+                    const uint32_t b[4] = {vb_[j][i].x, vb_[j][i].y, vb_[j][i].z, vb_[j][i].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t lo, hi;
+                        kv8_widen(b[k], &lo, &hi);
+                        st_shared_v2(at(32 * i + 8 * k + vg), lo, hi);
+                    }
+                }
+            } else {
+                const int have = pg.kind == kOpen ? length - pg.block * kKv8Tokens : 0;
+                const unsigned short* src = pg.kind == kOpen ? reinterpret_cast<const unsigned short*>(open_rows(pg.block, 1)) : nullptr;
+                uint32_t big = 0;   // of the whole block, as in store_k
+                for (int i = lane; i < have * (kDim / 2); i += 32) big = __vmaxu2(big, reinterpret_cast<const uint32_t*>(src)[i] & 0x7fff7fffu);
+                const int e = pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big)));
+                const float factor = e == 128 ? 0.f : pow2(-e);
+#pragma unroll 1
+                for (int i = 0; i < 4 * kC; ++i) {
+                    const int d = 8 * i + vg;
+                    uint32_t x[2];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const int token = 2 * t + 8 * r;
+                        const uint32_t lo = token < have ? src[token * kDim + d] : 0u, hi = token + 1 < have ? src[(token + 1) * kDim + d] : 0u;
+                        x[r] = bf16x2_to_f16x2(lo | hi << 16, factor);
+                    }
+                    st_shared_v2(at(d), x[0], x[1]);
+                }
+            }
+        };
+        Page pages[2], next[2];
+        if (n_blocks > 0) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) pages[j] = find(0, j);
+            load_k(pages);
+        }
+        for (int kb = 0; kb < n_blocks; ++kb) {
+            const int st = kb & 1;
+            load_v(pages);
+            if (kb >= 2 && !wait(&k_empty[st], (uint32_t)((kb - 2) >> 1) & 1u)) break;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) store_k(pages[j], j, kb, sK + st * kKBytes);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0 && !(params.starve && kb == 0)) mbar_arrive(&k_full[st]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) next[j] = find(kb + 1, j);
+            if (kb + 1 < n_blocks) load_k(next);
+            if (kb >= 2 && !wait(&v_empty[st], (uint32_t)((kb - 2) >> 1) & 1u)) break;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) { store_v(pages[j], j, sV + st * 2 * kVHalf); pages[j] = next[j]; }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_full[st]);
+        }
+        if (failed && lane == 0) atomicExch(p.status, 3);
+    } else if (warp == kMmaWarp) {
+        // ================= warp 8: every product =================================================================================================
+        const bool one = elect_one();
+        auto issue_s = [&](int i, int kb) {
+            if (one) {
+                const uint64_t a_desc = make_smem_desc(sQ + i * kQBytes), b_desc = make_smem_desc(sK + (kb & 1) * kKBytes);
+#pragma unroll
+                for (int ks = 0; ks < kDim / 16; ++ks) {
+                    const uint64_t off = (uint64_t)((ks >> 2) * (kHalfBytes >> 4) + 2 * (ks & 3));
+                    umma_f16(tmem + (uint32_t)i * kKeys, a_desc + off, b_desc + off, kIdescS, ks > 0 ? 1u : 0u);
+                }
+                umma_commit(&s_full[i]);
+            }
+            __syncwarp();
+        };
+        if (n_blocks > 0 && wait(&k_full[0], 0)) {
+            tc_fence_after();
+            for (int i = 0; i < kTiles; ++i) if (nb_t[i] > 0) issue_s(i, 0);
+            if (one) umma_commit(&k_empty[0]);
+            __syncwarp();
+        }
+        for (int kb = 0; kb < n_blocks && !failed; ++kb) {
+            const int st = kb & 1;
+            bool v_ready = false, k_ready = false;
+            for (int i = 0; i < kTiles && !failed; ++i) {
+                if (kb < nb_t[i]) {
+                    if (!wait(&p_full[i], (uint32_t)kb & 1u)) break;
+                    if (!v_ready) {
+                        if (!wait(&v_full[st], (uint32_t)(kb >> 1) & 1u)) break;
+                        v_ready = true;
+                    }
+                    tc_fence_after();
+                    if (one) {
+                        const uint64_t b_desc = make_smem_desc(sV + st * 2 * kVHalf);
+#pragma unroll
+                        for (int ks = 0; ks < kKeys / 16; ++ks)
+                            umma_bf16_ts(tmem + kOCol + (uint32_t)i * kDim, tmem + (uint32_t)i * kKeys + kPCol + 8u * ks,
+                                         b_desc + (uint64_t)((ks >> 2) * (kVHalf >> 4) + 2 * (ks & 3)), kIdescO, (kb > 0 || ks > 0) ? 1u : 0u);
+                        if (kb == nb_t[i] - 1) umma_commit(&o_full[i]);
+                    }
+                    __syncwarp();
+                }
+                if (kb + 1 < nb_t[i]) {
+                    if (!k_ready) {
+                        if (!wait(&k_full[st ^ 1], (uint32_t)((kb + 1) >> 1) & 1u)) break;
+                        k_ready = true;
+                        tc_fence_after();
+                    }
+                    issue_s(i, kb + 1);
+                }
+            }
+            if (failed) break;
+            if (one) {
+                umma_commit(&v_empty[st]);
+                if (kb + 1 < n_blocks) umma_commit(&k_empty[st ^ 1]);
+            }
+            __syncwarp();
+        }
+        if (failed) {   // products in flight read shared and tensor memory: let them end before the CTA does
+            if (one) umma_commit(&drained);
+            __syncwarp();
+            mbar_wait_parked(smem_u32(&drained), 0, params.wait_limit);
+            if (lane == 0) atomicExch(p.status, 3);
+        }
+    } else {
+        // ================= warps 0 - 7: a row per thread =========================================================================================
+        const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t t_s = t_lane + (uint32_t)ti * kKeys, t_p = t_s + kPCol, t_o = t_lane + kOCol + (uint32_t)ti * kDim;
+        const int my_blocks = nb_t[ti];
+        const uint32_t s_bar = smem_u32(&s_full[ti]), p_bar = smem_u32(&p_full[ti]), sc0 = smem_u32(&scales[0][0][0]);
+        float m_run = -1e30f, l_run = 0.f;
+        for (int kb = 0; kb < my_blocks; ++kb) {
+            if (!mbar_wait_parked(s_bar, (uint32_t)kb & 1u, params.wait_limit)) failed = true;
+            failed = __any_sync(0xffffffffu, failed);
+            if (failed) break;
+            tc_fence_after();
+            const uint32_t sc = sc0 + (uint32_t)(kb % kScaleSlots) * (kPages * 16);
+            const int key0 = first_key + kb * kKeys;
+            const bool whole = __all_sync(0xffffffffu, begin <= key0 && end >= key0 + kKeys);   // this warp's rows see all of the block
+            uint32_t s[64];
+            float m_blk = -INFINITY;
+            auto load = [&](int half) {
+                tmem_ld_32_async(t_s + 64u * half, s);
+                tmem_ld_32_async(t_s + 64u * half + 32u, s + 32);
+                tmem_wait_ld();
+            };
+            auto largest = [&](int half) {
+#pragma unroll
+                for (int pg = 0; pg < 4; ++pg) {
+                    const float4 x = ld_shared_f4(sc + (4 * half + pg) * 16);
+                    float mx[2] = {-INFINITY, -INFINITY};
+                    const int key = key0 + 64 * half + 16 * pg;
+                    if (whole) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) mx[j & 1] = fmaxf(mx[j & 1], __uint_as_float(s[16 * pg + j]));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (key + j >= begin && key + j < end) mx[j & 1] = fmaxf(mx[j & 1], __uint_as_float(s[16 * pg + j]));
+                    }
+                    m_blk = fmaxf(m_blk, fmaf(fmaxf(mx[0], mx[1]), x.x * q_scale, x.y));
+                }
+            };
+            load(0);
+            largest(0);
+            load(1);
+            largest(1);
+            // the reference moves only when a maximum is more than 2^8 above it: the quotient is the same, the weights stay below 2^8
+            float alpha = 1.f;
+            if (m_blk > m_run + kRescaleStep || (kb == 0 && m_blk > m_run)) {
+                alpha = kv8_exp2(m_run - m_blk);
+                m_run = m_blk;
+            }
+            float sum = 0.f;
+            auto weights = [&](int half) {   // over the scores: pairs of weights in the order of V's keys
+#pragma unroll
+                for (int pg = 0; pg < 4; ++pg) {
+                    const float4 x = ld_shared_f4(sc + (4 * half + pg) * 16);
+                    const float c = x.x * q_scale, b = x.y - m_run;
+                    const uint64_t c2 = pair_of(c, c), b2 = pair_of(b, b);
+                    uint64_t part = 0;
+                    uint32_t packed[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {   // keys 2 i, 2 i + 1
+                        const float2 tt = split(fma2(pair_of(__uint_as_float(s[16 * pg + 2 * i]), __uint_as_float(s[16 * pg + 2 * i + 1])), c2, b2));
+                        float w0 = kv8_exp2(tt.x), w1 = kv8_exp2(tt.y);
+                        if (!whole) {
+                            const int key = key0 + 64 * half + 16 * pg + 2 * i;
+                            w0 = key >= begin && key < end ? w0 : 0.f;
+                            w1 = key + 1 >= begin && key + 1 < end ? w1 : 0.f;
+                        }
+                        part = add2(part, pair_of(w0, w1));
+                        packed[i < 4 ? 2 * i : 2 * (i - 4) + 1] = pack_f16x2(w0, w1);
+                    }
+                    const float2 ps = split(part);
+                    sum = fmaf(ps.x + ps.y, x.z, sum);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s[8 * pg + i] = packed[i];   // (all scores of this and earlier pages are consumed)
+                }
+                tmem_st_32(t_p + 32u * half, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+            };
+            weights(1);
+            load(0);
+            weights(0);
+            if (kb > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {   // the tile's previous product with V is complete: it was issued before this S
+#pragma unroll 1
+                for (int c = 0; c < kDim / 32; ++c) {
+                    uint32_t r[32];
+                    tmem_ld_32_async(t_o + 32u * c, r);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+                    tmem_st_32(t_o + 32u * c, r);
+                }
+            }
+            l_run = fmaf(l_run, alpha, sum);
+            asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+            tc_fence_before();
+            mbar_arrive_addr(p_bar);
+        }
+        // ---- the output, or this split's part of it --------------------------------------------------------------------------------------------
+        if (my_blocks > 0 && !failed) {
+            if (!mbar_wait_parked(smem_u32(&o_full[ti]), 0, params.wait_limit)) failed = true;
+            failed = __any_sync(0xffffffffu, failed);
+        }
+        const long long at = (long long)my_row * p.q_heads + my_head;
+        if (!failed && p.splits == 1) {
+            tc_fence_after();
+            const float inv = l_run == 0.f ? 0.f : __fdividef(1.f, l_run);
+            uint4* dst = reinterpret_cast<uint4*>(p.out + at * kDim);
+#pragma unroll 1
+            for (int c = 0; c < kDim / 32; ++c) {
+                float o[32];
+                if (my_blocks > 0) {
+                    tmem_ld_32(t_o + 32u * c, o);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0.f;
+                }
+                if (live) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        dst[4 * c + i] = make_uint4(pack_bf16x2(o[8 * i] * inv, o[8 * i + 1] * inv), pack_bf16x2(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
+                                                    pack_bf16x2(o[8 * i + 4] * inv, o[8 * i + 5] * inv), pack_bf16x2(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+                }
+            }
+        } else if (!failed) {
+            tc_fence_after();
+            const long long part = at * p.splits + blockIdx.z;
+            const bool seen = my_blocks > 0 && (l_run != 0.f);
+            if (live) { p.part_ml[2 * part] = seen ? m_run : -INFINITY; p.part_ml[2 * part + 1] = seen ? l_run : 0.f; }
+            if (my_blocks > 0) {
+                float4* dst = reinterpret_cast<float4*>(p.part_o + part * kDim);
+#pragma unroll 1
+                for (int c = 0; c < kDim / 32; ++c) {
+                    float o[32];
+                    tmem_ld_32(t_o + 32u * c, o);
+                    if (live) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) dst[8 * c + i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    }
+                }
+            }
+        }
+        if (failed && lane == 0) atomicExch(p.status, 3);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+template <int kDim>
+int launch_prompt(const PromptParams& p, cudaStream_t stream) {
+    static PerDeviceOnce attr_once;
+    if (attr_once.first_time())
+        GPTRS_CUDA_OK(cudaFuncSetAttribute(kv8_prompt_kernel<kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<kDim>()));
+    return launch_kernel(kv8_prompt_kernel<kDim>, dim3((unsigned)p.a.kv_heads, (unsigned)p.a.n_tiles, (unsigned)p.a.splits), dim3(kThreads), prompt_smem<kDim>(), stream, 1, p);
+}
+
+}  // namespace
+
+int kv8_prompt_attention(const Kv8Attention& a, int dim, cudaStream_t stream) {
+    PromptParams p = {};
+    p.a = a;
+    prefill_tc_fault(&p.starve, &p.wait_limit);
+    return dim == 64 ? launch_prompt<64>(p, stream) : launch_prompt<128>(p, stream);
+}
+
+}  // namespace gptrs

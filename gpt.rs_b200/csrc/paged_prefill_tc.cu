@@ -423,6 +423,12 @@ int g_prefill_starve = 0;                // test switch: see gptrs_cuda_debug_pr
 uint32_t g_prefill_wait_limit = 0;
 
 }  // namespace
+
+void prefill_tc_fault(int* starve, uint32_t* wait_limit) {
+    *starve = g_prefill_starve;
+    *wait_limit = (g_prefill_starve && g_prefill_wait_limit) ? g_prefill_wait_limit : kWaitLimit;
+}
+
 }  // namespace gptrs
 
 using namespace gptrs;
