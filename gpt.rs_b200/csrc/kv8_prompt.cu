@@ -6,16 +6,18 @@
 // One CTA (one per SM) takes the rows of a tile x the query heads of one kv head, as two row tiles of 128 (row = token x group + head), and walks
 // the visible keys in blocks of 128 (8 pages):
 //   S_i[128 x 128] = Q_i . K^T     both operands f16 in shared memory (K-major, 128-byte swizzle), accumulator in tensor memory
-//   softmax                        warps 4 i .. 4 i + 3, a thread per row: running maximum with a lazy rescale (the weights stay below 2^8), weights
-//                                  rounded to f16 and written over the last 64 columns of S_i
+//   softmax                        warps 4 i .. 4 i + 3, a thread per row, in one pass over its scores: the reference M stays what it is until a weight would
+//                                  no longer be an f16 (a page's weights add up to more than 2^15), so there is no pass for the maximum. Weights
+//                                  go as f16 over the first 64 columns of S_i; a quarter of the exponentials is computed on the multiply-add
+//                                  units, which have more room than the special function unit
 //   O_i[128 x dim] += P_i . V      A = P_i from tensor memory, B = V^T in shared memory (keys contiguous), accumulator in tensor memory
-// Warp 8 issues every product; warps 9 - 12 widen the pages, two of a block each: bytes from global memory to registers ahead of time, f16 into the
+// Warp 12 issues every product; warps 8 - 11 widen the pages, two of a block each: bytes from global memory to registers ahead of time, f16 into the
 // stage when the products that read it are complete. A thread of theirs takes the 16 bytes that the row kernel's lane would; which 16
 // is chosen so that eight (K) or sixteen (V) threads store to different banks. The order of the keys inside a page is the cache's
 // (pairs 0, 1, 8, 9, 2, 3, ...): P's columns are written in the same order.
-// The score registers: 64 columns at a time, first for the maximum, then again for the weights (columns 64 .. stay in registers between the two),
-// so that 416 threads fit their 152 registers.
 // Every wait is bounded: on a timeout code 3 goes to the status word and every role leaves its loop.
+#include <type_traits>
+
 #include "kv8_attention.cuh"
 #include "umma_common.cuh"
 
@@ -28,15 +30,15 @@ namespace {
 constexpr int kRows = 128;                 // of a row tile = lanes of tensor memory
 constexpr int kTiles = 2;
 constexpr int kSoftmaxThreads = kTiles * kRows;
-constexpr int kMmaWarp = kSoftmaxThreads / 32;
 constexpr int kLoadWarps = 4;
-constexpr int kThreads = kSoftmaxThreads + 32 + kLoadWarps * 32;
+constexpr int kLoadWarp = kSoftmaxThreads / 32, kMmaWarp = kLoadWarp + kLoadWarps;
+constexpr int kThreads = kSoftmaxThreads + kLoadWarps * 32 + 32;
 constexpr int kKeys = 128;                 // of a block
 constexpr int kPages = kKeys / kKv8Tokens;
 constexpr int kHalfBytes = 128 * 128;      // 128 rows x 64 f16
 constexpr uint32_t kTmemCols = 512;        // S_0, S_1, O_0, O_1
-constexpr uint32_t kOCol = 256, kPCol = 64;
-constexpr float kRescaleStep = 8.f;
+constexpr uint32_t kOCol = 256;
+constexpr float kLargestSum = 32768.f;     // of a page's weights: each is an f16 then
 constexpr int kScaleSlots = 4;             // blocks whose scales may be in use at a time are three at most
 
 struct PromptParams {
@@ -58,11 +60,38 @@ __device__ __forceinline__ void tmem_ld_32_async(uint32_t taddr, uint32_t* r) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+                 "r"(r[15])
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
     return d;
+}
+// 2^t of a pair on the multiply-add units: t = n + f with f in [-1/2, 1/2], 2^f by the cubic that is nearest to it in relative error there (7.5e-5,
+// a sixth of f16's rounding), n added to the exponent. t is held to -126 .. 127.
+__device__ __forceinline__ float2 exp2_pair(uint64_t t2) {
+    const float2 t = split(t2);
+    const uint64_t x = pair_of(fminf(fmaxf(t.x, -126.f), 127.f), fminf(fmaxf(t.y, -126.f), 127.f));
+    const uint64_t y = add2(x, pair_of(12582912.f, 12582912.f));                    // 1.5 * 2^23: n in the lowest bits
+    const uint64_t n = add2(y, pair_of(-12582912.f, -12582912.f));
+    const uint64_t f = fma2(n, pair_of(-1.f, -1.f), x);
+    uint64_t p = fma2(f, pair_of(0.05517166853f, 0.05517166853f), pair_of(0.24261112511f, 0.24261112511f));
+    p = fma2(p, f, pair_of(0.69326096773f, 0.69326096773f));
+    p = fma2(p, f, pair_of(0.99992805719f, 0.99992805719f));
+    const float2 m = split(p), k = split(y);
+    return make_float2(__int_as_float(__float_as_int(m.x) + (__float_as_int(k.x) << 23)), __int_as_float(__float_as_int(m.y) + (__float_as_int(k.y) << 23)));
 }
 __device__ __forceinline__ void st_shared_v2(uint32_t addr, uint32_t a, uint32_t b) {
     asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(addr), "r"(a), "r"(b) : "memory");
@@ -181,27 +210,38 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         return !failed;
     };
 
-    if (warp > kMmaWarp) {
-        // ================= warps 9 - 12: pages 2 w, 2 w + 1 of every block ===================================================================
-        const int w = warp - kMmaWarp - 1;
+    if (warp >= kLoadWarp && warp < kMmaWarp) {
+        // ================= warps 8 - 11: pages 2 w, 2 w + 1 of every block ===================================================================
+        const int w = warp - kLoadWarp;
         const int length = p.length[slot < 0 ? 0 : slot];
         const int end_block = (last_key + kKv8Tokens - 1) / kKv8Tokens;         // of the sequence's blocks of 16 tokens
         const int kg = lane >> 3, kc = (lane >> 2) & 1, t = lane & 3;           // K: token, chunk of 32 channels, eight channels
         const int vg = 2 * ((lane & 15) >> 2) + (lane >> 4);                    // V: channel, four tokens
         enum { kNone, kClosed, kOpen };
         struct Page { const unsigned char* at; int block, kind; };
-        auto find = [&](int kb, int j) {
-            Page pg = {nullptr, first_key / kKv8Tokens + kb * kPages + 2 * w + j, kNone};
+        auto block_of = [&](int kb, int j) { return first_key / kKv8Tokens + kb * kPages + 2 * w + j; };
+        // entry of the page table, asked for a block before it is needed (the load is not waited for here)
+        auto number = [&](int kb, int j) {
+            const int block = block_of(kb, j);
+            return block < end_block && (block + 1) * kKv8Tokens <= length ? p.table[slot * p.max_pages + block] : 0;
+        };
+        auto find = [&](int kb, int j, int page) {
+            Page pg = {nullptr, block_of(kb, j), kNone};
             if (pg.block >= end_block) return pg;
             if ((pg.block + 1) * kKv8Tokens > length) { pg.kind = kOpen; return pg; }
-            const int page = kv8_page(p.table, slot, p.max_pages, pg.block, p.n_pages, p.status);
-            if (page < 0) { atomicExch(p.status, 2); return pg; }
+            if (page < 0 || page >= p.n_pages) { atomicExch(p.status, 2); return pg; }
             pg.at = p.pool + ((long long)page * p.kv_heads + kv_head) * kv8_block_bytes(kDim);
             pg.kind = kClosed;
             return pg;
         };
         auto open_rows = [&](int block, int is_value) {
             return p.open + (long long)slot * kv8_open_elems(p.kv_heads, kDim) + kv8_open_at(block, p.kv_heads, kv_head, is_value, kDim);
+        };
+        auto exponent = [&](const void* rows, int have) {   // of the largest magnitude of `have` bf16 rows
+            uint32_t big = 0;
+#pragma unroll 1
+            for (int i = lane; i < have * (kDim / 2); i += 32) big = __vmaxu2(big, static_cast<const uint32_t*>(rows)[i] & 0x7fff7fffu);
+            return pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big)));
         };
         uint4 kb_[2][kC], vb_[2][kC];
         float2 sc[2];
@@ -241,40 +281,27 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                     st_shared_v4(at(i, 1), x[4], x[5], x[6], x[7]);
                 }
             } else {
-                // the rows of the block that is not complete, or nothing: zeros
+                // the rows of the block that is not complete, or nothing: zeros (once in a sequence: short code rather than fast)
                 const int have = pg.kind == kOpen ? length - pg.block * kKv8Tokens : 0;
-                const __nv_bfloat16* src = pg.kind == kOpen ? open_rows(pg.block, 0) : nullptr;
-                uint4 x[kC][2];
-                uint32_t big = 0, big_v = 0;
-#pragma unroll
-                for (int i = 0; i < kC; ++i)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const int token = kg + 4 * (i & 1) + 8 * r, d = ((i >> 1) * 2 + kc) * 32 + 8 * t;
-                        x[i][r] = token < have ? *reinterpret_cast<const uint4*>(src + token * kDim + d) : make_uint4(0, 0, 0, 0);
-                        const uint4 y = token < have ? *reinterpret_cast<const uint4*>(src + kKv8Tokens * kDim + token * kDim + d) : make_uint4(0, 0, 0, 0);
-                        big = __vmaxu2(big, __vmaxu2(abs_bits_max2(x[i][r].x, x[i][r].y), abs_bits_max2(x[i][r].z, x[i][r].w)));
-                        big_v = __vmaxu2(big_v, __vmaxu2(abs_bits_max2(y.x, y.y), abs_bits_max2(y.z, y.w)));
-                    }
-                const int e = pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big))), ev = pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big_v)));
+                const __nv_bfloat16* src = open_rows(pg.block, 0);
+                const int e = exponent(src, have), ev = exponent(src + kKv8Tokens * kDim, have);
                 const float factor = e == 128 ? 0.f : pow2(-e);
                 if (pg.kind == kOpen) {
                     k_scale = e == 128 ? __uint_as_float(0x7fc00000u) : pow2(e);
                     v_scale = ev == 128 ? __uint_as_float(0x7fc00000u) : pow2(ev);
                 }
-#pragma unroll
-                for (int i = 0; i < kC; ++i)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r)
-                        st_shared_v4(at(i, r), bf16x2_to_f16x2(x[i][r].x, factor), bf16x2_to_f16x2(x[i][r].y, factor), bf16x2_to_f16x2(x[i][r].z, factor),
-                                     bf16x2_to_f16x2(x[i][r].w, factor));
+#pragma unroll 1
+                for (int i = 0; i < 2 * kC; ++i) {
+                    const int token = kg + 4 * ((i >> 1) & 1) + 8 * (i & 1), d = ((i >> 2) * 2 + kc) * 32 + 8 * t;
+                    const uint4 x = token < have ? *reinterpret_cast<const uint4*>(src + token * kDim + d) : make_uint4(0, 0, 0, 0);
+                    st_shared_v4(at(i >> 1, i & 1), bf16x2_to_f16x2(x.x, factor), bf16x2_to_f16x2(x.y, factor), bf16x2_to_f16x2(x.z, factor), bf16x2_to_f16x2(x.w, factor));
+                }
             }
             if (lane == 0) {
-                // a value scale that is not a number makes the weights none where the key is seen, and nothing else
                 float* s = scales[kb % kScaleSlots][page];
                 s[0] = k_scale * p.scale_log2;
                 s[1] = __log2f(v_scale);
-                s[2] = v_scale == v_scale ? __fdividef(1.f, v_scale) : 1.f;
+                s[2] = k_scale == k_scale ? __fdividef(1.f, v_scale) : k_scale;
             }
         };
         auto store_v = [&](const Page& pg, int j, uint32_t base) {
@@ -295,10 +322,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 }
             } else {
                 const int have = pg.kind == kOpen ? length - pg.block * kKv8Tokens : 0;
-                const unsigned short* src = pg.kind == kOpen ? reinterpret_cast<const unsigned short*>(open_rows(pg.block, 1)) : nullptr;
-                uint32_t big = 0;   // of the whole block, as in store_k
-                for (int i = lane; i < have * (kDim / 2); i += 32) big = __vmaxu2(big, reinterpret_cast<const uint32_t*>(src)[i] & 0x7fff7fffu);
-                const int e = pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big)));
+                const unsigned short* src = reinterpret_cast<const unsigned short*>(open_rows(pg.block, 1));
+                const int e = exponent(src, have);
                 const float factor = e == 128 ? 0.f : pow2(-e);
 #pragma unroll 1
                 for (int i = 0; i < 4 * kC; ++i) {
@@ -315,10 +340,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             }
         };
         Page pages[2], next[2];
+        int numbers[2];
         if (n_blocks > 0) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) pages[j] = find(0, j);
+            for (int j = 0; j < 2; ++j) pages[j] = find(0, j, number(0, j));
             load_k(pages);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) numbers[j] = number(1, j);
         }
         for (int kb = 0; kb < n_blocks; ++kb) {
             const int st = kb & 1;
@@ -330,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             __syncwarp();
             if (lane == 0 && !(params.starve && kb == 0)) mbar_arrive(&k_full[st]);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) next[j] = find(kb + 1, j);
+            for (int j = 0; j < 2; ++j) { next[j] = find(kb + 1, j, numbers[j]); numbers[j] = number(kb + 2, j); }
             if (kb + 1 < n_blocks) load_k(next);
             if (kb >= 2 && !wait(&v_empty[st], (uint32_t)((kb - 2) >> 1) & 1u)) break;
 #pragma unroll
@@ -341,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         }
         if (failed && lane == 0) atomicExch(p.status, 3);
     } else if (warp == kMmaWarp) {
-        // ================= warp 8: every product =================================================================================================
+        // ================= warp 12: every product =================================================================================================
         const bool one = elect_one();
         auto issue_s = [&](int i, int kb) {
             if (one) {
@@ -376,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                         const uint64_t b_desc = make_smem_desc(sV + st * 2 * kVHalf);
 #pragma unroll
                         for (int ks = 0; ks < kKeys / 16; ++ks)
-                            umma_bf16_ts(tmem + kOCol + (uint32_t)i * kDim, tmem + (uint32_t)i * kKeys + kPCol + 8u * ks,
+                            umma_bf16_ts(tmem + kOCol + (uint32_t)i * kDim, tmem + (uint32_t)i * kKeys + 8u * ks,
                                          b_desc + (uint64_t)((ks >> 2) * (kVHalf >> 4) + 2 * (ks & 3)), kIdescO, (kb > 0 || ks > 0) ? 1u : 0u);
                         if (kb == nb_t[i] - 1) umma_commit(&o_full[i]);
                     }
@@ -407,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     } else {
         // ================= warps 0 - 7: a row per thread =========================================================================================
         const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t t_s = t_lane + (uint32_t)ti * kKeys, t_p = t_s + kPCol, t_o = t_lane + kOCol + (uint32_t)ti * kDim;
+        const uint32_t t_s = t_lane + (uint32_t)ti * kKeys, t_o = t_lane + kOCol + (uint32_t)ti * kDim;
         const int my_blocks = nb_t[ti];
         const uint32_t s_bar = smem_u32(&s_full[ti]), p_bar = smem_u32(&p_full[ti]), sc0 = smem_u32(&scales[0][0][0]);
         float m_run = -1e30f, l_run = 0.f;
@@ -419,83 +447,106 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             const uint32_t sc = sc0 + (uint32_t)(kb % kScaleSlots) * (kPages * 16);
             const int key0 = first_key + kb * kKeys;
             const bool whole = __all_sync(0xffffffffu, begin <= key0 && end >= key0 + kKeys);   // this warp's rows see all of the block
-            uint32_t s[64];
-            float m_blk = -INFINITY;
-            auto load = [&](int half) {
-                tmem_ld_32_async(t_s + 64u * half, s);
-                tmem_ld_32_async(t_s + 64u * half + 32u, s + 32);
-                tmem_wait_ld();
-            };
-            auto largest = [&](int half) {
+            uint32_t s[2][32];
+            float sum = 0.f;
+            // Raises the reference of rows whose weights of chunk c came out too large, to about that chunk's maximum: what was computed with the old one
+            // (output, sums, this block's weights so far) is scaled down. Rare behind a sequence's first keys.
+            auto raise = [&](const uint32_t* a, int c, bool over) {
+                float top = m_run;
 #pragma unroll
-                for (int pg = 0; pg < 4; ++pg) {
-                    const float4 x = ld_shared_f4(sc + (4 * half + pg) * 16);
-                    float mx[2] = {-INFINITY, -INFINITY};
-                    const int key = key0 + 64 * half + 16 * pg;
-                    if (whole) {
+                for (int j = 0; j < 32; ++j) {
+                    const float4 x = ld_shared_f4(sc + (2 * c + j / 16) * 16);
+                    const int key = key0 + 32 * c + j;
+                    if (over && key >= begin && key < end) top = fmaxf(top, fmaf(__uint_as_float(a[j]), x.x * q_scale, x.y));
+                }
+                // by whole powers of two, so that scaling f16 weights rounds none of them (but the first time, when there are none)
+                const float up = m_run == -1e30f ? 1e30f : floorf(top - m_run), alpha = kv8_exp2(-up);
+                m_run = m_run == -1e30f ? top : m_run + up;
+                l_run *= alpha;
+                sum *= alpha;
+                if (kb > 0) {   // the tile's previous product with V is complete: it was issued before this S
+#pragma unroll 1
+                    for (int i = 0; i < kDim / 16; ++i) {
+                        uint32_t r[16];
+                        tmem_ld_16(t_o + 16u * i, r);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) mx[j & 1] = fmaxf(mx[j & 1], __uint_as_float(s[16 * pg + j]));
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (key + j >= begin && key + j < end) mx[j & 1] = fmaxf(mx[j & 1], __uint_as_float(s[16 * pg + j]));
+                        for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
+                        tmem_st_16(t_o + 16u * i, r);
                     }
-                    m_blk = fmaxf(m_blk, fmaf(fmaxf(mx[0], mx[1]), x.x * q_scale, x.y));
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+#pragma unroll 1
+                for (int i = 0; i < c; ++i) {
+                    uint32_t r[16];
+                    tmem_ld_16(t_s + 16u * i, r);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&r[k]));   // alpha itself may be less than any f16
+                        r[k] = pack_f16x2(w.x * alpha, w.y * alpha);
+                    }
+                    tmem_st_16(t_s + 16u * i, r);
                 }
             };
-            load(0);
-            largest(0);
-            load(1);
-            largest(1);
-            // the reference moves only when a maximum is more than 2^8 above it: the quotient is the same, the weights stay below 2^8
-            float alpha = 1.f;
-            if (m_blk > m_run + kRescaleStep || (kb == 0 && m_blk > m_run)) {
-                alpha = kv8_exp2(m_run - m_blk);
-                m_run = m_blk;
-            }
-            float sum = 0.f;
-            auto weights = [&](int half) {   // over the scores: pairs of weights in the order of V's keys
+            // Weights of the 32 scores of chunk c, packed in the order of V's keys; returns whether a page's sum is too large for f16 weights (or no number)
+            auto weigh = [&](const uint32_t* a, int c, auto all_seen, uint32_t (&packed)[16], float (&ps)[2]) {
+                constexpr bool kWhole = decltype(all_seen)::value;
+                bool fits = true;
 #pragma unroll
-                for (int pg = 0; pg < 4; ++pg) {
-                    const float4 x = ld_shared_f4(sc + (4 * half + pg) * 16);
-                    const float c = x.x * q_scale, b = x.y - m_run;
-                    const uint64_t c2 = pair_of(c, c), b2 = pair_of(b, b);
+                for (int pg = 0; pg < 2; ++pg) {
+                    const float4 x = ld_shared_f4(sc + (2 * c + pg) * 16);
+                    const float cq = x.x * q_scale, b = x.y - m_run;
+                    const uint64_t c2 = pair_of(cq, cq), b2 = pair_of(b, b);
                     uint64_t part = 0;
-                    uint32_t packed[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {   // keys 2 i, 2 i + 1
-                        const float2 tt = split(fma2(pair_of(__uint_as_float(s[16 * pg + 2 * i]), __uint_as_float(s[16 * pg + 2 * i + 1])), c2, b2));
-                        float w0 = kv8_exp2(tt.x), w1 = kv8_exp2(tt.y);
-                        if (!whole) {
-                            const int key = key0 + 64 * half + 16 * pg + 2 * i;
-                            w0 = key >= begin && key < end ? w0 : 0.f;
-                            w1 = key + 1 >= begin && key + 1 < end ? w1 : 0.f;
+                        const uint64_t t2 = fma2(pair_of(__uint_as_float(a[16 * pg + 2 * i]), __uint_as_float(a[16 * pg + 2 * i + 1])), c2, b2);
+                        float2 w;
+                        if (kWhole && (i & 3) == 3) {
+                            w = exp2_pair(t2);
+                        } else {
+                            const float2 t = split(t2);
+                            w = make_float2(kv8_exp2(t.x), kv8_exp2(t.y));
                         }
-                        part = add2(part, pair_of(w0, w1));
-                        packed[i < 4 ? 2 * i : 2 * (i - 4) + 1] = pack_f16x2(w0, w1);
+                        if (!kWhole) {
+                            const int key = key0 + 32 * c + 16 * pg + 2 * i;
+                            w.x = key >= begin && key < end ? w.x : 0.f;
+                            w.y = key + 1 >= begin && key + 1 < end ? w.y : 0.f;
+                        }
+                        part = add2(part, pair_of(w.x, w.y));
+                        packed[8 * pg + (i < 4 ? 2 * i : 2 * (i - 4) + 1)] = pack_f16x2(w.x, w.y);
                     }
-                    const float2 ps = split(part);
-                    sum = fmaf(ps.x + ps.y, x.z, sum);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) s[8 * pg + i] = packed[i];   // (all scores of this and earlier pages are consumed)
+                    const float2 half = split(part);
+                    // 1 / s_V that is not a number belongs to a page that is none: of rows that see all of it. Others find that in their weights.
+                    const float page_sum = half.x + half.y;
+                    ps[pg] = page_sum * (kWhole || x.z == x.z ? x.z : 1.f);
+                    fits &= page_sum <= kLargestSum;
                 }
-                tmem_st_32(t_p + 32u * half, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+                return !fits;
             };
-            weights(1);
-            load(0);
-            weights(0);
-            if (kb > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {   // the tile's previous product with V is complete: it was issued before this S
-#pragma unroll 1
-                for (int c = 0; c < kDim / 32; ++c) {
-                    uint32_t r[32];
-                    tmem_ld_32_async(t_o + 32u * c, r);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-                    tmem_st_32(t_o + 32u * c, r);
+            auto chunk = [&](const uint32_t* a, int c, auto all_seen) {
+                uint32_t packed[16];
+                float ps[2];
+                bool over = weigh(a, c, all_seen, packed, ps);
+                if (__any_sync(0xffffffffu, over)) {
+                    raise(a, c, over);
+                    weigh(a, c, std::false_type{}, packed, ps);
                 }
-            }
-            l_run = fmaf(l_run, alpha, sum);
+                sum += ps[0] + ps[1];
+                tmem_st_16(t_s + 16u * c, packed);
+            };
+            auto all_chunks = [&](auto all_seen) {
+#pragma unroll
+                for (int c = 0; c < kKeys / 32; c += 2) {   // weights go where scores have been read
+                    tmem_ld_32_async(t_s + 32u * c, s[0]);
+                    tmem_ld_32_async(t_s + 32u * (c + 1), s[1]);
+                    tmem_wait_ld();                         // straight behind: nothing may touch the registers before
+                    chunk(s[0], c, all_seen);
+                    chunk(s[1], c + 1, all_seen);
+                }
+            };
+            if (whole) all_chunks(std::true_type{});
+            else all_chunks(std::false_type{});
+            l_run += sum;
             asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
             tc_fence_before();
             mbar_arrive_addr(p_bar);
@@ -505,6 +556,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             if (!mbar_wait_parked(smem_u32(&o_full[ti]), 0, params.wait_limit)) failed = true;
             failed = __any_sync(0xffffffffu, failed);
         }
+        // a query that is not a number, or scores that are infinite: the row is none (the polynomial knows no NaN)
+        if (end > begin && my_blocks > 0 && (q_scale != q_scale || m_run == INFINITY)) l_run = __uint_as_float(0x7fc00000u);
         const long long at = (long long)my_row * p.q_heads + my_head;
         if (!failed && p.splits == 1) {
             tc_fence_after();
