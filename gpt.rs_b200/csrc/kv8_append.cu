@@ -1,11 +1,12 @@
 // Append to the 8-bit cache (norm and rotation of queries and keys on the way), and reading tokens back.
 //
-// gptrs_cuda_kv8_append: a CTA takes a tile of consecutive rows x one kv head with its query heads. A group of dim / 8 lanes works on a
-// head's row at a time (four rotated pairs per lane). Queries and the tile's angles are read once. Blocks are written whole: the CTA with the row
-// that completes a block reads the keys and values of its 16 tokens (again, where they lie in front of the tile; from the open rows, where they
-// came with an earlier call), takes the largest magnitude over the CTA, and puts the bytes in order in shared memory. What a run does to a
-// slot's open rows is done by one CTA per kv head, the one with the run's first row: first the block that the run continues is read and
-// written, then the rows of the run's last two blocks are stored, so that no other CTA reads what this one overwrites.
+// gptrs_cuda_kv8_append: a CTA takes one row or a tile of 16 consecutive rows x one kv head with its query heads. A group of dim / 8 lanes works on a head's
+// row at a time (four rotated pairs per lane). What bounds it is the latency of loads that depend on each other (position, angle; slot, open rows), so the first
+// queries, the angles of the tile (kept in shared memory) and, for runs of one row, key, value and the open rows are asked for before anything is
+// computed. Blocks are written whole: the CTA with the row that completes a block reads the keys and values of its 16 tokens (again, where they lie in
+// front of the tile; from the open rows, where they came with an earlier call), takes the largest magnitude over the CTA, and puts the bytes in order in
+// shared memory. What a run does to a slot's open rows is done by one CTA per kv head, the one with the run's first row: first the block that the run
+// continues is read and written, then the rows of the run's last two blocks are stored, so that no other CTA reads what this one overwrites.
 #include "kv8_cache.cuh"
 #include "qk_rotate.cuh"
 
@@ -25,53 +26,7 @@ struct AppendParams {
     __nv_bfloat16* open;
     __nv_bfloat16* q;
     int* status;
-    int rows, q_heads, kv_heads, group, tile_rows;
-};
-
-template <int kDim>
-struct Appender {
-    static constexpr int kLanes = kDim / 8;                  // of a head's row
-    static constexpr int kGroups = kThreads / kLanes;        // rows at a time
-    static constexpr int kPer = kKv8Tokens / kGroups;        // tokens of a block per lane group
-    const AppendParams& p;
-    int lane, in_group, ca, cb, head;                        // lane group, lane in it, first channels of its two runs
-
-    __device__ Appender(const AppendParams& params, int kv_head) : p(params), head(kv_head) {
-        lane = threadIdx.x / kLanes;
-        in_group = threadIdx.x % kLanes;
-        pair_channels<4>(p.r, 4 * in_group, &ca, &cb);
-    }
-    // norm and rotation of a query's or key's row in registers; all lanes of the warp call it
-    __device__ void turn(const float* gain, float (&a)[4], float (&b)[4], const float (&c)[4], const float (&s)[4]) const {
-        if (gain) {
-            const float rms = rsqrtf(lane_group_sum(square_sum(a, b), kLanes) / kDim + p.r.eps);
-            times_gain(gain, ca, cb, rms, a, b);
-        }
-        if (4 * in_group < p.r.rot_half) rotate_pairs(!p.r.neighbours, a, b, c, s);
-    }
-    __device__ void angles(int row, float (&c)[4], float (&s)[4]) const {
-        if (p.rotates) pair_angles<4>(p.r, row, p.positions[row], 4 * in_group, p.status, c, s);
-    }
-    // key (which 0) or value (1) of a row of the call, rounded to bf16; live: of this lane group (the others only take part in the sum)
-    __device__ void fetch(int row, int which, bool live, float (&a)[4], float (&b)[4]) const {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) a[k] = b[k] = 0.f;
-        if (live) {
-            const __nv_bfloat16* src = p.qkv + row * p.ld + (long long)(p.q_heads + which * p.kv_heads + head) * kDim;
-            load_vec(src + ca, a);
-            load_vec(src + cb, b);
-        }
-        if (which == 0 && p.rotates) {
-            float c[4] = {}, s[4] = {};
-            if (live) angles(row, c, s);
-            turn(p.r.k_gain, a, b, c, s);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            a[k] = __bfloat162float(__float2bfloat16_rn(a[k]));
-            b[k] = __bfloat162float(__float2bfloat16_rn(b[k]));
-        }
-    }
+    int rows, q_heads, kv_heads, group;
 };
 
 // |x| as an ordered whole number that keeps infinities and NaN above all finite values
@@ -80,69 +35,146 @@ __device__ __forceinline__ uint32_t magnitude(const float (&a)[4], const float (
     for (int k = 0; k < 4; ++k) m = max(m, max(__float_as_uint(a[k]) & 0x7fffffffu, __float_as_uint(b[k]) & 0x7fffffffu));
     return m;
 }
+__device__ __forceinline__ void round_bf16(float (&a)[4], float (&b)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        a[k] = __bfloat162float(__float2bfloat16_rn(a[k]));
+        b[k] = __bfloat162float(__float2bfloat16_rn(b[k]));
+    }
+}
 
-template <int kDim>
+// kTile: consecutive rows of a CTA, 1 or 16
+template <int kDim, int kTile>
 __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams p) {
-    using A = Appender<kDim>;
+    constexpr int kLanes = kDim / 8, kGroups = kThreads / kLanes, kPer = kKv8Tokens / kGroups;   // lanes of a head's row, rows at a time, tokens of a block per lane group
+    constexpr int kPairs = kDim / 2;
+    using Raw = RawVec<__nv_bfloat16, 4>;
     __shared__ __align__(16) unsigned char bytes[32 * kDim + 16];
+    __shared__ __align__(16) float angles[2][kTile][kPairs];   // cos, sin of the tile's rows
     __shared__ uint32_t largest[2][kThreads / 32];
 
     pdl_launch_dependents();
     pdl_wait();
-    const int kv_head = blockIdx.y, tid = threadIdx.x;
-    const int row0 = blockIdx.x * p.tile_rows, row_end = min(row0 + p.tile_rows, p.rows);
-    A w(p, kv_head);
+    const int kv_head = blockIdx.y, tid = threadIdx.x, lane = tid / kLanes, in_group = tid % kLanes;   // lane group, lane in it
+    const int row0 = blockIdx.x * kTile, row_end = min(row0 + kTile, p.rows);
+    int ca, cb;   // first channels of a lane's two runs
+    pair_channels<4>(p.r, 4 * in_group, &ca, &cb);
+    const bool turned = 4 * in_group < p.r.rot_half;
 
-    // ---- queries: a lane group takes a row's heads one after the other (tiles) or the groups share the heads (few rows) -----------------
-    const int by_head = p.tile_rows < A::kGroups;
-    const int row_step = by_head ? 1 : A::kGroups, head_step = by_head ? A::kGroups : 1;
-    for (int r0 = row0; r0 < row_end; r0 += row_step) {
-        const int row = by_head ? r0 : r0 + w.lane;
-        const bool live_row = row < row_end && p.slot[row < row_end ? row : row0] >= 0;
-        float c[4] = {}, s[4] = {};
-        if (live_row) w.angles(row, c, s);
-        for (int h0 = 0; h0 < p.group; h0 += head_step) {
-            const int h = by_head ? h0 + w.lane : h0;
-            const bool live = live_row && h < p.group;
-            float a[4] = {}, b[4] = {};
-            if (live) {
-                const __nv_bfloat16* src = p.qkv + row * p.ld + (long long)(kv_head * p.group + h) * kDim;
-                load_vec(src + w.ca, a);
-                load_vec(src + w.cb, b);
+    auto load = [&](const __nv_bfloat16* src, Raw& a, Raw& b) { a.load(src + ca); b.load(src + cb); };
+    auto source = [&](int row, int head) { return p.qkv + row * p.ld + (long long)head * kDim; };
+    // norm and rotation of a query's or key's row in registers; all lanes of a warp take part. row -1: no row.
+    auto turn = [&](const float* gain, int row, float (&a)[4], float (&b)[4]) {
+        if (!p.rotates) return;
+        if (gain) {
+            const float rms = rsqrtf(lane_group_sum(square_sum(a, b), kLanes) * (1.f / kDim) + p.r.eps);
+            times_gain(gain, ca, cb, rms, a, b);
+        }
+        if (turned && row >= 0) {
+            float c[4], s[4];
+            if (row >= row0 && row < row_end) {
+                load_vec(&angles[0][row - row0][4 * in_group], c);
+                load_vec(&angles[1][row - row0][4 * in_group], s);
+            } else {
+                pair_angles<4>(p.r, row, p.positions[row], 4 * in_group, p.status, c, s);
             }
-            if (p.rotates) w.turn(p.r.q_gain, a, b, c, s);
-            if (live) {
-                __nv_bfloat16* dst = p.q + ((long long)row * p.q_heads + kv_head * p.group + h) * kDim;
-                store_vec(dst + w.ca, a);
-                store_vec(dst + w.cb, b);
+            rotate_pairs(!p.r.neighbours, a, b, c, s);
+        }
+    };
+
+    // ---- the first loads, then the angles (a chain: axis and position, table) -------------------------------------------------------------------
+    constexpr int kBatch = 4;   // heads of a row on their way
+    const bool by_head = kTile < kGroups;   // few rows: the lane groups share a row's heads; else each has a row and takes its heads one after the other
+    const int row_step = by_head ? 1 : kGroups, head_step = by_head ? kGroups : 1;
+    Raw qa[kBatch], qb[kBatch];
+    auto load_queries = [&](int row, int h0) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+            if (row < row_end && h0 + j * head_step < p.group) load(source(row, kv_head * p.group + h0 + j * head_step), qa[j], qb[j]);
+    };
+    const int my_row = by_head ? row0 : row0 + lane, my_head = by_head ? lane : 0;
+    load_queries(my_row, my_head);
+    // the row's own key and value, for runs of one row
+    Raw own_a, own_b;
+    if (kTile == 1 && lane < 2) load(source(row0, p.q_heads + lane * p.kv_heads + kv_head), own_a, own_b);
+    int slot0 = 0, position0 = 0, first0 = 0, last0 = 0;
+    if (kTile == 1) { slot0 = p.slot[row0]; position0 = p.positions[row0]; first0 = p.run_first[row0]; last0 = p.run_last[row0]; }
+    if (p.rotates && p.r.rot_half > 0) {
+        constexpr int kSteps = (kTile * kPairs + kThreads - 1) / kThreads;
+        long long at[kSteps];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const int pair = (tid + i * kThreads) % kPairs, row = row0 + (tid + i * kThreads) / kPairs;
+            at[i] = -1;
+            if (pair < p.r.rot_half && row < row_end && row < row0 + kTile && p.slot[row] >= 0) {
+                const int axis = p.r.pair_axis ? p.r.pair_axis[pair] : 0;
+                long long pos = -1;
+                if (axis < p.r.axes) pos = p.r.axis_positions ? p.r.axis_positions[axis * p.r.axis_stride + row] : p.positions[row];
+                if (pos < 0 || pos >= p.r.positions) { atomicExch(p.status, 2); pos = 0; }
+                at[i] = pos * p.r.rot_half + pair;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+            if (at[i] >= 0) {
+                const int pair = (tid + i * kThreads) % kPairs, row = (tid + i * kThreads) / kPairs;
+                angles[0][row][pair] = p.r.cos[at[i]];
+                angles[1][row][pair] = p.r.sin[at[i]];
+            }
+    }
+    // runs of one row: the rows in front of it in its block, if it completes that
+    const bool valid0 = kTile == 1 && slot0 >= 0 && slot0 < p.n_slots && position0 >= 0 && first0 == row0 && last0 == row0 && position0 <= 0x7fffffff - kKv8Tokens;
+    const bool completes0 = valid0 && position0 % kKv8Tokens == kKv8Tokens - 1;
+    Raw old_a[2][kTile == 1 ? kPer : 1], old_b[2][kTile == 1 ? kPer : 1];
+    int page0 = -1;
+    if (completes0) {
+        const int block = position0 / kKv8Tokens;
+        const __nv_bfloat16* old = p.open + (long long)slot0 * kv8_open_elems(p.kv_heads, kDim);
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int j = 0; j < (kTile == 1 ? kPer : 0); ++j)
+                load(old + kv8_open_at(block, p.kv_heads, kv_head, which, kDim) + (lane + j * kGroups) * kDim, old_a[which][j], old_b[which][j]);
+        if (block < p.max_pages) page0 = kv8_page(p.table, slot0, p.max_pages, block, p.n_pages, p.status);
+        else if (tid == 0) atomicExch(p.status, 2);
+    }
+    __syncthreads();
+
+    // ---- queries ------------------------------------------------------------------------------------------------------------------------------
+    for (int r0 = row0; r0 < row_end; r0 += row_step) {
+        const int row = by_head ? r0 : r0 + lane;
+        const bool live_row = row < row_end && p.slot[row < row_end ? row : row0] >= 0;
+        for (int h0 = 0; h0 < p.group; h0 += kBatch * head_step) {
+            Raw xa[kBatch], xb[kBatch];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) { xa[j] = qa[j]; xb[j] = qb[j]; }
+            if (h0 + kBatch * head_step < p.group) load_queries(row, h0 + kBatch * head_step + my_head);
+            else if (r0 + row_step < row_end) load_queries(row + row_step, my_head);
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                if (h0 + j * head_step >= p.group) break;
+                const int h = h0 + j * head_step + my_head;
+                const bool live = live_row && h < p.group;
+                float a[4] = {}, b[4] = {};
+                if (live) { xa[j].get(a); xb[j].get(b); }
+                turn(p.r.q_gain, live ? row : -1, a, b);
+                if (live) {
+                    __nv_bfloat16* dst = p.q + ((long long)row * p.q_heads + kv_head * p.group + h) * kDim;
+                    store_vec(dst + ca, a);
+                    store_vec(dst + cb, b);
+                }
             }
         }
     }
 
-    // ---- keys and values ----------------------------------------------------------------------------------------------------------------
-    // The block that row `last` completes, of whose tokens those from `first` on came with this call. All threads of the CTA.
-    auto write_block = [&](int last, int first, int slot, int position) {
-        const int block = position / kKv8Tokens;
-        const __nv_bfloat16* const old = p.open + (long long)slot * kv8_open_elems(p.kv_heads, kDim);
-        float x[2][A::kPer][2][4];
+    // ---- keys and values ------------------------------------------------------------------------------------------------------------------------
+    // The 16 tokens of a block, token lane + j kGroups of either kind in this thread's registers (f32, of bf16 value) -> the page. All threads.
+    auto write_block = [&](const float (&x)[2][kPer][2][4], int page) {
         uint32_t m[2] = {0, 0};
 #pragma unroll
-        for (int which = 0; which < 2; ++which)
-#pragma unroll
-            for (int j = 0; j < A::kPer; ++j) {
-                const int token = w.lane + j * A::kGroups, row = last - (kKv8Tokens - 1) + token;
-                w.fetch(max(row, 0), which, row >= first, x[which][j][0], x[which][j][1]);
-                if (row < first) {
-                    const __nv_bfloat16* src = old + kv8_open_at(block, p.kv_heads, kv_head, which, kDim) + token * kDim;
-                    load_vec(src + w.ca, x[which][j][0]);
-                    load_vec(src + w.cb, x[which][j][1]);
-                }
-                m[which] = magnitude(x[which][j][0], x[which][j][1], m[which]);
-            }
-        const int page = block < p.max_pages ? kv8_page(p.table, slot, p.max_pages, block, p.n_pages, p.status) : -1;
-        if (block >= p.max_pages && tid == 0) atomicExch(p.status, 2);
-#pragma unroll
         for (int which = 0; which < 2; ++which) {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) m[which] = magnitude(x[which][j][0], x[which][j][1], m[which]);
             m[which] = __reduce_max_sync(0xffffffffu, m[which]);
             if ((tid & 31) == 0) largest[which][tid >> 5] = m[which];
         }
@@ -155,11 +187,11 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
             const bool finite = all < 0x7f800000u;
             const float scale = finite ? fmaxf(__fdiv_rn(__uint_as_float(all), 127.f), kKv8MinScale) : __uint_as_float(0x7fc00000u);
 #pragma unroll
-            for (int j = 0; j < A::kPer; ++j) {
-                const int token = w.lane + j * A::kGroups;
+            for (int j = 0; j < kPer; ++j) {
+                const int token = lane + j * kGroups;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const int ch = half ? w.cb : w.ca;
+                    const int ch = half ? cb : ca;
                     uint32_t u[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) u[k] = finite ? (uint32_t)(__float2int_rn(__fdiv_rn(x[which][j][half][k], scale)) + 128) : 128u;
@@ -181,6 +213,82 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
         }
         __syncthreads();   // `bytes` and `largest` may be written again, and the open rows too
     };
+    // The block that row `last` completes, of whose tokens those from row `first` on came with this call.
+    auto complete = [&](int last, int first, int slot, int position) {
+        const int block = position / kKv8Tokens;
+        const __nv_bfloat16* const old = p.open + (long long)slot * kv8_open_elems(p.kv_heads, kDim);
+        Raw ra[2][kPer], rb[2][kPer];
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                const int token = lane + j * kGroups, row = last - (kKv8Tokens - 1) + token;
+                load(row >= first ? source(row, p.q_heads + which * p.kv_heads + kv_head) : old + kv8_open_at(block, p.kv_heads, kv_head, which, kDim) + token * kDim, ra[which][j], rb[which][j]);
+            }
+        const int page = block < p.max_pages ? kv8_page(p.table, slot, p.max_pages, block, p.n_pages, p.status) : -1;
+        if (block >= p.max_pages && tid == 0) atomicExch(p.status, 2);
+        float x[2][kPer][2][4];
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                const int row = last - (kKv8Tokens - 1) + lane + j * kGroups;
+                ra[which][j].get(x[which][j][0]);
+                rb[which][j].get(x[which][j][1]);
+                if (which == 0) {   // rows of earlier calls are as they are to be
+                    float a[4], b[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) { a[k] = x[0][j][0][k]; b[k] = x[0][j][1][k]; }
+                    turn(p.r.k_gain, row >= first ? row : -1, a, b);
+                    if (row >= first) {
+                        round_bf16(a, b);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) { x[0][j][0][k] = a[k]; x[0][j][1][k] = b[k]; }
+                    }
+                }
+            }
+        write_block(x, page);
+    };
+
+    if (kTile == 1 && slot0 >= 0 && valid0) {
+        // a run of one row (warp 0 has its key and value): its place in the open rows, and the block, if this completes it
+        float own[2][4] = {};
+        if (lane < 2) { own_a.get(own[0]); own_b.get(own[1]); }
+        {
+            float a[4], b[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { a[k] = own[0][k]; b[k] = own[1][k]; }
+            turn(p.r.k_gain, lane == 0 ? row0 : -1, a, b);
+            if (lane == 0) {
+                round_bf16(a, b);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { own[0][k] = a[k]; own[1][k] = b[k]; }
+            }
+        }
+        if (completes0) {   // by way of shared memory to the threads that have the block's last token
+            float (*const last_token)[kDim] = reinterpret_cast<float(*)[kDim]>(bytes);
+            if (lane < 2) { store_vec(last_token[lane] + ca, own[0]); store_vec(last_token[lane] + cb, own[1]); }
+            __syncthreads();
+            float x[2][kPer][2][4];
+#pragma unroll
+            for (int which = 0; which < 2; ++which)
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) {
+                    old_a[which][kTile == 1 ? j : 0].get(x[which][j][0]);
+                    old_b[which][kTile == 1 ? j : 0].get(x[which][j][1]);
+                    if (lane + j * kGroups == kKv8Tokens - 1) { load_vec(last_token[which] + ca, x[which][j][0]); load_vec(last_token[which] + cb, x[which][j][1]); }
+                }
+            __syncthreads();
+            write_block(x, page0);
+        }
+        if (lane < 2) {
+            __nv_bfloat16* dst = p.open + (long long)slot0 * kv8_open_elems(p.kv_heads, kDim) + kv8_open_at(position0 / kKv8Tokens, p.kv_heads, kv_head, lane, kDim) +
+                                 position0 % kKv8Tokens * kDim;
+            store_vec(dst + ca, own[0]);
+            store_vec(dst + cb, own[1]);
+        }
+        return;
+    }
 
     for (int row = row0; row < row_end; ++row) {
         const int slot = p.slot[row], position = p.positions[row], first = p.run_first[row], last = p.run_last[row];
@@ -192,24 +300,29 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
         const int to_end = kKv8Tokens - 1 - position % kKv8Tokens;         // rows until the block of this one is complete
         const bool continued = (position - (row - first)) % kKv8Tokens != 0;   // the run's first block holds tokens of an earlier call
         const bool in_first = row - first < kKv8Tokens && (position - (row - first)) / kKv8Tokens == position / kKv8Tokens;
-        if (to_end == 0 && !(continued && in_first)) write_block(row, first, slot, position);
+        if (to_end == 0 && !(continued && in_first)) complete(row, first, slot, position);
         if (row != first) continue;
-        if (continued && row + to_end <= last) write_block(row + to_end, first, slot, position);
+        if (continued && row + to_end <= last) complete(row + to_end, first, slot, position);
         // the rows of the run's last two blocks stay as they are
         const int end = position + (last - row);
         const int keep = max(position, (end / kKv8Tokens - 1) * kKv8Tokens);
         __nv_bfloat16* const open = p.open + (long long)slot * kv8_open_elems(p.kv_heads, kDim);
-        for (int q0 = keep; q0 <= end; q0 += A::kGroups) {
-            const int at = q0 + w.lane;
+        for (int q0 = keep; q0 <= end; q0 += kGroups) {
+            const int at = q0 + lane, from = row + (at - position);
             const bool live = at <= end;
+            Raw ra[2], rb[2];
+#pragma unroll
+            for (int which = 0; which < 2; ++which)
+                if (live) load(source(from, p.q_heads + which * p.kv_heads + kv_head), ra[which], rb[which]);
 #pragma unroll
             for (int which = 0; which < 2; ++which) {
-                float a[4], b[4];
-                w.fetch(live ? row + (at - position) : row, which, live, a, b);
+                float a[4] = {}, b[4] = {};
+                if (live) { ra[which].get(a); rb[which].get(b); }
+                if (which == 0) turn(p.r.k_gain, live ? from : -1, a, b);
                 if (live) {
                     __nv_bfloat16* dst = open + kv8_open_at(at / kKv8Tokens, p.kv_heads, kv_head, which, kDim) + at % kKv8Tokens * kDim;
-                    store_vec(dst + w.ca, a);
-                    store_vec(dst + w.cb, b);
+                    store_vec(dst + ca, a);
+                    store_vec(dst + cb, b);
                 }
             }
         }
@@ -336,10 +449,10 @@ int gptrs_cuda_kv8_append(const gptrs_kv8_cache* c, const gptrs_kv8_append_step*
     p.q = static_cast<__nv_bfloat16*>(s->d_q);
     p.status = s->d_status;
     p.rows = (int)s->rows; p.q_heads = c->q_heads; p.kv_heads = c->kv_heads; p.group = c->q_heads / c->kv_heads;
-    p.tile_rows = s->rows <= 256 ? 1 : kKv8Tokens;
-    const dim3 grid((unsigned)ceil_div(s->rows, p.tile_rows), (unsigned)c->kv_heads);
-    if (c->dim == 64) return launch_kernel(kv8_append_kernel<64>, grid, dim3(kThreads), 0, as_stream(stream), 1, p);
-    return launch_kernel(kv8_append_kernel<128>, grid, dim3(kThreads), 0, as_stream(stream), 1, p);
+    const bool few = s->rows <= 256;
+    const dim3 grid((unsigned)ceil_div(s->rows, few ? 1 : kKv8Tokens), (unsigned)c->kv_heads);
+    auto kernel = c->dim == 64 ? (few ? kv8_append_kernel<64, 1> : kv8_append_kernel<64, 16>) : (few ? kv8_append_kernel<128, 1> : kv8_append_kernel<128, 16>);
+    return launch_kernel(kernel, grid, dim3(kThreads), 0, as_stream(stream), 1, p);
 }
 
 int gptrs_cuda_kv8_gather(const gptrs_kv8_cache* c, const void* d_pool, int64_t n_pages, const void* d_open, int64_t n_slots, const int32_t* d_page_table,

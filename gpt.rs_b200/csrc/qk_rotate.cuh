@@ -29,6 +29,37 @@ __device__ __forceinline__ void load_vec(const __nv_bfloat16* p, float (&v)[4]) 
     const uint2 x = *reinterpret_cast<const uint2*>(p);
     v[0] = bf16_lo(x.x); v[1] = bf16_hi(x.x); v[2] = bf16_lo(x.y); v[3] = bf16_hi(x.y);
 }
+// kVec consecutive values as they come from memory, and as floats
+template <typename T, int kVec> struct RawVec;
+template <> struct RawVec<__nv_bfloat16, 8> {
+    uint4 x;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { x = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void store(__nv_bfloat16* p) const { *reinterpret_cast<uint4*>(p) = x; }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(w[i]); v[2 * i + 1] = bf16_hi(w[i]); }
+    }
+};
+template <> struct RawVec<__nv_bfloat16, 4> {
+    uint2 x;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { x = *reinterpret_cast<const uint2*>(p); }
+    __device__ __forceinline__ void store(__nv_bfloat16* p) const { *reinterpret_cast<uint2*>(p) = x; }
+    __device__ __forceinline__ void get(float (&v)[4]) const { v[0] = bf16_lo(x.x); v[1] = bf16_hi(x.x); v[2] = bf16_lo(x.y); v[3] = bf16_hi(x.y); }
+};
+template <> struct RawVec<float, 4> {
+    float4 x;
+    __device__ __forceinline__ void load(const float* p) { x = *reinterpret_cast<const float4*>(p); }
+    __device__ __forceinline__ void store(float* p) const { *reinterpret_cast<float4*>(p) = x; }
+    __device__ __forceinline__ void get(float (&v)[4]) const { v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; }
+};
+__device__ __forceinline__ void load_vec(const float* p, float (&v)[8]) {
+    const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+}
+__device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
 __device__ __forceinline__ void load_vec(const float* p, float (&v)[1]) { v[0] = *p; }
 __device__ __forceinline__ void load_vec(const __nv_bfloat16* p, float (&v)[1]) { v[0] = __bfloat162float(*p); }
 __device__ __forceinline__ void store_vec(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }

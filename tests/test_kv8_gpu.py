@@ -42,6 +42,7 @@ def _rotation(rng, heads, kv, dim, pairs, rows, cuda, gains, neighbours, axes, p
 ROTATIONS = [  # heads, kv, dim, pairs, rows, gains, neighbours, axes
     (4, 2, 128, 64, 1, True, False, 1), (32, 8, 128, 64, 19, True, False, 3), (3, 1, 64, 32, 257, True, True, 1), (5, 5, 96, 24, 7, True, False, 2),
     (2, 1, 80, 40, 3, False, False, 1), (2, 2, 6, 3, 5, True, False, 3), (1, 1, 512, 256, 2, True, False, 1), (2, 1, 256, 128, 4, True, True, 4),
+    (32, 8, 128, 64, 1201, True, False, 3), (3, 1, 64, 16, 901, True, True, 1), (40, 10, 64, 32, 610, False, False, 2), (2, 2, 32, 0, 700, True, False, 1), (5, 1, 96, 40, 400, True, False, 2),
     (2, 1, 62, 13, 9, True, True, 2), (8, 2, 128, 0, 6, True, False, 1), (7, 7, 64, 30, 8, False, True, 1), (2, 1, 2, 1, 33, True, False, 1), (1, 1, 264, 100, 3, True, False, 1)]
 
 
