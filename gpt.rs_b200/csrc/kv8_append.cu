@@ -1,12 +1,10 @@
 // Append to the 8-bit cache (norm and rotation of queries and keys on the way), and reading tokens back.
 //
-// gptrs_cuda_kv8_append: a CTA takes one row or a tile of 16 consecutive rows x one kv head with its query heads. A group of dim / 8 lanes works on a head's
-// row at a time (four rotated pairs per lane). What bounds it is the latency of loads that depend on each other (position, angle; slot, open rows), so the first
-// queries, the angles of the tile (kept in shared memory) and, for runs of one row, key, value and the open rows are asked for before anything is
-// computed. Blocks are written whole: the CTA with the row that completes a block reads the keys and values of its 16 tokens (again, where they lie in
-// front of the tile; from the open rows, where they came with an earlier call), takes the largest magnitude over the CTA, and puts the bytes in order in
-// shared memory. What a run does to a slot's open rows is done by one CTA per kv head, the one with the run's first row: first the block that the run
-// continues is read and written, then the rows of the run's last two blocks are stored, so that no other CTA reads what this one overwrites.
+// gptrs_cuda_kv8_append: a CTA takes the rows of a run that fall into one block (16 tokens) x one kv head with its query heads; it finds them from the last
+// of these rows, which lies in the 16 rows (of short lists, the one row) it looks at. A group of dim / 8 lanes works on a head's row at a time (four
+// rotated pairs per lane). What bounds it is the latency of loads that depend on each other (slot and position; angles; open rows), so keys, values, the
+// first queries and the angles (kept in shared memory) are asked for before anything is computed; for runs of one row (decode steps) with the rows in front of
+// it in its block. A block is written once, by the CTA with its last token: the largest magnitude over the CTA, then the bytes in order in shared memory.
 #include "kv8_cache.cuh"
 #include "qk_rotate.cuh"
 
@@ -43,131 +41,71 @@ __device__ __forceinline__ void round_bf16(float (&a)[4], float (&b)[4]) {
     }
 }
 
-// kTile: consecutive rows of a CTA, 1 or 16
+// kTile: consecutive rows that a CTA looks at, 1 or 16. It works on the segments (rows of one run and block) whose last row is among them.
 template <int kDim, int kTile>
 __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams p) {
     constexpr int kLanes = kDim / 8, kGroups = kThreads / kLanes, kPer = kKv8Tokens / kGroups;   // lanes of a head's row, rows at a time, tokens of a block per lane group
     constexpr int kPairs = kDim / 2;
     using Raw = RawVec<__nv_bfloat16, 4>;
     __shared__ __align__(16) unsigned char bytes[32 * kDim + 16];
-    __shared__ __align__(16) float angles[2][kTile][kPairs];   // cos, sin of the tile's rows
+    __shared__ __align__(16) float angles[2][kKv8Tokens][kPairs];   // cos, sin of the rows that are worked on
     __shared__ uint32_t largest[2][kThreads / 32];
 
     pdl_launch_dependents();
     pdl_wait();
     const int kv_head = blockIdx.y, tid = threadIdx.x, lane = tid / kLanes, in_group = tid % kLanes;   // lane group, lane in it
-    const int row0 = blockIdx.x * kTile, row_end = min(row0 + kTile, p.rows);
+    const int row0 = blockIdx.x * kTile;
     int ca, cb;   // first channels of a lane's two runs
     pair_channels<4>(p.r, 4 * in_group, &ca, &cb);
     const bool turned = 4 * in_group < p.r.rot_half;
 
     auto load = [&](const __nv_bfloat16* src, Raw& a, Raw& b) { a.load(src + ca); b.load(src + cb); };
     auto source = [&](int row, int head) { return p.qkv + row * p.ld + (long long)head * kDim; };
-    // norm and rotation of a query's or key's row in registers; all lanes of a warp take part. row -1: no row.
-    auto turn = [&](const float* gain, int row, float (&a)[4], float (&b)[4]) {
+    auto open_row = [&](int slot, int position, int which) {
+        return p.open + (long long)slot * kv8_open_elems(p.kv_heads, kDim) + kv8_open_at(position / kKv8Tokens, p.kv_heads, kv_head, which, kDim) + position % kKv8Tokens * kDim;
+    };
+    // Angles of rows [from, from + n), n <= 16, to shared memory: a chain of loads (axis and position, table), all rows' at a time.
+    auto fetch_angles = [&](int from, int n) {
+        if (!p.rotates || p.r.rot_half == 0) return;
+        constexpr int kSteps = kTile == 1 ? 4 : kKv8Tokens * kPairs / kThreads;
+        for (int i0 = tid; i0 < n * kPairs; i0 += kSteps * kThreads) {
+            long long at[kSteps];
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const int pair = (i0 + i * kThreads) % kPairs, k = (i0 + i * kThreads) / kPairs, row = from + k;
+                at[i] = -1;
+                if (pair < p.r.rot_half && k < n) {
+                    const int axis = p.r.pair_axis ? p.r.pair_axis[pair] : 0;
+                    long long pos = -1;
+                    if (axis < p.r.axes) pos = p.r.axis_positions ? p.r.axis_positions[axis * p.r.axis_stride + row] : p.positions[row];
+                    if (pos < 0 || pos >= p.r.positions) { atomicExch(p.status, 2); pos = 0; }
+                    at[i] = pos * p.r.rot_half + pair;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+                if (at[i] >= 0) {
+                    const int pair = (i0 + i * kThreads) % kPairs, k = (i0 + i * kThreads) / kPairs;
+                    angles[0][k][pair] = p.r.cos[at[i]];
+                    angles[1][k][pair] = p.r.sin[at[i]];
+                }
+        }
+    };
+    // Norm and rotation of a query's or key's row in registers; all lanes of a warp take part. k: its place in `angles`.
+    auto turn = [&](const float* gain, int k, float (&a)[4], float (&b)[4]) {
         if (!p.rotates) return;
         if (gain) {
             const float rms = rsqrtf(lane_group_sum(square_sum(a, b), kLanes) * (1.f / kDim) + p.r.eps);
             times_gain(gain, ca, cb, rms, a, b);
         }
-        if (turned && row >= 0) {
+        if (turned) {
             float c[4], s[4];
-            if (row >= row0 && row < row_end) {
-                load_vec(&angles[0][row - row0][4 * in_group], c);
-                load_vec(&angles[1][row - row0][4 * in_group], s);
-            } else {
-                pair_angles<4>(p.r, row, p.positions[row], 4 * in_group, p.status, c, s);
-            }
+            load_vec(&angles[0][k][4 * in_group], c);
+            load_vec(&angles[1][k][4 * in_group], s);
             rotate_pairs(!p.r.neighbours, a, b, c, s);
         }
     };
-
-    // ---- the first loads, then the angles (a chain: axis and position, table) -------------------------------------------------------------------
-    constexpr int kBatch = 4;   // heads of a row on their way
-    const bool by_head = kTile < kGroups;   // few rows: the lane groups share a row's heads; else each has a row and takes its heads one after the other
-    const int row_step = by_head ? 1 : kGroups, head_step = by_head ? kGroups : 1;
-    Raw qa[kBatch], qb[kBatch];
-    auto load_queries = [&](int row, int h0) {
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-            if (row < row_end && h0 + j * head_step < p.group) load(source(row, kv_head * p.group + h0 + j * head_step), qa[j], qb[j]);
-    };
-    const int my_row = by_head ? row0 : row0 + lane, my_head = by_head ? lane : 0;
-    load_queries(my_row, my_head);
-    // the row's own key and value, for runs of one row
-    Raw own_a, own_b;
-    if (kTile == 1 && lane < 2) load(source(row0, p.q_heads + lane * p.kv_heads + kv_head), own_a, own_b);
-    int slot0 = 0, position0 = 0, first0 = 0, last0 = 0;
-    if (kTile == 1) { slot0 = p.slot[row0]; position0 = p.positions[row0]; first0 = p.run_first[row0]; last0 = p.run_last[row0]; }
-    if (p.rotates && p.r.rot_half > 0) {
-        constexpr int kSteps = (kTile * kPairs + kThreads - 1) / kThreads;
-        long long at[kSteps];
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            const int pair = (tid + i * kThreads) % kPairs, row = row0 + (tid + i * kThreads) / kPairs;
-            at[i] = -1;
-            if (pair < p.r.rot_half && row < row_end && row < row0 + kTile && p.slot[row] >= 0) {
-                const int axis = p.r.pair_axis ? p.r.pair_axis[pair] : 0;
-                long long pos = -1;
-                if (axis < p.r.axes) pos = p.r.axis_positions ? p.r.axis_positions[axis * p.r.axis_stride + row] : p.positions[row];
-                if (pos < 0 || pos >= p.r.positions) { atomicExch(p.status, 2); pos = 0; }
-                at[i] = pos * p.r.rot_half + pair;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i)
-            if (at[i] >= 0) {
-                const int pair = (tid + i * kThreads) % kPairs, row = (tid + i * kThreads) / kPairs;
-                angles[0][row][pair] = p.r.cos[at[i]];
-                angles[1][row][pair] = p.r.sin[at[i]];
-            }
-    }
-    // runs of one row: the rows in front of it in its block, if it completes that
-    const bool valid0 = kTile == 1 && slot0 >= 0 && slot0 < p.n_slots && position0 >= 0 && first0 == row0 && last0 == row0 && position0 <= 0x7fffffff - kKv8Tokens;
-    const bool completes0 = valid0 && position0 % kKv8Tokens == kKv8Tokens - 1;
-    Raw old_a[2][kTile == 1 ? kPer : 1], old_b[2][kTile == 1 ? kPer : 1];
-    int page0 = -1;
-    if (completes0) {
-        const int block = position0 / kKv8Tokens;
-        const __nv_bfloat16* old = p.open + (long long)slot0 * kv8_open_elems(p.kv_heads, kDim);
-#pragma unroll
-        for (int which = 0; which < 2; ++which)
-#pragma unroll
-            for (int j = 0; j < (kTile == 1 ? kPer : 0); ++j)
-                load(old + kv8_open_at(block, p.kv_heads, kv_head, which, kDim) + (lane + j * kGroups) * kDim, old_a[which][j], old_b[which][j]);
-        if (block < p.max_pages) page0 = kv8_page(p.table, slot0, p.max_pages, block, p.n_pages, p.status);
-        else if (tid == 0) atomicExch(p.status, 2);
-    }
-    __syncthreads();
-
-    // ---- queries ------------------------------------------------------------------------------------------------------------------------------
-    for (int r0 = row0; r0 < row_end; r0 += row_step) {
-        const int row = by_head ? r0 : r0 + lane;
-        const bool live_row = row < row_end && p.slot[row < row_end ? row : row0] >= 0;
-        for (int h0 = 0; h0 < p.group; h0 += kBatch * head_step) {
-            Raw xa[kBatch], xb[kBatch];
-#pragma unroll
-            for (int j = 0; j < kBatch; ++j) { xa[j] = qa[j]; xb[j] = qb[j]; }
-            if (h0 + kBatch * head_step < p.group) load_queries(row, h0 + kBatch * head_step + my_head);
-            else if (r0 + row_step < row_end) load_queries(row + row_step, my_head);
-#pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
-                if (h0 + j * head_step >= p.group) break;
-                const int h = h0 + j * head_step + my_head;
-                const bool live = live_row && h < p.group;
-                float a[4] = {}, b[4] = {};
-                if (live) { xa[j].get(a); xb[j].get(b); }
-                turn(p.r.q_gain, live ? row : -1, a, b);
-                if (live) {
-                    __nv_bfloat16* dst = p.q + ((long long)row * p.q_heads + kv_head * p.group + h) * kDim;
-                    store_vec(dst + ca, a);
-                    store_vec(dst + cb, b);
-                }
-            }
-        }
-    }
-
-    // ---- keys and values ------------------------------------------------------------------------------------------------------------------------
+    auto put = [&](__nv_bfloat16* dst, const float (&a)[4], const float (&b)[4]) { store_vec(dst + ca, a); store_vec(dst + cb, b); };
     // The 16 tokens of a block, token lane + j kGroups of either kind in this thread's registers (f32, of bf16 value) -> the page. All threads.
     auto write_block = [&](const float (&x)[2][kPer][2][4], int page) {
         uint32_t m[2] = {0, 0};
@@ -211,119 +149,186 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
             uint4* dst = reinterpret_cast<uint4*>(p.pool + ((long long)page * p.kv_heads + kv_head) * kv8_block_bytes(kDim));
             for (int i = tid; i < 2 * kDim + 1; i += kThreads) dst[i] = reinterpret_cast<const uint4*>(bytes)[i];
         }
-        __syncthreads();   // `bytes` and `largest` may be written again, and the open rows too
     };
-    // The block that row `last` completes, of whose tokens those from row `first` on came with this call.
-    auto complete = [&](int last, int first, int slot, int position) {
-        const int block = position / kKv8Tokens;
-        const __nv_bfloat16* const old = p.open + (long long)slot * kv8_open_elems(p.kv_heads, kDim);
-        Raw ra[2][kPer], rb[2][kPer];
-#pragma unroll
-        for (int which = 0; which < 2; ++which)
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                const int token = lane + j * kGroups, row = last - (kKv8Tokens - 1) + token;
-                load(row >= first ? source(row, p.q_heads + which * p.kv_heads + kv_head) : old + kv8_open_at(block, p.kv_heads, kv_head, which, kDim) + token * kDim, ra[which][j], rb[which][j]);
-            }
-        const int page = block < p.max_pages ? kv8_page(p.table, slot, p.max_pages, block, p.n_pages, p.status) : -1;
-        if (block >= p.max_pages && tid == 0) atomicExch(p.status, 2);
-        float x[2][kPer][2][4];
-#pragma unroll
-        for (int which = 0; which < 2; ++which)
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                const int row = last - (kKv8Tokens - 1) + lane + j * kGroups;
-                ra[which][j].get(x[which][j][0]);
-                rb[which][j].get(x[which][j][1]);
-                if (which == 0) {   // rows of earlier calls are as they are to be
-                    float a[4], b[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) { a[k] = x[0][j][0][k]; b[k] = x[0][j][1][k]; }
-                    turn(p.r.k_gain, row >= first ? row : -1, a, b);
-                    if (row >= first) {
-                        round_bf16(a, b);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) { x[0][j][0][k] = a[k]; x[0][j][1][k] = b[k]; }
-                    }
-                }
-            }
-        write_block(x, page);
+    auto page_of = [&](int slot, int block) {
+        if (block < p.max_pages) return kv8_page(p.table, slot, p.max_pages, block, p.n_pages, p.status);
+        if (tid == 0) atomicExch(p.status, 2);
+        return -1;
     };
 
-    if (kTile == 1 && slot0 >= 0 && valid0) {
-        // a run of one row (warp 0 has its key and value): its place in the open rows, and the block, if this completes it
-        float own[2][4] = {};
-        if (lane < 2) { own_a.get(own[0]); own_b.get(own[1]); }
-        {
-            float a[4], b[4];
+    if (kTile == 1) {
+        // ---- a run of one row: everything is asked for at once ---------------------------------------------------------------------------------
+        Raw qa, qb, own_a, own_b;
+        if (lane < p.group) load(source(row0, kv_head * p.group + lane), qa, qb);
+        if (lane < 2) load(source(row0, p.q_heads + lane * p.kv_heads + kv_head), own_a, own_b);
+        const int slot = p.slot[row0], position = p.positions[row0], first = p.run_first[row0], last = p.run_last[row0];
+        if (slot < 0) return;
+        if (first == row0 && last == row0 && slot < p.n_slots && position >= 0 && position <= 0x7fffffff - kKv8Tokens) {
+            fetch_angles(row0, 1);
+            const bool completes = position % kKv8Tokens == kKv8Tokens - 1;
+            Raw old_a[2][kPer], old_b[2][kPer];
+            int page = -1;
+            if (completes) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) { a[k] = own[0][k]; b[k] = own[1][k]; }
-            turn(p.r.k_gain, lane == 0 ? row0 : -1, a, b);
+                for (int which = 0; which < 2; ++which)
+#pragma unroll
+                    for (int j = 0; j < kPer; ++j)
+                        load(open_row(slot, position - (kKv8Tokens - 1) + lane + j * kGroups, which), old_a[which][j], old_b[which][j]);
+                page = page_of(slot, position / kKv8Tokens);
+            }
+            __syncthreads();
+            for (int h0 = 0; h0 < p.group; h0 += kGroups) {
+                const int h = h0 + lane;
+                float a[4] = {}, b[4] = {};
+                if (h0 > 0 && h < p.group) load(source(row0, kv_head * p.group + h), qa, qb);
+                if (h < p.group) { qa.get(a); qb.get(b); }
+                turn(p.r.q_gain, 0, a, b);
+                if (h < p.group) put(p.q + ((long long)row0 * p.q_heads + kv_head * p.group + h) * kDim, a, b);
+            }
+            float own[2][4] = {}, a[4] = {}, b[4] = {};   // lane group 0 has the key, 1 the value (which stays as it is)
+            if (lane < 2) { own_a.get(own[0]); own_b.get(own[1]); own_a.get(a); own_b.get(b); }
+            turn(p.r.k_gain, 0, a, b);
             if (lane == 0) {
                 round_bf16(a, b);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) { own[0][k] = a[k]; own[1][k] = b[k]; }
             }
+            if (completes) {   // by way of shared memory to the threads that have the block's last token
+                float (*const last_token)[kDim] = reinterpret_cast<float(*)[kDim]>(bytes);
+                if (lane < 2) { store_vec(last_token[lane] + ca, own[0]); store_vec(last_token[lane] + cb, own[1]); }
+                __syncthreads();
+                float x[2][kPer][2][4];
+#pragma unroll
+                for (int which = 0; which < 2; ++which)
+#pragma unroll
+                    for (int j = 0; j < kPer; ++j) {
+                        old_a[which][j].get(x[which][j][0]);
+                        old_b[which][j].get(x[which][j][1]);
+                        if (lane + j * kGroups == kKv8Tokens - 1) { load_vec(last_token[which] + ca, x[which][j][0]); load_vec(last_token[which] + cb, x[which][j][1]); }
+                    }
+                write_block(x, page);   // (its first barrier stands between this and its writing over last_token)
+            }
+            if (lane < 2) put(open_row(slot, position, lane), own[0], own[1]);
+            return;
         }
-        if (completes0) {   // by way of shared memory to the threads that have the block's last token
-            float (*const last_token)[kDim] = reinterpret_cast<float(*)[kDim]>(bytes);
-            if (lane < 2) { store_vec(last_token[lane] + ca, own[0]); store_vec(last_token[lane] + cb, own[1]); }
-            __syncthreads();
-            float x[2][kPer][2][4];
+    }
+
+    // ---- segments --------------------------------------------------------------------------------------------------------------------------------
+    // lane i of every warp: row row0 + i
+    int slot_i = -1, position_i = 0, first_i = 0, last_i = 0;
+    const int row_i = row0 + (tid & 31);
+    if ((tid & 31) < kTile && row_i < p.rows) { slot_i = p.slot[row_i]; position_i = p.positions[row_i]; first_i = p.run_first[row_i]; last_i = p.run_last[row_i]; }
+    bool ends = false;
+    if (slot_i >= 0) {
+        if (slot_i >= p.n_slots || first_i < 0 || first_i > row_i || last_i < row_i || last_i >= p.rows || position_i < row_i - first_i ||
+            position_i > 0x7fffffff - kKv8Tokens - (last_i - row_i))
+            atomicExch(p.status, 2);
+        else
+            ends = position_i % kKv8Tokens == kKv8Tokens - 1 || row_i == last_i;
+    }
+    for (uint32_t todo = __ballot_sync(0xffffffffu, ends); todo; todo &= todo - 1) {
+        const int from = __ffs(todo) - 1, row_b = row0 + from;
+        const int slot = __shfl_sync(0xffffffffu, slot_i, from), position = __shfl_sync(0xffffffffu, position_i, from), first = __shfl_sync(0xffffffffu, first_i, from),
+                  last = __shfl_sync(0xffffffffu, last_i, from);
+        const int block = position / kKv8Tokens, token_b = position % kKv8Tokens, row_a = max(first, row_b - token_b), token_a = token_b - (row_b - row_a), n = row_b - row_a + 1;
+        const int start = position - (row_b - first), end = position + (last - row_b);   // of the run
+        const bool continued = start % kKv8Tokens != 0, completes = token_b == kKv8Tokens - 1;
+        // keys and values of tokens lane + j kGroups: new rows, or open ones of the run's first block
+        Raw ka[2][kPer], kb[2][kPer];
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                const int token = lane + j * kGroups;
+                if (token >= token_a && token <= token_b) load(source(row_a + token - token_a, p.q_heads + which * p.kv_heads + kv_head), ka[which][j], kb[which][j]);
+                else if (completes) load(open_row(slot, block * kKv8Tokens + token, which), ka[which][j], kb[which][j]);
+            }
+        // queries: a lane group has a row and takes its heads kBatch at a time
+        constexpr int kBatch = 4;
+        Raw qa[kBatch], qb[kBatch];
+        auto load_queries = [&](int row, int h0) {
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+                if (row <= row_b && h0 + j < p.group) load(source(row, kv_head * p.group + h0 + j), qa[j], qb[j]);
+        };
+        load_queries(row_a + lane, 0);
+        fetch_angles(row_a, n);
+        const int page = completes ? page_of(slot, block) : -1;
+        __syncthreads();
+        for (int r0 = row_a; r0 <= row_b; r0 += kGroups) {
+            const int row = r0 + lane;
+            for (int h0 = 0; h0 < p.group; h0 += kBatch) {
+                Raw xa[kBatch], xb[kBatch];
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) { xa[j] = qa[j]; xb[j] = qb[j]; }
+                if (h0 + kBatch < p.group) load_queries(row, h0 + kBatch);
+                else if (r0 + kGroups <= row_b) load_queries(row + kGroups, 0);
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) {
+                    if (h0 + j >= p.group) break;
+                    float a[4] = {}, b[4] = {};
+                    if (row <= row_b) { xa[j].get(a); xb[j].get(b); }
+                    turn(p.r.q_gain, min(row, row_b) - row_a, a, b);
+                    if (row <= row_b) put(p.q + ((long long)row * p.q_heads + kv_head * p.group + h0 + j) * kDim, a, b);
+                }
+            }
+        }
+        float x[2][kPer][2][4];
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                const int token = lane + j * kGroups;
+                const bool fresh = token >= token_a && token <= token_b;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[which][j][0][k] = x[which][j][1][k] = 0.f;
+                if (fresh || completes) { ka[which][j].get(x[which][j][0]); kb[which][j].get(x[which][j][1]); }
+                if (which == 0) {   // rows of earlier calls are as they are to be
+                    float a[4], b[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) { a[k] = x[0][j][0][k]; b[k] = x[0][j][1][k]; }
+                    turn(p.r.k_gain, fresh ? token - token_a : 0, a, b);
+                    round_bf16(a, b);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) { x[0][j][0][k] = fresh ? a[k] : x[0][j][0][k]; x[0][j][1][k] = fresh ? b[k] : x[0][j][1][k]; }
+                }
+            }
+        if (completes) write_block(x, page);
+        // The rows of the run's last two blocks stay as they are, in the open rows. A run that goes on from the middle of a block and ends two blocks or more
+        // further on would have them written over rows of that block that another CTA may not have read yet: there the CTA with the run's first segment, which
+        // has read them (all its threads have, in front of write_block's barriers), does it for all.
+        const bool by_first = continued && end / kKv8Tokens >= start / kKv8Tokens + 2;
+        if (!by_first && block >= end / kKv8Tokens - 1) {
 #pragma unroll
             for (int which = 0; which < 2; ++which)
 #pragma unroll
                 for (int j = 0; j < kPer; ++j) {
-                    old_a[which][kTile == 1 ? j : 0].get(x[which][j][0]);
-                    old_b[which][kTile == 1 ? j : 0].get(x[which][j][1]);
-                    if (lane + j * kGroups == kKv8Tokens - 1) { load_vec(last_token[which] + ca, x[which][j][0]); load_vec(last_token[which] + cb, x[which][j][1]); }
+                    const int token = lane + j * kGroups;
+                    if (token >= token_a && token <= token_b) put(open_row(slot, block * kKv8Tokens + token, which), x[which][j][0], x[which][j][1]);
                 }
-            __syncthreads();
-            write_block(x, page0);
         }
-        if (lane < 2) {
-            __nv_bfloat16* dst = p.open + (long long)slot0 * kv8_open_elems(p.kv_heads, kDim) + kv8_open_at(position0 / kKv8Tokens, p.kv_heads, kv_head, lane, kDim) +
-                                 position0 % kKv8Tokens * kDim;
-            store_vec(dst + ca, own[0]);
-            store_vec(dst + cb, own[1]);
-        }
-        return;
-    }
-
-    for (int row = row0; row < row_end; ++row) {
-        const int slot = p.slot[row], position = p.positions[row], first = p.run_first[row], last = p.run_last[row];
-        if (slot < 0) continue;
-        if (slot >= p.n_slots || first < 0 || first > row || last < row || last >= p.rows || position < row - first || position > 0x7fffffff - kKv8Tokens - (last - row)) {
-            if (tid == 0) atomicExch(p.status, 2);
-            continue;
-        }
-        const int to_end = kKv8Tokens - 1 - position % kKv8Tokens;         // rows until the block of this one is complete
-        const bool continued = (position - (row - first)) % kKv8Tokens != 0;   // the run's first block holds tokens of an earlier call
-        const bool in_first = row - first < kKv8Tokens && (position - (row - first)) / kKv8Tokens == position / kKv8Tokens;
-        if (to_end == 0 && !(continued && in_first)) complete(row, first, slot, position);
-        if (row != first) continue;
-        if (continued && row + to_end <= last) complete(row + to_end, first, slot, position);
-        // the rows of the run's last two blocks stay as they are
-        const int end = position + (last - row);
-        const int keep = max(position, (end / kKv8Tokens - 1) * kKv8Tokens);
-        __nv_bfloat16* const open = p.open + (long long)slot * kv8_open_elems(p.kv_heads, kDim);
-        for (int q0 = keep; q0 <= end; q0 += kGroups) {
-            const int at = q0 + lane, from = row + (at - position);
-            const bool live = at <= end;
-            Raw ra[2], rb[2];
+        __syncthreads();   // `bytes`, `largest` and `angles` may be written again
+        if (by_first && row_a == first) {
+            for (int b0 = (end / kKv8Tokens - 1) * kKv8Tokens; b0 <= end; b0 += kKv8Tokens) {
+                const int count = min(kKv8Tokens, end - b0 + 1), from_row = first + (b0 - start);
+                fetch_angles(from_row, count);
+                __syncthreads();
 #pragma unroll
-            for (int which = 0; which < 2; ++which)
-                if (live) load(source(from, p.q_heads + which * p.kv_heads + kv_head), ra[which], rb[which]);
+                for (int which = 0; which < 2; ++which)
 #pragma unroll
-            for (int which = 0; which < 2; ++which) {
-                float a[4] = {}, b[4] = {};
-                if (live) { ra[which].get(a); rb[which].get(b); }
-                if (which == 0) turn(p.r.k_gain, live ? from : -1, a, b);
-                if (live) {
-                    __nv_bfloat16* dst = open + kv8_open_at(at / kKv8Tokens, p.kv_heads, kv_head, which, kDim) + at % kKv8Tokens * kDim;
-                    store_vec(dst + ca, a);
-                    store_vec(dst + cb, b);
-                }
+                    for (int j = 0; j < kPer; ++j) {
+                        const int token = lane + j * kGroups;
+                        float a[4] = {}, b[4] = {};
+                        if (token < count) {
+                            Raw ra, rb;
+                            load(source(from_row + token, p.q_heads + which * p.kv_heads + kv_head), ra, rb);
+                            ra.get(a);
+                            rb.get(b);
+                        }
+                        if (which == 0) turn(p.r.k_gain, min(token, count - 1), a, b);
+                        if (token < count) put(open_row(slot, b0 + token, which), a, b);
+                    }
+                __syncthreads();
             }
         }
     }
@@ -449,7 +454,7 @@ int gptrs_cuda_kv8_append(const gptrs_kv8_cache* c, const gptrs_kv8_append_step*
     p.q = static_cast<__nv_bfloat16*>(s->d_q);
     p.status = s->d_status;
     p.rows = (int)s->rows; p.q_heads = c->q_heads; p.kv_heads = c->kv_heads; p.group = c->q_heads / c->kv_heads;
-    const bool few = s->rows <= 256;
+    const bool few = s->rows <= 1024;   // (which are often runs of one row)
     const dim3 grid((unsigned)ceil_div(s->rows, few ? 1 : kKv8Tokens), (unsigned)c->kv_heads);
     auto kernel = c->dim == 64 ? (few ? kv8_append_kernel<64, 1> : kv8_append_kernel<64, 16>) : (few ? kv8_append_kernel<128, 1> : kv8_append_kernel<128, 16>);
     return launch_kernel(kernel, grid, dim3(kThreads), 0, as_stream(stream), 1, p);
