@@ -1,8 +1,8 @@
 // Append to the 8-bit cache (norm and rotation of queries and keys on the way), and reading tokens back.
 //
 // gptrs_cuda_kv8_append: a CTA takes the rows of a run that fall into one block (16 tokens) x one kv head with its query heads; it finds them from the last
-// of these rows, which lies in the 16 rows (of short lists, the one row) it looks at. A group of dim / 8 lanes works on a head's row at a time (four
-// rotated pairs per lane). What bounds it is the latency of loads that depend on each other (slot and position; angles; open rows), so keys, values, the
+// of these rows, which lies in the 16 rows (of short lists, the one row) it looks at. Queries go by eight pairs a
+// lane, with the products of gains and angles made once per row; keys and values by four (what bounds long lists is the number of instructions beside latency). What bounds it is the latency of loads that depend on each other (slot and position; angles; open rows), so keys, values, the
 // first queries and the angles (kept in shared memory) are asked for before anything is computed; for runs of one row (decode steps) with the rows in front of
 // it in its block. A block is written once, by the CTA with its last token: the largest magnitude over the CTA, then the bytes in order in shared memory.
 #include "kv8_cache.cuh"
@@ -27,23 +27,33 @@ struct AppendParams {
     int rows, q_heads, kv_heads, group;
 };
 
-// |x| as an ordered whole number that keeps infinities and NaN above all finite values
-__device__ __forceinline__ uint32_t magnitude(const float (&a)[4], const float (&b)[4], uint32_t m) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) m = max(m, max(__float_as_uint(a[k]) & 0x7fffffffu, __float_as_uint(b[k]) & 0x7fffffffu));
-    return m;
-}
-__device__ __forceinline__ void round_bf16(float (&a)[4], float (&b)[4]) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        a[k] = __bfloat162float(__float2bfloat16_rn(a[k]));
-        b[k] = __bfloat162float(__float2bfloat16_rn(b[k]));
+// A lane's eight channels of a key or value in bf16: four of its first run, four of its second.
+struct Packed {
+    uint2 a, b;
+    __device__ __forceinline__ void load(const __nv_bfloat16* src, int ca, int cb) { a = *reinterpret_cast<const uint2*>(src + ca); b = *reinterpret_cast<const uint2*>(src + cb); }
+    __device__ __forceinline__ void store(__nv_bfloat16* dst, int ca, int cb) const { *reinterpret_cast<uint2*>(dst + ca) = a; *reinterpret_cast<uint2*>(dst + cb) = b; }
+    __device__ __forceinline__ void get(float (&x)[4], float (&y)[4]) const {
+        x[0] = bf16_lo(a.x); x[1] = bf16_hi(a.x); x[2] = bf16_lo(a.y); x[3] = bf16_hi(a.y);
+        y[0] = bf16_lo(b.x); y[1] = bf16_hi(b.x); y[2] = bf16_lo(b.y); y[3] = bf16_hi(b.y);
     }
+    __device__ __forceinline__ void set(const float (&x)[4], const float (&y)[4]) {
+        a = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+        b = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+    }
+    // |x| of pairs as ordered whole numbers, with infinities and NaN above all finite values
+    __device__ __forceinline__ uint32_t magnitude(uint32_t m) const { return __vmaxu2(__vmaxu2(abs_bits_max2(a.x, a.y), abs_bits_max2(b.x, b.y)), m); }
+};
+
+// x / scale rounded to the nearest whole number, plus 128, in the lowest byte. The quotient is what a division gives: the product with the correctly rounded
+// inverse, and one correction by its exact remainder (Markstein). Adding 1.5 * 2^23 rounds it (ties to even).
+__device__ __forceinline__ uint32_t biased_byte(float x, float scale, float inverse) {
+    const float q = x * inverse;
+    return __float_as_uint(fmaf(fmaf(-scale, q, x), inverse, q) + (12582912.f + 128.f));
 }
 
 // kTile: consecutive rows that a CTA looks at, 1 or 16. It works on the segments (rows of one run and block) whose last row is among them.
 template <int kDim, int kTile>
-__global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kThreads, 4) kv8_append_kernel(const AppendParams p) {
     constexpr int kLanes = kDim / 8, kGroups = kThreads / kLanes, kPer = kKv8Tokens / kGroups;   // lanes of a head's row, rows at a time, tokens of a block per lane group
     constexpr int kPairs = kDim / 2;
     using Raw = RawVec<__nv_bfloat16, 4>;
@@ -59,36 +69,36 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
     pair_channels<4>(p.r, 4 * in_group, &ca, &cb);
     const bool turned = 4 * in_group < p.r.rot_half;
 
-    auto load = [&](const __nv_bfloat16* src, Raw& a, Raw& b) { a.load(src + ca); b.load(src + cb); };
     auto source = [&](int row, int head) { return p.qkv + row * p.ld + (long long)head * kDim; };
     auto open_row = [&](int slot, int position, int which) {
         return p.open + (long long)slot * kv8_open_elems(p.kv_heads, kDim) + kv8_open_at(position / kKv8Tokens, p.kv_heads, kv_head, which, kDim) + position % kKv8Tokens * kDim;
     };
     // Angles of rows [from, from + n), n <= 16, to shared memory: a chain of loads (axis and position, table), all rows' at a time.
-    auto fetch_angles = [&](int from, int n) {
-        if (!p.rotates || p.r.rot_half == 0) return;
-        constexpr int kSteps = kTile == 1 ? 4 : kKv8Tokens * kPairs / kThreads;
-        for (int i0 = tid; i0 < n * kPairs; i0 += kSteps * kThreads) {
-            long long at[kSteps];
+    const int my_pair = tid % kPairs, my_axis = p.rotates && p.r.pair_axis && my_pair < p.r.rot_half ? p.r.pair_axis[my_pair] : 0;
+    auto fetch_angles = [&](int from, int n) {   // a thread has one pair
+        if (!p.rotates || my_pair >= p.r.rot_half) return;
+        constexpr int kRows = kThreads / kPairs, kSteps = kTile == 1 ? 2 : kKv8Tokens / kRows;
+        const int* const at = p.r.axis_positions ? p.r.axis_positions + my_axis * p.r.axis_stride + from : p.positions + from;
+        for (int k0 = tid / kPairs; k0 < n; k0 += kSteps * kRows) {
+            int pos[kSteps];
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) pos[i] = k0 + i * kRows < n && my_axis < p.r.axes ? at[k0 + i * kRows] : -1;
+            // (all loads in front of the first store or atomic, which would keep the ones behind them waiting)
+            float c[kSteps], s[kSteps];
+            bool bad = false;
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
-                const int pair = (i0 + i * kThreads) % kPairs, k = (i0 + i * kThreads) / kPairs, row = from + k;
-                at[i] = -1;
-                if (pair < p.r.rot_half && k < n) {
-                    const int axis = p.r.pair_axis ? p.r.pair_axis[pair] : 0;
-                    long long pos = -1;
-                    if (axis < p.r.axes) pos = p.r.axis_positions ? p.r.axis_positions[axis * p.r.axis_stride + row] : p.positions[row];
-                    if (pos < 0 || pos >= p.r.positions) { atomicExch(p.status, 2); pos = 0; }
-                    at[i] = pos * p.r.rot_half + pair;
-                }
+                if (k0 + i * kRows < n && (pos[i] < 0 || pos[i] >= p.r.positions)) bad = true;
+                const long long place = (pos[i] < 0 || pos[i] >= p.r.positions ? 0ll : (long long)pos[i] * p.r.rot_half) + my_pair;
+                c[i] = p.r.cos[place];
+                s[i] = p.r.sin[place];
             }
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i)
-                if (at[i] >= 0) {
-                    const int pair = (i0 + i * kThreads) % kPairs, k = (i0 + i * kThreads) / kPairs;
-                    angles[0][k][pair] = p.r.cos[at[i]];
-                    angles[1][k][pair] = p.r.sin[at[i]];
-                }
+            for (int i = 0; i < kSteps; ++i) {
+                const int k = k0 + i * kRows;
+                if (k < n) { angles[0][k][my_pair] = c[i]; angles[1][k][my_pair] = s[i]; }
+            }
+            if (bad) atomicExch(p.status, 2);
         }
     };
     // Norm and rotation of a query's or key's row in registers; all lanes of a warp take part. k: its place in `angles`.
@@ -106,39 +116,67 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
         }
     };
     auto put = [&](__nv_bfloat16* dst, const float (&a)[4], const float (&b)[4]) { store_vec(dst + ca, a); store_vec(dst + cb, b); };
-    // The 16 tokens of a block, token lane + j kGroups of either kind in this thread's registers (f32, of bf16 value) -> the page. All threads.
-    auto write_block = [&](const float (&x)[2][kPer][2][4], int page) {
-        uint32_t m[2] = {0, 0};
+    // The 16 tokens of a block, token lane + j kGroups of either kind in this thread's registers -> the page. All threads.
+    auto write_block = [&](const Packed (&x)[2][kPer], int page) {
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
+            uint32_t m = 0;
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) m[which] = magnitude(x[which][j][0], x[which][j][1], m[which]);
-            m[which] = __reduce_max_sync(0xffffffffu, m[which]);
-            if ((tid & 31) == 0) largest[which][tid >> 5] = m[which];
+            for (int j = 0; j < kPer; ++j) m = x[which][j].magnitude(m);
+            m = __reduce_max_sync(0xffffffffu, widest_half(m));
+            if ((tid & 31) == 0) largest[which][tid >> 5] = m;
         }
         __syncthreads();
+        const bool even = (lane & 1) == 0;
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             uint32_t all = 0;
 #pragma unroll
             for (int i = 0; i < kThreads / 32; ++i) all = max(all, largest[which][i]);
-            const bool finite = all < 0x7f800000u;
-            const float scale = finite ? fmaxf(__fdiv_rn(__uint_as_float(all), 127.f), kKv8MinScale) : __uint_as_float(0x7fc00000u);
+            const bool finite = all < 0x7f80u;
+            const float scale = finite ? fmaxf(__fdiv_rn(__uint_as_float(all << 16), 127.f), kKv8MinScale) : __uint_as_float(0x7fc00000u);
+            const float inverse = __frcp_rn(scale);
+            uint32_t w[kPer][2];   // four bytes of either run
 #pragma unroll
             for (int j = 0; j < kPer; ++j) {
-                const int token = lane + j * kGroups;
+                float v[2][4];
+                x[which][j].get(v[0], v[1]);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const int ch = half ? cb : ca;
                     uint32_t u[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) u[k] = finite ? (uint32_t)(__float2int_rn(__fdiv_rn(x[which][j][half][k], scale)) + 128) : 128u;
-                    if (which == 0) {
-                        *reinterpret_cast<uint32_t*>(bytes + kv8_key_at(token, ch)) = u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24;
-                    } else {
+                    for (int k = 0; k < 4; ++k) u[k] = biased_byte(v[half][k], scale, inverse);
+                    w[j][half] = finite ? __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410) : 0x80808080u;
+                }
+            }
+            if (which == 0) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) bytes[kv8_value_at(token, ch + k, kDim)] = (unsigned char)u[k];
-                    }
+                for (int j = 0; j < kPer; ++j) {
+                    *reinterpret_cast<uint32_t*>(bytes + kv8_key_at(lane + j * kGroups, ca)) = w[j][0];
+                    *reinterpret_cast<uint32_t*>(bytes + kv8_key_at(lane + j * kGroups, cb)) = w[j][1];
+                }
+            } else {
+                // an even and an odd token next to each other: their lane groups exchange a run, so that either has four channels of both
+                uint32_t e[kPer], o[kPer];
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) {
+                    const uint32_t got = __shfl_xor_sync(0xffffffffu, even ? w[j][1] : w[j][0], kLanes);
+                    e[j] = even ? w[j][0] : got;
+                    o[j] = even ? got : w[j][1];
+                }
+                const int ch = even ? ca : cb, token = lane & ~1;
+                const uint32_t t0 = __byte_perm(e[0], o[0], 0x5140), t1 = __byte_perm(e[0], o[0], 0x7362);   // (channel 0, 1), (2, 3) of both tokens
+                if constexpr (kPer == 2) {
+                    const uint32_t u0 = __byte_perm(e[1], o[1], 0x5140), u1 = __byte_perm(e[1], o[1], 0x7362);
+                    *reinterpret_cast<uint32_t*>(bytes + kv8_value_at(token, ch, kDim)) = __byte_perm(t0, u0, 0x5410);
+                    *reinterpret_cast<uint32_t*>(bytes + kv8_value_at(token, ch + 1, kDim)) = __byte_perm(t0, u0, 0x7632);
+                    *reinterpret_cast<uint32_t*>(bytes + kv8_value_at(token, ch + 2, kDim)) = __byte_perm(t1, u1, 0x5410);
+                    *reinterpret_cast<uint32_t*>(bytes + kv8_value_at(token, ch + 3, kDim)) = __byte_perm(t1, u1, 0x7632);
+                } else {
+                    *reinterpret_cast<uint16_t*>(bytes + kv8_value_at(token, ch, kDim)) = (uint16_t)t0;
+                    *reinterpret_cast<uint16_t*>(bytes + kv8_value_at(token, ch + 1, kDim)) = (uint16_t)(t0 >> 16);
+                    *reinterpret_cast<uint16_t*>(bytes + kv8_value_at(token, ch + 2, kDim)) = (uint16_t)t1;
+                    *reinterpret_cast<uint16_t*>(bytes + kv8_value_at(token, ch + 3, kDim)) = (uint16_t)(t1 >> 16);
                 }
             }
             if (tid == 0) reinterpret_cast<float*>(bytes + 32 * kDim)[which] = scale;
@@ -150,6 +188,14 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
             for (int i = tid; i < 2 * kDim + 1; i += kThreads) dst[i] = reinterpret_cast<const uint4*>(bytes)[i];
         }
     };
+    // a key as it comes -> normed, rotated, rounded. k: its place in `angles`.
+    auto finish_key = [&](Packed x, int k) {
+        float a[4], b[4];
+        x.get(a, b);
+        turn(p.r.k_gain, k, a, b);
+        if (p.rotates) x.set(a, b);
+        return x;
+    };
     auto page_of = [&](int slot, int block) {
         if (block < p.max_pages) return kv8_page(p.table, slot, p.max_pages, block, p.n_pages, p.status);
         if (tid == 0) atomicExch(p.status, 2);
@@ -158,57 +204,46 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
 
     if (kTile == 1) {
         // ---- a run of one row: everything is asked for at once ---------------------------------------------------------------------------------
-        Raw qa, qb, own_a, own_b;
-        if (lane < p.group) load(source(row0, kv_head * p.group + lane), qa, qb);
-        if (lane < 2) load(source(row0, p.q_heads + lane * p.kv_heads + kv_head), own_a, own_b);
+        Raw qa, qb;
+        Packed own = {};
+        if (lane < p.group) { const __nv_bfloat16* src = source(row0, kv_head * p.group + lane); qa.load(src + ca); qb.load(src + cb); }
+        if (lane < 2) own.load(source(row0, p.q_heads + lane * p.kv_heads + kv_head), ca, cb);   // lane group 0 has the key, 1 the value
         const int slot = p.slot[row0], position = p.positions[row0], first = p.run_first[row0], last = p.run_last[row0];
         if (slot < 0) return;
         if (first == row0 && last == row0 && slot < p.n_slots && position >= 0 && position <= 0x7fffffff - kKv8Tokens) {
             fetch_angles(row0, 1);
             const bool completes = position % kKv8Tokens == kKv8Tokens - 1;
-            Raw old_a[2][kPer], old_b[2][kPer];
+            Packed x[2][kPer];
             int page = -1;
             if (completes) {
 #pragma unroll
                 for (int which = 0; which < 2; ++which)
 #pragma unroll
-                    for (int j = 0; j < kPer; ++j)
-                        load(open_row(slot, position - (kKv8Tokens - 1) + lane + j * kGroups, which), old_a[which][j], old_b[which][j]);
+                    for (int j = 0; j < kPer; ++j) x[which][j].load(open_row(slot, position - (kKv8Tokens - 1) + lane + j * kGroups, which), ca, cb);
                 page = page_of(slot, position / kKv8Tokens);
             }
             __syncthreads();
             for (int h0 = 0; h0 < p.group; h0 += kGroups) {
                 const int h = h0 + lane;
                 float a[4] = {}, b[4] = {};
-                if (h0 > 0 && h < p.group) load(source(row0, kv_head * p.group + h), qa, qb);
+                if (h0 > 0 && h < p.group) { const __nv_bfloat16* src = source(row0, kv_head * p.group + h); qa.load(src + ca); qb.load(src + cb); }
                 if (h < p.group) { qa.get(a); qb.get(b); }
                 turn(p.r.q_gain, 0, a, b);
                 if (h < p.group) put(p.q + ((long long)row0 * p.q_heads + kv_head * p.group + h) * kDim, a, b);
             }
-            float own[2][4] = {}, a[4] = {}, b[4] = {};   // lane group 0 has the key, 1 the value (which stays as it is)
-            if (lane < 2) { own_a.get(own[0]); own_b.get(own[1]); own_a.get(a); own_b.get(b); }
-            turn(p.r.k_gain, 0, a, b);
-            if (lane == 0) {
-                round_bf16(a, b);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) { own[0][k] = a[k]; own[1][k] = b[k]; }
-            }
+            const Packed key = finish_key(own, 0);
+            if (lane == 0) own = key;
             if (completes) {   // by way of shared memory to the threads that have the block's last token
-                float (*const last_token)[kDim] = reinterpret_cast<float(*)[kDim]>(bytes);
-                if (lane < 2) { store_vec(last_token[lane] + ca, own[0]); store_vec(last_token[lane] + cb, own[1]); }
+                __nv_bfloat16* const last_token = reinterpret_cast<__nv_bfloat16*>(bytes);
+                if (lane < 2) own.store(last_token + lane * kDim, ca, cb);
                 __syncthreads();
-                float x[2][kPer][2][4];
-#pragma unroll
-                for (int which = 0; which < 2; ++which)
-#pragma unroll
-                    for (int j = 0; j < kPer; ++j) {
-                        old_a[which][j].get(x[which][j][0]);
-                        old_b[which][j].get(x[which][j][1]);
-                        if (lane + j * kGroups == kKv8Tokens - 1) { load_vec(last_token[which] + ca, x[which][j][0]); load_vec(last_token[which] + cb, x[which][j][1]); }
-                    }
+                if (lane + (kPer - 1) * kGroups == kKv8Tokens - 1) {
+                    x[0][kPer - 1].load(last_token, ca, cb);
+                    x[1][kPer - 1].load(last_token + kDim, ca, cb);
+                }
                 write_block(x, page);   // (its first barrier stands between this and its writing over last_token)
             }
-            if (lane < 2) put(open_row(slot, position, lane), own[0], own[1]);
+            if (lane < 2) own.store(open_row(slot, position, lane), ca, cb);
             return;
         }
     }
@@ -234,65 +269,73 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
         const int start = position - (row_b - first), end = position + (last - row_b);   // of the run
         const bool continued = start % kKv8Tokens != 0, completes = token_b == kKv8Tokens - 1;
         // keys and values of tokens lane + j kGroups: new rows, or open ones of the run's first block
-        Raw ka[2][kPer], kb[2][kPer];
+        Packed x[2][kPer] = {};
 #pragma unroll
         for (int which = 0; which < 2; ++which)
 #pragma unroll
             for (int j = 0; j < kPer; ++j) {
                 const int token = lane + j * kGroups;
-                if (token >= token_a && token <= token_b) load(source(row_a + token - token_a, p.q_heads + which * p.kv_heads + kv_head), ka[which][j], kb[which][j]);
-                else if (completes) load(open_row(slot, block * kKv8Tokens + token, which), ka[which][j], kb[which][j]);
+                if (token >= token_a && token <= token_b) x[which][j].load(source(row_a + token - token_a, p.q_heads + which * p.kv_heads + kv_head), ca, cb);
+                else if (completes) x[which][j].load(open_row(slot, block * kKv8Tokens + token, which), ca, cb);
             }
-        // queries: a lane group has a row and takes its heads kBatch at a time
-        constexpr int kBatch = 4;
-        Raw qa[kBatch], qb[kBatch];
-        auto load_queries = [&](int row, int h0) {
+        // queries: eight pairs a lane, so that dim / 16 lanes have a row (one of 16) and take its heads, kBatch on their way
+        constexpr int kQLanes = kDim / 16, kAtOnce = kThreads / kQLanes / kKv8Tokens, kBatch = 4;
+        const int q_lane = tid % kQLanes, q_row = tid / kQLanes % kKv8Tokens, q_first = tid / kQLanes / kKv8Tokens;
+        const bool q_live = q_row < n, q_turned = 8 * q_lane < p.r.rot_half;
+        int qca, qcb;
+        pair_channels<8>(p.r, 8 * q_lane, &qca, &qcb);
+        const __nv_bfloat16* const q_src = source(row_a + min(q_row, n - 1), kv_head * p.group);
+        __nv_bfloat16* const q_dst = p.q + ((long long)(row_a + min(q_row, n - 1)) * p.q_heads + kv_head * p.group) * kDim;
+        RawVec<__nv_bfloat16, 8> qa[kBatch], qb[kBatch];
+        auto load_queries = [&](int h0) {
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j)
-                if (row <= row_b && h0 + j < p.group) load(source(row, kv_head * p.group + h0 + j), qa[j], qb[j]);
+            for (int j = 0; j < kBatch; ++j) {
+                const int h = h0 + j * kAtOnce + q_first;
+                if (q_live && h < p.group) { qa[j].load(q_src + h * kDim + qca); qb[j].load(q_src + h * kDim + qcb); }
+            }
         };
-        load_queries(row_a + lane, 0);
+        load_queries(0);
         fetch_angles(row_a, n);
         const int page = completes ? page_of(slot, block) : -1;
         __syncthreads();
-        for (int r0 = row_a; r0 <= row_b; r0 += kGroups) {
-            const int row = r0 + lane;
-            for (int h0 = 0; h0 < p.group; h0 += kBatch) {
-                Raw xa[kBatch], xb[kBatch];
-#pragma unroll
-                for (int j = 0; j < kBatch; ++j) { xa[j] = qa[j]; xb[j] = qb[j]; }
-                if (h0 + kBatch < p.group) load_queries(row, h0 + kBatch);
-                else if (r0 + kGroups <= row_b) load_queries(row + kGroups, 0);
+        {
+            const bool apart = !p.r.neighbours;
+            Turn<8> t;
+            if (p.rotates && apart) t.set(p.r.q_gain, qca, qcb, q_turned, &angles[0][min(q_row, n - 1)][8 * q_lane], &angles[1][min(q_row, n - 1)][8 * q_lane]);
+            for (int h0 = 0; h0 < p.group; h0 += kBatch * kAtOnce) {
 #pragma unroll
                 for (int j = 0; j < kBatch; ++j) {
-                    if (h0 + j >= p.group) break;
-                    float a[4] = {}, b[4] = {};
-                    if (row <= row_b) { xa[j].get(a); xb[j].get(b); }
-                    turn(p.r.q_gain, min(row, row_b) - row_a, a, b);
-                    if (row <= row_b) put(p.q + ((long long)row * p.q_heads + kv_head * p.group + h0 + j) * kDim, a, b);
+                    if (h0 + j * kAtOnce >= p.group) break;
+                    const int h = h0 + j * kAtOnce + q_first;
+                    const bool live = q_live && h < p.group;
+                    float a[8] = {}, b[8] = {};
+                    if (live) { qa[j].get(a); qb[j].get(b); }
+                    if (p.rotates) {
+                        const float rms = p.r.q_gain ? rsqrtf(lane_group_sum(square_sum2(a, b), kQLanes) * (1.f / kDim) + p.r.eps) : 1.f;
+                        if (apart) {
+                            t.apply(a, b, rms, q_turned);
+                        } else {
+                            if (p.r.q_gain) times_gain(p.r.q_gain, qca, qcb, rms, a, b);
+                            if (q_turned) {
+                                float c[8], s[8];
+                                load_vec(&angles[0][min(q_row, n - 1)][8 * q_lane], c);
+                                load_vec(&angles[1][min(q_row, n - 1)][8 * q_lane], s);
+                                rotate_pairs(false, a, b, c, s);
+                            }
+                        }
+                    }
+                    if (live) { store_vec(q_dst + h * kDim + qca, a); store_vec(q_dst + h * kDim + qcb, b); }
                 }
+                if (h0 + kBatch * kAtOnce < p.group) load_queries(h0 + kBatch * kAtOnce);
             }
         }
-        float x[2][kPer][2][4];
 #pragma unroll
-        for (int which = 0; which < 2; ++which)
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                const int token = lane + j * kGroups;
-                const bool fresh = token >= token_a && token <= token_b;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[which][j][0][k] = x[which][j][1][k] = 0.f;
-                if (fresh || completes) { ka[which][j].get(x[which][j][0]); kb[which][j].get(x[which][j][1]); }
-                if (which == 0) {   // rows of earlier calls are as they are to be
-                    float a[4], b[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) { a[k] = x[0][j][0][k]; b[k] = x[0][j][1][k]; }
-                    turn(p.r.k_gain, fresh ? token - token_a : 0, a, b);
-                    round_bf16(a, b);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) { x[0][j][0][k] = fresh ? a[k] : x[0][j][0][k]; x[0][j][1][k] = fresh ? b[k] : x[0][j][1][k]; }
-                }
-            }
+        for (int j = 0; j < kPer; ++j) {   // rows of earlier calls are as they are to be
+            const int token = lane + j * kGroups;
+            const bool fresh = token >= token_a && token <= token_b;
+            const Packed key = finish_key(x[0][j], fresh ? token - token_a : 0);
+            if (fresh) x[0][j] = key;
+        }
         if (completes) write_block(x, page);
         // The rows of the run's last two blocks stay as they are, in the open rows. A run that goes on from the middle of a block and ends two blocks or more
         // further on would have them written over rows of that block that another CTA may not have read yet: there the CTA with the run's first segment, which
@@ -304,7 +347,7 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
 #pragma unroll
                 for (int j = 0; j < kPer; ++j) {
                     const int token = lane + j * kGroups;
-                    if (token >= token_a && token <= token_b) put(open_row(slot, block * kKv8Tokens + token, which), x[which][j][0], x[which][j][1]);
+                    if (token >= token_a && token <= token_b) x[which][j].store(open_row(slot, block * kKv8Tokens + token, which), ca, cb);
                 }
         }
         __syncthreads();   // `bytes`, `largest` and `angles` may be written again
@@ -318,15 +361,10 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
 #pragma unroll
                     for (int j = 0; j < kPer; ++j) {
                         const int token = lane + j * kGroups;
-                        float a[4] = {}, b[4] = {};
-                        if (token < count) {
-                            Raw ra, rb;
-                            load(source(from_row + token, p.q_heads + which * p.kv_heads + kv_head), ra, rb);
-                            ra.get(a);
-                            rb.get(b);
-                        }
-                        if (which == 0) turn(p.r.k_gain, min(token, count - 1), a, b);
-                        if (token < count) put(open_row(slot, b0 + token, which), a, b);
+                        Packed row = {};
+                        if (token < count) row.load(source(from_row + token, p.q_heads + which * p.kv_heads + kv_head), ca, cb);
+                        if (which == 0) row = finish_key(row, min(token, count - 1));
+                        if (token < count) row.store(open_row(slot, b0 + token, which), ca, cb);
                     }
                 __syncthreads();
             }
@@ -439,7 +477,7 @@ int gptrs_cuda_kv8_append(const gptrs_kv8_cache* c, const gptrs_kv8_append_step*
         const int rr = qk_rotation_of(*s->rotation, s->rows, &p.r);
         if (rr) return rr;
         GPTRS_REQUIRE(p.r.q_heads == c->q_heads && p.r.kv_heads == c->kv_heads && p.r.dim == c->dim, "the rotation is of other heads");
-        if (p.r.rot_half % 4) return fail(GPTRS_UNIMPLEMENTED, "the append takes rotations of a multiple of 4 pairs");
+        if (p.r.rot_half % 8) return fail(GPTRS_UNIMPLEMENTED, "the append takes rotations of a multiple of 8 pairs");
         GPTRS_REQUIRE(aligned16(p.r.cos) && aligned16(p.r.sin) && aligned16(p.r.q_gain) && aligned16(p.r.k_gain), "tables and gains must be 16-byte aligned");
         p.rotates = 1;
     } else {

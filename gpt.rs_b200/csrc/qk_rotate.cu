@@ -48,10 +48,11 @@ constexpr int kThreads = 256;
 template <int kVec>
 __device__ __forceinline__ void lane_angles(const NormRopeParams& p, int row, int first, const uint32_t (&axes)[kVec / 4], float (&c)[kVec], float (&s)[kVec]) {
     const QkRotation& r = p.r;
+    bool bad = false;   // (reported behind the loads: an atomic in between would keep the next ones waiting)
     auto place = [&](int axis) {
         long long pos = -1;
         if (axis < r.axes) pos = r.axis_positions ? r.axis_positions[axis * r.axis_stride + row] : p.positions[row];
-        if (pos < 0 || pos >= r.positions) { atomicExch(p.status, 2); pos = 0; }
+        if (pos < 0 || pos >= r.positions) { bad = true; pos = 0; }
         return pos * r.rot_half + first;
     };
 #pragma unroll
@@ -71,6 +72,7 @@ __device__ __forceinline__ void lane_angles(const NormRopeParams& p, int row, in
             }
         }
     }
+    if (bad) atomicExch(p.status, 2);
 }
 
 constexpr int kAhead = 2;   // heads of a lane group on their way

@@ -86,22 +86,17 @@ __device__ __forceinline__ void pair_angles(const QkRotation& r, int row, int po
         return;
     }
     const float *cos = r.cos + i, *sin = r.sin + i;
-    if (r.pair_axis == nullptr) {
-        long long pos = r.axis_positions ? r.axis_positions[row] : position;
-        if (pos < 0 || pos >= r.positions) { atomicExch(status, 2); pos = 0; }
-        load_vec(cos + pos * r.rot_half, c);
-        load_vec(sin + pos * r.rot_half, s);
-    } else {
+    bool bad = false;   // (reported behind the loads: an atomic in between would keep the next ones waiting)
 #pragma unroll
-        for (int k = 0; k < kVec; ++k) {
-            const int axis = r.pair_axis[i + k];
-            long long pos = -1;
-            if (axis < r.axes) pos = r.axis_positions ? r.axis_positions[axis * r.axis_stride + row] : position;
-            if (pos < 0 || pos >= r.positions) { atomicExch(status, 2); pos = 0; }
-            c[k] = cos[pos * r.rot_half + k];
-            s[k] = sin[pos * r.rot_half + k];
-        }
+    for (int k = 0; k < kVec; ++k) {
+        const int axis = r.pair_axis ? r.pair_axis[i + k] : 0;
+        long long pos = -1;
+        if (axis < r.axes) pos = r.axis_positions ? r.axis_positions[axis * r.axis_stride + row] : position;
+        if (pos < 0 || pos >= r.positions) { bad = true; pos = 0; }
+        c[k] = cos[pos * r.rot_half + k];
+        s[k] = sin[pos * r.rot_half + k];
     }
+    if (bad) atomicExch(status, 2);
 }
 
 // the rotation of a lane's pairs, whose channels are `apart` (pair k = a[k], b[k]) or neighbours
@@ -141,6 +136,47 @@ __device__ __forceinline__ void times_gain(const float* gain, int ca, int cb, fl
     load_vec(gain + cb, gb);
 #pragma unroll
     for (int k = 0; k < kVec; ++k) { a[k] = a[k] * r * ga[k]; b[k] = b[k] * r * gb[k]; }
+}
+// With gains g and angles (c, s) of pairs apart, out_a = r (x_a g_a c - x_b g_b s) and out_b = r (x_b g_b c + x_a g_a s): the four products of gains and angles
+// are made once for several heads, two pairs at a time.
+template <int kVec>
+struct Turn {
+    uint64_t ac[kVec / 2], bs[kVec / 2], bc[kVec / 2], as[kVec / 2];
+    // gain NULL: no norm; turned false: angles (1, 0)
+    __device__ __forceinline__ void set(const float* gain, int ca, int cb, bool turned, const float* cos, const float* sin) {
+        float ga[kVec], gb[kVec], c[kVec], s[kVec];
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) { ga[k] = gb[k] = c[k] = 1.f; s[k] = 0.f; }
+        if (gain) { load_vec(gain + ca, ga); load_vec(gain + cb, gb); }
+        if (turned) { load_vec(cos, c); load_vec(sin, s); }
+#pragma unroll
+        for (int k = 0; k < kVec / 2; ++k) {
+            const uint64_t c2 = pair_of(c[2 * k], c[2 * k + 1]), s2 = pair_of(s[2 * k], s[2 * k + 1]);
+            const uint64_t a2 = pair_of(ga[2 * k], ga[2 * k + 1]), b2 = pair_of(gb[2 * k], gb[2 * k + 1]);
+            ac[k] = mul2(a2, c2); as[k] = mul2(a2, s2); bc[k] = mul2(b2, c2); bs[k] = mul2(b2, s2) ^ 0x8000000080000000ull;
+        }
+    }
+    __device__ __forceinline__ void apply(float (&a)[kVec], float (&b)[kVec], float rms, bool turned) const {
+        const uint64_t rms2 = pair_of(rms, rms);
+#pragma unroll
+        for (int k = 0; k < kVec / 2; ++k) {
+            const uint64_t ar = mul2(pair_of(a[2 * k], a[2 * k + 1]), rms2), br = mul2(pair_of(b[2 * k], b[2 * k + 1]), rms2);
+            // (a channel that stays does not meet the other one, which may be infinite)
+            const float2 x = split(turned ? fma2(ar, ac[k], mul2(br, bs[k])) : mul2(ar, ac[k])), y = split(turned ? fma2(br, bc[k], mul2(ar, as[k])) : mul2(br, bc[k]));
+            a[2 * k] = x.x; a[2 * k + 1] = x.y; b[2 * k] = y.x; b[2 * k + 1] = y.y;
+        }
+    }
+};
+template <int kVec>
+__device__ __forceinline__ float square_sum2(const float (&a)[kVec], const float (&b)[kVec]) {
+    uint64_t t = 0;
+#pragma unroll
+    for (int k = 0; k < kVec / 2; ++k) {
+        const uint64_t a2 = pair_of(a[2 * k], a[2 * k + 1]), b2 = pair_of(b[2 * k], b[2 * k + 1]);
+        t = fma2(a2, a2, fma2(b2, b2, t));
+    }
+    const float2 v = split(t);
+    return v.x + v.y;
 }
 // sum over the `lanes` (a power of two) neighbouring lanes of a head
 __device__ __forceinline__ float lane_group_sum(float v, int lanes) {

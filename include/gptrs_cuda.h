@@ -759,7 +759,7 @@ int gptrs_cuda_kv8_layout(gptrs_kv8_cache* c);
  * rotation NULL: queries and keys as they are. A block whose page_table entry is negative is not kept. *d_status = 2: a slot, position, page
  * or run out of range (the keys and values of that row or block are left out). */
 typedef struct {
-    const gptrs_qk_rotation* rotation; /* rot_half a multiple of 4 */
+    const gptrs_qk_rotation* rotation; /* rot_half a multiple of 8 */
     const void* d_qkv;
     int64_t ld;                        /* 0 = packed */
     const int32_t *d_positions, *d_slot, *d_run_first, *d_run_last;
