@@ -8,17 +8,32 @@
 // A warp takes a block at a time. Keys are the rows of the matrix product, heads its columns (eight query heads of a kv head at most): S^T = K Q^T
 // and O^T = V^T P^T, so that little of a matrix instruction is padding. The cache's byte order makes 16 bytes of a lane two k-steps of keys, or two
 // row tiles of values. The 8 x 8 transposition between the two products is one instruction per eight tokens.
-// Grid: (splits of the keys, kv head x eights of its query heads, row); four warps deal a split's blocks among them and merge through shared memory;
-// several splits of a row go through scratch and a second kernel.
+// Four warps deal the blocks of a part of the keys among them, each with a ring of its own in shared memory that bulk copies fill (a block is one piece of
+// memory, its scales included), and merge at the end. Up to eight parts of a row and kv head (of eight of its query heads) are a cluster that merges
+// through distributed shared memory; more go through scratch and a second kernel.
 #include <algorithm>
 
 #include "kv8_attention.cuh"
 
 namespace gptrs {
+
+void prefill_tc_fault(int* starve, uint32_t* wait_limit);   // the test switch of paged_prefill_tc.cu
+
 namespace {
 
 constexpr int kWarps = 4;
 constexpr int kCols = 8;    // query heads of a CTA
+constexpr int kDepth = 4;   // blocks of a warp's ring
+constexpr int kCtas = 3;    // of an SM
+constexpr int kMostRanks = 8;   // parts that a cluster merges
+
+// Weight of a part (warp, CTA, split) with maximum m and sum l beside the largest maximum; one without a maximum has seen nothing (0) or nothing but NaN.
+__device__ __forceinline__ float part_factor(float m, float l, float top) { return m == -INFINITY ? (l == 0.f ? 0.f : l) : kv8_exp2(m - top); }
+__device__ __forceinline__ uint4 lds_16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
 
 // A row's blocks in parts of equal size, at most chunk_blocks each.
 __device__ __forceinline__ void parts_of(const Kv8Attention& p, const Kv8Span& s, int* first, int* blocks, int* parts, int* per) {
@@ -29,37 +44,77 @@ __device__ __forceinline__ void parts_of(const Kv8Attention& p, const Kv8Span& s
     *parts = (*blocks + *per - 1) / *per;
 }
 
-template <int kDim>
-__global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(const Kv8Attention p) {
-    constexpr int kC = kDim / 32;      // chunks of 32 channels
-    __shared__ float o_part[kWarps][kCols][kDim + 1];
-    __shared__ float ml_part[kWarps][kCols][2];
+struct AttentionLaunch {
+    Kv8Attention a;
+    uint32_t spins;               // polls of a bounded wait
+    int starve;                   // test switch: the first block of a warp is never asked for
+};
 
+// kCluster: the splits of a row and kv head are a cluster (grid.y) that merges through distributed shared memory; else they are grid.x and write parts.
+template <int kDim, bool kCluster>
+__global__ void __launch_bounds__(kWarps * 32, kCtas) kv8_attention_kernel(const AttentionLaunch launch) {
+    constexpr int kC = kDim / 32;      // chunks of 32 channels
+    constexpr int kBlockBytes = (int)kv8_block_bytes(kDim);
+    extern __shared__ __align__(128) unsigned char ring[];
+    __shared__ __align__(8) uint64_t full[kWarps][kDepth];
+    __shared__ float ml_part[kWarps][kCols][2];
+    __shared__ __align__(16) float own_part[kCluster ? kCols * (kDim + 4) : 4];   // kCluster: output, maximum and sum of this CTA's part
+
+    const Kv8Attention& p = launch.a;
+    const int split = kCluster ? blockIdx.y : blockIdx.x, pair = kCluster ? blockIdx.x : blockIdx.y, eights = (p.group + kCols - 1) / kCols;
+    const int kv_head = pair / eights, head0 = kv_head * p.group + (pair % eights) * kCols;
+    const int cols = min(kCols, p.group - (pair % eights) * kCols);
+    const int row = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    if (lane == 0) {
+        for (int i = 0; i < kDepth; ++i) mbar_init(&full[warp][i], 1);
+        mbar_fence_init();
+    }
+    __syncwarp();
     pdl_launch_dependents();
     pdl_wait();
-    const int split = blockIdx.x, eights = (p.group + kCols - 1) / kCols;
-    const int kv_head = blockIdx.y / eights, head0 = kv_head * p.group + (blockIdx.y % eights) * kCols;
-    const int cols = min(kCols, p.group - (int)(blockIdx.y % eights) * kCols);
-    const int row = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    // the query, on its way while the lengths are
+    const __nv_bfloat16* const q_src = p.q + row * p.ldq + (long long)(head0 + min(g, cols - 1)) * kDim + 8 * t;
+    uint4 raw[kC];
+#pragma unroll
+    for (int c = 0; c < kC; ++c) raw[c] = __ldg(reinterpret_cast<const uint4*>(q_src + 32 * c));
     const Kv8Span span = kv8_span(p, row);
-    if (span.slot < 0) return;
+    if (span.slot < 0) return;                    // (the whole cluster)
     int first, blocks, parts, per;
     parts_of(p, span, &first, &blocks, &parts, &per);
-    if (split >= parts && !(split == 0 && parts == 0)) return;
-    const int b_end = first + min((split + 1) * per, blocks);
+    if (!kCluster && split >= parts && !(split == 0 && parts == 0)) return;
+    const int b0 = first + min(split * per, blocks) + warp, b_end = first + min((split + 1) * per, blocks);
+    const int n_my = b_end > b0 ? (b_end - b0 + kWarps - 1) / kWarps : 0;                        // blocks b0, b0 + kWarps, ..
+    const bool last_open = n_my > 0 && (b0 + (n_my - 1) * kWarps + 1) * kKv8Tokens > span.length;   // only a sequence's last block is not complete
+    const int n_closed = n_my - (last_open ? 1 : 0);
 
-    // ---- queries: column g of B, channels 32 c + 8 t + 4 s .. + 3 -------------------------------------------------------------------------
+    // ---- the warp's ring: blocks by bulk copies, their pages' numbers 32 at a time --------------------------------------------------------------
+    unsigned char* const my_ring = ring + warp * (kDepth * kBlockBytes);
+    const int* const numbers = p.table + span.slot * p.max_pages + b0;
+    int my_page = 0;
+    uint32_t bad[2] = {0, 0};                     // numbers that are none, of the 32 blocks asked for last and of those before them
+    auto ask = [&](int j) {                       // whole warp, j one after the other
+        if ((j & 31) == 0) {
+            my_page = j + lane < n_closed ? numbers[(j + lane) * kWarps] : 0;
+            const bool none = my_page < 0 || my_page >= p.n_pages;
+            if (none) { atomicExch(p.status, 2); my_page = 0; }
+            bad[(j >> 5) & 1] = __ballot_sync(0xffffffffu, none);
+        }
+        const int page = __shfl_sync(0xffffffffu, my_page, j & 31);
+        if (lane == 0) {
+            uint64_t* const bar = &full[warp][j % kDepth];
+            mbar_expect_tx(bar, kBlockBytes);
+            if (!(launch.starve && j == 0)) bulk_g2s(my_ring + j % kDepth * kBlockBytes, p.pool + ((long long)page * p.kv_heads + kv_head) * kBlockBytes, kBlockBytes, bar);
+        }
+    };
+    for (int j = 0; j < kDepth && j < n_closed; ++j) ask(j);
+
+    // ---- queries: column g of B, channels 32 c + 8 t + 4 s .. + 3; f16 with a power of two in front --------------------------------------------------
     uint32_t qf[kC][2][2];
     float q_scale;
     {
-        uint32_t raw[kC][2][2], big = 0;
-        const __nv_bfloat16* src = p.q + row * p.ldq + (long long)(head0 + min(g, cols - 1)) * kDim;
+        uint32_t big = 0;
 #pragma unroll
-        for (int c = 0; c < kC; ++c) {
-            const uint4 v = *reinterpret_cast<const uint4*>(src + 32 * c + 8 * t);
-            raw[c][0][0] = v.x; raw[c][0][1] = v.y; raw[c][1][0] = v.z; raw[c][1][1] = v.w;
-            big = __vmaxu2(big, __vmaxu2(abs_bits_max2(v.x, v.y), abs_bits_max2(v.z, v.w)));
-        }
+        for (int c = 0; c < kC; ++c) big = __vmaxu2(big, __vmaxu2(abs_bits_max2(raw[c].x, raw[c].y), abs_bits_max2(raw[c].z, raw[c].w)));
         uint32_t top = widest_half(big);
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -67,11 +122,10 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(const Kv8Att
         const float factor = e == 128 ? 0.f : pow2(-e);
         q_scale = e == 128 ? __uint_as_float(0x7fc00000u) : pow2(e) * p.scale_log2;
 #pragma unroll
-        for (int c = 0; c < kC; ++c)
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) qf[c][s][i] = bf16x2_to_f16x2(raw[c][s][i], factor);
+        for (int c = 0; c < kC; ++c) {
+            qf[c][0][0] = bf16x2_to_f16x2(raw[c].x, factor); qf[c][0][1] = bf16x2_to_f16x2(raw[c].y, factor);
+            qf[c][1][0] = bf16x2_to_f16x2(raw[c].z, factor); qf[c][1][1] = bf16x2_to_f16x2(raw[c].w, factor);
+        }
     }
     // the lane's two columns of S^T: heads 2 t, 2 t + 1
     const float qs0 = __shfl_sync(0xffffffffu, q_scale, 8 * t), qs1 = __shfl_sync(0xffffffffu, q_scale, 8 * t + 4);
@@ -82,89 +136,15 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(const Kv8Att
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    bool failed = false;
 
-    for (int b = first + split * per + warp; b < b_end; b += kWarps) {
-        uint32_t kf[kC][2][4], vf[2 * kC][4];
-        float k_scale, v_scale;
-        if ((b + 1) * kKv8Tokens <= span.length) {
-            const int page = kv8_page(p.table, span.slot, p.max_pages, b, p.n_pages, p.status);
-            if (page < 0) { atomicExch(p.status, 2); continue; }
-            const unsigned char* src = p.pool + ((long long)page * p.kv_heads + kv_head) * kv8_block_bytes(kDim);
-            const float2 scale = __ldg(reinterpret_cast<const float2*>(src + 32 * kDim));
-            k_scale = scale.x; v_scale = scale.y;
-            uint4 kb[kC], vb[kC];
-#pragma unroll
-            for (int c = 0; c < kC; ++c) kb[c] = ldg_stream_16(src + c * 512 + lane * 16);
-#pragma unroll
-            for (int c = 0; c < kC; ++c) vb[c] = ldg_stream_16(src + 16 * kDim + c * 512 + lane * 16);
-#pragma unroll
-            for (int c = 0; c < kC; ++c) {
-                kv8_widen(kb[c].x, &kf[c][0][0], &kf[c][0][2]);
-                kv8_widen(kb[c].y, &kf[c][1][0], &kf[c][1][2]);
-                kv8_widen(kb[c].z, &kf[c][0][1], &kf[c][0][3]);
-                kv8_widen(kb[c].w, &kf[c][1][1], &kf[c][1][3]);
-                kv8_widen(vb[c].x, &vf[2 * c][0], &vf[2 * c][2]);
-                kv8_widen(vb[c].y, &vf[2 * c][1], &vf[2 * c][3]);
-                kv8_widen(vb[c].z, &vf[2 * c + 1][0], &vf[2 * c + 1][2]);
-                kv8_widen(vb[c].w, &vf[2 * c + 1][1], &vf[2 * c + 1][3]);
-            }
-        } else {
-            // the block that is not complete: bf16 rows; what lies behind the last token may be anything and counts as zero
-            const int have = span.length - b * kKv8Tokens;
-            const __nv_bfloat16* ks = p.open + (long long)span.slot * kv8_open_elems(p.kv_heads, kDim) + kv8_open_at(b, p.kv_heads, kv_head, 0, kDim);
-            const __nv_bfloat16* vs = ks + kKv8Tokens * kDim;
-            uint4 kr[kC][2];
-            uint32_t big = 0;
-#pragma unroll
-            for (int c = 0; c < kC; ++c)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    kr[c][r] = g + 8 * r < have ? *reinterpret_cast<const uint4*>(ks + (g + 8 * r) * kDim + 32 * c + 8 * t) : make_uint4(0, 0, 0, 0);
-                    big = __vmaxu2(big, __vmaxu2(abs_bits_max2(kr[c][r].x, kr[c][r].y), abs_bits_max2(kr[c][r].z, kr[c][r].w)));
-                }
-            int e = pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big)));
-            float factor = e == 128 ? 0.f : pow2(-e);
-            k_scale = e == 128 ? __uint_as_float(0x7fc00000u) : pow2(e);
-#pragma unroll
-            for (int c = 0; c < kC; ++c)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    kf[c][0][r] = bf16x2_to_f16x2(kr[c][r].x, factor);
-                    kf[c][0][2 + r] = bf16x2_to_f16x2(kr[c][r].y, factor);
-                    kf[c][1][r] = bf16x2_to_f16x2(kr[c][r].z, factor);
-                    kf[c][1][2 + r] = bf16x2_to_f16x2(kr[c][r].w, factor);
-                }
-            big = 0;
-            const unsigned short* vbits = reinterpret_cast<const unsigned short*>(vs);
-#pragma unroll
-            for (int i = 0; i < 2 * kC; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int d = 16 * i + 8 * (j & 1) + g, tok = 2 * t + 8 * (j >> 1);
-                    const uint32_t lo = tok < have ? vbits[tok * kDim + d] : 0u, hi = tok + 1 < have ? vbits[(tok + 1) * kDim + d] : 0u;
-                    vf[i][j] = lo | hi << 16;
-                    big = __vmaxu2(big, vf[i][j] & 0x7fff7fffu);
-                }
-            e = pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big)));
-            factor = e == 128 ? 0.f : pow2(-e);
-            v_scale = e == 128 ? __uint_as_float(0x7fc00000u) : pow2(e);
-#pragma unroll
-            for (int i = 0; i < 2 * kC; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) vf[i][j] = bf16x2_to_f16x2(vf[i][j], factor);
-        }
-
-        float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < kC; ++c) {
-            mma_f16_16816(s, kf[c][0][0], kf[c][0][1], kf[c][0][2], kf[c][0][3], qf[c][0][0], qf[c][0][1]);
-            mma_f16_16816(s2, kf[c][1][0], kf[c][1][1], kf[c][1][2], kf[c][1][3], qf[c][1][0], qf[c][1][1]);
-        }
+    // scores of block b -> weights, packed as the second operand of O^T = V^T P^T; o scaled to the new maxima. none: no token of it counts
+    auto weigh = [&](const float (&s)[4], const float (&s2)[4], int b, float k_scale, float v_scale, bool none, uint32_t& p0, uint32_t& p1) {
         // tokens g, g + 8 of the block x heads 2 t, 2 t + 1. A scale that is not a number makes the weights of the tokens that are seen none,
         // and nothing else: 1 / scale stays 1.
         const float lv = __log2f(v_scale), inv = v_scale == v_scale ? __fdividef(1.f, v_scale) : 1.f;
         const int tok = b * kKv8Tokens + g;
-        const bool see_lo = tok >= span.begin && tok < span.end, see_hi = tok + 8 >= span.begin && tok + 8 < span.end;
+        const bool see_lo = tok >= span.begin && tok < span.end && !none, see_hi = tok + 8 >= span.begin && tok + 8 < span.end && !none;
         const float c0 = k_scale * qs0, c1 = k_scale * qs1;
         float w[4];
         w[0] = see_lo ? fmaf(s[0] + s2[0], c0, lv) : -INFINITY;
@@ -189,16 +169,102 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(const Kv8Att
 #pragma unroll
             for (int i = 0; i < 2 * kC; ++i) { o[i][0] *= a0; o[i][1] *= a1; o[i][2] *= a0; o[i][3] *= a1; }
         }
-        const uint32_t p0 = movmatrix_trans(pack_f16x2(w[0], w[1])), p1 = movmatrix_trans(pack_f16x2(w[2], w[3]));
+        p0 = movmatrix_trans(pack_f16x2(w[0], w[1]));
+        p1 = movmatrix_trans(pack_f16x2(w[2], w[3]));
+    };
+
+    for (int j = 0; j < n_closed; ++j) {
+        const int st = j % kDepth;
+        bool got = false;
+        for (uint32_t i = 0; i < launch.spins && !got; ++i) got = mbar_try_wait(&full[warp][st], (uint32_t)(j / kDepth) & 1u);
+        if (__any_sync(0xffffffffu, !got)) {
+            failed = true;
+            // copies on their way write this CTA's shared memory: wait for them too
+            for (int k = j; k < min(j + kDepth, n_closed); ++k)
+                for (uint32_t i = 0; i < launch.spins && !mbar_try_wait(&full[warp][k % kDepth], (uint32_t)(k / kDepth) & 1u); ++i) {}
+            if (lane == 0) atomicExch(p.status, 3);
+            break;
+        }
+        const uint32_t at = smem_u32(my_ring + st * kBlockBytes) + lane * 16;
+        const float2 scale = *reinterpret_cast<const float2*>(my_ring + st * kBlockBytes + 32 * kDim);
+        float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 2 * kC; ++i) mma_f16_16816(o[i], vf[i][0], vf[i][1], vf[i][2], vf[i][3], p0, p1);
+        for (int c = 0; c < kC; ++c) {
+            const uint4 kb = lds_16(at + c * 512);
+            uint32_t k[8];
+            kv8_widen(kb.x, &k[0], &k[1]); kv8_widen(kb.z, &k[2], &k[3]);
+            kv8_widen(kb.y, &k[4], &k[5]); kv8_widen(kb.w, &k[6], &k[7]);
+            mma_f16_16816(s, k[0], k[2], k[1], k[3], qf[c][0][0], qf[c][0][1]);
+            mma_f16_16816(s2, k[4], k[6], k[5], k[7], qf[c][1][0], qf[c][1][1]);
+        }
+        uint4 vb[kC];
+#pragma unroll
+        for (int c = 0; c < kC; ++c) vb[c] = lds_16(at + 16 * kDim + c * 512);
+        __syncwarp();
+        const bool none = (bad[(j >> 5) & 1] >> (j & 31)) & 1;
+        if (j + kDepth < n_closed) {              // every lane has read the stage
+            fence_proxy_async();
+            ask(j + kDepth);
+        }
+        uint32_t p0, p1;
+        weigh(s, s2, b0 + j * kWarps, scale.x, scale.y, none, p0, p1);
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            uint32_t v[8];
+            kv8_widen(vb[c].x, &v[0], &v[2]); kv8_widen(vb[c].y, &v[1], &v[3]);
+            kv8_widen(vb[c].z, &v[4], &v[6]); kv8_widen(vb[c].w, &v[5], &v[7]);
+            mma_f16_16816(o[2 * c], v[0], v[1], v[2], v[3], p0, p1);
+            mma_f16_16816(o[2 * c + 1], v[4], v[5], v[6], v[7], p0, p1);
+        }
+    }
+    if (last_open && !failed) {
+        // the block that is not complete: bf16 rows; what lies behind the last token may be anything and counts as zero
+        const int b = b0 + (n_my - 1) * kWarps, have = span.length - b * kKv8Tokens;
+        const __nv_bfloat16* ks = p.open + (long long)span.slot * kv8_open_elems(p.kv_heads, kDim) + kv8_open_at(b, p.kv_heads, kv_head, 0, kDim);
+        uint4 kr[kC][2];
+        uint32_t v[2 * kC][4], big = 0, big_v = 0;
+#pragma unroll
+        for (int c = 0; c < kC; ++c)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) kr[c][r] = g + 8 * r < have ? *reinterpret_cast<const uint4*>(ks + (g + 8 * r) * kDim + 32 * c + 8 * t) : make_uint4(0, 0, 0, 0);
+        const unsigned short* vs = reinterpret_cast<const unsigned short*>(ks + kKv8Tokens * kDim);
+#pragma unroll
+        for (int i = 0; i < 2 * kC; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int d = 16 * i + 8 * (j & 1) + g, tok = 2 * t + 8 * (j >> 1);
+                const uint32_t lo = tok < have ? vs[tok * kDim + d] : 0u, hi = tok + 1 < have ? vs[(tok + 1) * kDim + d] : 0u;
+                v[i][j] = lo | hi << 16;
+                big_v = __vmaxu2(big_v, v[i][j] & 0x7fff7fffu);
+            }
+#pragma unroll
+        for (int c = 0; c < kC; ++c)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) big = __vmaxu2(big, __vmaxu2(abs_bits_max2(kr[c][r].x, kr[c][r].y), abs_bits_max2(kr[c][r].z, kr[c][r].w)));
+        const int e = pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big))), ev = pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big_v)));
+        const float factor = e == 128 ? 0.f : pow2(-e), factor_v = ev == 128 ? 0.f : pow2(-ev);
+        float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            mma_f16_16816(s, bf16x2_to_f16x2(kr[c][0].x, factor), bf16x2_to_f16x2(kr[c][1].x, factor), bf16x2_to_f16x2(kr[c][0].y, factor), bf16x2_to_f16x2(kr[c][1].y, factor),
+                          qf[c][0][0], qf[c][0][1]);
+            mma_f16_16816(s2, bf16x2_to_f16x2(kr[c][0].z, factor), bf16x2_to_f16x2(kr[c][1].z, factor), bf16x2_to_f16x2(kr[c][0].w, factor), bf16x2_to_f16x2(kr[c][1].w, factor),
+                          qf[c][1][0], qf[c][1][1]);
+        }
+        uint32_t p0, p1;
+        weigh(s, s2, b, e == 128 ? __uint_as_float(0x7fc00000u) : pow2(e), ev == 128 ? __uint_as_float(0x7fc00000u) : pow2(ev), false, p0, p1);
+#pragma unroll
+        for (int i = 0; i < 2 * kC; ++i)
+            mma_f16_16816(o[i], bf16x2_to_f16x2(v[i][0], factor_v), bf16x2_to_f16x2(v[i][1], factor_v), bf16x2_to_f16x2(v[i][2], factor_v), bf16x2_to_f16x2(v[i][3], factor_v), p0, p1);
     }
 #pragma unroll
     for (int d = 4; d < 32; d *= 2) {
         l0 += __shfl_xor_sync(0xffffffffu, l0, d);
         l1 += __shfl_xor_sync(0xffffffffu, l1, d);
     }
-    // ---- the warps' parts -----------------------------------------------------------------------------------------------------------------
+    // ---- the warps' parts (their rings are done with) -------------------------------------------------------------------------------------------------
+    __syncthreads();
+    float (*const o_part)[kCols][kDim + 1] = reinterpret_cast<float(*)[kCols][kDim + 1]>(ring);
 #pragma unroll
     for (int i = 0; i < 2 * kC; ++i)
 #pragma unroll
@@ -208,30 +274,62 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_attention_kernel(const Kv8Att
         ml_part[warp][2 * t + 1][0] = m1; ml_part[warp][2 * t + 1][1] = l1;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < cols * (kDim / 2); i += kWarps * 32) {
-        const int h = i / (kDim / 2), d = i % (kDim / 2) * 2;
-        float top = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
+    const bool cluster = kCluster && gridDim.y > 1;
+    for (int i = threadIdx.x; i < cols * (kDim / 4); i += kWarps * 32) {
+        const int h = i / (kDim / 4), d = i % (kDim / 4) * 4;
+        float top = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int v = 0; v < kWarps; ++v) top = fmaxf(top, ml_part[v][h][0]);
-        const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int v = 0; v < kWarps; ++v) {
-            const float f = kv8_exp2(ml_part[v][h][0] - ref);
-            // a warp whose blocks all count for nothing but NaN has no maximum and a sum of NaN
-            const float fl = ml_part[v][h][0] == -INFINITY && ml_part[v][h][1] == 0.f ? 0.f : ml_part[v][h][0] == -INFINITY ? ml_part[v][h][1] : f;
-            l += ml_part[v][h][1] * fl;
-            x += o_part[v][h][d] * fl;
-            y += o_part[v][h][d + 1] * fl;
+            const float f = part_factor(ml_part[v][h][0], ml_part[v][h][1], top);
+            l += ml_part[v][h][1] * f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] += o_part[v][h][d + k] * f;
         }
         const long long at = (long long)row * p.q_heads + head0 + h;
-        if (parts <= 1) {
-            const float r = blocks == 0 ? 0.f : l == 0.f ? 0.f : __fdividef(1.f, l);
-            *reinterpret_cast<uint32_t*>(p.out + at * kDim + d) = pack_bf16x2(x * r, y * r);
+        if (cluster) {
+            float* const mine = own_part + h * (kDim + 4);
+            *reinterpret_cast<float4*>(mine + d) = make_float4(x[0], x[1], x[2], x[3]);
+            if (d == 0) { mine[kDim] = top; mine[kDim + 1] = l; }
+        } else if (kCluster || parts <= 1) {
+            const float r = l == 0.f ? 0.f : __fdividef(1.f, l);
+            *reinterpret_cast<uint2*>(p.out + at * kDim + d) = make_uint2(pack_bf16x2(x[0] * r, x[1] * r), pack_bf16x2(x[2] * r, x[3] * r));
         } else {
             const long long part = at * p.splits + split;
-            *reinterpret_cast<float2*>(p.part_o + part * kDim + d) = make_float2(x, y);
+            *reinterpret_cast<float4*>(p.part_o + part * kDim + d) = make_float4(x[0], x[1], x[2], x[3]);
             if (d == 0) { p.part_ml[2 * part] = top; p.part_ml[2 * part + 1] = l; }
         }
+    }
+    if (cluster) {   // the parts in the order of the ranks, four channels of a head per thread, the work dealt over the ranks
+        const int ranks = gridDim.y, rank = (int)cluster_ctarank();
+        cluster_sync_all();
+        const uint32_t base = smem_u32(own_part);
+        for (int i = threadIdx.x * ranks + rank; i < cols * (kDim / 4); i += kWarps * 32 * ranks) {
+            const int h = i / (kDim / 4), d = i % (kDim / 4) * 4;
+            float4 o4[kMostRanks];
+            float2 ml[kMostRanks];
+            float top = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int r = 0; r < kMostRanks; ++r)
+                if (r < ranks) {
+                    const uint32_t at = map_to_cta(base + (uint32_t)(h * (kDim + 4)) * 4, (uint32_t)r);
+                    o4[r] = ld_dsmem_f4(at + d * 4);
+                    const float4 y = ld_dsmem_f4(at + kDim * 4);
+                    ml[r] = make_float2(y.x, y.y);
+                    top = fmaxf(top, ml[r].x);
+                }
+#pragma unroll
+            for (int r = 0; r < kMostRanks; ++r)
+                if (r < ranks) {
+                    const float f = part_factor(ml[r].x, ml[r].y, top);
+                    l += ml[r].y * f;
+                    x[0] += o4[r].x * f; x[1] += o4[r].y * f; x[2] += o4[r].z * f; x[3] += o4[r].w * f;
+                }
+            const float r = l == 0.f ? 0.f : __fdividef(1.f, l);
+            *reinterpret_cast<uint2*>(p.out + ((long long)row * p.q_heads + head0 + h) * kDim + d) = make_uint2(pack_bf16x2(x[0] * r, x[1] * r), pack_bf16x2(x[2] * r, x[3] * r));
+        }
+        cluster_sync_all();   // the parts stay until every rank has read them
     }
 }
 
@@ -250,9 +348,8 @@ __global__ void __launch_bounds__(kDim / 2) kv8_merge_kernel(const Kv8Attention 
     const float* ml = p.part_ml + 2 * at * p.splits;
     float top = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
     for (int i = 0; i < parts; ++i) top = fmaxf(top, ml[2 * i]);
-    const float ref = top == -INFINITY ? 0.f : top;
     for (int i = 0; i < parts; ++i) {
-        const float f = ml[2 * i] == -INFINITY ? ml[2 * i + 1] : kv8_exp2(ml[2 * i] - ref);   // no maximum: nothing (0) or nothing but NaN
+        const float f = part_factor(ml[2 * i], ml[2 * i + 1], top);
         if (ml[2 * i] == -INFINITY && f == 0.f) continue;                                             // and its part of the output is not there
         const float2 v = *reinterpret_cast<const float2*>(p.part_o + (at * p.splits + i) * kDim + d);
         l += ml[2 * i + 1] * f;
@@ -267,9 +364,22 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 template <int kDim>
 int launch_attention(const Kv8Attention& p, cudaStream_t st) {
-    const int eights = (p.group + kCols - 1) / kCols;
-    const int rc = p.n_tiles ? kv8_prompt_attention(p, kDim, st)
-                             : launch_kernel(kv8_attention_kernel<kDim>, dim3((unsigned)p.splits, (unsigned)(p.kv_heads * eights), (unsigned)p.rows), dim3(kWarps * 32), 0, st, 1, p);
+    const unsigned pairs = (unsigned)(p.kv_heads * ((p.group + kCols - 1) / kCols));
+    constexpr size_t smem = (size_t)kWarps * kDepth * kv8_block_bytes(kDim);
+    static_assert(smem >= sizeof(float) * kWarps * kCols * (kDim + 1), "the warps' parts go where the rings were");
+    static PerDeviceOnce attr_once;
+    if (attr_once.first_time()) {
+        GPTRS_CUDA_OK(cudaFuncSetAttribute(kv8_attention_kernel<kDim, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        GPTRS_CUDA_OK(cudaFuncSetAttribute(kv8_attention_kernel<kDim, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    }
+    AttentionLaunch launch = {p, kSpinLimit, 0};
+    uint32_t limit;
+    prefill_tc_fault(&launch.starve, &limit);
+    if (launch.starve) launch.spins = limit;
+    int rc;
+    if (p.n_tiles) rc = kv8_prompt_attention(p, kDim, st);
+    else if (p.splits <= kMostRanks) return launch_kernel(kv8_attention_kernel<kDim, true>, dim3(pairs, (unsigned)p.splits, (unsigned)p.rows), dim3(kWarps * 32), smem, st, p.splits, launch);
+    else rc = launch_kernel(kv8_attention_kernel<kDim, false>, dim3((unsigned)p.splits, pairs, (unsigned)p.rows), dim3(kWarps * 32), smem, st, 1, launch);
     if (rc || p.splits == 1) return rc;
     return launch_kernel(kv8_merge_kernel<kDim>, dim3((unsigned)p.q_heads, (unsigned)p.rows), dim3(kDim / 2), 0, st, 1, p);
 }
@@ -290,14 +400,17 @@ int gptrs_cuda_kv8_splits(const gptrs_kv8_cache* c, int64_t rows, int64_t n_tile
     }
     const int64_t seen = c->window > 0 ? std::min<int64_t>(max_ctx_len, c->window + kKv8Tokens) : max_ctx_len;
     const int64_t blocks = (seen + kKv8Tokens - 1) / kKv8Tokens;
-    const int64_t ctas = rows * c->kv_heads;
-    const int64_t want = (8 * (int64_t)sm_count() + ctas - 1) / ctas;       // several CTAs per SM
-    const int64_t most = (blocks + 4 * kWarps - 1) / (4 * kWarps);          // a warp takes four blocks at least
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 256));
+    const int64_t pairs = rows * c->kv_heads * ((c->q_heads / c->kv_heads + kCols - 1) / kCols), slots = (int64_t)kCtas * sm_count();
+    // up to eight parts are merged by their cluster in the same launch, as long as a warp has no more than 64 blocks
+    const int64_t ranks = std::max<int64_t>(1, std::min<int64_t>({kMostRanks, (slots + pairs - 1) / pairs, (blocks + kWarps - 1) / kWarps}));
+    if (blocks <= ranks * kWarps * 64) return (int)ranks;
+    // longer ones: parts of 64 to 256 blocks, several for every place of a CTA where there are enough
+    const int64_t part = std::max<int64_t>(64, std::min<int64_t>(256, pairs * blocks / (4 * slots)));
+    return (int)std::min<int64_t>((blocks + part - 1) / part, 65535);
 }
 
 size_t gptrs_cuda_kv8_scratch_bytes(const gptrs_kv8_cache* c, int64_t rows, int64_t n_tiles, int splits) {
-    if (!c || splits <= 1 || rows < 1) return 0;
+    if (!c || splits <= 1 || rows < 1 || (n_tiles == 0 && splits <= kMostRanks)) return 0;
     return (size_t)rows * c->q_heads * splits * (c->dim + 2) * sizeof(float);
 }
 
@@ -315,7 +428,8 @@ int gptrs_cuda_kv8_attention(const gptrs_kv8_cache* c, const gptrs_kv8_attention
     Kv8Attention p = {};
     p.ldq = s->ldq ? s->ldq : width;
     GPTRS_REQUIRE(p.ldq >= width && p.ldq % 8 == 0, "rows of queries overlap, or do not start at multiples of 16 bytes");
-    GPTRS_REQUIRE(s->splits == 1 || (s->d_scratch && s->scratch_bytes >= gptrs_cuda_kv8_scratch_bytes(c, s->rows, s->n_tiles, s->splits)), "scratch is too small");
+    const size_t scratch = gptrs_cuda_kv8_scratch_bytes(c, s->rows, s->n_tiles, s->splits);
+    GPTRS_REQUIRE(scratch == 0 || (s->d_scratch && s->scratch_bytes >= scratch), "scratch is too small");
     if (s->rows == 0) return GPTRS_OK;
     p.q = static_cast<const __nv_bfloat16*>(s->d_q);
     p.pool = static_cast<const unsigned char*>(s->d_pool);

@@ -93,8 +93,8 @@ def test_attention_and_gather_refusals():
     changes = [{n: None} for n in ("d_q", "d_pool", "d_open", "d_page_table", "d_slot", "d_ctx_len", "d_length", "d_out", "d_status")]
     changes += [{n: 4104} for n in ("d_q", "d_pool", "d_open", "d_out")]
     changes += [dict(rows=-1), dict(n_tiles=-1), dict(n_tiles=1), dict(n_tiles=1, d_tile_row=64), dict(max_pages=0), dict(max_pages=1 << 28), dict(n_pages=0), dict(n_slots=0), dict(n_slots=1 << 31),
-                dict(max_ctx_len=-1), dict(max_ctx_len=1 << 31), dict(splits=0), dict(splits=1 << 17), dict(ldq=504), dict(ldq=513), dict(splits=2),
-                dict(splits=2, d_scratch=4096, scratch_bytes=16)]
+                dict(max_ctx_len=-1), dict(max_ctx_len=1 << 31), dict(splits=0), dict(splits=1 << 17), dict(ldq=504), dict(ldq=513), dict(splits=9),
+                dict(splits=9, d_scratch=4096, scratch_bytes=16), dict(splits=2, n_tiles=1, d_tile_row=64, d_tile_rows=64)]
     for change in changes:
         assert _status("gptrs_cuda_kv8_attention", ctypes.byref(a), ctypes.byref(step(**change)), None) == SPEC, change
     assert _status("gptrs_cuda_kv8_attention", ctypes.byref(a), ctypes.byref(step(rows=0)), None) == 0
