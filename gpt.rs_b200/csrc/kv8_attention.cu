@@ -12,6 +12,7 @@
 // memory, its scales included), and merge at the end. Up to eight parts of a row and kv head (of eight of its query heads) are a cluster that merges
 // through distributed shared memory; more go through scratch and a second kernel.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv8_attention.cuh"
 
@@ -138,20 +139,25 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) kv8_attention_kernel(const
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
     bool failed = false;
 
-    // scores of block b -> weights, packed as the second operand of O^T = V^T P^T; o scaled to the new maxima. none: no token of it counts
-    auto weigh = [&](const float (&s)[4], const float (&s2)[4], int b, float k_scale, float v_scale, bool none, uint32_t& p0, uint32_t& p1) {
-        // tokens g, g + 8 of the block x heads 2 t, 2 t + 1. A scale that is not a number makes the weights of the tokens that are seen none,
-        // and nothing else: 1 / scale stays 1.
-        const float lv = __log2f(v_scale), inv = v_scale == v_scale ? __fdividef(1.f, v_scale) : 1.f;
-        const int tok = b * kKv8Tokens + g;
-        const bool see_lo = tok >= span.begin && tok < span.end && !none, see_hi = tok + 8 >= span.begin && tok + 8 < span.end && !none;
-        const float c0 = k_scale * qs0, c1 = k_scale * qs1;
-        float w[4];
-        w[0] = see_lo ? fmaf(s[0] + s2[0], c0, lv) : -INFINITY;
-        w[1] = see_lo ? fmaf(s[1] + s2[1], c1, lv) : -INFINITY;
-        w[2] = see_hi ? fmaf(s[2] + s2[2], c0, lv) : -INFINITY;
-        w[3] = see_hi ? fmaf(s[3] + s2[3], c1, lv) : -INFINITY;
-        float x0 = fmaxf(w[0], w[2]), x1 = fmaxf(w[1], w[3]);
+    // Scores of kCount blocks (the first one's number and the distance to the next) -> weights, packed as the second operand of O^T = V^T P^T; o scaled to the
+    // new maxima. count: tokens of a block with bit i of `none` do not count
+    auto weigh = [&](auto count, const float (*s)[4], int b, const float2* scale, uint32_t none, uint32_t (*packed)[2]) {
+        constexpr int kCount = decltype(count)::value;
+        // tokens g, g + 8 of a block x heads 2 t, 2 t + 1. A scale that is not a number makes the weights of the tokens that are seen none, and
+        // nothing else: 1 / scale stays 1.
+        float w[kCount][4], x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kCount; ++u) {
+            const float lv = __log2f(scale[u].y), c0 = scale[u].x * qs0, c1 = scale[u].x * qs1;
+            const int tok = (b + u * kWarps) * kKv8Tokens + g;
+            const bool counts = !((none >> u) & 1), see_lo = tok >= span.begin && tok < span.end && counts, see_hi = tok + 8 >= span.begin && tok + 8 < span.end && counts;
+            w[u][0] = see_lo ? fmaf(s[u][0], c0, lv) : -INFINITY;
+            w[u][1] = see_lo ? fmaf(s[u][1], c1, lv) : -INFINITY;
+            w[u][2] = see_hi ? fmaf(s[u][2], c0, lv) : -INFINITY;
+            w[u][3] = see_hi ? fmaf(s[u][3], c1, lv) : -INFINITY;
+            x0 = fmaxf(x0, fmaxf(w[u][0], w[u][2]));
+            x1 = fmaxf(x1, fmaxf(w[u][1], w[u][3]));
+        }
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) {
             x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
@@ -161,62 +167,84 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) kv8_attention_kernel(const
         const float u0 = n0 == -INFINITY ? 0.f : n0, u1 = n1 == -INFINITY ? 0.f : n1;   // nothing seen yet (or nothing but NaN)
         const float a0 = kv8_exp2(m0 - u0), a1 = kv8_exp2(m1 - u1);
         m0 = n0; m1 = n1;
-        w[0] = kv8_exp2(w[0] - u0); w[2] = kv8_exp2(w[2] - u0);
-        w[1] = kv8_exp2(w[1] - u1); w[3] = kv8_exp2(w[3] - u1);
-        l0 = l0 * a0 + (w[0] + w[2]) * inv;
-        l1 = l1 * a1 + (w[1] + w[3]) * inv;
+        l0 *= a0;
+        l1 *= a1;
+#pragma unroll
+        for (int u = 0; u < kCount; ++u) {
+            const float inv = scale[u].y == scale[u].y ? __fdividef(1.f, scale[u].y) : 1.f;
+            w[u][0] = kv8_exp2(w[u][0] - u0); w[u][2] = kv8_exp2(w[u][2] - u0);
+            w[u][1] = kv8_exp2(w[u][1] - u1); w[u][3] = kv8_exp2(w[u][3] - u1);
+            l0 = fmaf(w[u][0] + w[u][2], inv, l0);
+            l1 = fmaf(w[u][1] + w[u][3], inv, l1);
+            packed[u][0] = movmatrix_trans(pack_f16x2(w[u][0], w[u][1]));
+            packed[u][1] = movmatrix_trans(pack_f16x2(w[u][2], w[u][3]));
+        }
         if (__any_sync(0xffffffffu, a0 != 1.f || a1 != 1.f)) {
 #pragma unroll
             for (int i = 0; i < 2 * kC; ++i) { o[i][0] *= a0; o[i][1] *= a1; o[i][2] *= a0; o[i][3] *= a1; }
         }
-        p0 = movmatrix_trans(pack_f16x2(w[0], w[1]));
-        p1 = movmatrix_trans(pack_f16x2(w[2], w[3]));
     };
-
-    for (int j = 0; j < n_closed; ++j) {
-        const int st = j % kDepth;
-        bool got = false;
-        for (uint32_t i = 0; i < launch.spins && !got; ++i) got = mbar_try_wait(&full[warp][st], (uint32_t)(j / kDepth) & 1u);
-        if (__any_sync(0xffffffffu, !got)) {
-            failed = true;
-            // copies on their way write this CTA's shared memory: wait for them too
-            for (int k = j; k < min(j + kDepth, n_closed); ++k)
-                for (uint32_t i = 0; i < launch.spins && !mbar_try_wait(&full[warp][k % kDepth], (uint32_t)(k / kDepth) & 1u); ++i) {}
-            if (lane == 0) atomicExch(p.status, 3);
-            break;
-        }
-        const uint32_t at = smem_u32(my_ring + st * kBlockBytes) + lane * 16;
-        const float2 scale = *reinterpret_cast<const float2*>(my_ring + st * kBlockBytes + 32 * kDim);
-        float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+    // kCount blocks of the ring from the j-th on: two at a time share the maxima's exchange between lanes and hide each other's latencies
+    auto visit = [&](auto count, int j) {
+        constexpr int kCount = decltype(count)::value;
+        float s[kCount][4];
+        float2 scale[kCount];
+        uint4 vb[kCount][kC];
+        uint32_t none = 0;
 #pragma unroll
-        for (int c = 0; c < kC; ++c) {
-            const uint4 kb = lds_16(at + c * 512);
-            uint32_t k[8];
-            kv8_widen(kb.x, &k[0], &k[1]); kv8_widen(kb.z, &k[2], &k[3]);
-            kv8_widen(kb.y, &k[4], &k[5]); kv8_widen(kb.w, &k[6], &k[7]);
-            mma_f16_16816(s, k[0], k[2], k[1], k[3], qf[c][0][0], qf[c][0][1]);
-            mma_f16_16816(s2, k[4], k[6], k[5], k[7], qf[c][1][0], qf[c][1][1]);
-        }
-        uint4 vb[kC];
+        for (int u = 0; u < kCount; ++u) {
+            const int st = (j + u) % kDepth;
+            bool got = false;
+            for (uint32_t i = 0; i < launch.spins && !got; ++i) got = mbar_try_wait(&full[warp][st], (uint32_t)((j + u) / kDepth) & 1u);
+            if (__any_sync(0xffffffffu, !got)) {
+                // copies on their way write this CTA's shared memory: wait for them too
+                for (int k = j + u; k < min(j + kDepth, n_closed); ++k)
+                    for (uint32_t i = 0; i < launch.spins && !mbar_try_wait(&full[warp][k % kDepth], (uint32_t)(k / kDepth) & 1u); ++i) {}
+                if (lane == 0) atomicExch(p.status, 3);
+                failed = true;
+                return;
+            }
+            const uint32_t at = smem_u32(my_ring + st * kBlockBytes) + lane * 16;
+            scale[u] = *reinterpret_cast<const float2*>(my_ring + st * kBlockBytes + 32 * kDim);
 #pragma unroll
-        for (int c = 0; c < kC; ++c) vb[c] = lds_16(at + 16 * kDim + c * 512);
+            for (int i = 0; i < 4; ++i) s[u][i] = 0.f;
+#pragma unroll
+            for (int c = 0; c < kC; ++c) {
+                const uint4 kb = lds_16(at + c * 512);
+                uint32_t k[8];
+                kv8_widen(kb.x, &k[0], &k[1]); kv8_widen(kb.z, &k[2], &k[3]);
+                kv8_widen(kb.y, &k[4], &k[5]); kv8_widen(kb.w, &k[6], &k[7]);
+                mma_f16_16816(s[u], k[0], k[2], k[1], k[3], qf[c][0][0], qf[c][0][1]);
+                mma_f16_16816(s[u], k[4], k[6], k[5], k[7], qf[c][1][0], qf[c][1][1]);
+            }
+#pragma unroll
+            for (int c = 0; c < kC; ++c) vb[u][c] = lds_16(at + 16 * kDim + c * 512);
+            none |= ((bad[((j + u) >> 5) & 1] >> ((j + u) & 31)) & 1) << u;
+        }
         __syncwarp();
-        const bool none = (bad[(j >> 5) & 1] >> (j & 31)) & 1;
-        if (j + kDepth < n_closed) {              // every lane has read the stage
+        if (j + kDepth < n_closed) {              // every lane has read the stages
             fence_proxy_async();
             ask(j + kDepth);
+            if (kCount == 2 && j + 1 + kDepth < n_closed) ask(j + 1 + kDepth);
         }
-        uint32_t p0, p1;
-        weigh(s, s2, b0 + j * kWarps, scale.x, scale.y, none, p0, p1);
+        uint32_t packed[kCount][2];
+        weigh(count, s, b0 + j * kWarps, scale, none, packed);
 #pragma unroll
-        for (int c = 0; c < kC; ++c) {
-            uint32_t v[8];
-            kv8_widen(vb[c].x, &v[0], &v[2]); kv8_widen(vb[c].y, &v[1], &v[3]);
-            kv8_widen(vb[c].z, &v[4], &v[6]); kv8_widen(vb[c].w, &v[5], &v[7]);
-            mma_f16_16816(o[2 * c], v[0], v[1], v[2], v[3], p0, p1);
-            mma_f16_16816(o[2 * c + 1], v[4], v[5], v[6], v[7], p0, p1);
-        }
-    }
+        for (int u = 0; u < kCount; ++u)
+#pragma unroll
+            for (int c = 0; c < kC; ++c) {
+                uint32_t v[8];
+                kv8_widen(vb[u][c].x, &v[0], &v[2]); kv8_widen(vb[u][c].y, &v[1], &v[3]);
+                kv8_widen(vb[u][c].z, &v[4], &v[6]); kv8_widen(vb[u][c].w, &v[5], &v[7]);
+                mma_f16_16816(o[2 * c], v[0], v[1], v[2], v[3], packed[u][0], packed[u][1]);
+                mma_f16_16816(o[2 * c + 1], v[4], v[5], v[6], v[7], packed[u][0], packed[u][1]);
+            }
+    };
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    int j = 0;
+    for (; j + 1 < n_closed && !failed; j += 2) visit(Two{}, j);
+    if (j < n_closed && !failed) visit(One{}, j);
     if (last_open && !failed) {
         // the block that is not complete: bf16 rows; what lies behind the last token may be anything and counts as zero
         const int b = b0 + (n_my - 1) * kWarps, have = span.length - b * kKv8Tokens;
@@ -243,19 +271,21 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) kv8_attention_kernel(const
             for (int r = 0; r < 2; ++r) big = __vmaxu2(big, __vmaxu2(abs_bits_max2(kr[c][r].x, kr[c][r].y), abs_bits_max2(kr[c][r].z, kr[c][r].w)));
         const int e = pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big))), ev = pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big_v)));
         const float factor = e == 128 ? 0.f : pow2(-e), factor_v = ev == 128 ? 0.f : pow2(-ev);
-        float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+        float s[1][4] = {};
 #pragma unroll
         for (int c = 0; c < kC; ++c) {
-            mma_f16_16816(s, bf16x2_to_f16x2(kr[c][0].x, factor), bf16x2_to_f16x2(kr[c][1].x, factor), bf16x2_to_f16x2(kr[c][0].y, factor), bf16x2_to_f16x2(kr[c][1].y, factor),
+            mma_f16_16816(s[0], bf16x2_to_f16x2(kr[c][0].x, factor), bf16x2_to_f16x2(kr[c][1].x, factor), bf16x2_to_f16x2(kr[c][0].y, factor), bf16x2_to_f16x2(kr[c][1].y, factor),
                           qf[c][0][0], qf[c][0][1]);
-            mma_f16_16816(s2, bf16x2_to_f16x2(kr[c][0].z, factor), bf16x2_to_f16x2(kr[c][1].z, factor), bf16x2_to_f16x2(kr[c][0].w, factor), bf16x2_to_f16x2(kr[c][1].w, factor),
+            mma_f16_16816(s[0], bf16x2_to_f16x2(kr[c][0].z, factor), bf16x2_to_f16x2(kr[c][1].z, factor), bf16x2_to_f16x2(kr[c][0].w, factor), bf16x2_to_f16x2(kr[c][1].w, factor),
                           qf[c][1][0], qf[c][1][1]);
         }
-        uint32_t p0, p1;
-        weigh(s, s2, b, e == 128 ? __uint_as_float(0x7fc00000u) : pow2(e), ev == 128 ? __uint_as_float(0x7fc00000u) : pow2(ev), false, p0, p1);
+        uint32_t packed[1][2];
+        const float2 scale = make_float2(e == 128 ? __uint_as_float(0x7fc00000u) : pow2(e), ev == 128 ? __uint_as_float(0x7fc00000u) : pow2(ev));
+        weigh(One{}, s, b, &scale, 0, packed);
 #pragma unroll
         for (int i = 0; i < 2 * kC; ++i)
-            mma_f16_16816(o[i], bf16x2_to_f16x2(v[i][0], factor_v), bf16x2_to_f16x2(v[i][1], factor_v), bf16x2_to_f16x2(v[i][2], factor_v), bf16x2_to_f16x2(v[i][3], factor_v), p0, p1);
+            mma_f16_16816(o[i], bf16x2_to_f16x2(v[i][0], factor_v), bf16x2_to_f16x2(v[i][1], factor_v), bf16x2_to_f16x2(v[i][2], factor_v), bf16x2_to_f16x2(v[i][3], factor_v), packed[0][0],
+                          packed[0][1]);
     }
 #pragma unroll
     for (int d = 4; d < 32; d *= 2) {
@@ -333,12 +363,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) kv8_attention_kernel(const
     }
 }
 
-// The parts of a row's head, added up in their order.
+// The parts of a row's head: dim / 4 threads take every kMergers-th part, four channels each, and their sums are added up in order.
+constexpr int kMergers = 8;
 template <int kDim>
-__global__ void __launch_bounds__(kDim / 2) kv8_merge_kernel(const Kv8Attention p) {
+__global__ void __launch_bounds__(kMergers * kDim / 4) kv8_merge_kernel(const Kv8Attention p) {
+    __shared__ __align__(16) float sum[kMergers][kDim], total[kMergers];
     pdl_launch_dependents();
     pdl_wait();
-    const int row = blockIdx.y, d = threadIdx.x * 2;
+    const int row = blockIdx.y, d = threadIdx.x % (kDim / 4) * 4, m = threadIdx.x / (kDim / 4);
     const Kv8Span span = kv8_span(p, row);
     if (span.slot < 0) return;
     int first, blocks, parts = p.splits, per;
@@ -346,18 +378,28 @@ __global__ void __launch_bounds__(kDim / 2) kv8_merge_kernel(const Kv8Attention 
     if (parts <= 1) return;
     const long long at = (long long)row * p.q_heads + blockIdx.x;
     const float* ml = p.part_ml + 2 * at * p.splits;
-    float top = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
+    float top = -INFINITY;
     for (int i = 0; i < parts; ++i) top = fmaxf(top, ml[2 * i]);
-    for (int i = 0; i < parts; ++i) {
+    float l = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = m; i < parts; i += kMergers) {
         const float f = part_factor(ml[2 * i], ml[2 * i + 1], top);
-        if (ml[2 * i] == -INFINITY && f == 0.f) continue;                                             // and its part of the output is not there
-        const float2 v = *reinterpret_cast<const float2*>(p.part_o + (at * p.splits + i) * kDim + d);
+        if (ml[2 * i] == -INFINITY && f == 0.f) continue;                     // and its part of the output is not there
+        const float4 v = *reinterpret_cast<const float4*>(p.part_o + (at * p.splits + i) * kDim + d);
         l += ml[2 * i + 1] * f;
-        x += v.x * f;
-        y += v.y * f;
+        x.x += v.x * f; x.y += v.y * f; x.z += v.z * f; x.w += v.w * f;
+    }
+    *reinterpret_cast<float4*>(&sum[m][d]) = x;
+    if (d == 0) total[m] = l;
+    __syncthreads();
+    if (m > 0) return;
+    for (int i = 1; i < kMergers; ++i) {
+        const float4 v = *reinterpret_cast<const float4*>(&sum[i][d]);
+        x.x += v.x; x.y += v.y; x.z += v.z; x.w += v.w;
+        l += total[i];
     }
     const float r = l == 0.f ? 0.f : __fdividef(1.f, l);
-    *reinterpret_cast<uint32_t*>(p.out + at * kDim + d) = pack_bf16x2(x * r, y * r);
+    *reinterpret_cast<uint2*>(p.out + at * kDim + d) = make_uint2(pack_bf16x2(x.x * r, x.y * r), pack_bf16x2(x.z * r, x.w * r));
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -381,7 +423,12 @@ int launch_attention(const Kv8Attention& p, cudaStream_t st) {
     else if (p.splits <= kMostRanks) return launch_kernel(kv8_attention_kernel<kDim, true>, dim3(pairs, (unsigned)p.splits, (unsigned)p.rows), dim3(kWarps * 32), smem, st, p.splits, launch);
     else rc = launch_kernel(kv8_attention_kernel<kDim, false>, dim3((unsigned)p.splits, pairs, (unsigned)p.rows), dim3(kWarps * 32), smem, st, 1, launch);
     if (rc || p.splits == 1) return rc;
-    return launch_kernel(kv8_merge_kernel<kDim>, dim3((unsigned)p.q_heads, (unsigned)p.rows), dim3(kDim / 2), 0, st, 1, p);
+    // the merge waits for the parts itself (griddepcontrol.wait), so it may be launched ahead of their end
+    const int pdl = g_use_pdl;
+    g_use_pdl = 1;
+    rc = launch_kernel(kv8_merge_kernel<kDim>, dim3((unsigned)p.q_heads, (unsigned)p.rows), dim3(kMergers * kDim / 4), 0, st, 1, p);
+    g_use_pdl = pdl;
+    return rc;
 }
 
 }  // namespace
@@ -401,12 +448,12 @@ int gptrs_cuda_kv8_splits(const gptrs_kv8_cache* c, int64_t rows, int64_t n_tile
     const int64_t seen = c->window > 0 ? std::min<int64_t>(max_ctx_len, c->window + kKv8Tokens) : max_ctx_len;
     const int64_t blocks = (seen + kKv8Tokens - 1) / kKv8Tokens;
     const int64_t pairs = rows * c->kv_heads * ((c->q_heads / c->kv_heads + kCols - 1) / kCols), slots = (int64_t)kCtas * sm_count();
-    // up to eight parts are merged by their cluster in the same launch, as long as a warp has no more than 64 blocks
-    const int64_t ranks = std::max<int64_t>(1, std::min<int64_t>({kMostRanks, (slots + pairs - 1) / pairs, (blocks + kWarps - 1) / kWarps}));
-    if (blocks <= ranks * kWarps * 64) return (int)ranks;
-    // longer ones: parts of 64 to 256 blocks, several for every place of a CTA where there are enough
-    const int64_t part = std::max<int64_t>(64, std::min<int64_t>(256, pairs * blocks / (4 * slots)));
-    return (int)std::min<int64_t>((blocks + part - 1) / part, 65535);
+    // One wave of CTAs. Up to eight parts are merged by their cluster in the same launch, down to a block per warp; more, with a second kernel, pay where a warp
+    // keeps about a dozen blocks (one sequence, 32 / 8 heads of 128, us with 8 / 16 / 32 / 55 parts: 4000 tokens 9.4 / 8.5 / 9.4 / -, 10000 15.7 / 11.7 /
+    // 11.7 / 14.0, 30000 37.4 / 24.0 / 20.7 / 24.0).
+    const int64_t wave = std::max<int64_t>(1, slots / pairs), many = std::min(wave, blocks / (12 * kWarps));
+    if (many > kMostRanks) return (int)std::min<int64_t>(many, 65535);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({wave, kMostRanks, (blocks + kWarps - 1) / kWarps}));
 }
 
 size_t gptrs_cuda_kv8_scratch_bytes(const gptrs_kv8_cache* c, int64_t rows, int64_t n_tiles, int splits) {
