@@ -370,9 +370,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         if (failed && lane == 0) atomicExch(p.status, 3);
     } else if (warp == kMmaWarp) {
         // ================= warp 12: every product =================================================================================================
-        const bool one = elect_one();
-        auto issue_s = [&](int i, int kb) {
-            if (one) {
+        if (elect_one()) {
+            auto wait_one = [&](uint64_t* bar, uint32_t parity) { return !failed && !(failed = !mbar_wait_parked(smem_u32(bar), parity, params.wait_limit)); };
+            auto issue_s = [&](int i, int kb) {
                 const uint64_t a_desc = make_smem_desc(sQ + i * kQBytes), b_desc = make_smem_desc(sK + (kb & 1) * kKBytes);
 #pragma unroll
                 for (int ks = 0; ks < kDim / 16; ++ks) {
@@ -380,27 +380,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                     umma_f16(tmem + (uint32_t)i * kKeys, a_desc + off, b_desc + off, kIdescS, ks > 0 ? 1u : 0u);
                 }
                 umma_commit(&s_full[i]);
+            };
+            if (n_blocks > 0 && wait_one(&k_full[0], 0)) {
+                tc_fence_after();
+                for (int i = 0; i < kTiles; ++i) if (nb_t[i] > 0) issue_s(i, 0);
+                umma_commit(&k_empty[0]);
             }
-            __syncwarp();
-        };
-        if (n_blocks > 0 && wait(&k_full[0], 0)) {
-            tc_fence_after();
-            for (int i = 0; i < kTiles; ++i) if (nb_t[i] > 0) issue_s(i, 0);
-            if (one) umma_commit(&k_empty[0]);
-            __syncwarp();
-        }
-        for (int kb = 0; kb < n_blocks && !failed; ++kb) {
-            const int st = kb & 1;
-            bool v_ready = false, k_ready = false;
-            for (int i = 0; i < kTiles && !failed; ++i) {
-                if (kb < nb_t[i]) {
-                    if (!wait(&p_full[i], (uint32_t)kb & 1u)) break;
-                    if (!v_ready) {
-                        if (!wait(&v_full[st], (uint32_t)(kb >> 1) & 1u)) break;
-                        v_ready = true;
-                    }
-                    tc_fence_after();
-                    if (one) {
+            for (int kb = 0; kb < n_blocks && !failed; ++kb) {
+                const int st = kb & 1;
+                // V of this block and K of the next arrive long before P: waiting for them here keeps these waits out of the way from P to the products
+                if (!wait_one(&v_full[st], (uint32_t)(kb >> 1) & 1u)) break;
+                if (kb + 1 < n_blocks && !wait_one(&k_full[st ^ 1], (uint32_t)((kb + 1) >> 1) & 1u)) break;
+                for (int i = 0; i < kTiles; ++i) {
+                    if (kb < nb_t[i]) {
+                        if (!wait_one(&p_full[i], (uint32_t)kb & 1u)) break;
+                        tc_fence_after();
                         const uint64_t b_desc = make_smem_desc(sV + st * 2 * kVHalf);
 #pragma unroll
                         for (int ks = 0; ks < kKeys / 16; ++ks)
@@ -408,30 +402,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                                          b_desc + (uint64_t)((ks >> 2) * (kVHalf >> 4) + 2 * (ks & 3)), kIdescO, (kb > 0 || ks > 0) ? 1u : 0u);
                         if (kb == nb_t[i] - 1) umma_commit(&o_full[i]);
                     }
-                    __syncwarp();
+                    if (kb + 1 < nb_t[i]) issue_s(i, kb + 1);
                 }
-                if (kb + 1 < nb_t[i]) {
-                    if (!k_ready) {
-                        if (!wait(&k_full[st ^ 1], (uint32_t)((kb + 1) >> 1) & 1u)) break;
-                        k_ready = true;
-                        tc_fence_after();
-                    }
-                    issue_s(i, kb + 1);
-                }
-            }
-            if (failed) break;
-            if (one) {
+                if (failed) break;
                 umma_commit(&v_empty[st]);
                 if (kb + 1 < n_blocks) umma_commit(&k_empty[st ^ 1]);
             }
-            __syncwarp();
+            if (failed) {   // products in flight read shared and tensor memory: let them end before the CTA does
+                umma_commit(&drained);
+                mbar_wait_parked(smem_u32(&drained), 0, params.wait_limit);
+                atomicExch(p.status, 3);
+            }
         }
-        if (failed) {   // products in flight read shared and tensor memory: let them end before the CTA does
-            if (one) umma_commit(&drained);
-            __syncwarp();
-            mbar_wait_parked(smem_u32(&drained), 0, params.wait_limit);
-            if (lane == 0) atomicExch(p.status, 3);
-        }
+        __syncwarp();
     } else {
         // ================= warps 0 - 7: a row per thread =========================================================================================
         const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -447,17 +430,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             const uint32_t sc = sc0 + (uint32_t)(kb % kScaleSlots) * (kPages * 16);
             const int key0 = first_key + kb * kKeys;
             const bool whole = __all_sync(0xffffffffu, begin <= key0 && end >= key0 + kKeys);   // this warp's rows see all of the block
-            uint32_t s[2][32];
+            uint32_t s[64];   // scores of half a block, then their weights
             float sum = 0.f;
-            // Raises the reference of rows whose weights of chunk c came out too large, to about that chunk's maximum: what was computed with the old one
-            // (output, sums, this block's weights so far) is scaled down. Rare behind a sequence's first keys.
-            auto raise = [&](const uint32_t* a, int c, bool over) {
+            auto load = [&](int half) {
+                tmem_ld_32_async(t_s + 64u * half, s);
+                tmem_ld_32_async(t_s + 64u * half + 32u, s + 32);
+                tmem_wait_ld();   // straight behind: nothing may touch the registers before
+            };
+            // Raises the reference of rows whose weights of a half came out too large, to about that half's maximum: what was computed with the old one
+            // (output, sums, the first half's weights) is scaled down. Rare behind a sequence's first keys.
+            auto raise = [&](int half, bool over) {
                 float top = m_run;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float4 x = ld_shared_f4(sc + (2 * c + j / 16) * 16);
-                    const int key = key0 + 32 * c + j;
-                    if (over && key >= begin && key < end) top = fmaxf(top, fmaf(__uint_as_float(a[j]), x.x * q_scale, x.y));
+                for (int j = 0; j < 64; ++j) {
+                    const float4 x = ld_shared_f4(sc + (4 * half + j / 16) * 16);
+                    const int key = key0 + 64 * half + j;
+                    if (over && key >= begin && key < end) top = fmaxf(top, fmaf(__uint_as_float(s[j]), x.x * q_scale, x.y));
                 }
                 // by whole powers of two, so that scaling f16 weights rounds none of them (but the first time, when there are none)
                 const float up = m_run == -1e30f ? 1e30f : floorf(top - m_run), alpha = kv8_exp2(-up);
@@ -476,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
 #pragma unroll 1
-                for (int i = 0; i < c; ++i) {
+                for (int i = 0; i < 2 * half; ++i) {
                     uint32_t r[16];
                     tmem_ld_16(t_s + 16u * i, r);
 #pragma unroll
@@ -487,19 +475,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                     tmem_st_16(t_s + 16u * i, r);
                 }
             };
-            // Weights of the 32 scores of chunk c, packed in the order of V's keys; returns whether a page's sum is too large for f16 weights (or no number)
-            auto weigh = [&](const uint32_t* a, int c, auto all_seen, uint32_t (&packed)[16], float (&ps)[2]) {
+            // Scores of a half -> weights, packed in the order of V's keys, and their share of the sum; returns whether a page's weights add up to more
+            // than keeps each an f16 (or to no number)
+            auto weigh = [&](int half, auto all_seen, float& share) {
                 constexpr bool kWhole = decltype(all_seen)::value;
                 bool fits = true;
+                share = 0.f;
 #pragma unroll
-                for (int pg = 0; pg < 2; ++pg) {
-                    const float4 x = ld_shared_f4(sc + (2 * c + pg) * 16);
+                for (int pg = 0; pg < 4; ++pg) {
+                    const float4 x = ld_shared_f4(sc + (4 * half + pg) * 16);
                     const float cq = x.x * q_scale, b = x.y - m_run;
                     const uint64_t c2 = pair_of(cq, cq), b2 = pair_of(b, b);
                     uint64_t part = 0;
+                    uint32_t packed[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {   // keys 2 i, 2 i + 1
-                        const uint64_t t2 = fma2(pair_of(__uint_as_float(a[16 * pg + 2 * i]), __uint_as_float(a[16 * pg + 2 * i + 1])), c2, b2);
+                        const uint64_t t2 = fma2(pair_of(__uint_as_float(s[16 * pg + 2 * i]), __uint_as_float(s[16 * pg + 2 * i + 1])), c2, b2);
                         float2 w;
                         if (kWhole && (i & 3) == 3) {
                             w = exp2_pair(t2);
@@ -508,44 +499,40 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                             w = make_float2(kv8_exp2(t.x), kv8_exp2(t.y));
                         }
                         if (!kWhole) {
-                            const int key = key0 + 32 * c + 16 * pg + 2 * i;
+                            const int key = key0 + 64 * half + 16 * pg + 2 * i;
                             w.x = key >= begin && key < end ? w.x : 0.f;
                             w.y = key + 1 >= begin && key + 1 < end ? w.y : 0.f;
                         }
                         part = add2(part, pair_of(w.x, w.y));
-                        packed[8 * pg + (i < 4 ? 2 * i : 2 * (i - 4) + 1)] = pack_f16x2(w.x, w.y);
+                        packed[i < 4 ? 2 * i : 2 * (i - 4) + 1] = pack_f16x2(w.x, w.y);
                     }
-                    const float2 half = split(part);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s[8 * pg + i] = packed[i];   // the scores of this and earlier pages are consumed
+                    const float2 both = split(part);
+                    const float page_sum = both.x + both.y;
                     // 1 / s_V that is not a number belongs to a page that is none: of rows that see all of it. Others find that in their weights.
-                    const float page_sum = half.x + half.y;
-                    ps[pg] = page_sum * (kWhole || x.z == x.z ? x.z : 1.f);
+                    share = fmaf(page_sum, kWhole || x.z == x.z ? x.z : 1.f, share);
                     fits &= page_sum <= kLargestSum;
                 }
                 return !fits;
             };
-            auto chunk = [&](const uint32_t* a, int c, auto all_seen) {
-                uint32_t packed[16];
-                float ps[2];
-                bool over = weigh(a, c, all_seen, packed, ps);
-                if (__any_sync(0xffffffffu, over)) {
-                    raise(a, c, over);
-                    weigh(a, c, std::false_type{}, packed, ps);
-                }
-                sum += ps[0] + ps[1];
-                tmem_st_16(t_s + 16u * c, packed);
-            };
-            auto all_chunks = [&](auto all_seen) {
+            auto both_halves = [&](auto all_seen) {
 #pragma unroll
-                for (int c = 0; c < kKeys / 32; c += 2) {   // weights go where scores have been read
-                    tmem_ld_32_async(t_s + 32u * c, s[0]);
-                    tmem_ld_32_async(t_s + 32u * (c + 1), s[1]);
-                    tmem_wait_ld();                         // straight behind: nothing may touch the registers before
-                    chunk(s[0], c, all_seen);
-                    chunk(s[1], c + 1, all_seen);
+                for (int half = 0; half < 2; ++half) {
+                    float share;
+                    load(half);
+                    const bool over = weigh(half, all_seen, share);
+                    if (__any_sync(0xffffffffu, over)) {
+                        load(half);   // the weights have not been stored over the scores yet
+                        raise(half, over);
+                        weigh(half, std::false_type{}, share);
+                    }
+                    sum += share;
+                    tmem_st_32(t_s + 32u * half, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
                 }
             };
-            if (whole) all_chunks(std::true_type{});
-            else all_chunks(std::false_type{});
+            if (whole) both_halves(std::true_type{});
+            else both_halves(std::false_type{});
             l_run += sum;
             asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
             tc_fence_before();
