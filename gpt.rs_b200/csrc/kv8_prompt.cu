@@ -32,7 +32,10 @@ constexpr int kTiles = 2;
 constexpr int kSoftmaxThreads = kTiles * kRows;
 constexpr int kLoadWarps = 4;
 constexpr int kLoadWarp = kSoftmaxThreads / 32, kMmaWarp = kLoadWarp + kLoadWarps;
-constexpr int kThreads = kSoftmaxThreads + kLoadWarps * 32 + 32;
+constexpr int kThreads = kSoftmaxThreads + kLoadWarps * 32 + 128;   // the MMA warp and three that only make its group whole
+// Registers of a thread at launch, and what the groups of four warps make of them: the shares add up to what the block has, so every request ends.
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 160, kLoadRegs = kLaunchRegs, kMmaRegs = 64;
+static_assert(kThreads == 512 && 2 * kSoftmaxRegs + kLoadRegs + kMmaRegs <= 4 * kLaunchRegs, "more registers than the block is launched with");
 constexpr int kKeys = 128;                 // of a block
 constexpr int kPages = kKeys / kKv8Tokens;
 constexpr int kHalfBytes = 128 * 128;      // 128 rows x 64 f16
@@ -113,7 +116,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     constexpr uint32_t kIdescS = kIdesc | ((uint32_t)(kKeys >> 3) << 17), kIdescO = kIdesc | ((uint32_t)(kDim >> 3) << 17);
 
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[kTiles], p_full[kTiles], o_full[kTiles], drained;
+    __shared__ __align__(8) uint64_t k_first, full[2], empty[2], s_full[kTiles], p_full[kTiles][2], o_half[kTiles], o_full[kTiles], drained;
     __shared__ uint32_t tmem_holder;
     __shared__ int s_begin[kSoftmaxThreads / 32], s_end[kSoftmaxThreads / 32];
     __shared__ __align__(16) float scales[kScaleSlots][kPages][4];   // s_K scale log2 e, log2 s_V, 1 / s_V
@@ -136,8 +139,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     const int slot = p.slot[row0];
 
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) { mbar_init(&k_full[i], kLoadWarps); mbar_init(&v_full[i], kLoadWarps); mbar_init(&k_empty[i], 1); mbar_init(&v_empty[i], 1); }
-        for (int i = 0; i < kTiles; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], kRows); mbar_init(&o_full[i], 1); }
+        mbar_init(&k_first, kLoadWarps);
+        for (int i = 0; i < 2; ++i) { mbar_init(&full[i], kLoadWarps); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < kTiles; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i][0], kRows); mbar_init(&p_full[i][1], kRows); mbar_init(&o_half[i], 1); mbar_init(&o_full[i], 1); }
         mbar_init(&drained, 1);
         mbar_fence_init();
     }
@@ -210,7 +214,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         return !failed;
     };
 
-    if (warp >= kLoadWarp && warp < kMmaWarp) {
+    if (warp > kMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kMmaRegs));
+    } else if (warp >= kLoadWarp && warp < kMmaWarp) {
         // ================= warps 8 - 11: pages 2 w, 2 w + 1 of every block ===================================================================
         const int w = warp - kLoadWarp;
         const int length = p.length[slot < 0 ? 0 : slot];
@@ -339,37 +345,45 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 }
             }
         };
+        // stage kb & 1: V of block kb and K of block kb + 1, which the products of one round read; K of block 0 by itself
         Page pages[2], next[2];
         int numbers[2];
+        auto store_keys = [&](const Page (&pg)[2], int kb) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) store_k(pg[j], j, kb, sK + (kb & 1) * kKBytes);
+        };
         if (n_blocks > 0) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) pages[j] = find(0, j, number(0, j));
             load_k(pages);
+            load_v(pages);
 #pragma unroll
             for (int j = 0; j < 2; ++j) numbers[j] = number(1, j);
+            store_keys(pages, 0);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0 && !params.starve) mbar_arrive(&k_first);
         }
         for (int kb = 0; kb < n_blocks; ++kb) {
             const int st = kb & 1;
-            load_v(pages);
-            if (kb >= 2 && !wait(&k_empty[st], (uint32_t)((kb - 2) >> 1) & 1u)) break;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) store_k(pages[j], j, kb, sK + st * kKBytes);
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0 && !(params.starve && kb == 0)) mbar_arrive(&k_full[st]);
 #pragma unroll
             for (int j = 0; j < 2; ++j) { next[j] = find(kb + 1, j, numbers[j]); numbers[j] = number(kb + 2, j); }
             if (kb + 1 < n_blocks) load_k(next);
-            if (kb >= 2 && !wait(&v_empty[st], (uint32_t)((kb - 2) >> 1) & 1u)) break;
+            if (kb >= 2 && !wait(&empty[st], (uint32_t)((kb - 2) >> 1) & 1u)) break;
 #pragma unroll
             for (int j = 0; j < 2; ++j) { store_v(pages[j], j, sV + st * 2 * kVHalf); pages[j] = next[j]; }
+            if (kb + 1 < n_blocks) {
+                load_v(pages);
+                store_keys(pages, kb + 1);
+            }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&v_full[st]);
+            if (lane == 0) mbar_arrive(&full[st]);
         }
         if (failed && lane == 0) atomicExch(p.status, 3);
     } else if (warp == kMmaWarp) {
         // ================= warp 12: every product =================================================================================================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kMmaRegs));
         if (elect_one()) {
             auto wait_one = [&](uint64_t* bar, uint32_t parity) { return !failed && !(failed = !mbar_wait_parked(smem_u32(bar), parity, params.wait_limit)); };
             auto issue_s = [&](int i, int kb) {
@@ -381,32 +395,32 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 }
                 umma_commit(&s_full[i]);
             };
-            if (n_blocks > 0 && wait_one(&k_full[0], 0)) {
+            if (n_blocks > 0 && wait_one(&k_first, 0)) {
                 tc_fence_after();
                 for (int i = 0; i < kTiles; ++i) if (nb_t[i] > 0) issue_s(i, 0);
-                umma_commit(&k_empty[0]);
             }
             for (int kb = 0; kb < n_blocks && !failed; ++kb) {
                 const int st = kb & 1;
-                // V of this block and K of the next arrive long before P: waiting for them here keeps these waits out of the way from P to the products
-                if (!wait_one(&v_full[st], (uint32_t)(kb >> 1) & 1u)) break;
-                if (kb + 1 < n_blocks && !wait_one(&k_full[st ^ 1], (uint32_t)((kb + 1) >> 1) & 1u)) break;
+                if (!wait_one(&full[st], (uint32_t)(kb >> 1) & 1u)) break;
                 for (int i = 0; i < kTiles; ++i) {
                     if (kb < nb_t[i]) {
-                        if (!wait_one(&p_full[i], (uint32_t)kb & 1u)) break;
-                        tc_fence_after();
                         const uint64_t b_desc = make_smem_desc(sV + st * 2 * kVHalf);
 #pragma unroll
-                        for (int ks = 0; ks < kKeys / 16; ++ks)
-                            umma_bf16_ts(tmem + kOCol + (uint32_t)i * kDim, tmem + (uint32_t)i * kKeys + 8u * ks,
-                                         b_desc + (uint64_t)((ks >> 2) * (kVHalf >> 4) + 2 * (ks & 3)), kIdescO, (kb > 0 || ks > 0) ? 1u : 0u);
+                        for (int h = 0; h < 2; ++h) {   // 64 keys at a time, as their weights arrive
+                            if (!wait_one(&p_full[i][h], (uint32_t)kb & 1u)) break;
+                            tc_fence_after();
+#pragma unroll
+                            for (int ks = 0; ks < kKeys / 32; ++ks)
+                                umma_bf16_ts(tmem + kOCol + (uint32_t)i * kDim, tmem + (uint32_t)i * kKeys + 32u * h + 8u * ks, b_desc + (uint64_t)(h * (kVHalf >> 4) + 2 * ks), kIdescO,
+                                             (kb > 0 || h > 0 || ks > 0) ? 1u : 0u);
+                            if (h == 0) umma_commit(&o_half[i]);
+                        }
+                        if (failed) break;
                         if (kb == nb_t[i] - 1) umma_commit(&o_full[i]);
                     }
                     if (kb + 1 < nb_t[i]) issue_s(i, kb + 1);
                 }
-                if (failed) break;
-                umma_commit(&v_empty[st]);
-                if (kb + 1 < n_blocks) umma_commit(&k_empty[st ^ 1]);
+                if (!failed) umma_commit(&empty[st]);
             }
             if (failed) {   // products in flight read shared and tensor memory: let them end before the CTA does
                 umma_commit(&drained);
@@ -420,7 +434,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t t_s = t_lane + (uint32_t)ti * kKeys, t_o = t_lane + kOCol + (uint32_t)ti * kDim;
         const int my_blocks = nb_t[ti];
-        const uint32_t s_bar = smem_u32(&s_full[ti]), p_bar = smem_u32(&p_full[ti]), sc0 = smem_u32(&scales[0][0][0]);
+        const uint32_t s_bar = smem_u32(&s_full[ti]), p_bar = smem_u32(&p_full[ti][0]), sc0 = smem_u32(&scales[0][0][0]);
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
         float m_run = -1e30f, l_run = 0.f;
         for (int kb = 0; kb < my_blocks; ++kb) {
             if (!mbar_wait_parked(s_bar, (uint32_t)kb & 1u, params.wait_limit)) failed = true;
@@ -431,14 +446,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             const int key0 = first_key + kb * kKeys;
             const bool whole = __all_sync(0xffffffffu, begin <= key0 && end >= key0 + kKeys);   // this warp's rows see all of the block
             uint32_t s[64];   // scores of half a block, then their weights
-            float sum = 0.f;
             auto load = [&](int half) {
                 tmem_ld_32_async(t_s + 64u * half, s);
                 tmem_ld_32_async(t_s + 64u * half + 32u, s + 32);
                 tmem_wait_ld();   // straight behind: nothing may touch the registers before
             };
             // Raises the reference of rows whose weights of a half came out too large, to about that half's maximum: what was computed with the old one
-            // (output, sums, the first half's weights) is scaled down. Rare behind a sequence's first keys.
+            // (output and sum) is scaled down. Rare behind a sequence's first keys.
             auto raise = [&](int half, bool over) {
                 float top = m_run;
 #pragma unroll
@@ -447,32 +461,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                     const int key = key0 + 64 * half + j;
                     if (over && key >= begin && key < end) top = fmaxf(top, fmaf(__uint_as_float(s[j]), x.x * q_scale, x.y));
                 }
-                // by whole powers of two, so that scaling f16 weights rounds none of them (but the first time, when there are none)
-                const float up = m_run == -1e30f ? 1e30f : floorf(top - m_run), alpha = kv8_exp2(-up);
-                m_run = m_run == -1e30f ? top : m_run + up;
+                const float alpha = kv8_exp2(m_run - top);   // (0 the first time)
+                m_run = top;
                 l_run *= alpha;
-                sum *= alpha;
-                if (kb > 0) {   // the tile's previous product with V is complete: it was issued before this S
-#pragma unroll 1
-                    for (int i = 0; i < kDim / 16; ++i) {
-                        uint32_t r[16];
-                        tmem_ld_16(t_o + 16u * i, r);
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
-                        tmem_st_16(t_o + 16u * i, r);
-                    }
+                if (kb == 0 && half == 0) return;
+                // the tile's products with V so far are complete: those of earlier blocks were issued before these scores, the first half's is waited for
+                if (half == 1) {
+                    if (!mbar_wait_parked(smem_u32(&o_half[ti]), (uint32_t)kb & 1u, params.wait_limit)) failed = true;
+                    failed = __any_sync(0xffffffffu, failed);
+                    tc_fence_after();
                 }
-                asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
 #pragma unroll 1
-                for (int i = 0; i < 2 * half; ++i) {
+                for (int i = 0; i < kDim / 16; ++i) {
                     uint32_t r[16];
-                    tmem_ld_16(t_s + 16u * i, r);
+                    tmem_ld_16(t_o + 16u * i, r);
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&r[k]));   // alpha itself may be less than any f16
-                        r[k] = pack_f16x2(w.x * alpha, w.y * alpha);
-                    }
-                    tmem_st_16(t_s + 16u * i, r);
+                    for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
+                    tmem_st_16(t_o + 16u * i, r);
                 }
             };
             // Scores of a half -> weights, packed in the order of V's keys, and their share of the sum; returns whether a page's weights add up to more
@@ -492,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                     for (int i = 0; i < 8; ++i) {   // keys 2 i, 2 i + 1
                         const uint64_t t2 = fma2(pair_of(__uint_as_float(s[16 * pg + 2 * i]), __uint_as_float(s[16 * pg + 2 * i + 1])), c2, b2);
                         float2 w;
-                        if (kWhole && (i & 3) == 3) {
+                        if (kWhole && (i & 7) == 7) {
                             w = exp2_pair(t2);
                         } else {
                             const float2 t = split(t2);
@@ -516,27 +521,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 }
                 return !fits;
             };
-            auto both_halves = [&](auto all_seen) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    float share;
-                    load(half);
-                    const bool over = weigh(half, all_seen, share);
-                    if (__any_sync(0xffffffffu, over)) {
-                        load(half);   // the weights have not been stored over the scores yet
-                        raise(half, over);
-                        weigh(half, std::false_type{}, share);
-                    }
-                    sum += share;
-                    tmem_st_32(t_s + 32u * half, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+            bool exact = !whole;   // which of the two ways
+#pragma unroll 1   // (the code of a half is long: copies of it do not stay in the instruction cache)
+            for (int half = 0; half < 2; ++half) {
+                float share;
+                load(half);
+#pragma unroll 1
+                for (int round = 0; ; ++round) {
+                    const bool over = exact ? weigh(half, std::false_type{}, share) : weigh(half, std::true_type{}, share);
+                    if (round == 1 || !__any_sync(0xffffffffu, over)) break;
+                    load(half);   // the weights have not been stored over the scores yet
+                    raise(half, over);
+                    exact = true;
                 }
-            };
-            if (whole) both_halves(std::true_type{});
-            else both_halves(std::false_type{});
-            l_run += sum;
-            asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-            tc_fence_before();
-            mbar_arrive_addr(p_bar);
+                l_run += share;
+                tmem_st_32(t_s + 32u * half, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+                asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+                tc_fence_before();
+                mbar_arrive_addr(p_bar + 8u * half);
+            }
         }
         // ---- the output, or this split's part of it --------------------------------------------------------------------------------------------
         if (my_blocks > 0 && !failed) {
@@ -593,6 +596,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 
 template <int kDim>
 int launch_prompt(const PromptParams& p, cudaStream_t stream) {
+    // a kernel compiled for fewer registers than its groups ask for would wait for them without end
+    static const int regs = [] {
+        cudaFuncAttributes attr;
+        return cudaFuncGetAttributes(&attr, kv8_prompt_kernel<kDim>) == cudaSuccess ? attr.numRegs : 0;
+    }();
+    if (regs != kLaunchRegs) return fail(GPTRS_EXECUTION, "kv8_prompt_kernel has " + std::to_string(regs) + " registers a thread, not those that its warps share out");
     static PerDeviceOnce attr_once;
     if (attr_once.first_time())
         GPTRS_CUDA_OK(cudaFuncSetAttribute(kv8_prompt_kernel<kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<kDim>()));
