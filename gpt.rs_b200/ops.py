@@ -691,7 +691,7 @@ PAIRS_HALVES, PAIRS_NEIGHBOURS = 0, 1
 
 
 class _Step:
-    """A prepared call: keeps its tensors alive and checks that they are on the current device."""
+    """A prepared call: keeps its tensors alive, checks that they are on the current device, and launches on the current stream."""
 
     def _hold(self, **tensors):
         self._tensors = {k: t for k, t in tensors.items() if t is not None}
@@ -700,12 +700,19 @@ class _Step:
             raise ValueError(f"expected CUDA tensors of one device, got {sorted(map(str, devices))}")
         self._device = next(iter(devices)).index
 
-    def _run(self, fn, *args):
-        if torch.cuda.current_device() != self._device:
-            raise ValueError(f"the tensors are on cuda:{self._device}, the current device is cuda:{torch.cuda.current_device()}")
-        status = fn(*args, _stream())
+    def _bind(self, fn, args, result):
+        """The arguments are converted once: a step of a few microseconds on the GPU has no time for it in every call."""
+        self._fn, self._result = fn, result
+        self._args = tuple(a if t is ctypes.c_void_p and not isinstance(a, (int, type(None))) else t(a) for t, a in zip(fn.argtypes, args))
+
+    def __call__(self):
+        device = torch._C._cuda_getDevice()
+        if device != self._device:
+            raise ValueError(f"the tensors are on cuda:{self._device}, the current device is cuda:{device}")
+        status = self._fn(*self._args, torch._C._cuda_getCurrentRawStream(device))
         if status:
             check(status)
+        return self._result
 
 
 def _need(t, name, dtype, *shape):
@@ -768,12 +775,8 @@ class QkNormRope(_Step):
             raise ValueError("out has another number of rows")
         positions = None if positions is None else _need(positions, "positions", torch.int32, self.rows)
         self._hold(qkv=qkv, out=self.out, positions=positions, status=self.status, **rotation.tensors)
-        self._args = (ctypes.byref(r), src, _dt(qkv), ld_in, None if positions is None else positions.data_ptr(), dst, ld_out, self.status.data_ptr(), self.rows)
-        self._fn = lib().gptrs_cuda_qk_norm_rope
-
-    def __call__(self):
-        self._run(self._fn, *self._args)
-        return self.out
+        self._bind(lib().gptrs_cuda_qk_norm_rope, (ctypes.byref(r), src, _dt(qkv), ld_in, None if positions is None else positions.data_ptr(), dst, ld_out,
+                                                  self.status.data_ptr(), self.rows), self.out)
 
 
 def qk_norm_rope(rotation, qkv, positions, out=None, status=None):
@@ -822,12 +825,7 @@ class Kv8Append(_Step):
             s.rotation = ctypes.addressof(rotation.struct)
         self._hold(qkv=qkv, positions=positions, slot=slot, run_first=run_first, run_last=run_last, page_table=page_table, pool=pool, open_rows=open_rows, q=self.q,
                    status=self.status, **(rotation.tensors if rotation is not None else {}))
-        self._args = (ctypes.byref(a), ctypes.byref(s))
-        self._fn = lib().gptrs_cuda_kv8_append
-
-    def __call__(self):
-        self._run(self._fn, *self._args)
-        return self.q
+        self._bind(lib().gptrs_cuda_kv8_append, (ctypes.byref(a), ctypes.byref(s)), self.q)
 
 
 def kv8_append(*args, **kw):
@@ -847,13 +845,9 @@ class Kv8Gather(_Step):
         _need(positions, "positions", torch.int32, rows)
         _need(lengths, "lengths", torch.int32, n_slots)
         self._hold(pool=pool, open_rows=open_rows, page_table=page_table, slot=slot, positions=positions, lengths=lengths, k=self.k, v=self.v, status=self.status)
-        self._args = (ctypes.byref(a), pool.data_ptr(), n_pages, open_rows.data_ptr(), n_slots, page_table.data_ptr(), page_table.shape[1], slot.data_ptr(),
-                      positions.data_ptr(), lengths.data_ptr(), _dt(self.k), self.k.data_ptr(), self.v.data_ptr(), self.status.data_ptr(), rows)
-        self._fn = lib().gptrs_cuda_kv8_gather
-
-    def __call__(self):
-        self._run(self._fn, *self._args)
-        return self.k, self.v
+        self._bind(lib().gptrs_cuda_kv8_gather, (ctypes.byref(a), pool.data_ptr(), n_pages, open_rows.data_ptr(), n_slots, page_table.data_ptr(), page_table.shape[1],
+                                                slot.data_ptr(), positions.data_ptr(), lengths.data_ptr(), _dt(self.k), self.k.data_ptr(), self.v.data_ptr(),
+                                                self.status.data_ptr(), rows), (self.k, self.v))
 
 
 def kv8_gather(*args, **kw):
@@ -900,12 +894,7 @@ class Kv8Attention(_Step):
         s.d_out, s.d_status, s.rows = self.out.data_ptr(), self.status.data_ptr(), rows
         self._hold(q=q, pool=pool, open_rows=open_rows, page_table=page_table, slot=slot, ctx_len=ctx_len, lengths=lengths, tile_row=tile_row, tile_rows=tile_rows,
                    scratch=scratch, out=self.out, status=self.status)
-        self._args = (ctypes.byref(a), ctypes.byref(s))
-        self._fn = lib().gptrs_cuda_kv8_attention
-
-    def __call__(self):
-        self._run(self._fn, *self._args)
-        return self.out
+        self._bind(lib().gptrs_cuda_kv8_attention, (ctypes.byref(a), ctypes.byref(s)), self.out)
 
 
 def kv8_attention(*args, **kw):
