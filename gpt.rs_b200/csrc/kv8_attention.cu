@@ -45,6 +45,42 @@ __device__ __forceinline__ void parts_of(const Kv8Attention& p, const Kv8Span& s
     *parts = (*blocks + *per - 1) / *per;
 }
 
+// The same for few parts: dim / 4 threads have a row's head to themselves.
+template <int kDim>
+__global__ void __launch_bounds__(256) kv8_merge_few_kernel(const Kv8Attention p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const long long item = (long long)blockIdx.x * (256 / (kDim / 4)) + threadIdx.x / (kDim / 4);
+    const int row = kv8_row(p, (int)(item / p.q_heads)), d = threadIdx.x % (kDim / 4) * 4;
+    if (row < 0) return;
+    const long long at = (long long)row * p.q_heads + item % p.q_heads;
+    const Kv8Span span = kv8_span(p, row);
+    if (span.slot < 0) return;
+    int first, blocks, parts = p.splits, per;
+    if (p.n_tiles == 0) parts_of(p, span, &first, &blocks, &parts, &per);
+    if (parts <= 1) return;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + at * p.splits;
+    float2 x[kMostRanks];
+    float4 v[kMostRanks];
+    float top = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMostRanks; ++i)
+        if (i < parts) { x[i] = ml[i]; top = fmaxf(top, x[i].x); }
+#pragma unroll
+    for (int i = 0; i < kMostRanks; ++i)   // a part that has seen nothing has no output
+        v[i] = i < parts && !(x[i].x == -INFINITY && x[i].y == 0.f) ? *reinterpret_cast<const float4*>(p.part_o + (at * p.splits + i) * kDim + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kMostRanks; ++i)
+        if (i < parts) {
+            const float f = part_factor(x[i].x, x[i].y, top);
+            l += x[i].y * f;
+            o.x += v[i].x * f; o.y += v[i].y * f; o.z += v[i].z * f; o.w += v[i].w * f;
+        }
+    const float r = l == 0.f ? 0.f : __fdividef(1.f, l);
+    *reinterpret_cast<uint2*>(p.out + at * kDim + d) = make_uint2(pack_bf16x2(o.x * r, o.y * r), pack_bf16x2(o.z * r, o.w * r));
+}
+
 struct AttentionLaunch {
     Kv8Attention a;
     uint32_t spins;               // polls of a bounded wait
@@ -65,7 +101,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) kv8_attention_kernel(const
     const int split = kCluster ? blockIdx.y : blockIdx.x, pair = kCluster ? blockIdx.x : blockIdx.y, eights = (p.group + kCols - 1) / kCols;
     const int kv_head = pair / eights, head0 = kv_head * p.group + (pair % eights) * kCols;
     const int cols = min(kCols, p.group - (pair % eights) * kCols);
-    const int row = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     if (lane == 0) {
         for (int i = 0; i < kDepth; ++i) mbar_init(&full[warp][i], 1);
         mbar_fence_init();
@@ -73,6 +109,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) kv8_attention_kernel(const
     __syncwarp();
     pdl_launch_dependents();
     pdl_wait();
+    const int row = kv8_row(p, blockIdx.z);
+    if (row < 0) return;                          // (the whole cluster)
     // the query, on its way while the lengths are
     const __nv_bfloat16* const q_src = p.q + row * p.ldq + (long long)(head0 + min(g, cols - 1)) * kDim + 8 * t;
     uint4 raw[kC];
@@ -370,13 +408,14 @@ __global__ void __launch_bounds__(kMergers * kDim / 4) kv8_merge_kernel(const Kv
     __shared__ __align__(16) float sum[kMergers][kDim], total[kMergers];
     pdl_launch_dependents();
     pdl_wait();
-    const int row = blockIdx.y, d = threadIdx.x % (kDim / 4) * 4, m = threadIdx.x / (kDim / 4);
+    const int row = kv8_row(p, blockIdx.x), d = threadIdx.x % (kDim / 4) * 4, m = threadIdx.x / (kDim / 4);
+    if (row < 0) return;
     const Kv8Span span = kv8_span(p, row);
     if (span.slot < 0) return;
     int first, blocks, parts = p.splits, per;
     if (p.n_tiles == 0) parts_of(p, span, &first, &blocks, &parts, &per);   // of a tile every part has its sum
     if (parts <= 1) return;
-    const long long at = (long long)row * p.q_heads + blockIdx.x;
+    const long long at = (long long)row * p.q_heads + blockIdx.y;
     const float* ml = p.part_ml + 2 * at * p.splits;
     float top = -INFINITY;
     for (int i = 0; i < parts; ++i) top = fmaxf(top, ml[2 * i]);
@@ -402,6 +441,17 @@ __global__ void __launch_bounds__(kMergers * kDim / 4) kv8_merge_kernel(const Kv
     *reinterpret_cast<uint2*>(p.out + at * kDim + d) = make_uint2(pack_bf16x2(x.x * r, x.y * r), pack_bf16x2(x.z * r, x.w * r));
 }
 
+// Whether the rows of tiles are faster one by one than a tile at a time, from estimates in us. One by one: a wave of CTAs (row x kv head) takes 3 us and what its
+// longest row does; a tile takes about 12 us, and 2.3 for every 128 keys. (One prompt, 32 / 8 heads of 128: 16 tokens 4.0 against 12.2 us, 128 12.7 against
+// 16.9, 256 26 against 19.6; 8 / 1 heads: 512 tokens 13.6 against 24, 2048 86 against 52.)
+bool rows_one_by_one(const gptrs_kv8_cache& c, int64_t rows, int64_t n_tiles, int64_t max_len) {
+    const int64_t seen = c.window > 0 ? std::min<int64_t>(max_len, c.window) : max_len, pairs = c.kv_heads * ((c.q_heads / c.kv_heads + kCols - 1) / kCols);
+    if (n_tiles * c.tile_tokens > 65535) return false;
+    const double by_row = (double)((rows * pairs + kCtas * sm_count() - 1) / (kCtas * sm_count())) * (3. + seen / 2 / 64. * .9);
+    const double by_tile = 12. + (double)((n_tiles * c.kv_heads + sm_count() - 1) / sm_count()) * (seen / 128.) * 2.3;
+    return by_row < by_tile;
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <int kDim>
@@ -419,14 +469,21 @@ int launch_attention(const Kv8Attention& p, cudaStream_t st) {
     prefill_tc_fault(&launch.starve, &limit);
     if (launch.starve) launch.spins = limit;
     int rc;
-    if (p.n_tiles) rc = kv8_prompt_attention(p, kDim, st);
-    else if (p.splits <= kMostRanks) return launch_kernel(kv8_attention_kernel<kDim, true>, dim3(pairs, (unsigned)p.splits, (unsigned)p.rows), dim3(kWarps * 32), smem, st, p.splits, launch);
+    const int64_t rows = p.n_tiles ? (int64_t)p.n_tiles * p.tile_tokens : p.rows;   // that kv8_row goes through
+    if (p.n_tiles && !p.one_by_one) rc = kv8_prompt_attention(p, kDim, st);
+    else if (p.splits <= kMostRanks)
+        return launch_kernel(kv8_attention_kernel<kDim, true>, dim3(pairs, (unsigned)p.splits, (unsigned)rows), dim3(kWarps * 32), smem, st,
+                             p.splits, launch);
     else rc = launch_kernel(kv8_attention_kernel<kDim, false>, dim3((unsigned)p.splits, pairs, (unsigned)p.rows), dim3(kWarps * 32), smem, st, 1, launch);
     if (rc || p.splits == 1) return rc;
     // the merge waits for the parts itself (griddepcontrol.wait), so it may be launched ahead of their end
     const int pdl = g_use_pdl;
     g_use_pdl = 1;
-    rc = launch_kernel(kv8_merge_kernel<kDim>, dim3((unsigned)p.q_heads, (unsigned)p.rows), dim3(kMergers * kDim / 4), 0, st, 1, p);
+    constexpr int kAtOnce = 256 / (kDim / 4);
+    if (p.splits <= kMostRanks)
+        rc = launch_kernel(kv8_merge_few_kernel<kDim>, dim3((unsigned)ceil_div(rows * p.q_heads, kAtOnce)), dim3(256), 0, st, 1, p);
+    else
+        rc = launch_kernel(kv8_merge_kernel<kDim>, dim3((unsigned)rows, (unsigned)p.q_heads), dim3(kMergers * kDim / 4), 0, st, 1, p);
     g_use_pdl = pdl;
     return rc;
 }
@@ -441,9 +498,10 @@ extern "C" {
 int gptrs_cuda_kv8_splits(const gptrs_kv8_cache* c, int64_t rows, int64_t n_tiles, int64_t max_ctx_len) {
     if (!c || rows < 1 || c->kv_heads < 1) return 1;
     if (n_tiles > 0) {
-        // a CTA per tile and kv head has an SM to itself: parts only where many SMs would have nothing, of 512 keys at least
+        // a CTA per tile and kv head has an SM to itself: parts only where many SMs would have nothing, of 4096 keys at least (one prompt of 2048 tokens, 8 / 1
+        // heads of 128: one part 52 us, two 62; 500 tokens behind 32768, 32 / 8 heads: NN, two 378)
         const int64_t ctas = n_tiles * c->kv_heads, keys = c->window > 0 ? std::min<int64_t>(max_ctx_len, c->window + c->tile_tokens) : max_ctx_len;
-        return rows > 65535 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(sm_count() / ctas, keys / 512));
+        return rows > 65535 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(sm_count() / ctas, keys / 4096));
     }
     const int64_t seen = c->window > 0 ? std::min<int64_t>(max_ctx_len, c->window + kKv8Tokens) : max_ctx_len;
     const int64_t blocks = (seen + kKv8Tokens - 1) / kKv8Tokens;
@@ -494,7 +552,14 @@ int gptrs_cuda_kv8_attention(const gptrs_kv8_cache* c, const gptrs_kv8_attention
     p.chunk_blocks = std::max(1, ceil_div(seen, s->splits));
     p.part_o = static_cast<float*>(s->d_scratch);
     p.part_ml = p.part_o + (size_t)p.rows * p.q_heads * p.splits * c->dim;
-    p.tile_row = s->d_tile_row; p.tile_rows = s->d_tile_rows; p.n_tiles = (int)s->n_tiles;
+    p.tile_row = s->d_tile_row; p.tile_rows = s->d_tile_rows; p.n_tiles = (int)s->n_tiles; p.tile_tokens = c->tile_tokens;
+    if (p.n_tiles > 0 && p.splits == 1 && rows_one_by_one(*c, s->rows, s->n_tiles, p.max_len)) {
+        p.one_by_one = 1;
+        p.splits = gptrs_cuda_kv8_splits(c, s->rows, 0, p.max_len);
+        p.splits = std::min(p.splits, kMostRanks);
+        p.chunk_blocks = std::max(1, ceil_div(seen, p.splits));
+        return c->dim == 64 ? launch_attention<64>(p, as_stream(stream)) : launch_attention<128>(p, as_stream(stream));
+    }
     // a grid's last dimension holds 65535 rows: longer lists go in several launches over their own part of the scratch
     const int64_t most = s->n_tiles && s->splits == 1 ? s->rows : 65535;
     GPTRS_REQUIRE(s->n_tiles == 0 || s->rows <= most, "tiles of more than 65535 rows are not split along the keys");

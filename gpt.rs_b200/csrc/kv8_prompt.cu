@@ -130,12 +130,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     const int kv_head = blockIdx.x, tile = (int)gridDim.y - 1 - (int)blockIdx.y;   // the longest contexts come last in a chunk: start them first
 
     pdl_wait();
-    const int row0 = p.tile_row[tile], n_rows = p.tile_rows[tile];
-    if (row0 < 0 || n_rows < 0 || n_rows > kTiles * tq || row0 > p.rows - n_rows) {
-        if (tid == 0) atomicExch(p.status, 2);
-        return;
-    }
-    if (n_rows == 0) return;
+    const int row0 = kv8_row(p, tile * p.tile_tokens);   // (tile_tokens: 2 tq)
+    if (row0 < 0) return;
+    const int n_rows = p.tile_rows[tile];
     const int slot = p.slot[row0];
 
     if (tid == 0) {
@@ -526,13 +523,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             for (int half = 0; half < 2; ++half) {
                 float share;
                 load(half);
+                // the first scores of all have their maximum taken first; others only where the weights turn out too large
+                bool raised = kb == 0 && half == 0;
+                if (raised) raise(half, true);
 #pragma unroll 1
-                for (int round = 0; ; ++round) {
+                while (true) {
                     const bool over = exact ? weigh(half, std::false_type{}, share) : weigh(half, std::true_type{}, share);
-                    if (round == 1 || !__any_sync(0xffffffffu, over)) break;
+                    if (raised || !__any_sync(0xffffffffu, over)) break;
                     load(half);   // the weights have not been stored over the scores yet
                     raise(half, over);
-                    exact = true;
+                    raised = exact = true;
                 }
                 l_run += share;
                 tmem_st_32(t_s + 32u * half, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));

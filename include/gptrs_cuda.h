@@ -665,7 +665,8 @@ int gptrs_cuda_paged_attention_prefill_tc(const void* d_q, const void* d_kv_pool
  * `starve` is non-zero the K pages of every CTA's first key block are never requested, so the waits that depend on them
  * run out after `wait_limit` parked polls of about a microsecond (0 = the built-in 2^16); every warp then leaves its
  * loop, code 3 lands in *d_status, the tensor memory is freed and the kernel returns with an unspecified result. Nothing
- * faults and nothing waits without a bound. Process-wide; call with (0, 0) to switch it off again. */
+ * faults and nothing waits without a bound. The kernels of gptrs_cuda_kv8_attention go by the same switch. Process-wide; call with (0, 0) to switch
+ * it off again. */
 int gptrs_cuda_debug_prefill_tc_fault(int starve, uint32_t wait_limit);
 
 /* Debug: later launches of gptrs_cuda_paged_attention_prefill_tc record clock64 samples of one CTA (the longest tile of
@@ -782,7 +783,7 @@ int gptrs_cuda_kv8_gather(const gptrs_kv8_cache* c, const void* d_pool, int64_t 
 /* out [rows][q_heads][dim] (bf16) = softmax over the visible keys . values; row t belongs to slot[t] and sees the last `window` of its first
  * ctx_len[t] tokens (the cache as it is behind the append). A row that sees nothing gives zeros, one with a negative slot is left as it was.
  * n_tiles = 0: every row by itself (single tokens of many sequences); else tile i is the rows tile_row[i] .. + tile_rows[i], at most tile_tokens
- * rows of one sequence at consecutive positions (prompts, chunks of prompts). The keys of a row or tile are read in at most `splits` parts
+ * rows of one sequence at consecutive positions (prompts, chunks of prompts); rows in no tile are left as they were, no row is in two. The keys of a row or tile are read in at most `splits` parts
  * (gptrs_cuda_kv8_splits; scratch: gptrs_cuda_kv8_scratch_bytes). max_ctx_len bounds ctx_len. *d_status = 2: a length, slot or
  * page out of range, 3: a bounded wait ran out. */
 typedef struct {

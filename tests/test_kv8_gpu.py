@@ -440,7 +440,82 @@ def test_prompts(cuda, heads, kv, dim, window, prompts):
     """Every token of a chunk sees the cache as it is behind the append, up to itself."""
     c = Cache(cuda, heads, kv, dim, len(prompts), max(s + n for s, n in prompts) // 16 + 2, window=window, seed=heads + sum(n for _, n in prompts))
     c.fill([s + n for s, n in prompts])
-    c.attend([(i, p + 1) for i, (s, n) in enumerate(prompts) for p in range(s, s + n)], tiles=[n for _, n in prompts])
+    for splits in (None, 2):   # short ones go row by row unless they are cut
+        c.attend([(i, p + 1) for i, (s, n) in enumerate(prompts) for p in range(s, s + n)], tiles=[n for _, n in prompts], splits=splits)
+
+
+@pytest.mark.parametrize("heads,kv,dim,window", [(32, 8, 128, 0), (12, 12, 64, 0), (24, 8, 128, 300), (20, 4, 64, 0), (16, 8, 64, 129)])
+@pytest.mark.parametrize("prompts", [[(0, 1100)], [(700, 333), (5, 800), (0, 64)]])
+def test_longer_prompts(cuda, heads, kv, dim, window, prompts):
+    c = Cache(cuda, heads, kv, dim, len(prompts), max(s + n for s, n in prompts) // 16 + 2, window=window, seed=heads + sum(n for _, n in prompts))
+    c.fill([s + n for s, n in prompts])
+    rows = [(i, p + 1) for i, (s, n) in enumerate(prompts) for p in range(s, s + n)]
+    q, out = c.attend(rows, tiles=[n for _, n in prompts], splits=1, want=False)
+    c.check(rows, q, out, every=41)
+    assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("splits", [1, 2, 9])
+@pytest.mark.parametrize("n", [40, 1000])
+def test_rows_in_no_tile_and_tiles_that_are_none(cuda, splits, n):
+    """Rows that no tile holds stay as they were; a tile outside the rows is reported and the others are right."""
+    c = Cache(cuda, 32, 8, 128, 1, 70, seed=n)
+    c.fill([n])
+    rows = [(0, i + 1) for i in range(n)]
+    q = torch.randn((n, 32, 128), device=cuda).bfloat16()
+    for extra in ((), ((n - 10, 11),), ((-1, 5),), ((0, 65),), ((3, -1),)):
+        first, count = zip(*([(5, 20), (30, 0)] + ([(100, 64), (200, 1), (300, 64)] if n > 40 else []) + list(extra)))
+        out = torch.full((n, 32 * 128), 3.0, dtype=torch.bfloat16, device=cuda)
+        c.status.zero_()
+        ops.kv8_attention(c.a, q, c.pool, c.rows, c.table, _ints([0] * n, cuda), _ints([x for _, x in rows], cuda), c.lengths(), n, tiles=(_ints(first, cuda), _ints(count, cuda)), splits=splits,
+                          out=out, status=c.status)
+        assert int(c.status) == (2 if extra else 0)
+        inside = sorted({r for f, k in zip(first[:2 if n == 40 else 5], count) for r in range(f, f + k)})
+        outside = [r for r in range(n) if r not in set(inside)]
+        assert (out[outside] == 3).all()
+        c.status.zero_()
+        at = inside[::7]
+        c.check([rows[r] for r in at], q[at], out[at])
+
+
+def test_scores_that_grow_along_the_keys(cuda):
+    """The reference of the weights has to follow: every block's scores are far above the one before, and then far below."""
+    c = Cache(cuda, 32, 8, 128, 1, 72, seed=3)
+    n = 1100
+    qkv = torch.randn((n, 48 * 128), device=cuda)
+    ramp = torch.cat([torch.linspace(0, 30, n // 2), torch.linspace(30, -30, n - n // 2)]).to(cuda)
+    qkv[:, 32 * 128:40 * 128] = ramp[:, None]
+    c.append([(0, 0, n)], qkv.bfloat16())
+    q = (torch.rand((n, 32, 128), device=cuda) * 0.3).bfloat16()
+    rows = [(0, i + 1) for i in range(n)]
+    _, out = c.attend(rows, tiles=[n], q=q, splits=1, want=False)
+    c.check(rows, q, out, every=23)
+    for splits in (2, 3):
+        _, out = c.attend(rows, tiles=[n], q=q, splits=splits, want=False)
+        c.check(rows, q, out, every=61)
+    _, out = c.attend(rows[-40:], q=q[-40:].contiguous(), want=False)
+    c.check(rows[-40:], q[-40:], out)
+    assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+def test_waits_that_run_out_end_the_kernel(cuda, tiles):
+    """Keys that are never asked for: every wait ends, the status says so, and the next call is right."""
+    from gptrs_b200 import lib
+    c = Cache(cuda, 32, 8, 128, 1, 72, seed=5)
+    c.fill([1100])
+    rows = [(0, i + 1) for i in range(1100)] if tiles else [(0, 1100), (0, 300)]
+    try:
+        assert lib().gptrs_cuda_debug_prefill_tc_fault(1, 64) == 0
+        q, _ = c.attend(rows, tiles=[1100] if tiles else None, splits=1, want=False)
+        torch.cuda.synchronize()
+    finally:
+        lib().gptrs_cuda_debug_prefill_tc_fault(0, 0)
+    assert int(c.status) == 3
+    c.status.zero_()
+    q, out = c.attend(rows, tiles=[1100] if tiles else None, splits=1, want=False, q=q)
+    c.check(rows, q, out, every=97)
+    assert int(c.status) == 0
 
 
 @pytest.mark.parametrize("splits", [1, 2, 5])
