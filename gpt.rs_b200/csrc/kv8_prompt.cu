@@ -113,10 +113,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     constexpr int kQBytes = kRows * kDim * 2, kKBytes = kKeys * kDim * 2, kVHalf = kDim * 128;   // a half of V^T: 64 keys
     constexpr int kC = kDim / 32;
     constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(kRows >> 4) << 24);                       // f32 accumulator, f16 operands, M = 128
-    constexpr uint32_t kIdescS = kIdesc | ((uint32_t)(kKeys >> 3) << 17), kIdescO = kIdesc | ((uint32_t)(kDim >> 3) << 17);
+    constexpr uint32_t kIdescS = kIdesc | ((uint32_t)(kKeys / 2 >> 3) << 17), kIdescO = kIdesc | ((uint32_t)(kDim >> 3) << 17);
 
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t k_first, full[2], empty[2], s_full[kTiles], p_full[kTiles][2], o_half[kTiles], o_full[kTiles], drained;
+    __shared__ __align__(8) uint64_t k_first, full[2], empty[2], s_full[kTiles][2], p_full[kTiles][2], o_first[kTiles], o_full[kTiles], drained;
     __shared__ uint32_t tmem_holder;
     __shared__ int s_begin[kSoftmaxThreads / 32], s_end[kSoftmaxThreads / 32];
     __shared__ __align__(16) float scales[kScaleSlots][kPages][4];   // s_K scale log2 e, log2 s_V, 1 / s_V
@@ -138,7 +138,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     if (tid == 0) {
         mbar_init(&k_first, kLoadWarps);
         for (int i = 0; i < 2; ++i) { mbar_init(&full[i], kLoadWarps); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < kTiles; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i][0], kRows); mbar_init(&p_full[i][1], kRows); mbar_init(&o_half[i], 1); mbar_init(&o_full[i], 1); }
+        for (int i = 0; i < kTiles; ++i) {
+            for (int h = 0; h < 2; ++h) { mbar_init(&s_full[i][h], 1); mbar_init(&p_full[i][h], kRows); }
+            mbar_init(&o_first[i], 1);
+            mbar_init(&o_full[i], 1);
+        }
         mbar_init(&drained, 1);
         mbar_fence_init();
     }
@@ -383,40 +387,39 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kMmaRegs));
         if (elect_one()) {
             auto wait_one = [&](uint64_t* bar, uint32_t parity) { return !failed && !(failed = !mbar_wait_parked(smem_u32(bar), parity, params.wait_limit)); };
-            auto issue_s = [&](int i, int kb) {
-                const uint64_t a_desc = make_smem_desc(sQ + i * kQBytes), b_desc = make_smem_desc(sK + (kb & 1) * kKBytes);
+            auto issue_s = [&](int i, int h, int kb) {   // 64 keys
+                const uint64_t a_desc = make_smem_desc(sQ + i * kQBytes), b_desc = make_smem_desc(sK + (kb & 1) * kKBytes + h * (kKeys / 2) * 128);
 #pragma unroll
                 for (int ks = 0; ks < kDim / 16; ++ks) {
                     const uint64_t off = (uint64_t)((ks >> 2) * (kHalfBytes >> 4) + 2 * (ks & 3));
-                    umma_f16(tmem + (uint32_t)i * kKeys, a_desc + off, b_desc + off, kIdescS, ks > 0 ? 1u : 0u);
+                    umma_f16(tmem + (uint32_t)(i * kKeys + h * (kKeys / 2)), a_desc + off, b_desc + off, kIdescS, ks > 0 ? 1u : 0u);
                 }
-                umma_commit(&s_full[i]);
+                umma_commit(&s_full[i][h]);
             };
             if (n_blocks > 0 && wait_one(&k_first, 0)) {
                 tc_fence_after();
-                for (int i = 0; i < kTiles; ++i) if (nb_t[i] > 0) issue_s(i, 0);
+                for (int h = 0; h < 2; ++h)
+                    for (int i = 0; i < kTiles; ++i) if (nb_t[i] > 0) issue_s(i, h, 0);
             }
             for (int kb = 0; kb < n_blocks && !failed; ++kb) {
                 const int st = kb & 1;
                 if (!wait_one(&full[st], (uint32_t)(kb >> 1) & 1u)) break;
-                for (int i = 0; i < kTiles; ++i) {
-                    if (kb < nb_t[i]) {
-                        const uint64_t b_desc = make_smem_desc(sV + st * 2 * kVHalf);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {   // 64 keys at a time, as their weights arrive
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < kTiles; ++i) {
+                        if (kb < nb_t[i] && !failed) {
                             if (!wait_one(&p_full[i][h], (uint32_t)kb & 1u)) break;
                             tc_fence_after();
+                            const uint64_t b_desc = make_smem_desc(sV + st * 2 * kVHalf + h * kVHalf);
 #pragma unroll
                             for (int ks = 0; ks < kKeys / 32; ++ks)
-                                umma_bf16_ts(tmem + kOCol + (uint32_t)i * kDim, tmem + (uint32_t)i * kKeys + 32u * h + 8u * ks, b_desc + (uint64_t)(h * (kVHalf >> 4) + 2 * ks), kIdescO,
+                                umma_bf16_ts(tmem + kOCol + (uint32_t)i * kDim, tmem + (uint32_t)(i * kKeys + h * (kKeys / 2)) + 8u * ks, b_desc + (uint64_t)(2 * ks), kIdescO,
                                              (kb > 0 || h > 0 || ks > 0) ? 1u : 0u);
-                            if (h == 0) umma_commit(&o_half[i]);
+                            if (kb == nb_t[i] - 1) umma_commit(h ? &o_full[i] : &o_first[i]);
+                            if (kb + 1 < nb_t[i]) issue_s(i, h, kb + 1);
                         }
-                        if (failed) break;
-                        if (kb == nb_t[i] - 1) umma_commit(&o_full[i]);
                     }
-                    if (kb + 1 < nb_t[i]) issue_s(i, kb + 1);
-                }
                 if (!failed) umma_commit(&empty[st]);
             }
             if (failed) {   // products in flight read shared and tensor memory: let them end before the CTA does
@@ -431,43 +434,45 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t t_s = t_lane + (uint32_t)ti * kKeys, t_o = t_lane + kOCol + (uint32_t)ti * kDim;
         const int my_blocks = nb_t[ti];
-        const uint32_t s_bar = smem_u32(&s_full[ti]), p_bar = smem_u32(&p_full[ti][0]), sc0 = smem_u32(&scales[0][0][0]);
+        const uint32_t s_bar = smem_u32(&s_full[ti][0]), p_bar = smem_u32(&p_full[ti][0]), sc0 = smem_u32(&scales[0][0][0]);
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
         float m_run = -1e30f, l_run = 0.f;
-        for (int kb = 0; kb < my_blocks; ++kb) {
-            if (!mbar_wait_parked(s_bar, (uint32_t)kb & 1u, params.wait_limit)) failed = true;
+#pragma unroll 1   // (the code of a half is long: copies of it do not stay in the instruction cache)
+        for (int step = 0; step < 2 * my_blocks; ++step) {
+            const int kb = step >> 1, half = step & 1;
+            if (!mbar_wait_parked(s_bar + 8u * half, (uint32_t)kb & 1u, params.wait_limit)) failed = true;
             failed = __any_sync(0xffffffffu, failed);
             if (failed) break;
             tc_fence_after();
-            const uint32_t sc = sc0 + (uint32_t)(kb % kScaleSlots) * (kPages * 16);
-            const int key0 = first_key + kb * kKeys;
-            const bool whole = __all_sync(0xffffffffu, begin <= key0 && end >= key0 + kKeys);   // this warp's rows see all of the block
+            const uint32_t sc = sc0 + (uint32_t)(kb % kScaleSlots) * (kPages * 16) + half * (kPages / 2 * 16), t_h = t_s + half * (kKeys / 2);
+            const int key0 = first_key + kb * kKeys + half * (kKeys / 2);
+            const bool whole = __all_sync(0xffffffffu, begin <= key0 && end >= key0 + kKeys / 2);   // this warp's rows see all of the half
             uint32_t s[64];   // scores of half a block, then their weights
-            auto load = [&](int half) {
-                tmem_ld_32_async(t_s + 64u * half, s);
-                tmem_ld_32_async(t_s + 64u * half + 32u, s + 32);
+            auto load = [&] {
+                tmem_ld_32_async(t_h, s);
+                tmem_ld_32_async(t_h + 32u, s + 32);
                 tmem_wait_ld();   // straight behind: nothing may touch the registers before
             };
             // Raises the reference of rows whose weights of a half came out too large, to about that half's maximum: what was computed with the old one
             // (output and sum) is scaled down. Rare behind a sequence's first keys.
-            auto raise = [&](int half, bool over) {
+            auto raise = [&](bool over) {
                 float top = m_run;
 #pragma unroll
                 for (int j = 0; j < 64; ++j) {
-                    const float4 x = ld_shared_f4(sc + (4 * half + j / 16) * 16);
-                    const int key = key0 + 64 * half + j;
+                    const float4 x = ld_shared_f4(sc + (j / 16) * 16);
+                    const int key = key0 + j;
                     if (over && key >= begin && key < end) top = fmaxf(top, fmaf(__uint_as_float(s[j]), x.x * q_scale, x.y));
                 }
                 const float alpha = kv8_exp2(m_run - top);   // (0 the first time)
                 m_run = top;
                 l_run *= alpha;
                 if (kb == 0 && half == 0) return;
-                // the tile's products with V so far are complete: those of earlier blocks were issued before these scores, the first half's is waited for
-                if (half == 1) {
-                    if (!mbar_wait_parked(smem_u32(&o_half[ti]), (uint32_t)kb & 1u, params.wait_limit)) failed = true;
-                    failed = __any_sync(0xffffffffu, failed);
-                    tc_fence_after();
-                }
+                // The products with V so far have to be complete. Those of this half came before these scores; of the other half, behind its next scores (or the
+                // last block's: o_first).
+                const bool last = half == 1 && kb + 1 == my_blocks;
+                if (!mbar_wait_parked(last ? smem_u32(&o_first[ti]) : s_bar + 8u * (half ^ 1), last ? 0u : (uint32_t)(kb + half) & 1u, params.wait_limit)) failed = true;
+                failed = __any_sync(0xffffffffu, failed);
+                tc_fence_after();
 #pragma unroll 1
                 for (int i = 0; i < kDim / 16; ++i) {
                     uint32_t r[16];
@@ -479,13 +484,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             };
             // Scores of a half -> weights, packed in the order of V's keys, and their share of the sum; returns whether a page's weights add up to more
             // than keeps each an f16 (or to no number)
-            auto weigh = [&](int half, auto all_seen, float& share) {
+            auto weigh = [&](auto all_seen, float& share) {
                 constexpr bool kWhole = decltype(all_seen)::value;
                 bool fits = true;
                 share = 0.f;
 #pragma unroll
                 for (int pg = 0; pg < 4; ++pg) {
-                    const float4 x = ld_shared_f4(sc + (4 * half + pg) * 16);
+                    const float4 x = ld_shared_f4(sc + pg * 16);
                     const float cq = x.x * q_scale, b = x.y - m_run;
                     const uint64_t c2 = pair_of(cq, cq), b2 = pair_of(b, b);
                     uint64_t part = 0;
@@ -501,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                             w = make_float2(kv8_exp2(t.x), kv8_exp2(t.y));
                         }
                         if (!kWhole) {
-                            const int key = key0 + 64 * half + 16 * pg + 2 * i;
+                            const int key = key0 + 16 * pg + 2 * i;
                             w.x = key >= begin && key < end ? w.x : 0.f;
                             w.y = key + 1 >= begin && key + 1 < end ? w.y : 0.f;
                         }
@@ -518,28 +523,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 }
                 return !fits;
             };
-            bool exact = !whole;   // which of the two ways
-#pragma unroll 1   // (the code of a half is long: copies of it do not stay in the instruction cache)
-            for (int half = 0; half < 2; ++half) {
-                float share;
-                load(half);
-                // the first scores of all have their maximum taken first; others only where the weights turn out too large
-                bool raised = kb == 0 && half == 0;
-                if (raised) raise(half, true);
+            float share;
+            load();
+            // the first scores of all have their maximum taken first; others only where the weights turn out too large
+            bool exact = !whole, raised = step == 0;
+            if (raised) raise(true);
 #pragma unroll 1
-                while (true) {
-                    const bool over = exact ? weigh(half, std::false_type{}, share) : weigh(half, std::true_type{}, share);
-                    if (raised || !__any_sync(0xffffffffu, over)) break;
-                    load(half);   // the weights have not been stored over the scores yet
-                    raise(half, over);
-                    raised = exact = true;
-                }
-                l_run += share;
-                tmem_st_32(t_s + 32u * half, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
-                asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-                tc_fence_before();
-                mbar_arrive_addr(p_bar + 8u * half);
+            while (true) {
+                const bool over = exact ? weigh(std::false_type{}, share) : weigh(std::true_type{}, share);
+                if (raised || !__any_sync(0xffffffffu, over)) break;
+                load();   // the weights have not been stored over the scores yet
+                raise(over);
+                raised = exact = true;
             }
+            l_run += share;
+            tmem_st_32(t_h, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+            asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+            tc_fence_before();
+            mbar_arrive_addr(p_bar + 8u * half);
         }
         // ---- the output, or this split's part of it --------------------------------------------------------------------------------------------
         if (my_blocks > 0 && !failed) {
