@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             const uint32_t sc = sc0 + (uint32_t)(kb % kScaleSlots) * (kPages * 16) + half * (kPages / 2 * 16), t_h = t_s + half * (kKeys / 2);
             const int key0 = first_key + kb * kKeys + half * (kKeys / 2);
             const bool whole = __all_sync(0xffffffffu, begin <= key0 && end >= key0 + kKeys / 2);   // this warp's rows see all of the half
-            uint32_t s[64];   // scores of half a block, then their weights
+            uint32_t s[64], weights[32];   // scores of half a block; two weights each
             auto load = [&] {
                 tmem_ld_32_async(t_h, s);
                 tmem_ld_32_async(t_h + 32u, s + 32);
@@ -494,7 +494,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                     const float cq = x.x * q_scale, b = x.y - m_run;
                     const uint64_t c2 = pair_of(cq, cq), b2 = pair_of(b, b);
                     uint64_t part = 0;
-                    uint32_t packed[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {   // keys 2 i, 2 i + 1
                         const uint64_t t2 = fma2(pair_of(__uint_as_float(s[16 * pg + 2 * i]), __uint_as_float(s[16 * pg + 2 * i + 1])), c2, b2);
@@ -511,10 +510,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                             w.y = key + 1 >= begin && key + 1 < end ? w.y : 0.f;
                         }
                         part = add2(part, pair_of(w.x, w.y));
-                        packed[i < 4 ? 2 * i : 2 * (i - 4) + 1] = pack_f16x2(w.x, w.y);
+                        weights[8 * pg + (i < 4 ? 2 * i : 2 * (i - 4) + 1)] = pack_f16x2(w.x, w.y);
                     }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) s[8 * pg + i] = packed[i];   // the scores of this and earlier pages are consumed
                     const float2 both = split(part);
                     const float page_sum = both.x + both.y;
                     // 1 / s_V that is not a number belongs to a page that is none: of rows that see all of it. Others find that in their weights.
@@ -523,22 +520,36 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 }
                 return !fits;
             };
-            float share;
-            load();
+            auto store = [&] {
+                tmem_st_32(t_h, weights);
+                asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+            };
             // the first scores of all have their maximum taken first; others only where the weights turn out too large
-            bool exact = !whole, raised = step == 0;
-            if (raised) raise(true);
-#pragma unroll 1
-            while (true) {
-                const bool over = exact ? weigh(std::false_type{}, share) : weigh(std::true_type{}, share);
-                if (raised || !__any_sync(0xffffffffu, over)) break;
-                load();   // the weights have not been stored over the scores yet
-                raise(over);
-                raised = exact = true;
+            float share;
+            bool over = true, raises = true, done = false;
+            if (whole && step > 0) {
+                load();
+                over = weigh(std::true_type{}, share);
+                done = !__any_sync(0xffffffffu, over);
+                if (done) {
+                    l_run += share;
+                    store();
+                }
+            } else {
+                raises = step == 0;
             }
-            l_run += share;
-            tmem_st_32(t_h, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
-            asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+            if (!done) {   // (apart, so that the registers of the usual way need not meet those of this one)
+#pragma unroll 1
+                for (int pass = 0; pass < 2; ++pass) {
+                    load();   // the weights have not been stored over the scores yet
+                    if (raises) raise(over);
+                    over = weigh(std::false_type{}, share);
+                    if (raises || !__any_sync(0xffffffffu, over)) break;
+                    raises = true;
+                }
+                l_run += share;
+                store();
+            }
             tc_fence_before();
             mbar_arrive_addr(p_bar + 8u * half);
         }
