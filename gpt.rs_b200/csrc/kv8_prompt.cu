@@ -436,17 +436,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         const int my_blocks = nb_t[ti];
         const uint32_t s_bar = smem_u32(&s_full[ti][0]), p_bar = smem_u32(&p_full[ti][0]), sc0 = smem_u32(&scales[0][0][0]);
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
-        float m_run = -1e30f, l_run = 0.f;
-#pragma unroll 1   // (the code of a half is long: copies of it do not stay in the instruction cache)
-        for (int step = 0; step < 2 * my_blocks; ++step) {
-            const int kb = step >> 1, half = step & 1;
-            if (!mbar_wait_parked(s_bar + 8u * half, (uint32_t)kb & 1u, params.wait_limit)) failed = true;
+        // Halves of blocks (64 keys; steps, two of a block) that all rows of this warp see: most. Rows that are nobody's see what the others do.
+        const int seen_from = __reduce_max_sync(0xffffffffu, live ? begin : 0) - first_key, seen_to = __reduce_min_sync(0xffffffffu, live ? end : 0x7fffffff) - first_key;
+        const int steps = 2 * my_blocks, whole_from = max(1, (seen_from + kKeys / 2 - 1) / (kKeys / 2)), whole_to = min(steps, seen_to / (kKeys / 2));
+        float m_run = live ? -1e30f : 0.f, l_run = 0.f;
+        int step = 0;
+        auto scores_there = [&] {   // of this step; whole warp
+            if (!mbar_wait_parked(s_bar + 8u * (step & 1), (uint32_t)(step >> 1) & 1u, params.wait_limit)) failed = true;
             failed = __any_sync(0xffffffffu, failed);
-            if (failed) break;
             tc_fence_after();
-            const uint32_t sc = sc0 + (uint32_t)(kb % kScaleSlots) * (kPages * 16) + half * (kPages / 2 * 16), t_h = t_s + half * (kKeys / 2);
-            const int key0 = first_key + kb * kKeys + half * (kKeys / 2);
-            const bool whole = __all_sync(0xffffffffu, begin <= key0 && end >= key0 + kKeys / 2);   // this warp's rows see all of the half
+            return !failed;
+        };
+#pragma unroll 1   // (the code of a half is long: copies of it do not stay in the instruction cache)
+        while (step < steps) {
+            uint32_t sc, t_h;   // this step's scales; its scores, later its weights
+            auto place = [&] {
+                sc = sc0 + (uint32_t)((step >> 1) % kScaleSlots) * (kPages * 16) + (step & 1) * (kPages / 2 * 16);
+                t_h = t_s + (uint32_t)(step & 1) * (kKeys / 2);
+            };
             uint32_t s[64], weights[32];   // scores of half a block; two weights each
             auto load = [&] {
                 tmem_ld_32_async(t_h, s);
@@ -456,6 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             // Raises the reference of rows whose weights of a half came out too large, to about that half's maximum: what was computed with the old one
             // (output and sum) is scaled down. Rare behind a sequence's first keys.
             auto raise = [&](bool over) {
+                const int kb = step >> 1, half = step & 1, key0 = first_key + step * (kKeys / 2);
                 float top = m_run;
 #pragma unroll
                 for (int j = 0; j < 64; ++j) {
@@ -486,6 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             // than keeps each an f16 (or to no number)
             auto weigh = [&](auto all_seen, float& share) {
                 constexpr bool kWhole = decltype(all_seen)::value;
+                const int key0 = first_key + step * (kKeys / 2);
                 bool fits = true;
                 share = 0.f;
 #pragma unroll
@@ -518,40 +527,38 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                     share = fmaf(page_sum, kWhole || x.z == x.z ? x.z : 1.f, share);
                     fits &= page_sum <= kLargestSum;
                 }
-                return !fits;
+                return !fits && live;
             };
-            auto store = [&] {
+            float share;
+            auto hand_over = [&] {
+                l_run += share;
                 tmem_st_32(t_h, weights);
                 asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+                tc_fence_before();
+                mbar_arrive_addr(p_bar + 8u * (step & 1));
+                ++step;
             };
-            // the first scores of all have their maximum taken first; others only where the weights turn out too large
-            float share;
-            bool over = true, raises = true, done = false;
-            if (whole && step > 0) {
+            bool over = true, raises = step == 0;   // the first scores of all have their maximum taken first; others only where the weights turn out too large
+#pragma unroll 1
+            while (step >= whole_from && step < whole_to) {   // the usual way, apart from the other one so that their registers need not meet
+                if (!scores_there()) break;
+                place();
                 load();
                 over = weigh(std::true_type{}, share);
-                done = !__any_sync(0xffffffffu, over);
-                if (done) {
-                    l_run += share;
-                    store();
-                }
-            } else {
-                raises = step == 0;
+                if (__any_sync(0xffffffffu, over)) { raises = true; break; }
+                hand_over();
             }
-            if (!done) {   // (apart, so that the registers of the usual way need not meet those of this one)
+            if (failed || step == steps || !scores_there()) break;
+            place();
 #pragma unroll 1
-                for (int pass = 0; pass < 2; ++pass) {
-                    load();   // the weights have not been stored over the scores yet
-                    if (raises) raise(over);
-                    over = weigh(std::false_type{}, share);
-                    if (raises || !__any_sync(0xffffffffu, over)) break;
-                    raises = true;
-                }
-                l_run += share;
-                store();
+            for (int pass = 0; pass < 2; ++pass) {
+                load();   // the weights have not been stored over the scores yet
+                if (raises) raise(over);
+                over = weigh(std::false_type{}, share);
+                if (raises || !__any_sync(0xffffffffu, over)) break;
+                raises = true;
             }
-            tc_fence_before();
-            mbar_arrive_addr(p_bar + 8u * half);
+            hand_over();
         }
         // ---- the output, or this split's part of it --------------------------------------------------------------------------------------------
         if (my_blocks > 0 && !failed) {
