@@ -32,7 +32,7 @@ constexpr int kTiles = 2;
 constexpr int kSoftmaxThreads = kTiles * kRows;
 constexpr int kLoadWarps = 4;
 constexpr int kLoadWarp = kSoftmaxThreads / 32, kMmaWarp = kLoadWarp + kLoadWarps;
-constexpr int kThreads = kSoftmaxThreads + kLoadWarps * 32 + 128;   // the MMA warp and three that only make its group whole
+constexpr int kThreads = kSoftmaxThreads + kLoadWarps * 32 + 128;   // two warps for the products and two that only make their group whole
 // Registers of a thread at launch, and what the groups of four warps make of them: the shares add up to what the block has, so every request ends.
 constexpr int kLaunchRegs = 128, kSoftmaxRegs = 160, kLoadRegs = kLaunchRegs, kMmaRegs = 64;
 static_assert(kThreads == 512 && 2 * kSoftmaxRegs + kLoadRegs + kMmaRegs <= 4 * kLaunchRegs, "more registers than the block is launched with");
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     constexpr uint32_t kIdescS = kIdesc | ((uint32_t)(kKeys / 2 >> 3) << 17), kIdescO = kIdesc | ((uint32_t)(kDim >> 3) << 17);
 
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t k_first, full[2], empty[2], s_full[kTiles][2], p_full[kTiles][2], o_first[kTiles], o_full[kTiles], drained;
+    __shared__ __align__(8) uint64_t k_first, full[2], empty[2], s_full[kTiles][2], p_full[kTiles][2], o_first[kTiles], o_full[kTiles], drained[kTiles];
     __shared__ uint32_t tmem_holder;
     __shared__ int s_begin[kSoftmaxThreads / 32], s_end[kSoftmaxThreads / 32];
     __shared__ __align__(16) float scales[kScaleSlots][kPages][4];   // s_K scale log2 e, log2 s_V, 1 / s_V
@@ -137,13 +137,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 
     if (tid == 0) {
         mbar_init(&k_first, kLoadWarps);
-        for (int i = 0; i < 2; ++i) { mbar_init(&full[i], kLoadWarps); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&full[i], kLoadWarps); mbar_init(&empty[i], kTiles); }
         for (int i = 0; i < kTiles; ++i) {
             for (int h = 0; h < 2; ++h) { mbar_init(&s_full[i][h], 1); mbar_init(&p_full[i][h], kRows); }
             mbar_init(&o_first[i], 1);
             mbar_init(&o_full[i], 1);
+            mbar_init(&drained[i], 1);
         }
-        mbar_init(&drained, 1);
         mbar_fence_init();
     }
     if (warp == kMmaWarp) {
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         return !failed;
     };
 
-    if (warp > kMmaWarp) {
+    if (warp >= kMmaWarp + kTiles) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kMmaRegs));
     } else if (warp >= kLoadWarp && warp < kMmaWarp) {
         // ================= warps 8 - 11: pages 2 w, 2 w + 1 of every block ===================================================================
@@ -382,49 +382,46 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             if (lane == 0) mbar_arrive(&full[st]);
         }
         if (failed && lane == 0) atomicExch(p.status, 3);
-    } else if (warp == kMmaWarp) {
-        // ================= warp 12: every product =================================================================================================
+    } else if (warp >= kMmaWarp) {
+        // ================= warps 12, 13: the products of a tile each, so that neither waits for the other's weights ================================
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kMmaRegs));
         if (elect_one()) {
+            const int i = warp - kMmaWarp, my_blocks = nb_t[i];
             auto wait_one = [&](uint64_t* bar, uint32_t parity) { return !failed && !(failed = !mbar_wait_parked(smem_u32(bar), parity, params.wait_limit)); };
-            auto issue_s = [&](int i, int h, int kb) {   // 64 keys
-                const uint64_t a_desc = make_smem_desc(sQ + i * kQBytes), b_desc = make_smem_desc(sK + (kb & 1) * kKBytes + h * (kKeys / 2) * 128);
+            const uint64_t q_desc = make_smem_desc(sQ + i * kQBytes), k_desc = make_smem_desc(sK), v_desc = make_smem_desc(sV);
+            const uint32_t t_s = tmem + (uint32_t)(i * kKeys), t_o = tmem + kOCol + (uint32_t)(i * kDim);
+            auto issue_s = [&](int h, int kb) {   // 64 keys
+                const uint64_t b_desc = k_desc + (uint64_t)(((kb & 1) * kKBytes + h * (kKeys / 2) * 128) >> 4);
 #pragma unroll
                 for (int ks = 0; ks < kDim / 16; ++ks) {
                     const uint64_t off = (uint64_t)((ks >> 2) * (kHalfBytes >> 4) + 2 * (ks & 3));
-                    umma_f16(tmem + (uint32_t)(i * kKeys + h * (kKeys / 2)), a_desc + off, b_desc + off, kIdescS, ks > 0 ? 1u : 0u);
+                    umma_f16(t_s + (uint32_t)(h * (kKeys / 2)), q_desc + off, b_desc + off, kIdescS, ks > 0 ? 1u : 0u);
                 }
                 umma_commit(&s_full[i][h]);
             };
-            if (n_blocks > 0 && wait_one(&k_first, 0)) {
+            if (my_blocks > 0 && wait_one(&k_first, 0)) {
                 tc_fence_after();
-                for (int h = 0; h < 2; ++h)
-                    for (int i = 0; i < kTiles; ++i) if (nb_t[i] > 0) issue_s(i, h, 0);
+                for (int h = 0; h < 2; ++h) issue_s(h, 0);
             }
             for (int kb = 0; kb < n_blocks && !failed; ++kb) {
                 const int st = kb & 1;
                 if (!wait_one(&full[st], (uint32_t)(kb >> 1) & 1u)) break;
+#pragma unroll 1
+                for (int h = 0; h < 2 && kb < my_blocks; ++h) {
+                    if (!wait_one(&p_full[i][h], (uint32_t)kb & 1u)) break;
+                    tc_fence_after();
+                    const uint64_t b_desc = v_desc + (uint64_t)(((2 * st + h) * kVHalf) >> 4);
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < kTiles; ++i) {
-                        if (kb < nb_t[i] && !failed) {
-                            if (!wait_one(&p_full[i][h], (uint32_t)kb & 1u)) break;
-                            tc_fence_after();
-                            const uint64_t b_desc = make_smem_desc(sV + st * 2 * kVHalf + h * kVHalf);
-#pragma unroll
-                            for (int ks = 0; ks < kKeys / 32; ++ks)
-                                umma_bf16_ts(tmem + kOCol + (uint32_t)i * kDim, tmem + (uint32_t)(i * kKeys + h * (kKeys / 2)) + 8u * ks, b_desc + (uint64_t)(2 * ks), kIdescO,
-                                             (kb > 0 || h > 0 || ks > 0) ? 1u : 0u);
-                            if (kb == nb_t[i] - 1) umma_commit(h ? &o_full[i] : &o_first[i]);
-                            if (kb + 1 < nb_t[i]) issue_s(i, h, kb + 1);
-                        }
-                    }
+                    for (int ks = 0; ks < kKeys / 32; ++ks)
+                        umma_bf16_ts(t_o, t_s + (uint32_t)(h * (kKeys / 2)) + 8u * ks, b_desc + (uint64_t)(2 * ks), kIdescO, (kb > 0 || h > 0 || ks > 0) ? 1u : 0u);
+                    if (kb == my_blocks - 1) umma_commit(h ? &o_full[i] : &o_first[i]);
+                    if (kb + 1 < my_blocks) issue_s(h, kb + 1);
+                }
                 if (!failed) umma_commit(&empty[st]);
             }
             if (failed) {   // products in flight read shared and tensor memory: let them end before the CTA does
-                umma_commit(&drained);
-                mbar_wait_parked(smem_u32(&drained), 0, params.wait_limit);
+                umma_commit(&drained[i]);
+                mbar_wait_parked(smem_u32(&drained[i]), 0, params.wait_limit);
                 atomicExch(p.status, 3);
             }
         }
