@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(kMergers * kDim / 4) kv8_merge_kernel(const Kv
 
 // Whether the rows of tiles are faster one by one than a tile at a time, from estimates in us. One by one: a wave of CTAs (row x kv head) takes 3 us and what its
 // longest row does; a tile takes about 12 us, and 2.3 for every 128 keys. (One prompt, 32 / 8 heads of 128: 16 tokens 4.0 against 12.2 us, 128 12.7 against
-// 16.9, 256 26 against 19.6; 8 / 1 heads: 512 tokens 13.6 against 24, 2048 86 against 52.)
+// 16.9, 256 26 against 19; 8 / 1 heads: 512 tokens 13.6 against 24, 2048 86 against 46.)
 bool rows_one_by_one(const gptrs_kv8_cache& c, int64_t rows, int64_t n_tiles, int64_t max_len) {
     const int64_t seen = c.window > 0 ? std::min<int64_t>(max_len, c.window) : max_len, pairs = c.kv_heads * ((c.q_heads / c.kv_heads + kCols - 1) / kCols);
     if (n_tiles * c.tile_tokens > 65535) return false;
@@ -498,10 +498,11 @@ extern "C" {
 int gptrs_cuda_kv8_splits(const gptrs_kv8_cache* c, int64_t rows, int64_t n_tiles, int64_t max_ctx_len) {
     if (!c || rows < 1 || c->kv_heads < 1) return 1;
     if (n_tiles > 0) {
-        // a CTA per tile and kv head has an SM to itself: parts only where many SMs would have nothing, of 4096 keys at least (one prompt of 2048 tokens, 8 / 1
-        // heads of 128: one part 52 us, two 62; 500 tokens behind 32768, 32 / 8 heads: NN, two 378)
+        // a CTA per tile and kv head has an SM to itself: parts only where SMs would have nothing, at most one wave of them, of 1024 keys at least (us with 1 / 2 /
+        // 4 / 8 parts: 500 tokens behind 32768, 32 / 8 heads of 128, 64 CTAs: 515 / 288 / 303 / -; 128 behind 8192: 136 / 84 / 55 / 42; 512 behind 16384, 8 / 1
+        // heads: 343 / 143 / 84 / 56; 2048 behind nothing: 46 / 46 / 58 / -; 1024 behind nothing: 31 / 33 / 30 / -)
         const int64_t ctas = n_tiles * c->kv_heads, keys = c->window > 0 ? std::min<int64_t>(max_ctx_len, c->window + c->tile_tokens) : max_ctx_len;
-        return rows > 65535 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(sm_count() / ctas, keys / 4096));
+        return rows > 65535 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(sm_count() / ctas, keys / 1024));
     }
     const int64_t seen = c->window > 0 ? std::min<int64_t>(max_ctx_len, c->window + kKv8Tokens) : max_ctx_len;
     const int64_t blocks = (seen + kKv8Tokens - 1) / kKv8Tokens;

@@ -4,17 +4,24 @@
 // become f16 in shared memory (exact), the scales of a block of 16 keys meet the scores of its 16 columns, so the matrix products see no scale.
 //
 // One CTA (one per SM) takes the rows of a tile x the query heads of one kv head, as two row tiles of 128 (row = token x group + head), and walks
-// the visible keys in blocks of 128 (8 pages):
-//   S_i[128 x 128] = Q_i . K^T     both operands f16 in shared memory (K-major, 128-byte swizzle), accumulator in tensor memory
+// the visible keys in blocks of 128 (8 pages), two halves of 64 keys in flight on their own (h):
+//   S_ih[128 x 64] = Q_i . K_h^T   both operands f16 in shared memory (K-major, 128-byte swizzle), accumulator in tensor memory
 //   softmax                        warps 4 i .. 4 i + 3, a thread per row, in one pass over its scores: the reference M stays what it is until a weight would
 //                                  no longer be an f16 (a page's weights add up to more than 2^15), so there is no pass for the maximum. Weights
-//                                  go as f16 over the first 64 columns of S_i; a quarter of the exponentials is computed on the multiply-add
-//                                  units, which have more room than the special function unit
-//   O_i[128 x dim] += P_i . V      A = P_i from tensor memory, B = V^T in shared memory (keys contiguous), accumulator in tensor memory
-// Warp 12 issues every product; warps 8 - 11 widen the pages, two of a block each: bytes from global memory to registers ahead of time, f16 into the
-// stage when the products that read it are complete. A thread of theirs takes the 16 bytes that the row kernel's lane would; which 16
-// is chosen so that eight (K) or sixteen (V) threads store to different banks. The order of the keys inside a page is the cache's
-// (pairs 0, 1, 8, 9, 2, 3, ...): P's columns are written in the same order.
+//                                  go as f16 over the first 32 columns of S_ih
+//   O_i[128 x dim] += P_ih . V_h   A = P_ih from tensor memory, B = V^T in shared memory (keys contiguous), accumulator in tensor memory
+// Warps 8 - 11 widen the pages, two of a block each: bytes from global memory to registers ahead of time, f16 into the stage when the products that read
+// it are complete. A thread of theirs takes the 16 bytes that the row kernel's lane would; which 16 is chosen so that eight (K) or sixteen (V) threads
+// store to different banks. The order of the keys inside a page is the cache's (pairs 0, 1, 8, 9, 2, 3, ...): P's columns are written in the same
+// order. Warps 12 and 13 issue the products of a row tile each: behind P_ih come O_i += P_ih . V_h and the next block's S_ih, while the softmax is at the
+// other half. One thread for both tiles had the one wait for the other's weights (547 us for the prompt below).
+//
+// One prompt of 16384 tokens, 32 / 8 heads of 128: 524 us, 1049 TFLOP/s (64 % of what a large bf16 product of the library reaches); 500 tokens behind
+// 32768: 288 us; seven ragged prompts of 91 - 1777 tokens, 12 heads of 64: 62 us. What bounds it is the softmax warps' chain: a half takes a warp about
+// 1700 cycles (1150 of weights, 230 until the scores are seen, 150 of storing them), of which the special function unit needs 512 for each of the two
+// warps of a scheduler; it issues in 45 % of the cycles, a third of that for the loaders, and the tensor pipe is busy for 40 %. Measured and left: two
+// threads a row (16 softmax warps, 667 us where one had 606), eight loader warps (539), an eighth of the exponentials as a polynomial on the
+// multiply-add units (519, and 292 where the chunk takes 288), whole blocks of scores instead of halves (690).
 // Every wait is bounded: on a timeout code 3 goes to the status word and every role leaves its loop.
 #include <type_traits>
 
@@ -81,20 +88,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
     return d;
-}
-// 2^t of a pair on the multiply-add units: t = n + f with f in [-1/2, 1/2], 2^f by the cubic that is nearest to it in relative error there (7.5e-5,
-// a sixth of f16's rounding), n added to the exponent. t is held to -126 .. 127.
-__device__ __forceinline__ float2 exp2_pair(uint64_t t2) {
-    const float2 t = split(t2);
-    const uint64_t x = pair_of(fminf(fmaxf(t.x, -126.f), 127.f), fminf(fmaxf(t.y, -126.f), 127.f));
-    const uint64_t y = add2(x, pair_of(12582912.f, 12582912.f));                    // 1.5 * 2^23: n in the lowest bits
-    const uint64_t n = add2(y, pair_of(-12582912.f, -12582912.f));
-    const uint64_t f = fma2(n, pair_of(-1.f, -1.f), x);
-    uint64_t p = fma2(f, pair_of(0.05517166853f, 0.05517166853f), pair_of(0.24261112511f, 0.24261112511f));
-    p = fma2(p, f, pair_of(0.69326096773f, 0.69326096773f));
-    p = fma2(p, f, pair_of(0.99992805719f, 0.99992805719f));
-    const float2 m = split(p), k = split(y);
-    return make_float2(__int_as_float(__float_as_int(m.x) + (__float_as_int(k.x) << 23)), __int_as_float(__float_as_int(m.y) + (__float_as_int(k.y) << 23)));
 }
 __device__ __forceinline__ void st_shared_v2(uint32_t addr, uint32_t a, uint32_t b) {
     asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(addr), "r"(a), "r"(b) : "memory");
@@ -503,13 +496,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {   // keys 2 i, 2 i + 1
                         const uint64_t t2 = fma2(pair_of(__uint_as_float(s[16 * pg + 2 * i]), __uint_as_float(s[16 * pg + 2 * i + 1])), c2, b2);
-                        float2 w;
-                        if (kWhole && (i & 7) == 7) {
-                            w = exp2_pair(t2);
-                        } else {
-                            const float2 t = split(t2);
-                            w = make_float2(kv8_exp2(t.x), kv8_exp2(t.y));
-                        }
+                        const float2 t = split(t2);
+                        float2 w = make_float2(kv8_exp2(t.x), kv8_exp2(t.y));
                         if (!kWhole) {
                             const int key = key0 + 16 * pg + 2 * i;
                             w.x = key >= begin && key < end ? w.x : 0.f;
@@ -562,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             if (!mbar_wait_parked(smem_u32(&o_full[ti]), 0, params.wait_limit)) failed = true;
             failed = __any_sync(0xffffffffu, failed);
         }
-        // a query that is not a number, or scores that are infinite: the row is none (the polynomial knows no NaN)
+        // a query that is not a number, or scores that are infinite: the row is none
         if (end > begin && my_blocks > 0 && (q_scale != q_scale || m_run == INFINITY)) l_run = __uint_as_float(0x7fc00000u);
         const long long at = (long long)my_row * p.q_heads + my_head;
         if (!failed && p.splits == 1) {
