@@ -1,10 +1,14 @@
 // Append to the 8-bit cache (norm and rotation of queries and keys on the way), and reading tokens back.
 //
 // gptrs_cuda_kv8_append: a CTA takes the rows of a run that fall into one block (16 tokens) x one kv head with its query heads; it finds them from the last
-// of these rows, which lies in the 16 rows (of short lists, the one row) it looks at. Queries go by eight pairs a
-// lane, with the products of gains and angles made once per row; keys and values by four (what bounds long lists is the number of instructions beside latency). What bounds it is the latency of loads that depend on each other (slot and position; angles; open rows), so keys, values, the
-// first queries and the angles (kept in shared memory) are asked for before anything is computed; for runs of one row (decode steps) with the rows in front of
-// it in its block. A block is written once, by the CTA with its last token: the largest magnitude over the CTA, then the bytes in order in shared memory.
+// of these rows, which lies in the 16 rows (of short lists, the one row) that it looks at. Queries go by eight pairs a lane, with the products of gains and
+// angles made once per row; keys and values by four. A block is written once, by the CTA with its last token: the largest magnitude over the CTA, then the
+// bytes in order in shared memory; for runs of one row (decode steps) with the rows in front of it in its block, from the open rows.
+// What bounds it is latency: of loads that depend on each other (slot and position; angles; open rows), so keys, values, the first queries and the angles
+// (kept in shared memory) are asked for before anything is computed, and of the arithmetic behind them. 64 single tokens, 32 / 8 heads of 128: 4.4 us; six
+// prompts of 2777 tokens, 16 / 4 heads, three axes: 58.6 us (148 MB, 39 % of the copy bandwidth; 38.6 us without the queries and the blocks; a warp
+// instruction per scheduler in 44 % of the cycles, four CTAs an SM). Measured and left: CTAs that stay and fetch ahead into L2 (62.9), CTAs for queries
+// and for keys apart (65.1).
 #include "kv8_cache.cuh"
 #include "qk_rotate.cuh"
 
@@ -261,8 +265,10 @@ __global__ void __launch_bounds__(kThreads, 4) kv8_append_kernel(const AppendPar
         else
             ends = position_i % kKv8Tokens == kKv8Tokens - 1 || row_i == last_i;
     }
-    for (uint32_t todo = __ballot_sync(0xffffffffu, ends); todo; todo &= todo - 1) {
+    const uint32_t segments = __ballot_sync(0xffffffffu, ends);
+    for (uint32_t todo = segments; todo; todo &= todo - 1) {
         const int from = __ffs(todo) - 1, row_b = row0 + from;
+        if (kTile > 1 && __popc(segments & ((1u << from) - 1u)) % gridDim.z != blockIdx.z) continue;   // another CTA's
         const int slot = __shfl_sync(0xffffffffu, slot_i, from), position = __shfl_sync(0xffffffffu, position_i, from), first = __shfl_sync(0xffffffffu, first_i, from),
                   last = __shfl_sync(0xffffffffu, last_i, from);
         const int block = position / kKv8Tokens, token_b = position % kKv8Tokens, row_a = max(first, row_b - token_b), token_a = token_b - (row_b - row_a), n = row_b - row_a + 1;
@@ -492,8 +498,12 @@ int gptrs_cuda_kv8_append(const gptrs_kv8_cache* c, const gptrs_kv8_append_step*
     p.q = static_cast<__nv_bfloat16*>(s->d_q);
     p.status = s->d_status;
     p.rows = (int)s->rows; p.q_heads = c->q_heads; p.kv_heads = c->kv_heads; p.group = c->q_heads / c->kv_heads;
-    const bool few = s->rows <= 1024;   // (which are often runs of one row)
-    const dim3 grid((unsigned)ceil_div(s->rows, few ? 1 : kKv8Tokens), (unsigned)c->kv_heads);
+    // A CTA per row and kv head for lists that are short or may be single tokens, else per 16 rows: a prompt has one segment in them. Where they are single tokens
+    // after all, four CTAs deal the segments among them, as long as the three that find nothing cost little. us, 32 / 8 heads of 128, per row / per 16 / four
+    // for 16: 64 single tokens 4.2 / 64 / 20, 512 14 / 66 / 44; a prompt of 256 10.9 / 7.8 / 8.4, of 1000 23 / 10.4 / 11.0, of 4 x 1000 62 / 35 / 31, of
+    // 6 x 2777 - / 105 / 120.
+    const bool few = s->rows <= 256 || s->rows <= s->n_slots;
+    const dim3 grid((unsigned)ceil_div(s->rows, few ? 1 : kKv8Tokens), (unsigned)c->kv_heads, few || s->rows > 4096 ? 1u : 4u);
     auto kernel = c->dim == 64 ? (few ? kv8_append_kernel<64, 1> : kv8_append_kernel<64, 16>) : (few ? kv8_append_kernel<128, 1> : kv8_append_kernel<128, 16>);
     return launch_kernel(kernel, grid, dim3(kThreads), 0, as_stream(stream), 1, p);
 }

@@ -194,6 +194,49 @@ def test_append_writes_these_bytes(cuda, heads, kv, dim, runs):
     c.check_bytes()
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (3, 3, 64)])
+@pytest.mark.parametrize("prompts", [[150, 90], [2500, 1800], []])
+def test_single_tokens_beside_prompts(cuda, heads, kv, dim, prompts):
+    """Many runs of one row between long ones, some of them in the middle of a block: lists that are short, longer than the slots, and long."""
+    c = Cache(cuda, heads, kv, dim, 40, 320, seed=sum(prompts) + dim)   # (9 + 2 x 2500 tokens: 314 blocks)
+    singles = list(range(len(prompts), 40))
+    c.append([(i, 0, 1 + (7 * i) % 33) for i in singles] + [(i, 0, 9) for i in range(len(prompts))])
+    for turn in range(2):
+        at = {i: 1 + (7 * i) % 33 + turn for i in singles}
+        runs = [(i, at[i], 1) for i in singles]
+        for i, n in enumerate(prompts):
+            runs.insert(5 + 17 * i, (i, 9 + turn * n, n))
+        qkv, q = c.append(runs, pad=(3,))
+        q, flat = q.flatten(1), qkv[:, :heads * dim]
+        pad = sum(n for _, _, n in runs[:3])
+        assert (q[pad] == 5).all() and torch.equal(q[:pad], flat[:pad]) and torch.equal(q[pad + 1:], flat[pad + 1:])
+        c.check_bytes()
+    assert int(c.status) == 0
+
+
+def test_bad_rows_among_many(cuda):
+    """The same where sixteen rows go together: what is bad is reported, the others arrive."""
+    c = Cache(cuda, 4, 2, 64, 3, 22)
+    n = 310
+    slot, pos = [0] * n + [7] * 20 + [1] * 17 + [2] * 16, list(range(n)) + list(range(20)) + list(range(17)) + list(range(-1, 15))
+    first = [0] * n + [n] * 20 + [n + 20] * 17 + [n + 37] * 16
+    last = [n - 1] * n + [n + 19] * 20 + [n + 36] * 17 + [n + 52] * 16
+    rows = len(slot)
+    qkv = torch.randn((rows, 8 * 64), device=cuda).bfloat16()
+    before = c.pool.clone()
+    ops.kv8_append(c.a, None, qkv, _ints(pos, cuda), _ints(slot, cuda), _ints(first, cuda), _ints(last, cuda), c.table, c.pool, c.rows, status=c.status)
+    assert int(c.status) == 2
+    x = _np(qkv).reshape(rows, -1, 64)
+    for s, at, m in ((0, 0, n), (1, n + 20, 17)):
+        c.seq[s].append(0, x[at:at + m, 4:6], x[at:at + m, 6:8])
+        for b in range(max(0, (m - 1) // 16 - 1), (m - 1) // 16 + 1):
+            c.halves[s][b % 2] = b
+    c.check_bytes()
+    table = c.table.cpu().numpy()
+    others = [i for i in range(before.shape[0]) if i not in list(table[0, :n // 16]) + [table[1, 0]]]
+    assert torch.equal(c.pool[others], before[others])
+
+
 @pytest.mark.parametrize("step", [1, 3, 16, 21, 37, 300])
 def test_cuts_do_not_matter(cuda, step):
     """The same tokens in calls of any size leave the same bytes; both sequences at once, out of step."""
