@@ -1,11 +1,15 @@
 // Norms of queries and keys per head and their rotation in one pass, positions on several axes (see qk_rotate.cuh).
 //
-// A warp takes some heads of one kind (queries, keys, values) of a row, a group of its lanes a head at a time, kVec pairs a lane, so that loads and stores are
-// 16 bytes a lane. With gains g and angles (c, s), out_a = x_a r g_a c - x_b r g_b s and out_b = x_b r g_b c + x_a r g_a s: the four products of gains and
-// angles are made once for the warp's heads. The next head is on its way while one is worked on. What bounds it is the number of instructions (about
-// five per value) beside bandwidth; versions with more of them per value (four pairs a lane, gains and angles apart) took 60 - 90 us where this takes
-// NN: 9001 rows of 32 + 8 + 8 heads of 128 in bf16, three axes. Sizes that do not come in such pieces go pair by pair (up to 512 channels).
-// Every value is read and written once; the norm is f32, the result is rounded once.
+// With gains g and angles (c, s), out_a = x_a r g_a c - x_b r g_b s and out_b = x_b r g_b c + x_a r g_a s, r = 1 / rms of the head. Every value is read and
+// written once; sums of squares are f32, the result is rounded once. 9001 rows of 32 + 8 + 8 heads of 128 in bf16 on three axes: 43.4 us (28.2 at the copy
+// bandwidth for the queries and keys alone, which are all that is written in place; a plain copy of the same bytes takes 35).
+//
+// Three kernels. qk_norm_rope_ring_kernel streams rows through shared memory. qk_norm_rope_wide_kernel holds them in registers: a warp takes some heads of one
+// kind (queries, keys, values) of a row, a group of its lanes a head at a time, kVec pairs a lane, so that loads and stores are 16 bytes a lane; the four
+// products of gains and angles are made once for the warp's heads, and the next head is on its way while one is worked on. What holds it up is that little is
+// on its way beside the instructions. us, 32 / 8 heads of 128, ring / wide: bf16, three axes, 1 row 3.3 / 3.4, 148 3.4 / 4.2, 2000 13.4 / 20.6, 9001 43.4 /
+// 69.2; f32, one axis, 1 row 3.3 / 2.5, 64 3.6 / 3.0, 148 3.8 / 4.2, 2000 22.3 / 25.1: so the ring is taken but for few rows of f32. Sizes that do not come
+// in pieces of four go pair by pair (up to 512 channels).
 #include <algorithm>
 
 #include "qk_rotate.cuh"
@@ -186,15 +190,15 @@ __global__ void __launch_bounds__(kThreads, 2) qk_norm_rope_wide_kernel(const No
     }
 }
 
-// The same for many rows. Rows come into a ring in shared memory by bulk copies, are worked on in place and leave by bulk copies, so that what is on its way
+// Rows come into a ring in shared memory by bulk copies, are worked on in place and leave by bulk copies, so that what is on its way
 // needs no registers; angles (a chain of loads: axis, position, table) are put beside them by warps of their own, which also ask for the rows. A thread keeps its
-// channels' gains over all rows where every lane group has one head.
+// channels' gains over all rows where every lane group has one head. A row is at most a stage of 24 KB: four of them and three CTAs fill an SM
+// for rows of up to 18 KB.
 constexpr int kRing = 4, kRingThreads = 384, kMostAngleThreads = 128, kRingCtas = 3;   // CTAs: of an SM
 struct RingParams {
     NormRopeParams n;
     long long rows;
     int row_bytes, store_bytes, stage_bytes, angle_threads, groups;
-    uint32_t wait_limit;
 };
 template <typename T, int kVec, bool kNeighbours>
 __global__ void __launch_bounds__(kRingThreads, kRingCtas) qk_norm_rope_ring_kernel(const RingParams q) {
@@ -413,7 +417,8 @@ int launch_norm_rope(NormRopeParams& p, int64_t rows, cudaStream_t st) {
     };
     constexpr int kPiece = 16 / sizeof(T);
     const int64_t row_bytes = (int64_t)(r.q_heads + 2 * r.kv_heads) * r.dim * sizeof(T);
-    if (rows >= 2 * (int64_t)sm_count() && in_pieces(kPiece) && row_bytes <= 24576 && r.rot_half <= kMostAngleThreads) return launch_ring<T, kPiece>(p, rows, (int)row_bytes, st);
+    const bool many = sizeof(T) == 2 || rows >= sm_count();
+    if (many && in_pieces(kPiece) && row_bytes <= 24576 && r.rot_half <= kMostAngleThreads) return launch_ring<T, kPiece>(p, rows, (int)row_bytes, st);
     if (sizeof(T) == 2 && in_pieces(8)) return launch_wide<T, sizeof(T) == 2 ? 8 : 4>(p, rows, st);
     if (in_pieces(4)) return launch_wide<T, 4>(p, rows, st);
     p.lanes = lanes_of(r.dim / 2);

@@ -724,7 +724,7 @@ typedef struct {
 } gptrs_qk_rotation;
 /* qkv rows (f32 or bf16, ld_in apart, 0 = packed) -> the same rows with queries and keys normed and rotated, rounded once. d_out may be
  * d_qkv with the same stride; otherwise the values are copied. dim even, at most 512. A position outside the tables or an axis that does
- * not exist sets *d_status = 2 and turns by position 0. */
+ * not exist sets *d_status = 2 and turns by position 0; 3: a bounded wait ran out. */
 int gptrs_cuda_qk_norm_rope(const gptrs_qk_rotation* r, const void* d_qkv, int dtype, int64_t ld_in, const int32_t* d_positions, void* d_out,
                             int64_t ld_out, int32_t* d_status, int64_t rows, void* stream);
 
@@ -783,9 +783,9 @@ int gptrs_cuda_kv8_gather(const gptrs_kv8_cache* c, const void* d_pool, int64_t 
 /* out [rows][q_heads][dim] (bf16) = softmax over the visible keys . values; row t belongs to slot[t] and sees the last `window` of its first
  * ctx_len[t] tokens (the cache as it is behind the append). A row that sees nothing gives zeros, one with a negative slot is left as it was.
  * n_tiles = 0: every row by itself (single tokens of many sequences); else tile i is the rows tile_row[i] .. + tile_rows[i], at most tile_tokens
- * rows of one sequence at consecutive positions (prompts, chunks of prompts); rows in no tile are left as they were, no row is in two. The keys of a row or tile are read in at most `splits` parts
- * (gptrs_cuda_kv8_splits; scratch: gptrs_cuda_kv8_scratch_bytes). max_ctx_len bounds ctx_len. *d_status = 2: a length, slot or
- * page out of range, 3: a bounded wait ran out. */
+ * rows of one sequence at consecutive positions (prompts, chunks of prompts); rows in no tile are left as they were, no row is in two. Tiles are
+ * begun from the last one on. The keys of a row or tile are read in at most `splits` parts (gptrs_cuda_kv8_splits; scratch:
+ * gptrs_cuda_kv8_scratch_bytes). max_ctx_len bounds ctx_len. *d_status = 2: a length, slot or page out of range, 3: a bounded wait ran out. */
 typedef struct {
     const void* d_q;                   /* [rows][q_heads][dim], rows ldq apart (0 = packed) */
     int64_t ldq;

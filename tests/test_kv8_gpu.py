@@ -75,6 +75,13 @@ def test_norm_rope(cuda, dtype, heads, kv, dim, pairs, rows, gains, neighbours, 
     assert (wide[:, :8] == 7).all() and (wide[:, 8 + width:] == 7).all() and (to[:, :3] == 9).all() and (to[:, 3 + width:] == 9).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim,pairs,rows,gains,neighbours,axes", [  # pieces of eight bytes in bf16; rows that no stage of the ring holds; few and many rows
+    (6, 2, 64, 20, 50, True, False, 3), (3, 1, 72, 36, 301, True, True, 1), (64, 8, 128, 64, 149, True, False, 1), (96, 8, 128, 48, 307, True, True, 2), (32, 8, 128, 64, 147, True, False, 1)])
+def test_norm_rope_in_other_pieces(cuda, dtype, heads, kv, dim, pairs, rows, gains, neighbours, axes):
+    test_norm_rope(cuda, dtype, heads, kv, dim, pairs, rows, gains, neighbours, axes)
+
+
 def test_norm_rope_positions_outside_and_channels_that_stay(cuda):
     rng = np.random.default_rng(3)
     rot, pos, c, s, _ = _rotation(rng, 2, 1, 64, 16, 4, cuda, False, False, 1)
