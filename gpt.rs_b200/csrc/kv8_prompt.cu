@@ -126,7 +126,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     const int row0 = kv8_row(p, tile * p.tile_tokens);   // (tile_tokens: 2 tq)
     if (row0 < 0) return;
     const int n_rows = p.tile_rows[tile];
-    const int slot = p.slot[row0];
+    int slot = p.slot[row0];
+    if (slot >= p.n_slots) slot = -1;   // (the rows' spans report it)
 
     if (tid == 0) {
         mbar_init(&k_first, kLoadWarps);
@@ -143,18 +144,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_holder)), "r"(kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = tmem_holder;
-    pdl_launch_dependents();   // every CTA of this grid holds its tensor memory (or has left)
-
     // ---- a softmax thread's row ------------------------------------------------------------------------------------------------------------
     const int in_tile = ti * tq + row / group, my_row = row0 + in_tile, my_head = kv_head * group + row % group;
     bool live = is_softmax && row < tq * group && in_tile < n_rows;   // the output of this row is this thread's
     int begin = 0, end = 0;
     float q_scale = 0.f;
     if (is_softmax) {
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + (live ? my_row : row0) * p.ldq + (long long)my_head * kDim);
+        uint4 v[kDim / 8];
+#pragma unroll
+        for (int c = 0; c < kDim / 8; ++c) v[c] = live ? __ldg(src + c) : make_uint4(0, 0, 0, 0);   // (on its way beside the span)
         if (live) {
             const Kv8Span s = kv8_span(p, my_row);
             live = s.slot >= 0 && s.slot == slot;
@@ -164,12 +163,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         const int warp_begin = __reduce_min_sync(0xffffffffu, end > begin ? begin : 0x7fffffff), warp_end = __reduce_max_sync(0xffffffffu, end > begin ? end : 0);
         if (lane == 0) { s_begin[warp] = warp_begin; s_end[warp] = warp_end; }
         // ---- its query: f16 with a power of two in front (kv8_cache.cuh) -> shared memory --------------------------------------------------------
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + (live ? my_row : row0) * p.ldq + (long long)my_head * kDim);
-        uint4 v[kDim / 8];
         uint32_t big = 0;
 #pragma unroll
         for (int c = 0; c < kDim / 8; ++c) {
-            v[c] = live ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+            if (!live) v[c] = make_uint4(0, 0, 0, 0);
             big = __vmaxu2(big, __vmaxu2(abs_bits_max2(v[c].x, v[c].y), abs_bits_max2(v[c].z, v[c].w)));
         }
         const int e = pow2_exponent(widest_half(big));
@@ -182,7 +179,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                          bf16x2_to_f16x2(v[c].z, factor), bf16x2_to_f16x2(v[c].w, factor));
         fence_proxy_async();
     }
+    tc_fence_before();
     __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_holder;
+    pdl_launch_dependents();   // every CTA of this grid holds its tensor memory (or has left)
     // keys of this CTA: [first_key, last_key) of the tile, whole blocks of the split's share; nb_t[i] of them for row tile i
     int tile_end[kTiles], first_key = 0x7fffffff, last_key = 0;
 #pragma unroll

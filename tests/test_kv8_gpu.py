@@ -454,6 +454,18 @@ def test_bad_entries_of_the_attention_are_reported(cuda):
             c.check(rows[:1], q[:1], out[:1])
 
 
+@pytest.mark.parametrize("slot", [2, 1 << 30])
+@pytest.mark.parametrize("splits", [None, 2])
+def test_tiles_of_no_sequence_are_reported(cuda, slot, splits):
+    """A tile whose slot is none: nothing is looked up with it, the other tile's rows are right."""
+    c = Cache(cuda, 4, 2, 64, 2, 12)
+    c.fill([190, 60])
+    rows = [(0, i + 1) for i in range(60, 190)] + [(slot, i + 1) for i in range(20)]
+    q, out = c.attend(rows, tiles=[130, 20], splits=splits, want=False)
+    assert int(c.status) == 2
+    c.check(rows[:130], q[:130], out[:130])
+
+
 def test_positions_past_32_bits_of_bytes(cuda):
     """Pages whose bytes lie more than 4 GB into the pool, and a page table row far into its table."""
     c = Cache(cuda, 8, 8, 128, 1, 4)
