@@ -179,29 +179,95 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                          bf16x2_to_f16x2(v[c].z, factor), bf16x2_to_f16x2(v[c].w, factor));
         fence_proxy_async();
     }
+    // ---- what a loader's thread does (warps 8 - 11: pages 2 w, 2 w + 1 of every block) -------------------------------------------------------
+    int first_key = 0x7fffffff, last_key = 0, n_blocks = 0, length = 0, end_block = 0;   // of this CTA: keys [first_key, last_key), blocks of 128; tokens, blocks of 16
+    // whole blocks of the split's share of a tile's keys
+    auto cut = [&](int from, int to) {
+        first_key = from; last_key = to; n_blocks = 0;
+        if (last_key <= 0) return;
+        first_key = first_key / kKv8Tokens * kKv8Tokens;
+        const int all = (last_key - first_key + kKeys - 1) / kKeys, per = (all + p.splits - 1) / p.splits, skip = min((int)blockIdx.z * per, all);
+        n_blocks = min(per, all - skip);
+        first_key += skip * kKeys;
+        end_block = (last_key + kKv8Tokens - 1) / kKv8Tokens;
+    };
+    const int w = warp - kLoadWarp;
+    const int kg = lane >> 3, kc = (lane >> 2) & 1, t = lane & 3;           // K: token, chunk of 32 channels, eight channels
+    const int vg = 2 * ((lane & 15) >> 2) + (lane >> 4);                    // V: channel, four tokens
+    enum { kNone, kClosed, kOpen };
+    struct Page { const unsigned char* at; int block, kind; };
+    auto block_of = [&](int kb, int j) { return first_key / kKv8Tokens + kb * kPages + 2 * w + j; };
+    // entry of the page table, asked for a block before it is needed (the load is not waited for here)
+    auto number = [&](int kb, int j) {
+        const int block = block_of(kb, j);
+        return block < end_block && (block + 1) * kKv8Tokens <= length ? p.table[slot * p.max_pages + block] : 0;
+    };
+    auto find = [&](int kb, int j, int page) {
+        Page pg = {nullptr, block_of(kb, j), kNone};
+        if (pg.block >= end_block) return pg;
+        if ((pg.block + 1) * kKv8Tokens > length) { pg.kind = kOpen; return pg; }
+        if (page < 0 || page >= p.n_pages) { atomicExch(p.status, 2); return pg; }
+        pg.at = p.pool + ((long long)page * p.kv_heads + kv_head) * kv8_block_bytes(kDim);
+        pg.kind = kClosed;
+        return pg;
+    };
+    uint4 kb_[2][kC], vb_[2][kC];
+    float2 sc[2];
+    auto load_k = [&](const Page (&pg)[2]) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            if (pg[j].kind != kClosed) continue;
+            sc[j] = __ldg(reinterpret_cast<const float2*>(pg[j].at + 32 * kDim));
+#pragma unroll
+            for (int i = 0; i < kC; ++i)   // two channel chunks and tokens kg, kg + 4 of them
+                kb_[j][i] = __ldg(reinterpret_cast<const uint4*>(pg[j].at + ((i >> 1) * 2 + kc) * 512 + ((kg + 4 * (i & 1)) * 4 + t) * 16));
+        }
+    };
+    auto load_v = [&](const Page (&pg)[2]) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            if (pg[j].kind != kClosed) continue;
+#pragma unroll
+            for (int i = 0; i < kC; ++i) vb_[j][i] = __ldg(reinterpret_cast<const uint4*>(pg[j].at + 16 * kDim + i * 512 + (vg * 4 + t) * 16));
+        }
+    };
+    Page pages[2], next[2];
+    int numbers[2];
+    int asked_first = -1, asked_last = -1;
+    auto ask_first = [&] {   // for block 0
+#pragma unroll
+        for (int j = 0; j < 2; ++j) pages[j] = find(0, j, number(0, j));
+        load_k(pages);
+        load_v(pages);
+        asked_first = first_key;
+        asked_last = last_key;
+    };
+    if (warp >= kLoadWarp && warp < kMmaWarp && slot >= 0) {
+        // Pages of block 0 are asked for beside the queries: rows come at consecutive positions, so the keys go from the first row's to the last row's. Asked
+        // for again where the rows say otherwise.
+        const int last_row = row0 + n_rows - 1, last_slot = p.slot[last_row];
+        length = p.length[slot];
+        const int first_end = min(min(p.ctx_len[row0], p.max_len), length), last_end = min(min(p.ctx_len[last_row], p.max_len), length);
+        if (last_slot == slot && first_end > 0 && last_end >= first_end) {
+            cut(p.window > 0 ? max(0, first_end - p.window) : 0, last_end);
+            if (n_blocks > 0) ask_first();
+        }
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_holder;
     pdl_launch_dependents();   // every CTA of this grid holds its tensor memory (or has left)
-    // keys of this CTA: [first_key, last_key) of the tile, whole blocks of the split's share; nb_t[i] of them for row tile i
-    int tile_end[kTiles], first_key = 0x7fffffff, last_key = 0;
+    int tile_end[kTiles], from = 0x7fffffff, to = 0, nb_t[kTiles] = {0, 0};   // blocks of row tile i
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
         tile_end[i] = max(max(s_end[4 * i], s_end[4 * i + 1]), max(s_end[4 * i + 2], s_end[4 * i + 3]));
-        last_key = max(last_key, tile_end[i]);
-        first_key = min(first_key, min(min(s_begin[4 * i], s_begin[4 * i + 1]), min(s_begin[4 * i + 2], s_begin[4 * i + 3])));
+        to = max(to, tile_end[i]);
+        from = min(from, min(min(s_begin[4 * i], s_begin[4 * i + 1]), min(s_begin[4 * i + 2], s_begin[4 * i + 3])));
     }
-    int n_blocks = 0, nb_t[kTiles] = {0, 0};
-    if (last_key > 0) {
-        first_key = first_key / kKv8Tokens * kKv8Tokens;
-        const int all = (last_key - first_key + kKeys - 1) / kKeys;
-        const int per = (all + p.splits - 1) / p.splits, skip = min((int)blockIdx.z * per, all);
-        n_blocks = min(per, all - skip);
-        first_key += skip * kKeys;
+    cut(from, to);
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) nb_t[i] = min(n_blocks, max(0, (tile_end[i] - first_key + kKeys - 1) / kKeys));
-    }
+    for (int i = 0; i < kTiles; ++i) nb_t[i] = min(n_blocks, max(0, (tile_end[i] - first_key + kKeys - 1) / kKeys));
     bool failed = false;
     auto wait = [&](uint64_t* bar, uint32_t parity) {   // whole warp
         if (!failed && !mbar_wait_parked(smem_u32(bar), parity, params.wait_limit)) failed = true;
@@ -213,28 +279,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kMmaRegs));
     } else if (warp >= kLoadWarp && warp < kMmaWarp) {
         // ================= warps 8 - 11: pages 2 w, 2 w + 1 of every block ===================================================================
-        const int w = warp - kLoadWarp;
-        const int length = p.length[slot < 0 ? 0 : slot];
-        const int end_block = (last_key + kKv8Tokens - 1) / kKv8Tokens;         // of the sequence's blocks of 16 tokens
-        const int kg = lane >> 3, kc = (lane >> 2) & 1, t = lane & 3;           // K: token, chunk of 32 channels, eight channels
-        const int vg = 2 * ((lane & 15) >> 2) + (lane >> 4);                    // V: channel, four tokens
-        enum { kNone, kClosed, kOpen };
-        struct Page { const unsigned char* at; int block, kind; };
-        auto block_of = [&](int kb, int j) { return first_key / kKv8Tokens + kb * kPages + 2 * w + j; };
-        // entry of the page table, asked for a block before it is needed (the load is not waited for here)
-        auto number = [&](int kb, int j) {
-            const int block = block_of(kb, j);
-            return block < end_block && (block + 1) * kKv8Tokens <= length ? p.table[slot * p.max_pages + block] : 0;
-        };
-        auto find = [&](int kb, int j, int page) {
-            Page pg = {nullptr, block_of(kb, j), kNone};
-            if (pg.block >= end_block) return pg;
-            if ((pg.block + 1) * kKv8Tokens > length) { pg.kind = kOpen; return pg; }
-            if (page < 0 || page >= p.n_pages) { atomicExch(p.status, 2); return pg; }
-            pg.at = p.pool + ((long long)page * p.kv_heads + kv_head) * kv8_block_bytes(kDim);
-            pg.kind = kClosed;
-            return pg;
-        };
         auto open_rows = [&](int block, int is_value) {
             return p.open + (long long)slot * kv8_open_elems(p.kv_heads, kDim) + kv8_open_at(block, p.kv_heads, kv_head, is_value, kDim);
         };
@@ -243,26 +287,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 #pragma unroll 1
             for (int i = lane; i < have * (kDim / 2); i += 32) big = __vmaxu2(big, static_cast<const uint32_t*>(rows)[i] & 0x7fff7fffu);
             return pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big)));
-        };
-        uint4 kb_[2][kC], vb_[2][kC];
-        float2 sc[2];
-        auto load_k = [&](const Page (&pg)[2]) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                if (pg[j].kind != kClosed) continue;
-                sc[j] = __ldg(reinterpret_cast<const float2*>(pg[j].at + 32 * kDim));
-#pragma unroll
-                for (int i = 0; i < kC; ++i)   // two channel chunks and tokens kg, kg + 4 of them
-                    kb_[j][i] = __ldg(reinterpret_cast<const uint4*>(pg[j].at + ((i >> 1) * 2 + kc) * 512 + ((kg + 4 * (i & 1)) * 4 + t) * 16));
-            }
-        };
-        auto load_v = [&](const Page (&pg)[2]) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                if (pg[j].kind != kClosed) continue;
-#pragma unroll
-                for (int i = 0; i < kC; ++i) vb_[j][i] = __ldg(reinterpret_cast<const uint4*>(pg[j].at + 16 * kDim + i * 512 + (vg * 4 + t) * 16));
-            }
         };
         auto store_k = [&](const Page& pg, int j, int kb, uint32_t base) {
             float k_scale = 0.f, v_scale = 1.f;
@@ -341,17 +365,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             }
         };
         // stage kb & 1: V of block kb and K of block kb + 1, which the products of one round read; K of block 0 by itself
-        Page pages[2], next[2];
-        int numbers[2];
         auto store_keys = [&](const Page (&pg)[2], int kb) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) store_k(pg[j], j, kb, sK + (kb & 1) * kKBytes);
         };
         if (n_blocks > 0) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) pages[j] = find(0, j, number(0, j));
-            load_k(pages);
-            load_v(pages);
+            if (first_key != asked_first || last_key != asked_last) ask_first();
 #pragma unroll
             for (int j = 0; j < 2; ++j) numbers[j] = number(1, j);
             store_keys(pages, 0);
