@@ -16,12 +16,14 @@
 // order. Warps 12 and 13 issue the products of a row tile each: behind P_ih come O_i += P_ih . V_h and the next block's S_ih, while the softmax is at the
 // other half. One thread for both tiles had the one wait for the other's weights (547 us for the prompt below).
 //
-// One prompt of 16384 tokens, 32 / 8 heads of 128: 524 us, 1049 TFLOP/s (64 % of what a large bf16 product of the library reaches); 500 tokens behind
-// 32768: 288 us; seven ragged prompts of 91 - 1777 tokens, 12 heads of 64: 62 us. What bounds it is the softmax warps' chain: a half takes a warp about
-// 1700 cycles (1150 of weights, 230 until the scores are seen, 150 of storing them), of which the special function unit needs 512 for each of the two
-// warps of a scheduler; it issues in 45 % of the cycles, a third of that for the loaders, and the tensor pipe is busy for 40 %. Measured and left: two
-// threads a row (16 softmax warps, 667 us where one had 606), eight loader warps (539), an eighth of the exponentials as a polynomial on the
-// multiply-add units (519, and 292 where the chunk takes 288), whole blocks of scores instead of halves (690).
+// One prompt of 8192 tokens, 32 / 8 heads of 128: 521 us, 1055 TFLOP/s (64 % of what a large bf16 product of the library reaches); 500 tokens behind
+// 32768: 288 us; seven ragged prompts of 91 - 1777 tokens, 12 heads of 64: 59.5 us. What bounds long ones is the softmax warps' chain: a half takes a warp
+// about 1700 cycles (1150 of weights, 230 until the scores are seen, 150 of storing them), of which the special function unit needs 512 for each of the two
+// warps of a scheduler; it issues in 39 % of the cycles, a third of that for the loaders, and the tensor pipe is busy for 38 %. Short ones pay 8.5 us per CTA
+// beside their keys: 2 of loads that depend on each other (tile, slot, length), 2 until the first scores, 2 for these (maximum and masks), 1.5 for the
+// output and 1 between CTAs; a half is 0.95 us. Measured and left: two threads a row (16 softmax warps, 667 us where one had 606), eight loader warps (539
+// where four had 518), an eighth of the exponentials as a polynomial on the multiply-add units (519 and, for the chunk, 292, where all on the special
+// function unit took 524 and 288), whole blocks of scores instead of halves (690), first halves without masks where all see them (no difference).
 // Every wait is bounded: on a timeout code 3 goes to the status word and every role leaves its loop.
 #include <type_traits>
 
