@@ -490,6 +490,8 @@ int gptrs_cuda_kv8_append(const gptrs_kv8_cache* c, const gptrs_kv8_append_step*
         p.r.dim = c->dim;
     }
     if (s->rows == 0) return GPTRS_OK;
+    const char *in = static_cast<const char*>(s->d_qkv), *q = static_cast<const char*>(s->d_q);
+    GPTRS_REQUIRE(q >= in + 2 * ((s->rows - 1) * p.ld + width) || in >= q + 2 * s->rows * c->q_heads * c->dim, "queries go into rows that other heads are still read from");
     p.qkv = static_cast<const __nv_bfloat16*>(s->d_qkv);
     p.positions = s->d_positions; p.slot = s->d_slot; p.run_first = s->d_run_first; p.run_last = s->d_run_last; p.table = s->d_page_table;
     p.max_pages = s->max_pages; p.n_pages = s->n_pages; p.n_slots = s->n_slots;

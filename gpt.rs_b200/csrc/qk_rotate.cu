@@ -446,6 +446,11 @@ extern "C" int gptrs_cuda_qk_norm_rope(const gptrs_qk_rotation* r, const void* d
     const bool in_place = d_qkv == d_out;
     GPTRS_REQUIRE(!in_place || p.ld_in == p.ld_out, "in place the strides are the same");
     if (rows == 0) return GPTRS_OK;
+    if (!in_place) {   // rows are worked on in no order: the target may lie between the source's rows, not in them
+        const int64_t size = dtype == GPTRS_F32 ? 4 : 2, apart = ((intptr_t)d_out - (intptr_t)d_qkv) / size, in_end = (rows - 1) * p.ld_in + width, out_end = (rows - 1) * p.ld_out + width;
+        const int64_t shift = p.ld_in == p.ld_out ? (apart % p.ld_in + p.ld_in) % p.ld_in : 0;
+        GPTRS_REQUIRE(apart >= in_end || -apart >= out_end || (shift >= width && shift <= p.ld_in - width), "the target's rows lie in the source's");
+    }
     p.in = d_qkv; p.out = d_out; p.positions = d_positions; p.status = d_status;
     p.copies = !in_place;
     p.heads = r->q_heads + (in_place ? 1 : 2) * r->kv_heads;

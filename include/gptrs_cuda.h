@@ -723,7 +723,7 @@ typedef struct {
     const uint8_t* d_pair_axis;        /* [rot_half]: axis of every pair; NULL: all on the first one */
 } gptrs_qk_rotation;
 /* qkv rows (f32 or bf16, ld_in apart, 0 = packed) -> the same rows with queries and keys normed and rotated, rounded once. d_out may be
- * d_qkv with the same stride; otherwise the values are copied. dim even, at most 512. A position outside the tables or an axis that does
+ * d_qkv with the same stride; otherwise its rows lie in none of d_qkv's, and the values are copied. dim even, at most 512. A position outside the tables or an axis that does
  * not exist sets *d_status = 2 and turns by position 0; 3: a bounded wait ran out. */
 int gptrs_cuda_qk_norm_rope(const gptrs_qk_rotation* r, const void* d_qkv, int dtype, int64_t ld_in, const int32_t* d_positions, void* d_out,
                             int64_t ld_out, int32_t* d_status, int64_t rows, void* stream);
@@ -770,7 +770,7 @@ typedef struct {
     int64_t n_pages;
     void* d_open;
     int64_t n_slots;
-    void* d_q;
+    void* d_q;                         /* not in d_qkv's rows */
     int32_t* d_status;
     int64_t rows;
 } gptrs_kv8_append_step;

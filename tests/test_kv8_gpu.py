@@ -97,6 +97,17 @@ def test_norm_rope_positions_outside_and_channels_that_stay(cuda):
     assert torch.equal(out[:, 32:64].nan_to_num(nan=-5.0), x[:, 32:64].nan_to_num(nan=-5.0))
 
 
+@pytest.mark.parametrize("rows", [3, 400])
+def test_norm_rope_between_the_rows_of_the_source(cuda, rows):
+    rng = np.random.default_rng(rows)
+    rot, pos, c, s, _ = _rotation(rng, 4, 2, 64, 32, rows, cuda, True, False, 1)
+    both = torch.randn((rows, 2 * 512), device=cuda).bfloat16()
+    x = both[:, :512].clone()
+    want = ops.qk_norm_rope(rot, x, _ints(pos, cuda))
+    ops.qk_norm_rope(rot, both[:, :512], _ints(pos, cuda), out=both[:, 512:])
+    assert torch.equal(both[:, :512], x) and torch.equal(both[:, 512:], want)
+
+
 # ---- the cache -----------------------------------------------------------------------------------------------------------------
 class Cache:
     """A cache on the GPU beside the oracle's sequences."""

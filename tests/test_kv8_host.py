@@ -77,6 +77,18 @@ def test_append_refusals():
     assert _status("gptrs_cuda_kv8_append", ctypes.byref(a), ctypes.byref(_append_step(a, rows=0)), None) == 0
 
 
+def test_targets_in_the_source_are_refused():
+    """Rows are worked on in no order, so the target may lie beside or between the source's rows, not in them; rows of 768 f32 or bf16 values."""
+    r, at = _rotation(), 1 << 20
+    for out, ld in [(at + 4 * 4, 0), (at - 4 * 4, 0), (at + 4 * 768 * 4, 0), (at + 767 * 4, 1536), (at + 769 * 4, 1536), (at - 1000 * 4, 1536)]:
+        assert _status("gptrs_cuda_qk_norm_rope", ctypes.byref(r), at, 0, ld, 64, out, ld, 64, 5, None) == SPEC, (out, ld)
+        assert "lie in the source" in gptrs_b200.lib().gptrs_cuda_last_error().decode()
+    a = ops.kv8_layout(8, 2, 64)
+    for d_q in (4096, 4096 + 2 * 768 * 3 + 2 * 752, 4096 - 2 * 512 * 4 + 16):
+        assert _status("gptrs_cuda_kv8_append", ctypes.byref(a), ctypes.byref(_append_step(a, d_q=d_q)), None) == SPEC, d_q
+        assert "queries go into rows" in gptrs_b200.lib().gptrs_cuda_last_error().decode()
+
+
 def test_attention_and_gather_refusals():
     a = ops.kv8_layout(8, 2, 64)
 
