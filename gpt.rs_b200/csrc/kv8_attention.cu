@@ -441,11 +441,21 @@ __global__ void __launch_bounds__(kMergers * kDim / 4) kv8_merge_kernel(const Kv
     *reinterpret_cast<uint2*>(p.out + at * kDim + d) = make_uint2(pack_bf16x2(x.x * r, x.y * r), pack_bf16x2(x.z * r, x.w * r));
 }
 
+// Parts of a row and kv head (of eight of its query heads) that all fit into one wave of CTAs are merged by their cluster; others go one by one, as places
+// come free, and meet in scratch.
+int64_t pairs_of(const gptrs_kv8_cache& c) { return (int64_t)c.kv_heads * ((c.q_heads / c.kv_heads + kCols - 1) / kCols); }
+int64_t places() { return (int64_t)kCtas * sm_count(); }
+bool in_cluster(const gptrs_kv8_cache& c, int64_t rows, int splits) { return splits == 1 || (splits <= kMostRanks && rows * pairs_of(c) * splits <= places()); }
+// One wave of clusters, down to a block per warp.
+int cluster_parts(const gptrs_kv8_cache& c, int64_t rows, int64_t blocks) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>({places() / (rows * pairs_of(c)), kMostRanks, (blocks + kWarps - 1) / kWarps}));
+}
+
 // Whether the rows of tiles are faster one by one than a tile at a time, from estimates in us. One by one: a wave of CTAs (row x kv head) takes 3 us and what its
 // longest row does; a tile takes about 12 us, and 2.3 for every 128 keys. (One prompt, 32 / 8 heads of 128: 16 tokens 4.0 against 12.2 us, 128 12.7 against
 // 16.9, 256 26 against 19; 8 / 1 heads: 512 tokens 13.6 against 24, 2048 86 against 46.)
 bool rows_one_by_one(const gptrs_kv8_cache& c, int64_t rows, int64_t n_tiles, int64_t max_len) {
-    const int64_t seen = c.window > 0 ? std::min<int64_t>(max_len, c.window) : max_len, pairs = c.kv_heads * ((c.q_heads / c.kv_heads + kCols - 1) / kCols);
+    const int64_t seen = c.window > 0 ? std::min<int64_t>(max_len, c.window) : max_len, pairs = pairs_of(c);
     if (n_tiles * c.tile_tokens > 65535) return false;
     const double by_row = (double)((rows * pairs + kCtas * sm_count() - 1) / (kCtas * sm_count())) * (3. + seen / 2 / 64. * .9);
     const double by_tile = 12. + (double)((n_tiles * c.kv_heads + sm_count() - 1) / sm_count()) * (seen / 128.) * 2.3;
@@ -471,7 +481,7 @@ int launch_attention(const Kv8Attention& p, cudaStream_t st) {
     int rc;
     const int64_t rows = p.n_tiles ? (int64_t)p.n_tiles * p.tile_tokens : p.rows;   // that kv8_row goes through
     if (p.n_tiles && !p.one_by_one) rc = kv8_prompt_attention(p, kDim, st);
-    else if (p.splits <= kMostRanks)
+    else if (p.clustered)
         return launch_kernel(kv8_attention_kernel<kDim, true>, dim3(pairs, (unsigned)p.splits, (unsigned)rows), dim3(kWarps * 32), smem, st,
                              p.splits, launch);
     else rc = launch_kernel(kv8_attention_kernel<kDim, false>, dim3((unsigned)p.splits, pairs, (unsigned)p.rows), dim3(kWarps * 32), smem, st, 1, launch);
@@ -496,7 +506,7 @@ using namespace gptrs;
 extern "C" {
 
 int gptrs_cuda_kv8_splits(const gptrs_kv8_cache* c, int64_t rows, int64_t n_tiles, int64_t max_ctx_len) {
-    if (!c || rows < 1 || c->kv_heads < 1) return 1;
+    if (!c || rows < 1 || c->kv_heads < 1 || c->q_heads < c->kv_heads) return 1;
     if (n_tiles > 0) {
         // a CTA per tile and kv head has an SM to itself: parts only where SMs would have nothing, at most one wave of them, of 1024 keys at least (us with 1 / 2 /
         // 4 / 8 parts: 500 tokens behind 32768, 32 / 8 heads of 128, 64 CTAs: 515 / 288 / 303 / -; 128 behind 8192: 136 / 84 / 55 / 42; 512 behind 16384, 8 / 1
@@ -505,18 +515,23 @@ int gptrs_cuda_kv8_splits(const gptrs_kv8_cache* c, int64_t rows, int64_t n_tile
         return rows > 65535 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(sm_count() / ctas, keys / 1024));
     }
     const int64_t seen = c->window > 0 ? std::min<int64_t>(max_ctx_len, c->window + kKv8Tokens) : max_ctx_len;
-    const int64_t blocks = (seen + kKv8Tokens - 1) / kKv8Tokens;
-    const int64_t pairs = rows * c->kv_heads * ((c->q_heads / c->kv_heads + kCols - 1) / kCols), slots = (int64_t)kCtas * sm_count();
-    // One wave of CTAs. Up to eight parts are merged by their cluster in the same launch, down to a block per warp; more, with a second kernel, pay where a warp
-    // keeps about a dozen blocks (one sequence, 32 / 8 heads of 128, us with 8 / 16 / 32 / 55 parts: 4000 tokens 9.4 / 8.5 / 9.4 / -, 10000 15.7 / 11.7 /
-    // 11.7 / 14.0, 30000 37.4 / 24.0 / 20.7 / 24.0).
-    const int64_t wave = std::max<int64_t>(1, slots / pairs), many = std::min(wave, blocks / (12 * kWarps));
+    const int64_t blocks = (seen + kKv8Tokens - 1) / kKv8Tokens, ctas = rows * pairs_of(*c), wave = places() / ctas;
+    // Few rows: one wave of CTAs. Up to eight parts are merged by their cluster in the same launch; more, with a second kernel, pay where a warp keeps about a dozen
+    // blocks (one sequence, 32 / 8 heads of 128, us with 8 / 16 / 32 / 55 parts: 4000 tokens 9.4 / 8.5 / 9.4 / -, 10000 15.7 / 11.7 / 11.7 / 14.0, 30000
+    // 37.4 / 24.0 / 20.7 / 24.0).
+    const int64_t many = std::min(wave, blocks / (12 * kWarps));
     if (many > kMostRanks) return (int)std::min<int64_t>(many, 65535);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({wave, kMostRanks, (blocks + kWarps - 1) / kWarps}));
+    // Many rows: parts of about 1600 tokens, eight waves at most, since places that short sequences leave are taken by parts of long ones (32 / 8 heads of 128, us in
+    // one wave / like this: 64 sequences of 512 - 8192 tokens 119 / 104, 32 of them 84 / 60, 16 38 / 36, 128 of them 209 / 189; 64 of 4000 - 32768 459 / 378, 8 of
+    // them 75 / 66; 64 of 500 - 4000 68 / 64). Below 2600 tokens, and for few rows of moderate length, one wave is better (32 of 1000 - 2000 26.8 / 33.5; 8 of 512 -
+    // 8192 24.1 / 29.3).
+    const int64_t pieces = std::min((blocks + 40) / 100, std::max<int64_t>(1, 8 * places() / ctas));
+    if (pieces > 1 && (wave <= 4 || pieces > kMostRanks)) return (int)std::min<int64_t>(pieces, 65535);
+    return cluster_parts(*c, rows, blocks);
 }
 
 size_t gptrs_cuda_kv8_scratch_bytes(const gptrs_kv8_cache* c, int64_t rows, int64_t n_tiles, int splits) {
-    if (!c || splits <= 1 || rows < 1 || (n_tiles == 0 && splits <= kMostRanks)) return 0;
+    if (!c || splits <= 1 || rows < 1 || c->kv_heads < 1 || c->q_heads < c->kv_heads || (n_tiles == 0 && in_cluster(*c, rows, splits))) return 0;
     return (size_t)rows * c->q_heads * splits * (c->dim + 2) * sizeof(float);
 }
 
@@ -553,11 +568,12 @@ int gptrs_cuda_kv8_attention(const gptrs_kv8_cache* c, const gptrs_kv8_attention
     p.chunk_blocks = std::max(1, ceil_div(seen, s->splits));
     p.part_o = static_cast<float*>(s->d_scratch);
     p.part_ml = p.part_o + (size_t)p.rows * p.q_heads * p.splits * c->dim;
+    p.clustered = in_cluster(*c, s->rows, s->splits);
     p.tile_row = s->d_tile_row; p.tile_rows = s->d_tile_rows; p.n_tiles = (int)s->n_tiles; p.tile_tokens = c->tile_tokens;
     if (p.n_tiles > 0 && p.splits == 1 && rows_one_by_one(*c, s->rows, s->n_tiles, p.max_len)) {
         p.one_by_one = 1;
-        p.splits = gptrs_cuda_kv8_splits(c, s->rows, 0, p.max_len);
-        p.splits = std::min(p.splits, kMostRanks);
+        p.clustered = 1;
+        p.splits = cluster_parts(*c, s->rows, seen);
         p.chunk_blocks = std::max(1, ceil_div(seen, p.splits));
         return c->dim == 64 ? launch_attention<64>(p, as_stream(stream)) : launch_attention<128>(p, as_stream(stream));
     }

@@ -19,6 +19,7 @@ struct Kv8Attention {
     const int *tile_row, *tile_rows;
     int n_tiles, tile_tokens;     // most rows of a tile
     int one_by_one;               // the rows of the tiles go one by one
+    int clustered;                // parts of a row are merged by their cluster
 };
 int kv8_prompt_attention(const Kv8Attention& p, int dim, cudaStream_t stream);   // tiles of rows (kv8_prompt.cu)
 

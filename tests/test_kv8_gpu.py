@@ -425,6 +425,21 @@ def test_windows_and_splits(cuda, splits, window):
     c.attend([(2, 500), (2, 512), (1, 299), (2, 1), (-1, 77), (2, 1024), (3, 0)], splits=splits)    # less than the sequence has; padding; the same slot often
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(8, 4, 64), (16, 4, 128)])
+@pytest.mark.parametrize("splits", [2, 5, 8, None])
+def test_many_rows_in_parts(cuda, heads, kv, dim, splits):
+    """More parts than places: they meet in scratch, whatever their number; rows of one part, of none and padding among them."""
+    lengths = [1, 300, 1024, 1000, 17, 0, 3000]
+    c = Cache(cuda, heads, kv, dim, 7, 190, seed=dim)
+    c.fill(lengths)
+    rows = [(i, n) for i, n in enumerate(lengths)] * 20 + [(-1, 5), (6, 2999), (6, 64), (2, 1), (1, 17)] * 10
+    q = torch.tensor(c.rng.normal(0, 1.5, (len(rows), heads, dim)), dtype=torch.float32).bfloat16().to(cuda)
+    _, out = c.attend(rows, splits=splits, q=q, want=False)
+    assert int(c.status) == 0
+    c.check(rows, q, out, every=13)
+    assert all((out[i] == 3).all() for i, (s, _) in enumerate(rows) if s < 0)
+
+
 def test_scales_of_very_different_size(cuda):
     """Blocks whose values differ by many powers of two, blocks of zeros, and scores that pick a block of small values."""
     c = Cache(cuda, 4, 1, 64, 1, 20)

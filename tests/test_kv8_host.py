@@ -135,6 +135,20 @@ def test_objects_refuse_wrong_tensors():
         ops.QkNormRope(ops.QkRotation(8, 2, 64, axis_positions=torch.zeros((1, 4), dtype=torch.int32)), qkv, ints)
 
 
+def test_parts_and_scratch():
+    """Scratch is asked for where parts are more than a wave or more than a cluster holds; nothing is computed from heads that are none."""
+    a, lib = ops.kv8_layout(32, 8, 128), gptrs_b200.lib()
+    parts = lambda rows, n_tiles, longest: lib.gptrs_cuda_kv8_splits(ctypes.byref(a), rows, n_tiles, longest)
+    assert parts(0, 0, 100) == 1 and parts(1, 0, 0) == 1 and parts(1, 0, 17) == 1 and parts(1, 0, 1000) == 8 and parts(4096, 0, 131072) == 1
+    for rows, longest in [(1, 100), (1, 1 << 20), (7, 5000), (64, 8192), (64, 300), (300, 131072), (70000, 4000)]:
+        n = parts(rows, 0, longest)
+        size = lib.gptrs_cuda_kv8_scratch_bytes(ctypes.byref(a), rows, 0, n)
+        assert 1 <= n <= 65535 and size in (0, rows * 32 * n * 130 * 4) and (size == 0 if n == 1 else size > 0 if n > 8 else True)
+    assert lib.gptrs_cuda_kv8_scratch_bytes(ctypes.byref(a), 1, 0, 8) == 0 and lib.gptrs_cuda_kv8_scratch_bytes(ctypes.byref(a), 64, 0, 8) == 64 * 32 * 8 * 130 * 4
+    for bad in (_abi.Kv8Cache(0, 0, 128), _abi.Kv8Cache(4, 0, 128), _abi.Kv8Cache(1, 2, 128)):
+        assert lib.gptrs_cuda_kv8_splits(ctypes.byref(bad), 5, 0, 1000) == 1 and lib.gptrs_cuda_kv8_scratch_bytes(ctypes.byref(bad), 5, 0, 4) == 0
+
+
 def test_tiles():
     a = ops.kv8_layout(32, 8, 128)
     first, n = ops.kv8_tiles(a, [1, 64, 0, 130], "cpu")
