@@ -867,7 +867,8 @@ def kv8_tiles(a, counts, device):
 
 class Kv8Attention(_Step):
     """gptrs_cuda_kv8_attention: q [T][heads][dim] (rows may lie a stride apart) -> out [T][heads * dim]. lengths [slots]: tokens that the
-    cache holds. `tiles` (kv8_tiles): rows of prompts; None: every row by itself."""
+    cache holds. `tiles` (kv8_tiles): rows of prompts; None: every row by itself. The object owns its scratch: calls that may overlap (two
+    streams, two graphs) need one object each."""
 
     def __init__(self, a, q, pool, open_rows, page_table, slot, ctx_len, lengths, max_ctx_len, tiles=None, splits=None, out=None, status=None):
         rows = q.shape[0]

@@ -802,7 +802,7 @@ typedef struct {
     int64_t max_ctx_len;
     int splits;
     void* d_out;
-    void* d_scratch;                   /* 16-byte aligned */
+    void* d_scratch;                   /* 16-byte aligned; of one call at a time: calls and graphs that may overlap have their own */
     size_t scratch_bytes;
     int32_t* d_status;
     int64_t rows;

@@ -670,3 +670,37 @@ def test_other_streams_and_two_calls_at_once(cuda):
     torch.cuda.synchronize()
     for ref, got in zip(refs, outs):
         assert all(torch.equal(ref, g) for g in got)
+
+
+@pytest.mark.parametrize("tiles", [None, [70, 60]])
+def test_two_graphs_of_one_cache_at_once(cuda, tiles):
+    """Two objects over one cache whose parts meet in scratch, captured each and replayed side by side: either has scratch of its own."""
+    c = Cache(cuda, 8, 2, 128, 2, 130, seed=5)
+    c.fill([2000, 1900])
+    rows = [(0, 2000), (1, 1900)] if tiles is None else [(0, i + 1) for i in range(1930, 2000)] + [(1, i + 1) for i in range(1840, 1900)]
+    slot, ctx, lengths = _ints([s for s, _ in rows], cuda), _ints([n for _, n in rows], cuda), c.lengths()
+    tiled = None if tiles is None else ops.kv8_tiles(c.a, tiles, cuda)
+    qs = [torch.randn((len(rows), 8, 128), device=cuda).bfloat16() for _ in range(2)]
+    steps = [ops.Kv8Attention(c.a, q, c.pool, c.rows, c.table, slot, ctx, lengths, 2000, tiles=tiled, splits=12, status=c.status) for q in qs]
+    streams, graphs = [torch.cuda.Stream() for _ in qs], [torch.cuda.CUDAGraph() for _ in qs]
+    for step, stream in zip(steps, streams):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            step()
+    torch.cuda.synchronize()
+    wants = [step.out.clone() for step in steps]
+    for step, q, want in zip(steps, qs, wants):
+        c.check(rows, q, want, every=17)
+    for step, stream, graph in zip(steps, streams, graphs):
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+    for _ in range(30):
+        for step in steps:
+            step.out.zero_()
+        torch.cuda.synchronize()
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(step.out, want) for step, want in zip(steps, wants))
+    assert int(c.status) == 0
