@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
     constexpr uint32_t kIdescS = kIdesc | ((uint32_t)(kKeys / 2 >> 3) << 17), kIdescO = kIdesc | ((uint32_t)(kDim >> 3) << 17);
 
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t k_first, full[2], empty[2], s_full[kTiles][2], p_full[kTiles][2], o_first[kTiles], o_full[kTiles], drained[kTiles];
+    __shared__ __align__(8) uint64_t k_first, k_read, full[2], empty[2], s_full[kTiles][2], p_full[kTiles][2], o_first[kTiles], o_full[kTiles], drained[kTiles];
     __shared__ uint32_t tmem_holder;
     __shared__ int s_begin[kSoftmaxThreads / 32], s_end[kSoftmaxThreads / 32];
     __shared__ __align__(16) float scales[kScaleSlots][kPages][4];   // s_K scale log2 e, log2 s_V, 1 / s_V
@@ -133,6 +133,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 
     if (tid == 0) {
         mbar_init(&k_first, kLoadWarps);
+        mbar_init(&k_read, kTiles);
         for (int i = 0; i < 2; ++i) { mbar_init(&full[i], kLoadWarps); mbar_init(&empty[i], kTiles); }
         for (int i = 0; i < kTiles; ++i) {
             for (int h = 0; h < 2; ++h) { mbar_init(&s_full[i][h], 1); mbar_init(&p_full[i][h], kRows); }
@@ -366,7 +367,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 }
             }
         };
-        // stage kb & 1: V of block kb and K of block kb + 1, which the products of one round read; K of block 0 by itself
+        // Round kb stores V of block kb (stage kb & 1) and K of block kb + 1 (the other stage). What lies there, V of block kb - 2 and K of block kb - 1, is read
+        // by the products of round kb - 2, whose end `empty` tells; only K of block 0 is read in front of all rounds: `k_read` tells the end of the first
+        // scores, before K of block 2 takes its place.
         auto store_keys = [&](const Page (&pg)[2], int kb) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) store_k(pg[j], j, kb, sK + (kb & 1) * kKBytes);
@@ -386,6 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             for (int j = 0; j < 2; ++j) { next[j] = find(kb + 1, j, numbers[j]); numbers[j] = number(kb + 2, j); }
             if (kb + 1 < n_blocks) load_k(next);
             if (kb >= 2 && !wait(&empty[st], (uint32_t)((kb - 2) >> 1) & 1u)) break;
+            if (kb == 1 && n_blocks > 2 && !wait(&k_read, 0)) break;
 #pragma unroll
             for (int j = 0; j < 2; ++j) { store_v(pages[j], j, sV + st * 2 * kVHalf); pages[j] = next[j]; }
             if (kb + 1 < n_blocks) {
@@ -417,6 +421,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             if (my_blocks > 0 && wait_one(&k_first, 0)) {
                 tc_fence_after();
                 for (int h = 0; h < 2; ++h) issue_s(h, 0);
+                umma_commit(&k_read);
+            } else if (!failed) {
+                mbar_arrive(&k_read);
             }
             for (int kb = 0; kb < n_blocks && !failed; ++kb) {
                 const int st = kb & 1;

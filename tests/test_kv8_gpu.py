@@ -613,6 +613,27 @@ def test_prompt_in_parts(cuda, splits):
     c.attend([(0, p + 1) for p in range(1100, 1200)] + [(1, p + 1) for p in range(640, 700)], tiles=[100, 60], splits=splits)
 
 
+@pytest.mark.parametrize("rows,splits", [(1100, 1), (20, 2)])
+def test_pages_that_arrive_at_different_times(cuda, rows, splits):
+    """Pages of one of the warps that widen them are in L2, the others' are not: that warp is ahead of the others and of the products, whose operands stay
+    as they are until they have been read. The bits are those of a run whose pages are all there. 20 rows: a row tile without a row."""
+    c = Cache(cuda, 32, 8, 128, 1, 72, seed=rows)
+    c.fill([1100])
+    seen = [(0, p + 1) for p in range(1100 - rows, 1100)]
+    q, out = c.attend(seen, tiles=[rows], splits=splits, want=False)
+    c.check(seen, q, out, every=67)
+    slot, ctx = _ints([0] * rows, cuda), _ints([n for _, n in seen], cuda)
+    step = ops.Kv8Attention(c.a, q, c.pool, c.rows, c.table, slot, ctx, c.lengths(), 1100, tiles=ops.kv8_tiles(c.a, [rows], cuda), splits=splits, status=c.status)
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device=cuda)
+    for turn in range(12):
+        flush.fill_(turn)
+        warm = c.table[0, [b for b in range(68) if b % 8 // 2 == turn % 4]].long()
+        c.pool[warm].sum()
+        torch.cuda.synchronize()
+        assert torch.equal(step(), out), turn
+    assert int(c.status) == 0
+
+
 # ---- together ----------------------------------------------------------------------------------------------------------------------
 def test_prompt_then_steps_in_a_graph(cuda):
     """A prompt, then tokens one by one as a server has them: append and attention recorded once, replayed with new rows, positions and lengths."""
