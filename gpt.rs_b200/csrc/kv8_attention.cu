@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) kv8_attention_kernel(const
         const int b = b0 + (n_my - 1) * kWarps, have = span.length - b * kKv8Tokens;
         const __nv_bfloat16* ks = p.open + (long long)span.slot * kv8_open_elems(p.kv_heads, kDim) + kv8_open_at(b, p.kv_heads, kv_head, 0, kDim);
         uint4 kr[kC][2];
-        uint32_t v[2 * kC][4], big = 0, big_v = 0;
+        uint32_t v[2 * kC][4];
 #pragma unroll
         for (int c = 0; c < kC; ++c)
 #pragma unroll
@@ -301,14 +301,39 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) kv8_attention_kernel(const
                 const int d = 16 * i + 8 * (j & 1) + g, tok = 2 * t + 8 * (j >> 1);
                 const uint32_t lo = tok < have ? vs[tok * kDim + d] : 0u, hi = tok + 1 < have ? vs[(tok + 1) * kDim + d] : 0u;
                 v[i][j] = lo | hi << 16;
-                big_v = __vmaxu2(big_v, v[i][j] & 0x7fff7fffu);
             }
+        int e, ev;
+        auto exponents = [&] {
+            uint32_t big = 0, big_v = 0;
 #pragma unroll
-        for (int c = 0; c < kC; ++c)
+            for (int c = 0; c < kC; ++c)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) big = __vmaxu2(big, __vmaxu2(abs_bits_max2(kr[c][r].x, kr[c][r].y), abs_bits_max2(kr[c][r].z, kr[c][r].w)));
-        const int e = pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big))), ev = pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big_v)));
-        const float factor = e == 128 ? 0.f : pow2(-e), factor_v = ev == 128 ? 0.f : pow2(-ev);
+                for (int r = 0; r < 2; ++r) big = __vmaxu2(big, __vmaxu2(abs_bits_max2(kr[c][r].x, kr[c][r].y), abs_bits_max2(kr[c][r].z, kr[c][r].w)));
+#pragma unroll
+            for (int i = 0; i < 2 * kC; ++i) big_v = __vmaxu2(big_v, __vmaxu2(abs_bits_max2(v[i][0], v[i][1]), abs_bits_max2(v[i][2], v[i][3])));
+            e = pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big)));
+            ev = pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big_v)));
+        };
+        exponents();
+        // What is not finite makes its token's weights none for the rows that see it. It counts as zero itself, or 0 x infinity would reach the others.
+        uint32_t none = 0;   // tokens
+        if (e == 128 || ev == 128) {   // (the whole warp)
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                    if (drop_not_finite(kr[c][r].x) | drop_not_finite(kr[c][r].y) | drop_not_finite(kr[c][r].z) | drop_not_finite(kr[c][r].w)) none |= 1u << (g + 8 * r);
+#pragma unroll
+            for (int i = 0; i < 2 * kC; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t halves = drop_not_finite(v[i][j]);
+                    none |= ((halves & 1u) | (halves >> 31) << 1) << (2 * t + 8 * (j >> 1));
+                }
+            none = __reduce_or_sync(0xffffffffu, none);
+            exponents();
+        }
+        const float factor = pow2(-e), factor_v = pow2(-ev);
         float s[1][4] = {};
 #pragma unroll
         for (int c = 0; c < kC; ++c) {
@@ -317,8 +342,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) kv8_attention_kernel(const
             mma_f16_16816(s[0], bf16x2_to_f16x2(kr[c][0].z, factor), bf16x2_to_f16x2(kr[c][1].z, factor), bf16x2_to_f16x2(kr[c][0].w, factor), bf16x2_to_f16x2(kr[c][1].w, factor),
                           qf[c][1][0], qf[c][1][1]);
         }
+        if ((none >> g) & 1) s[0][0] = s[0][1] = __uint_as_float(0x7fc00000u);
+        if ((none >> (g + 8)) & 1) s[0][2] = s[0][3] = __uint_as_float(0x7fc00000u);
         uint32_t packed[1][2];
-        const float2 scale = make_float2(e == 128 ? __uint_as_float(0x7fc00000u) : pow2(e), ev == 128 ? __uint_as_float(0x7fc00000u) : pow2(ev));
+        const float2 scale = make_float2(pow2(e), pow2(ev));
         weigh(One{}, s, b, &scale, 0, packed);
 #pragma unroll
         for (int i = 0; i < 2 * kC; ++i)

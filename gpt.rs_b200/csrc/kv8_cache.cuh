@@ -75,6 +75,12 @@ __device__ __forceinline__ int pow2_exponent(uint32_t largest_abs_bits) {   // -
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }   // -126 .. 127
 __device__ __forceinline__ uint32_t abs_bits_max2(uint32_t a, uint32_t b) { return __vmaxu2(a & 0x7fff7fffu, b & 0x7fff7fffu); }
+// The halves of v that are not finite become zero; ones in their place.
+__device__ __forceinline__ uint32_t drop_not_finite(uint32_t& v) {
+    const uint32_t none = __vcmpgeu2(v & 0x7fff7fffu, 0x7f807f80u);
+    v &= ~none;
+    return none;
+}
 __device__ __forceinline__ uint32_t widest_half(uint32_t v) { return max(v & 0xffffu, v >> 16); }
 __device__ __forceinline__ uint32_t bf16x2_to_f16x2(uint32_t v, float factor) { return pack_f16x2(bf16_lo(v) * factor, bf16_hi(v) * factor); }
 

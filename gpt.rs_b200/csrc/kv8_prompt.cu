@@ -285,11 +285,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         auto open_rows = [&](int block, int is_value) {
             return p.open + (long long)slot * kv8_open_elems(p.kv_heads, kDim) + kv8_open_at(block, p.kv_heads, kv_head, is_value, kDim);
         };
-        auto exponent = [&](const void* rows, int have) {   // of the largest magnitude of `have` bf16 rows
-            uint32_t big = 0;
+        // The block that is not complete: exponents of its largest finite key and value, and its tokens with one that is not finite. Their keys go as NaN, so that
+        // their weights are none for the rows that see them, and values that are not finite as zero, or 0 x infinity would reach the other rows.
+        struct Open { int key, value; uint32_t none; };
+        auto look_at = [&](const __nv_bfloat16* rows, int have) {
+            uint32_t big = 0, big_v = 0, none = 0;
 #pragma unroll 1
-            for (int i = lane; i < have * (kDim / 2); i += 32) big = __vmaxu2(big, static_cast<const uint32_t*>(rows)[i] & 0x7fff7fffu);
-            return pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big)));
+            for (int i = lane; i < have * (kDim / 2); i += 32) {
+                uint32_t x = reinterpret_cast<const uint32_t*>(rows)[i], y = reinterpret_cast<const uint32_t*>(rows)[i + kKv8Tokens * (kDim / 2)];
+                if (drop_not_finite(x) | drop_not_finite(y)) none |= 1u << (i / (kDim / 2));
+                big = __vmaxu2(big, x & 0x7fff7fffu);
+                big_v = __vmaxu2(big_v, y & 0x7fff7fffu);
+            }
+            return Open{pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big))), pow2_exponent(__reduce_max_sync(0xffffffffu, widest_half(big_v))),
+                        __reduce_or_sync(0xffffffffu, none)};
         };
         auto store_k = [&](const Page& pg, int j, int kb, uint32_t base) {
             float k_scale = 0.f, v_scale = 1.f;
@@ -312,16 +321,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 // the rows of the block that is not complete, or nothing: zeros (once in a sequence: short code rather than fast)
                 const int have = pg.kind == kOpen ? length - pg.block * kKv8Tokens : 0;
                 const __nv_bfloat16* src = open_rows(pg.block, 0);
-                const int e = exponent(src, have), ev = exponent(src + kKv8Tokens * kDim, have);
-                const float factor = e == 128 ? 0.f : pow2(-e);
-                if (pg.kind == kOpen) {
-                    k_scale = e == 128 ? __uint_as_float(0x7fc00000u) : pow2(e);
-                    v_scale = ev == 128 ? __uint_as_float(0x7fc00000u) : pow2(ev);
-                }
+                const Open o = look_at(src, have);
+                const float factor = pow2(-o.key);
+                if (pg.kind == kOpen) { k_scale = pow2(o.key); v_scale = pow2(o.value); }
 #pragma unroll 1
                 for (int i = 0; i < 2 * kC; ++i) {
                     const int token = kg + 4 * ((i >> 1) & 1) + 8 * (i & 1), d = ((i >> 2) * 2 + kc) * 32 + 8 * t;
-                    const uint4 x = token < have ? *reinterpret_cast<const uint4*>(src + token * kDim + d) : make_uint4(0, 0, 0, 0);
+                    uint4 x = token < have ? *reinterpret_cast<const uint4*>(src + token * kDim + d) : make_uint4(0, 0, 0, 0);
+                    if ((o.none >> token) & 1) x = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
                     st_shared_v4(at(i >> 1, i & 1), bf16x2_to_f16x2(x.x, factor), bf16x2_to_f16x2(x.y, factor), bf16x2_to_f16x2(x.z, factor), bf16x2_to_f16x2(x.w, factor));
                 }
             }
@@ -351,8 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             } else {
                 const int have = pg.kind == kOpen ? length - pg.block * kKv8Tokens : 0;
                 const unsigned short* src = reinterpret_cast<const unsigned short*>(open_rows(pg.block, 1));
-                const int e = exponent(src, have);
-                const float factor = e == 128 ? 0.f : pow2(-e);
+                const float factor = pow2(-look_at(open_rows(pg.block, 0), have).value);
 #pragma unroll 1
                 for (int i = 0; i < 4 * kC; ++i) {
                     const int d = 8 * i + vg;
@@ -361,7 +367,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                     for (int r = 0; r < 2; ++r) {
                         const int token = 2 * t + 8 * r;
                         const uint32_t lo = token < have ? src[token * kDim + d] : 0u, hi = token + 1 < have ? src[(token + 1) * kDim + d] : 0u;
-                        x[r] = bf16x2_to_f16x2(lo | hi << 16, factor);
+                        uint32_t both = lo | hi << 16;
+                        drop_not_finite(both);
+                        x[r] = bf16x2_to_f16x2(both, factor);
                     }
                     st_shared_v2(at(d), x[0], x[1]);
                 }

@@ -781,7 +781,8 @@ int gptrs_cuda_kv8_gather(const gptrs_kv8_cache* c, const void* d_pool, int64_t 
                           int64_t max_pages, const int32_t* d_slot, const int32_t* d_positions, const int32_t* d_length, int dtype, void* d_k,
                           void* d_v, int32_t* d_status, int64_t rows, void* stream);
 /* out [rows][q_heads][dim] (bf16) = softmax over the visible keys . values; row t belongs to slot[t] and sees the last `window` of its first
- * ctx_len[t] tokens (the cache as it is behind the append). A row that sees nothing gives zeros, one with a negative slot is left as it was.
+ * ctx_len[t] tokens (the cache as it is behind the append). A row that sees nothing gives zeros, one with a negative slot is left as it was. A row that sees a token
+ * of a block with a NaN scale, or a token among the open rows whose key or value is not finite, is NaN for the query heads of that kv head; others know nothing of it.
  * n_tiles = 0: every row by itself (single tokens of many sequences); else tile i is the rows tile_row[i] .. + tile_rows[i], at most tile_tokens
  * rows of one sequence at consecutive positions (prompts, chunks of prompts); rows in no tile are left as they were, no row is in two. Tiles are
  * begun from the last one on. The keys of a row or tile are read in at most `splits` parts (gptrs_cuda_kv8_splits; scratch:

@@ -634,6 +634,35 @@ def test_pages_that_arrive_at_different_times(cuda, rows, splits):
     assert int(c.status) == 0
 
 
+@pytest.mark.parametrize("tiles,splits", [(False, 1), (False, 3), (True, 1), (True, 2)])
+@pytest.mark.parametrize("window", [0, 5])
+def test_open_block_that_is_not_finite(cuda, window, tiles, splits):
+    """A key or value that is not finite in the block that is not complete: rows that see its token are NaN there, others know nothing of it, row by row and in
+    tiles alike."""
+    n = 300
+    c = Cache(cuda, 32, 8, 128, 1, 20, window=window)
+    qkv = torch.randn((n, 48 * 128), device=cuda).bfloat16()
+    bad = {290: (40 + 3, "nan"), 294: (32 + 5, "inf"), 296: (40 + 6, "-inf")}     # token: head of the row (32 keys, 40 values)
+    for token, (head, x) in bad.items():
+        qkv[token, head * 128 + 7] = float(x)
+    c.append([(0, 0, n)], qkv)
+    rows = [(0, p + 1) for p in range(0 if tiles else 280, n)]
+    q, out = c.attend(rows, tiles=[n] if tiles else None, splits=splits, want=False)
+    assert int(c.status) == 0
+    s, got = c.seq[0], _np(out).reshape(-1, 32, 128)
+    s.k, s.v = (np.where(np.isfinite(x), x, np.float32(0)) for x in (s.k, s.v))
+    (k, v), vs, qn = s.held(), s.value_scales(), _np(q)
+    for i, (_, end) in enumerate(rows):
+        if end < 280 and end % 37:
+            continue
+        begin = max(0, end - window) if window else 0
+        w, size, unit = kr.attention(qn[i], k, v, begin, end, c.a.scale, vs)
+        sees = np.isin(np.arange(32) // 4, [(head - 32) % 8 for token, (head, _) in bad.items() if begin <= token < end])
+        assert np.isnan(got[i, sees]).all(), end
+        off = np.abs(got[i] - w) - 2 ** -8 * np.abs(w) - (1 + 2 ** -8) * (2 ** -10 * size + 2 ** -25 * unit)
+        assert (off[~sees] <= 0).all(), end
+
+
 # ---- together ----------------------------------------------------------------------------------------------------------------------
 def test_prompt_then_steps_in_a_graph(cuda):
     """A prompt, then tokens one by one as a server has them: append and attention recorded once, replayed with new rows, positions and lengths."""
