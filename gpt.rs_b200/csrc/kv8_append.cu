@@ -9,6 +9,8 @@
 // prompts of 2777 tokens, 16 / 4 heads, three axes: 58.6 us (148 MB, 39 % of the copy bandwidth; 38.6 us without the queries and the blocks; a warp
 // instruction per scheduler in 44 % of the cycles, four CTAs an SM). Measured and left: CTAs that stay and fetch ahead into L2 (62.9), CTAs for queries
 // and for keys apart (65.1).
+#include <algorithm>
+
 #include "kv8_cache.cuh"
 #include "qk_rotate.cuh"
 
@@ -29,6 +31,7 @@ struct AppendParams {
     __nv_bfloat16* q;
     int* status;
     int rows, q_heads, kv_heads, group;
+    int tokens;   // of a sequence: positions that the table has pages for
 };
 
 // A lane's eight channels of a key or value in bf16: four of its first run, four of its second.
@@ -200,11 +203,7 @@ __global__ void __launch_bounds__(kThreads, 4) kv8_append_kernel(const AppendPar
         if (p.rotates) x.set(a, b);
         return x;
     };
-    auto page_of = [&](int slot, int block) {
-        if (block < p.max_pages) return kv8_page(p.table, slot, p.max_pages, block, p.n_pages, p.status);
-        if (tid == 0) atomicExch(p.status, 2);
-        return -1;
-    };
+    auto page_of = [&](int slot, int block) { return kv8_page(p.table, slot, p.max_pages, block, p.n_pages, p.status); };
 
     if (kTile == 1) {
         // ---- a run of one row: everything is asked for at once ---------------------------------------------------------------------------------
@@ -214,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 4) kv8_append_kernel(const AppendPar
         if (lane < 2) own.load(source(row0, p.q_heads + lane * p.kv_heads + kv_head), ca, cb);   // lane group 0 has the key, 1 the value
         const int slot = p.slot[row0], position = p.positions[row0], first = p.run_first[row0], last = p.run_last[row0];
         if (slot < 0) return;
-        if (first == row0 && last == row0 && slot < p.n_slots && position >= 0 && position <= 0x7fffffff - kKv8Tokens) {
+        if (first == row0 && last == row0 && slot < p.n_slots && position >= 0 && position < p.tokens) {
             fetch_angles(row0, 1);
             const bool completes = position % kKv8Tokens == kKv8Tokens - 1;
             Packed x[2][kPer];
@@ -260,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 4) kv8_append_kernel(const AppendPar
     bool ends = false;
     if (slot_i >= 0) {
         if (slot_i >= p.n_slots || first_i < 0 || first_i > row_i || last_i < row_i || last_i >= p.rows || position_i < row_i - first_i ||
-            position_i > 0x7fffffff - kKv8Tokens - (last_i - row_i))
+            position_i >= p.tokens)   // (rows in front of the table's end, which is a block's, go on)
             atomicExch(p.status, 2);
         else
             ends = position_i % kKv8Tokens == kKv8Tokens - 1 || row_i == last_i;
@@ -272,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 4) kv8_append_kernel(const AppendPar
         const int slot = __shfl_sync(0xffffffffu, slot_i, from), position = __shfl_sync(0xffffffffu, position_i, from), first = __shfl_sync(0xffffffffu, first_i, from),
                   last = __shfl_sync(0xffffffffu, last_i, from);
         const int block = position / kKv8Tokens, token_b = position % kKv8Tokens, row_a = max(first, row_b - token_b), token_a = token_b - (row_b - row_a), n = row_b - row_a + 1;
-        const int start = position - (row_b - first), end = position + (last - row_b);   // of the run
+        const int start = position - (row_b - first), end = (int)min((long long)position + (last - row_b), p.tokens - 1ll);   // of the run
         const bool continued = start % kKv8Tokens != 0, completes = token_b == kKv8Tokens - 1;
         // keys and values of tokens lane + j kGroups: new rows, or open ones of the run's first block
         Packed x[2][kPer] = {};
@@ -399,11 +398,11 @@ __global__ void __launch_bounds__(kThreads) kv8_gather_kernel(const GatherParams
     const int head = (int)(item % per_row) / (kDim / 8), d0 = (int)(item % (kDim / 8)) * 8;
     const int slot = p.slot[row], position = p.positions[row];
     float k[8] = {}, v[8] = {};
-    bool found = slot >= 0 && slot < p.n_slots && position >= 0 && position < p.length[slot >= 0 && slot < p.n_slots ? slot : 0];
+    bool found = slot >= 0 && slot < p.n_slots && position >= 0 && position / kKv8Tokens < p.max_pages && position < p.length[slot >= 0 && slot < p.n_slots ? slot : 0];
     if (found) {
         const int block = position / kKv8Tokens, token = position % kKv8Tokens;
         if (block < p.length[slot] / kKv8Tokens) {
-            const int page = block < p.max_pages ? kv8_page(p.table, slot, p.max_pages, block, p.n_pages, p.status) : -1;
+            const int page = kv8_page(p.table, slot, p.max_pages, block, p.n_pages, p.status);
             found = page >= 0;
             if (found) {
                 const unsigned char* b = p.pool + ((long long)page * p.kv_heads + head) * kv8_block_bytes(kDim);
@@ -500,6 +499,7 @@ int gptrs_cuda_kv8_append(const gptrs_kv8_cache* c, const gptrs_kv8_append_step*
     p.q = static_cast<__nv_bfloat16*>(s->d_q);
     p.status = s->d_status;
     p.rows = (int)s->rows; p.q_heads = c->q_heads; p.kv_heads = c->kv_heads; p.group = c->q_heads / c->kv_heads;
+    p.tokens = (int)std::min<int64_t>(std::min<int64_t>(s->max_pages, 0x7fffffff) * kKv8Tokens, 0x7fffffff - kKv8Tokens + 1);   // a whole number of blocks
     // A CTA per row and kv head for lists that are short or may be single tokens, else per 16 rows: a prompt has one segment in them. Where they are single tokens
     // after all, four CTAs deal the segments among them, as long as the three that find nothing cost little. us, 32 / 8 heads of 128, per row / per 16 / four
     // for 16: 64 single tokens 4.2 / 64 / 20, 512 14 / 66 / 44; a prompt of 256 10.9 / 7.8 / 8.4, of 1000 23 / 10.4 / 11.0, of 4 x 1000 62 / 35 / 31, of

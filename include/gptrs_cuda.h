@@ -757,8 +757,9 @@ int gptrs_cuda_kv8_layout(gptrs_kv8_cache* c);
 /* Projection rows [queries | keys | values] (bf16) -> normed and rotated queries in d_q [rows][q_heads][dim], keys (normed, rotated, rounded
  * to bf16) and values into the cache. Rows come in runs of consecutive positions of one sequence, one run per slot and call; run_first and
  * run_last give the first and the last row of the run of every row. Rows with a negative slot are padding: nothing of them is read or written.
- * rotation NULL: queries and keys as they are. A block whose page_table entry is negative is not kept. *d_status = 2: a slot, position, page
- * or run out of range (the keys and values of that row or block are left out). */
+ * rotation NULL: queries and keys as they are. A block whose page_table entry is negative is not kept. *d_status = 2: a slot, run or position (16 max_pages and
+ * above) out of range: that row is left out, its query included; a page out of range: that block is left out; a position outside the rotation's tables: turned by
+ * position 0. */
 typedef struct {
     const gptrs_qk_rotation* rotation; /* rot_half a multiple of 8 */
     const void* d_qkv;

@@ -330,6 +330,32 @@ def test_bad_rows_are_reported_and_left_out(cuda, what):
         assert torch.equal(c.rows[1].view(torch.int16), rows_before[1].view(torch.int16)) or what == "before"
 
 
+@pytest.mark.parametrize("n", [1, 5, 40, 300])
+def test_positions_behind_the_page_table(cuda, n):
+    """Rows behind the table's pages are reported and left out, whether they complete a block or not; rows in front of them arrive. Nothing is read back from there."""
+    c = Cache(cuda, 4, 2, 64, 2, 4)       # 64 tokens
+    c.append([(0, 0, 60), (1, 0, 64)])
+    for slot, start in ((1, 64), (1, 70), (0, 60)):
+        rows = n + (4 if start == 60 else 0)
+        pool, opened = c.pool.clone(), c.rows.clone()
+        qkv = torch.randn((rows, 8 * 64), device=cuda).bfloat16()
+        q = torch.full((rows, 4, 64), 5.0, dtype=torch.bfloat16, device=cuda)
+        c.status.zero_()
+        ops.kv8_append(c.a, None, qkv, _ints(range(start, start + rows), cuda), _ints([slot] * rows, cuda), _ints([0] * rows, cuda), _ints([rows - 1] * rows, cuda), c.table, c.pool, c.rows,
+                       q=q, status=c.status)
+        assert int(c.status) == 2
+        if start == 60:
+            x = _np(qkv).reshape(rows, 8, 64)
+            c.seq[0].append(60, x[:4, 4:6], x[:4, 6:])
+            assert torch.equal(q[:4].flatten(1), qkv[:4, :256]) and (q[4:] == 5).all()
+        else:
+            assert torch.equal(c.pool, pool) and torch.equal(c.rows.view(torch.int16), opened.view(torch.int16)) and (q == 5).all()
+        c.check_bytes()
+    c.status.zero_()
+    k, v = ops.kv8_gather(c.a, c.pool, c.rows, c.table, _ints([0, 0], cuda), _ints([63, 64], cuda), _ints([65, 65], cuda), status=c.status)
+    assert int(c.status) == 2 and k[0].any() and not k[1].any() and not v[1].any()
+
+
 @pytest.mark.parametrize("heads,kv,dim,pairs,neighbours,axes", [(8, 2, 128, 64, False, 1), (6, 3, 64, 32, True, 3), (8, 8, 128, 32, False, 2), (4, 1, 64, 8, True, 1), (16, 2, 128, 64, False, 3)])
 @pytest.mark.parametrize("n", [1, 45, 700])
 def test_append_norms_and_rotates(cuda, heads, kv, dim, pairs, neighbours, axes, n):
