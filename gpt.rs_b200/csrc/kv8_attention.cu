@@ -2,8 +2,10 @@
 //
 // With keys k = s_K a and values v = s_V b of whole numbers a, b and a scale per block of 16 tokens, for every query head
 //     t_j = (s_K scale log2 e) q . a_j + log2 s_V        w_j = 2^(t_j - M)        out = sum_j w_j b_j / sum_j (w_j / s_V)
-// The value's scale rides in the exponent, so one running maximum M bounds the weights by 1 whatever the scales are, f16 holds them with 11 bits,
-// and no product needs a scale of its own. Queries are f16 with a power of two in front (kv8_cache.cuh), sums and maxima f32.
+// The value's scale rides in the exponent, so one running reference M bounds the weights whatever the scales are, and no product needs a scale of its own. M is
+// the maximum less 15: weights go as f16 up to 2^15, with 11 bits down to 2^-29 of the largest and off by at most 2^-40 of it below, so that the
+// tokens of a long tail still count beside one that has nearly all of the weight (2^20 of them lose 2^-20 of it). Queries are f16 with a power of two in front
+// (kv8_cache.cuh), sums and maxima f32.
 //
 // A warp takes a block at a time. Keys are the rows of the matrix product, heads its columns (eight query heads of a kv head at most): S^T = K Q^T
 // and O^T = V^T P^T, so that little of a matrix instruction is padding. The cache's byte order makes 16 bytes of a lane two k-steps of keys, or two
@@ -27,8 +29,9 @@ constexpr int kCols = 8;    // query heads of a CTA
 constexpr int kDepth = 4;   // blocks of a warp's ring
 constexpr int kCtas = 3;    // of an SM
 constexpr int kMostRanks = 8;   // parts that a cluster merges
+constexpr float kHeadroom = 15.f;   // log2 of the largest weight
 
-// Weight of a part (warp, CTA, split) with maximum m and sum l beside the largest maximum; one without a maximum has seen nothing (0) or nothing but NaN.
+// Weight of a part (warp, CTA, split) with reference m and sum l beside the largest reference; one without a reference has seen nothing (0) or nothing but NaN.
 __device__ __forceinline__ float part_factor(float m, float l, float top) { return m == -INFINITY ? (l == 0.f ? 0.f : l) : kv8_exp2(m - top); }
 __device__ __forceinline__ uint4 lds_16(uint32_t at) {
     uint4 v;
@@ -95,7 +98,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) kv8_attention_kernel(const
     extern __shared__ __align__(128) unsigned char ring[];
     __shared__ __align__(8) uint64_t full[kWarps][kDepth];
     __shared__ float ml_part[kWarps][kCols][2];
-    __shared__ __align__(16) float own_part[kCluster ? kCols * (kDim + 4) : 4];   // kCluster: output, maximum and sum of this CTA's part
+    __shared__ __align__(16) float own_part[kCluster ? kCols * (kDim + 4) : 4];   // kCluster: output, reference and sum of this CTA's part
 
     const Kv8Attention& p = launch.a;
     const int split = kCluster ? blockIdx.y : blockIdx.x, pair = kCluster ? blockIdx.x : blockIdx.y, eights = (p.group + kCols - 1) / kCols;
@@ -178,7 +181,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) kv8_attention_kernel(const
     bool failed = false;
 
     // Scores of kCount blocks (the first one's number and the distance to the next) -> weights, packed as the second operand of O^T = V^T P^T; o scaled to the
-    // new maxima. count: tokens of a block with bit i of `none` do not count
+    // new references. count: tokens of a block with bit i of `none` do not count
     auto weigh = [&](auto count, const float (*s)[4], int b, const float2* scale, uint32_t none, uint32_t (*packed)[2]) {
         constexpr int kCount = decltype(count)::value;
         // tokens g, g + 8 of a block x heads 2 t, 2 t + 1. A scale that is not a number makes the weights of the tokens that are seen none, and
@@ -201,7 +204,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) kv8_attention_kernel(const
             x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
             x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
         }
-        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+        const float n0 = fmaxf(m0, x0 - kHeadroom), n1 = fmaxf(m1, x1 - kHeadroom);
         const float u0 = n0 == -INFINITY ? 0.f : n0, u1 = n1 == -INFINITY ? 0.f : n1;   // nothing seen yet (or nothing but NaN)
         const float a0 = kv8_exp2(m0 - u0), a1 = kv8_exp2(m1 - u1);
         m0 = n0; m1 = n1;

@@ -689,6 +689,27 @@ def test_open_block_that_is_not_finite(cuda, window, tiles, splits):
         assert (off[~sees] <= 0).all(), end
 
 
+@pytest.mark.parametrize("tiles", [False, True])
+def test_a_long_tail_beside_one_token(cuda, tiles):
+    """One token with nearly all of the weight in front of 131071 with 2^-24.9 or 2^-25.2 of it each: together they are 0.3 to 0.4 % of the sum and all of the output.
+    Their weights are f16, off by 2^-25 at most, with 2^15 for the largest of a row, 2^3 or more in tiles."""
+    n = 1 << 17
+    c = Cache(cuda, 2, 1, 64, 1, n // 16)
+    qkv = torch.zeros((n, 4 * 64), device=cuda)
+    qkv[0, 2 * 64] = 16
+    qkv[1:, 3 * 64:] = 1
+    c.append([(0, 0, n)], qkv.bfloat16())
+    rows = [(0, p + 1) for p in range(n - (1000 if tiles else 3), n)]
+    q = torch.zeros((len(rows), 2, 64), device=cuda)
+    q[:, 0, 0], q[:, 1, 0] = 8.625, 8.75
+    q, out = c.attend(rows, tiles=[len(rows)] if tiles else None, splits=1, q=q.bfloat16(), want=False)
+    assert int(c.status) == 0
+    (k, v), vs, qn, got = c.seq[0].held(), c.seq[0].value_scales(), _np(q), _np(out).reshape(-1, 2, 64)
+    for i in [0, len(rows) // 2, len(rows) - 1]:
+        w, size, unit = kr.attention(qn[i], k, v, 0, rows[i][1], c.a.scale, vs)
+        assert (np.abs(got[i] - w) <= 2 ** -8 * w + (1 + 2 ** -8) * (2 ** -10 * size + 2 ** (-25 - (3 if tiles else 15)) * unit)).all(), (got[i, :, 0], w[:, 0])
+
+
 # ---- together ----------------------------------------------------------------------------------------------------------------------
 def test_prompt_then_steps_in_a_graph(cuda):
     """A prompt, then tokens one by one as a server has them: append and attention recorded once, replayed with new rows, positions and lengths."""
