@@ -469,8 +469,8 @@ int gptrs_cuda_kv8_layout(gptrs_kv8_cache* c) {
 int gptrs_cuda_kv8_append(const gptrs_kv8_cache* c, const gptrs_kv8_append_step* s, void* stream) {
     const int rc = kv8_check(c);
     if (rc) return rc;
-    GPTRS_REQUIRE(s && s->d_qkv && s->d_positions && s->d_slot && s->d_run_first && s->d_run_last && s->d_page_table && s->d_pool && s->d_open && s->d_q && s->d_status,
-                  "null pointer");
+    GPTRS_REQUIRE(s && s->d_page_table && s->d_pool && s->d_open && s->d_status, "null pointer");
+    GPTRS_REQUIRE(s->rows == 0 || (s->d_qkv && s->d_positions && s->d_slot && s->d_run_first && s->d_run_last && s->d_q), "null pointer");   // (tensors without rows have none)
     GPTRS_REQUIRE(s->rows >= 0 && s->rows <= 0x3fffffff, "bad row count");
     GPTRS_REQUIRE(s->max_pages >= 1 && s->n_pages >= 1 && s->n_slots >= 1, "empty cache");
     AppendParams p = {};
@@ -515,7 +515,8 @@ int gptrs_cuda_kv8_gather(const gptrs_kv8_cache* c, const void* d_pool, int64_t 
                           void* d_v, int32_t* d_status, int64_t rows, void* stream) {
     const int rc = kv8_check(c);
     if (rc) return rc;
-    GPTRS_REQUIRE(d_pool && d_open && d_page_table && d_slot && d_positions && d_length && d_k && d_v && d_status, "null pointer");
+    GPTRS_REQUIRE(d_pool && d_open && d_page_table && d_length && d_status, "null pointer");
+    GPTRS_REQUIRE(rows == 0 || (d_slot && d_positions && d_k && d_v), "null pointer");
     GPTRS_REQUIRE(dtype == GPTRS_BF16 || dtype == GPTRS_F32, "keys and values come back in bf16 or f32");
     GPTRS_REQUIRE(rows >= 0 && rows <= 0x3fffffff, "bad row count");
     GPTRS_REQUIRE(max_pages >= 1 && n_pages >= 1 && n_slots >= 1, "empty cache");

@@ -568,7 +568,8 @@ size_t gptrs_cuda_kv8_scratch_bytes(const gptrs_kv8_cache* c, int64_t rows, int6
 int gptrs_cuda_kv8_attention(const gptrs_kv8_cache* c, const gptrs_kv8_attention_step* s, void* stream) {
     const int rc = kv8_check(c);
     if (rc) return rc;
-    GPTRS_REQUIRE(s && s->d_q && s->d_pool && s->d_open && s->d_page_table && s->d_slot && s->d_ctx_len && s->d_length && s->d_out && s->d_status, "null pointer");
+    GPTRS_REQUIRE(s && s->d_pool && s->d_open && s->d_page_table && s->d_length && s->d_status, "null pointer");
+    GPTRS_REQUIRE(s->rows == 0 || (s->d_q && s->d_slot && s->d_ctx_len && s->d_out), "null pointer");   // (tensors without rows have none)
     GPTRS_REQUIRE(s->rows >= 0 && s->rows <= 0x3fffffff && s->n_tiles >= 0 && s->n_tiles <= 65535, "bad row count");
     GPTRS_REQUIRE(s->n_tiles == 0 || (s->d_tile_row && s->d_tile_rows), "tiles are missing");
     GPTRS_REQUIRE(s->max_pages >= 1 && s->max_pages * kKv8Tokens < ((int64_t)1 << 31) && s->n_pages >= 1 && s->n_slots >= 1 && s->n_slots <= 0x7fffffff, "bad cache sizes");

@@ -24,7 +24,7 @@ int qk_rotation_of(const gptrs_qk_rotation& r, int64_t rows, QkRotation* out) {
     GPTRS_REQUIRE((r.d_q_gain == nullptr) == (r.d_k_gain == nullptr), "gains of queries and keys come together");
     GPTRS_REQUIRE(r.rot_half == 0 || (r.d_cos && r.d_sin && r.positions > 0), "tables are missing");
     GPTRS_REQUIRE(r.axes >= 0 && r.axes <= 255, "bad number of axes");
-    GPTRS_REQUIRE(r.axes <= 1 || (r.d_axis_positions && r.d_pair_axis), "several axes need their positions and the axis of every pair");
+    GPTRS_REQUIRE(r.axes <= 1 || ((r.d_axis_positions || rows == 0) && r.d_pair_axis), "several axes need their positions and the axis of every pair");
     GPTRS_REQUIRE(r.axis_stride == 0 || r.axis_stride >= rows, "axis_stride is shorter than the rows");
     *out = QkRotation{r.q_heads, r.kv_heads, r.dim, r.rot_half, r.pairs == GPTRS_PAIRS_NEIGHBOURS, r.axes > 1 ? r.axes : 1, r.eps, r.d_q_gain, r.d_k_gain, r.d_cos,
                       r.d_sin, (long long)r.positions, (long long)(r.axis_stride ? r.axis_stride : rows), r.d_axis_positions, r.d_pair_axis};
@@ -432,13 +432,14 @@ using namespace gptrs;
 
 extern "C" int gptrs_cuda_qk_norm_rope(const gptrs_qk_rotation* r, const void* d_qkv, int dtype, int64_t ld_in, const int32_t* d_positions, void* d_out,
                                        int64_t ld_out, int32_t* d_status, int64_t rows, void* stream) {
-    GPTRS_REQUIRE(r && d_qkv && d_out && d_status, "null pointer");
+    GPTRS_REQUIRE(r && d_status, "null pointer");
+    GPTRS_REQUIRE(rows == 0 || (d_qkv && d_out), "null pointer");   // (tensors without rows have none)
     GPTRS_REQUIRE(dtype == GPTRS_F32 || dtype == GPTRS_BF16, "rows are f32 or bf16");
     GPTRS_REQUIRE(rows >= 0 && rows <= 0x7fffffff, "bad row count");
     NormRopeParams p = {};
     const int rc = qk_rotation_of(*r, rows, &p.r);
     if (rc) return rc;
-    GPTRS_REQUIRE(p.r.rot_half == 0 || p.r.axis_positions || d_positions, "positions are missing");
+    GPTRS_REQUIRE(rows == 0 || p.r.rot_half == 0 || p.r.axis_positions || d_positions, "positions are missing");
     const int64_t width = (int64_t)(r->q_heads + 2 * r->kv_heads) * r->dim;
     p.ld_in = ld_in ? ld_in : width;
     p.ld_out = ld_out ? ld_out : width;

@@ -710,6 +710,21 @@ def test_a_long_tail_beside_one_token(cuda, tiles):
         assert (np.abs(got[i] - w) <= 2 ** -8 * w + (1 + 2 ** -8) * (2 ** -10 * size + 2 ** (-25 - (3 if tiles else 15)) * unit)).all(), (got[i, :, 0], w[:, 0])
 
 
+def test_calls_without_rows(cuda):
+    """No rows: nothing to do, whatever the tensors' addresses."""
+    c = Cache(cuda, 8, 2, 128, 2, 4)
+    c.fill([20, 7])
+    none, empty = _ints([], cuda), torch.empty((0, 12 * 128), dtype=torch.bfloat16, device=cuda)
+    rot = ops.QkRotation(8, 2, 128)
+    assert ops.qk_norm_rope(rot, empty, none).shape == (0, 12 * 128)
+    before = c.pool.clone()
+    assert ops.kv8_append(c.a, rot, empty, none, none, none, none, c.table, c.pool, c.rows, status=c.status).shape == (0, 8, 128)
+    for tiles in (None, ops.kv8_tiles(c.a, [], cuda)):
+        assert ops.kv8_attention(c.a, empty.reshape(0, 12, 128)[:, :8], c.pool, c.rows, c.table, none, none, c.lengths(), 100, tiles=tiles, status=c.status).shape == (0, 8 * 128)
+    k, v = ops.kv8_gather(c.a, c.pool, c.rows, c.table, none, none, c.lengths(), status=c.status)
+    assert k.shape == v.shape == (0, 2, 128) and torch.equal(c.pool, before) and int(c.status) == 0
+
+
 # ---- together ----------------------------------------------------------------------------------------------------------------------
 def test_prompt_then_steps_in_a_graph(cuda):
     """A prompt, then tokens one by one as a server has them: append and attention recorded once, replayed with new rows, positions and lengths."""

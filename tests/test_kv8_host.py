@@ -117,6 +117,26 @@ def test_attention_and_gather_refusals():
         assert _status("gptrs_cuda_kv8_gather", *args) == SPEC, (at, bad)
 
 
+def test_calls_without_rows_need_no_rows():
+    """Empty tensors have no address: a call without rows does nothing, and still refuses what is wrong with the rest."""
+    a = ops.kv8_layout(8, 2, 64)
+    r = _rotation(axes=2, d_pair_axis=64)
+    assert _status("gptrs_cuda_qk_norm_rope", ctypes.byref(r), None, 0, 0, None, None, 0, 64, 0, None) == 0
+    s = _append_step(a, rows=0, **{n: None for n in ("d_qkv", "d_positions", "d_slot", "d_run_first", "d_run_last", "d_q")})
+    assert _status("gptrs_cuda_kv8_append", ctypes.byref(a), ctypes.byref(s), None) == 0
+    t = _abi.Kv8AttentionStep()
+    for n in ("d_pool", "d_open", "d_page_table", "d_length", "d_status"):
+        setattr(t, n, 4096)
+    t.n_pages = t.n_slots = t.max_pages = 4
+    t.max_ctx_len, t.splits = 64, 1
+    assert _status("gptrs_cuda_kv8_attention", ctypes.byref(a), ctypes.byref(t), None) == 0
+    assert _status("gptrs_cuda_kv8_gather", ctypes.byref(a), 4096, 4, 4096, 4, 4096, 4, None, None, 4096, 2, None, None, 4096, 0, None) == 0
+    s.d_pool = t.d_pool = None
+    assert _status("gptrs_cuda_kv8_append", ctypes.byref(a), ctypes.byref(s), None) == SPEC
+    assert _status("gptrs_cuda_kv8_attention", ctypes.byref(a), ctypes.byref(t), None) == SPEC
+    assert _status("gptrs_cuda_qk_norm_rope", ctypes.byref(_rotation(dim=63)), None, 0, 0, None, None, 0, 64, 0, None) == SPEC
+
+
 def test_objects_refuse_wrong_tensors():
     """Shapes and types are looked at in front of the device."""
     import torch
