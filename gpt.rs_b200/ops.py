@@ -691,7 +691,8 @@ PAIRS_HALVES, PAIRS_NEIGHBOURS = 0, 1
 
 
 class _Step:
-    """A prepared call: keeps its tensors alive, checks that they are on the current device, and launches on the current stream."""
+    """A prepared call: keeps its tensors alive, checks that they are on the current device, and launches on the current stream, whichever that is. A graph
+    that has recorded the call needs the object for as long as it is replayed."""
 
     def _hold(self, **tensors):
         self._tensors = {k: t for k, t in tensors.items() if t is not None}
@@ -699,17 +700,28 @@ class _Step:
         if len(devices) != 1 or next(iter(devices)).type != "cuda":
             raise ValueError(f"expected CUDA tensors of one device, got {sorted(map(str, devices))}")
         self._device = next(iter(devices)).index
+        self._streams = {torch._C._cuda_getCurrentRawStream(self._device)}   # that the allocator knows of
 
     def _bind(self, fn, args, result):
         """The arguments are converted once: a step of a few microseconds on the GPU has no time for it in every call."""
         self._fn, self._result = fn, result
         self._args = tuple(a if t is ctypes.c_void_p and not isinstance(a, (int, type(None))) else t(a) for t, a in zip(fn.argtypes, args))
 
+    def _use_on(self, stream):
+        """Memory of the tensors is not given out again before what another stream has been asked for has ended, whoever drops them when."""
+        if not torch.cuda.is_current_stream_capturing():
+            for t in self._tensors.values():
+                t.record_stream(torch.cuda.current_stream())
+            self._streams.add(stream)
+
     def __call__(self):
         device = torch._C._cuda_getDevice()
         if device != self._device:
             raise ValueError(f"the tensors are on cuda:{self._device}, the current device is cuda:{device}")
-        status = self._fn(*self._args, torch._C._cuda_getCurrentRawStream(device))
+        stream = torch._C._cuda_getCurrentRawStream(device)
+        if stream not in self._streams:
+            self._use_on(stream)
+        status = self._fn(*self._args, stream)
         if status:
             check(status)
         return self._result

@@ -784,6 +784,34 @@ def test_other_streams_and_two_calls_at_once(cuda):
         assert all(torch.equal(ref, g) for g in got)
 
 
+@pytest.mark.parametrize("what", ["attention", "append", "gather", "rope"])
+def test_an_object_that_goes_away_while_its_call_runs_elsewhere(cuda, what):
+    """Memory of an object that was called on another stream is not given out again before that call has ended."""
+    c = Cache(cuda, 8, 2, 128, 2, 130, seed=5)
+    c.fill([2000, 1900])
+    slot, ctx = _ints([0, 1], cuda), _ints([2000, 1900], cuda)
+    rows = torch.zeros((2, 12 * 128), dtype=torch.bfloat16, device=cuda)
+    q = torch.zeros((2, 8, 128), dtype=torch.bfloat16, device=cuda)
+    make = {"attention": lambda: ops.Kv8Attention(c.a, q, c.pool, c.rows, c.table, slot, ctx, ctx, 2000, splits=200),
+            "append": lambda: ops.Kv8Append(c.a, None, rows, ctx, slot, _ints([0, 1], cuda), _ints([0, 1], cuda), c.table, c.pool, c.rows),
+            "gather": lambda: ops.Kv8Gather(c.a, c.pool, c.rows, c.table, slot, slot, ctx), "rope": lambda: ops.QkNormRope(ops.QkRotation(8, 2, 128), rows, None)}[what]
+    make()()                                     # (kernels are loaded)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    step = make()
+    owned = {t.data_ptr(): t.untyped_storage().nbytes() for n, t in step._tensors.items() if n in ("scratch", "out", "q", "k", "v", "status") and t is not q}
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(400_000_000)           # a fifth of a second, and then the call
+        step()
+        step()
+    del step
+    new = [torch.empty(size, dtype=torch.uint8, device=cuda) for size in list(owned.values()) * 40]
+    assert not stream.query()
+    assert not {t.data_ptr() for t in new} & set(owned)
+    torch.cuda.synchronize()
+
+
 @pytest.mark.parametrize("tiles", [None, [70, 60]])
 def test_two_graphs_of_one_cache_at_once(cuda, tiles):
     """Two objects over one cache whose parts meet in scratch, captured each and replayed side by side: either has scratch of its own."""
