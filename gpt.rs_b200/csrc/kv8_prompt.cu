@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
             if (lane == 0) {
                 float* s = scales[kb % kScaleSlots][page];
                 s[0] = k_scale * p.scale_log2;
-                s[1] = __log2f(v_scale);
+                s[1] = pg.kind == kNone ? -INFINITY : __log2f(v_scale);   // tokens of a page that is none do not count
                 s[2] = k_scale == k_scale ? __fdividef(1.f, v_scale) : k_scale;
             }
         };

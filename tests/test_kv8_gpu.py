@@ -506,6 +506,28 @@ def test_bad_entries_of_the_attention_are_reported(cuda):
             c.check(rows[:1], q[:1], out[:1])
 
 
+@pytest.mark.parametrize("tiles,splits", [(False, 1), (False, 2), (True, 1), (True, 2)])
+def test_tokens_of_a_page_that_is_none_do_not_count(cuda, tiles, splits):
+    """A page that is not there is reported, and its tokens are left out of the sums, row by row and in tiles alike."""
+    n = 300
+    for page in (-1, 1 << 30):
+        c = Cache(cuda, 32, 8, 128, 1, 20)
+        c.fill([n])
+        c.table[0, 3] = page
+        rows = [(0, p + 1) for p in range(0 if tiles else 290, n)]
+        q, out = c.attend(rows, tiles=[n] if tiles else None, splits=splits, want=False)
+        assert int(c.status) == 2
+        s, got, qn = c.seq[0], _np(out).reshape(-1, 32, 128), _np(q)
+        (k, v), vs = s.held(), s.value_scales()
+        for i, (_, end) in enumerate(rows):
+            if i % 23 and end < n - 2:
+                continue
+            at = [t for t in range(end) if t // 16 != 3]
+            w, size, unit = kr.attention(qn[i], k[at], v[at], 0, len(at), c.a.scale, vs[at])
+            off = np.abs(got[i] - w) - 2 ** -8 * np.abs(w) - (1 + 2 ** -8) * (2 ** -10 * size + 2 ** -25 * unit)
+            assert (off <= 0).all(), (end, off.max())
+
+
 @pytest.mark.parametrize("slot", [2, 1 << 30])
 @pytest.mark.parametrize("splits", [None, 2])
 def test_tiles_of_no_sequence_are_reported(cuda, slot, splits):
