@@ -904,7 +904,7 @@ class Kv8Attention(_Step):
         s.scratch_bytes = lib().gptrs_cuda_kv8_scratch_bytes(ctypes.byref(a), rows, s.n_tiles, s.splits)
         scratch = torch.empty(s.scratch_bytes, dtype=torch.uint8, device=q.device) if s.scratch_bytes else None
         s.d_scratch = None if scratch is None else scratch.data_ptr()
-        s.d_out, s.d_status, s.rows = self.out.data_ptr(), self.status.data_ptr(), rows
+        s.d_out, s.d_status, s.rows = self.out.data_ptr(), self.status.data_ptr(), rows if tiles is None or s.n_tiles else 0   # (no tile: no row is in one)
         self._hold(q=q, pool=pool, open_rows=open_rows, page_table=page_table, slot=slot, ctx_len=ctx_len, lengths=lengths, tile_row=tile_row, tile_rows=tile_rows,
                    scratch=scratch, out=self.out, status=self.status)
         self._bind(lib().gptrs_cuda_kv8_attention, (ctypes.byref(a), ctypes.byref(s)), self.out)

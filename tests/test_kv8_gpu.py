@@ -614,6 +614,14 @@ def test_rows_in_no_tile_and_tiles_that_are_none(cuda, splits, n):
         c.check([rows[r] for r in at], q[at], out[at])
 
 
+def test_no_tiles_at_all(cuda):
+    """Rows that no tile holds stay as they were, where there is no tile too."""
+    c = Cache(cuda, 8, 2, 128, 1, 4)
+    c.fill([40])
+    q, out = c.attend([(0, 5), (0, 40)], tiles=[0, 0], want=False)
+    assert (out == 3).all() and int(c.status) == 0
+
+
 def test_scores_that_grow_along_the_keys(cuda):
     """The reference of the weights has to follow: every block's scores are far above the one before, and then far below."""
     c = Cache(cuda, 32, 8, 128, 1, 72, seed=3)
