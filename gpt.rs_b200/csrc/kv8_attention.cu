@@ -583,6 +583,9 @@ int gptrs_cuda_kv8_attention(const gptrs_kv8_cache* c, const gptrs_kv8_attention
     const size_t scratch = gptrs_cuda_kv8_scratch_bytes(c, s->rows, s->n_tiles, s->splits);
     GPTRS_REQUIRE(scratch == 0 || (s->d_scratch && s->scratch_bytes >= scratch), "scratch is too small");
     if (s->rows == 0) return GPTRS_OK;
+    // (a CTA has read its rows' queries of its heads before it or the merge writes there, and nobody else reads those)
+    const char *q = static_cast<const char*>(s->d_q), *out = static_cast<const char*>(s->d_out);
+    GPTRS_REQUIRE((q == out && p.ldq == width) || out >= q + 2 * ((s->rows - 1) * p.ldq + width) || q >= out + 2 * s->rows * width, "the output lies in rows of other queries");
     p.q = static_cast<const __nv_bfloat16*>(s->d_q);
     p.pool = static_cast<const unsigned char*>(s->d_pool);
     p.open = static_cast<const __nv_bfloat16*>(s->d_open);

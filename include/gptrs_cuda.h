@@ -804,7 +804,7 @@ typedef struct {
     int64_t n_tiles;
     int64_t max_ctx_len;
     int splits;
-    void* d_out;
+    void* d_out;                       /* d_q itself, where its rows are packed, or none of its rows */
     void* d_scratch;                   /* 16-byte aligned; of one call at a time: calls and graphs that may overlap have their own */
     size_t scratch_bytes;
     int32_t* d_status;

@@ -755,6 +755,21 @@ def test_calls_without_rows(cuda):
     assert k.shape == v.shape == (0, 2, 128) and torch.equal(c.pool, before) and int(c.status) == 0
 
 
+@pytest.mark.parametrize("tiles", [False, True])
+@pytest.mark.parametrize("splits", [1, 2, 20])
+def test_output_over_the_queries(cuda, tiles, splits):
+    """The output in the place of packed queries: the same bits."""
+    c = Cache(cuda, 24, 2, 128, 1, 40, seed=splits)
+    c.fill([600])
+    rows = [(0, p + 1) for p in range(0 if tiles else 560, 600)]
+    q, out = c.attend(rows, tiles=[600] if tiles else None, splits=splits, want=False)
+    c.check(rows, q, out, every=41)
+    same = q.clone()
+    ops.kv8_attention(c.a, same, c.pool, c.rows, c.table, _ints([0] * len(rows), cuda), _ints([n for _, n in rows], cuda), c.lengths(), 600,
+                      tiles=ops.kv8_tiles(c.a, [600], cuda) if tiles else None, splits=splits, out=same.view(len(rows), -1), status=c.status)
+    assert torch.equal(same.view(len(rows), -1), out) and int(c.status) == 0
+
+
 # ---- together ----------------------------------------------------------------------------------------------------------------------
 def test_prompt_then_steps_in_a_graph(cuda):
     """A prompt, then tokens one by one as a server has them: append and attention recorded once, replayed with new rows, positions and lengths."""

@@ -137,6 +137,19 @@ def test_calls_without_rows_need_no_rows():
     assert _status("gptrs_cuda_qk_norm_rope", ctypes.byref(_rotation(dim=63)), None, 0, 0, None, None, 0, 64, 0, None) == SPEC
 
 
+def test_outputs_in_the_queries_are_refused():
+    """Rows are worked on in no order: the output may be the packed queries themselves (which this test leaves alone) or lie beside them."""
+    a, at = ops.kv8_layout(8, 2, 64), 1 << 20
+    for out, ldq in [(at + 16, 0), (at - 16, 0), (at + 1024 * 3, 512), (at - 1024 * 3 - 1008, 0), (at, 768), (at + 1024, 1024), (at + 3 * 1536 + 1008, 768)]:
+        s = _abi.Kv8AttentionStep()
+        for n in ("d_pool", "d_open", "d_page_table", "d_slot", "d_ctx_len", "d_length", "d_status"):
+            setattr(s, n, 4096)
+        s.n_pages = s.n_slots = s.max_pages = s.rows = 4
+        s.max_ctx_len, s.splits, s.d_q, s.d_out, s.ldq = 64, 1, at, out, ldq
+        assert _status("gptrs_cuda_kv8_attention", ctypes.byref(a), ctypes.byref(s), None) == SPEC, (out, ldq)
+        assert "rows of other queries" in gptrs_b200.lib().gptrs_cuda_last_error().decode()
+
+
 def test_objects_refuse_wrong_tensors():
     """Shapes and types are looked at in front of the device."""
     import torch
