@@ -204,7 +204,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) kv8_attention_kernel(const
             x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
             x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
         }
-        const float n0 = fmaxf(m0, x0 - kHeadroom), n1 = fmaxf(m1, x1 - kHeadroom);
+        // (rounded up: where a step of a score is more than 1, a reference further down would make the largest weight infinite)
+        const float n0 = fmaxf(m0, __fadd_ru(x0, -kHeadroom)), n1 = fmaxf(m1, __fadd_ru(x1, -kHeadroom));
         const float u0 = n0 == -INFINITY ? 0.f : n0, u1 = n1 == -INFINITY ? 0.f : n1;   // nothing seen yet (or nothing but NaN)
         const float a0 = kv8_exp2(m0 - u0), a1 = kv8_exp2(m1 - u1);
         m0 = n0; m1 = n1;

@@ -622,6 +622,32 @@ def test_no_tiles_at_all(cuda):
     assert (out == 3).all() and int(c.status) == 0
 
 
+@pytest.mark.parametrize("size", [1e3, 3e3, 1e4, 3e4, 1e12, 1e15])
+@pytest.mark.parametrize("tiles,splits", [(False, 1), (False, 3), (False, 20)])
+def test_scores_of_any_size(cuda, size, tiles, splits):
+    """Queries and keys so large that a step of an f32 score is many powers of two of a weight: the largest score has all of the weight."""
+    n = 400
+    c = Cache(cuda, 32, 8, 128, 1, 26, seed=9)
+    qkv = torch.randn((n, 48 * 128), device=cuda)
+    qkv[:, 32 * 128:40 * 128] *= size
+    c.append([(0, 0, n)], qkv.bfloat16())
+    rows = [(0, p + 1) for p in range(n)]
+    q = (torch.randn((n, 32, 128), device=cuda) * size).bfloat16()
+    _, out = c.attend(rows, tiles=[n] if tiles else None, q=q, splits=splits, want=False)
+    assert int(c.status) == 0
+    (k, v), qn = c.seq[0].held(), _np(q).astype(np.float64)
+    got = _np(out).reshape(n, 32, 128)
+    assert np.isfinite(got).all()
+    for i in list(range(0, n, 29)) + [n - 1]:
+        for h in range(32):
+            s = k[:i + 1, h // 4] @ qn[i, h]
+            top = np.argsort(s)[::-1]
+            if i and s[top[0]] - s[top[1]] < 2 ** -10 * np.abs(s).max():   # (f32 sums of 128 products: 2^-17 of the largest; 2^-10 of 2^20 is far more than 40)
+                continue
+            want = v[top[0], h // 4]
+            assert (np.abs(got[i, h] - want) <= 2 ** -7 * np.abs(want)).all(), (i, h)     # bf16, and as much for the weight in front and behind
+
+
 def test_scores_that_grow_along_the_keys(cuda):
     """The reference of the weights has to follow: every block's scores are far above the one before, and then far below."""
     c = Cache(cuda, 32, 8, 128, 1, 72, seed=3)
