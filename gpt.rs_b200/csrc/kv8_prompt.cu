@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
         // Halves of blocks (64 keys; steps, two of a block) that all rows of this warp see: most. Rows that are nobody's see what the others do.
         const int seen_from = __reduce_max_sync(0xffffffffu, live ? begin : 0) - first_key, seen_to = __reduce_min_sync(0xffffffffu, live ? end : 0x7fffffff) - first_key;
         const int steps = 2 * my_blocks, whole_from = max(1, (seen_from + kKeys / 2 - 1) / (kKeys / 2)), whole_to = min(steps, seen_to / (kKeys / 2));
-        float m_run = live ? -1e30f : 0.f, l_run = 0.f;
+        float m_run = live ? -3e38f : 0.f, l_run = 0.f;
         int step = 0;
         auto scores_there = [&] {   // of this step; whole warp
             if (!mbar_wait_parked(s_bar + 8u * (step & 1), (uint32_t)(step >> 1) & 1u, params.wait_limit)) failed = true;
@@ -522,9 +522,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                     for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
                     tmem_st_16(t_o + 16u * i, r);
                 }
+                asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
             };
             // Scores of a half -> weights, packed in the order of V's keys, and their share of the sum; returns whether a page's weights add up to more
-            // than keeps each an f16 (or to no number)
+            // than keeps each an f16 (or to no number). The usual way takes the reference off inside the multiply-add. Scores of 2^27 and more are rounded to steps
+            // that are exponents of their own, so where the reference has just been set it is taken off the rounded score, whose maximum it is.
             auto weigh = [&](auto all_seen, float& share) {
                 constexpr bool kWhole = decltype(all_seen)::value;
                 const int key0 = first_key + step * (kKeys / 2);
@@ -533,13 +535,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
 #pragma unroll
                 for (int pg = 0; pg < 4; ++pg) {
                     const float4 x = ld_shared_f4(sc + pg * 16);
-                    const float cq = x.x * q_scale, b = x.y - m_run;
-                    const uint64_t c2 = pair_of(cq, cq), b2 = pair_of(b, b);
+                    const float cq = x.x * q_scale, b = kWhole ? x.y - m_run : x.y;
+                    const uint64_t c2 = pair_of(cq, cq), b2 = pair_of(b, b), m2 = pair_of(-m_run, -m_run);
                     uint64_t part = 0;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {   // keys 2 i, 2 i + 1
                         const uint64_t t2 = fma2(pair_of(__uint_as_float(s[16 * pg + 2 * i]), __uint_as_float(s[16 * pg + 2 * i + 1])), c2, b2);
-                        const float2 t = split(t2);
+                        const float2 t = split(kWhole ? t2 : add2(t2, m2));
                         float2 w = make_float2(kv8_exp2(t.x), kv8_exp2(t.y));
                         if (!kWhole) {
                             const int key = key0 + 16 * pg + 2 * i;
@@ -583,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const __grid_co
                 load();   // the weights have not been stored over the scores yet
                 if (raises) raise(over);
                 over = weigh(std::false_type{}, share);
-                if (raises || !__any_sync(0xffffffffu, over)) break;
+                if (!__any_sync(0xffffffffu, over)) break;   // (behind a raise: of rows that fitted in the usual way, or that are none)
                 raises = true;
             }
             hand_over();

@@ -623,7 +623,7 @@ def test_no_tiles_at_all(cuda):
 
 
 @pytest.mark.parametrize("size", [1e3, 3e3, 1e4, 3e4, 1e12, 1e15])
-@pytest.mark.parametrize("tiles,splits", [(False, 1), (False, 3), (False, 20)])
+@pytest.mark.parametrize("tiles,splits", [(False, 1), (False, 3), (False, 20), (True, 1), (True, 2)])
 def test_scores_of_any_size(cuda, size, tiles, splits):
     """Queries and keys so large that a step of an f32 score is many powers of two of a weight: the largest score has all of the weight."""
     n = 400
