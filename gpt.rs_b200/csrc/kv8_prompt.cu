@@ -8,8 +8,8 @@
 //   S_ih[128 x 64] = Q_i . K_h^T   both operands f16 in shared memory (K-major, 128-byte swizzle), accumulator in tensor memory
 //   softmax                        warps 4 i .. 4 i + 3, a thread per row, in one pass over its scores: the reference M stays what it is until a weight would
 //                                  no longer be an f16 (a page's weights add up to more than 65504), so there is no pass for the maximum. It is set
-//                                  to 3 below a maximum: a row's largest weight is 2^3 or more, others have 11 bits down to 2^-17 of it and are off
-//                                  by at most 2^-28 of it below (the 2^20 tokens of a tail lose 2^-8 of the sum at most, as much as the result's rounding).
+//                                  to 2 below a maximum: a row's largest weight is 2^2 or more, others have 11 bits down to 2^-16 of it and are off
+//                                  by at most 2^-27 of it below (the 2^19 tokens of a tail lose 2^-8 of the sum at most, as much as the result's rounding).
 //                                  Weights go as f16 over the first 32 columns of S_ih
 //   O_i[128 x dim] += P_ih . V_h   A = P_ih from tensor memory, B = V^T in shared memory (keys contiguous), accumulator in tensor memory
 // Warps 8 - 11 widen the pages, two of a block each: bytes from global memory to registers ahead of time, f16 into the stage when the products that read
@@ -55,7 +55,7 @@ constexpr uint32_t kOCol = 256;
 constexpr float kLargestSum = 65504.f;     // of a page's weights: each is an f16 then
 // log2 of the largest weight behind a new reference: bits for the tail, which scores that grow along the keys cannot use (the reference is raised more often). us
 // of 8192 tokens, 32 / 8 heads of 128, with 0 / 2 / 3 / 4: scores with a standard deviation of 2 520 for all, of 4 542 / 556 / 581 / 620; keys of scales that differ 541 / 547 / 553 / 561.
-constexpr float kHeadroom = 3.f;
+constexpr float kHeadroom = 2.f;
 constexpr int kScaleSlots = 4;             // blocks whose scales may be in use at a time are three at most
 
 struct PromptParams {
