@@ -6,8 +6,8 @@
 // bytes in order in shared memory; for runs of one row (decode steps) with the rows in front of it in its block, from the open rows.
 // What bounds it is latency: of loads that depend on each other (slot and position; angles; open rows), so keys, values, the first queries and the angles
 // (kept in shared memory) are asked for before anything is computed, and of the arithmetic behind them. 64 single tokens, 32 / 8 heads of 128: 4.4 us; six
-// prompts of 2777 tokens, 16 / 4 heads, three axes: 58.6 us (148 MB, 39 % of the copy bandwidth; 38.6 us without the queries and the blocks; a warp
-// instruction per scheduler in 44 % of the cycles, four CTAs an SM). Measured and left: CTAs that stay and fetch ahead into L2 (62.9), CTAs for queries
+// prompts of 925 to 2777 tokens (11104 rows), 16 / 4 heads, three axes: 58.6 us (125 MB, 33 % of the copy bandwidth; 38.6 us without the queries and the blocks;
+// a warp instruction per scheduler in 44 % of the cycles, four CTAs an SM). Measured and left: CTAs that stay and fetch ahead into L2 (62.9), CTAs for queries
 // and for keys apart (65.1).
 #include <algorithm>
 
@@ -502,8 +502,8 @@ int gptrs_cuda_kv8_append(const gptrs_kv8_cache* c, const gptrs_kv8_append_step*
     p.tokens = (int)std::min<int64_t>(std::min<int64_t>(s->max_pages, 0x7fffffff) * kKv8Tokens, 0x7fffffff - kKv8Tokens + 1);   // a whole number of blocks
     // A CTA per row and kv head for lists that are short or may be single tokens, else per 16 rows: a prompt has one segment in them. Where they are single tokens
     // after all, four CTAs deal the segments among them, as long as the three that find nothing cost little. us, 32 / 8 heads of 128, per row / per 16 / four
-    // for 16: 64 single tokens 4.2 / 64 / 20, 512 14 / 66 / 44; a prompt of 256 10.9 / 7.8 / 8.4, of 1000 23 / 10.4 / 11.0, of 4 x 1000 62 / 35 / 31, of
-    // 6 x 2777 - / 105 / 120.
+    // for 16: 64 single tokens 4.2 / 64 / 20, 512 14 / 66 / 44; a prompt of 256 10.9 / 7.8 / 8.4, of 1000 23 / 10.5 / 11.2, of 4 x 1000 62 / 41 / 42, six of
+    // 925 to 2777 - / 104 / 119, 6 x 2777 - / 146 / 176.
     const bool few = s->rows <= 256 || s->rows <= s->n_slots;
     const dim3 grid((unsigned)ceil_div(s->rows, few ? 1 : kKv8Tokens), (unsigned)c->kv_heads, few || s->rows > 4096 ? 1u : 4u);
     auto kernel = c->dim == 64 ? (few ? kv8_append_kernel<64, 1> : kv8_append_kernel<64, 16>) : (few ? kv8_append_kernel<128, 1> : kv8_append_kernel<128, 16>);

@@ -11,8 +11,10 @@
 // and O^T = V^T P^T, so that little of a matrix instruction is padding. The cache's byte order makes 16 bytes of a lane two k-steps of keys, or two
 // row tiles of values. The 8 x 8 transposition between the two products is one instruction per eight tokens.
 // Four warps deal the blocks of a part of the keys among them, each with a ring of its own in shared memory that bulk copies fill (a block is one piece of
-// memory, its scales included), and merge at the end. Up to eight parts of a row and kv head (of eight of its query heads) are a cluster that merges
-// through distributed shared memory; more go through scratch and a second kernel.
+// memory, its scales included), and merge at the end. Up to eight parts of a row and kv head (of eight of its query heads) that fit into one wave
+// of CTAs are a cluster that merges through distributed shared memory; others go through scratch and a second kernel. Parts are cut by the bound of the
+// lengths that the caller gives, so a bound far above a row's length leaves it fewer of them: one sequence of 1500 tokens, 32 / 8 heads of 128, takes 8.1 us with a
+// bound of 1504, 14.6 with 32768 and 20.0 with 131072; 64 of 512 to 8192 104 us with 8192 and 123 with 131072.
 #include <algorithm>
 #include <type_traits>
 
@@ -48,7 +50,7 @@ __device__ __forceinline__ void parts_of(const Kv8Attention& p, const Kv8Span& s
     *parts = (*blocks + *per - 1) / *per;
 }
 
-// The same for few parts: dim / 4 threads have a row's head to themselves.
+// Merges few parts (eight at most, see kv8_merge_kernel for more): dim / 4 threads have a row's head to themselves.
 template <int kDim>
 __global__ void __launch_bounds__(256) kv8_merge_few_kernel(const Kv8Attention p) {
     pdl_launch_dependents();

@@ -18,8 +18,9 @@
 // order. Warps 12 and 13 issue the products of a row tile each: behind P_ih come O_i += P_ih . V_h and the next block's S_ih, while the softmax is at the
 // other half. One thread for both tiles had the one wait for the other's weights (547 us for the prompt below).
 //
-// One prompt of 8192 tokens, 32 / 8 heads of 128: 521 us, 1055 TFLOP/s (64 % of what a large bf16 product of the library reaches); 500 tokens behind
-// 32768: 288 us; seven ragged prompts of 91 - 1777 tokens, 12 heads of 64: 59.5 us. What bounds long ones is the softmax warps' chain: a half takes a warp
+// One prompt of 8192 tokens, 32 / 8 heads of 128: 521 us, 1055 TFLOP/s (64 % of what a large bf16 product of the library reaches), where the reference is hardly
+// ever raised, 552 us where blocks' scales and scores scatter widely; 500 tokens behind 32768 282 and 311 us; seven ragged prompts of 91 - 1777 tokens, 12 heads
+// of 64: 54.5 us. What bounds long ones is the softmax warps' chain: a half takes a warp
 // about 1700 cycles (1150 of weights, 230 until the scores are seen, 150 of storing them), of which the special function unit needs 512 for each of the two
 // warps of a scheduler; it issues in 39 % of the cycles, a third of that for the loaders, and the tensor pipe is busy for 38 %. Short ones pay 8.5 us per CTA
 // beside their keys: 2 of loads that depend on each other (tile, slot, length), 2 until the first scores, 2 for these (maximum and masks), 1.5 for the

@@ -2,7 +2,8 @@
 //
 // With gains g and angles (c, s), out_a = x_a r g_a c - x_b r g_b s and out_b = x_b r g_b c + x_a r g_a s, r = 1 / rms of the head. Every value is read and
 // written once; sums of squares are f32, the result is rounded once. 9001 rows of 32 + 8 + 8 heads of 128 in bf16 on three axes: 43.4 us (28.2 at the copy
-// bandwidth for the queries and keys alone, which are all that is written in place; a plain copy of the same bytes takes 35).
+// bandwidth for the queries and keys alone; a plain copy of the same bytes takes 35). In place only queries and keys are written; the ring reads the
+// values beside them all the same, since a row is one piece.
 //
 // Three kernels. qk_norm_rope_ring_kernel streams rows through shared memory. qk_norm_rope_wide_kernel holds them in registers: a warp takes some heads of one
 // kind (queries, keys, values) of a row, a group of its lanes a head at a time, kVec pairs a lane, so that loads and stores are 16 bytes a lane; the four

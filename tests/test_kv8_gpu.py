@@ -877,7 +877,7 @@ def test_an_object_that_goes_away_while_its_call_runs_elsewhere(cuda, what):
         step()
         step()
     del step
-    new = [torch.empty(size, dtype=torch.uint8, device=cuda) for size in list(owned.values()) * 40]
+    new = [torch.empty(size, dtype=torch.uint8, device=cuda) for size in list(owned.values()) * 400]
     assert not stream.query()
     assert not {t.data_ptr() for t in new} & set(owned)
     torch.cuda.synchronize()
