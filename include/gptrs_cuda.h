@@ -787,8 +787,8 @@ int gptrs_cuda_kv8_gather(const gptrs_kv8_cache* c, const void* d_pool, int64_t 
  * n_tiles = 0: every row by itself (single tokens of many sequences); else tile i is the rows tile_row[i] .. + tile_rows[i], at most tile_tokens
  * rows of one sequence at consecutive positions (prompts, chunks of prompts); rows in no tile are left as they were, no row is in two. Tiles are
  * begun from the last one on. The keys of a row or tile are read in at most `splits` parts (gptrs_cuda_kv8_splits; scratch:
- * gptrs_cuda_kv8_scratch_bytes), which are cut by max_ctx_len, a bound of ctx_len: the nearer it is to the lengths, the more parts each row has. *d_status = 2: a length, slot or page out of range (tokens of such a page do
- * not count), 3: a bounded wait ran out. */
+ * gptrs_cuda_kv8_scratch_bytes), which are cut by max_ctx_len, a bound of ctx_len: the nearer it is to the lengths, the more parts each row has.
+ * *d_status = 2: a length, slot or page out of range (tokens of such a page do not count), 3: a bounded wait ran out. */
 typedef struct {
     const void* d_q;                   /* [rows][q_heads][dim], rows ldq apart (0 = packed) */
     int64_t ldq;

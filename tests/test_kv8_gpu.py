@@ -785,7 +785,7 @@ def test_calls_without_rows(cuda):
 @pytest.mark.parametrize("splits", [1, 2, 20])
 def test_output_over_the_queries(cuda, tiles, splits):
     """The output in the place of packed queries: the same bits."""
-    c = Cache(cuda, 24, 2, 128, 1, 40, seed=splits)
+    c = Cache(cuda, 20, 2, 128, 1, 40, seed=splits)
     c.fill([600])
     rows = [(0, p + 1) for p in range(0 if tiles else 560, 600)]
     q, out = c.attend(rows, tiles=[600] if tiles else None, splits=splits, want=False)

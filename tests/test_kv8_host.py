@@ -140,7 +140,7 @@ def test_calls_without_rows_need_no_rows():
 def test_outputs_in_the_queries_are_refused():
     """Rows are worked on in no order: the output may be the packed queries themselves (which this test leaves alone) or lie beside them."""
     a, at = ops.kv8_layout(8, 2, 64), 1 << 20
-    for out, ldq in [(at + 16, 0), (at - 16, 0), (at + 1024 * 3, 512), (at - 1024 * 3 - 1008, 0), (at, 768), (at + 1024, 1024), (at + 3 * 1536 + 1008, 768)]:
+    for out, ldq in [(at + 16, 0), (at - 16, 0), (at + 1024 * 2, 512), (at - 1024 * 2 - 1008, 0), (at, 768), (at + 1024, 1024), (at + 3 * 1536 + 1008, 768)]:
         s = _abi.Kv8AttentionStep()
         for n in ("d_pool", "d_open", "d_page_table", "d_slot", "d_ctx_len", "d_length", "d_status"):
             setattr(s, n, 4096)
