@@ -190,6 +190,39 @@ class Kv8AttentionStep(ctypes.Structure):
          ("scratch_bytes", ctypes.c_size_t), ("d_status", ctypes.c_void_p), ("rows", ctypes.c_int64)]
 
 
+class DraftTrees(ctypes.Structure):
+    """gptrs_draft_trees."""
+    _fields_ = [(n, ctypes.c_int) for n in ("q_heads", "kv_heads", "dim", "max_nodes")] + [("scale", ctypes.c_float)] + \
+        [(n, ctypes.c_void_p) for n in ("d_first", "d_slot", "d_length", "d_parent")] + [("n_trees", ctypes.c_int64), ("rows", ctypes.c_int64), ("d_page_table", ctypes.c_void_p)] + \
+        [(n, ctypes.c_int64) for n in ("n_slots", "max_pages", "n_pages")]
+
+
+class TreeAppendStep(ctypes.Structure):
+    """gptrs_tree_append_step."""
+    _fields_ = [("d_qkv", ctypes.c_void_p), ("ld", ctypes.c_int64), ("d_cos", ctypes.c_void_p), ("d_sin", ctypes.c_void_p), ("rotary_dim", ctypes.c_int64),
+                ("positions", ctypes.c_int64), ("d_q", ctypes.c_void_p), ("d_pool", ctypes.c_void_p), ("d_status", ctypes.c_void_p)]
+
+
+class TreeAttentionStep(ctypes.Structure):
+    """gptrs_tree_attention_step."""
+    _fields_ = [("d_q", ctypes.c_void_p), ("ldq", ctypes.c_int64), ("d_pool", ctypes.c_void_p), ("d_out", ctypes.c_void_p), ("d_scratch", ctypes.c_void_p),
+                ("scratch_bytes", ctypes.c_size_t), ("d_status", ctypes.c_void_p)]
+
+
+class TreeAcceptStep(ctypes.Structure):
+    """gptrs_tree_accept_step."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_token", "d_pick", "d_pools")] + [("n_layers", ctypes.c_int64)] + \
+        [(n, ctypes.c_void_p) for n in ("d_count", "d_path", "d_next", "d_new_length", "d_status")]
+
+
+class VocabScores(ctypes.Structure):
+    """gptrs_vocab_scores."""
+    _fields_ = [("d_hidden", ctypes.c_void_p), ("ldh", ctypes.c_int64), ("d_weight", ctypes.c_void_p), ("ldw", ctypes.c_int64), ("rows", ctypes.c_int64),
+                ("dim", ctypes.c_int64), ("vocab", ctypes.c_int64), ("d_bias", ctypes.c_void_p), ("soft_cap", ctypes.c_float), ("temperature", ctypes.c_float),
+                ("seed", ctypes.c_uint32)] + [(n, ctypes.c_void_p) for n in ("d_seed", "d_target", "d_pick", "d_pick_logprob", "d_logprob", "d_lse", "d_scratch")] + \
+        [("scratch_bytes", ctypes.c_size_t), ("d_status", ctypes.c_void_p)]
+
+
 def prototypes(header_text: str | None = None) -> dict[str, tuple[str, list[str]]]:
     """Returns {name: (return type, [parameter declarations])} for every exported function."""
     text = header_text if header_text is not None else HEADER.read_text()

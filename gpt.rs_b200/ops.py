@@ -5,6 +5,7 @@ torch kernel runs on behalf of these functions except output allocation.
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -912,3 +913,159 @@ class Kv8Attention(_Step):
 
 def kv8_attention(*args, **kw):
     return Kv8Attention(*args, **kw)()
+
+
+# ---- trees of drafted tokens over the paged bf16 cache, scores against a vocabulary -------------------------------------------
+class DraftTrees:
+    """The drafted tokens of a step (gptrs_draft_trees): tree s is the rows first[s] .. first[s + 1] - 1 of a call, behind the length[s] tokens that the sequence of
+    slot[s] (negative: padding) has in the cache; parent[row] is the number of a node's parent in its tree, -1: it has none. All int32; no slot is in two trees. The
+    calls below read them when they run, so a loop keeps one object and writes its next trees into the same tensors."""
+
+    def __init__(self, q_heads, kv_heads, first, slot, length, parent, page_table, max_nodes, scale=0.0, dim=128):
+        n = slot.shape[0]
+        t = self.struct = _abi.DraftTrees(q_heads, kv_heads, dim, max_nodes, scale)
+        self.n_trees, self.rows = n, parent.shape[0]
+        self.tensors = dict(first=_need(first, "first", torch.int32, n + 1), slot=_need(slot, "slot", torch.int32, n), length=_need(length, "length", torch.int32, n),
+                            parent=_need(parent, "parent", torch.int32, None), page_table=_need(page_table, "page_table", torch.int32, None, None))
+        t.d_first, t.d_slot, t.d_length, t.d_parent, t.d_page_table = (self.tensors[k].data_ptr() for k in ("first", "slot", "length", "parent", "page_table"))
+        t.n_trees, t.rows, t.n_slots, t.max_pages = n, self.rows, page_table.shape[0], page_table.shape[1]
+
+    def over(self, pool):
+        """The arguments of a call over a pool of that size."""
+        t = _abi.DraftTrees.from_buffer_copy(self.struct)
+        _need(pool, "pool", torch.uint8, None)
+        page = kv_pool_bytes(1, t.kv_heads, t.dim)
+        if page == 0 or pool.numel() == 0 or pool.numel() % page:
+            raise ValueError(f"pool: {pool.numel()} bytes are no whole number of pages of {page} bytes")
+        t.n_pages = pool.numel() // page
+        return t
+
+
+class TreeAppend(_Step):
+    """gptrs_cuda_tree_append: rows bf16 [rows][queries | keys | values] -> rotated queries [rows][heads][128]; keys and values into the pool. Tables cos / sin f32
+    [positions][rotary_dim / 2], None: nothing turns."""
+
+    def __init__(self, trees, qkv, cos, sin, pool, q=None, status=None):
+        t = self.t = trees.over(pool)
+        s = self.step = _abi.TreeAppendStep()
+        if qkv.shape[0] != trees.rows:
+            raise ValueError(f"qkv has {qkv.shape[0]} rows, the trees {trees.rows}")
+        self.q = torch.empty((trees.rows, t.q_heads, t.dim), dtype=torch.bfloat16, device=qkv.device) if q is None else _need(q, "q", torch.bfloat16, trees.rows, t.q_heads, t.dim)
+        self.status = _status(qkv.device, status)
+        s.d_qkv, s.ld = _rows_of(qkv, "qkv", (t.q_heads + 2 * t.kv_heads) * t.dim, (torch.bfloat16,))
+        if cos is not None:
+            _need(cos, "cos", torch.float32, None, None)
+            _need(sin, "sin", torch.float32, *cos.shape)
+            s.d_cos, s.d_sin, s.positions, s.rotary_dim = cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1]
+        s.d_q, s.d_pool, s.d_status = self.q.data_ptr(), pool.data_ptr(), self.status.data_ptr()
+        self._hold(qkv=qkv, cos=cos, sin=sin, pool=pool, q=self.q, status=self.status, **trees.tensors)
+        self._bind(lib().gptrs_cuda_tree_append, (ctypes.byref(t), ctypes.byref(s)), self.q)
+
+
+def tree_append(*args, **kw):
+    return TreeAppend(*args, **kw)()
+
+
+class TreeAttention(_Step):
+    """gptrs_cuda_tree_attention: q [rows][heads][128] (rows may lie a stride apart) -> out [rows][heads * 128]. The object owns its scratch: calls that may overlap (two
+    streams, two graphs) need one object each."""
+
+    def __init__(self, trees, q, pool, out=None, status=None):
+        t, rows = trees.over(pool), trees.rows
+        self.t = t
+        s = self.step = _abi.TreeAttentionStep()
+        if q.dtype != torch.bfloat16 or q.shape != (rows, t.q_heads, t.dim) or q.stride(2) != 1 or q.stride(1) != t.dim or (rows > 1 and q.stride(0) < t.q_heads * t.dim):
+            raise ValueError(f"q: expected bf16 [{rows}][{t.q_heads}][{t.dim}], got {q.dtype} {list(q.shape)} with strides {q.stride()}")
+        self.out = torch.empty((rows, t.q_heads * t.dim), dtype=torch.bfloat16, device=q.device) if out is None else _need(out, "out", torch.bfloat16, rows, t.q_heads * t.dim)
+        self.status = _status(q.device, status)
+        s.scratch_bytes = lib().gptrs_cuda_tree_scratch_bytes(ctypes.byref(t))
+        scratch = torch.empty(s.scratch_bytes, dtype=torch.uint8, device=q.device) if s.scratch_bytes else None
+        s.d_q, s.ldq = q.data_ptr(), q.stride(0) if rows > 1 else t.q_heads * t.dim
+        s.d_pool, s.d_out, s.d_scratch, s.d_status = pool.data_ptr(), self.out.data_ptr(), None if scratch is None else scratch.data_ptr(), self.status.data_ptr()
+        self._hold(q=q, pool=pool, out=self.out, scratch=scratch, status=self.status, **trees.tensors)
+        self._bind(lib().gptrs_cuda_tree_attention, (ctypes.byref(t), ctypes.byref(s)), self.out)
+
+
+def tree_attention(*args, **kw):
+    return TreeAttention(*args, **kw)()
+
+
+class Accepted(NamedTuple):
+    count: torch.Tensor    # [trees]: nodes of the accepted path
+    path: torch.Tensor     # [trees][max_nodes]: their numbers, -1 behind them
+    next: torch.Tensor     # [trees]: the pick behind the last one, -1 where there is none
+    length: torch.Tensor   # [trees]: tokens that the cache then holds
+
+
+class TreeAccept(_Step):
+    """gptrs_cuda_tree_accept: tokens and picks int32 [rows] -> Accepted; the path's keys and values move to their places in `pools`, the layers' pools (of one size;
+    none: nothing moves)."""
+
+    def __init__(self, trees, token, pick, pools=(), status=None):
+        n, dev = trees.n_trees, token.device
+        pools = list(pools)
+        t = self.t = trees.over(pools[0]) if pools else _abi.DraftTrees.from_buffer_copy(trees.struct)
+        if not pools:
+            t.n_pages = 1
+        if len({p.data_ptr() for p in pools}) != len(pools):
+            raise ValueError("a pool is in the list twice")
+        for i, p in enumerate(pools):
+            _need(p, f"pools[{i}]", torch.uint8, pools[0].shape[0])
+        s = self.step = _abi.TreeAcceptStep()
+        self.result = Accepted(*(torch.empty(shape, dtype=torch.int32, device=dev) for shape in ((n,), (n, t.max_nodes), (n,), (n,))))
+        self.status = _status(dev, status)
+        s.d_token, s.d_pick = _need(token, "token", torch.int32, trees.rows).data_ptr(), _need(pick, "pick", torch.int32, trees.rows).data_ptr()
+        at = torch.tensor([p.data_ptr() for p in pools], dtype=torch.int64, device=dev) if pools else None
+        s.d_pools, s.n_layers = None if at is None else at.data_ptr(), len(pools)
+        s.d_count, s.d_path, s.d_next, s.d_new_length = (r.data_ptr() for r in self.result)
+        s.d_status = self.status.data_ptr()
+        self._hold(token=token, pick=pick, at=at, status=self.status, **dict(zip(Accepted._fields, self.result)), **{f"pool{i}": p for i, p in enumerate(pools)},
+                   **{f"trees.{k}": v for k, v in trees.tensors.items()})
+        self._bind(lib().gptrs_cuda_tree_accept, (ctypes.byref(t), ctypes.byref(s)), self.result)
+
+
+def tree_accept(*args, **kw):
+    return TreeAccept(*args, **kw)()
+
+
+class Scores(NamedTuple):
+    pick: torch.Tensor                 # [rows] int32: the largest logit's token, or a drawn one
+    pick_logprob: torch.Tensor         # [rows] f32
+    logprob: torch.Tensor | None       # [rows] f32: of the targets
+    lse: torch.Tensor                  # [rows] f32: log sum exp of the logits
+
+
+class VocabScores(_Step):
+    """gptrs_cuda_vocab_scores: hidden bf16 [rows][dim] against weight bf16 [vocab][dim] (rows of both may lie a stride apart) -> Scores, without logits in
+    memory. bias f32 [vocab]; target int32 [rows] (negative: none); temperature 0: greedy. seed: a number, or an int32 CUDA tensor of one element that is read when the
+    call runs. The object owns its scratch: calls that may overlap need one object each."""
+
+    def __init__(self, hidden, weight, target=None, bias=None, soft_cap=0.0, temperature=0.0, seed=0, status=None):
+        rows, dim, dev = hidden.shape[0], hidden.shape[1], hidden.device
+        s = self.step = _abi.VocabScores()
+        s.d_hidden, s.ldh = _rows_of(hidden, "hidden", dim, (torch.bfloat16,))
+        s.d_weight, s.ldw = _rows_of(weight, "weight", dim, (torch.bfloat16,))
+        s.rows, s.dim, s.vocab, s.soft_cap, s.temperature = rows, dim, weight.shape[0], soft_cap, temperature
+        seeds = seed if isinstance(seed, torch.Tensor) else None
+        if seeds is None:
+            s.seed = seed & 0xffffffff
+        else:
+            s.d_seed = _need(seeds, "seed", torch.int32, 1).data_ptr()
+        if bias is not None:
+            s.d_bias = _need(bias, "bias", torch.float32, s.vocab).data_ptr()
+        if target is not None:
+            s.d_target = _need(target, "target", torch.int32, rows).data_ptr()
+        floats = [torch.empty(rows, device=dev) for _ in range(3)]
+        self.result = Scores(torch.empty(rows, dtype=torch.int32, device=dev), floats[0], None if target is None else floats[1], floats[2])
+        s.d_pick, s.d_pick_logprob, s.d_logprob, s.d_lse = (None if r is None else r.data_ptr() for r in self.result)
+        self.status = _status(dev, status)
+        s.d_status = self.status.data_ptr()
+        s.scratch_bytes = lib().gptrs_cuda_vocab_scores_scratch_bytes(ctypes.byref(s))
+        scratch = torch.empty(s.scratch_bytes, dtype=torch.uint8, device=dev) if s.scratch_bytes else None
+        s.d_scratch = None if scratch is None else scratch.data_ptr()
+        self._hold(hidden=hidden, weight=weight, target=target, bias=bias, seeds=seeds, scratch=scratch, status=self.status, **dict(zip(Scores._fields, self.result)))
+        self._bind(lib().gptrs_cuda_vocab_scores, (ctypes.byref(s),), self.result)
+
+
+def vocab_scores(*args, **kw):
+    return VocabScores(*args, **kw)()

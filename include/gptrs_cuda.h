@@ -815,6 +815,102 @@ size_t gptrs_cuda_kv8_scratch_bytes(const gptrs_kv8_cache* c, int64_t rows, int6
 int gptrs_cuda_kv8_attention(const gptrs_kv8_cache* c, const gptrs_kv8_attention_step* s, void* stream);
 
 /* ==============================================================================================
+ * Trees of drafted tokens over the paged bf16 cache (no counterpart in gpt.rs, which generates token by token, inference/generate.rs): the rows of
+ * a step in which several tokens of a sequence are verified at once. Tree s is the rows d_first[s] .. d_first[s + 1] - 1 of the call, its nodes. Node i
+ * has the parent d_parent[row] < i, a node of the same tree, or -1; depth(i) = 0 without a parent, else depth(parent) + 1. The sequence of the
+ * tree has d_length[s] tokens in the cache, through page_table[d_slot[s]]. Node i lies behind them at position length + i, is rotated by
+ * position length + depth(i), and sees those tokens, its ancestors and itself. What is appended of a tree can be overwritten: the cache counts as holding length tokens
+ * until a caller says otherwise.
+ * A tree with a negative slot is padding: nothing of it is read or written but what gptrs_cuda_tree_accept says. *d_status = 2: a slot, d_first, a length or a number of
+ * nodes out of range (more than max_nodes, or behind position 16 max_pages): that tree counts as padding; a parent out of range: it counts as -1;
+ * a page out of range: its tokens are not written, not moved, and not seen. Waits inside the kernels are bounded (3).
+ * ============================================================================================ */
+typedef struct {
+    int q_heads, kv_heads, dim;        /* dim 128; at most 32 query heads per kv head */
+    int max_nodes;                     /* of a tree, 1 .. 256 */
+    float scale;                       /* of the scores; 0 = 1 / sqrt(dim) */
+    const int32_t* d_first;            /* [n_trees + 1] */
+    const int32_t *d_slot, *d_length;  /* [n_trees] */
+    const int32_t* d_parent;           /* [rows] */
+    int64_t n_trees, rows;
+    const int32_t* d_page_table;       /* [n_slots][max_pages] */
+    int64_t n_slots, max_pages, n_pages;
+} gptrs_draft_trees;
+/* Projection rows [queries | keys | values] (bf16, ld apart, 0 = packed) -> rotated queries in d_q [rows][q_heads][dim], rotated keys, and values, into
+ * the pool. Tables cos / sin f32 [positions][rotary_dim / 2] (half-split pairing; rotary_dim a multiple of 16, the channels behind it stay; 0: none
+ * turns). A position outside the tables: 2 in *d_status, turned by position 0. */
+typedef struct {
+    const void* d_qkv;
+    int64_t ld;
+    const float *d_cos, *d_sin;
+    int64_t rotary_dim, positions;
+    void* d_q;                         /* not in d_qkv's rows */
+    void* d_pool;
+    int32_t* d_status;
+} gptrs_tree_append_step;
+int gptrs_cuda_tree_append(const gptrs_draft_trees* t, const gptrs_tree_append_step* s, void* stream);
+/* out [rows][q_heads][dim] (bf16) = softmax over what the node sees . values. A node that sees nothing (its pages are out of range) gives zeros. Keys and values of nodes
+ * that a node does not see do not touch it, whatever they are. Scratch: gptrs_cuda_tree_scratch_bytes, 16-byte aligned, of one call at a time: calls and graphs
+ * that may overlap have their own. */
+typedef struct {
+    const void* d_q;                   /* [rows][q_heads][dim], rows ldq apart (0 = packed) */
+    int64_t ldq;
+    const void* d_pool;
+    void* d_out;                       /* in none of d_q's rows */
+    void* d_scratch;
+    size_t scratch_bytes;
+    int32_t* d_status;
+} gptrs_tree_attention_step;
+size_t gptrs_cuda_tree_scratch_bytes(const gptrs_draft_trees* t);
+int gptrs_cuda_tree_attention(const gptrs_draft_trees* t, const gptrs_tree_attention_step* s, void* stream);
+/* The path through every tree that its picks agree with: node 0 (the token that the step before chose), then the child with the lowest number whose d_token is
+ * d_pick of its parent (what the model says behind it, greedy or sampled), until there is none. d_count[s] = nodes of the path, d_path[s][max_nodes] = their numbers
+ * and -1 behind them, d_next[s] = the last one's pick, d_new_length[s] = length + count (not d_length itself). In each of n_layers pools the
+ * keys and values of the path's k-th node move from position length + path[k] to length + k; d_pools is an array in device memory, n_layers 0: nothing moves. A tree
+ * without nodes, or padding: count 0, path and next -1, the length as it is. */
+typedef struct {
+    const int32_t *d_token, *d_pick;   /* [rows] */
+    void* const* d_pools;
+    int64_t n_layers;
+    int32_t *d_count, *d_path, *d_next, *d_new_length;
+    int32_t* d_status;
+} gptrs_tree_accept_step;
+int gptrs_cuda_tree_accept(const gptrs_draft_trees* t, const gptrs_tree_accept_step* s, void* stream);
+
+/* ==============================================================================================
+ * Scores of rows against a vocabulary without logits in memory (the reference's samplers read them, inference/sampler.rs:35-52): z = hidden . weight^T (+ bias), then
+ * cap tanh(z / cap) where soft_cap > 0, and of every row
+ *     lse          log sum exp z
+ *     logprob      z[target] - lse, the target's log-probability (the cross entropy with its sign turned); a negative target: 0; one behind the vocabulary: NaN and 2 in *d_status
+ *     pick         the largest z (the first of equals), or with temperature > 0 the largest z / temperature + g, a draw from softmax(z / temperature):
+ *                  g = -log(-log(1 - v)), v = (h + 1/2) / 2^32 in f32, h = mix(seed ^ mix(token + 0x9e3779b9 (row + 1))) with the 32-bit mix
+ *                  x ^= x >> 16, x *= 0x7feb352d, x ^= x >> 15, x *= 0x846ca68b, x ^= x >> 16
+ *     pick_logprob z[pick] - lse
+ * Every result is left out where its pointer is null. bf16 operands, products summed in f32. A token whose bias is -inf has no probability; NaN in a row's hidden
+ * state makes its lse and log-probabilities NaN, and its pick a token of the vocabulary. dim and both strides are multiples of 8, hidden and weight 16-byte aligned. Waits inside the kernel are bounded (3
+ * in *d_status).
+ * ============================================================================================ */
+typedef struct {
+    const void* d_hidden;              /* bf16 [rows][dim], ldh apart (0 = packed) */
+    int64_t ldh;
+    const void* d_weight;              /* bf16 [vocab][dim], ldw apart (0 = packed) */
+    int64_t ldw;
+    int64_t rows, dim, vocab;
+    const float* d_bias;               /* [vocab] or NULL */
+    float soft_cap, temperature;
+    uint32_t seed;
+    const uint32_t* d_seed;            /* NULL, or one word that takes seed's place, read when the kernel runs (a graph draws anew) */
+    const int32_t* d_target;           /* [rows] or NULL */
+    int32_t* d_pick;
+    float *d_pick_logprob, *d_logprob, *d_lse;
+    void* d_scratch;                   /* of one call at a time, 16-byte aligned */
+    size_t scratch_bytes;
+    int32_t* d_status;
+} gptrs_vocab_scores;
+size_t gptrs_cuda_vocab_scores_scratch_bytes(const gptrs_vocab_scores* s);
+int gptrs_cuda_vocab_scores(const gptrs_vocab_scores* s, void* stream);
+
+/* ==============================================================================================
  * Row-wise functionals.
  * ============================================================================================ */
 /* hidden[T][D] (f32) += delta (optional, f32 or bf16), then rms_norm
