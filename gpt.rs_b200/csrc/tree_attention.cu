@@ -647,18 +647,37 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
-// Joins the parts of the items in which a group begins: one CTA per (group, tile, 32 rows, 64 channels); the first group that begins inside an item does it.
+// Joins the parts of the items in which a group begins. A piece of work is (group, tile, 32 rows, 64 channels); a CTA looks at all of its own at once, most of which are
+// none (a CTA for each of them: 14 us for one tree, where this takes 5).
 constexpr int kJoinThreads = 256;
+__device__ __forceinline__ void join_part(const AttentionParams& p, const Part& item, int j, int tile_of_group, int quarter, int half, __nv_bfloat16 (*s_out)[64 + 8]);
 __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_constant__ AttentionParams p) {
     __shared__ __align__(16) __nv_bfloat16 s_out[32][64 + 8];
+    __shared__ Part s_items[32];
     pdl_launch_dependents();
     pdl_wait();
-    const int j = blockIdx.x + 1, half = blockIdx.y & 1, quarters = p.row_cap / 32, quarter = (blockIdx.y >> 1) % quarters, tile_of_group = (blockIdx.y >> 1) / quarters;
-    const Part item = p.begins[j];
-    if (item.last < 0) return;
+    const int per_group = p.tiles * (p.row_cap / 32) * 2, all = (p.groups - 1) * per_group;
+    for (int w0 = blockIdx.x; w0 < all; w0 += 32 * gridDim.x) {
+        if (threadIdx.x < 32) {
+            const int w = w0 + threadIdx.x * gridDim.x;
+            Part item = {-1};
+            if (w < all) item = p.begins[w / per_group + 1];
+            s_items[threadIdx.x] = item;
+        }
+        __syncthreads();
+        for (int i = 0; i < 32; ++i) {
+            const int w = w0 + i * gridDim.x, j = w / per_group + 1, y = w % per_group;
+            if (w >= all) break;
+            if (s_items[i].last < 0) continue;
+            join_part(p, s_items[i], j, (y >> 1) / (p.row_cap / 32), (y >> 1) % (p.row_cap / 32), y & 1, s_out);
+        }
+        __syncthreads();
+    }
+}
+__device__ __forceinline__ void join_part(const AttentionParams& p, const Part& item, int j, int tile_of_group, int quarter, int half, __nv_bfloat16 (*s_out)[64 + 8]) {
     const int tile = item.round * p.tiles + tile_of_group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = quarter * 32 + lane;
     const int rows = min(p.tile_nodes, item.nodes - tile * p.tile_nodes) * p.t.group;
-    if (quarter * 32 >= rows) return;
+    if (quarter * 32 >= rows) return;   // the whole CTA
     const bool live = row < rows;
     auto slot = [&](int k) { return 2 * ((size_t)k * p.tiles + tile_of_group) + (k == j - 1 ? 1 : 0); };
     float top = -INFINITY, l = 0.f;
@@ -702,6 +721,7 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
     if (rr < rows)
         *reinterpret_cast<uint4*>(p.out + ((long long)(item.row0 + tile * p.tile_nodes + rr / p.t.group) * p.t.q_heads + item.head * p.t.group + rr % p.t.group) * kTreeDim + 64 * half +
                                   8 * (threadIdx.x & 7)) = *reinterpret_cast<const uint4*>(&s_out[r][8 * (threadIdx.x & 7)]);
+    __syncthreads();
 }
 
 // The pool as rows of a token and head of 256 bytes (z), two halves (y) of 64 channels (x); a block (page, kv head, keys or values) begins at row
@@ -797,7 +817,7 @@ int gptrs_cuda_tree_attention(const gptrs_draft_trees* t, const gptrs_tree_atten
     // the second kernel waits for the first one itself (griddepcontrol.wait), so it may be launched ahead of its end
     const int pdl = g_use_pdl;
     g_use_pdl = 1;
-    const int joined = launch_kernel(tree_join_kernel, dim3((unsigned)(p.groups - 1), (unsigned)(p.row_cap / 32 * 2 * p.tiles)), dim3(kJoinThreads), 0, as_stream(stream), 1, p);
+    const int joined = launch_kernel(tree_join_kernel, dim3((unsigned)(8 * sm_count())), dim3(kJoinThreads), 0, as_stream(stream), 1, p);
     g_use_pdl = pdl;
     return joined;
 }

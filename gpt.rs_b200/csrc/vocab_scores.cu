@@ -1,116 +1,333 @@
 // Scores of rows against a vocabulary without logits in memory: log sum exp, log-probabilities of given tokens, greedy or sampled picks.
 //
-// A row's result is put together from parts of the vocabulary: (m, l) with sum exp z = l exp m, the best token with its z, the target's z. Parts are
-// joined in their order by a second kernel, so results do not depend on which CTA is done first.
-#include "common.cuh"
+// z = x . w^T on the tcgen05 tensor cores, x rows as the M side: a CTA (one per SM) takes a unit, a tile of 128 rows x a stretch of the vocabulary, and walks over it in
+// tiles of 256 tokens. What a row needs to know of its logits is a running state in registers (maximum and sum, best token, the target's logit), so a logit lives
+// from the accumulator to the exponential and nowhere else.
+//   warps 0 - 7   a thread per row and half of the tile's tokens. The accumulator in tensor memory is read out every 128 of dim and added up in f32 registers: the tensor
+//                 cores cut what does not fit into the sum that they add to, 16 products at a time, which over all of dim would cost log-probabilities five digits
+//   warp 8        requests stages of 64 of dim: 128 rows of x, up to 256 of w (in copies of `box` rows, so that a stretch may end anywhere and nothing behind it is read)
+//   warp 9        one thread issues the products into one of two accumulators
+// Units go row tile first, so that the CTAs that run at one time share stretches of w through L2. A second kernel joins the parts of a row; it compares tokens where
+// values are equal, so results do not depend on an order.
+// Every wait is bounded: on a timeout code 3 goes to the status word, the roles leave their loops, tensor memory is freed.
+#include "umma_common.cuh"
 
 namespace gptrs {
+
+void prefill_tc_fault(int* starve, uint32_t* wait_limit);   // the test switch of paged_prefill_tc.cu
+
 namespace {
 
-constexpr int kTile = 64, kStep = 32, kThreads = 256;
+constexpr int kRows = 128, kCols = 256;         // of a tile
+constexpr int kStageDim = 64;                   // bf16 of a 128-byte swizzle span
+constexpr int kDrain = 2;                       // stages that an accumulator adds up
+constexpr int kStages = 4;
+constexpr int kABytes = kRows * 128, kStageBytes = kABytes + kCols * 128;
+constexpr int kEpilogue = 256, kThreads = kEpilogue + 64;
+constexpr size_t kSmem = (size_t)kStages * kStageBytes + 1024;
+constexpr uint32_t kTmemCols = 2 * kCols;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kJoinThreads = 256;
 
-struct Part { float m, l, best, z; int token; float given; };   // of a row and a part of the vocabulary; token -1, given NaN: none in it
+struct __align__(32) Part { float m, l, best, z; int token; float given; float pad[2]; };   // of a row and a stretch: sum exp z = l exp m, the best token (-1: none) and its z, the target's z (NaN: not here)
 
 struct ScoreParams {
-    const __nv_bfloat16 *x, *w;
-    long long ldx, ldw;
+    CUtensorMap x_map, w_map;
     const float* bias;
     const uint32_t* seed_at;
     const int* target;
-    Part* parts;                  // [rows][n_parts]
+    Part* parts;                  // [rows][2 stretches]
     int *pick, *status;
     float *pick_logprob, *logprob, *lse;
-    int rows, dim, vocab, n_parts;
+    int rows, dim, vocab;
+    int row_tiles, stretches, boxes, box;   // a stretch is boxes / stretches boxes of w
     float cap, inv_t;             // inv_t 0: greedy
-    uint32_t seed;
+    uint32_t seed, wait_limit;
+    int starve;
 };
 
 __device__ __forceinline__ uint32_t mix(uint32_t x) {
     x ^= x >> 16; x *= 0x7feb352du; x ^= x >> 15; x *= 0x846ca68bu; x ^= x >> 16;
     return x;
 }
-__device__ __forceinline__ float gumbel(uint32_t seed, int row, int token) {
-    const uint32_t h = mix(seed ^ mix((uint32_t)token + 0x9e3779b9u * (uint32_t)(row + 1)));
-    return -logf(-log1pf(-(((float)h + 0.5f) * (1.f / 4294967296.f))));
+__device__ __forceinline__ uint32_t draw(uint32_t seed, int row, int token) { return mix(seed ^ mix((uint32_t)token + 0x9e3779b9u * (uint32_t)(row + 1))); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
 }
-__device__ __forceinline__ void join(Part& a, const Part& b) {   // b behind a in the vocabulary
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// A token whose noise may take it above the best: its noise in full. (Few of a row's tokens come here: the first ones, and then about as many as a running maximum has steps.)
+__device__ __noinline__ void try_token(Part& a, float z, float scaled, uint32_t h, int token) {
+    const float g = -logf(-log1pf(-(((float)h + 0.5f) * (1.f / 4294967296.f))));
+    if (scaled + g > a.best || a.token < 0) { a.best = scaled + g; a.z = z; a.token = token; }
+}
+__device__ __noinline__ float capped(float z, float cap) { return cap * tanhf(z / cap); }
+__device__ __forceinline__ void join(Part& a, const Part& b) {
     const float m = fmaxf(a.m, b.m);
     if (m != -INFINITY) a.l = a.l * (a.m == m ? 1.f : expf(a.m - m)) + b.l * (b.m == m ? 1.f : expf(b.m - m));
     else a.l += b.l;   // (a sum that is NaN stays one)
     a.m = m;
-    if (b.token >= 0 && (a.token < 0 || b.best > a.best)) { a.best = b.best; a.z = b.z; a.token = b.token; }
+    if (b.token >= 0 && (a.token < 0 || b.best > a.best || (b.best == a.best && b.token < a.token))) { a.best = b.best; a.z = b.z; a.token = b.token; }
     if (b.given == b.given) a.given = b.given;
 }
 
-__global__ void __launch_bounds__(kThreads) vocab_scores_kernel(const ScoreParams p) {
-    __shared__ float sx[kStep][kTile + 1], sw[kStep][kTile + 1];
+template <bool kSample>
+__global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_constant__ ScoreParams p) {
+    constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kRows >> 4) << 24);   // f32 accumulator, bf16 operands, M = 128
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
+    __shared__ uint32_t tmem_holder;
+    const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], kEpilogue / 32); }
+        mbar_fence_init();
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_holder)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_holder;
     pdl_launch_dependents();
     pdl_wait();
-    const int row0 = blockIdx.x * kTile, n0 = blockIdx.y * kTile, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < p.dim; k0 += kStep) {
-        for (int i = threadIdx.x; i < kTile * kStep; i += kThreads) {
-            const int r = i / kStep, k = i % kStep;
-            sx[k][r] = row0 + r < p.rows && k0 + k < p.dim ? __bfloat162float(p.x[(row0 + r) * p.ldx + k0 + k]) : 0.f;
-            sw[k][r] = n0 + r < p.vocab && k0 + k < p.dim ? __bfloat162float(p.w[(n0 + r) * p.ldw + k0 + k]) : 0.f;
+    const int steps = (p.dim + kStageDim - 1) / kStageDim, units = p.row_tiles * p.stretches;
+    struct Unit { int row0, begin, end; };
+    auto unit_of = [&](int u) {
+        const int part = u / p.row_tiles;
+        return Unit{(u % p.row_tiles) * kRows, (int)((long long)p.boxes * part / p.stretches) * p.box, min(p.vocab, (int)((long long)p.boxes * (part + 1) / p.stretches) * p.box)};
+    };
+    bool failed = false;
+
+    if (warp == 8) {
+        if (elect_one()) {
+            int it = 0, s = 0;
+            uint32_t phase = 1;
+            for (int u = blockIdx.x; u < units && !failed; u += gridDim.x) {
+                const Unit unit = unit_of(u);
+                for (int n0 = unit.begin; n0 < unit.end && !failed; n0 += kCols) {
+                    const int copies = (min(kCols, unit.end - n0) + p.box - 1) / p.box;
+                    for (int k = 0; k < steps; ++k, ++it) {
+                        if (it >= kStages && !mbar_wait_parked(smem_u32(&empty[s]), phase, p.wait_limit)) { failed = true; break; }
+                        const uint32_t bar = smem_u32(&full[s]), at = smem + s * kStageBytes;
+                        mbar_expect_tx_addr(bar, (uint32_t)(kABytes + copies * p.box * 128));
+                        if (!(p.starve && it == 0))
+                            asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(at), "l"(&p.x_map),
+                                         "r"(k * kStageDim), "r"(unit.row0), "r"(bar)
+                                         : "memory");
+                        for (int c = 0; c < copies; ++c)
+                            asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(at + kABytes + c * p.box * 128),
+                                         "l"(&p.w_map), "r"(k * kStageDim), "r"(n0 + c * p.box), "r"(bar)
+                                         : "memory");
+                        if (++s == kStages) { s = 0; phase ^= 1u; }
+                    }
+                }
+            }
+            // stages in flight write this CTA's shared memory (only after a timeout are there any left unread)
+            for (int i = max(it - kStages, 0); i < it; ++i) mbar_wait_parked(smem_u32(&full[i % kStages]), (uint32_t)(i / kStages) & 1u, p.wait_limit);
+            if (failed) atomicExch(p.status, 3);
         }
-        __syncthreads();
-        for (int k = 0; k < kStep; ++k)
+        __syncwarp();
+    } else if (warp == 9) {
+        if (elect_one()) {
+            int s = 0, n = 0;
+            uint32_t phase = 0;
+            for (int u = blockIdx.x; u < units && !failed; u += gridDim.x) {
+                const Unit unit = unit_of(u);
+                for (int n0 = unit.begin; n0 < unit.end && !failed; n0 += kCols) {
+                    const uint32_t idesc = kIdesc | ((uint32_t)((min(kCols, unit.end - n0) + 15) >> 4) << 18);   // (N in eights from bit 17)
+                    for (int k0 = 0; k0 < steps && !failed; k0 += kDrain, ++n) {
+                        const int buf = n & 1, k1 = min(k0 + kDrain, steps);
+                        if (n >= 2 && !mbar_wait_parked(smem_u32(&acc_empty[buf]), (uint32_t)((n >> 1) - 1) & 1u, p.wait_limit)) { failed = true; break; }
+                        tc_fence_after();
+                        for (int k = k0; k < k1; ++k) {
+                            if (!mbar_wait_parked(smem_u32(&full[s]), phase, p.wait_limit)) { failed = true; break; }
+                            tc_fence_after();
+                            const uint64_t a = make_smem_desc(smem + s * kStageBytes), b = make_smem_desc(smem + s * kStageBytes + kABytes);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+                            for (int i = 0; i < 4; ++i) umma_bf16(tmem + (uint32_t)(buf * kCols), a + 2 * i, b + 2 * i, idesc, (k > k0 || i > 0) ? 1u : 0u);
+                            umma_commit(&empty[s]);
+                            if (++s == kStages) { s = 0; phase ^= 1u; }
+                        }
+                        if (!failed) umma_commit(&acc_full[buf]);
+                    }
+                }
+            }
+            if (failed) atomicExch(p.status, 3);
+        }
+        __syncwarp();
+    } else {
+        const int half = warp >> 2, in_tile = (warp & 3) * 32 + lane;
+        const uint32_t acc0 = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * (kCols / 2));
+        const uint32_t seed = p.seed_at ? *p.seed_at : p.seed;
+        int n = 0;
+        for (int u = blockIdx.x; u < units && !failed; u += gridDim.x) {
+            const Unit unit = unit_of(u);
+            const int row = unit.row0 + in_tile;
+            const int target = p.target && row < p.rows ? p.target[row] : -1;
+            Part a = {-INFINITY, 0.f, -INFINITY, 0.f, -1, NAN};
+            for (int n0 = unit.begin; n0 < unit.end && !failed; n0 += kCols) {
+                const int first = n0 + half * (kCols / 2), some = min(kCols / 2, unit.end - first);   // this half's tokens
+                uint64_t acc[kCols / 4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sx[k][ty * 4 + i], sw[k][tx * 4 + j], acc[i][j]);
-        __syncthreads();
+                for (int i = 0; i < kCols / 4; ++i) acc[i] = 0;
+                for (int k0 = 0; k0 < steps; k0 += kDrain, ++n) {
+                    const int buf = n & 1;
+                    if (!failed && !mbar_wait_parked(smem_u32(&acc_full[buf]), (uint32_t)(n >> 1) & 1u, p.wait_limit)) failed = true;
+                    failed = __any_sync(0xffffffffu, failed);
+                    if (failed) break;
+                    tc_fence_after();
+                    if (some > 0) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            float v[32];
+                            tmem_ld_32(acc0 + (uint32_t)(buf * kCols + 32 * c), v);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) acc[16 * c + i] = add2(acc[16 * c + i], pair_of(v[2 * i], v[2 * i + 1]));
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&acc_empty[buf]);
+                }
+                if (failed || some <= 0) continue;
+                float z[kCols / 2];
+#pragma unroll
+                for (int i = 0; i < kCols / 4; ++i) {
+                    const float2 two = split(acc[i]);
+                    z[2 * i] = two.x;
+                    z[2 * i + 1] = two.y;
+                }
+                if (p.bias) {
+#pragma unroll
+                    for (int i = 0; i < kCols / 2; ++i)
+                        if (i < some) z[i] += __ldg(p.bias + first + i);
+                }
+                if (p.cap > 0.f) {
+#pragma unroll
+                    for (int i = 0; i < kCols / 2; ++i) z[i] = capped(z[i], p.cap);
+                }
+                if (some < kCols / 2) {
+#pragma unroll
+                    for (int i = 0; i < kCols / 2; ++i)
+                        if (i >= some) z[i] = -INFINITY;
+                }
+                const int wanted = (unsigned)(target - first) < (unsigned)some ? target - first : -1;
+                if (__any_sync(0xffffffffu, wanted >= 0)) {
+#pragma unroll
+                    for (int i = 0; i < kCols / 2; ++i)
+                        if (wanted == i) a.given = z[i];
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < kCols / 2; ++i) mx[i & 3] = fmaxf(mx[i & 3], z[i]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                if constexpr (!kSample) {
+                    if (__any_sync(0xffffffffu, top > a.best)) {
+                        int at = 0;
+#pragma unroll
+                        for (int i = kCols / 2 - 1; i >= 0; --i)
+                            if (z[i] == top) at = i;
+                        if (top > a.best) { a.best = a.z = top; a.token = first + at; }
+                    }
+                } else {
+                    // g <= -log v: a bound of one logarithm on the special function unit, with room for its error, keeps all but a few tokens from the noise in full
+#pragma unroll
+                    for (int i = 0; i < kCols / 2; ++i) {
+                        const uint32_t h = draw(seed, row, first + i);
+                        const float low = __uint_as_float((h >> 9) | 0x3f800000u) - 1.f;   // v from below
+                        const float scaled = z[i] * p.inv_t;
+                        if (fmaf(lg2(low), -kLn2, scaled) + 1e-3f > a.best && i < some) try_token(a, z[i], scaled, h, first + i);
+                    }
+                }
+                // sum exp z: differences first, so that what is rounded is small where it counts
+                const float to = fmaxf(a.m, top), ref = to == -INFINITY ? 0.f : to;
+                const uint64_t ref2 = pair_of(-ref, -ref), log2 = pair_of(kLog2e, kLog2e);
+                uint64_t sums[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < kCols / 4; ++i) {
+                    const float2 e = split(mul2(add2(pair_of(z[2 * i], z[2 * i + 1]), ref2), log2));
+                    sums[i & 3] = add2(sums[i & 3], pair_of(ex2(e.x), ex2(e.y)));
+                }
+                const float2 s = split(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+                a.l = a.l * (a.m == to ? 1.f : ex2((a.m - ref) * kLog2e)) + (s.x + s.y);
+                a.m = to;
+            }
+            if (row < p.rows && !failed) p.parts[(size_t)row * (2 * p.stretches) + 2 * (u / p.row_tiles) + half] = a;
+        }
+        if (failed && lane == 0) atomicExch(p.status, 3);
     }
-    const uint32_t seed = p.seed_at ? *p.seed_at : p.seed;
-#pragma unroll 1
-    for (int i = 0; i < 4; ++i) {
-        const int row = row0 + ty * 4 + i;
-        const int target = p.target && row < p.rows ? p.target[row] : -1;
-        Part a = {-INFINITY, 0.f, -INFINITY, 0.f, -1, NAN};
-        for (int j = 0; j < 4; ++j) {
-            const int n = n0 + tx * 4 + j;
-            if (n >= p.vocab || row >= p.rows) break;
-            float z = acc[i][j] + (p.bias ? p.bias[n] : 0.f);
-            if (p.cap > 0.f) z = p.cap * tanhf(z / p.cap);
-            const Part b = {z != z ? 0.f : z, z != z ? z : z == -INFINITY ? 0.f : 1.f, p.inv_t > 0.f ? z * p.inv_t + gumbel(seed, row, n) : z, z, n, n == target ? z : NAN};
-            join(a, b);
-        }
-#pragma unroll
-        for (int o = 1; o < 16; o *= 2) {   // the lane in front has the tokens in front
-            Part b = {__shfl_down_sync(0xffffffffu, a.m, o), __shfl_down_sync(0xffffffffu, a.l, o), __shfl_down_sync(0xffffffffu, a.best, o),
-                      __shfl_down_sync(0xffffffffu, a.z, o), __shfl_down_sync(0xffffffffu, a.token, o), __shfl_down_sync(0xffffffffu, a.given, o)};
-            if (tx + o < 16) join(a, b);
-        }
-        if (tx == 0 && row < p.rows) p.parts[(size_t)row * p.n_parts + blockIdx.y] = a;
-    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
-__global__ void __launch_bounds__(kThreads) vocab_join_kernel(const ScoreParams p) {
+// A warp per row.
+__global__ void __launch_bounds__(kJoinThreads) vocab_join_kernel(const __grid_constant__ ScoreParams p) {
     pdl_launch_dependents();
     pdl_wait();
-    const int row = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int row = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31, n = 2 * p.stretches;
     if (row >= p.rows) return;
-    const Part* parts = p.parts + (size_t)row * p.n_parts;
-    const int per = (p.n_parts + 31) / 32;
+    const Part* parts = p.parts + (size_t)row * n;
     Part a = {-INFINITY, 0.f, -INFINITY, 0.f, -1, NAN};
-    for (int i = lane * per; i < min((lane + 1) * per, p.n_parts); ++i) join(a, parts[i]);
+    for (int i = lane; i < n; i += 32) join(a, parts[i]);
 #pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-        Part b = {__shfl_down_sync(0xffffffffu, a.m, o), __shfl_down_sync(0xffffffffu, a.l, o), __shfl_down_sync(0xffffffffu, a.best, o),
-                  __shfl_down_sync(0xffffffffu, a.z, o), __shfl_down_sync(0xffffffffu, a.token, o), __shfl_down_sync(0xffffffffu, a.given, o)};
-        if (lane + o < 32) join(a, b);
+    for (int o = 16; o > 0; o >>= 1) {
+        const Part b = {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.l, o), __shfl_xor_sync(0xffffffffu, a.best, o),
+                        __shfl_xor_sync(0xffffffffu, a.z, o), __shfl_xor_sync(0xffffffffu, a.token, o), __shfl_xor_sync(0xffffffffu, a.given, o)};
+        join(a, b);
     }
     if (lane) return;
     const float log_l = logf(a.l);
     if (p.lse) p.lse[row] = a.m + log_l;
-    if (p.pick) p.pick[row] = a.token;
+    if (p.pick) p.pick[row] = max(a.token, 0);   // (nothing compares with NaN: the first token)
     if (p.pick_logprob) p.pick_logprob[row] = a.z - a.m - log_l;
     if (p.logprob) {
-        const int target = p.target ? p.target[row] : -1;
+        const int target = p.target[row];
         if (target >= p.vocab) atomicExch(p.status, 2);
         p.logprob[row] = target < 0 ? 0.f : a.given - a.m - log_l;
     }
+}
+
+// Stretches of the vocabulary: units (row tiles x stretches) of one CTA per SM. One row tile: as many as there are SMs, in copies of 32 rows, since the bytes of w are all
+// that counts. More: as many as leave the fewest tokens to the SM that has most, a unit's own cost counted as 32 tokens.
+void cut(int64_t rows, int64_t vocab, int* row_tiles, int* stretches, int* boxes, int* box) {
+    *row_tiles = ceil_div(rows, kRows);
+    *box = *row_tiles == 1 ? 32 : 64;
+    *boxes = ceil_div(vocab, *box);
+    const int sms = sm_count(), most = *boxes < 4 * sms ? *boxes : 4 * sms;
+    int64_t best = -1;
+    *stretches = 1;
+    for (int n = 1; n <= (*row_tiles == 1 ? (most < sms ? most : sms) : most); ++n) {
+        const int64_t waves = ceil_div((int64_t)*row_tiles * n, sms), cost = waves * ((int64_t)ceil_div(*boxes, n) * *box + 32);
+        if (best < 0 || cost < best) { best = cost; *stretches = n; }
+    }
+}
+
+int encode(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_rows) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return fail(GPTRS_EXECUTION, "cuTensorMapEncodeTiled is not available");
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    cuuint32_t box[2] = {kStageDim, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(GPTRS_EXECUTION, "cuTensorMapEncodeTiled failed for scores (" + std::to_string((int)r) + ")");
+    return GPTRS_OK;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -124,31 +341,50 @@ extern "C" {
 
 size_t gptrs_cuda_vocab_scores_scratch_bytes(const gptrs_vocab_scores* s) {
     if (!s || s->rows < 1 || s->vocab < 1) return 0;
-    return (size_t)s->rows * ceil_div(s->vocab, kTile) * sizeof(Part);
+    if (s->rows > 0x3fffffff || s->vocab > 0x3fffffff) return 0;
+    int row_tiles, stretches, boxes, box;
+    cut(s->rows, s->vocab, &row_tiles, &stretches, &boxes, &box);
+    return (size_t)s->rows * 2 * stretches * sizeof(Part);
 }
 
 int gptrs_cuda_vocab_scores(const gptrs_vocab_scores* s, void* stream) {
     GPTRS_REQUIRE(s && s->d_weight && s->d_status && (s->rows == 0 || s->d_hidden), "null pointer");
     GPTRS_REQUIRE(s->rows >= 0 && s->rows <= 0x3fffffff && s->vocab >= 1 && s->vocab <= 0x3fffffff && s->dim >= 8 && s->dim <= 0x3fffffff, "bad sizes");
     ScoreParams p = {};
-    p.ldx = s->ldh ? s->ldh : s->dim;
-    p.ldw = s->ldw ? s->ldw : s->dim;
-    GPTRS_REQUIRE(s->dim % 8 == 0 && p.ldx % 8 == 0 && p.ldw % 8 == 0 && p.ldx >= s->dim && p.ldw >= s->dim && p.ldx < ((int64_t)1 << 31) && p.ldw < ((int64_t)1 << 31),
+    const int64_t ldx = s->ldh ? s->ldh : s->dim, ldw = s->ldw ? s->ldw : s->dim;
+    GPTRS_REQUIRE(s->dim % 8 == 0 && ldx % 8 == 0 && ldw % 8 == 0 && ldx >= s->dim && ldw >= s->dim && ldx < ((int64_t)1 << 31) && ldw < ((int64_t)1 << 31),
                   "dim and the strides must be multiples of 8, and rows must not overlap");
-    GPTRS_REQUIRE(aligned16(s->d_hidden) && aligned16(s->d_weight) && aligned16(s->d_scratch), "pointers must be 16-byte aligned");
+    GPTRS_REQUIRE(aligned16(s->d_hidden) && aligned16(s->d_weight) && (reinterpret_cast<uintptr_t>(s->d_scratch) & 31) == 0, "pointers must be 16-byte aligned, scratch 32");
     GPTRS_REQUIRE(s->temperature == s->temperature && s->soft_cap >= 0.f && s->soft_cap < 3e38f, "bad temperature or soft cap");
     GPTRS_REQUIRE(!s->d_logprob || s->d_target, "log-probabilities of targets need targets");
     GPTRS_REQUIRE(s->rows == 0 || (s->d_scratch && s->scratch_bytes >= gptrs_cuda_vocab_scores_scratch_bytes(s)), "scratch is too small");
     if (s->rows == 0) return GPTRS_OK;
-    p.x = static_cast<const __nv_bfloat16*>(s->d_hidden); p.w = static_cast<const __nv_bfloat16*>(s->d_weight);
+    cut(s->rows, s->vocab, &p.row_tiles, &p.stretches, &p.boxes, &p.box);
+    int rc = encode(&p.x_map, s->d_hidden, s->dim, s->rows, ldx, kRows);
+    if (!rc) rc = encode(&p.w_map, s->d_weight, s->dim, s->vocab, ldw, p.box);
+    if (rc) return rc;
     p.bias = s->d_bias; p.seed_at = s->d_seed; p.target = s->d_target;
     p.parts = static_cast<Part*>(s->d_scratch);
     p.pick = s->d_pick; p.pick_logprob = s->d_pick_logprob; p.logprob = s->d_logprob; p.lse = s->d_lse; p.status = s->d_status;
-    p.rows = (int)s->rows; p.dim = (int)s->dim; p.vocab = (int)s->vocab; p.n_parts = ceil_div(s->vocab, kTile);
+    p.rows = (int)s->rows; p.dim = (int)s->dim; p.vocab = (int)s->vocab;
     p.cap = s->soft_cap; p.inv_t = s->temperature > 0.f ? 1.f / s->temperature : 0.f; p.seed = s->seed;
-    const int rc = launch_kernel(vocab_scores_kernel, dim3((unsigned)ceil_div(p.rows, kTile), (unsigned)p.n_parts), dim3(kThreads), 0, as_stream(stream), 1, p);
+    prefill_tc_fault(&p.starve, &p.wait_limit);
+    static PerDeviceOnce attr_once;
+    if (attr_once.first_time()) {
+        GPTRS_CUDA_OK(cudaFuncSetAttribute(vocab_scores_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
+        GPTRS_CUDA_OK(cudaFuncSetAttribute(vocab_scores_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
+    }
+    const int64_t units = (int64_t)p.row_tiles * p.stretches;
+    GPTRS_REQUIRE(units < ((int64_t)1 << 31), "too many rows");
+    rc = launch_kernel(p.inv_t > 0.f ? vocab_scores_kernel<true> : vocab_scores_kernel<false>, dim3((unsigned)(units < sm_count() ? units : sm_count())), dim3(kThreads), kSmem,
+                       as_stream(stream), 1, p);
     if (rc) return rc;
-    return launch_kernel(vocab_join_kernel, dim3((unsigned)ceil_div(p.rows, kThreads / 32)), dim3(kThreads), 0, as_stream(stream), 1, p);
+    // the second kernel waits for the first one itself (griddepcontrol.wait), so it may be launched ahead of its end
+    const int pdl = g_use_pdl;
+    g_use_pdl = 1;
+    rc = launch_kernel(vocab_join_kernel, dim3((unsigned)ceil_div(p.rows, kJoinThreads / 32)), dim3(kJoinThreads), 0, as_stream(stream), 1, p);
+    g_use_pdl = pdl;
+    return rc;
 }
 
 }  // extern "C"

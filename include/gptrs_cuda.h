@@ -903,7 +903,7 @@ typedef struct {
     const int32_t* d_target;           /* [rows] or NULL */
     int32_t* d_pick;
     float *d_pick_logprob, *d_logprob, *d_lse;
-    void* d_scratch;                   /* of one call at a time, 16-byte aligned */
+    void* d_scratch;                   /* of one call at a time, 32-byte aligned */
     size_t scratch_bytes;
     int32_t* d_status;
 } gptrs_vocab_scores;

@@ -64,7 +64,7 @@ def test_null_arguments_are_refused():
 
 
 def _scores(**kw):
-    s = _abi.VocabScores(16, 0, 16, 0, 4, 64, 100, None, 0.0, 0.0, 0, None, 16, 16, 16, 16, 16, 16, 1 << 40, 16)
+    s = _abi.VocabScores(16, 0, 16, 0, 4, 64, 100, None, 0.0, 0.0, 0, None, 16, 16, 16, 16, 16, 32, 1 << 40, 16)
     for k, v in kw.items():
         setattr(s, k, v)
     return s
