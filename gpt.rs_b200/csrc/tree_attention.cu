@@ -135,35 +135,10 @@ __device__ __forceinline__ uint64_t make_smem_desc_mn(uint32_t smem_addr) {
     d |= (uint64_t)2 << 61;
     return d;
 }
-__device__ __forceinline__ void tmem_ld_32_async(uint32_t taddr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-          "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-}
-// Waits for the loads in front; the registers of one of them pass through, so that nothing that uses them moves ahead.
-__device__ __forceinline__ void tmem_wait_ld(uint32_t* r) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
-                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
-                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
-                 :
-                 : "memory");
-    asm volatile("" : "+r"(r[30]), "+r"(r[31]));
-}
 __device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
                  "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
-    return d;
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -483,10 +458,10 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
                     for (bool look = live && m == -INFINITY;;) {
                         uint32_t sr[kKeys];
                         if (fresh) {   // a new reference for some rows: the maximum of this block
-                            tmem_ld_32_async(t_s, sr);
-                            tmem_ld_32_async(t_s + 32, sr + 32);
-                            tmem_wait_ld(sr);
-                            tmem_wait_ld(sr + 32);
+                            tmem_ld_32_begin(t_s, sr);
+                            tmem_ld_32_begin(t_s + 32, sr + 32);
+                            tmem_ld_32_end(sr);
+                            tmem_ld_32_end(sr + 32);
                             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                             for (int j = 0; j < kKeys; ++j)
@@ -502,8 +477,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
 #pragma unroll 1
                                 for (int c = 0; c < 4; ++c) {
                                     uint32_t r[32];
-                                    tmem_ld_32_async(t_o + 32u * c, r);
-                                    tmem_wait_ld(r);
+                                    tmem_ld_32_begin(t_o + 32u * c, r);
+                                    tmem_ld_32_end(r);
 #pragma unroll
                                     for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * keep);
                                     tmem_st_32(t_o + 32u * c, r);
@@ -515,13 +490,13 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
                         const float ref = m == -INFINITY ? 0.f : m;
                         const uint64_t scale2 = pair_of(p.scale_log2, p.scale_log2), ref2 = pair_of(-ref, -ref);
                         uint64_t sums[2] = {0, 0};
-                        tmem_ld_32_async(t_s, sr);
-                        tmem_wait_ld(sr);
-                        tmem_ld_32_async(t_s + 32, sr + 32);
+                        tmem_ld_32_begin(t_s, sr);
+                        tmem_ld_32_end(sr);
+                        tmem_ld_32_begin(t_s + 32, sr + 32);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             uint32_t* x = sr + 32 * h;
-                            if (h) tmem_wait_ld(x);
+                            if (h) tmem_ld_32_end(x);
                             if (tail || bad) {
 #pragma unroll
                                 for (int j = 0; j < 32; ++j)

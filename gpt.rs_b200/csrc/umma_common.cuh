@@ -59,6 +59,41 @@ __device__ __forceinline__ bool mbar_wait_parked(uint32_t bar_addr, uint32_t par
     }
     return false;
 }
+// The same with some polls in front that park nothing: waking up costs hundreds of cycles, which a chain of short steps does not hide.
+__device__ __forceinline__ bool mbar_wait_polled(uint64_t* bar, uint32_t parity, uint32_t limit, int polls) {
+    const uint32_t at = smem_u32(bar);
+    for (int i = 0; i < polls; ++i) {
+        uint32_t ok;
+        asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(at), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    return mbar_wait_parked(at, parity, limit);
+}
+// 32 consecutive columns of this thread's lane of tensor memory without the wait, and the wait for it: the registers pass through, so that nothing that uses them moves ahead.
+__device__ __forceinline__ void tmem_ld_32_begin(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_32_end(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
+                 :
+                 : "memory");
+    asm volatile("" : "+r"(r[30]), "+r"(r[31]));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {   // pairs of f32
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ bool mbar_wait_relaxed(uint64_t* bar, uint32_t parity, uint32_t limit = kSpinLimit) {
     return mbar_wait_parked(smem_u32(bar), parity, limit);
 }

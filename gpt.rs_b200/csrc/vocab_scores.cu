@@ -3,7 +3,7 @@
 // z = x . w^T on the tcgen05 tensor cores, x rows as the M side: a CTA (one per SM) takes a unit, a tile of 128 rows x a stretch of the vocabulary, and walks over it in
 // tiles of 256 tokens. What a row needs to know of its logits is a running state in registers (maximum and sum, best token, the target's logit), so a logit lives
 // from the accumulator to the exponential and nowhere else.
-//   warps 0 - 7   a thread per row and half of the tile's tokens. The accumulator in tensor memory is read out every 128 of dim and added up in f32 registers: the tensor
+//   warps 0 - 7   a thread per row and half of the tile's tokens. The accumulator in tensor memory is read out every 256 of dim and added up in f32 registers: the tensor
 //                 cores cut what does not fit into the sum that they add to, 16 products at a time, which over all of dim would cost log-probabilities five digits
 //   warp 8        requests stages of 64 of dim: 128 rows of x, up to 256 of w (in copies of `box` rows, so that a stretch may end anywhere and nothing behind it is read)
 //   warp 9        one thread issues the products into one of two accumulators
@@ -20,10 +20,13 @@ namespace {
 
 constexpr int kRows = 128, kCols = 256;         // of a tile
 constexpr int kStageDim = 64;                   // bf16 of a 128-byte swizzle span
-constexpr int kDrain = 2;                       // stages that an accumulator adds up
+constexpr int kDrain = 4;                       // stages that an accumulator adds up
 constexpr int kStages = 4;
 constexpr int kABytes = kRows * 128, kStageBytes = kABytes + kCols * 128;
-constexpr int kEpilogue = 256, kThreads = kEpilogue + 64;
+constexpr int kEpilogue = 256, kThreads = kEpilogue + 128;   // two warps of the last four only make their group whole
+// Registers of a thread at launch, and what the groups of four warps make of them: the shares add up to less than the block has, so every request ends.
+constexpr int kLaunchRegs = 168, kEpilogueRegs = 208, kOtherRegs = 80;
+static_assert(2 * kEpilogueRegs + kOtherRegs <= 3 * kLaunchRegs, "more registers than the block is launched with");
 constexpr size_t kSmem = (size_t)kStages * kStageBytes + 1024;
 constexpr uint32_t kTmemCols = 2 * kCols;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -61,16 +64,7 @@ __device__ __forceinline__ float lg2(float x) {
     asm("lg2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-// A token whose noise may take it above the best: its noise in full. (Few of a row's tokens come here: the first ones, and then about as many as a running maximum has steps.)
-__device__ __noinline__ void try_token(Part& a, float z, float scaled, uint32_t h, int token) {
-    const float g = -logf(-log1pf(-(((float)h + 0.5f) * (1.f / 4294967296.f))));
-    if (scaled + g > a.best || a.token < 0) { a.best = scaled + g; a.z = z; a.token = token; }
-}
+__device__ __forceinline__ float gumbel(uint32_t h) { return -logf(-log1pf(-(((float)h + 0.5f) * (1.f / 4294967296.f)))); }
 __device__ __noinline__ float capped(float z, float cap) { return cap * tanhf(z / cap); }
 __device__ __forceinline__ void join(Part& a, const Part& b) {
     const float m = fmaxf(a.m, b.m);
@@ -112,7 +106,10 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
     };
     bool failed = false;
 
-    if (warp == 8) {
+    if (warp >= 10) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
+    } else if (warp == 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
         if (elect_one()) {
             int it = 0, s = 0;
             uint32_t phase = 1;
@@ -121,7 +118,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                 for (int n0 = unit.begin; n0 < unit.end && !failed; n0 += kCols) {
                     const int copies = (min(kCols, unit.end - n0) + p.box - 1) / p.box;
                     for (int k = 0; k < steps; ++k, ++it) {
-                        if (it >= kStages && !mbar_wait_parked(smem_u32(&empty[s]), phase, p.wait_limit)) { failed = true; break; }
+                        if (it >= kStages && !mbar_wait_polled(&empty[s], phase, p.wait_limit, 256)) { failed = true; break; }
                         const uint32_t bar = smem_u32(&full[s]), at = smem + s * kStageBytes;
                         mbar_expect_tx_addr(bar, (uint32_t)(kABytes + copies * p.box * 128));
                         if (!(p.starve && it == 0))
@@ -142,6 +139,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
         }
         __syncwarp();
     } else if (warp == 9) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
         if (elect_one()) {
             int s = 0, n = 0;
             uint32_t phase = 0;
@@ -151,10 +149,10 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                     const uint32_t idesc = kIdesc | ((uint32_t)((min(kCols, unit.end - n0) + 15) >> 4) << 18);   // (N in eights from bit 17)
                     for (int k0 = 0; k0 < steps && !failed; k0 += kDrain, ++n) {
                         const int buf = n & 1, k1 = min(k0 + kDrain, steps);
-                        if (n >= 2 && !mbar_wait_parked(smem_u32(&acc_empty[buf]), (uint32_t)((n >> 1) - 1) & 1u, p.wait_limit)) { failed = true; break; }
+                        if (n >= 2 && !mbar_wait_polled(&acc_empty[buf], (uint32_t)((n >> 1) - 1) & 1u, p.wait_limit, 256)) { failed = true; break; }
                         tc_fence_after();
                         for (int k = k0; k < k1; ++k) {
-                            if (!mbar_wait_parked(smem_u32(&full[s]), phase, p.wait_limit)) { failed = true; break; }
+                            if (!mbar_wait_polled(&full[s], phase, p.wait_limit, 256)) { failed = true; break; }
                             tc_fence_after();
                             const uint64_t a = make_smem_desc(smem + s * kStageBytes), b = make_smem_desc(smem + s * kStageBytes + kABytes);
 #pragma unroll
@@ -170,6 +168,8 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
         }
         __syncwarp();
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kEpilogueRegs));
+        // (a warp without rows only hands accumulators back)
         const int half = warp >> 2, in_tile = (warp & 3) * 32 + lane;
         const uint32_t acc0 = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * (kCols / 2));
         const uint32_t seed = p.seed_at ? *p.seed_at : p.seed;
@@ -180,23 +180,26 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
             const int target = p.target && row < p.rows ? p.target[row] : -1;
             Part a = {-INFINITY, 0.f, -INFINITY, 0.f, -1, NAN};
             for (int n0 = unit.begin; n0 < unit.end && !failed; n0 += kCols) {
-                const int first = n0 + half * (kCols / 2), some = min(kCols / 2, unit.end - first);   // this half's tokens
+                const int first = n0 + half * (kCols / 2), some = unit.row0 + (warp & 3) * 32 < p.rows ? min(kCols / 2, unit.end - first) : 0;   // this half's tokens
                 uint64_t acc[kCols / 4];
 #pragma unroll
                 for (int i = 0; i < kCols / 4; ++i) acc[i] = 0;
                 for (int k0 = 0; k0 < steps; k0 += kDrain, ++n) {
                     const int buf = n & 1;
-                    if (!failed && !mbar_wait_parked(smem_u32(&acc_full[buf]), (uint32_t)(n >> 1) & 1u, p.wait_limit)) failed = true;
+                    if (!failed && !mbar_wait_polled(&acc_full[buf], (uint32_t)(n >> 1) & 1u, p.wait_limit, 64)) failed = true;
                     failed = __any_sync(0xffffffffu, failed);
                     if (failed) break;
                     tc_fence_after();
                     if (some > 0) {
+uint32_t v[2][32];   // a quarter on its way while the one in front is added
+                        tmem_ld_32_begin(acc0 + (uint32_t)(buf * kCols), v[0]);
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
-                            float v[32];
-                            tmem_ld_32(acc0 + (uint32_t)(buf * kCols + 32 * c), v);
+                            tmem_ld_32_end(v[c & 1]);
+                            if (c < 3) tmem_ld_32_begin(acc0 + (uint32_t)(buf * kCols + 32 * (c + 1)), v[(c + 1) & 1]);
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) acc[16 * c + i] = add2(acc[16 * c + i], pair_of(v[2 * i], v[2 * i + 1]));
+                            for (int i = 0; i < 16; ++i)
+                                acc[16 * c + i] = add2(acc[16 * c + i], pair_of(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])));
                         }
                     }
                     tc_fence_before();
@@ -244,13 +247,26 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                         if (top > a.best) { a.best = a.z = top; a.token = first + at; }
                     }
                 } else {
-                    // g <= -log v: a bound of one logarithm on the special function unit, with room for its error, keeps all but a few tokens from the noise in full
+                    // g <= -log v: a bound of one logarithm on the special function unit, with room for its error, keeps all but a few tokens (as many as a running maximum
+                    // has steps, about) from the noise in full. Sixteen at a time, so that the best of the ones in front counts.
 #pragma unroll
-                    for (int i = 0; i < kCols / 2; ++i) {
-                        const uint32_t h = draw(seed, row, first + i);
-                        const float low = __uint_as_float((h >> 9) | 0x3f800000u) - 1.f;   // v from below
-                        const float scaled = z[i] * p.inv_t;
-                        if (fmaf(lg2(low), -kLn2, scaled) + 1e-3f > a.best && i < some) try_token(a, z[i], scaled, h, first + i);
+                    for (int c = 0; c < kCols / 2; c += 16) {
+                        uint32_t may = 0;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float low = __uint_as_float((draw(seed, row, first + c + i) >> 9) | 0x3f800000u) - 1.f;   // v from below
+                            if (fmaf(lg2(low), -kLn2, z[c + i] * p.inv_t) + 1e-3f > a.best) may |= 1u << i;
+                        }
+                        if (some - c < 16) may &= (1u << max(some - c, 0)) - 1u;
+                        while (may) {
+                            const int i = __ffs(may) - 1;
+                            may &= may - 1;
+                            float zi = z[c];
+#pragma unroll
+                            for (int j = 1; j < 16; ++j) zi = i == j ? z[c + j] : zi;
+                            const float value = fmaf(zi, p.inv_t, gumbel(draw(seed, row, first + c + i)));
+                            if (value > a.best || a.token < 0) { a.best = value; a.z = zi; a.token = first + c + i; }
+                        }
                     }
                 }
                 // sum exp z: differences first, so that what is rounded is small where it counts
