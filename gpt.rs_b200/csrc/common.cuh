@@ -67,11 +67,11 @@ extern thread_local int g_use_pdl;
 extern thread_local int g_launch_priority;  // 0 = default; otherwise the stream priority value given to kernel launches
 
 #ifdef __CUDACC__
-// Launch through cudaLaunchKernelEx with the optional cluster (along grid.y) and
-// programmatic-dependent-launch attributes.
+// Launch through cudaLaunchKernelEx with the optional cluster (along grid.y; CTAs whose tensor cores work in pairs have to be
+// neighbours along grid.x) and programmatic-dependent-launch attributes.
 template <typename P>
 int launch_kernel(void (*kern)(P), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
-                  int cluster_y, const P& params) {
+                  int cluster_y, const P& params, int cluster_x = 1) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -84,9 +84,9 @@ int launch_kernel(void (*kern)(P), dim3 grid, dim3 block, size_t smem, cudaStrea
         attrs[na].val.priority = g_launch_priority;
         ++na;
     }
-    if (cluster_y > 1) {
+    if (cluster_y > 1 || cluster_x > 1) {
         attrs[na].id = cudaLaunchAttributeClusterDimension;
-        attrs[na].val.clusterDim.x = 1;
+        attrs[na].val.clusterDim.x = (unsigned)cluster_x;
         attrs[na].val.clusterDim.y = (unsigned)cluster_y;
         attrs[na].val.clusterDim.z = 1;
         ++na;

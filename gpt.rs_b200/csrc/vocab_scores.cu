@@ -1,12 +1,14 @@
 // Scores of rows against a vocabulary without logits in memory: log sum exp, log-probabilities of given tokens, greedy or sampled picks.
 //
-// z = x . w^T on the tcgen05 tensor cores, x rows as the M side: a CTA (one per SM) takes a unit, a tile of 128 rows x a stretch of the vocabulary, and walks over it in
-// tiles of 256 tokens. What a row needs to know of its logits is a running state in registers (maximum and sum, best token, the target's logit), so a logit lives
+// z = x . w^T on the tcgen05 tensor cores, x rows as the M side. A unit is a tile of rows x a stretch of the vocabulary, which a CTA (one per SM) walks over in tiles of
+// up to 256 tokens. What a row needs to know of its logits is a running state in registers (maximum and sum, best token, the target's logit), so a logit lives
 // from the accumulator to the exponential and nowhere else.
 //   warps 0 - 7   a thread per row and half of the tile's tokens. The accumulator in tensor memory is read out every 256 of dim and added up in f32 registers: the tensor
-//                 cores cut what does not fit into the sum that they add to, 16 products at a time, which over all of dim would cost log-probabilities five digits
-//   warp 8        requests stages of 64 of dim: 128 rows of x, up to 256 of w (in copies of `box` rows, so that a stretch may end anywhere and nothing behind it is read)
+//                 cores cut what does not fit into the sum that they add to, 16 products at a time, which over all of dim would cost log-probabilities digits
+//   warp 8        requests stages of 64 of dim
 //   warp 9        one thread issues the products into one of two accumulators
+// Up to 128 rows a tile is 128 rows and one CTA's. Above, a cluster of two CTAs works on 256 rows (cta_group::2): each brings its 128 rows of x and half of the tokens, 32 KB
+// for 64 of dim where a CTA by itself brings 48, and an SM takes about 64 bytes a cycle out of L2.
 // Units go row tile first, so that the CTAs that run at one time share stretches of w through L2. A second kernel joins the parts of a row; it compares tokens where
 // values are equal, so results do not depend on an order.
 // Every wait is bounded: on a timeout code 3 goes to the status word, the roles leave their loops, tensor memory is freed.
@@ -18,16 +20,18 @@ void prefill_tc_fault(int* starve, uint32_t* wait_limit);   // the test switch o
 
 namespace {
 
-constexpr int kRows = 128, kCols = 256;         // of a tile
+constexpr int kRows = 128;                      // of a CTA
+constexpr int kCols = 256;                      // most tokens of a tile
 constexpr int kStageDim = 64;                   // bf16 of a 128-byte swizzle span
 constexpr int kDrain = 4;                       // stages that an accumulator adds up
-constexpr int kStages = 4;
-constexpr int kABytes = kRows * 128, kStageBytes = kABytes + kCols * 128;
+constexpr int kABytes = kRows * 128;
 constexpr int kEpilogue = 256, kThreads = kEpilogue + 128;   // two warps of the last four only make their group whole
 // Registers of a thread at launch, and what the groups of four warps make of them: the shares add up to less than the block has, so every request ends.
 constexpr int kLaunchRegs = 168, kEpilogueRegs = 208, kOtherRegs = 80;
 static_assert(2 * kEpilogueRegs + kOtherRegs <= 3 * kLaunchRegs, "more registers than the block is launched with");
-constexpr size_t kSmem = (size_t)kStages * kStageBytes + 1024;
+constexpr int stages_of(bool pair) { return pair ? 6 : 4; }
+constexpr int stage_bytes(bool pair) { return kABytes + kCols / (pair ? 2 : 1) * 128; }
+constexpr size_t smem_bytes(bool pair) { return (size_t)stages_of(pair) * stage_bytes(pair) + 1024; }
 constexpr uint32_t kTmemCols = 2 * kCols;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kJoinThreads = 256;
@@ -43,7 +47,8 @@ struct ScoreParams {
     int *pick, *status;
     float *pick_logprob, *logprob, *lse;
     int rows, dim, vocab;
-    int row_tiles, stretches, boxes, box;   // a stretch is boxes / stretches boxes of w
+    int row_tiles, stretches, tiles, cols;   // a stretch is `tiles` tiles of `cols` tokens
+    int x_rows;                   // of a copy of x
     float cap, inv_t;             // inv_t 0: greedy
     uint32_t seed, wait_limit;
     int starve;
@@ -75,34 +80,66 @@ __device__ __forceinline__ void join(Part& a, const Part& b) {
     if (b.given == b.given) a.given = b.given;
 }
 
-template <bool kSample>
+template <bool kPair>
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    if constexpr (kPair)   // the barrier may be the other CTA's
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+template <bool kPair>
+__device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (kPair)
+        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                     : "memory");
+    else
+        umma_bf16(d, a, b, idesc, accumulate);
+}
+template <bool kPair>
+__device__ __forceinline__ void commit(uint64_t* bar) {   // to the barrier of both CTAs
+    if constexpr (kPair)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+    else
+        umma_commit(bar);
+}
+
+template <bool kPair, bool kSample>
 __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_constant__ ScoreParams p) {
-    constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kRows >> 4) << 24);   // f32 accumulator, bf16 operands, M = 128
+    constexpr int kStages = stages_of(kPair), kStageBytes = stage_bytes(kPair), kCtas = kPair ? 2 : 1;
+    constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kCtas * kRows >> 4) << 24);   // f32 accumulator, bf16 operands
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_holder;
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = kPair ? (int)cluster_ctarank() : 0;   // the first CTA's thread issues the products of both
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], kEpilogue / 32); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], kCtas * kEpilogue / 32); }
         mbar_fence_init();
     }
     if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_holder)), "r"(kTmemCols) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+        if constexpr (kPair) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_holder)), "r"(kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_holder)), "r"(kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+        }
     }
     tc_fence_before();
-    __syncthreads();
+    if constexpr (kPair) cluster_sync_all();   // the other CTA's barriers are there
+    else __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_holder;
     pdl_launch_dependents();
     pdl_wait();
-    const int steps = (p.dim + kStageDim - 1) / kStageDim, units = p.row_tiles * p.stretches;
+    const int steps = (p.dim + kStageDim - 1) / kStageDim, units = p.row_tiles * p.stretches, my_cols = p.cols / kCtas;
     struct Unit { int row0, begin, end; };
     auto unit_of = [&](int u) {
-        const int part = u / p.row_tiles;
-        return Unit{(u % p.row_tiles) * kRows, (int)((long long)p.boxes * part / p.stretches) * p.box, min(p.vocab, (int)((long long)p.boxes * (part + 1) / p.stretches) * p.box)};
+        const int begin = u / p.row_tiles * (p.tiles * p.cols);
+        return Unit{(u % p.row_tiles) * (kCtas * kRows) + rank * kRows, begin, min(p.vocab, begin + p.tiles * p.cols)};
     };
     bool failed = false;
 
@@ -113,40 +150,35 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
         if (elect_one()) {
             int it = 0, s = 0;
             uint32_t phase = 1;
-            for (int u = blockIdx.x; u < units && !failed; u += gridDim.x) {
+            const uint32_t bytes = (uint32_t)(kCtas * (p.x_rows + my_cols) * 128);
+            for (int u = blockIdx.x / kCtas; u < units && !failed; u += gridDim.x / kCtas) {
                 const Unit unit = unit_of(u);
-                for (int n0 = unit.begin; n0 < unit.end && !failed; n0 += kCols) {
-                    const int copies = (min(kCols, unit.end - n0) + p.box - 1) / p.box;
+                for (int n0 = unit.begin; n0 < unit.end && !failed; n0 += p.cols) {
                     for (int k = 0; k < steps; ++k, ++it) {
                         if (it >= kStages && !mbar_wait_polled(&empty[s], phase, p.wait_limit, 256)) { failed = true; break; }
-                        const uint32_t bar = smem_u32(&full[s]), at = smem + s * kStageBytes;
-                        mbar_expect_tx_addr(bar, (uint32_t)(kABytes + copies * p.box * 128));
-                        if (!(p.starve && it == 0))
-                            asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(at), "l"(&p.x_map),
-                                         "r"(k * kStageDim), "r"(unit.row0), "r"(bar)
-                                         : "memory");
-                        for (int c = 0; c < copies; ++c)
-                            asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(at + kABytes + c * p.box * 128),
-                                         "l"(&p.w_map), "r"(k * kStageDim), "r"(n0 + c * p.box), "r"(bar)
-                                         : "memory");
+                        const uint32_t at = smem + s * kStageBytes, bar = kPair ? map_to_cta(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
+                        if (rank == 0) mbar_expect_tx(&full[s], bytes);
+                        if (!(p.starve && it == 0)) load_2d<kPair>(at, &p.x_map, k * kStageDim, unit.row0, bar);
+                        load_2d<kPair>(at + kABytes, &p.w_map, k * kStageDim, n0 + rank * my_cols, bar);
                         if (++s == kStages) { s = 0; phase ^= 1u; }
                     }
                 }
             }
-            // stages in flight write this CTA's shared memory (only after a timeout are there any left unread)
-            for (int i = max(it - kStages, 0); i < it; ++i) mbar_wait_parked(smem_u32(&full[i % kStages]), (uint32_t)(i / kStages) & 1u, p.wait_limit);
+            // Stages in flight write the CTAs' shared memory (only after a timeout are there any left unread). Of a pair the first CTA waits for both: the other one stays until the end.
+            if (rank == 0)
+                for (int i = max(it - kStages, 0); i < it; ++i) mbar_wait_parked(smem_u32(&full[i % kStages]), (uint32_t)(i / kStages) & 1u, p.wait_limit);
             if (failed) atomicExch(p.status, 3);
         }
         __syncwarp();
     } else if (warp == 9) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
-        if (elect_one()) {
+        if (rank == 0 && elect_one()) {
             int s = 0, n = 0;
             uint32_t phase = 0;
-            for (int u = blockIdx.x; u < units && !failed; u += gridDim.x) {
+            const uint32_t idesc = kIdesc | ((uint32_t)(p.cols >> 3) << 17);
+            for (int u = blockIdx.x / kCtas; u < units && !failed; u += gridDim.x / kCtas) {
                 const Unit unit = unit_of(u);
-                for (int n0 = unit.begin; n0 < unit.end && !failed; n0 += kCols) {
-                    const uint32_t idesc = kIdesc | ((uint32_t)((min(kCols, unit.end - n0) + 15) >> 4) << 18);   // (N in eights from bit 17)
+                for (int n0 = unit.begin; n0 < unit.end && !failed; n0 += p.cols) {
                     for (int k0 = 0; k0 < steps && !failed; k0 += kDrain, ++n) {
                         const int buf = n & 1, k1 = min(k0 + kDrain, steps);
                         if (n >= 2 && !mbar_wait_polled(&acc_empty[buf], (uint32_t)((n >> 1) - 1) & 1u, p.wait_limit, 256)) { failed = true; break; }
@@ -156,11 +188,11 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                             tc_fence_after();
                             const uint64_t a = make_smem_desc(smem + s * kStageBytes), b = make_smem_desc(smem + s * kStageBytes + kABytes);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) umma_bf16(tmem + (uint32_t)(buf * kCols), a + 2 * i, b + 2 * i, idesc, (k > k0 || i > 0) ? 1u : 0u);
-                            umma_commit(&empty[s]);
+                            for (int i = 0; i < 4; ++i) multiply<kPair>(tmem + (uint32_t)(buf * kCols), a + 2 * i, b + 2 * i, idesc, (k > k0 || i > 0) ? 1u : 0u);
+                            commit<kPair>(&empty[s]);
                             if (++s == kStages) { s = 0; phase ^= 1u; }
                         }
-                        if (!failed) umma_commit(&acc_full[buf]);
+                        if (!failed) commit<kPair>(&acc_full[buf]);
                     }
                 }
             }
@@ -169,18 +201,22 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
         __syncwarp();
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kEpilogueRegs));
-        // (a warp without rows only hands accumulators back)
-        const int half = warp >> 2, in_tile = (warp & 3) * 32 + lane;
-        const uint32_t acc0 = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * (kCols / 2));
+        // Quarters of 32 tokens that a warp has none of are left out; a warp without rows only hands accumulators back.
+        const int half = warp >> 2, in_tile = (warp & 3) * 32 + lane, width = (p.cols / 2 + 15) / 16 * 16;   // of the first half
+        const uint32_t acc0 = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * width);
         const uint32_t seed = p.seed_at ? *p.seed_at : p.seed;
+        uint32_t handed[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) handed[i] = kPair ? map_to_cta(smem_u32(&acc_empty[i]), 0) : smem_u32(&acc_empty[i]);
         int n = 0;
-        for (int u = blockIdx.x; u < units && !failed; u += gridDim.x) {
+        for (int u = blockIdx.x / kCtas; u < units && !failed; u += gridDim.x / kCtas) {
             const Unit unit = unit_of(u);
             const int row = unit.row0 + in_tile;
+            const bool rows = unit.row0 + (warp & 3) * 32 < p.rows;
             const int target = p.target && row < p.rows ? p.target[row] : -1;
             Part a = {-INFINITY, 0.f, -INFINITY, 0.f, -1, NAN};
-            for (int n0 = unit.begin; n0 < unit.end && !failed; n0 += kCols) {
-                const int first = n0 + half * (kCols / 2), some = unit.row0 + (warp & 3) * 32 < p.rows ? min(kCols / 2, unit.end - first) : 0;   // this half's tokens
+            for (int n0 = unit.begin; n0 < unit.end && !failed; n0 += p.cols) {
+                const int first = n0 + half * width, some = rows ? min(half ? p.cols - width : width, unit.end - first) : 0;   // this half's tokens
                 uint64_t acc[kCols / 4];
 #pragma unroll
                 for (int i = 0; i < kCols / 4; ++i) acc[i] = 0;
@@ -191,12 +227,13 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                     if (failed) break;
                     tc_fence_after();
                     if (some > 0) {
-uint32_t v[2][32];   // a quarter on its way while the one in front is added
+                        uint32_t v[2][32];   // a quarter on its way while the one in front is added
                         tmem_ld_32_begin(acc0 + (uint32_t)(buf * kCols), v[0]);
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
+                            if (32 * c >= some) break;
                             tmem_ld_32_end(v[c & 1]);
-                            if (c < 3) tmem_ld_32_begin(acc0 + (uint32_t)(buf * kCols + 32 * (c + 1)), v[(c + 1) & 1]);
+                            if (c < 3 && 32 * (c + 1) < some) tmem_ld_32_begin(acc0 + (uint32_t)(buf * kCols + 32 * (c + 1)), v[(c + 1) & 1]);
 #pragma unroll
                             for (int i = 0; i < 16; ++i)
                                 acc[16 * c + i] = add2(acc[16 * c + i], pair_of(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])));
@@ -204,91 +241,105 @@ uint32_t v[2][32];   // a quarter on its way while the one in front is added
                     }
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&acc_empty[buf]);
+                    if (lane == 0) {
+                        if constexpr (kPair)   // (the reads of tensor memory are complete, and nothing else is handed over: no fence over the cluster, which takes as long as they do)
+                            asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(handed[buf]) : "memory");
+                        else mbar_arrive_addr(handed[buf]);
+                    }
                 }
                 if (failed || some <= 0) continue;
-                float z[kCols / 2];
-#pragma unroll
-                for (int i = 0; i < kCols / 4; ++i) {
-                    const float2 two = split(acc[i]);
-                    z[2 * i] = two.x;
-                    z[2 * i + 1] = two.y;
-                }
-                if (p.bias) {
-#pragma unroll
-                    for (int i = 0; i < kCols / 2; ++i)
-                        if (i < some) z[i] += __ldg(p.bias + first + i);
-                }
-                if (p.cap > 0.f) {
-#pragma unroll
-                    for (int i = 0; i < kCols / 2; ++i) z[i] = capped(z[i], p.cap);
-                }
-                if (some < kCols / 2) {
-#pragma unroll
-                    for (int i = 0; i < kCols / 2; ++i)
-                        if (i >= some) z[i] = -INFINITY;
-                }
                 const int wanted = (unsigned)(target - first) < (unsigned)some ? target - first : -1;
-                if (__any_sync(0xffffffffu, wanted >= 0)) {
+                const bool given = __any_sync(0xffffffffu, wanted >= 0);
 #pragma unroll
-                    for (int i = 0; i < kCols / 2; ++i)
-                        if (wanted == i) a.given = z[i];
-                }
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                for (int c = 0; c < 4; ++c) {
+                    if (32 * c >= some) break;
+                    float z[32];
 #pragma unroll
-                for (int i = 0; i < kCols / 2; ++i) mx[i & 3] = fmaxf(mx[i & 3], z[i]);
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                if constexpr (!kSample) {
-                    if (__any_sync(0xffffffffu, top > a.best)) {
-                        int at = 0;
-#pragma unroll
-                        for (int i = kCols / 2 - 1; i >= 0; --i)
-                            if (z[i] == top) at = i;
-                        if (top > a.best) { a.best = a.z = top; a.token = first + at; }
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 two = split(acc[16 * c + i]);
+                        z[2 * i] = two.x;
+                        z[2 * i + 1] = two.y;
                     }
-                } else {
-                    // g <= -log v: a bound of one logarithm on the special function unit, with room for its error, keeps all but a few tokens (as many as a running maximum
-                    // has steps, about) from the noise in full. Sixteen at a time, so that the best of the ones in front counts.
+                    const int n_c = first + 32 * c, some_c = some - 32 * c;
+                    if (p.bias) {
 #pragma unroll
-                    for (int c = 0; c < kCols / 2; c += 16) {
-                        uint32_t may = 0;
+                        for (int i = 0; i < 32; ++i)
+                            if (i < some_c) z[i] += __ldg(p.bias + n_c + i);
+                    }
+                    if (p.cap > 0.f) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float low = __uint_as_float((draw(seed, row, first + c + i) >> 9) | 0x3f800000u) - 1.f;   // v from below
-                            if (fmaf(lg2(low), -kLn2, z[c + i] * p.inv_t) + 1e-3f > a.best) may |= 1u << i;
+                        for (int i = 0; i < 32; ++i) z[i] = capped(z[i], p.cap);
+                    }
+                    if (some_c < 32) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (i >= some_c) z[i] = -INFINITY;
+                    }
+                    if (given) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (wanted == 32 * c + i) a.given = z[i];
+                    }
+                    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) mx[i & 1] = fmaxf(mx[i & 1], z[i]);
+                    const float top = fmaxf(mx[0], mx[1]);
+                    if constexpr (!kSample) {
+                        if (__any_sync(0xffffffffu, top > a.best)) {
+                            int at = 0;
+#pragma unroll
+                            for (int i = 31; i >= 0; --i)
+                                if (z[i] == top) at = i;
+                            if (top > a.best) { a.best = a.z = top; a.token = n_c + at; }
                         }
-                        if (some - c < 16) may &= (1u << max(some - c, 0)) - 1u;
-                        while (may) {
-                            const int i = __ffs(may) - 1;
-                            may &= may - 1;
-                            float zi = z[c];
+                    } else {
+                        // g <= -log v: a bound of one logarithm on the special function unit, with room for its error, keeps all but a few tokens (as many as a running maximum
+                        // has steps, about) from the noise in full. Sixteen at a time, so that the best of the ones in front counts.
 #pragma unroll
-                            for (int j = 1; j < 16; ++j) zi = i == j ? z[c + j] : zi;
-                            const float value = fmaf(zi, p.inv_t, gumbel(draw(seed, row, first + c + i)));
-                            if (value > a.best || a.token < 0) { a.best = value; a.z = zi; a.token = first + c + i; }
+                        for (int d = 0; d < 32; d += 16) {
+                            uint32_t may = 0;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const float low = __uint_as_float((draw(seed, row, n_c + d + i) >> 9) | 0x3f800000u) - 1.f;   // v from below
+                                if (fmaf(lg2(low), -kLn2, z[d + i] * p.inv_t) + 1e-3f > a.best) may |= 1u << i;
+                            }
+                            if (some_c - d < 16) may &= (1u << max(some_c - d, 0)) - 1u;
+                            while (may) {
+                                const int i = __ffs(may) - 1;
+                                may &= may - 1;
+                                float zi = z[d];
+#pragma unroll
+                                for (int j = 1; j < 16; ++j) zi = i == j ? z[d + j] : zi;
+                                const float value = fmaf(zi, p.inv_t, gumbel(draw(seed, row, n_c + d + i)));
+                                if (value > a.best || a.token < 0) { a.best = value; a.z = zi; a.token = n_c + d + i; }
+                            }
                         }
                     }
-                }
-                // sum exp z: differences first, so that what is rounded is small where it counts
-                const float to = fmaxf(a.m, top), ref = to == -INFINITY ? 0.f : to;
-                const uint64_t ref2 = pair_of(-ref, -ref), log2 = pair_of(kLog2e, kLog2e);
-                uint64_t sums[4] = {0, 0, 0, 0};
+                    // sum exp z: differences first, so that what is rounded is small where it counts
+                    const float to = fmaxf(a.m, top), ref = to == -INFINITY ? 0.f : to;
+                    const uint64_t ref2 = pair_of(-ref, -ref), log2 = pair_of(kLog2e, kLog2e);
+                    uint64_t sums[2] = {0, 0};
 #pragma unroll
-                for (int i = 0; i < kCols / 4; ++i) {
-                    const float2 e = split(mul2(add2(pair_of(z[2 * i], z[2 * i + 1]), ref2), log2));
-                    sums[i & 3] = add2(sums[i & 3], pair_of(ex2(e.x), ex2(e.y)));
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 e = split(mul2(add2(pair_of(z[2 * i], z[2 * i + 1]), ref2), log2));
+                        sums[i & 1] = add2(sums[i & 1], pair_of(ex2(e.x), ex2(e.y)));
+                    }
+                    const float2 s = split(add2(sums[0], sums[1]));
+                    a.l = a.l * (a.m == to ? 1.f : ex2((a.m - ref) * kLog2e)) + (s.x + s.y);
+                    a.m = to;
                 }
-                const float2 s = split(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
-                a.l = a.l * (a.m == to ? 1.f : ex2((a.m - ref) * kLog2e)) + (s.x + s.y);
-                a.m = to;
             }
             if (row < p.rows && !failed) p.parts[(size_t)row * (2 * p.stretches) + 2 * (u / p.row_tiles) + half] = a;
         }
         if (failed && lane == 0) atomicExch(p.status, 3);
     }
     tc_fence_before();
-    __syncthreads();
-    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    if constexpr (kPair) cluster_sync_all();   // what the other CTA signals and reads is here until both are done
+    else __syncthreads();
+    if (warp == 9) {
+        if constexpr (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    }
 }
 
 // A warp per row.
@@ -318,19 +369,23 @@ __global__ void __launch_bounds__(kJoinThreads) vocab_join_kernel(const __grid_c
     }
 }
 
-// Stretches of the vocabulary: units (row tiles x stretches) of one CTA per SM. One row tile: as many as there are SMs, in copies of 32 rows, since the bytes of w are all
-// that counts. More: as many as leave the fewest tokens to the SM that has most, a unit's own cost counted as 32 tokens.
-void cut(int64_t rows, int64_t vocab, int* row_tiles, int* stretches, int* boxes, int* box) {
-    *row_tiles = ceil_div(rows, kRows);
-    *box = *row_tiles == 1 ? 32 : 64;
-    *boxes = ceil_div(vocab, *box);
-    const int sms = sm_count(), most = *boxes < 4 * sms ? *boxes : 4 * sms;
+// How a call is cut. Stretches of equal numbers of equal tiles, and as many of them as leave the fewest tokens to the CTA (or pair) that has most; a tile's own cost counts as 8
+// tokens, a unit's as 32.
+struct Cut { int row_tiles, stretches, tiles, cols; };
+Cut cut(int64_t rows, int64_t vocab) {
+    const bool pair = rows > kRows;
+    const int places = pair ? sm_count() / 2 : sm_count(), grain = pair ? 32 : 16, row_tiles = ceil_div(rows, pair ? 2 * kRows : kRows);
+    const int most = (int)(ceil_div(vocab, grain) < 8 * places ? ceil_div(vocab, grain) : 8 * places);
+    Cut c = {row_tiles, 1, 1, grain};
     int64_t best = -1;
-    *stretches = 1;
-    for (int n = 1; n <= (*row_tiles == 1 ? (most < sms ? most : sms) : most); ++n) {
-        const int64_t waves = ceil_div((int64_t)*row_tiles * n, sms), cost = waves * ((int64_t)ceil_div(*boxes, n) * *box + 32);
-        if (best < 0 || cost < best) { best = cost; *stretches = n; }
+    for (int n = 1; n <= most; ++n) {
+        if (n > 1 && (int64_t)row_tiles * n > 8 * places) break;   // (rows alone fill every place many times)
+        const int tiles = ceil_div(vocab, (int64_t)n * kCols), cols = (ceil_div(vocab, (int64_t)n * tiles) + grain - 1) / grain * grain;
+        const int stretches = ceil_div(vocab, (int64_t)tiles * cols);
+        const int64_t cost = (int64_t)ceil_div((int64_t)row_tiles * stretches, places) * (tiles * (cols + 8) + 32);
+        if (best < 0 || cost < best) { best = cost; c = {row_tiles, stretches, tiles, cols}; }
     }
+    return c;
 }
 
 int encode(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_rows) {
@@ -358,9 +413,7 @@ extern "C" {
 size_t gptrs_cuda_vocab_scores_scratch_bytes(const gptrs_vocab_scores* s) {
     if (!s || s->rows < 1 || s->vocab < 1) return 0;
     if (s->rows > 0x3fffffff || s->vocab > 0x3fffffff) return 0;
-    int row_tiles, stretches, boxes, box;
-    cut(s->rows, s->vocab, &row_tiles, &stretches, &boxes, &box);
-    return (size_t)s->rows * 2 * stretches * sizeof(Part);
+    return (size_t)s->rows * 2 * cut(s->rows, s->vocab).stretches * sizeof(Part);
 }
 
 int gptrs_cuda_vocab_scores(const gptrs_vocab_scores* s, void* stream) {
@@ -375,9 +428,12 @@ int gptrs_cuda_vocab_scores(const gptrs_vocab_scores* s, void* stream) {
     GPTRS_REQUIRE(!s->d_logprob || s->d_target, "log-probabilities of targets need targets");
     GPTRS_REQUIRE(s->rows == 0 || (s->d_scratch && s->scratch_bytes >= gptrs_cuda_vocab_scores_scratch_bytes(s)), "scratch is too small");
     if (s->rows == 0) return GPTRS_OK;
-    cut(s->rows, s->vocab, &p.row_tiles, &p.stretches, &p.boxes, &p.box);
-    int rc = encode(&p.x_map, s->d_hidden, s->dim, s->rows, ldx, kRows);
-    if (!rc) rc = encode(&p.w_map, s->d_weight, s->dim, s->vocab, ldw, p.box);
+    const Cut c = cut(s->rows, s->vocab);
+    const bool pair = s->rows > kRows;
+    p.row_tiles = c.row_tiles; p.stretches = c.stretches; p.tiles = c.tiles; p.cols = c.cols;
+    p.x_rows = s->rows < kRows ? (int)(s->rows + 7) / 8 * 8 : kRows;   // (rows that nobody has are not read out: whatever lies there)
+    int rc = encode(&p.x_map, s->d_hidden, s->dim, s->rows, ldx, p.x_rows);
+    if (!rc) rc = encode(&p.w_map, s->d_weight, s->dim, s->vocab, ldw, pair ? c.cols / 2 : c.cols);
     if (rc) return rc;
     p.bias = s->d_bias; p.seed_at = s->d_seed; p.target = s->d_target;
     p.parts = static_cast<Part*>(s->d_scratch);
@@ -385,15 +441,14 @@ int gptrs_cuda_vocab_scores(const gptrs_vocab_scores* s, void* stream) {
     p.rows = (int)s->rows; p.dim = (int)s->dim; p.vocab = (int)s->vocab;
     p.cap = s->soft_cap; p.inv_t = s->temperature > 0.f ? 1.f / s->temperature : 0.f; p.seed = s->seed;
     prefill_tc_fault(&p.starve, &p.wait_limit);
+    void (*kerns[4])(ScoreParams) = {vocab_scores_kernel<false, false>, vocab_scores_kernel<false, true>, vocab_scores_kernel<true, false>, vocab_scores_kernel<true, true>};
     static PerDeviceOnce attr_once;
-    if (attr_once.first_time()) {
-        GPTRS_CUDA_OK(cudaFuncSetAttribute(vocab_scores_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
-        GPTRS_CUDA_OK(cudaFuncSetAttribute(vocab_scores_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
-    }
-    const int64_t units = (int64_t)p.row_tiles * p.stretches;
+    if (attr_once.first_time())
+        for (int i = 0; i < 4; ++i) GPTRS_CUDA_OK(cudaFuncSetAttribute(kerns[i], cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(i >= 2)));
+    const int64_t units = (int64_t)p.row_tiles * p.stretches, places = pair ? sm_count() / 2 : sm_count();
     GPTRS_REQUIRE(units < ((int64_t)1 << 31), "too many rows");
-    rc = launch_kernel(p.inv_t > 0.f ? vocab_scores_kernel<true> : vocab_scores_kernel<false>, dim3((unsigned)(units < sm_count() ? units : sm_count())), dim3(kThreads), kSmem,
-                       as_stream(stream), 1, p);
+    rc = launch_kernel(kerns[2 * pair + (p.inv_t > 0.f)], dim3((unsigned)((units < places ? units : places) * (pair ? 2 : 1))), dim3(kThreads), smem_bytes(pair), as_stream(stream), 1, p,
+                       pair ? 2 : 1);
     if (rc) return rc;
     // the second kernel waits for the first one itself (griddepcontrol.wait), so it may be launched ahead of its end
     const int pdl = g_use_pdl;
