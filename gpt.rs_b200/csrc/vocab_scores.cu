@@ -3,8 +3,9 @@
 // z = x . w^T on the tcgen05 tensor cores, x rows as the M side. A unit is a tile of rows x a stretch of the vocabulary, which a CTA (one per SM) walks over in tiles of
 // up to 256 tokens. What a row needs to know of its logits is a running state in registers (maximum and sum, best token, the target's logit), so a logit lives
 // from the accumulator to the exponential and nowhere else.
-//   warps 0 - 7   a thread per row and half of the tile's tokens. The accumulator in tensor memory is read out every 256 of dim and added up in f32 registers: the tensor
-//                 cores cut what does not fit into the sum that they add to, 16 products at a time, which over all of dim would cost log-probabilities digits
+//   warps 0 - 7   a thread per row and half of the tile's tokens. The accumulator in tensor memory is read out every 128 or 512 of dim and added up in f32 registers: the
+//                 tensor cores cut what does not fit into the sum that they add to, 16 products at a time, which over all of dim would cost log-probabilities digits.
+//                 Up to 16 rows the logits then go through shared memory, and a warp takes a row with a token per lane
 //   warp 8        requests stages of 64 of dim
 //   warp 9        one thread issues the products into one of two accumulators
 // Up to 128 rows a tile is 128 rows and one CTA's. Above, a cluster of two CTAs works on 256 rows (cta_group::2): each brings its 128 rows of x and half of the tokens, 32 KB
@@ -21,18 +22,22 @@ void prefill_tc_fault(int* starve, uint32_t* wait_limit);   // the test switch o
 namespace {
 
 constexpr int kRows = 128;                      // of a CTA
-constexpr int kCols = 256;                      // most tokens of a tile
 constexpr int kStageDim = 64;                   // bf16 of a 128-byte swizzle span
-constexpr int kDrain = 4;                       // stages that an accumulator adds up
+// How a call's rows are worked on: up to 16 of them, up to 128, more (by pairs of CTAs).
+enum { kFew, kOne, kPairs };
+constexpr int cols_of(int mode) { return mode == kFew ? 128 : 256; }               // most tokens of a tile
+constexpr int stages_of(int mode) { return mode == kOne ? 4 : 6; }
+// Stages that an accumulator adds up. 128 of dim where w's bytes bound the call, 512 where the products do and each handing over takes time from them: relative errors of lse
+// at a dim of 4096 1.0e-7 and 4.0e-7 (f32 sums one by one 5.8e-7), of 4001 rows in 131072 tokens 1.72 ms with 256, 1.54 with 512.
+constexpr int drain_of(int mode) { return mode == kPairs ? 8 : 2; }
 constexpr int kABytes = kRows * 128;
 constexpr int kEpilogue = 256, kThreads = kEpilogue + 128;   // two warps of the last four only make their group whole
 // Registers of a thread at launch, and what the groups of four warps make of them: the shares add up to less than the block has, so every request ends.
 constexpr int kLaunchRegs = 168, kEpilogueRegs = 208, kOtherRegs = 80;
 static_assert(2 * kEpilogueRegs + kOtherRegs <= 3 * kLaunchRegs, "more registers than the block is launched with");
-constexpr int stages_of(bool pair) { return pair ? 6 : 4; }
-constexpr int stage_bytes(bool pair) { return kABytes + kCols / (pair ? 2 : 1) * 128; }
-constexpr size_t smem_bytes(bool pair) { return (size_t)stages_of(pair) * stage_bytes(pair) + 1024; }
-constexpr uint32_t kTmemCols = 2 * kCols;
+constexpr int kZRow = 132;                      // floats of a row of logits in shared memory (kFew)
+constexpr int stage_bytes(int mode) { return kABytes + 128 * (mode == kOne ? 256 : 128); }
+constexpr size_t smem_bytes(int mode) { return (size_t)stages_of(mode) * stage_bytes(mode) + 1024; }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kJoinThreads = 256;
 
@@ -43,12 +48,13 @@ struct ScoreParams {
     const float* bias;
     const uint32_t* seed_at;
     const int* target;
-    Part* parts;                  // [rows][2 stretches]
+    Part* parts;                  // [rows][row_parts]: of stretches (kFew), or halves of them
     int *pick, *status;
     float *pick_logprob, *logprob, *lse;
     int rows, dim, vocab;
     int row_tiles, stretches, tiles, cols;   // a stretch is `tiles` tiles of `cols` tokens
     int x_rows;                   // of a copy of x
+    int row_parts;
     float cap, inv_t;             // inv_t 0: greedy
     uint32_t seed, wait_limit;
     int starve;
@@ -104,13 +110,27 @@ __device__ __forceinline__ void commit(uint64_t* bar) {   // to the barrier of b
         umma_commit(bar);
 }
 
-template <bool kPair, bool kSample>
+// The best token among the lanes' and the sum of all.
+__device__ __forceinline__ Part join_lanes(Part a) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const Part b = {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.l, o), __shfl_xor_sync(0xffffffffu, a.best, o),
+                        __shfl_xor_sync(0xffffffffu, a.z, o), __shfl_xor_sync(0xffffffffu, a.token, o), __shfl_xor_sync(0xffffffffu, a.given, o)};
+        join(a, b);
+    }
+    return a;
+}
+
+template <int kMode, bool kSample>
 __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_constant__ ScoreParams p) {
-    constexpr int kStages = stages_of(kPair), kStageBytes = stage_bytes(kPair), kCtas = kPair ? 2 : 1;
+    constexpr bool kPair = kMode == kPairs;
+    constexpr int kStages = stages_of(kMode), kStageBytes = stage_bytes(kMode), kDrain = drain_of(kMode), kCols = cols_of(kMode), kCtas = kPair ? 2 : 1;
+    constexpr uint32_t kTmemCols = 2 * kCols;
     constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kCtas * kRows >> 4) << 24);   // f32 accumulator, bf16 operands
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_holder;
+    __shared__ __align__(16) float s_z[kMode == kFew ? 2 : 1][kMode == kFew ? 16 : 1][kZRow];
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = kPair ? (int)cluster_ctarank() : 0;   // the first CTA's thread issues the products of both
@@ -199,6 +219,84 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
             if (failed) atomicExch(p.status, 3);
         }
         __syncwarp();
+    } else if constexpr (kMode == kFew) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kEpilogueRegs));
+        // Warps 0 and 4 hold the rows in their first 16 lanes, 64 tokens each, and hand the logits to all eight: warp w has the rows w and w + 8, a lane every 32nd token. After a
+        // timeout every warp still goes through all tiles, without waiting, so that the barriers are met.
+        const int half = warp >> 2;
+        const bool holds = (warp & 3) == 0;
+        const uint32_t seed = p.seed_at ? *p.seed_at : p.seed;
+        int n = 0, tile = 0;
+        for (int u = blockIdx.x; u < units; u += gridDim.x) {
+            const Unit unit = unit_of(u);
+            Part a[2];
+            int target[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                a[r] = {-INFINITY, 0.f, -INFINITY, 0.f, -1, NAN};
+                target[r] = p.target && warp + 8 * r < p.rows ? p.target[warp + 8 * r] : -1;
+            }
+            for (int n0 = unit.begin; n0 < unit.end; n0 += p.cols, ++tile) {
+                uint64_t acc[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) acc[i] = 0;
+                for (int k0 = 0; k0 < steps; k0 += kDrain, ++n) {
+                    const int buf = n & 1;
+                    if (!failed && !mbar_wait_polled(&acc_full[buf], (uint32_t)(n >> 1) & 1u, p.wait_limit, 64)) failed = true;
+                    failed = __any_sync(0xffffffffu, failed);
+                    if (failed) break;
+                    tc_fence_after();
+                    if (holds) {
+                        uint32_t v[2][32];
+                        tmem_ld_32_begin(tmem + (uint32_t)(buf * kCols + 64 * half), v[0]);
+                        tmem_ld_32_begin(tmem + (uint32_t)(buf * kCols + 64 * half + 32), v[1]);
+                        tmem_ld_32_end(v[0]);
+                        tmem_ld_32_end(v[1]);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) acc[i] = add2(acc[i], pair_of(__uint_as_float(v[i >> 4][2 * (i & 15)]), __uint_as_float(v[i >> 4][2 * (i & 15) + 1])));
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&acc_empty[buf]);
+                }
+                if (holds && lane < 16) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 x = split(acc[2 * i]), y = split(acc[2 * i + 1]);
+                        *reinterpret_cast<float4*>(&s_z[tile & 1][lane][64 * half + 4 * i]) = make_float4(x.x, x.y, y.x, y.y);
+                    }
+                }
+                asm volatile("bar.sync 1, %0;\n" ::"n"(kEpilogue) : "memory");   // (of two copies in turn: who writes the next but one has seen this one read)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int row = warp + 8 * r;
+                    if (row >= p.rows) break;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int at = 32 * i + lane, token = n0 + at;
+                        if (at >= p.cols || token >= unit.end) continue;
+                        float z = s_z[tile & 1][row][at];
+                        if (p.bias) z += __ldg(p.bias + token);
+                        if (p.cap > 0.f) z = capped(z, p.cap);
+                        if (token == target[r]) a[r].given = z;
+                        float value = z;
+                        if constexpr (kSample) value = fmaf(z, p.inv_t, gumbel(draw(seed, row, token)));
+                        if (value > a[r].best) { a[r].best = value; a[r].z = z; a[r].token = token; }
+                        const float to = fmaxf(a[r].m, z), ref = to == -INFINITY ? 0.f : to;
+                        a[r].l = a[r].l * (a[r].m == to ? 1.f : ex2((a[r].m - ref) * kLog2e)) + ex2((z - ref) * kLog2e);
+                        a[r].m = to;
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = warp + 8 * r;
+                if (row >= p.rows) break;
+                const Part all = join_lanes(a[r]);
+                if (lane == 0 && !failed) p.parts[(size_t)row * p.stretches + u] = all;
+            }
+        }
+        if (failed && lane == 0) atomicExch(p.status, 3);
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kEpilogueRegs));
         // Quarters of 32 tokens that a warp has none of are left out; a warp without rows only hands accumulators back.
@@ -329,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                     a.m = to;
                 }
             }
-            if (row < p.rows && !failed) p.parts[(size_t)row * (2 * p.stretches) + 2 * (u / p.row_tiles) + half] = a;
+            if (row < p.rows && !failed) p.parts[(size_t)row * p.row_parts + 2 * (u / p.row_tiles) + half] = a;
         }
         if (failed && lane == 0) atomicExch(p.status, 3);
     }
@@ -346,44 +444,40 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
 __global__ void __launch_bounds__(kJoinThreads) vocab_join_kernel(const __grid_constant__ ScoreParams p) {
     pdl_launch_dependents();
     pdl_wait();
-    const int row = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31, n = 2 * p.stretches;
+    const int row = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31, n = p.row_parts;
     if (row >= p.rows) return;
     const Part* parts = p.parts + (size_t)row * n;
     Part a = {-INFINITY, 0.f, -INFINITY, 0.f, -1, NAN};
     for (int i = lane; i < n; i += 32) join(a, parts[i]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const Part b = {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.l, o), __shfl_xor_sync(0xffffffffu, a.best, o),
-                        __shfl_xor_sync(0xffffffffu, a.z, o), __shfl_xor_sync(0xffffffffu, a.token, o), __shfl_xor_sync(0xffffffffu, a.given, o)};
-        join(a, b);
-    }
+    a = join_lanes(a);
     if (lane) return;
-    const float log_l = logf(a.l);
-    if (p.lse) p.lse[row] = a.m + log_l;
+    const float lse = a.m + logf(a.l);
+    if (p.lse) p.lse[row] = lse;
     if (p.pick) p.pick[row] = max(a.token, 0);   // (nothing compares with NaN: the first token)
-    if (p.pick_logprob) p.pick_logprob[row] = a.z - a.m - log_l;
+    if (p.pick_logprob) p.pick_logprob[row] = a.z - lse;
     if (p.logprob) {
         const int target = p.target[row];
         if (target >= p.vocab) atomicExch(p.status, 2);
-        p.logprob[row] = target < 0 ? 0.f : a.given - a.m - log_l;
+        p.logprob[row] = target < 0 ? 0.f : a.given - lse;
     }
 }
 
 // How a call is cut. Stretches of equal numbers of equal tiles, and as many of them as leave the fewest tokens to the CTA (or pair) that has most; a tile's own cost counts as 8
 // tokens, a unit's as 32.
-struct Cut { int row_tiles, stretches, tiles, cols; };
+struct Cut { int mode, row_tiles, stretches, tiles, cols; };
 Cut cut(int64_t rows, int64_t vocab) {
-    const bool pair = rows > kRows;
+    const int mode = rows <= 16 ? kFew : rows <= kRows ? kOne : kPairs, widest = cols_of(mode);
+    const bool pair = mode == kPairs;
     const int places = pair ? sm_count() / 2 : sm_count(), grain = pair ? 32 : 16, row_tiles = ceil_div(rows, pair ? 2 * kRows : kRows);
     const int most = (int)(ceil_div(vocab, grain) < 8 * places ? ceil_div(vocab, grain) : 8 * places);
-    Cut c = {row_tiles, 1, 1, grain};
+    Cut c = {mode, row_tiles, 1, 1, grain};
     int64_t best = -1;
     for (int n = 1; n <= most; ++n) {
         if (n > 1 && (int64_t)row_tiles * n > 8 * places) break;   // (rows alone fill every place many times)
-        const int tiles = ceil_div(vocab, (int64_t)n * kCols), cols = (ceil_div(vocab, (int64_t)n * tiles) + grain - 1) / grain * grain;
+        const int tiles = ceil_div(vocab, (int64_t)n * widest), cols = (ceil_div(vocab, (int64_t)n * tiles) + grain - 1) / grain * grain;
         const int stretches = ceil_div(vocab, (int64_t)tiles * cols);
         const int64_t cost = (int64_t)ceil_div((int64_t)row_tiles * stretches, places) * (tiles * (cols + 8) + 32);
-        if (best < 0 || cost < best) { best = cost; c = {row_tiles, stretches, tiles, cols}; }
+        if (best < 0 || cost < best) { best = cost; c = {mode, row_tiles, stretches, tiles, cols}; }
     }
     return c;
 }
@@ -413,7 +507,8 @@ extern "C" {
 size_t gptrs_cuda_vocab_scores_scratch_bytes(const gptrs_vocab_scores* s) {
     if (!s || s->rows < 1 || s->vocab < 1) return 0;
     if (s->rows > 0x3fffffff || s->vocab > 0x3fffffff) return 0;
-    return (size_t)s->rows * 2 * cut(s->rows, s->vocab).stretches * sizeof(Part);
+    const Cut c = cut(s->rows, s->vocab);
+    return (size_t)s->rows * (c.mode == kFew ? 1 : 2) * c.stretches * sizeof(Part);
 }
 
 int gptrs_cuda_vocab_scores(const gptrs_vocab_scores* s, void* stream) {
@@ -429,7 +524,8 @@ int gptrs_cuda_vocab_scores(const gptrs_vocab_scores* s, void* stream) {
     GPTRS_REQUIRE(s->rows == 0 || (s->d_scratch && s->scratch_bytes >= gptrs_cuda_vocab_scores_scratch_bytes(s)), "scratch is too small");
     if (s->rows == 0) return GPTRS_OK;
     const Cut c = cut(s->rows, s->vocab);
-    const bool pair = s->rows > kRows;
+    const bool pair = c.mode == kPairs;
+    p.row_parts = c.mode == kFew ? c.stretches : 2 * c.stretches;
     p.row_tiles = c.row_tiles; p.stretches = c.stretches; p.tiles = c.tiles; p.cols = c.cols;
     p.x_rows = s->rows < kRows ? (int)(s->rows + 7) / 8 * 8 : kRows;   // (rows that nobody has are not read out: whatever lies there)
     int rc = encode(&p.x_map, s->d_hidden, s->dim, s->rows, ldx, p.x_rows);
@@ -441,13 +537,15 @@ int gptrs_cuda_vocab_scores(const gptrs_vocab_scores* s, void* stream) {
     p.rows = (int)s->rows; p.dim = (int)s->dim; p.vocab = (int)s->vocab;
     p.cap = s->soft_cap; p.inv_t = s->temperature > 0.f ? 1.f / s->temperature : 0.f; p.seed = s->seed;
     prefill_tc_fault(&p.starve, &p.wait_limit);
-    void (*kerns[4])(ScoreParams) = {vocab_scores_kernel<false, false>, vocab_scores_kernel<false, true>, vocab_scores_kernel<true, false>, vocab_scores_kernel<true, true>};
+    void (*kerns[3][2])(ScoreParams) = {{vocab_scores_kernel<kFew, false>, vocab_scores_kernel<kFew, true>},
+                                        {vocab_scores_kernel<kOne, false>, vocab_scores_kernel<kOne, true>},
+                                        {vocab_scores_kernel<kPairs, false>, vocab_scores_kernel<kPairs, true>}};
     static PerDeviceOnce attr_once;
     if (attr_once.first_time())
-        for (int i = 0; i < 4; ++i) GPTRS_CUDA_OK(cudaFuncSetAttribute(kerns[i], cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(i >= 2)));
+        for (int i = 0; i < 6; ++i) GPTRS_CUDA_OK(cudaFuncSetAttribute(kerns[i / 2][i & 1], cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(i / 2)));
     const int64_t units = (int64_t)p.row_tiles * p.stretches, places = pair ? sm_count() / 2 : sm_count();
     GPTRS_REQUIRE(units < ((int64_t)1 << 31), "too many rows");
-    rc = launch_kernel(kerns[2 * pair + (p.inv_t > 0.f)], dim3((unsigned)((units < places ? units : places) * (pair ? 2 : 1))), dim3(kThreads), smem_bytes(pair), as_stream(stream), 1, p,
+    rc = launch_kernel(kerns[c.mode][p.inv_t > 0.f], dim3((unsigned)((units < places ? units : places) * (pair ? 2 : 1))), dim3(kThreads), smem_bytes(c.mode), as_stream(stream), 1, p,
                        pair ? 2 : 1);
     if (rc) return rc;
     // the second kernel waits for the first one itself (griddepcontrol.wait), so it may be launched ahead of its end
