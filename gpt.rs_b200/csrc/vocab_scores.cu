@@ -25,18 +25,18 @@ constexpr int kRows = 128;                      // of a CTA
 constexpr int kStageDim = 64;                   // bf16 of a 128-byte swizzle span
 // How a call's rows are worked on: up to 16 of them, up to 128, more (by pairs of CTAs).
 enum { kFew, kOne, kPairs };
-constexpr int cols_of(int mode) { return mode == kFew ? 128 : 256; }               // most tokens of a tile
-constexpr int stages_of(int mode) { return mode == kOne ? 4 : 6; }
+constexpr int kCols = 256;                      // most tokens of a tile
+constexpr int stages_of(int mode) { return mode == kFew ? 5 : mode == kOne ? 4 : 6; }
+constexpr int x_bytes(int mode) { return 128 * (mode == kFew ? 64 : 128); }        // of a stage; products of 64 rows where there are 16 at most
 // Stages that an accumulator adds up. 128 of dim where w's bytes bound the call, 512 where the products do and each handing over takes time from them: relative errors of lse
 // at a dim of 4096 1.0e-7 and 4.0e-7 (f32 sums one by one 5.8e-7), of 4001 rows in 131072 tokens 1.72 ms with 256, 1.54 with 512.
 constexpr int drain_of(int mode) { return mode == kPairs ? 8 : 2; }
-constexpr int kABytes = kRows * 128;
 constexpr int kEpilogue = 256, kThreads = kEpilogue + 128;   // two warps of the last four only make their group whole
 // Registers of a thread at launch, and what the groups of four warps make of them: the shares add up to less than the block has, so every request ends.
 constexpr int kLaunchRegs = 168, kEpilogueRegs = 208, kOtherRegs = 80;
 static_assert(2 * kEpilogueRegs + kOtherRegs <= 3 * kLaunchRegs, "more registers than the block is launched with");
-constexpr int kZRow = 132;                      // floats of a row of logits in shared memory (kFew)
-constexpr int stage_bytes(int mode) { return kABytes + 128 * (mode == kOne ? 256 : 128); }
+constexpr int kZRow = kCols + 4;                // floats of a row of logits in shared memory (kFew)
+constexpr int stage_bytes(int mode) { return x_bytes(mode) + 128 * (mode == kPairs ? kCols / 2 : kCols); }
 constexpr size_t smem_bytes(int mode) { return (size_t)stages_of(mode) * stage_bytes(mode) + 1024; }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kJoinThreads = 256;
@@ -124,13 +124,13 @@ __device__ __forceinline__ Part join_lanes(Part a) {
 template <int kMode, bool kSample>
 __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_constant__ ScoreParams p) {
     constexpr bool kPair = kMode == kPairs;
-    constexpr int kStages = stages_of(kMode), kStageBytes = stage_bytes(kMode), kDrain = drain_of(kMode), kCols = cols_of(kMode), kCtas = kPair ? 2 : 1;
+    constexpr int kStages = stages_of(kMode), kStageBytes = stage_bytes(kMode), kDrain = drain_of(kMode), kABytes = x_bytes(kMode), kCtas = kPair ? 2 : 1;
     constexpr uint32_t kTmemCols = 2 * kCols;
-    constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kCtas * kRows >> 4) << 24);   // f32 accumulator, bf16 operands
+    constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)((kMode == kFew ? 64 : kCtas * kRows) >> 4) << 24);   // f32 accumulator, bf16 operands
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_holder;
-    __shared__ __align__(16) float s_z[kMode == kFew ? 2 : 1][kMode == kFew ? 16 : 1][kZRow];
+    __shared__ __align__(16) float s_z[kMode == kFew ? 16 : 1][kZRow];
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = kPair ? (int)cluster_ctarank() : 0;   // the first CTA's thread issues the products of both
@@ -221,12 +221,12 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
         __syncwarp();
     } else if constexpr (kMode == kFew) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kEpilogueRegs));
-        // Warps 0 and 4 hold the rows in their first 16 lanes, 64 tokens each, and hand the logits to all eight: warp w has the rows w and w + 8, a lane every 32nd token. After a
+        // Warps 0 and 4 hold the rows in their first 16 lanes, 128 tokens each, and hand the logits to all eight: warp w has the rows w and w + 8, a lane every 32nd token. After a
         // timeout every warp still goes through all tiles, without waiting, so that the barriers are met.
         const int half = warp >> 2;
         const bool holds = (warp & 3) == 0;
         const uint32_t seed = p.seed_at ? *p.seed_at : p.seed;
-        int n = 0, tile = 0;
+        int n = 0;
         for (int u = blockIdx.x; u < units; u += gridDim.x) {
             const Unit unit = unit_of(u);
             Part a[2];
@@ -236,10 +236,10 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                 a[r] = {-INFINITY, 0.f, -INFINITY, 0.f, -1, NAN};
                 target[r] = p.target && warp + 8 * r < p.rows ? p.target[warp + 8 * r] : -1;
             }
-            for (int n0 = unit.begin; n0 < unit.end; n0 += p.cols, ++tile) {
-                uint64_t acc[32];
+            for (int n0 = unit.begin; n0 < unit.end; n0 += p.cols) {
+                uint64_t acc[kCols / 4];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) acc[i] = 0;
+                for (int i = 0; i < kCols / 4; ++i) acc[i] = 0;
                 for (int k0 = 0; k0 < steps; k0 += kDrain, ++n) {
                     const int buf = n & 1;
                     if (!failed && !mbar_wait_polled(&acc_full[buf], (uint32_t)(n >> 1) & 1u, p.wait_limit, 64)) failed = true;
@@ -247,13 +247,17 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                     if (failed) break;
                     tc_fence_after();
                     if (holds) {
-                        uint32_t v[2][32];
-                        tmem_ld_32_begin(tmem + (uint32_t)(buf * kCols + 64 * half), v[0]);
-                        tmem_ld_32_begin(tmem + (uint32_t)(buf * kCols + 64 * half + 32), v[1]);
-                        tmem_ld_32_end(v[0]);
-                        tmem_ld_32_end(v[1]);
+                        uint32_t v[2][32];   // a quarter on its way while the one in front is added
+                        const uint32_t at = tmem + (uint32_t)(buf * kCols + 128 * half);
+                        tmem_ld_32_begin(at, v[0]);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) acc[i] = add2(acc[i], pair_of(__uint_as_float(v[i >> 4][2 * (i & 15)]), __uint_as_float(v[i >> 4][2 * (i & 15) + 1])));
+                        for (int c = 0; c < 4; ++c) {
+                            tmem_ld_32_end(v[c & 1]);
+                            if (c < 3) tmem_ld_32_begin(at + 32u * (c + 1), v[(c + 1) & 1]);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                acc[16 * c + i] = add2(acc[16 * c + i], pair_of(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])));
+                        }
                     }
                     tc_fence_before();
                     __syncwarp();
@@ -261,21 +265,21 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                 }
                 if (holds && lane < 16) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
+                    for (int i = 0; i < kCols / 8; ++i) {
                         const float2 x = split(acc[2 * i]), y = split(acc[2 * i + 1]);
-                        *reinterpret_cast<float4*>(&s_z[tile & 1][lane][64 * half + 4 * i]) = make_float4(x.x, x.y, y.x, y.y);
+                        *reinterpret_cast<float4*>(&s_z[lane][128 * half + 4 * i]) = make_float4(x.x, x.y, y.x, y.y);
                     }
                 }
-                asm volatile("bar.sync 1, %0;\n" ::"n"(kEpilogue) : "memory");   // (of two copies in turn: who writes the next but one has seen this one read)
+                asm volatile("bar.sync 1, %0;\n" ::"n"(kEpilogue) : "memory");
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     const int row = warp + 8 * r;
                     if (row >= p.rows) break;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < kCols / 32; ++i) {
                         const int at = 32 * i + lane, token = n0 + at;
                         if (at >= p.cols || token >= unit.end) continue;
-                        float z = s_z[tile & 1][row][at];
+                        float z = s_z[row][at];
                         if (p.bias) z += __ldg(p.bias + token);
                         if (p.cap > 0.f) z = capped(z, p.cap);
                         if (token == target[r]) a[r].given = z;
@@ -287,6 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                         a[r].m = to;
                     }
                 }
+                asm volatile("bar.sync 1, %0;\n" ::"n"(kEpilogue) : "memory");
             }
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
@@ -466,7 +471,7 @@ __global__ void __launch_bounds__(kJoinThreads) vocab_join_kernel(const __grid_c
 // tokens, a unit's as 32.
 struct Cut { int mode, row_tiles, stretches, tiles, cols; };
 Cut cut(int64_t rows, int64_t vocab) {
-    const int mode = rows <= 16 ? kFew : rows <= kRows ? kOne : kPairs, widest = cols_of(mode);
+    const int mode = rows <= 16 ? kFew : rows <= kRows ? kOne : kPairs;
     const bool pair = mode == kPairs;
     const int places = pair ? sm_count() / 2 : sm_count(), grain = pair ? 32 : 16, row_tiles = ceil_div(rows, pair ? 2 * kRows : kRows);
     const int most = (int)(ceil_div(vocab, grain) < 8 * places ? ceil_div(vocab, grain) : 8 * places);
@@ -474,7 +479,7 @@ Cut cut(int64_t rows, int64_t vocab) {
     int64_t best = -1;
     for (int n = 1; n <= most; ++n) {
         if (n > 1 && (int64_t)row_tiles * n > 8 * places) break;   // (rows alone fill every place many times)
-        const int tiles = ceil_div(vocab, (int64_t)n * widest), cols = (ceil_div(vocab, (int64_t)n * tiles) + grain - 1) / grain * grain;
+        const int tiles = ceil_div(vocab, (int64_t)n * kCols), cols = (ceil_div(vocab, (int64_t)n * tiles) + grain - 1) / grain * grain;
         const int stretches = ceil_div(vocab, (int64_t)tiles * cols);
         const int64_t cost = (int64_t)ceil_div((int64_t)row_tiles * stretches, places) * (tiles * (cols + 8) + 32);
         if (best < 0 || cost < best) { best = cost; c = {mode, row_tiles, stretches, tiles, cols}; }
