@@ -11,9 +11,12 @@
 // Blocks that reach behind the sequence's tokens are masked by a bit per node. In them values of nodes that are not finite are taken out of the stage before the product
 // (a weight of 0 does not help there) and added to the rows that see them at the end.
 //
-// Work. A unit is a block of 64 keys of a (tree, kv head, pair of row tiles). Every group of CTAs (two for trees of more than 128 rows, which then share the keys
-// through L2; else one) takes the same number of consecutive units, whatever the trees' lengths: where a group begins or ends inside an item, its rows' sums go to
-// scratch, and a second kernel joins the parts in the order of the keys. So the result depends on the call alone, not on what runs beside it.
+// Work, where contexts may be long: an item is a (tree, kv head, row tile or pair of them), a unit a block of an item, and an item has some more that stand for what it costs
+// beside its keys; every group of CTAs (one, or two for trees of more rows than a tile has, which then share the keys through L2) takes the same number of consecutive
+// units, whatever the trees' lengths. Where an item is cut, its parts are counted in warp by warp (a warp has the same rows in all of them): the last warp to finish waits until
+// the others' sums are in scratch and joins them with its own, four at a time, in the order of the keys, and such joins are joined again. So the result depends on the call
+// alone, not on who was last. Where contexts are short (kSmall) a cluster of up to eight CTAs takes a (tree, kv head, row tile), a share of its keys each, and joins through
+// distributed shared memory: nothing has to be added up or looked for in front.
 // Every wait is bounded: on a timeout code 3 goes to the status word, the roles leave their loops, tensor memory is freed.
 #include "draft_tree.cuh"
 #include "umma_common.cuh"
@@ -38,13 +41,12 @@ constexpr size_t kSmem = 2 * kQHalf + 4 * kStage + 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kMostSum = 16384.f;             // of a row's weights in a block: above it the reference is raised
 constexpr float kLargeScore = 1048576.f;        // above it a product and a sum rounded once (fma) are further apart than an exponent may be off
-constexpr int kMinUnits = 2;                    // of a group
+constexpr int kMinUnits = 8;                    // of a group
+constexpr int kORow = kTreeDim + 4;             // floats of a row of sums in shared memory
 constexpr int kWords = kMostNodes / 32;
+constexpr int kJoin = 4;                        // parts that are joined at a time
+constexpr int kLevels = 5;                      // 4^5 groups
 constexpr int kReaders = kSoftmaxWarps + 3;     // of a piece of work: the softmax's warps, the products' thread, the two that load
-
-// What a group tells the kernel that joins parts about the item that it begins inside of: the last group that has a part of it (-1: the group begins with an item, or another one
-// in front of it tells).
-struct Part { int last, row0, nodes, head, round, pad[3]; };
 
 struct AttentionParams {
     CUtensorMap map, q_map;
@@ -53,13 +55,14 @@ struct AttentionParams {
     long long ldq;
     const unsigned char* pool;
     __nv_bfloat16* out;
-    Part* begins;                // [groups]
-    float2* ml;                  // [2 groups tiles][row_cap]: reference and sum of a row; the first of a group's two slots for what others began
+    uint32_t *done, *stored;     // [levels][2 groups tiles][4]: parts of a join that are worked out, and in scratch, by warp; 0 again when it is made
+    float2* ml;                  // [2 groups tiles][row_cap]: reference and sum of a row; the first of a CTA's two slots is for items that others began
     float4* sums;                // [2 groups tiles][32][row_cap]
     int* status;
     float scale_log2;
     int groups, tiles, row_cap;  // tiles: of a group, 1 or 2
     int tile_nodes;              // of a tile: as many as 128 rows hold
+    int cluster, most_tiles;     // small calls: CTAs of a tile; tiles that a tree may have
     uint32_t wait_limit;
     int starve;
 };
@@ -69,27 +72,38 @@ __device__ __forceinline__ int rounds_of(const AttentionParams& p, const TreeSpa
     const int tiles = (s.nodes + p.tile_nodes - 1) / p.tile_nodes;
     return p.tiles == 2 ? (tiles + 1) >> 1 : tiles;
 }
+// What an item costs beside its blocks, in units: its queries, its output, and the masks of the blocks with nodes in them.
+__device__ __forceinline__ int extra_of(const TreeSpan& s) { return 2 + (s.nodes + kKeys - 1) / kKeys; }
 __device__ __forceinline__ uint32_t units_of(const AttentionParams& p, const TreeSpan& s) {   // (the host has made sure that they fit)
-    return s.nodes == 0 ? 0u : (uint32_t)blocks_of(s) * (uint32_t)rounds_of(p, s) * (uint32_t)p.t.kv_heads;
+    return s.nodes == 0 ? 0u : (uint32_t)(blocks_of(s) + extra_of(s)) * (uint32_t)rounds_of(p, s) * (uint32_t)p.t.kv_heads;
 }
-__device__ __forceinline__ long long begin_of(long long units, int groups, int j) { return units * j / groups; }
+// The first unit of group j, and the group that has a unit (at most 2^9 groups: 32 bits are enough for most calls).
+__device__ __forceinline__ long long begin_of(long long units, int groups, int j) {
+    return units < (1 << 22) ? (long long)((uint32_t)units * (uint32_t)j / (uint32_t)groups) : units * j / groups;
+}
+__device__ __forceinline__ int group_of(long long units, int groups, long long unit) {   // the last j with units j / groups < unit + 1
+    const long long x = (unit + 1) * groups - 1;
+    return units < (1 << 22) ? (int)((uint32_t)x / (uint32_t)units) : (int)(x / units);
+}
 
 // A piece of work: blocks kb0 .. kb1 - 1 of an item; kb1 0: there is none any more.
-struct Piece { TreeSpan span; int head, tile, kb0, kb1; };
+struct Piece { TreeSpan span; int head, tile, kb0, kb1, part, parts; };   // part: which of the item's
 
 // The pieces that a group goes through, in order.
 struct Walk {
     const AttentionParams& p;
-    int s, tile_of_group;
+    long long units, pos;        // of all; the one that comes next
+    int groups, s, tile_of_group;
     TreeSpan span;
-    uint32_t at, left;           // unit within the tree, units left
+    uint32_t at, left;           // pos within the tree, units left
     uint32_t tree_units;
-    int blocks, rounds;
-    int head, round, tile, kb0, kb1;
-    __device__ __forceinline__ Walk(const AttentionParams& p_, int s_, const TreeSpan& span_, uint32_t at_, uint32_t left_, int tile_)
-        : p(p_), s(s_), tile_of_group(tile_), span(span_), at(at_), left(left_) { measure(); }
+    int size, extra, rounds;     // an item's units, those in front of its blocks
+    Piece piece;
+    __device__ __forceinline__ Walk(const AttentionParams& p_, long long units_, int groups_, long long pos_, long long end, int s_, const TreeSpan& span_, uint32_t at_, int tile_)
+        : p(p_), units(units_), pos(pos_), groups(groups_), s(s_), tile_of_group(tile_), span(span_), at(at_), left((uint32_t)(end - pos_)) { measure(); }
     __device__ __forceinline__ void measure() {
-        blocks = blocks_of(span);
+        extra = extra_of(span);
+        size = blocks_of(span) + extra;
         rounds = rounds_of(p, span);
         tree_units = units_of(p, span);
     }
@@ -101,16 +115,21 @@ struct Walk {
                 measure();
                 continue;
             }
-            const uint32_t item = at / (uint32_t)blocks;
-            kb0 = (int)(at - item * (uint32_t)blocks);
-            kb1 = (int)min((uint32_t)blocks, (uint32_t)kb0 + left);
-            head = rounds == 1 ? (int)item : (int)(item / (uint32_t)rounds);
-            round = (int)item - head * rounds;
-            tile = round * p.tiles + tile_of_group;
-            at += (uint32_t)(kb1 - kb0);
-            left -= (uint32_t)(kb1 - kb0);
-            if (tile * p.tile_nodes < span.nodes) return true;
+            const uint32_t item = at / (uint32_t)size;
+            const int in_item = (int)(at - item * (uint32_t)size), n = (int)min((uint32_t)(size - in_item), left);
+            const long long first = pos - in_item;
+            at += n; left -= n; pos += n;
+            const int head = rounds == 1 ? (int)item : (int)(item / (uint32_t)rounds), tile = ((int)item - head * rounds) * p.tiles + tile_of_group;
+            piece = {span, head, tile, max(0, in_item - extra), in_item + n - extra, 0, 1};
+            if (piece.kb1 <= piece.kb0 || tile * p.tile_nodes >= span.nodes) continue;
+            if (piece.kb1 - piece.kb0 < size - extra) {
+                const int from = group_of(units, groups, first + extra);
+                piece.part = group_of(units, groups, pos - 1) - from;
+                piece.parts = group_of(units, groups, first + size - 1) - from + 1;
+            }
+            return true;
         }
+        piece.kb1 = 0;
         return false;
     }
 };
@@ -135,6 +154,15 @@ __device__ __forceinline__ uint64_t make_smem_desc_mn(uint32_t smem_addr) {
     d |= (uint64_t)2 << 61;
     return d;
 }
+__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+        "tcgen05.wait::ld.sync.aligned;\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
                  "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
@@ -155,6 +183,130 @@ __device__ __forceinline__ uint32_t bits_from(const uint32_t* row, int at) {
     return __funnelshift_r(row[w], w + 1 < kWords ? row[w + 1] : 0u, at & 31);
 }
 
+// Waits (bounded) until `n` parts of a join are in scratch, and sets the count back.
+__device__ __forceinline__ bool parts_stored(uint32_t* at, uint32_t n, uint32_t limit) {
+    for (uint32_t i = 0; i < 8 * limit; ++i) {
+        uint32_t v;
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];\n" : "=r"(v) : "l"(at) : "memory");
+        if (v >= n) { *at = 0; return true; }
+    }
+    return false;
+}
+// A load that stays where it is written: the ones of several parts are all under way before the first is used (left to the compiler a join of four took 15000 cycles).
+__device__ __forceinline__ float4 load_now(const float4* at) {
+    float4 v;
+    asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(at) : "memory");
+    return v;
+}
+// A warp's part of an item: to scratch, unless this warp is the last of its join's four; then it joins them, to the first one's place or, all of the item, to the output. Returns
+// false if a wait ran out.
+__device__ __forceinline__ bool join_parts(const AttentionParams& p, const Piece& piece, bool live, uint32_t t_o, float m, float l, uint4* dst) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, from = blockIdx.x / p.tiles - piece.part;
+    const size_t slots = 2 * (size_t)p.groups * p.tiles;
+    auto slot = [&](int part) { return 2 * ((size_t)(from + part) * p.tiles + blockIdx.x % p.tiles) + (part == 0 ? 1 : 0); };
+    int n = piece.parts, at = piece.part, apart = 1;   // parts of this level, this one's number, how far they lie apart
+    bool mine = true;                                  // the sums are in tensor memory; else in scratch
+    for (int level = 0; n > 1; ++level) {
+        const int first = at / kJoin * kJoin, members = min(kJoin, n - first), me = mine ? at - first : kJoin;
+        const size_t count = ((size_t)level * slots + slot(first * apart)) * kSoftmaxWarps + warp;
+        uint32_t before = members - 1;
+        if (members > 1) {
+            if (lane == 0) before = atomicInc(p.done + count, members - 1);   // (back to 0 by the last one)
+            before = __shfl_sync(0xffffffffu, before, 0);
+        }
+        const bool last = before == members - 1;
+        if (mine && (!last || members == 1)) {
+            float4* to = p.sums + slot(at) * 32 * p.row_cap + tid;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+                float o[32];
+                __syncwarp();
+                tmem_ld_32(t_o + 32u * c, o);
+                if (!live) continue;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) to[(8 * c + i) * p.row_cap] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
+            if (live) p.ml[slot(at) * p.row_cap + tid] = make_float2(m, l);
+            mine = false;
+        }
+        if (members > 1) {
+            if (!last) {
+                __threadfence();
+                __syncwarp();
+                if (lane == 0) atomicAdd(p.stored + count, 1u);
+                return true;
+            }
+            bool there = true;
+            if (lane == 0) there = parts_stored(p.stored + count, members - 1, p.wait_limit);
+            if (!__shfl_sync(0xffffffffu, (int)there, 0)) return false;
+            __threadfence();
+            const bool all = n <= kJoin;
+            // (loads without conditions, so that they are under way together: the first part's where there is none, or the own one is taken)
+            const float4* part[kJoin];
+            float2 ml[kJoin];
+            float f[kJoin], top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < kJoin; ++k) {
+                const size_t at_k = slot((first + (k < members ? k : 0)) * apart);
+                part[k] = p.sums + at_k * 32 * p.row_cap + tid;
+                ml[k] = __ldcg(p.ml + at_k * p.row_cap + tid);
+            }
+#pragma unroll
+            for (int k = 0; k < kJoin; ++k) {
+                if (k == me) ml[k] = make_float2(m, l);
+                if (k >= members) ml[k] = make_float2(-INFINITY, 0.f);
+                top = fmaxf(top, ml[k].x);
+            }
+            const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int k = 0; k < kJoin; ++k) {
+                f[k] = ex2(ml[k].x - ref);
+                sum += ml[k].x == -INFINITY ? ml[k].y : ml[k].y * f[k];   // (without a score 0, or NaN)
+            }
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            float4* to = p.sums + slot(first * apart) * 32 * p.row_cap + tid;
+            const int cap = p.row_cap;
+#pragma unroll 1
+            for (int c = 0; c < 32; c += 4) {
+                float4 v[kJoin][4], o[4];
+                uint32_t own[16];
+#pragma unroll
+                for (int k = 0; k < kJoin; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[k][i] = load_now(part[k] + (c + i) * cap);
+                __syncwarp();
+                if (mine) tmem_ld_16(t_o + 4u * c, own);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int k = 0; k < kJoin; ++k) {
+                        if (k >= members) break;
+                        if (k == me) v[k][i] = make_float4(__uint_as_float(own[4 * i]), __uint_as_float(own[4 * i + 1]), __uint_as_float(own[4 * i + 2]), __uint_as_float(own[4 * i + 3]));
+                        o[i].x += v[k][i].x * f[k]; o[i].y += v[k][i].y * f[k]; o[i].z += v[k][i].z * f[k]; o[i].w += v[k][i].w * f[k];
+                    }
+                }
+                if (!live) continue;
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    if (all) dst[(c + i) / 2] = make_uint4(pack_bf16x2(o[i].x * inv, o[i].y * inv), pack_bf16x2(o[i].z * inv, o[i].w * inv), pack_bf16x2(o[i + 1].x * inv, o[i + 1].y * inv),
+                                                           pack_bf16x2(o[i + 1].z * inv, o[i + 1].w * inv));
+                    else { to[(c + i) * cap] = o[i]; to[(c + i + 1) * cap] = o[i + 1]; }
+                }
+            }
+            if (!all && live) p.ml[slot(first * apart) * p.row_cap + tid] = make_float2(top, sum);
+            mine = false;
+            m = top;
+            l = sum;
+        }
+        at /= kJoin;
+        n = (n + kJoin - 1) / kJoin;
+        apart *= kJoin;
+    }
+    return true;
+}
+
+template <bool kSmall>
 __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __grid_constant__ AttentionParams p) {
     // f32 accumulator, bf16 operands, M = 128; N = 64, or 128 with B's contraction index as rows
     constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kRows >> 4) << 24);
@@ -163,6 +315,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
     __shared__ __align__(8) uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], q_full, q_empty, piece_full[2], piece_empty[2], sees_full[2];
     __shared__ uint32_t tmem_holder;
     __shared__ long long s_sum[kSoftmaxWarps], s_first;
+    __shared__ float2 s_ml[kSmall ? kRows : 1];         // of the rows of a share
     __shared__ int s_tree;
     __shared__ TreeSpan s_span;
     __shared__ Piece s_piece[2];                        // this one and the next
@@ -174,7 +327,6 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t sQ = smem, sK = smem + 2 * kQHalf, sV = sK + 2 * kStage;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int group = blockIdx.x / p.tiles, tile_of_group = blockIdx.x % p.tiles;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&k_full[i], 1); mbar_init(&v_full[i], 1); mbar_init(&k_empty[i], 1); mbar_init(&v_empty[i], 1); mbar_init(&s_full[i], 1);
@@ -190,11 +342,27 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
     }
     pdl_wait();
 
-    // ---- this group's units: warps 0 - 3 of every CTA add up the trees' -----------------------------------------------------------
+    // ---- this CTA's work
     const int per = (p.t.n_trees + kRows - 1) / kRows;
-    long long mine = 0, upto = 0;
+    const int rank = kSmall && p.cluster > 1 ? blockIdx.x % p.cluster : 0, group = blockIdx.x / p.tiles, tile_of_group = blockIdx.x % p.tiles;
     TreeSpan last = {-1, 0, 0, 0};
-    if (warp < kSoftmaxWarps) {
+    Piece only = {};                                    // a small call's
+    int groups = 1;
+    long long units = 0, begin = 0, end = 0, mine = 0, upto = 0;
+    bool idles = false;
+    if constexpr (kSmall) {
+        const int task = blockIdx.x / p.cluster, s = task / (p.t.kv_heads * p.most_tiles), in_tree = task - s * (p.t.kv_heads * p.most_tiles);
+        only.span = tree_span(p.t, s, p.status);
+        only.head = in_tree / p.most_tiles;
+        only.tile = in_tree - only.head * p.most_tiles;
+        only.parts = 1;
+        idles = only.tile * p.tile_nodes >= only.span.nodes;
+        if (!idles) {
+            const int blocks = blocks_of(only.span);
+            only.kb0 = blocks * rank / p.cluster;
+            only.kb1 = blocks * (rank + 1) / p.cluster;
+        }
+    } else if (warp < kSoftmaxWarps) {   // warps 0 - 3 add up the trees' units
         for (int s = tid * per; s < min((tid + 1) * per, p.t.n_trees); ++s) {
             last = tree_span(p.t, s, p.status);
             mine += units_of(p, last);
@@ -211,40 +379,44 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_holder;
-    long long units = 0;
+    if constexpr (!kSmall) {
 #pragma unroll
-    for (int w = 0; w < kSoftmaxWarps; ++w) {
-        if (w == warp) upto += units;
-        units += s_sum[w];
-    }
-    const int groups = (int)max(1ll, min((long long)p.groups, units / kMinUnits));
-    if (units == 0 || group >= groups) {                // the whole CTA
-        if (tile_of_group == 0 && tid == 0) p.begins[group].last = -1;
-        __syncthreads();
-        if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
-        return;
-    }
-    const long long begin = begin_of(units, groups, group), end = begin_of(units, groups, group + 1);
-    if (warp < kSoftmaxWarps && begin >= upto - mine && begin < upto) {
-        long long first = upto - mine;
-        int s = tid * per;
-        if (per > 1) {
-            for (;; ++s) {
-                last = tree_span(p.t, s, p.status);
-                const long long here = units_of(p, last);
-                if (begin < first + here) break;
-                first += here;
-            }
+        for (int w = 0; w < kSoftmaxWarps; ++w) {
+            if (w == warp) upto += units;
+            units += s_sum[w];
         }
-        s_tree = s;
-        s_first = first;
-        s_span = last;
+        groups = (int)max(1ll, min((long long)p.groups, units / kMinUnits));
+        idles = units == 0 || group >= groups;
+        if (!idles) {
+            begin = begin_of(units, groups, group);
+            end = begin_of(units, groups, group + 1);
+        }
+        if (warp < kSoftmaxWarps && !idles && begin >= upto - mine && begin < upto) {
+            long long first = upto - mine;
+            int s = tid * per;
+            if (per > 1) {
+                for (;; ++s) {
+                    last = tree_span(p.t, s, p.status);
+                    const long long here = units_of(p, last);
+                    if (begin < first + here) break;
+                    first += here;
+                }
+            }
+            s_tree = s;
+            s_first = first;
+            s_span = last;
+        }
+        __syncthreads();
     }
-    __syncthreads();
     pdl_launch_dependents();
     bool failed = false;
     // A piece's place in the ring, for those that read it: the i-th of this CTA.
     auto take = [&](int i, Piece* piece) {
+        if constexpr (kSmall) {
+            *piece = only;
+            return i == 0 && only.kb1 > only.kb0;
+        }
+        if (idles) return false;
         if (!failed && !mbar_wait_parked(smem_u32(&piece_full[i & 1]), (uint32_t)(i >> 1) & 1u, p.wait_limit)) failed = true;
         if (failed) return false;
         *piece = s_piece[i & 1];
@@ -253,7 +425,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
 
     if (warp == kMmaWarp + 3) {
         // ================= warp 7: the next piece, its queries, and who sees whom =====================================================
-        Walk walk(p, s_tree, s_span, (uint32_t)(begin - s_first), (uint32_t)(end - begin), tile_of_group);
+        Walk walk(p, units, groups, begin, end, kSmall ? 0 : s_tree, kSmall ? only.span : s_span, kSmall ? 0u : (uint32_t)(begin - s_first), tile_of_group);
+        if constexpr (kSmall) walk.piece = only;
         int tree = -1;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
             if (!failed && !mbar_wait_parked(smem_u32(bar), parity & 1u, p.wait_limit)) failed = true;
@@ -261,11 +434,12 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
             return !failed;
         };
         int asked = 0;
-        for (int i = 0;; ++i) {
-            const bool more = walk.next();
+        for (int i = 0; !idles; ++i) {
+            bool more = kSmall && i == 0 && only.kb1 > only.kb0;
+            if constexpr (!kSmall) more = walk.next();
             if (i >= 2 && !wait(&piece_empty[i & 1], (uint32_t)((i >> 1) - 1))) break;
-            if (lane == 0) {
-                s_piece[i & 1] = {walk.span, walk.head, walk.tile, walk.kb0, more ? walk.kb1 : 0};
+            if (!kSmall && lane == 0) {
+                s_piece[i & 1] = walk.piece;
                 mbar_arrive(&piece_full[i & 1]);
             }
             __syncwarp();
@@ -275,18 +449,19 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
                     const uint32_t bar = smem_u32(&q_full);
                     mbar_expect_tx_addr(bar, (uint32_t)(p.tile_nodes * p.t.group) * 256u);
                     for (int h = 0; h < 2; ++h)
-                        tma_load_4d(sQ + h * kQHalf, &p.q_map, 0, h, walk.head * p.t.group, walk.span.row0 + walk.tile * p.tile_nodes, bar);
+                        tma_load_4d(sQ + h * kQHalf, &p.q_map, 0, h, walk.piece.head * p.t.group, walk.piece.span.row0 + walk.piece.tile * p.tile_nodes, bar);
                 }
                 ++asked;
                 __syncwarp();
             };
             if (i == 0) ask();
+            const TreeSpan& span = walk.piece.span;
             if (walk.s != tree) {
-                for (int k = lane; k < walk.span.nodes; k += 32) s_up[k] = tree_parent(p.t, walk.span, k, p.status);
+                for (int k = lane; k < span.nodes; k += 32) s_up[k] = tree_parent(p.t, span, k, p.status);
                 tree = walk.s;
                 __syncwarp();
             }
-            const int node0 = walk.tile * p.tile_nodes, nodes = min(p.tile_nodes, walk.span.nodes - node0);
+            const int node0 = walk.piece.tile * p.tile_nodes, nodes = min(p.tile_nodes, span.nodes - node0);
             for (int k = lane; k < nodes; k += 32) {
                 uint32_t bits[kWords] = {};
                 for (int up = node0 + k; up >= 0; up = s_up[up])
@@ -303,13 +478,6 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
                 if (!wait(&q_empty, (uint32_t)(i - 1))) break;   // the products with the last piece's queries are complete
                 ask();
             }
-        }
-        if (lane == 0 && tile_of_group == 0) {   // for the kernel that joins parts
-            const TreeSpan span = s_span;
-            const int blocks = blocks_of(span), rounds = rounds_of(p, span), item = (int)((begin - s_first) / blocks);
-            const long long first = s_first + (long long)item * blocks;
-            const bool tells = begin != first && begin_of(units, groups, group - 1) <= first;
-            p.begins[group] = {tells ? (int)min((long long)groups, ((first + blocks) * groups + units - 1) / units) - 1 : -1, span.row0, span.nodes, item / rounds, item % rounds};
         }
         if (asked) mbar_wait_parked(smem_u32(&q_full), (uint32_t)(asked - 1) & 1u, p.wait_limit);   // (queries in flight write this CTA's shared memory)
         if (failed && lane == 0) atomicExch(p.status, 3);
@@ -425,6 +593,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
         const int my_node = tid / p.t.group, my_head = tid - my_node * p.t.group;
         int g = 0;
         Piece piece;
+        if constexpr (kSmall) s_ml[tid] = make_float2(-INFINITY, 0.f);
         for (int at = 0; __all_sync(0xffffffffu, take(at, &piece)); ++at) {
             const TreeSpan& span = piece.span;
             const int node0 = piece.tile * p.tile_nodes, node = node0 + my_node;
@@ -538,24 +707,27 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
                     if (!wait(&v_full[g & 1], (uint32_t)(g >> 1))) break;
                     // values behind the last node, and those of nodes that are not finite: the product sees zeros
                     const int from = max(0, span.length - kb * kKeys), total = span.length + span.nodes;
-                    for (int i = tid; i < (kKeys - from) * 16; i += kRows) {
-                        const int r = from + (i >> 4), token = kb * kKeys + r;
-                        const uint32_t to = sV + (g & 1) * kStage + (i >> 3 & 1) * kHalf + r * 128 + ((i & 7) << 4);
-                        uint4 v = ld_shared_v4(to);
-                        if (token >= total) {
-                            st_shared_v4(to, 0, 0, 0, 0);
-                        } else {
-                            uint32_t *w = &v.x, odd = 0;
+                    const int chunk = tid & 15, r0 = tid >> 4;
+                    const uint32_t stage = sV + (g & 1) * kStage + (chunk >> 3) * kHalf + ((chunk & 7) << 4);
+                    uint4 v[kKeys / 8];
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const uint32_t none = __vcmpgeu2(w[k] & 0x7fff7fffu, 0x7f807f80u);
-                                w[k] &= ~none;
-                                odd |= none;
-                            }
-                            if (odd) {
-                                st_shared_v4(to, v.x, v.y, v.z, v.w);
-                                atomicOr(&s_odd[at & 1][(token - span.length) >> 5], 1u << ((token - span.length) & 31));
-                            }
+                    for (int k = 0; k < kKeys / 8; ++k) v[k] = ld_shared_v4(stage + (8 * k + r0) * 128);
+                    uint32_t odd_rows = 0;
+#pragma unroll
+                    for (int k = 0; k < kKeys / 8; ++k)
+                        odd_rows |= ((__vcmpgeu2(v[k].x & 0x7fff7fffu, 0x7f807f80u) | __vcmpgeu2(v[k].y & 0x7fff7fffu, 0x7f807f80u) | __vcmpgeu2(v[k].z & 0x7fff7fffu, 0x7f807f80u) |
+                                      __vcmpgeu2(v[k].w & 0x7fff7fffu, 0x7f807f80u)) ? 1u : 0u) << k;
+                    for (int k = 0; k < kKeys / 8; ++k) {
+                        const int r = 8 * k + r0, token = kb * kKeys + r;
+                        if (token >= total) {
+                            st_shared_v4(stage + r * 128, 0, 0, 0, 0);
+                        } else if (odd_rows >> k & 1 && r >= from) {
+                            uint4 x = ld_shared_v4(stage + r * 128);
+                            uint32_t* w = &x.x;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) w[j] &= ~__vcmpgeu2(w[j] & 0x7fff7fffu, 0x7f807f80u);
+                            st_shared_v4(stage + r * 128, x.x, x.y, x.z, x.w);
+                            atomicOr(&s_odd[at & 1][(token - span.length) >> 5], 1u << ((token - span.length) & 31));
                         }
                     }
                     fence_proxy_async();
@@ -568,25 +740,20 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
             if (failed || !wait(&v_empty[(g - 1) & 1], (uint32_t)((g - 1) >> 1))) break;
             tc_fence_after();
             if (!idle) {
-                const bool whole = piece.kb0 == 0 && piece.kb1 == blocks_of(span);
-                const size_t slot = 2 * (size_t)blockIdx.x + (piece.kb0 == 0 ? 1 : 0);
                 if (any && m == -INFINITY) l = NAN;             // scores of -inf alone
-                const float inv = whole ? (any ? 1.f / l : 0.f) : 1.f;
                 uint32_t odd = 0;
                 if (masked) {
 #pragma unroll
                     for (int w = 0; w < kWords; ++w) odd |= s_odd[at & 1][w] & sees[w];
                 }
-                if (!whole && live) p.ml[slot * p.row_cap + tid] = make_float2(m, l);
-                uint4* dst = reinterpret_cast<uint4*>(p.out + ((long long)(span.row0 + node) * p.t.q_heads + piece.head * p.t.group + my_head) * kTreeDim);
+                if (__any_sync(0xffffffffu, live && odd)) {     // the values that the products left out, for the rows that see them
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    float o[32];
-                    __syncwarp();
-                    tmem_ld_32(t_o + 32u * c, o);
-                    if (!live) continue;
-                    if (odd) {
-                        for (int i = 0; i < span.nodes; ++i) {
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t o[32];
+                        __syncwarp();
+                        tmem_ld_32_begin(t_o + 32u * c, o);
+                        tmem_ld_32_end(o);
+                        for (int i = 0; live && i < span.nodes; ++i) {
                             if (!(s_odd[at & 1][i >> 5] & sees[i >> 5] & 1u << (i & 31))) continue;
                             const int where = span.length + i;
                             const long long place = tree_place(p.t, span.slot, where, p.status);
@@ -595,19 +762,44 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
                             for (int j = 0; j < 32; ++j) {
                                 const int chunk = 4 * c + (j >> 3);
                                 const uint16_t v = *reinterpret_cast<const uint16_t*>(p.pool + place + (2 * piece.head + 1) * kTreeBlock + ((chunk ^ (where & 7)) << 4) + 2 * (j & 7));
-                                if (not_finite(v)) o[j] += __uint_as_float((uint32_t)v << 16);
+                                if (not_finite(v)) o[j] = __float_as_uint(__uint_as_float(o[j]) + __uint_as_float((uint32_t)v << 16));
                             }
                         }
+                        __syncwarp();
+                        tmem_st_32(t_o + 32u * c, o);
                     }
-                    if (whole) {
+                    asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+                }
+                uint4* dst = reinterpret_cast<uint4*>(p.out + ((long long)(span.row0 + node) * p.t.q_heads + piece.head * p.t.group + my_head) * kTreeDim);
+                if (kSmall && p.cluster > 1) {                  // the share's sums to shared memory, where the stages and the queries were
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        float o[32];
+                        __syncwarp();
+                        tmem_ld_32(t_o + 32u * c, o);
+                        if (!live) continue;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            st_shared_v4(sQ + (tid * kORow + 32 * c + 4 * i) * 4, __float_as_uint(o[4 * i]), __float_as_uint(o[4 * i + 1]), __float_as_uint(o[4 * i + 2]), __float_as_uint(o[4 * i + 3]));
+                    }
+                    if (kSmall && live) s_ml[tid] = make_float2(m, l);
+                } else if (piece.parts == 1) {
+                    const float inv = any ? 1.f / l : 0.f;
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        float o[32];
+                        __syncwarp();
+                        tmem_ld_32(t_o + 32u * c, o);
+                        if (!live) continue;
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             dst[4 * c + i] = make_uint4(pack_bf16x2(o[8 * i] * inv, o[8 * i + 1] * inv), pack_bf16x2(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
                                                         pack_bf16x2(o[8 * i + 4] * inv, o[8 * i + 5] * inv), pack_bf16x2(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            p.sums[(slot * 32 + 8 * c + i) * p.row_cap + tid] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    }
+                } else if constexpr (!kSmall) {
+                    if (!join_parts(p, piece, live, t_o, m, l, dst)) {
+                        failed = true;
+                        break;
                     }
                 }
             }
@@ -617,86 +809,46 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
         }
         if (__any_sync(0xffffffffu, failed) && lane == 0) atomicExch(p.status, 3);
     }
+    __syncwarp();
     tc_fence_before();
+    if (kSmall && p.cluster > 1) {
+        // ---- the shares of the cluster's task, in the order of the keys: a CTA takes every cluster-th row, a warp a row at a time, four channels a lane
+        cluster_sync_all();
+        const TreeSpan& span = only.span;
+        const int node0 = only.tile * p.tile_nodes, rows = idles ? 0 : min(p.tile_nodes, span.nodes - node0) * p.t.group;
+        const uint32_t ml_at = smem_u32(s_ml);
+        for (int row = rank + p.cluster * warp; row < rows; row += p.cluster * (kThreads / 32)) {
+            float2 ml[8];
+            float4 v[8];
+            float top = -INFINITY, l = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                ml[k] = make_float2(-INFINITY, 0.f);
+                if (k < p.cluster) {
+                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n" : "=f"(ml[k].x), "=f"(ml[k].y) : "r"(map_to_cta(ml_at + 8 * row, k)));
+                    v[k] = ld_dsmem_f4(map_to_cta(sQ + (row * kORow + 4 * lane) * 4, k));
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
+            const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float f = ex2(ml[k].x - ref);
+                if (ml[k].x == -INFINITY) { l += ml[k].y; continue; }   // (without a score 0, or NaN)
+                l += ml[k].y * f;
+                if (k < p.cluster) { o.x += v[k].x * f; o.y += v[k].y * f; o.z += v[k].z * f; o.w += v[k].w * f; }
+            }
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const int node = row / p.t.group;
+            *reinterpret_cast<uint2*>(p.out + ((long long)(span.row0 + node0 + node) * p.t.q_heads + only.head * p.t.group + (row - node * p.t.group)) * kTreeDim + 4 * lane) =
+                make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+        }
+        cluster_sync_all();   // nobody leaves while its sums are read
+    }
     __syncthreads();
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
-}
-
-// Joins the parts of the items in which a group begins. A piece of work is (group, tile, 32 rows, 64 channels); a CTA looks at all of its own at once, most of which are
-// none (a CTA for each of them: 14 us for one tree, where this takes 5).
-constexpr int kJoinThreads = 256;
-__device__ __forceinline__ void join_part(const AttentionParams& p, const Part& item, int j, int tile_of_group, int quarter, int half, __nv_bfloat16 (*s_out)[64 + 8]);
-__global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_constant__ AttentionParams p) {
-    __shared__ __align__(16) __nv_bfloat16 s_out[32][64 + 8];
-    __shared__ Part s_items[32];
-    pdl_launch_dependents();
-    pdl_wait();
-    const int per_group = p.tiles * (p.row_cap / 32) * 2, all = (p.groups - 1) * per_group;
-    for (int w0 = blockIdx.x; w0 < all; w0 += 32 * gridDim.x) {
-        if (threadIdx.x < 32) {
-            const int w = w0 + threadIdx.x * gridDim.x;
-            Part item = {-1};
-            if (w < all) item = p.begins[w / per_group + 1];
-            s_items[threadIdx.x] = item;
-        }
-        __syncthreads();
-        for (int i = 0; i < 32; ++i) {
-            const int w = w0 + i * gridDim.x, j = w / per_group + 1, y = w % per_group;
-            if (w >= all) break;
-            if (s_items[i].last < 0) continue;
-            join_part(p, s_items[i], j, (y >> 1) / (p.row_cap / 32), (y >> 1) % (p.row_cap / 32), y & 1, s_out);
-        }
-        __syncthreads();
-    }
-}
-__device__ __forceinline__ void join_part(const AttentionParams& p, const Part& item, int j, int tile_of_group, int quarter, int half, __nv_bfloat16 (*s_out)[64 + 8]) {
-    const int tile = item.round * p.tiles + tile_of_group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = quarter * 32 + lane;
-    const int rows = min(p.tile_nodes, item.nodes - tile * p.tile_nodes) * p.t.group;
-    if (quarter * 32 >= rows) return;   // the whole CTA
-    const bool live = row < rows;
-    auto slot = [&](int k) { return 2 * ((size_t)k * p.tiles + tile_of_group) + (k == j - 1 ? 1 : 0); };
-    float top = -INFINITY, l = 0.f;
-    float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-    constexpr int kAtOnce = 4;
-    for (int k0 = j - 1; k0 <= item.last && live; k0 += kAtOnce) {
-        float2 ml[kAtOnce];
-        float4 v[kAtOnce][2];
-#pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) {
-            ml[k] = make_float2(-INFINITY, 0.f);
-            v[k][0] = v[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (k0 + k <= item.last) {
-                ml[k] = p.ml[slot(k0 + k) * p.row_cap + row];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) v[k][i] = p.sums[(slot(k0 + k) * 32 + 16 * half + 8 * i + warp) * p.row_cap + row];
-            }
-        }
-        float to = top;
-#pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) to = fmaxf(to, ml[k].x);
-        const float ref = to == -INFINITY ? 0.f : to, keep = ex2(top - ref);   // (top -inf: nothing yet, 0)
-        top = to;
-        l = l == 0.f ? 0.f : l * keep;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) { o[i].x *= keep; o[i].y *= keep; o[i].z *= keep; o[i].w *= keep; }
-#pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) {
-            const float f = ex2(ml[k].x - ref);
-            l += ml[k].x == -INFINITY ? ml[k].y : ml[k].y * f;   // (without a score 0, or NaN)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) { o[i].x += v[k][i].x * f; o[i].y += v[k][i].y * f; o[i].z += v[k][i].z * f; o[i].w += v[k][i].w * f; }
-        }
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        *reinterpret_cast<uint2*>(&s_out[lane][4 * (8 * i + warp)]) = make_uint2(pack_bf16x2(o[i].x * inv, o[i].y * inv), pack_bf16x2(o[i].z * inv, o[i].w * inv));
-    __syncthreads();
-    const int r = threadIdx.x >> 3, rr = quarter * 32 + r;
-    if (rr < rows)
-        *reinterpret_cast<uint4*>(p.out + ((long long)(item.row0 + tile * p.tile_nodes + rr / p.t.group) * p.t.q_heads + item.head * p.t.group + rr % p.t.group) * kTreeDim + 64 * half +
-                                  8 * (threadIdx.x & 7)) = *reinterpret_cast<const uint4*>(&s_out[r][8 * (threadIdx.x & 7)]);
-    __syncthreads();
 }
 
 // The pool as rows of a token and head of 256 bytes (z), two halves (y) of 64 channels (x); a block (page, kv head, keys or values) begins at row
@@ -730,15 +882,25 @@ int encode_queries(const void* q, int64_t ldq, const DraftTrees& t, int tile_nod
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// How a call is cut: groups of one CTA, or of two where trees may have more rows than a tile.
-void cut(const gptrs_draft_trees* t, int* groups, int* tiles, int* row_cap, int* tile_nodes) {
+// How a call is cut. The host does not know the lengths, but the page table's width bounds them. Small: a cluster per (tree, kv head, row tile), with as many CTAs (8, 4, 2, 1) as
+// leave a processor, or half of one, to each; taken where the longest context can cost no more than equal shares of all of them and their joins, which take as long as
+// twenty blocks. Others: as many CTAs as there are places, in groups of one, or of two where trees may have more rows than a tile.
+struct Cut { int cluster, ctas, groups, tiles, row_cap, tile_nodes, most_tiles; bool small; };
+Cut cut(const gptrs_draft_trees* t) {
+    Cut c;
     const int group = t->q_heads / t->kv_heads, rows = t->max_nodes * group;
-    *tile_nodes = kRows / group;
-    *tiles = t->max_nodes > *tile_nodes ? 2 : 1;
-    *groups = 2 * sm_count() / *tiles;
-    *row_cap = rows < kRows ? (rows + 31) / 32 * 32 : kRows;
+    c.tile_nodes = kRows / group;
+    c.most_tiles = ceil_div(t->max_nodes, c.tile_nodes);
+    const int64_t sms = sm_count(), tasks = t->n_trees * t->kv_heads * c.most_tiles, longest = ceil_div(t->max_pages * kTreePage, kKeys);
+    c.cluster = tasks * 8 <= sms ? 8 : tasks * 4 <= sms ? 4 : tasks * 2 <= 2 * sms ? 2 : 1;
+    c.small = tasks * c.cluster <= 2 * sms ? longest / c.cluster <= tasks * longest / (2 * sms) + 20 : tasks < (1 << 24) && longest <= 20;
+    c.tiles = !c.small && c.most_tiles > 1 ? 2 : 1;
+    c.ctas = c.small ? (int)(tasks * c.cluster) : (int)(2 * sms);
+    c.groups = (int)(2 * sms) / c.tiles;
+    c.row_cap = rows < kRows ? (rows + 31) / 32 * 32 : kRows;
+    return c;
 }
-size_t head_bytes(int groups) { return (size_t)groups * sizeof(Part); }
+size_t count_words(int groups, int tiles) { return (size_t)kLevels * 2 * groups * tiles * kSoftmaxWarps; }
 
 }  // namespace
 }  // namespace gptrs
@@ -750,10 +912,10 @@ extern "C" {
 size_t gptrs_cuda_tree_scratch_bytes(const gptrs_draft_trees* t) {
     DraftTrees checked;
     if (draft_trees(t, &checked) != GPTRS_OK) return 0;
-    int groups, tiles, row_cap, tile_nodes;
-    cut(t, &groups, &tiles, &row_cap, &tile_nodes);
-    const size_t slots = 2 * (size_t)groups * tiles;
-    return head_bytes(groups) + slots * row_cap * (sizeof(float2) + 32 * sizeof(float4));
+    const Cut c = cut(t);
+    if (c.small) return 0;
+    const size_t slots = 2 * (size_t)c.groups * c.tiles;
+    return 2 * count_words(c.groups, c.tiles) * sizeof(uint32_t) + slots * c.row_cap * (sizeof(float2) + 32 * sizeof(float4));
 }
 
 int gptrs_cuda_tree_attention(const gptrs_draft_trees* t, const gptrs_tree_attention_step* s, void* stream) {
@@ -766,12 +928,19 @@ int gptrs_cuda_tree_attention(const gptrs_draft_trees* t, const gptrs_tree_atten
     p.ldq = s->ldq ? s->ldq : width;
     GPTRS_REQUIRE(p.ldq >= width && p.ldq % 8 == 0 && p.ldq < ((int64_t)1 << 31), "rows of queries overlap, or do not start at multiples of 16 bytes");
     GPTRS_REQUIRE(t->n_pages * t->kv_heads * 2 * kTreePage < ((int64_t)1 << 31), "the pool has too many pages");
-    GPTRS_REQUIRE(t->max_pages * kTreePage / kKeys + 1 < (((int64_t)1 << 31) / ceil_div(t->max_nodes, kRows / (t->q_heads / t->kv_heads)) / t->kv_heads), "the page table is too long for so many rows");
-    GPTRS_REQUIRE(s->d_scratch && s->scratch_bytes >= gptrs_cuda_tree_scratch_bytes(t), "scratch is too small");
+    GPTRS_REQUIRE(t->max_pages * kTreePage / kKeys + 8 < (((int64_t)1 << 31) / ceil_div(t->max_nodes, kRows / (t->q_heads / t->kv_heads)) / t->kv_heads), "the page table is too long for so many rows");
+    const size_t scratch = gptrs_cuda_tree_scratch_bytes(t);
+    GPTRS_REQUIRE(scratch == 0 || (s->d_scratch && s->scratch_bytes >= scratch), "scratch is too small");
     if (t->rows == 0) return GPTRS_OK;
     const char *q = static_cast<const char*>(s->d_q), *out = static_cast<const char*>(s->d_out);
     GPTRS_REQUIRE(out >= q + 2 * ((t->rows - 1) * p.ldq + width) || q >= out + 2 * t->rows * width, "the output lies in rows of queries");
-    cut(t, &p.groups, &p.tiles, &p.row_cap, &p.tile_nodes);
+    static PerDeviceOnce attr_once;
+    if (attr_once.first_time()) {
+        GPTRS_CUDA_OK(cudaFuncSetAttribute(tree_attention_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
+        GPTRS_CUDA_OK(cudaFuncSetAttribute(tree_attention_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
+    }
+    const Cut c = cut(t);
+    p.cluster = c.cluster; p.groups = c.groups; p.tiles = c.tiles; p.row_cap = c.row_cap; p.tile_nodes = c.tile_nodes; p.most_tiles = c.most_tiles;
     int bad = encode_pool(s->d_pool, p.t, &p.map);
     if (!bad) bad = encode_queries(s->d_q, p.ldq, p.t, p.tile_nodes, &p.q_map);
     if (bad) return bad;
@@ -781,20 +950,13 @@ int gptrs_cuda_tree_attention(const gptrs_draft_trees* t, const gptrs_tree_atten
     p.status = s->d_status;
     p.scale_log2 = (t->scale != 0.f ? t->scale : 1.f / sqrtf((float)kTreeDim)) * kLog2e;
     const size_t slots = 2 * (size_t)p.groups * p.tiles;
-    p.begins = static_cast<Part*>(s->d_scratch);
-    p.sums = reinterpret_cast<float4*>(static_cast<char*>(s->d_scratch) + head_bytes(p.groups));
+    p.done = static_cast<uint32_t*>(s->d_scratch);
+    p.stored = p.done + count_words(p.groups, p.tiles);
+    p.sums = reinterpret_cast<float4*>(p.stored + count_words(p.groups, p.tiles));
     p.ml = reinterpret_cast<float2*>(p.sums + slots * 32 * p.row_cap);
     prefill_tc_fault(&p.starve, &p.wait_limit);
-    static PerDeviceOnce attr_once;
-    if (attr_once.first_time()) GPTRS_CUDA_OK(cudaFuncSetAttribute(tree_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
-    const int failed = launch_kernel(tree_attention_kernel, dim3((unsigned)(p.groups * p.tiles)), dim3(kThreads), kSmem, as_stream(stream), 1, p);
-    if (failed) return failed;
-    // the second kernel waits for the first one itself (griddepcontrol.wait), so it may be launched ahead of its end
-    const int pdl = g_use_pdl;
-    g_use_pdl = 1;
-    const int joined = launch_kernel(tree_join_kernel, dim3((unsigned)(8 * sm_count())), dim3(kJoinThreads), 0, as_stream(stream), 1, p);
-    g_use_pdl = pdl;
-    return joined;
+    if (c.small) return launch_kernel(tree_attention_kernel<true>, dim3((unsigned)c.ctas), dim3(kThreads), kSmem, as_stream(stream), 1, p, c.cluster);
+    return launch_kernel(tree_attention_kernel<false>, dim3((unsigned)c.ctas), dim3(kThreads), kSmem, as_stream(stream), 1, p);
 }
 
 }  // extern "C"

@@ -979,7 +979,7 @@ class TreeAttention(_Step):
         self.out = torch.empty((rows, t.q_heads * t.dim), dtype=torch.bfloat16, device=q.device) if out is None else _need(out, "out", torch.bfloat16, rows, t.q_heads * t.dim)
         self.status = _status(q.device, status)
         s.scratch_bytes = lib().gptrs_cuda_tree_scratch_bytes(ctypes.byref(t))
-        scratch = torch.empty(s.scratch_bytes, dtype=torch.uint8, device=q.device) if s.scratch_bytes else None
+        scratch = torch.zeros(s.scratch_bytes, dtype=torch.uint8, device=q.device) if s.scratch_bytes else None
         s.d_q, s.ldq = q.data_ptr(), q.stride(0) if rows > 1 else t.q_heads * t.dim
         s.d_pool, s.d_out, s.d_scratch, s.d_status = pool.data_ptr(), self.out.data_ptr(), None if scratch is None else scratch.data_ptr(), self.status.data_ptr()
         self._hold(q=q, pool=pool, out=self.out, scratch=scratch, status=self.status, **trees.tensors)

@@ -850,8 +850,9 @@ typedef struct {
 } gptrs_tree_append_step;
 int gptrs_cuda_tree_append(const gptrs_draft_trees* t, const gptrs_tree_append_step* s, void* stream);
 /* out [rows][q_heads][dim] (bf16) = softmax over what the node sees . values. A node that sees nothing (its pages are out of range) gives zeros. Keys and values of nodes
- * that a node does not see do not touch it, whatever they are. Scratch: gptrs_cuda_tree_scratch_bytes, 16-byte aligned, of one call at a time: calls and graphs
- * that may overlap have their own. */
+ * that a node does not see do not touch it, whatever they are. Scratch: gptrs_cuda_tree_scratch_bytes, 16-byte aligned, all zero before its first
+ * call and after one that left 3 in *d_status (calls with other numbers of heads or nodes have their own, or zero it), of one call at a time: calls and graphs that may overlap
+ * have their own. */
 typedef struct {
     const void* d_q;                   /* [rows][q_heads][dim], rows ldq apart (0 = packed) */
     int64_t ldq;
