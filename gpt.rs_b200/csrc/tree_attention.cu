@@ -14,8 +14,8 @@
 // Work, where contexts may be long: an item is a (tree, kv head, row tile or pair of them), a unit a block of an item, and an item has some more that stand for what it costs
 // beside its keys; every group of CTAs (one, or two for trees of more rows than a tile has, which then share the keys through L2) takes the same number of consecutive
 // units, whatever the trees' lengths. Where an item is cut, its parts are counted in warp by warp (a warp has the same rows in all of them): the last warp to finish waits until
-// the others' sums are in scratch and joins them with its own, four at a time, in the order of the keys, and such joins are joined again. So the result depends on the call
-// alone, not on who was last. Where contexts are short (kSmall) a cluster of up to eight CTAs takes a (tree, kv head, row tile), a share of its keys each, and joins through
+// the others' sums are in scratch and joins them with its own, four at a time, in the order of the keys, and such joins are joined again. Few items have many parts each: those a
+// second kernel joins. So the result depends on the call alone, not on who was last. Where contexts are short (kSmall) a cluster of up to eight CTAs takes a (tree, kv head, row tile), a share of its keys each, and joins through
 // distributed shared memory: nothing has to be added up or looked for in front.
 // Every wait is bounded: on a timeout code 3 goes to the status word, the roles leave their loops, tensor memory is freed.
 #include "draft_tree.cuh"
@@ -48,6 +48,9 @@ constexpr int kJoin = 4;                        // parts that are joined at a ti
 constexpr int kLevels = 5;                      // 4^5 groups
 constexpr int kReaders = kSoftmaxWarps + 3;     // of a piece of work: the softmax's warps, the products' thread, the two that load
 
+// An item that a CTA has the first part of, for the kernel that joins parts (0 or 1 of them: none).
+struct Item { int parts, row0, nodes, head, tile, pad[3]; };
+
 struct AttentionParams {
     CUtensorMap map, q_map;
     DraftTrees t;
@@ -55,6 +58,7 @@ struct AttentionParams {
     long long ldq;
     const unsigned char* pool;
     __nv_bfloat16* out;
+    Item* items;                 // [groups tiles], where a second kernel joins the parts; NULL: the warps do
     uint32_t *done, *stored;     // [levels][2 groups tiles][4]: parts of a join that are worked out, and in scratch, by warp; 0 again when it is made
     float2* ml;                  // [2 groups tiles][row_cap]: reference and sum of a row; the first of a CTA's two slots is for items that others began
     float4* sums;                // [2 groups tiles][32][row_cap]
@@ -198,14 +202,28 @@ __device__ __forceinline__ float4 load_now(const float4* at) {
     asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(at) : "memory");
     return v;
 }
+__device__ __forceinline__ void store_part(const AttentionParams& p, size_t slot, bool live, uint32_t t_o, float m, float l) {
+    float4* to = p.sums + slot * 32 * p.row_cap + threadIdx.x;
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        float o[32];
+        __syncwarp();
+        tmem_ld_32(t_o + 32u * c, o);
+        if (!live) continue;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) to[(8 * c + i) * p.row_cap] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+    }
+    if (live) p.ml[slot * p.row_cap + threadIdx.x] = make_float2(m, l);
+}
 // A warp's part of an item: to scratch, unless this warp is the last of its join's four; then it joins them, to the first one's place or, all of the item, to the output. Returns
 // false if a wait ran out.
 __device__ __forceinline__ bool join_parts(const AttentionParams& p, const Piece& piece, bool live, uint32_t t_o, float m, float l, uint4* dst) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, from = blockIdx.x / p.tiles - piece.part;
     const size_t slots = 2 * (size_t)p.groups * p.tiles;
     auto slot = [&](int part) { return 2 * ((size_t)(from + part) * p.tiles + blockIdx.x % p.tiles) + (part == 0 ? 1 : 0); };
-    int n = piece.parts, at = piece.part, apart = 1;   // parts of this level, this one's number, how far they lie apart
+    int n = p.items ? 1 : piece.parts, at = piece.part, apart = 1;   // parts of this level, this one's number, how far they lie apart
     bool mine = true;                                  // the sums are in tensor memory; else in scratch
+    if (p.items) store_part(p, slot(at), live, t_o, m, l);
     for (int level = 0; n > 1; ++level) {
         const int first = at / kJoin * kJoin, members = min(kJoin, n - first), me = mine ? at - first : kJoin;
         const size_t count = ((size_t)level * slots + slot(first * apart)) * kSoftmaxWarps + warp;
@@ -216,17 +234,7 @@ __device__ __forceinline__ bool join_parts(const AttentionParams& p, const Piece
         }
         const bool last = before == members - 1;
         if (mine && (!last || members == 1)) {
-            float4* to = p.sums + slot(at) * 32 * p.row_cap + tid;
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-                float o[32];
-                __syncwarp();
-                tmem_ld_32(t_o + 32u * c, o);
-                if (!live) continue;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) to[(8 * c + i) * p.row_cap] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-            }
-            if (live) p.ml[slot(at) * p.row_cap + tid] = make_float2(m, l);
+            store_part(p, slot(at), live, t_o, m, l);
             mine = false;
         }
         if (members > 1) {
@@ -434,9 +442,13 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
             return !failed;
         };
         int asked = 0;
+        Item told = {};
         for (int i = 0; !idles; ++i) {
             bool more = kSmall && i == 0 && only.kb1 > only.kb0;
-            if constexpr (!kSmall) more = walk.next();
+            if constexpr (!kSmall) {
+                more = walk.next();
+                if (more && walk.piece.part == 0) told = {walk.piece.parts, walk.piece.span.row0, walk.piece.span.nodes, walk.piece.head, walk.piece.tile};   // (only the last one can have more)
+            }
             if (i >= 2 && !wait(&piece_empty[i & 1], (uint32_t)((i >> 1) - 1))) break;
             if (!kSmall && lane == 0) {
                 s_piece[i & 1] = walk.piece;
@@ -479,6 +491,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
                 ask();
             }
         }
+        if (!kSmall && p.items && lane == 0) p.items[blockIdx.x] = told;
         if (asked) mbar_wait_parked(smem_u32(&q_full), (uint32_t)(asked - 1) & 1u, p.wait_limit);   // (queries in flight write this CTA's shared memory)
         if (failed && lane == 0) atomicExch(p.status, 3);
     } else if (warp > kMmaWarp) {
@@ -851,6 +864,76 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
+// Joins the parts of items. A piece of work is (item, 32 rows, 32 channels), dealt out in turn: every CTA lists the items for itself.
+constexpr int kJoinThreads = 256, kMostItems = 512;
+__global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_constant__ AttentionParams p) {
+    __shared__ __align__(16) __nv_bfloat16 s_out[32][32 + 8];
+    __shared__ int s_cta[kMostItems], s_count[kMostItems / 32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int per = p.row_cap / 32 * 4, ctas = p.groups * p.tiles, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t has[kMostItems / kJoinThreads];
+#pragma unroll
+    for (int i = 0; i < kMostItems / kJoinThreads; ++i) {
+        const int cta = i * kJoinThreads + threadIdx.x;
+        has[i] = __ballot_sync(0xffffffffu, cta < ctas && p.items[cta].parts > 1);
+        if (lane == 0) s_count[i * (kJoinThreads / 32) + warp] = __popc(has[i]);
+    }
+    __syncthreads();
+    int items = 0;
+#pragma unroll
+    for (int i = 0; i < kMostItems / 32; ++i) {
+        if (i % (kJoinThreads / 32) == warp && (has[i / (kJoinThreads / 32)] >> lane & 1)) s_cta[items + __popc(has[i / (kJoinThreads / 32)] & ((1u << lane) - 1u))] = i * 32 + lane;
+        items += s_count[i];
+    }
+    __syncthreads();
+    for (int w = blockIdx.x; w < items * per; w += gridDim.x) {
+        const int cta = s_cta[w / per], quarter = w & 3, row = w % per / 4 * 32 + lane;
+        const Item item = p.items[cta];
+        const int rows = min(p.tile_nodes, item.nodes - item.tile * p.tile_nodes) * p.t.group;
+        if (row - lane >= rows) continue;   // the whole CTA
+        float top = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr int kAtOnce = 16;   // (with four at a time the loads' latencies of 18 parts added up to 15 us)
+        for (int k0 = 0; k0 < item.parts && row < rows; k0 += kAtOnce) {
+            float2 ml[kAtOnce];
+            float4 v[kAtOnce];
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                const int part = min(k0 + k, item.parts - 1);
+                const size_t slot = 2 * ((size_t)cta + (size_t)part * p.tiles) + (part == 0 ? 1 : 0);
+                v[k] = load_now(p.sums + (slot * 32 + 8 * quarter + warp) * p.row_cap + row);
+                ml[k] = p.ml[slot * p.row_cap + row];
+            }
+            float to = top;
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                if (k0 + k >= item.parts) ml[k] = make_float2(-INFINITY, 0.f);
+                to = fmaxf(to, ml[k].x);
+            }
+            const float ref = to == -INFINITY ? 0.f : to, keep = ex2(top - ref);   // (top -inf: nothing yet, 0)
+            top = to;
+            l = l == 0.f ? 0.f : l * keep;
+            o.x *= keep; o.y *= keep; o.z *= keep; o.w *= keep;
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                if (k0 + k >= item.parts) break;
+                const float f = ex2(ml[k].x - ref);
+                l += ml[k].x == -INFINITY ? ml[k].y : ml[k].y * f;   // (without a score 0, or NaN)
+                o.x += v[k].x * f; o.y += v[k].y * f; o.z += v[k].z * f; o.w += v[k].w * f;
+            }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        *reinterpret_cast<uint2*>(&s_out[lane][4 * warp]) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+        __syncthreads();
+        const int r = threadIdx.x >> 2, rr = row - lane + r, chunk = 8 * (threadIdx.x & 3);
+        if (r < 32 && rr < rows)
+            *reinterpret_cast<uint4*>(p.out + ((long long)(item.row0 + item.tile * p.tile_nodes + rr / p.t.group) * p.t.q_heads + item.head * p.t.group + rr % p.t.group) * kTreeDim +
+                                      32 * quarter + chunk) = *reinterpret_cast<const uint4*>(&s_out[r][chunk]);
+        __syncthreads();
+    }
+}
+
 // The pool as rows of a token and head of 256 bytes (z), two halves (y) of 64 channels (x); a block (page, kv head, keys or values) begins at row
 // ((page x kv heads + head) x 2 + is value) x 16. The kernel asks for pages below n_pages alone.
 int encode_pool(const void* pool, const DraftTrees& t, CUtensorMap* map) {
@@ -885,7 +968,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 // How a call is cut. The host does not know the lengths, but the page table's width bounds them. Small: a cluster per (tree, kv head, row tile), with as many CTAs (8, 4, 2, 1) as
 // leave a processor, or half of one, to each; taken where the longest context can cost no more than equal shares of all of them and their joins, which take as long as
 // twenty blocks. Others: as many CTAs as there are places, in groups of one, or of two where trees may have more rows than a tile.
-struct Cut { int cluster, ctas, groups, tiles, row_cap, tile_nodes, most_tiles; bool small; };
+struct Cut { int cluster, ctas, groups, tiles, row_cap, tile_nodes, most_tiles; bool small, joined_after; };
 Cut cut(const gptrs_draft_trees* t) {
     Cut c;
     const int group = t->q_heads / t->kv_heads, rows = t->max_nodes * group;
@@ -895,8 +978,10 @@ Cut cut(const gptrs_draft_trees* t) {
     c.cluster = tasks * 8 <= sms ? 8 : tasks * 4 <= sms ? 4 : tasks * 2 <= 2 * sms ? 2 : 1;
     c.small = tasks * c.cluster <= 2 * sms ? longest / c.cluster <= tasks * longest / (2 * sms) + 20 : tasks < (1 << 24) && longest <= 20;
     c.tiles = !c.small && c.most_tiles > 1 ? 2 : 1;
-    c.ctas = c.small ? (int)(tasks * c.cluster) : (int)(2 * sms);
-    c.groups = (int)(2 * sms) / c.tiles;
+    c.ctas = c.small ? (int)(tasks * c.cluster) : (int)(2 * sms < kMostItems ? 2 * sms : kMostItems);
+    // a level of joins by warps takes 6 to 8 us at the end of a call, the second kernel 7 us, but while others still work on their keys the former cost nothing
+    c.joined_after = !c.small && t->n_trees * t->kv_heads * ceil_div(c.most_tiles, c.tiles) * 4 <= 2 * sms / c.tiles;
+    c.groups = (int)(2 * sms < kMostItems ? 2 * sms : kMostItems) / c.tiles;
     c.row_cap = rows < kRows ? (rows + 31) / 32 * 32 : kRows;
     return c;
 }
@@ -951,12 +1036,20 @@ int gptrs_cuda_tree_attention(const gptrs_draft_trees* t, const gptrs_tree_atten
     p.scale_log2 = (t->scale != 0.f ? t->scale : 1.f / sqrtf((float)kTreeDim)) * kLog2e;
     const size_t slots = 2 * (size_t)p.groups * p.tiles;
     p.done = static_cast<uint32_t*>(s->d_scratch);
+    if (c.joined_after) p.items = reinterpret_cast<Item*>(p.done);   // (the counts are not used then; they take more room)
     p.stored = p.done + count_words(p.groups, p.tiles);
     p.sums = reinterpret_cast<float4*>(p.stored + count_words(p.groups, p.tiles));
     p.ml = reinterpret_cast<float2*>(p.sums + slots * 32 * p.row_cap);
     prefill_tc_fault(&p.starve, &p.wait_limit);
     if (c.small) return launch_kernel(tree_attention_kernel<true>, dim3((unsigned)c.ctas), dim3(kThreads), kSmem, as_stream(stream), 1, p, c.cluster);
-    return launch_kernel(tree_attention_kernel<false>, dim3((unsigned)c.ctas), dim3(kThreads), kSmem, as_stream(stream), 1, p);
+    bad = launch_kernel(tree_attention_kernel<false>, dim3((unsigned)c.ctas), dim3(kThreads), kSmem, as_stream(stream), 1, p);
+    if (bad || !c.joined_after) return bad;
+    // the second kernel waits for the first one itself (griddepcontrol.wait), so it may be launched ahead of its end
+    const int pdl = g_use_pdl;
+    g_use_pdl = 1;
+    bad = launch_kernel(tree_join_kernel, dim3((unsigned)(2 * sm_count())), dim3(kJoinThreads), 0, as_stream(stream), 1, p);
+    g_use_pdl = pdl;
+    return bad;
 }
 
 }  // extern "C"
