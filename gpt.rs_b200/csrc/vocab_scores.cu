@@ -246,14 +246,15 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                     failed = __any_sync(0xffffffffu, failed);
                     if (failed) break;
                     tc_fence_after();
-                    if (holds) {
+                    if (holds && 128 * half < p.cols) {
                         uint32_t v[2][32];   // a quarter on its way while the one in front is added
                         const uint32_t at = tmem + (uint32_t)(buf * kCols + 128 * half);
                         tmem_ld_32_begin(at, v[0]);
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
+                            if (128 * half + 32 * c >= p.cols) break;
                             tmem_ld_32_end(v[c & 1]);
-                            if (c < 3) tmem_ld_32_begin(at + 32u * (c + 1), v[(c + 1) & 1]);
+                            if (c < 3 && 128 * half + 32 * (c + 1) < p.cols) tmem_ld_32_begin(at + 32u * (c + 1), v[(c + 1) & 1]);
 #pragma unroll
                             for (int i = 0; i < 16; ++i)
                                 acc[16 * c + i] = add2(acc[16 * c + i], pair_of(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])));
