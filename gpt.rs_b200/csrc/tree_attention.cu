@@ -352,23 +352,27 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
 
     // ---- this CTA's work
     const int per = (p.t.n_trees + kRows - 1) / kRows;
-    const int rank = kSmall && p.cluster > 1 ? blockIdx.x % p.cluster : 0, group = blockIdx.x / p.tiles, tile_of_group = blockIdx.x % p.tiles;
+    const int rank = kSmall && p.cluster > 1 ? (int)cluster_ctarank() : 0, group = blockIdx.x / p.tiles, tile_of_group = blockIdx.x % p.tiles;
     TreeSpan last = {-1, 0, 0, 0};
     Piece only = {};                                    // a small call's
+    int first_page = -2;
     int groups = 1;
     long long units = 0, begin = 0, end = 0, mine = 0, upto = 0;
     bool idles = false;
     if constexpr (kSmall) {
-        const int task = blockIdx.x / p.cluster, s = task / (p.t.kv_heads * p.most_tiles), in_tree = task - s * (p.t.kv_heads * p.most_tiles);
-        only.span = tree_span(p.t, s, p.status);
-        only.head = in_tree / p.most_tiles;
-        only.tile = in_tree - only.head * p.most_tiles;
+        only.span = tree_span(p.t, blockIdx.z, p.status);
+        only.head = blockIdx.y;
+        only.tile = blockIdx.x >> (31 - __clz(p.cluster));
         only.parts = 1;
         idles = only.tile * p.tile_nodes >= only.span.nodes;
         if (!idles) {
             const int blocks = blocks_of(only.span);
-            only.kb0 = blocks * rank / p.cluster;
-            only.kb1 = blocks * (rank + 1) / p.cluster;
+            only.kb0 = (int)((uint32_t)blocks * (uint32_t)rank >> (31 - __clz(p.cluster)));
+            only.kb1 = (int)((uint32_t)blocks * (uint32_t)(rank + 1) >> (31 - __clz(p.cluster)));
+            // the first block's pages, which the loads of keys and values wait for
+            const int page = only.kb0 * kPages + lane;
+            if (warp > kMmaWarp && lane < kPages && only.kb0 < only.kb1 && page <= (only.span.length + only.span.nodes - 1) / kTreePage)
+                first_page = p.t.table[(long long)only.span.slot * p.t.max_pages + page];
         }
     } else if (warp < kSoftmaxWarps) {   // warps 0 - 3 add up the trees' units
         for (int s = tid * per; s < min((tid + 1) * per, p.t.n_trees); ++s) {
@@ -508,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
             const int last_page = (piece.span.length + piece.span.nodes - 1) / kTreePage;
             const int* table = p.t.table + (long long)piece.span.slot * p.t.max_pages;
             auto page_of = [&](int kb) { return lane < kPages && kb < piece.kb1 && kb * kPages + lane <= last_page ? table[kb * kPages + lane] : -2; };
-            int coming = page_of(piece.kb0);
+            int coming = kSmall ? first_page : page_of(piece.kb0);
             for (int kb = piece.kb0; kb < piece.kb1; ++kb, ++g) {
                 const int page = coming;
                 coming = page_of(kb + 1);
@@ -784,18 +788,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
                     asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
                 }
                 uint4* dst = reinterpret_cast<uint4*>(p.out + ((long long)(span.row0 + node) * p.t.q_heads + piece.head * p.t.group + my_head) * kTreeDim);
-                if (kSmall && p.cluster > 1) {                  // the share's sums to shared memory, where the stages and the queries were
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        float o[32];
-                        __syncwarp();
-                        tmem_ld_32(t_o + 32u * c, o);
-                        if (!live) continue;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            st_shared_v4(sQ + (tid * kORow + 32 * c + 4 * i) * 4, __float_as_uint(o[4 * i]), __float_as_uint(o[4 * i + 1]), __float_as_uint(o[4 * i + 2]), __float_as_uint(o[4 * i + 3]));
-                    }
-                    if (kSmall && live) s_ml[tid] = make_float2(m, l);
+                if (kSmall && p.cluster > 1) {                  // (the share's sums go to the other CTAs, see below)
+                    if (live) s_ml[kSmall ? tid : 0] = make_float2(m, l);
                 } else if (piece.parts == 1) {
                     const float inv = any ? 1.f / l : 0.f;
 #pragma unroll 1
@@ -825,10 +819,28 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
     __syncwarp();
     tc_fence_before();
     if (kSmall && p.cluster > 1) {
-        // ---- the shares of the cluster's task, in the order of the keys: a CTA takes every cluster-th row, a warp a row at a time, four channels a lane
-        cluster_sync_all();
+        // ---- the share's sums to shared memory, where the stages and the queries were: two warps for 32 rows, half of the channels each
         const TreeSpan& span = only.span;
         const int node0 = only.tile * p.tile_nodes, rows = idles ? 0 : min(p.tile_nodes, span.nodes - node0) * p.t.group;
+        __syncthreads();
+        tc_fence_after();
+        if (only.kb1 > only.kb0 && (warp & 3) * 32 < rows) {
+            const int row = (warp & 3) * 32 + lane, c0 = (warp >> 2) * (kTreeDim / 2);
+#pragma unroll 1
+            for (int c = c0; c < c0 + kTreeDim / 2; c += 32) {
+                float o[32];
+                __syncwarp();
+                tmem_ld_32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + kOCol + (uint32_t)c, o);
+                if (row >= rows) continue;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    st_shared_v4(sQ + (row * kORow + c + 4 * i) * 4, __float_as_uint(o[4 * i]), __float_as_uint(o[4 * i + 1]), __float_as_uint(o[4 * i + 2]), __float_as_uint(o[4 * i + 3]));
+            }
+            __syncwarp();
+        }
+        tc_fence_before();
+        // ---- the shares of the cluster's task, in the order of the keys: a CTA takes every cluster-th row, a warp a row at a time, four channels a lane
+        cluster_sync_all();
         const uint32_t ml_at = smem_u32(s_ml);
         for (int row = rank + p.cluster * warp; row < rows; row += p.cluster * (kThreads / 32)) {
             float2 ml[8];
@@ -978,7 +990,7 @@ Cut cut(const gptrs_draft_trees* t) {
     c.cluster = tasks * 8 <= sms ? 8 : tasks * 4 <= sms ? 4 : tasks * 2 <= 2 * sms ? 2 : 1;
     c.small = tasks * c.cluster <= 2 * sms ? longest / c.cluster <= tasks * longest / (2 * sms) + 20 : tasks < (1 << 24) && longest <= 20;
     c.tiles = !c.small && c.most_tiles > 1 ? 2 : 1;
-    c.ctas = c.small ? (int)(tasks * c.cluster) : (int)(2 * sms < kMostItems ? 2 * sms : kMostItems);
+    c.ctas = c.small ? c.most_tiles * c.cluster : (int)(2 * sms < kMostItems ? 2 * sms : kMostItems);
     // a level of joins by warps takes 6 to 8 us at the end of a call, the second kernel 7 us, but while others still work on their keys the former cost nothing
     c.joined_after = !c.small && t->n_trees * t->kv_heads * ceil_div(c.most_tiles, c.tiles) * 4 <= 2 * sms / c.tiles;
     c.groups = (int)(2 * sms < kMostItems ? 2 * sms : kMostItems) / c.tiles;
@@ -1041,7 +1053,7 @@ int gptrs_cuda_tree_attention(const gptrs_draft_trees* t, const gptrs_tree_atten
     p.sums = reinterpret_cast<float4*>(p.stored + count_words(p.groups, p.tiles));
     p.ml = reinterpret_cast<float2*>(p.sums + slots * 32 * p.row_cap);
     prefill_tc_fault(&p.starve, &p.wait_limit);
-    if (c.small) return launch_kernel(tree_attention_kernel<true>, dim3((unsigned)c.ctas), dim3(kThreads), kSmem, as_stream(stream), 1, p, c.cluster);
+    if (c.small) return launch_kernel(tree_attention_kernel<true>, dim3((unsigned)c.ctas, (unsigned)t->kv_heads, (unsigned)t->n_trees), dim3(kThreads), kSmem, as_stream(stream), 1, p, c.cluster);
     bad = launch_kernel(tree_attention_kernel<false>, dim3((unsigned)c.ctas), dim3(kThreads), kSmem, as_stream(stream), 1, p);
     if (bad || !c.joined_after) return bad;
     // the second kernel waits for the first one itself (griddepcontrol.wait), so it may be launched ahead of its end
