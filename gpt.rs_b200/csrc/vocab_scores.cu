@@ -13,6 +13,8 @@
 // Units go row tile first, so that the CTAs that run at one time share stretches of w through L2. A second kernel joins the parts of a row; it compares tokens where
 // values are equal, so results do not depend on an order.
 // Every wait is bounded: on a timeout code 3 goes to the status word, the roles leave their loops, tensor memory is freed.
+#include <algorithm>
+
 #include "umma_common.cuh"
 
 namespace gptrs {
@@ -468,18 +470,17 @@ __global__ void __launch_bounds__(kJoinThreads) vocab_join_kernel(const __grid_c
     }
 }
 
-// How a call is cut. Stretches of equal numbers of equal tiles, and as many of them as leave the fewest tokens to the CTA (or pair) that has most; a tile's own cost counts as 8
-// tokens, a unit's as 32.
+// How a call is cut: stretches of equal numbers of equal tiles, so many that units (row tiles x stretches) fill the SMs (or pairs of them) once, twice, up to eight times: whichever
+// leaves the fewest tokens to the one that has most, a tile's own cost counted as 8 tokens and a unit's as 32.
 struct Cut { int mode, row_tiles, stretches, tiles, cols; };
 Cut cut(int64_t rows, int64_t vocab) {
     const int mode = rows <= 16 ? kFew : rows <= kRows ? kOne : kPairs;
     const bool pair = mode == kPairs;
-    const int places = pair ? sm_count() / 2 : sm_count(), grain = pair ? 32 : 16, row_tiles = ceil_div(rows, pair ? 2 * kRows : kRows);
-    const int most = (int)(ceil_div(vocab, grain) < 8 * places ? ceil_div(vocab, grain) : 8 * places);
+    const int places = pair ? sm_count() / 2 : sm_count(), grain = pair ? 32 : 16, row_tiles = ceil_div(rows, pair ? 2 * kRows : kRows), grains = ceil_div(vocab, grain);
     Cut c = {mode, row_tiles, 1, 1, grain};
     int64_t best = -1;
-    for (int n = 1; n <= most; ++n) {
-        if (n > 1 && (int64_t)row_tiles * n > 8 * places) break;   // (rows alone fill every place many times)
+    for (int waves = 1; waves <= 8; ++waves) {
+        const int n = std::max(1, std::min(grains, places * waves / row_tiles));
         const int tiles = ceil_div(vocab, (int64_t)n * kCols), cols = (ceil_div(vocab, (int64_t)n * tiles) + grain - 1) / grain * grain;
         const int stretches = ceil_div(vocab, (int64_t)tiles * cols);
         const int64_t cost = (int64_t)ceil_div((int64_t)row_tiles * stretches, places) * (tiles * (cols + 8) + 32);
