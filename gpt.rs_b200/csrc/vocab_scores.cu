@@ -28,18 +28,18 @@ constexpr int kStageDim = 64;                   // bf16 of a 128-byte swizzle sp
 // How a call's rows are worked on: up to 16 of them, up to 128, more (by pairs of CTAs).
 enum { kFew, kOne, kPairs };
 constexpr int kCols = 256;                      // most tokens of a tile
-constexpr int stages_of(int mode) { return mode == kFew ? 5 : mode == kOne ? 4 : 6; }
+constexpr int kMostStages = 16;                 // (as many as fit: narrow tiles have small stages, and need more of them under way)
 constexpr int x_bytes(int mode) { return 128 * (mode == kFew ? 64 : 128); }        // of a stage; products of 64 rows where there are 16 at most
 // Stages that an accumulator adds up. 128 of dim where w's bytes bound the call, 512 where the products do and each handing over takes time from them: relative errors of lse
 // at a dim of 4096 1.0e-7 and 4.0e-7 (f32 sums one by one 5.8e-7), of 4001 rows in 131072 tokens 1.72 ms with 256, 1.54 with 512.
-constexpr int drain_of(int mode) { return mode == kPairs ? 8 : 2; }
+constexpr int drain_of(int mode) { return mode == kPairs ? 8 : mode == kFew ? 4 : 2; }
 constexpr int kEpilogue = 256, kThreads = kEpilogue + 128;   // two warps of the last four only make their group whole
 // Registers of a thread at launch, and what the groups of four warps make of them: the shares add up to less than the block has, so every request ends.
 constexpr int kLaunchRegs = 168, kEpilogueRegs = 208, kOtherRegs = 80;
 static_assert(2 * kEpilogueRegs + kOtherRegs <= 3 * kLaunchRegs, "more registers than the block is launched with");
 constexpr int kZRow = kCols + 4;                // floats of a row of logits in shared memory (kFew)
-constexpr int stage_bytes(int mode) { return x_bytes(mode) + 128 * (mode == kPairs ? kCols / 2 : kCols); }
-constexpr size_t smem_bytes(int mode) { return (size_t)stages_of(mode) * stage_bytes(mode) + 1024; }
+constexpr int stage_bytes(int mode, int cols) { return x_bytes(mode) + 128 * (mode == kPairs ? cols / 2 : cols); }
+constexpr size_t kSmem = 200 * 1024 + 1024;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kJoinThreads = 256;
 
@@ -56,7 +56,7 @@ struct ScoreParams {
     int rows, dim, vocab;
     int row_tiles, stretches, tiles, cols;   // a stretch is `tiles` tiles of `cols` tokens
     int x_rows;                   // of a copy of x
-    int row_parts;
+    int row_parts, stages;
     float cap, inv_t;             // inv_t 0: greedy
     uint32_t seed, wait_limit;
     int starve;
@@ -81,8 +81,8 @@ __device__ __forceinline__ float gumbel(uint32_t h) { return -logf(-log1pf(-(((f
 __device__ __noinline__ float capped(float z, float cap) { return cap * tanhf(z / cap); }
 __device__ __forceinline__ void join(Part& a, const Part& b) {
     const float m = fmaxf(a.m, b.m);
-    if (m != -INFINITY) a.l = a.l * (a.m == m ? 1.f : expf(a.m - m)) + b.l * (b.m == m ? 1.f : expf(b.m - m));
-    else a.l += b.l;   // (a sum that is NaN stays one)
+    const float ref = m == -INFINITY ? 0.f : m;   // (a sum that is NaN stays one)
+    a.l = a.l * (a.m == m ? 1.f : ex2((a.m - ref) * kLog2e)) + b.l * (b.m == m ? 1.f : ex2((b.m - ref) * kLog2e));
     a.m = m;
     if (b.token >= 0 && (a.token < 0 || b.best > a.best || (b.best == a.best && b.token < a.token))) { a.best = b.best; a.z = b.z; a.token = b.token; }
     if (b.given == b.given) a.given = b.given;
@@ -126,18 +126,18 @@ __device__ __forceinline__ Part join_lanes(Part a) {
 template <int kMode, bool kSample>
 __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_constant__ ScoreParams p) {
     constexpr bool kPair = kMode == kPairs;
-    constexpr int kStages = stages_of(kMode), kStageBytes = stage_bytes(kMode), kDrain = drain_of(kMode), kABytes = x_bytes(kMode), kCtas = kPair ? 2 : 1;
+    constexpr int kDrain = drain_of(kMode), kABytes = x_bytes(kMode), kCtas = kPair ? 2 : 1;
     constexpr uint32_t kTmemCols = 2 * kCols;
     constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)((kMode == kFew ? 64 : kCtas * kRows) >> 4) << 24);   // f32 accumulator, bf16 operands
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
+    __shared__ __align__(8) uint64_t full[kMostStages], empty[kMostStages], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_holder;
     __shared__ __align__(16) float s_z[kMode == kFew ? 16 : 1][kZRow];
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = kPair ? (int)cluster_ctarank() : 0;   // the first CTA's thread issues the products of both
     if (tid == 0) {
-        for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < kMostStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], kCtas * kEpilogue / 32); }
         mbar_fence_init();
     }
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
     const uint32_t tmem = tmem_holder;
     pdl_launch_dependents();
     pdl_wait();
-    const int steps = (p.dim + kStageDim - 1) / kStageDim, units = p.row_tiles * p.stretches, my_cols = p.cols / kCtas;
+    const int steps = (p.dim + kStageDim - 1) / kStageDim, units = p.row_tiles * p.stretches, my_cols = p.cols / kCtas, stages = p.stages, stage_size = stage_bytes(kMode, p.cols);
     struct Unit { int row0, begin, end; };
     auto unit_of = [&](int u) {
         const int begin = u / p.row_tiles * (p.tiles * p.cols);
@@ -177,18 +177,18 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                 const Unit unit = unit_of(u);
                 for (int n0 = unit.begin; n0 < unit.end && !failed; n0 += p.cols) {
                     for (int k = 0; k < steps; ++k, ++it) {
-                        if (it >= kStages && !mbar_wait_polled(&empty[s], phase, p.wait_limit, 256)) { failed = true; break; }
-                        const uint32_t at = smem + s * kStageBytes, bar = kPair ? map_to_cta(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
+                        if (it >= stages && !mbar_wait_polled(&empty[s], phase, p.wait_limit, 256)) { failed = true; break; }
+                        const uint32_t at = smem + s * stage_size, bar = kPair ? map_to_cta(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
                         if (rank == 0) mbar_expect_tx(&full[s], bytes);
                         if (!(p.starve && it == 0)) load_2d<kPair>(at, &p.x_map, k * kStageDim, unit.row0, bar);
                         load_2d<kPair>(at + kABytes, &p.w_map, k * kStageDim, n0 + rank * my_cols, bar);
-                        if (++s == kStages) { s = 0; phase ^= 1u; }
+                        if (++s == stages) { s = 0; phase ^= 1u; }
                     }
                 }
             }
             // Stages in flight write the CTAs' shared memory (only after a timeout are there any left unread). Of a pair the first CTA waits for both: the other one stays until the end.
             if (rank == 0)
-                for (int i = max(it - kStages, 0); i < it; ++i) mbar_wait_parked(smem_u32(&full[i % kStages]), (uint32_t)(i / kStages) & 1u, p.wait_limit);
+                for (int i = max(it - stages, 0); i < it; ++i) mbar_wait_parked(smem_u32(&full[i % stages]), (uint32_t)(i / stages) & 1u, p.wait_limit);
             if (failed) atomicExch(p.status, 3);
         }
         __syncwarp();
@@ -208,11 +208,11 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                         for (int k = k0; k < k1; ++k) {
                             if (!mbar_wait_polled(&full[s], phase, p.wait_limit, 256)) { failed = true; break; }
                             tc_fence_after();
-                            const uint64_t a = make_smem_desc(smem + s * kStageBytes), b = make_smem_desc(smem + s * kStageBytes + kABytes);
+                            const uint64_t a = make_smem_desc(smem + s * stage_size), b = make_smem_desc(smem + s * stage_size + kABytes);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) multiply<kPair>(tmem + (uint32_t)(buf * kCols), a + 2 * i, b + 2 * i, idesc, (k > k0 || i > 0) ? 1u : 0u);
                             commit<kPair>(&empty[s]);
-                            if (++s == kStages) { s = 0; phase ^= 1u; }
+                            if (++s == stages) { s = 0; phase ^= 1u; }
                         }
                         if (!failed) commit<kPair>(&acc_full[buf]);
                     }
@@ -533,6 +533,7 @@ int gptrs_cuda_vocab_scores(const gptrs_vocab_scores* s, void* stream) {
     const Cut c = cut(s->rows, s->vocab);
     const bool pair = c.mode == kPairs;
     p.row_parts = c.mode == kFew ? c.stretches : 2 * c.stretches;
+    p.stages = (int)std::min<int64_t>(kMostStages, (int64_t)(kSmem - 1024) / stage_bytes(c.mode, c.cols));
     p.row_tiles = c.row_tiles; p.stretches = c.stretches; p.tiles = c.tiles; p.cols = c.cols;
     p.x_rows = s->rows < kRows ? (int)(s->rows + 7) / 8 * 8 : kRows;   // (rows that nobody has are not read out: whatever lies there)
     int rc = encode(&p.x_map, s->d_hidden, s->dim, s->rows, ldx, p.x_rows);
@@ -549,10 +550,10 @@ int gptrs_cuda_vocab_scores(const gptrs_vocab_scores* s, void* stream) {
                                         {vocab_scores_kernel<kPairs, false>, vocab_scores_kernel<kPairs, true>}};
     static PerDeviceOnce attr_once;
     if (attr_once.first_time())
-        for (int i = 0; i < 6; ++i) GPTRS_CUDA_OK(cudaFuncSetAttribute(kerns[i / 2][i & 1], cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(i / 2)));
+        for (int i = 0; i < 6; ++i) GPTRS_CUDA_OK(cudaFuncSetAttribute(kerns[i / 2][i & 1], cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
     const int64_t units = (int64_t)p.row_tiles * p.stretches, places = pair ? sm_count() / 2 : sm_count();
     GPTRS_REQUIRE(units < ((int64_t)1 << 31), "too many rows");
-    rc = launch_kernel(kerns[c.mode][p.inv_t > 0.f], dim3((unsigned)((units < places ? units : places) * (pair ? 2 : 1))), dim3(kThreads), smem_bytes(c.mode), as_stream(stream), 1, p,
+    rc = launch_kernel(kerns[c.mode][p.inv_t > 0.f], dim3((unsigned)((units < places ? units : places) * (pair ? 2 : 1))), dim3(kThreads), kSmem, as_stream(stream), 1, p,
                        pair ? 2 : 1);
     if (rc) return rc;
     // the second kernel waits for the first one itself (griddepcontrol.wait), so it may be launched ahead of its end
