@@ -34,45 +34,58 @@ struct AppendParams {
     int* status;
 };
 
-// Parents of the nodes 0 .. last in shared memory, and the depth of the last one: a load for all of them, then a walk of shared reads instead of one of
-// global reads that wait for each other.
-__device__ __forceinline__ int depth_of(const DraftTrees& t, const TreeSpan& s, int last, int* up, int* status) {
-    for (int i = threadIdx.x; i <= last; i += kThreads) up[i] = tree_parent(t, s, i, status);
-    __syncthreads();
-    int depth = 0;
-    for (int i = up[last]; i >= 0; i = up[i]) ++depth;   // (a parent is below its child: this ends)
-    return depth;
-}
-
-// A CTA per node. A thread takes two chunks of eight channels of a head: a pair that rotates together (c, c + half / 8), or two that stay.
+// A CTA per node. A thread takes two chunks of eight channels of a head: a pair that rotates together (c, c + half / 8), or two that stay. Rows, parents and the page are asked for
+// together, in front of the walk up the tree (shared reads, where global ones would wait for each other): what bounds a small call is the two trips to memory, tree and row.
+// 64 trees of 20 to 64 nodes, 32 / 8 heads: with the rows behind the walk 17.5 us.
+constexpr int kAhead = 2;         // tasks of a thread that are asked for in front
 __global__ void __launch_bounds__(kThreads) tree_append_kernel(const AppendParams p) {
     __shared__ int up[kMostNodes];
     pdl_launch_dependents();
     pdl_wait();
-    const int node = blockIdx.x;
+    const int node = blockIdx.x, tid = threadIdx.x;
     const TreeSpan s = tree_span(p.t, blockIdx.y, p.status);
     if (node >= s.nodes) return;   // the whole CTA
-    const int heads = p.t.q_heads + 2 * p.t.kv_heads, row = s.row0 + node, turning = p.half / 8;
+    const int heads = p.t.q_heads + 2 * p.t.kv_heads, row = s.row0 + node, turning = p.half / 8, tasks = heads * 8;
     const uint4* src = reinterpret_cast<const uint4*>(p.qkv + row * p.ld);
-    const int depth = depth_of(p.t, s, node, up, p.status);
+    auto chunks = [&](int i, int* c0, int* c1) {
+        const int k = i & 7;
+        *c0 = k < turning ? k : 2 * k;
+        *c1 = k < turning ? k + turning : 2 * k + 1;
+    };
+    uint4 a[kAhead], b[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+        const int i = tid + j * kThreads;
+        int c0, c1;
+        chunks(i, &c0, &c1);
+        if (i < tasks) { a[j] = src[(i >> 3) * 16 + c0]; b[j] = src[(i >> 3) * 16 + c1]; }
+    }
+    const int parent = tid <= node ? tree_parent(p.t, s, tid, p.status) : -1;
     const long long place = tree_place(p.t, s.slot, s.length + node, p.status);
-    int at = s.length + depth;
+    up[tid] = parent;
+    static_assert(kThreads >= kMostNodes, "a thread per node");
+    __syncthreads();
+    int at = s.length;
+    for (int i = up[node]; i >= 0; i = up[i]) ++at;   // (a parent is below its child: this ends)
     if (at >= p.positions && p.half > 0) { atomicExch(p.status, 2); at = 0; }
-    for (int i = threadIdx.x; i < heads * 8; i += kThreads) {
+    auto finish = [&](int i, uint4 a, uint4 b) {
         const int head = i >> 3, k = i & 7;
         const bool is_q = head < p.t.q_heads, is_v = head >= p.t.q_heads + p.t.kv_heads;
-        const bool turns = k < turning && !is_v;
-        const int c0 = k < turning ? k : 2 * k, c1 = k < turning ? k + turning : 2 * k + 1;
-        uint4 a = src[head * 16 + c0], b = src[head * 16 + c1];
-        if (turns) {
+        int c0, c1;
+        chunks(i, &c0, &c1);
+        if (k < turning && !is_v) {
             const float *cos = p.cos + (long long)at * p.half + 8 * k, *sin = p.sin + (long long)at * p.half + 8 * k;
             uint32_t *aw = &a.x, *bw = &b.x;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 c = *reinterpret_cast<const float2*>(cos + 2 * j), sn = *reinterpret_cast<const float2*>(sin + 2 * j);
-                const float a0 = bf16_lo(aw[j]), a1 = bf16_hi(aw[j]), b0 = bf16_lo(bw[j]), b1 = bf16_hi(bw[j]);
-                aw[j] = pack_bf16x2(a0 * c.x - b0 * sn.x, a1 * c.y - b1 * sn.y);
-                bw[j] = pack_bf16x2(b0 * c.x + a0 * sn.x, b1 * c.y + a1 * sn.y);
+            for (int j = 0; j < 2; ++j) {
+                const float4 c = reinterpret_cast<const float4*>(cos)[j], n = reinterpret_cast<const float4*>(sin)[j];
+                const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {n.x, n.y, n.z, n.w};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float a0 = bf16_lo(aw[2 * j + h]), a1 = bf16_hi(aw[2 * j + h]), b0 = bf16_lo(bw[2 * j + h]), b1 = bf16_hi(bw[2 * j + h]);
+                    aw[2 * j + h] = pack_bf16x2(a0 * cs[2 * h] - b0 * sn[2 * h], a1 * cs[2 * h + 1] - b1 * sn[2 * h + 1]);
+                    bw[2 * j + h] = pack_bf16x2(b0 * cs[2 * h] + a0 * sn[2 * h], b1 * cs[2 * h + 1] + a1 * sn[2 * h + 1]);
+                }
             }
         }
         if (is_q) {
@@ -85,6 +98,14 @@ __global__ void __launch_bounds__(kThreads) tree_append_kernel(const AppendParam
             *reinterpret_cast<uint4*>(dst + ((c0 ^ turn) << 4)) = a;
             *reinterpret_cast<uint4*>(dst + ((c1 ^ turn) << 4)) = b;
         }
+    };
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+        if (tid + j * kThreads < tasks) finish(tid + j * kThreads, a[j], b[j]);
+    for (int i = tid + kAhead * kThreads; i < tasks; i += kThreads) {
+        int c0, c1;
+        chunks(i, &c0, &c1);
+        finish(i, src[(i >> 3) * 16 + c0], src[(i >> 3) * 16 + c1]);
     }
 }
 
@@ -99,7 +120,7 @@ struct AcceptParams {
 
 // A CTA per (layer, tree); each walks the tree by itself. The k-th node of the path comes from a place behind k (numbers grow along a path), so a thread that moves one column
 // of chunks in the order of k never reads what it has written.
-__global__ void __launch_bounds__(kThreads) tree_accept_kernel(const AcceptParams p) {
+__global__ void __launch_bounds__(kThreads, 8) tree_accept_kernel(const AcceptParams p) {
     __shared__ int pick[kMostNodes], follow[kMostNodes], path[kMostNodes];
     __shared__ long long from[kMostNodes], to[kMostNodes];
     static_assert(kThreads >= kMostNodes, "a thread per node");
@@ -141,7 +162,7 @@ __global__ void __launch_bounds__(kThreads) tree_accept_kernel(const AcceptParam
     }
     __syncthreads();
     unsigned char* pool = static_cast<unsigned char*>(p.pools[blockIdx.x]);
-    constexpr int kAtOnce = 8;
+    constexpr int kAtOnce = 4;   // with eight, and the registers for them, half as many CTAs are there at a time: 64 trees, 26 layers 18.4 us instead of 14.7
     for (int col = tid; col < p.t.kv_heads * 32; col += kThreads) {
         unsigned char* base = pool + (col >> 4) * kTreeBlock;
         const int chunk = col & 15;
