@@ -967,10 +967,11 @@ def tree_append(*args, **kw):
 
 
 class TreeAttention(_Step):
-    """gptrs_cuda_tree_attention: q [rows][heads][128] (rows may lie a stride apart) -> out [rows][heads * 128]. The object owns its scratch: calls that may overlap (two
-    streams, two graphs) need one object each."""
+    """gptrs_cuda_tree_attention: q [rows][heads][128] (rows may lie a stride apart) -> out [rows][heads * 128]. The object has its own scratch, or the one of another object
+    for the same trees (`scratch=other.scratch`: the layers of a model, one after another); calls that may overlap (two streams, two graphs) need one each. After a
+    3 in the status word the scratch has to be zero again."""
 
-    def __init__(self, trees, q, pool, out=None, status=None):
+    def __init__(self, trees, q, pool, out=None, status=None, scratch=None):
         t, rows = trees.over(pool), trees.rows
         self.t = t
         s = self.step = _abi.TreeAttentionStep()
@@ -979,7 +980,11 @@ class TreeAttention(_Step):
         self.out = torch.empty((rows, t.q_heads * t.dim), dtype=torch.bfloat16, device=q.device) if out is None else _need(out, "out", torch.bfloat16, rows, t.q_heads * t.dim)
         self.status = _status(q.device, status)
         s.scratch_bytes = lib().gptrs_cuda_tree_scratch_bytes(ctypes.byref(t))
-        scratch = torch.zeros(s.scratch_bytes, dtype=torch.uint8, device=q.device) if s.scratch_bytes else None
+        if s.scratch_bytes and scratch is None:
+            scratch = torch.zeros(s.scratch_bytes, dtype=torch.uint8, device=q.device)
+        if s.scratch_bytes and (scratch.dtype != torch.uint8 or not scratch.is_contiguous() or scratch.numel() < s.scratch_bytes):
+            raise ValueError(f"scratch: expected {s.scratch_bytes} bytes, got {scratch.dtype} {list(scratch.shape)}")
+        self.scratch = scratch
         s.d_q, s.ldq = q.data_ptr(), q.stride(0) if rows > 1 else t.q_heads * t.dim
         s.d_pool, s.d_out, s.d_scratch, s.d_status = pool.data_ptr(), self.out.data_ptr(), None if scratch is None else scratch.data_ptr(), self.status.data_ptr()
         self._hold(q=q, pool=pool, out=self.out, scratch=scratch, status=self.status, **trees.tensors)

@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 import torch
 
+import gptrs_b200
 from gptrs_b200 import ops
 from oracle import tree_ref as tr
 
@@ -308,6 +309,68 @@ def test_attention_behind_four_gigabytes(cuda):
     t.view()[far.long()] = old
     q = t.queries()
     t.check(t.attention(q), q)
+
+
+# How a call is cut goes by the table's width, the trees, heads and rows: clusters of 8, 4, 2 and 1 CTAs, more of them than are on the GPU at a time, equal shares with parts
+# joined by warps (at several levels), and by the second kernel; each with one row tile and with several.
+CUTS = [  # heads, kv, trees, nodes, lengths
+    (4, 2, 3, 20, (1, 1400)), (4, 1, 1, 33, (5000, 5000)), (8, 8, 4, 40, (10, 700)), (8, 8, 9, 17, (0, 900)), (12, 12, 13, 9, (0, 700)), (12, 12, 40, 5, (0, 300)),
+    (4, 1, 2, 256, (20, 1000)), (32, 4, 3, 100, (0, 400)),
+    (4, 2, 2, 20, (9000, 21000)), (2, 1, 1, 3, (30000, 30000)), (8, 1, 1, 100, (20000, 20000)), (8, 8, 30, 6, (1500, 3000)), (4, 4, 60, 11, (100, 6000)), (16, 2, 20, 60, (300, 5000))]
+
+
+@pytest.mark.parametrize("heads,kv,trees,nodes,lengths", CUTS)
+def test_attention_however_it_is_cut(cuda, heads, kv, trees, nodes, lengths):
+    rng = np.random.default_rng(trees * nodes)
+    low, high = lengths
+    forest = [(high if i == 0 else int(rng.integers(low, high + 1)), bushy(nodes if i == 0 else int(rng.integers(1, nodes + 1)), rng, 12)) for i in range(trees)]
+    t = Trees(cuda, heads, kv, forest, seed=nodes)
+    q = t.queries(1.3)
+    call = ops.TreeAttention(t.trees, q, t.pool, status=t.status)
+    got = call().clone()
+    t.check(got, q)
+    assert int(t.status) == 0
+    for _ in range(3):
+        assert call().equal(got)                                        # whoever was last
+    if call.scratch is not None:
+        other = ops.TreeAttention(t.trees, q, t.pool, status=t.status, scratch=call.scratch)
+        assert other().equal(got)
+
+
+@pytest.mark.parametrize("heads,kv,length", [(8, 2, 700), (2, 1, 30000), (4, 4, 6000)])
+def test_attention_waits_that_run_out(cuda, heads, kv, length):
+    """The keys of every CTA's first block are never asked for: code 3, and the GPU stays usable."""
+    rng = np.random.default_rng(17)
+    trees = 60 if kv == 4 else 1
+    t = Trees(cuda, heads, kv, [(length if i == 0 else 300, bushy(9, rng)) for i in range(trees)], seed=3)
+    q = t.queries()
+    lib = gptrs_b200.lib()
+    lib.gptrs_cuda_debug_prefill_tc_fault(1, 500)
+    try:
+        ops.tree_attention(t.trees, q, t.pool, status=t.status)
+        torch.cuda.synchronize()
+    finally:
+        lib.gptrs_cuda_debug_prefill_tc_fault(0, 0)
+    assert int(t.status) == 3
+    t.status.zero_()
+    t.check(t.attention(q), q)
+    assert int(t.status) == 0
+
+
+def test_attention_of_trees_that_change_in_place(cuda):
+    """One object, and trees, lengths and parents that are written into its tensors: fewer nodes, padding, longer contexts than the call before."""
+    rng = np.random.default_rng(18)
+    t = Trees(cuda, 8, 2, [(300, bushy(20, rng)), (2000, bushy(20, rng)), (90, bushy(20, rng))], seed=6, max_nodes=24)
+    q = t.queries()
+    call = ops.TreeAttention(t.trees, q, t.pool, status=t.status)
+    for step in range(4):
+        t.check(call(), q)
+        parents = [bushy(20, rng) for _ in range(3)]
+        t.parent[:] = _ints(sum(parents, []), cuda)
+        t.forest = [(f[0] - 7 * step, parents[i]) for i, f in enumerate(t.forest)]
+        t.length[:] = _ints([f[0] for f in t.forest], cuda)
+        t.kvs = [t.read(i, np.arange(f[0] + 20)) for i, f in enumerate(t.forest)]
+    assert int(t.status) == 0
 
 
 # ---- append --------------------------------------------------------------------------------------------------------------------

@@ -50,6 +50,19 @@ def test_steps_are_checked(call, bad):
     assert gptrs_b200.lib().gptrs_cuda_last_error()
 
 
+def test_scratch_is_checked():
+    fn, step = _calls()[1]
+    long = _trees(max_pages=4000)
+    need = gptrs_b200.lib().gptrs_cuda_tree_scratch_bytes(ctypes.byref(long))
+    assert need > 0 and gptrs_b200.lib().gptrs_cuda_tree_scratch_bytes(ctypes.byref(_trees())) == 0   # short contexts need none
+    for bad in (dict(d_scratch=None), dict(scratch_bytes=need - 1), dict(d_scratch=8)):
+        step = _abi.TreeAttentionStep(1 << 20, 0, 16, 1 << 24, 16, need, 16)
+        for k, v in bad.items():
+            setattr(step, k, v)
+        assert fn(ctypes.byref(long), ctypes.byref(step), None) == REFUSED
+    assert gptrs_b200.lib().gptrs_cuda_tree_scratch_bytes(None) == 0
+
+
 def test_calls_without_rows_do_nothing():
     for fn, step in _calls()[:2]:
         assert fn(ctypes.byref(_trees(rows=0, d_parent=None)), ctypes.byref(step), None) == OK

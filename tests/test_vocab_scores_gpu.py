@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 import torch
 
+import gptrs_b200
 from gptrs_b200 import ops
 from oracle import tree_ref as tr
 
@@ -186,6 +187,36 @@ def test_twice_and_two_at_once(cuda):
     torch.cuda.synchronize()
     for c in calls:
         assert all(a.equal(b) for a, b in zip(want, [r for r in c.result if r is not None]))
+
+
+@pytest.mark.parametrize("rows", [3, 100, 300])
+def test_waits_that_run_out(cuda, rows):
+    """The rows of every CTA's first stage are never asked for: code 3, and the GPU stays usable."""
+    rng, x, w = _inputs(cuda, rows, 256, 3000, seed=9)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    lib = gptrs_b200.lib()
+    lib.gptrs_cuda_debug_prefill_tc_fault(1, 500)
+    try:
+        ops.vocab_scores(x, w, status=status)
+        torch.cuda.synchronize()
+    finally:
+        lib.gptrs_cuda_debug_prefill_tc_fault(0, 0)
+    assert int(status) == 3
+    status.zero_()
+    _check(ops.vocab_scores(x, w, status=status), x, w, None)
+    assert int(status) == 0
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, 30), (17, 33), (128, 4096), (129, 100), (700, 12345), (1300, 64), (2500, 999)])
+def test_however_it_is_cut(cuda, rows, vocab):
+    rng, x, w = _inputs(cuda, rows, 80, vocab, seed=rows)
+    target = rng.integers(0, vocab, rows)
+    t = torch.tensor(target, dtype=torch.int32, device=cuda)
+    for temperature in (0.0, 1.0):
+        call = ops.VocabScores(x, w, target=t, temperature=temperature, seed=3)
+        got = [r.clone() for r in call()]
+        _check(call.result, x, w, target, temperature=temperature, seed=3)
+        assert all(a.equal(b) for a, b in zip(got, call()))
 
 
 def test_a_step_of_speculative_decoding(cuda):
