@@ -77,7 +77,8 @@ __device__ __forceinline__ float lg2(float x) {
     asm("lg2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float gumbel(uint32_t h) { return -logf(-log1pf(-(((float)h + 0.5f) * (1.f / 4294967296.f)))); }
+// (h + 1/2 rounds to 2^32 for the last 128 of h: below 1, so that no token's value is -inf for its noise)
+__device__ __forceinline__ float gumbel(uint32_t h) { return -logf(-log1pf(-fminf(((float)h + 0.5f) * (1.f / 4294967296.f), 1.f - 0x1p-24f))); }
 __device__ __noinline__ float capped(float z, float cap) { return cap * tanhf(z / cap); }
 __device__ __forceinline__ void join(Part& a, const Part& b) {
     const float m = fmaxf(a.m, b.m);
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
             int target[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                a[r] = {-INFINITY, 0.f, -INFINITY, 0.f, -1, NAN};
+                a[r] = {-INFINITY, 0.f, -INFINITY, -INFINITY, -1, NAN};
                 target[r] = p.target && warp + 8 * r < p.rows ? p.target[warp + 8 * r] : -1;
             }
             for (int n0 = unit.begin; n0 < unit.end; n0 += p.cols) {
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
             const int row = unit.row0 + in_tile;
             const bool rows = unit.row0 + (warp & 3) * 32 < p.rows;
             const int target = p.target && row < p.rows ? p.target[row] : -1;
-            Part a = {-INFINITY, 0.f, -INFINITY, 0.f, -1, NAN};
+            Part a = {-INFINITY, 0.f, -INFINITY, -INFINITY, -1, NAN};
             for (int n0 = unit.begin; n0 < unit.end && !failed; n0 += p.cols) {
                 const int first = n0 + half * width, some = rows ? min(half ? p.cols - width : width, unit.end - first) : 0;   // this half's tokens
                 uint64_t acc[kCols / 4];
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(kJoinThreads) vocab_join_kernel(const __grid_c
     const int row = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31, n = p.row_parts;
     if (row >= p.rows) return;
     const Part* parts = p.parts + (size_t)row * n;
-    Part a = {-INFINITY, 0.f, -INFINITY, 0.f, -1, NAN};
+    Part a = {-INFINITY, 0.f, -INFINITY, -INFINITY, -1, NAN};
     for (int i = lane; i < n; i += 32) join(a, parts[i]);
     a = join_lanes(a);
     if (lane) return;
@@ -526,7 +527,9 @@ int gptrs_cuda_vocab_scores(const gptrs_vocab_scores* s, void* stream) {
     GPTRS_REQUIRE(s->dim % 8 == 0 && ldx % 8 == 0 && ldw % 8 == 0 && ldx >= s->dim && ldw >= s->dim && ldx < ((int64_t)1 << 31) && ldw < ((int64_t)1 << 31),
                   "dim and the strides must be multiples of 8, and rows must not overlap");
     GPTRS_REQUIRE(aligned16(s->d_hidden) && aligned16(s->d_weight) && (reinterpret_cast<uintptr_t>(s->d_scratch) & 31) == 0, "pointers must be 16-byte aligned, scratch 32");
-    GPTRS_REQUIRE(s->temperature == s->temperature && s->soft_cap >= 0.f && s->soft_cap < 3e38f, "bad temperature or soft cap");
+    // (its reciprocal is a factor: far from 1 it, or logits times it, would leave f32)
+    GPTRS_REQUIRE(s->temperature <= 0.f || (s->temperature >= 1e-20f && s->temperature <= 1e20f), "a temperature above 0 must be 1e-20 .. 1e20");
+    GPTRS_REQUIRE(s->soft_cap >= 0.f && s->soft_cap < 3e38f, "bad soft cap");
     GPTRS_REQUIRE(!s->d_logprob || s->d_target, "log-probabilities of targets need targets");
     GPTRS_REQUIRE(s->rows == 0 || (s->d_scratch && s->scratch_bytes >= gptrs_cuda_vocab_scores_scratch_bytes(s)), "scratch is too small");
     if (s->rows == 0) return GPTRS_OK;
@@ -552,7 +555,8 @@ int gptrs_cuda_vocab_scores(const gptrs_vocab_scores* s, void* stream) {
     if (attr_once.first_time())
         for (int i = 0; i < 6; ++i) GPTRS_CUDA_OK(cudaFuncSetAttribute(kerns[i / 2][i & 1], cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
     const int64_t units = (int64_t)p.row_tiles * p.stretches, places = pair ? sm_count() / 2 : sm_count();
-    GPTRS_REQUIRE(units < ((int64_t)1 << 31), "too many rows");
+    // (a CTA counts its stages in 32 bits)
+    GPTRS_REQUIRE(units < ((int64_t)1 << 30) && (units / places + 1) * p.tiles * ceil_div(p.dim, kStageDim) < ((int64_t)1 << 31), "too many rows for one call");
     rc = launch_kernel(kerns[c.mode][p.inv_t > 0.f], dim3((unsigned)((units < places ? units : places) * (pair ? 2 : 1))), dim3(kThreads), kSmem, as_stream(stream), 1, p,
                        pair ? 2 : 1);
     if (rc) return rc;

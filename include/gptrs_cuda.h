@@ -820,7 +820,7 @@ int gptrs_cuda_kv8_attention(const gptrs_kv8_cache* c, const gptrs_kv8_attention
  * has the parent d_parent[row] < i, a node of the same tree, or -1; depth(i) = 0 without a parent, else depth(parent) + 1. The sequence of the
  * tree has d_length[s] tokens in the cache, through page_table[d_slot[s]]. Node i lies behind them at position length + i, is rotated by
  * position length + depth(i), and sees those tokens, its ancestors and itself. What is appended of a tree can be overwritten: the cache counts as holding length tokens
- * until a caller says otherwise.
+ * until a caller says otherwise. A slot is in one tree of a call, and the page of a node in no other slot's.
  * A tree with a negative slot is padding: nothing of it is read or written but what gptrs_cuda_tree_accept says. *d_status = 2: a slot, d_first, a length or a number of
  * nodes out of range (more than max_nodes, or behind position 16 max_pages): that tree counts as padding; a parent out of range: it counts as -1;
  * a page out of range: its tokens are not written, not moved, and not seen. Waits inside the kernels are bounded (3).
@@ -850,9 +850,9 @@ typedef struct {
 } gptrs_tree_append_step;
 int gptrs_cuda_tree_append(const gptrs_draft_trees* t, const gptrs_tree_append_step* s, void* stream);
 /* out [rows][q_heads][dim] (bf16) = softmax over what the node sees . values. A node that sees nothing (its pages are out of range) gives zeros. Keys and values of nodes
- * that a node does not see do not touch it, whatever they are. Scratch: gptrs_cuda_tree_scratch_bytes, 16-byte aligned, all zero before its first
- * call and after one that left 3 in *d_status (calls with other numbers of heads or nodes have their own, or zero it), of one call at a time: calls and graphs that may overlap
- * have their own. */
+ * that a node does not see do not touch it, whatever they are. Scratch: gptrs_cuda_tree_scratch_bytes (0: none), 16-byte aligned, all zero before its
+ * first call and after one that left 3 in *d_status; of one call at a time (calls and graphs that may overlap have their own), and of calls with the same heads, max_nodes,
+ * n_trees and max_pages: others have their own, or zero it. */
 typedef struct {
     const void* d_q;                   /* [rows][q_heads][dim], rows ldq apart (0 = packed) */
     int64_t ldq;
@@ -884,11 +884,11 @@ int gptrs_cuda_tree_accept(const gptrs_draft_trees* t, const gptrs_tree_accept_s
  *     lse          log sum exp z
  *     logprob      z[target] - lse, the target's log-probability (the cross entropy with its sign turned); a negative target: 0; one behind the vocabulary: NaN and 2 in *d_status
  *     pick         the largest z (the first of equals), or with temperature > 0 the largest z / temperature + g, a draw from softmax(z / temperature):
- *                  g = -log(-log(1 - v)), v = (h + 1/2) / 2^32 in f32, h = mix(seed ^ mix(token + 0x9e3779b9 (row + 1))) with the 32-bit mix
+ *                  (temperature 1e-20 .. 1e20) g = -log(-log(1 - v)), v = (h + 1/2) / 2^32 in f32 (1 - 2^-24 at most), h = mix(seed ^ mix(token + 0x9e3779b9 (row + 1))) with the 32-bit mix
  *                  x ^= x >> 16, x *= 0x7feb352d, x ^= x >> 15, x *= 0x846ca68b, x ^= x >> 16
  *     pick_logprob z[pick] - lse
- * Every result is left out where its pointer is null. bf16 operands, products summed in f32. A token whose bias is -inf has no probability; NaN in a row's hidden
- * state makes its lse and log-probabilities NaN, and its pick a token of the vocabulary. dim and both strides are multiples of 8, hidden and weight 16-byte aligned. Waits inside the kernel are bounded (3
+ * Every result is left out where its pointer is null. bf16 operands, products summed in f32. A bias is finite, or -inf: such a token has no probability (where no
+ * token has one: lse -inf, pick 0, log-probabilities NaN). NaN in a row's hidden state makes its lse and log-probabilities NaN, and its pick a token of the vocabulary. dim and both strides are multiples of 8, hidden and weight 16-byte aligned. Waits inside the kernel are bounded (3
  * in *d_status).
  * ============================================================================================ */
 typedef struct {

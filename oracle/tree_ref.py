@@ -65,9 +65,8 @@ def noise(seed, rows, vocab):
     with np.errstate(over="ignore"):
         at = np.arange(vocab, dtype=np.uint32)[None] + np.uint32(0x9e3779b9) * (np.arange(rows, dtype=np.uint32)[:, None] + np.uint32(1))
     h = _mix(np.uint32(seed) ^ _mix(at))
-    v = ((h.astype(np.float32) + np.float32(0.5)) * np.float32(2.0 ** -32)).astype(np.float64)
-    with np.errstate(divide="ignore"):
-        return -np.log(-np.log1p(-v))
+    v = np.minimum((h.astype(np.float32) + np.float32(0.5)) * np.float32(2.0 ** -32), np.float32(1 - 2.0 ** -24)).astype(np.float64)
+    return -np.log(-np.log1p(-v))
 
 
 def logits(hidden, weight, bias=None, cap=0.0):

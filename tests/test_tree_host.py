@@ -85,7 +85,7 @@ def _scores(**kw):
 
 @pytest.mark.parametrize("bad", [dict(d_hidden=None), dict(d_weight=None), dict(d_status=None), dict(rows=-1), dict(vocab=0), dict(dim=0), dict(dim=12), dict(ldh=56), dict(ldh=68),
                                  dict(ldw=56), dict(ldw=66), dict(d_hidden=8), dict(d_weight=24), dict(d_scratch=None), dict(d_scratch=8), dict(scratch_bytes=1), dict(d_target=None),
-                                 dict(soft_cap=-1.0), dict(soft_cap=float("nan")), dict(temperature=float("nan"))])
+                                 dict(soft_cap=-1.0), dict(soft_cap=float("nan")), dict(temperature=float("nan")), dict(temperature=float("inf")), dict(temperature=1e-30)])
 def test_scores_are_checked(bad):
     assert gptrs_b200.lib().gptrs_cuda_vocab_scores(ctypes.byref(_scores(**bad)), None) == REFUSED
 

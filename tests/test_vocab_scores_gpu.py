@@ -4,6 +4,8 @@ Tolerances. Products of bf16 are exact; the tensor cores add 16 of them at a tim
 A = sum |x w| each time: (dim / 16 + 8) 2^-23 A for a logit (e; a soft cap makes it no larger, a bias adds a rounding, 2^-24 of the logit). lse moves by the largest e at
 most, log-probabilities by twice that; exponentials, logarithms and the last differences are f32: 2^-20 of the numbers that meet. A pick is one whose own value is
 within the errors of the largest one's."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -187,6 +189,27 @@ def test_twice_and_two_at_once(cuda):
     torch.cuda.synchronize()
     for c in calls:
         assert all(a.equal(b) for a, b in zip(want, [r for r in c.result if r is not None]))
+
+
+@pytest.mark.parametrize("rows", [3, 100, 300])
+def test_the_only_token_is_picked_whatever_its_noise(cuda, rows):
+    """h of (this seed, row 0, token 5) is 2^32 - 94, which rounds to 2^32."""
+    rng, x, w = _inputs(cuda, rows, 64, 700, seed=4)
+    bias = torch.full((700,), -math.inf, device=cuda)
+    bias[5] = 0
+    got = ops.vocab_scores(x, w, bias=bias, temperature=1.0, seed=23192014)
+    assert (got.pick == 5).all() and (got.pick_logprob.abs() < 1e-5).all()
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+@pytest.mark.parametrize("rows", [3, 100, 300])
+def test_no_token_is_left(cuda, rows, temperature):
+    """A bias of -inf everywhere: lse -inf, and a pick, the first token, that has no log-probability."""
+    rng, x, w = _inputs(cuda, rows, 64, 700, seed=4)
+    bias = torch.full((700,), -math.inf, device=cuda)
+    target = torch.full((rows,), 5, dtype=torch.int32, device=cuda)
+    got = ops.vocab_scores(x, w, bias=bias, target=target, temperature=temperature)
+    assert (got.lse == -math.inf).all() and (got.pick == 0).all() and got.pick_logprob.isnan().all() and got.logprob.isnan().all()
 
 
 @pytest.mark.parametrize("rows", [3, 100, 300])
