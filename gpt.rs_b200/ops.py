@@ -967,11 +967,11 @@ def tree_append(*args, **kw):
 
 
 class TreeAttention(_Step):
-    """gptrs_cuda_tree_attention: q [rows][heads][128] (rows may lie a stride apart) -> out [rows][heads * 128]. The object has its own scratch, or the one of another object
-    for the same trees (`scratch=other.scratch`: the layers of a model, one after another); calls that may overlap (two streams, two graphs) need one each. After a
-    3 in the status word the scratch has to be zero again."""
+    """gptrs_cuda_tree_attention: q [rows][heads][128] (rows may lie a stride apart) -> out [rows][heads * 128]. The object has its own scratch, or that of another
+    object of the same shape (`scratch_of=other`: the layers of a model, one after another); calls that may overlap (two streams, two graphs) need one each. After a
+    3 in the status word it has to be zeroed, or made anew."""
 
-    def __init__(self, trees, q, pool, out=None, status=None, scratch=None):
+    def __init__(self, trees, q, pool, out=None, status=None, scratch_of=None):
         t, rows = trees.over(pool), trees.rows
         self.t = t
         s = self.step = _abi.TreeAttentionStep()
@@ -980,10 +980,10 @@ class TreeAttention(_Step):
         self.out = torch.empty((rows, t.q_heads * t.dim), dtype=torch.bfloat16, device=q.device) if out is None else _need(out, "out", torch.bfloat16, rows, t.q_heads * t.dim)
         self.status = _status(q.device, status)
         s.scratch_bytes = lib().gptrs_cuda_tree_scratch_bytes(ctypes.byref(t))
-        if s.scratch_bytes and scratch is None:
-            scratch = torch.zeros(s.scratch_bytes, dtype=torch.uint8, device=q.device)
-        if s.scratch_bytes and (scratch.dtype != torch.uint8 or not scratch.is_contiguous() or scratch.numel() < s.scratch_bytes):
-            raise ValueError(f"scratch: expected {s.scratch_bytes} bytes, got {scratch.dtype} {list(scratch.shape)}")
+        shape = ("q_heads", "kv_heads", "max_nodes", "n_trees", "max_pages")   # what a call is cut by
+        if scratch_of is not None and any(getattr(t, k) != getattr(scratch_of.t, k) for k in shape):
+            raise ValueError("scratch_of: the other call is of another shape (heads, nodes, trees, or width of the page table)")
+        scratch = scratch_of.scratch if scratch_of is not None else torch.zeros(s.scratch_bytes, dtype=torch.uint8, device=q.device) if s.scratch_bytes else None
         self.scratch = scratch
         s.d_q, s.ldq = q.data_ptr(), q.stride(0) if rows > 1 else t.q_heads * t.dim
         s.d_pool, s.d_out, s.d_scratch, s.d_status = pool.data_ptr(), self.out.data_ptr(), None if scratch is None else scratch.data_ptr(), self.status.data_ptr()

@@ -333,8 +333,16 @@ def test_attention_however_it_is_cut(cuda, heads, kv, trees, nodes, lengths):
     for _ in range(3):
         assert call().equal(got)                                        # whoever was last
     if call.scratch is not None:
-        other = ops.TreeAttention(t.trees, q, t.pool, status=t.status, scratch=call.scratch)
+        other = ops.TreeAttention(t.trees, q, t.pool, status=t.status, scratch_of=call)
         assert other().equal(got)
+
+
+def test_attention_shares_scratch_with_calls_of_its_shape_alone(cuda):
+    rng = np.random.default_rng(2)
+    a, b = (Trees(cuda, 4, 2, [(9000, bushy(5, rng))] * n, seed=1) for n in (1, 2))
+    first = ops.TreeAttention(a.trees, a.queries(), a.pool)
+    with pytest.raises(ValueError, match="another shape"):
+        ops.TreeAttention(b.trees, b.queries(), b.pool, scratch_of=first)
 
 
 @pytest.mark.parametrize("heads,kv,length", [(8, 2, 700), (2, 1, 30000), (4, 4, 6000)])
