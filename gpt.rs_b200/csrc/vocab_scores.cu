@@ -3,7 +3,7 @@
 // z = x . w^T on the tcgen05 tensor cores, x rows as the M side. A unit is a tile of rows x a stretch of the vocabulary, which a CTA (one per SM) walks over in tiles of
 // up to 256 tokens. What a row needs to know of its logits is a running state in registers (maximum and sum, best token, the target's logit), so a logit lives
 // from the accumulator to the exponential and nowhere else.
-//   warps 0 - 7   a thread per row and half of the tile's tokens. The accumulator in tensor memory is read out every 128 or 512 of dim and added up in f32 registers: the
+//   warps 0 - 7   a thread per row and half of the tile's tokens. The accumulator in tensor memory is read out every 128 to 512 of dim (up to 1024 where draws keep its readers busy) and added up in f32 registers: the
 //                 tensor cores cut what does not fit into the sum that they add to, 16 products at a time, which over all of dim would cost log-probabilities digits.
 //                 Up to 16 rows the logits then go through shared memory, and a warp takes a row with a token per lane
 //   warp 8        requests stages of 64 of dim
@@ -159,6 +159,10 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
     pdl_launch_dependents();
     pdl_wait();
     const int steps = (p.dim + kStageDim - 1) / kStageDim, units = p.row_tiles * p.stretches, my_cols = p.cols / kCtas, stages = p.stages, stage_size = stage_bytes(kMode, p.cols);
+    // Draws take the epilogue longer than two accumulators of kDrain last. With the first two of a tile up to twice as long (a quarter of dim) the products go on meanwhile: 416 rows of
+    // 131072 x 4096 430 -> 405 us, and lse is off by 6.2e-7 instead of 4.0e-7 (f32 sums one by one 5.8e-7).
+    const int lead = kPair && kSample ? min(2 * kDrain, max(kDrain, steps / 4)) : kDrain;
+    auto behind = [&](int k0) { return k0 + (k0 < 2 * lead ? lead : kDrain); };   // the first stage of the next accumulator
     struct Unit { int row0, begin, end; };
     auto unit_of = [&](int u) {
         const int begin = u / p.row_tiles * (p.tiles * p.cols);
@@ -202,8 +206,8 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
             for (int u = blockIdx.x / kCtas; u < units && !failed; u += gridDim.x / kCtas) {
                 const Unit unit = unit_of(u);
                 for (int n0 = unit.begin; n0 < unit.end && !failed; n0 += p.cols) {
-                    for (int k0 = 0; k0 < steps && !failed; k0 += kDrain, ++n) {
-                        const int buf = n & 1, k1 = min(k0 + kDrain, steps);
+                    for (int k0 = 0; k0 < steps && !failed; k0 = behind(k0), ++n) {
+                        const int buf = n & 1, k1 = min(behind(k0), steps);
                         if (n >= 2 && !mbar_wait_polled(&acc_empty[buf], (uint32_t)((n >> 1) - 1) & 1u, p.wait_limit, 256)) { failed = true; break; }
                         tc_fence_after();
                         for (int k = k0; k < k1; ++k) {
@@ -327,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                 uint64_t acc[kCols / 4];
 #pragma unroll
                 for (int i = 0; i < kCols / 4; ++i) acc[i] = 0;
-                for (int k0 = 0; k0 < steps; k0 += kDrain, ++n) {
+                for (int k0 = 0; k0 < steps; k0 = behind(k0), ++n) {
                     const int buf = n & 1;
                     if (!failed && !mbar_wait_polled(&acc_full[buf], (uint32_t)(n >> 1) & 1u, p.wait_limit, 64)) failed = true;
                     failed = __any_sync(0xffffffffu, failed);
