@@ -8,7 +8,7 @@
 //   O[128 x 128] += P . V      P from tensor memory, V as an MN-major operand
 // Warp 4 issues the products, S two blocks ahead of P . V; warps 5 and 6 request the pages of K and V; warp 7 looks ahead: it finds the next piece of work, collects
 // the ancestors of its nodes and requests its queries as soon as the products that read the last ones are complete.
-// Blocks that reach behind the sequence's tokens are masked by a bit per node. In them values of nodes that are not finite are taken out of the stage before the product
+// Blocks that reach behind the sequence's tokens are masked by a bit per node. In them values of nodes that are not finite are taken out of the stage by warp 6
 // (a weight of 0 does not help there) and added to the rows that see them at the end.
 //
 // Work, where contexts may be long: an item is a (tree, kv head, row tile or pair of them), a unit a block of an item, and an item has some more that stand for what it costs
@@ -187,6 +187,11 @@ __device__ __forceinline__ uint32_t bits_from(const uint32_t* row, int at) {
     return __funnelshift_r(row[w], w + 1 < kWords ? row[w + 1] : 0u, at & 31);
 }
 
+__device__ __forceinline__ bool mbar_ready(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok;
+}
 // Waits (bounded) until `n` parts of a join are in scratch, and sets the count back.
 __device__ __forceinline__ bool parts_stored(uint32_t* at, uint32_t n, uint32_t limit) {
     for (uint32_t i = 0; i < 8 * limit; ++i) {
@@ -314,6 +319,50 @@ __device__ __forceinline__ bool join_parts(const AttentionParams& p, const Piece
     return true;
 }
 
+// Values behind the last node, and those of nodes that are not finite: the product sees zeros, and `odd` says which nodes they are. By the warp that has asked for them, while the
+// softmax is at the block in front (by the softmax's own warps a block took 4900 cycles instead of 2900).
+__device__ __forceinline__ void clean_values(uint32_t stage, const TreeSpan& span, int kb, uint32_t* odd) {
+    const int lane = threadIdx.x & 31, from = max(0, span.length - kb * kKeys), total = span.length + span.nodes - kb * kKeys;   // rows of nodes
+#pragma unroll 1
+    for (int k0 = from / 4 & ~3; k0 < kKeys / 4; k0 += 4) {   // 16 rows, of both halves: a row is eight lanes'
+        uint4 v[8];
+        bool any = false;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t at = stage + (k >> 2) * kHalf + (k0 + (k & 3)) * 512 + lane * 16;
+            v[k] = ld_shared_v4(at);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {   // an exponent of ones and one more reach the sign's place
+            constexpr uint32_t kExponents = 0x7f807f80u, kOnes = 0x00800080u;
+            const uint32_t found = ((v[k].x & kExponents) + kOnes) | ((v[k].y & kExponents) + kOnes) | ((v[k].z & kExponents) + kOnes) | ((v[k].w & kExponents) + kOnes);
+            any |= (found & 0x80008000u) != 0;
+        }
+        if (!__any_sync(0xffffffffu, any) && total >= 4 * k0 + 16) continue;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int row = 4 * (k0 + (k & 3)) + (lane >> 3);
+            const uint32_t at = stage + (k >> 2) * kHalf + (k0 + (k & 3)) * 512 + lane * 16;
+            uint32_t* w = &v[k].x;
+            uint32_t found = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t m = (((w[j] & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15;
+                found |= m;
+                w[j] &= ~(m * 0xffffu);
+            }
+            if (row >= total) st_shared_v4(at, 0, 0, 0, 0);
+            else if (found && row >= from) {
+                st_shared_v4(at, w[0], w[1], w[2], w[3]);
+                const int node = kb * kKeys + row - span.length;
+                atomicOr(&odd[node >> 5], 1u << (node & 31));
+            }
+        }
+    }
+    fence_proxy_async();
+    __syncwarp();
+}
+
 template <bool kSmall>
 __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __grid_constant__ AttentionParams p) {
     // f32 accumulator, bf16 operands, M = 128; N = 64, or 128 with B's contraction index as rows
@@ -338,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&k_full[i], 1); mbar_init(&v_full[i], 1); mbar_init(&k_empty[i], 1); mbar_init(&v_empty[i], 1); mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], kSoftmaxWarps); mbar_init(&piece_full[i], 1); mbar_init(&piece_empty[i], kReaders); mbar_init(&sees_full[i], 1);
+            mbar_init(&p_full[i], kSoftmaxWarps + 1); mbar_init(&piece_full[i], 1); mbar_init(&piece_empty[i], kReaders); mbar_init(&sees_full[i], 1);
         }
         mbar_init(&q_full, 1);
         mbar_init(&q_empty, 1);
@@ -513,10 +562,26 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
             const int* table = p.t.table + (long long)piece.span.slot * p.t.max_pages;
             auto page_of = [&](int kb) { return lane < kPages && kb < piece.kb1 && kb * kPages + lane <= last_page ? table[kb * kPages + lane] : -2; };
             int coming = kSmall ? first_page : page_of(piece.kb0);
+            bool due = false;                                 // values of the block in front are to be looked through, before the product with them
+            auto clean = [&](int g, int kb) {
+                if (!mbar_wait_parked(smem_u32(&v_full[g & 1]), (uint32_t)(g >> 1) & 1u, p.wait_limit) ||
+                    !mbar_wait_parked(smem_u32(&sees_full[i & 1]), (uint32_t)(i >> 1) & 1u, p.wait_limit))
+                    failed = true;
+                failed = __any_sync(0xffffffffu, failed);
+                if (failed) return;
+                clean_values(base + (g & 1) * kStage, piece.span, kb, s_odd[i & 1]);
+                if (lane == 0) mbar_arrive(&p_full[g & 1]);
+            };
             for (int kb = piece.kb0; kb < piece.kb1; ++kb, ++g) {
                 const int page = coming;
                 coming = page_of(kb + 1);
-                if (g >= 2 && !mbar_wait_parked(smem_u32(&empty[g & 1]), (uint32_t)((g - 2) >> 1) & 1u, p.wait_limit)) failed = true;
+                if (g >= 2) {
+                    if (due && !__all_sync(0xffffffffu, mbar_ready(&empty[g & 1], (uint32_t)((g - 2) >> 1) & 1u))) {
+                        clean(g - 1, kb - 1);
+                        due = false;
+                    }
+                    if (!mbar_wait_parked(smem_u32(&empty[g & 1]), (uint32_t)((g - 2) >> 1) & 1u, p.wait_limit)) failed = true;
+                }
                 failed = __any_sync(0xffffffffu, failed);
                 if (failed) break;
                 const bool there = lane < kPages && kb * kPages + lane <= last_page, good = there && page >= 0 && page < p.t.n_pages;
@@ -541,7 +606,13 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
                     tma_load_3d(dst + kHalf + lane * (kTreePage * 128), &p.map, 0, 1, row0, bar);
                 }
                 __syncwarp();
+                if (is_v) {
+                    if (due) clean(g - 1, kb - 1);
+                    due = (kb + 1) * kKeys > piece.span.length;
+                    if (!due && lane == 0) mbar_arrive(&p_full[g & 1]);
+                }
             }
+            if (!failed && due) clean(g - 1, piece.kb1 - 1);
             if (failed) break;
         }
         // copies still in flight write this CTA's shared memory
@@ -720,35 +791,6 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
                     asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
                 }
                 if (failed) break;
-                if (tail) {
-                    if (!wait(&v_full[g & 1], (uint32_t)(g >> 1))) break;
-                    // values behind the last node, and those of nodes that are not finite: the product sees zeros
-                    const int from = max(0, span.length - kb * kKeys), total = span.length + span.nodes;
-                    const int chunk = tid & 15, r0 = tid >> 4;
-                    const uint32_t stage = sV + (g & 1) * kStage + (chunk >> 3) * kHalf + ((chunk & 7) << 4);
-                    uint4 v[kKeys / 8];
-#pragma unroll
-                    for (int k = 0; k < kKeys / 8; ++k) v[k] = ld_shared_v4(stage + (8 * k + r0) * 128);
-                    uint32_t odd_rows = 0;
-#pragma unroll
-                    for (int k = 0; k < kKeys / 8; ++k)
-                        odd_rows |= ((__vcmpgeu2(v[k].x & 0x7fff7fffu, 0x7f807f80u) | __vcmpgeu2(v[k].y & 0x7fff7fffu, 0x7f807f80u) | __vcmpgeu2(v[k].z & 0x7fff7fffu, 0x7f807f80u) |
-                                      __vcmpgeu2(v[k].w & 0x7fff7fffu, 0x7f807f80u)) ? 1u : 0u) << k;
-                    for (int k = 0; k < kKeys / 8; ++k) {
-                        const int r = 8 * k + r0, token = kb * kKeys + r;
-                        if (token >= total) {
-                            st_shared_v4(stage + r * 128, 0, 0, 0, 0);
-                        } else if (odd_rows >> k & 1 && r >= from) {
-                            uint4 x = ld_shared_v4(stage + r * 128);
-                            uint32_t* w = &x.x;
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) w[j] &= ~__vcmpgeu2(w[j] & 0x7fff7fffu, 0x7f807f80u);
-                            st_shared_v4(stage + r * 128, x.x, x.y, x.z, x.w);
-                            atomicOr(&s_odd[at & 1][(token - span.length) >> 5], 1u << ((token - span.length) & 31));
-                        }
-                    }
-                    fence_proxy_async();
-                }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[g & 1]);
@@ -759,7 +801,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
             if (!idle) {
                 if (any && m == -INFINITY) l = NAN;             // scores of -inf alone
                 uint32_t odd = 0;
-                if (masked) {
+                if (masked) {   // (the wait is over: it orders what the values' warp has found before the reads)
+                    if (!wait(&p_full[(g - 1) & 1], (uint32_t)((g - 1) >> 1))) break;
 #pragma unroll
                     for (int w = 0; w < kWords; ++w) odd |= s_odd[at & 1][w] & sees[w];
                 }
