@@ -33,12 +33,12 @@ __device__ __forceinline__ TreeSpan tree_span(const DraftTrees& t, int s, int* s
     }
     return r;
 }
-__device__ __forceinline__ int tree_parent(const DraftTrees& t, const TreeSpan& s, int i, int* status) {
-    const int up = t.parent[s.row0 + i];
+__device__ __forceinline__ int tree_parent_of(int up, int i, int* status) {
     if (up >= -1 && up < i) return up;
     atomicExch(status, 2);
     return -1;
 }
+__device__ __forceinline__ int tree_parent(const DraftTrees& t, const TreeSpan& s, int i, int* status) { return tree_parent_of(t.parent[s.row0 + i], i, status); }
 // First byte of the keys of (position, kv head 0) in a pool; -1: its page is out of range.
 __device__ __forceinline__ long long tree_place(const DraftTrees& t, int slot, int position, int* status) {
     const int page = t.table[(long long)slot * t.max_pages + position / kTreePage];

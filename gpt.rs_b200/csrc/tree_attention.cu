@@ -4,7 +4,8 @@
 // tcgen05 products: a CTA holds a tile of 128 rows and walks over keys in blocks of 64 (four pages), two CTAs to an SM:
 //   S[128 x 64] = Q . K^T      both from shared memory (K-major, 128-byte swizzle, which is how the pool holds a page), two accumulators in tensor memory
 //   softmax                    warps 0 - 3, a thread per row, one pass over its scores: the reference stays until a block's weights add up to more than 2^14, so there is
-//                              no pass for the maximum but in a row's first block; weights go as bf16 over S
+//                              no pass for the maximum but in a row's first block; weights go as bf16 over S (values are bf16, and a product has one type: results
+//                              are off by 0.0023 of their size, by 0.0017 with f32 weights, which is the result's own rounding)
 //   O[128 x 128] += P . V      P from tensor memory, V as an MN-major operand
 // Warp 4 issues the products, S two blocks ahead of P . V; warps 5 and 6 request the pages of K and V; warp 7 looks ahead: it finds the next piece of work, collects
 // the ancestors of its nodes and requests its queries as soon as the products that read the last ones are complete.
@@ -15,8 +16,13 @@
 // beside its keys; every group of CTAs (one, or two for trees of more rows than a tile has, which then share the keys through L2) takes the same number of consecutive
 // units, whatever the trees' lengths. Where an item is cut, its parts are counted in warp by warp (a warp has the same rows in all of them): the last warp to finish waits until
 // the others' sums are in scratch and joins them with its own, four at a time, in the order of the keys, and such joins are joined again. Few items have many parts each: those a
-// second kernel joins. So the result depends on the call alone, not on who was last. Where contexts are short (kSmall) a cluster of up to eight CTAs takes a (tree, kv head, row tile), a share of its keys each, and joins through
-// distributed shared memory: nothing has to be added up or looked for in front.
+// second kernel joins. So the result depends on the call alone, not on who was last. Where contexts are short (kSmall) a cluster of up to eight CTAs takes a (tree, kv head, row
+// tile), a share of its keys each, and joins through distributed shared memory: nothing has to be added up or looked for in front.
+//
+// What bounds it, 32 / 8 heads: 64 trees of 32 nodes at 512 to 8192 tokens 207 - 217 us for the 1.18 GB of the cache (181 at the rate of a copy), two trees at 100003 and 131072
+// 161 us (145), both HBM and the joins at the end. Where rows share keys (six trees of 250 nodes at 700 to 4000, 16 / 2 heads, 62 to 80 us) the softmax warps: about 1800 cycles a block
+// and CTA, of which 64 exponentials a thread, four lanes a cycle and scheduler, take 1024 for the two warps that a scheduler has. One tree of 26 nodes at 1500 tokens 12.6 us, a
+// chain of latencies: tree, table, pages, three blocks of the CTA's share, and the cluster's join. Two threads to a row took 284 us where one takes 207 (a barrier every block).
 // Every wait is bounded: on a timeout code 3 goes to the status word, the roles leave their loops, tensor memory is freed.
 #include "draft_tree.cuh"
 #include "umma_common.cuh"
@@ -522,7 +528,11 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
             if (i == 0) ask();
             const TreeSpan& span = walk.piece.span;
             if (walk.s != tree) {
-                for (int k = lane; k < span.nodes; k += 32) s_up[k] = tree_parent(p.t, span, k, p.status);
+                int up[kWords];   // (asked for together)
+#pragma unroll
+                for (int j = 0; j < kWords; ++j) up[j] = 32 * j + lane < span.nodes ? p.t.parent[span.row0 + 32 * j + lane] : -1;
+#pragma unroll
+                for (int j = 0; j < kWords; ++j) s_up[32 * j + lane] = tree_parent_of(up[j], 32 * j + lane, p.status);
                 tree = walk.s;
                 __syncwarp();
             }
