@@ -36,9 +36,10 @@ struct AppendParams {
 
 // A CTA per node. A thread takes two chunks of eight channels of a head: a pair that rotates together (c, c + half / 8), or two that stay. Rows, parents and the page are asked for
 // together, in front of the walk up the tree (shared reads, where global ones would wait for each other): what bounds a small call is the two trips to memory, tree and row.
-// 64 trees of 20 to 64 nodes, 32 / 8 heads: 16.2 us, 10 at the rate of a copy (with the rows behind the walk 17.5; with one task in front 18.3); one tree of 26 nodes 2.7, a launch.
-constexpr int kAhead = 2;         // tasks of a thread that are asked for in front
-__global__ void __launch_bounds__(kThreads) tree_append_kernel(const AppendParams p) {
+// 64 trees of 20 to 64 nodes, 32 / 8 heads: 14.3 us, 10 at the rate of a copy (256 threads, two tasks in front 16.2; with the rows behind
+// the walk 17.5; 64 threads 14.3); one tree of 26 nodes 2.7, a launch (64 threads 3.7).
+constexpr int kAppendThreads = 128, kAhead = 3;   // tasks of a thread that are asked for in front
+__global__ void __launch_bounds__(kAppendThreads) tree_append_kernel(const AppendParams p) {
     __shared__ int up[kMostNodes];
     pdl_launch_dependents();
     pdl_wait();
@@ -55,15 +56,17 @@ __global__ void __launch_bounds__(kThreads) tree_append_kernel(const AppendParam
     uint4 a[kAhead], b[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-        const int i = tid + j * kThreads;
+        const int i = tid + j * kAppendThreads;
         int c0, c1;
         chunks(i, &c0, &c1);
         if (i < tasks) { a[j] = src[(i >> 3) * 16 + c0]; b[j] = src[(i >> 3) * 16 + c1]; }
     }
-    const int parent = tid <= node ? tree_parent(p.t, s, tid, p.status) : -1;
+    int parent[kMostNodes / kAppendThreads];
+#pragma unroll
+    for (int j = 0; j < kMostNodes / kAppendThreads; ++j) parent[j] = tid + j * kAppendThreads <= node ? p.t.parent[s.row0 + tid + j * kAppendThreads] : -1;
     const long long place = tree_place(p.t, s.slot, s.length + node, p.status);
-    up[tid] = parent;
-    static_assert(kThreads >= kMostNodes, "a thread per node");
+#pragma unroll
+    for (int j = 0; j < kMostNodes / kAppendThreads; ++j) up[tid + j * kAppendThreads] = tree_parent_of(parent[j], tid + j * kAppendThreads, p.status);
     __syncthreads();
     int at = s.length;
     for (int i = up[node]; i >= 0; i = up[i]) ++at;   // (a parent is below its child: this ends)
@@ -101,8 +104,8 @@ __global__ void __launch_bounds__(kThreads) tree_append_kernel(const AppendParam
     };
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
-        if (tid + j * kThreads < tasks) finish(tid + j * kThreads, a[j], b[j]);
-    for (int i = tid + kAhead * kThreads; i < tasks; i += kThreads) {
+        if (tid + j * kAppendThreads < tasks) finish(tid + j * kAppendThreads, a[j], b[j]);
+    for (int i = tid + kAhead * kAppendThreads; i < tasks; i += kAppendThreads) {
         int c0, c1;
         chunks(i, &c0, &c1);
         finish(i, src[(i >> 3) * 16 + c0], src[(i >> 3) * 16 + c1]);
@@ -212,7 +215,7 @@ int gptrs_cuda_tree_append(const gptrs_draft_trees* t, const gptrs_tree_append_s
     p.q = static_cast<__nv_bfloat16*>(s->d_q);
     p.pool = static_cast<unsigned char*>(s->d_pool);
     p.status = s->d_status;
-    return launch_kernel(tree_append_kernel, dim3((unsigned)t->max_nodes, (unsigned)t->n_trees), dim3(kThreads), 0, as_stream(stream), 1, p);
+    return launch_kernel(tree_append_kernel, dim3((unsigned)t->max_nodes, (unsigned)t->n_trees), dim3(kAppendThreads), 0, as_stream(stream), 1, p);
 }
 
 int gptrs_cuda_tree_accept(const gptrs_draft_trees* t, const gptrs_tree_accept_step* s, void* stream) {
