@@ -47,7 +47,10 @@ constexpr size_t kSmem = 200 * 1024 + 1024;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kJoinThreads = 256;
 
-struct __align__(32) Part { float m, l, best, z; int token; float given; float pad[2]; };   // of a row and a stretch: sum exp z = l exp m, the best token (-1: none) and its z, the target's z (NaN: not here)
+// Of a row and a stretch: sum exp z = (1 + rest) exp m, the best token (-1: none) and its z, the target's z (NaN: not here). The largest term is apart from the others, so that what
+// is small beside it keeps its digits: a token that is nearly certain has a log-probability of about -rest.
+struct __align__(32) Part { float m, rest, best, z; int token; float given; float pad[2]; };
+__device__ __forceinline__ Part no_part() { return {-INFINITY, -1.f, -INFINITY, -INFINITY, -1, NAN}; }
 
 struct ScoreParams {
     CUtensorMap x_map, w_map;
@@ -87,7 +90,8 @@ __device__ __noinline__ float capped(float z, float cap) { return cap * tanhf(z 
 __device__ __forceinline__ void join(Part& a, const Part& b) {
     const float m = fmaxf(a.m, b.m);
     const float ref = m == -INFINITY ? 0.f : m;   // (a sum that is NaN stays one)
-    a.l = a.l * (a.m == m ? 1.f : ex2((a.m - ref) * kLog2e)) + b.l * (b.m == m ? 1.f : ex2((b.m - ref) * kLog2e));
+    const bool mine = a.m == m;
+    a.rest = (mine ? a.rest : b.rest) + (1.f + (mine ? b.rest : a.rest)) * ex2(((mine ? b.m : a.m) - ref) * kLog2e);
     a.m = m;
     if (b.token >= 0 && (a.token < 0 || b.best > a.best || (b.best == a.best && b.token < a.token))) { a.best = b.best; a.z = b.z; a.token = b.token; }
     if (b.given == b.given) a.given = b.given;
@@ -121,7 +125,7 @@ __device__ __forceinline__ void commit(uint64_t* bar) {   // to the barrier of b
 __device__ __forceinline__ Part join_lanes(Part a) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const Part b = {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.l, o), __shfl_xor_sync(0xffffffffu, a.best, o),
+        const Part b = {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.rest, o), __shfl_xor_sync(0xffffffffu, a.best, o),
                         __shfl_xor_sync(0xffffffffu, a.z, o), __shfl_xor_sync(0xffffffffu, a.token, o), __shfl_xor_sync(0xffffffffu, a.given, o)};
         join(a, b);
     }
@@ -244,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
             int target[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                a[r] = {-INFINITY, 0.f, -INFINITY, -INFINITY, -1, NAN};
+                a[r] = no_part();
                 target[r] = p.target && warp + 8 * r < p.rows ? p.target[warp + 8 * r] : -1;
             }
             for (int n0 = unit.begin; n0 < unit.end; n0 += p.cols) {
@@ -298,9 +302,10 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                         float value = z;
                         if constexpr (kSample) value = fmaf(z, p.inv_t, gumbel(draw(seed, row, token)));
                         if (value > a[r].best) { a[r].best = value; a[r].z = z; a[r].token = token; }
-                        const float to = fmaxf(a[r].m, z), ref = to == -INFINITY ? 0.f : to;
-                        a[r].l = a[r].l * (a[r].m == to ? 1.f : ex2((a[r].m - ref) * kLog2e)) + ex2((z - ref) * kLog2e);
-                        a[r].m = to;
+                        const bool up = z > a[r].m;
+                        const float e = ex2((up ? a[r].m - z : z - (a[r].m == -INFINITY ? 0.f : a[r].m)) * kLog2e);
+                        a[r].rest = up ? (1.f + a[r].rest) * e : a[r].rest + e;
+                        a[r].m = up ? z : a[r].m;
                     }
                 }
                 asm volatile("bar.sync 1, %0;\n" ::"n"(kEpilogue) : "memory");
@@ -329,7 +334,8 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
             const int row = unit.row0 + in_tile;
             const bool rows = unit.row0 + (warp & 3) * 32 < p.rows;
             const int target = p.target && row < p.rows ? p.target[row] : -1;
-            Part a = {-INFINITY, 0.f, -INFINITY, -INFINITY, -1, NAN};
+            Part a = no_part();
+            float l = 0.f;                                    // sum exp(z - m), the largest term among them
             for (int n0 = unit.begin; n0 < unit.end && !failed; n0 += p.cols) {
                 const int first = n0 + half * width, some = rows ? min(half ? p.cols - width : width, unit.end - first) : 0;   // this half's tokens
                 uint64_t acc[kCols / 4];
@@ -440,10 +446,11 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                         sums[i & 1] = add2(sums[i & 1], pair_of(ex2(e.x), ex2(e.y)));
                     }
                     const float2 s = split(add2(sums[0], sums[1]));
-                    a.l = a.l * (a.m == to ? 1.f : ex2((a.m - ref) * kLog2e)) + (s.x + s.y);
+                    l = l * (a.m == to ? 1.f : ex2((a.m - ref) * kLog2e)) + (s.x + s.y);
                     a.m = to;
                 }
             }
+            a.rest = l - 1.f;
             if (row < p.rows && !failed) p.parts[(size_t)row * p.row_parts + 2 * (u / p.row_tiles) + half] = a;
         }
         if (failed && lane == 0) atomicExch(p.status, 3);
@@ -464,11 +471,11 @@ __global__ void __launch_bounds__(kJoinThreads) vocab_join_kernel(const __grid_c
     const int row = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31, n = p.row_parts;
     if (row >= p.rows) return;
     const Part* parts = p.parts + (size_t)row * n;
-    Part a = {-INFINITY, 0.f, -INFINITY, -INFINITY, -1, NAN};
+    Part a = no_part();
     for (int i = lane; i < n; i += 32) join(a, parts[i]);
     a = join_lanes(a);
     if (lane) return;
-    const float lse = a.m + logf(a.l);
+    const float lse = a.m + log1pf(a.rest);
     if (p.lse) p.lse[row] = lse;
     if (p.pick) p.pick[row] = max(a.token, 0);   // (nothing compares with NaN: the first token)
     if (p.pick_logprob) p.pick_logprob[row] = a.z - lse;
