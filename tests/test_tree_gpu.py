@@ -381,6 +381,66 @@ def test_attention_of_trees_that_change_in_place(cuda):
     assert int(t.status) == 0
 
 
+@pytest.mark.parametrize("wide", [1, 4000])
+@pytest.mark.parametrize("heads,kv", [(2, 1), (32, 1), (12, 3)])
+def test_as_many_trees_as_a_call_may_have(cuda, heads, kv, wide):
+    """A few trees among 65535, the others padding or without nodes, under a narrow and a wide page table: the same as by themselves, within roundings."""
+    rng = np.random.default_rng(heads)
+    t = Trees(cuda, heads, kv, [(150, bushy(20, rng)), (0, bushy(3, rng)), (60, bushy(11, rng))], seed=1)
+    q, n, at = t.queries(), 65535, np.array([0, 40000, 65534])
+    table = torch.full((t.table.shape[0], max(wide, t.table.shape[1])), -1, dtype=torch.int32, device=cuda)
+    table[:, :t.table.shape[1]] = t.table
+    first = np.zeros(n + 1, dtype=np.int64)
+    for k, a in enumerate(at):
+        first[a + 1:] = t.row0[k + 1]
+    slot, length = np.full(n, -1), np.full(n, -5)
+    slot[1::7], length[1::7] = t.slots[0], 33                              # of no nodes
+    slot[at], length[at] = t.slots, [150, 0, 60]
+    many = ops.DraftTrees(heads, kv, _ints(first, cuda), _ints(slot, cuda), _ints(length, cuda), t.parent, table, t.max_nodes)
+    t.check(ops.tree_attention(many, q, t.pool, status=t.status), q)
+    token, pick = _ints(rng.integers(0, 3, t.rows), cuda), _ints(rng.integers(0, 3, t.rows), cuda)
+    got, alone = ops.tree_accept(many, token, pick, status=t.status), ops.tree_accept(t.trees, token, pick, status=t.status)
+    for a, b in zip(got, alone):
+        assert a[torch.as_tensor(at, device=cuda)].equal(b)
+    rest = torch.ones(n, dtype=torch.bool, device=cuda)
+    rest[torch.as_tensor(at, device=cuda)] = False
+    assert (got.count[rest] == 0).all() and (got.next[rest] == -1).all() and (got.path[rest] == -1).all() and got.length[rest].equal(many.tensors["length"][rest])
+    assert int(t.status) == 0
+
+
+def test_a_captured_step_reads_its_trees_when_it_runs(cuda):
+    """Append, attention and acceptance of one layer in a graph, replayed with other lengths and parents: as eager calls on the same pool."""
+    rng = np.random.default_rng(23)
+    t = Trees(cuda, 8, 2, [(300, bushy(20, rng)), (45, bushy(13, rng))], seed=8)
+    qkv = torch.randn((t.rows, 12 * DIM), device=cuda).bfloat16()
+    cos, sin = (torch.randn((400, 64), device=cuda) for _ in range(2))
+    token, pick = _ints(rng.integers(0, 3, t.rows), cuda), _ints(rng.integers(0, 3, t.rows), cuda)
+    start = t.pool.clone()
+    append = ops.TreeAppend(t.trees, qkv, cos, sin, t.pool, status=t.status)
+    attend = ops.TreeAttention(t.trees, append.q, t.pool, status=t.status)
+    accept = ops.TreeAccept(t.trees, token, pick, [t.pool], status=t.status)
+    for call in (append, attend, accept):
+        call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        append()
+        out = attend()
+        told = accept()
+    for step in range(3):
+        t.parent[:] = _ints(bushy(20, rng) + bushy(13, rng), cuda)
+        t.length[:] = _ints([300 - 50 * step, 45 - 20 * step], cuda)
+        t.pool.copy_(start)
+        graph.replay()
+        got, pool = [out.clone(), *(x.clone() for x in told)], t.pool.clone()
+        t.pool.copy_(start)
+        want = [append() is None or attend().clone(), *(x.clone() for x in accept())]
+        for a, b in zip(got, want):
+            assert a.equal(b)
+        assert pool.equal(t.pool)
+    assert int(t.status) == 0
+
+
 # ---- append --------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("heads,kv,rotary", [(32, 8, 128), (8, 1, 64), (12, 12, 16), (5, 1, 96), (3, 3, 0), (14, 2, 112)])
 def test_append(cuda, heads, kv, rotary):
