@@ -213,6 +213,11 @@ __device__ __forceinline__ float4 load_now(const float4* at) {
     asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(at) : "memory");
     return v;
 }
+// A part of a row has (m, l): its reference and its sum, or, where no score is above -inf, m = -inf and l = 0 (nothing is seen), 1 (scores of -inf) or NaN (some are NaN). Keys whose
+// scores are -inf weigh nothing beside finite ones of other parts; whether a row has none is known where all of its parts meet.
+// What a part adds to the sum of parts whose largest reference is top; f = 2^(m - that).
+__device__ __forceinline__ float share_of(float2 ml, float f, float top) { return ml.x == -INFINITY ? (top == -INFINITY ? ml.y : ml.y * 0.f) : ml.y * f; }
+__device__ __forceinline__ float inverse_of(float top, float sum) { return top == -INFINITY ? (sum == 0.f ? 0.f : NAN) : 1.f / sum; }
 __device__ __forceinline__ void store_part(const AttentionParams& p, size_t slot, bool live, uint32_t t_o, float m, float l) {
     float4* to = p.sums + slot * 32 * p.row_cap + threadIdx.x;
 #pragma unroll 1
@@ -280,9 +285,9 @@ __device__ __forceinline__ bool join_parts(const AttentionParams& p, const Piece
 #pragma unroll
             for (int k = 0; k < kJoin; ++k) {
                 f[k] = ex2(ml[k].x - ref);
-                sum += ml[k].x == -INFINITY ? ml[k].y : ml[k].y * f[k];   // (without a score 0, or NaN)
+                sum += share_of(ml[k], f[k], top);
             }
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const float inv = inverse_of(top, sum);
             float4* to = p.sums + slot(first * apart) * 32 * p.row_cap + tid;
             const int cap = p.row_cap;
 #pragma unroll 1
@@ -809,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
             if (failed || !wait(&v_empty[(g - 1) & 1], (uint32_t)((g - 1) >> 1))) break;
             tc_fence_after();
             if (!idle) {
-                if (any && m == -INFINITY) l = NAN;             // scores of -inf alone
+                if (any && m == -INFINITY && l == 0.f) l = 1.f;  // scores of -inf alone
                 uint32_t odd = 0;
                 if (masked) {   // (the wait is over: it orders what the values' warp has found before the reads)
                     if (!wait(&p_full[(g - 1) & 1], (uint32_t)((g - 1) >> 1))) break;
@@ -844,7 +849,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
                 if (kSmall && p.cluster > 1) {                  // (the share's sums go to the other CTAs, see below)
                     if (live) s_ml[kSmall ? tid : 0] = make_float2(m, l);
                 } else if (piece.parts == 1) {
-                    const float inv = any ? 1.f / l : 0.f;
+                    const float inv = inverse_of(m, l);
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
                         float o[32];
@@ -913,12 +918,12 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
             const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
+                if (ml[k].x == -INFINITY && ml[k].y == 0.f) continue;   // (a share without keys has no sums)
                 const float f = ex2(ml[k].x - ref);
-                if (ml[k].x == -INFINITY) { l += ml[k].y; continue; }   // (without a score 0, or NaN)
-                l += ml[k].y * f;
+                l += share_of(ml[k], f, top);
                 if (k < p.cluster) { o.x += v[k].x * f; o.y += v[k].y * f; o.z += v[k].z * f; o.w += v[k].w * f; }
             }
-            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const float inv = inverse_of(top, l);
             const int node = row / p.t.group;
             *reinterpret_cast<uint2*>(p.out + ((long long)(span.row0 + node0 + node) * p.t.q_heads + only.head * p.t.group + (row - node * p.t.group)) * kTreeDim + 4 * lane) =
                 make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
@@ -976,19 +981,19 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
                 if (k0 + k >= item.parts) ml[k] = make_float2(-INFINITY, 0.f);
                 to = fmaxf(to, ml[k].x);
             }
-            const float ref = to == -INFINITY ? 0.f : to, keep = ex2(top - ref);   // (top -inf: nothing yet, 0)
+            const float ref = to == -INFINITY ? 0.f : to, keep = to == top ? 1.f : ex2(top - ref);
+            l = share_of(make_float2(top, l), keep, to);
             top = to;
-            l = l == 0.f ? 0.f : l * keep;
             o.x *= keep; o.y *= keep; o.z *= keep; o.w *= keep;
 #pragma unroll
             for (int k = 0; k < kAtOnce; ++k) {
                 if (k0 + k >= item.parts) break;
                 const float f = ex2(ml[k].x - ref);
-                l += ml[k].x == -INFINITY ? ml[k].y : ml[k].y * f;   // (without a score 0, or NaN)
+                l += share_of(ml[k], f, to);
                 o.x += v[k].x * f; o.y += v[k].y * f; o.z += v[k].z * f; o.w += v[k].w * f;
             }
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = inverse_of(top, l);
         *reinterpret_cast<uint2*>(&s_out[lane][4 * warp]) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
         __syncthreads();
         const int r = threadIdx.x >> 2, rr = row - lane + r, chunk = 8 * (threadIdx.x & 3);

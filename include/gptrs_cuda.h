@@ -849,7 +849,8 @@ typedef struct {
     int32_t* d_status;
 } gptrs_tree_append_step;
 int gptrs_cuda_tree_append(const gptrs_draft_trees* t, const gptrs_tree_append_step* s, void* stream);
-/* out [rows][q_heads][dim] (bf16) = softmax over what the node sees . values. A node that sees nothing (its pages are out of range) gives zeros. Keys and values of nodes
+/* out [rows][q_heads][dim] (bf16) = softmax over what the node sees . values. A node that sees nothing (its pages are out of range) gives zeros. Scores of -inf weigh nothing beside
+ * finite ones; a row that has no others is NaN. Keys and values of nodes
  * that a node does not see do not touch it, whatever they are. Scratch: gptrs_cuda_tree_scratch_bytes (0: none), 16-byte aligned, all zero before its
  * first call and after one that left 3 in *d_status; of one call at a time (calls and graphs that may overlap have their own), and of calls with the same heads, max_nodes,
  * n_trees and max_pages: others have their own, or zero it. */

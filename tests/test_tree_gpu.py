@@ -337,6 +337,33 @@ def test_attention_however_it_is_cut(cuda, heads, kv, trees, nodes, lengths):
         assert other().equal(got)
 
 
+# (length of the first tree, of the others): clusters of eight (a node alone in its part, and many blocks to a part), several tiles, whole items, joins by warps at one level and at several,
+# with one tile and two, the second kernel.
+MINUS_INFINITY = [(4, 2, 1, 1, (64, 0)), (4, 2, 1, 1, (63, 0)), (4, 2, 3, 20, (1400, 1300)), (4, 1, 2, 256, (1000, 900)), (8, 8, 30, 6, (3000, 2900)), (4, 4, 60, 11, (9000, 8000)),
+                  (2, 1, 80, 3, (20000, 300)), (16, 2, 20, 60, (5000, 3000)), (2, 1, 1, 3, (30000, 0))]
+
+
+@pytest.mark.parametrize("finite", ["context", "first", "middle", "root", "none"])
+@pytest.mark.parametrize("heads,kv,trees,nodes,lengths", MINUS_INFINITY)
+def test_attention_parts_whose_scores_are_all_minus_infinity(cuda, heads, kv, trees, nodes, lengths, finite):
+    """Keys that make scores of -inf have weight 0 beside finite ones, whichever of a call's parts they are in; where a row sees no others it is NaN."""
+    rng = np.random.default_rng(nodes)
+    t = Trees(cuda, heads, kv, [(lengths[min(s, 1)], bushy(nodes, rng)) for s in range(trees)], seed=lengths[0])
+    q = t.queries()
+    q[..., 3] = q[..., 3].abs() + 0.5
+    for s, (n, _) in enumerate(t.forest):
+        keep = {"context": slice(0, n), "first": 0, "middle": n // 2, "root": n, "none": slice(0, 0)}[finite]
+        keys = t.kvs[s][0].copy()
+        t.kvs[s][0, ..., 3] = -np.inf
+        t.kvs[s][0, keep] = keys[keep]
+        t.write(s, np.arange(t.kvs[s].shape[1]), torch.tensor(t.kvs[s], dtype=torch.float32).bfloat16())
+    got = t.attention(q)
+    if finite == "none":
+        assert got.isnan().all()
+    else:
+        t.check(got, q)
+
+
 def test_attention_shares_scratch_with_calls_of_its_shape_alone(cuda):
     rng = np.random.default_rng(2)
     a, b = (Trees(cuda, 4, 2, [(9000, bushy(5, rng))] * n, seed=1) for n in (1, 2))
