@@ -4,9 +4,10 @@
 // tcgen05 products: a CTA holds a tile of 128 rows and walks over keys in blocks of 64 (four pages), two CTAs to an SM:
 //   S[128 x 64] = Q . K^T      both from shared memory (K-major, 128-byte swizzle, which is how the pool holds a page), two accumulators in tensor memory
 //   softmax                    warps 0 - 3, a thread per row, one pass over its scores: the reference stays until a block's weights add up to more than 2^14, so there is
-//                              no pass for the maximum but in a row's first block; weights go as bf16 over S (values are bf16, and a product has one type: results
-//                              are off by 0.0023 of their size, by 0.0017 with f32 weights, which is the result's own rounding)
-//   O[128 x 128] += P . V      P from tensor memory, V as an MN-major operand
+//                              no pass for the maximum but in a row's first block; weights go over S as two bf16 terms each, since values are bf16 and a product has one
+//                              type. With one term results were off by 0.0023 of their size, with two by 0.0017, which is their own rounding; it costs twice the
+//                              products of P . V and two conversions a weight (64 trees 211 -> 236 us, two long ones 162 -> 175, six wide ones 70 -> 75)
+//   O[128 x 128] += P . V      P's two terms from tensor memory, V as an MN-major operand
 // Warp 4 issues the products, S two blocks ahead of P . V; warps 5 and 6 request the pages of K and V; warp 7 looks ahead: it finds the next piece of work, collects
 // the ancestors of its nodes and requests its queries as soon as the products that read the last ones are complete.
 // Blocks that reach behind the sequence's tokens are masked by a bit per node. In them values of nodes that are not finite are taken out of the stage by warp 6
@@ -19,10 +20,11 @@
 // second kernel joins. So the result depends on the call alone, not on who was last. Where contexts are short (kSmall) a cluster of up to eight CTAs takes a (tree, kv head, row
 // tile), a share of its keys each, and joins through distributed shared memory: nothing has to be added up or looked for in front.
 //
-// What bounds it, 32 / 8 heads: 64 trees of 32 nodes at 512 to 8192 tokens 207 - 217 us for the 1.18 GB of the cache (181 at the rate of a copy), two trees at 100003 and 131072
-// 161 us (145), both HBM and the joins at the end. Where rows share keys (six trees of 250 nodes at 700 to 4000, 16 / 2 heads, 62 to 80 us) the softmax warps: about 1800 cycles a block
-// and CTA, of which 64 exponentials a thread, four lanes a cycle and scheduler, take 1024 for the two warps that a scheduler has. One tree of 26 nodes at 1500 tokens 12.6 us, a
-// chain of latencies: tree, table, pages, three blocks of the CTA's share, and the cluster's join. Two threads to a row took 284 us where one takes 207 (a barrier every block).
+// What bounds it (times of the kernels in a graph; calls from Python take 2 to 50 us more), 32 / 8 heads: 64 trees of 32 nodes at 512 to 8192 tokens 236 us for the 1.18 GB of the
+// cache (181 at the rate of a copy), two trees at 100003 and 131072 175 us (145): HBM, the wait for the products in front of a stage's reuse, and the joins at the end. Where rows share
+// keys (six trees of 250 nodes at 700 to 4000, 16 / 2 heads, 75 to 80 us) the softmax warps: 64 exponentials a thread and block, four lanes a cycle and scheduler, take 1024 cycles
+// for the two warps that a scheduler has. One tree of 26 nodes at 1500 tokens 13.0 us, a chain of latencies: tree, table, pages, three blocks of the CTA's share, and
+// the cluster's join. Two threads to a row took 284 us where one took 207 (a barrier every block).
 // Every wait is bounded: on a timeout code 3 goes to the status word, the roles leave their loops, tensor memory is freed.
 #include "draft_tree.cuh"
 #include "umma_common.cuh"
@@ -676,8 +678,9 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
                 tc_fence_after();
                 const uint64_t b = make_smem_desc_mn(sV + (g & 1) * kStage);
 #pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k)
-                    umma_bf16_ts(tmem + kOCol, tmem + (uint32_t)(g & 1) * kKeys + 8u * k, b + (uint64_t)(k * (16 * 128 >> 4)), kIdescO, (!begins || k > 0) ? 1u : 0u);
+                for (int k = 0; k < kKeys / 8; ++k)   // 16 keys: the weights' upper terms, and their lower ones
+                    umma_bf16_ts(tmem + kOCol, tmem + (uint32_t)(g & 1) * kKeys + (k & 1) * (kKeys / 2) + 8u * (k >> 1), b + (uint64_t)((k >> 1) * (16 * 128 >> 4)), kIdescO,
+                                 (!begins || k > 0) ? 1u : 0u);
                 umma_commit(&v_empty[g & 1]);
                 --left;
                 if (more) scores();
@@ -728,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
                     any |= (vis[0] | vis[1]) != 0;
                     float sum = 0.f;
                     for (bool look = live && m == -INFINITY;;) {
-                        uint32_t sr[kKeys];
+                        uint32_t sr[kKeys], low[kKeys / 2];
                         if (fresh) {   // a new reference for some rows: the maximum of this block
                             tmem_ld_32_begin(t_s, sr);
                             tmem_ld_32_begin(t_s + 32, sr + 32);
@@ -789,7 +792,10 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
                             for (int i = 0; i < 16; ++i) {
                                 const float w0 = ex2(__uint_as_float(x[2 * i])), w1 = ex2(__uint_as_float(x[2 * i + 1]));
                                 sums[i & 1] = add2(sums[i & 1], pair_of(w0, w1));
-                                sr[16 * h + i] = pack_bf16x2(w0, w1);   // (the places of scores that are done with)
+                                const uint32_t high = pack_bf16x2(w0, w1);
+                                const float2 rest = split(fma2(pair_of(__uint_as_float(high << 16), __uint_as_float(high & 0xffff0000u)), pair_of(-1.f, -1.f), pair_of(w0, w1)));
+                                sr[16 * h + i] = high;   // (the places of scores that are done with)
+                                low[16 * h + i] = pack_bf16x2(rest.x, rest.y);
                             }
                         }
                         const float2 s01 = split(add2(sums[0], sums[1]));
@@ -798,6 +804,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
                         if (!__any_sync(0xffffffffu, look)) {
                             tmem_st_16(t_s, sr);
                             tmem_st_16(t_s + 16, sr + 16);
+                            tmem_st_16(t_s + 32, low);
+                            tmem_st_16(t_s + 48, low + 16);
                             break;
                         }
                         fresh = true;
