@@ -336,7 +336,6 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
             const bool rows = unit.row0 + (warp & 3) * 32 < p.rows;
             const int target = p.target && row < p.rows ? p.target[row] : -1;
             Part a = no_part();
-            float l = 0.f;                                    // sum exp(z - m), the largest term among them
             for (int n0 = unit.begin; n0 < unit.end && !failed; n0 += p.cols) {
                 const int first = n0 + half * width, some = rows ? min(half ? p.cols - width : width, unit.end - first) : 0;   // this half's tokens
                 uint64_t acc[kCols / 4];
@@ -406,15 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
 #pragma unroll
                     for (int i = 0; i < 32; ++i) mx[i & 1] = fmaxf(mx[i & 1], z[i]);
                     const float top = fmaxf(mx[0], mx[1]);
-                    if constexpr (!kSample) {
-                        if (__any_sync(0xffffffffu, top > a.best)) {
-                            int at = 0;
-#pragma unroll
-                            for (int i = 31; i >= 0; --i)
-                                if (z[i] == top) at = i;
-                            if (top > a.best) { a.best = a.z = top; a.token = n_c + at; }
-                        }
-                    } else {
+                    if constexpr (kSample) {
                         // g <= -log v: a bound of one logarithm on the special function unit, with room for its error, keeps all but a few tokens (as many as a running maximum
                         // has steps, about) from the noise in full. Sixteen at a time, so that the best of the ones in front counts.
 #pragma unroll
@@ -437,8 +428,20 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                             }
                         }
                     }
+                    const bool up = top > a.m;
+                    if (__any_sync(0xffffffffu, up)) {   // the first of the largest: what a greedy pick takes, and what the sum of the others leaves out
+                        int at = 0;
+#pragma unroll
+                        for (int i = 31; i >= 0; --i)
+                            if (z[i] == top) at = i;
+                        if constexpr (!kSample)
+                            if (up) { a.best = a.z = top; a.token = n_c + at; }
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (up && i == at) z[i] = -INFINITY;
+                    }
                     // sum exp z: differences first, so that what is rounded is small where it counts
-                    const float to = fmaxf(a.m, top), ref = to == -INFINITY ? 0.f : to;
+                    const float to = up ? top : a.m, ref = to == -INFINITY ? 0.f : to;
                     const uint64_t ref2 = pair_of(-ref, -ref), log2 = pair_of(kLog2e, kLog2e);
                     uint64_t sums[2] = {0, 0};
 #pragma unroll
@@ -447,11 +450,10 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                         sums[i & 1] = add2(sums[i & 1], pair_of(ex2(e.x), ex2(e.y)));
                     }
                     const float2 s = split(add2(sums[0], sums[1]));
-                    l = l * (a.m == to ? 1.f : ex2((a.m - ref) * kLog2e)) + (s.x + s.y);
+                    a.rest = (up ? (1.f + a.rest) * ex2((a.m - ref) * kLog2e) : a.rest) + (s.x + s.y);
                     a.m = to;
                 }
             }
-            a.rest = l - 1.f;
             if (row < p.rows && !failed) p.parts[(size_t)row * p.row_parts + 2 * (u / p.row_tiles) + half] = a;
         }
         if (failed && lane == 0) atomicExch(p.status, 3);
@@ -476,14 +478,15 @@ __global__ void __launch_bounds__(kJoinThreads) vocab_join_kernel(const __grid_c
     for (int i = lane; i < n; i += 32) join(a, parts[i]);
     a = join_lanes(a);
     if (lane) return;
-    const float lse = a.m + log1pf(a.rest);
-    if (p.lse) p.lse[row] = lse;
+    // Log-probabilities from the difference to the largest logit, not to lse: rounded to f32 that is off by more than a token that is nearly certain has.
+    const float others = log1pf(a.rest);
+    if (p.lse) p.lse[row] = a.m + others;
     if (p.pick) p.pick[row] = max(a.token, 0);   // (nothing compares with NaN: the first token)
-    if (p.pick_logprob) p.pick_logprob[row] = a.z - lse;
+    if (p.pick_logprob) p.pick_logprob[row] = a.z - a.m - others;
     if (p.logprob) {
         const int target = p.target[row];
         if (target >= p.vocab) atomicExch(p.status, 2);
-        p.logprob[row] = target < 0 ? 0.f : a.given - lse;
+        p.logprob[row] = target < 0 ? 0.f : a.given - a.m - others;
     }
 }
 

@@ -230,6 +230,31 @@ def test_waits_that_run_out(cuda, rows):
     assert int(status) == 0
 
 
+@pytest.mark.parametrize("temperature", [0.0, 0.8])
+@pytest.mark.parametrize("rows", [3, 16, 100, 300])
+def test_tokens_that_are_nearly_certain_keep_their_digits(cuda, rows, temperature):
+    """One token of a row has all but 1e-7 to 1e-4 of the probability, lse is about 20. log p = z - m - log1p(rest), rest the sum of the others' exp(z - m): differences of logits are off by 2 e,
+    an exponential's argument (below 32) by two roundings, and the exponential itself by 2^-21, all of it relative to rest / (1 + rest) = 1 - p. The last two steps round the result."""
+    rng = np.random.default_rng(rows)
+    dim, vocab = 512, 1200
+    x, w = rng.normal(0, 1, (rows, dim)), rng.normal(0, dim ** -0.5, (vocab, dim))
+    sure, size = rng.permutation(vocab)[:rows], np.log(vocab * np.exp(0.5)) - rng.uniform(np.log(1e-7), np.log(1e-4), rows)
+    w[sure] = x * (size / (x * x).sum(-1))[:, None]
+    x, w = (torch.tensor(v, dtype=torch.float32).bfloat16().to(cuda) for v in (x, w))
+    target = np.where(rng.random(rows) < 0.5, sure, rng.integers(0, vocab, rows))
+    got = ops.vocab_scores(x, w, target=torch.tensor(target, dtype=torch.int32, device=cuda), temperature=temperature, seed=9)
+    z, mass = tr.logits(_np(x), _np(w))
+    e = ((dim / 16 + 8) * 2 ** -23 * mass).max(-1)
+    assert (z.argmax(-1) == sure).all()
+    for lp, at in ((got.logprob, target), (got.pick_logprob, got.pick.cpu().numpy())):
+        apart = np.exp(z - z[np.arange(rows), at][:, None])
+        apart[np.arange(rows), at] = 0
+        rest = apart.sum(-1)
+        want, others = -np.log1p(rest), rest / (1 + rest)
+        assert (np.abs(_np(lp) - want) <= others * (2 * e + 2 ** -20 + 32 * 2 ** -23) + 2 ** -22 * np.abs(want)).all()
+    assert (got.pick.cpu().numpy() == sure).mean() > 0.9
+
+
 @pytest.mark.parametrize("rows,vocab", [(2, 30), (17, 33), (128, 4096), (129, 100), (700, 12345), (1300, 64), (2500, 999)])
 def test_however_it_is_cut(cuda, rows, vocab):
     rng, x, w = _inputs(cuda, rows, 80, vocab, seed=rows)
