@@ -524,6 +524,25 @@ int encode(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+using Kernel = void (*)(ScoreParams);
+constexpr Kernel kKernels[3][2] = {{vocab_scores_kernel<kFew, false>, vocab_scores_kernel<kFew, true>},
+                                   {vocab_scores_kernel<kOne, false>, vocab_scores_kernel<kOne, true>},
+                                   {vocab_scores_kernel<kPairs, false>, vocab_scores_kernel<kPairs, true>}};
+
+// A kernel compiled for fewer registers than its groups ask for would wait for them without end: none is launched then.
+int registers_to_share() {
+    static const int regs = [] {   // a thread's; of a kernel that has others, or none that are known
+        for (int i = 0; i < 6; ++i) {
+            cudaFuncAttributes attr;
+            const int found = cudaFuncGetAttributes(&attr, kKernels[i / 2][i & 1]) == cudaSuccess ? attr.numRegs : 0;
+            if (found != kLaunchRegs) return found;
+        }
+        return kLaunchRegs;
+    }();
+    if (regs != kLaunchRegs) return fail(GPTRS_EXECUTION, "vocab_scores_kernel has " + std::to_string(regs) + " registers a thread, not those that its warps share out");
+    return GPTRS_OK;
+}
+
 }  // namespace
 }  // namespace gptrs
 
@@ -552,13 +571,15 @@ int gptrs_cuda_vocab_scores(const gptrs_vocab_scores* s, void* stream) {
     GPTRS_REQUIRE(!s->d_logprob || s->d_target, "log-probabilities of targets need targets");
     GPTRS_REQUIRE(s->rows == 0 || (s->d_scratch && s->scratch_bytes >= gptrs_cuda_vocab_scores_scratch_bytes(s)), "scratch is too small");
     if (s->rows == 0) return GPTRS_OK;
+    int rc = registers_to_share();
+    if (rc) return rc;
     const Cut c = cut(s->rows, s->vocab);
     const bool pair = c.mode == kPairs;
     p.row_parts = c.mode == kFew ? c.stretches : 2 * c.stretches;
     p.stages = (int)std::min<int64_t>(kMostStages, (int64_t)(kSmem - 1024) / stage_bytes(c.mode, c.cols));
     p.row_tiles = c.row_tiles; p.stretches = c.stretches; p.tiles = c.tiles; p.cols = c.cols;
     p.x_rows = s->rows < kRows ? (int)(s->rows + 7) / 8 * 8 : kRows;   // (rows that nobody has are not read out: whatever lies there)
-    int rc = encode(&p.x_map, s->d_hidden, s->dim, s->rows, ldx, p.x_rows);
+    rc = encode(&p.x_map, s->d_hidden, s->dim, s->rows, ldx, p.x_rows);
     if (!rc) rc = encode(&p.w_map, s->d_weight, s->dim, s->vocab, ldw, pair ? c.cols / 2 : c.cols);
     if (rc) return rc;
     p.bias = s->d_bias; p.seed_at = s->d_seed; p.target = s->d_target;
@@ -567,16 +588,13 @@ int gptrs_cuda_vocab_scores(const gptrs_vocab_scores* s, void* stream) {
     p.rows = (int)s->rows; p.dim = (int)s->dim; p.vocab = (int)s->vocab;
     p.cap = s->soft_cap; p.inv_t = s->temperature > 0.f ? 1.f / s->temperature : 0.f; p.seed = s->seed;
     prefill_tc_fault(&p.starve, &p.wait_limit);
-    void (*kerns[3][2])(ScoreParams) = {{vocab_scores_kernel<kFew, false>, vocab_scores_kernel<kFew, true>},
-                                        {vocab_scores_kernel<kOne, false>, vocab_scores_kernel<kOne, true>},
-                                        {vocab_scores_kernel<kPairs, false>, vocab_scores_kernel<kPairs, true>}};
     static PerDeviceOnce attr_once;
     if (attr_once.first_time())
-        for (int i = 0; i < 6; ++i) GPTRS_CUDA_OK(cudaFuncSetAttribute(kerns[i / 2][i & 1], cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
+        for (int i = 0; i < 6; ++i) GPTRS_CUDA_OK(cudaFuncSetAttribute(kKernels[i / 2][i & 1], cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
     const int64_t units = (int64_t)p.row_tiles * p.stretches, places = pair ? sm_count() / 2 : sm_count();
     // (a CTA counts its stages in 32 bits)
     GPTRS_REQUIRE(units < ((int64_t)1 << 30) && (units / places + 1) * p.tiles * ceil_div(p.dim, kStageDim) < ((int64_t)1 << 31), "too many rows for one call");
-    rc = launch_kernel(kerns[c.mode][p.inv_t > 0.f], dim3((unsigned)((units < places ? units : places) * (pair ? 2 : 1))), dim3(kThreads), kSmem, as_stream(stream), 1, p,
+    rc = launch_kernel(kKernels[c.mode][p.inv_t > 0.f], dim3((unsigned)((units < places ? units : places) * (pair ? 2 : 1))), dim3(kThreads), kSmem, as_stream(stream), 1, p,
                        pair ? 2 : 1);
     if (rc) return rc;
     // the second kernel waits for the first one itself (griddepcontrol.wait), so it may be launched ahead of its end

@@ -94,6 +94,15 @@ def test_scores_without_rows_do_nothing():
     assert gptrs_b200.lib().gptrs_cuda_vocab_scores(ctypes.byref(_scores(rows=0, d_hidden=None)), None) == OK
 
 
+@pytest.mark.skipif(torch.cuda.is_available(), reason="what a call does where kernels cannot be asked for their registers")
+def test_scores_are_not_launched_before_their_registers_are_known():
+    """The kernel's warps share out the registers that it was compiled for, and would wait without end for more than there are."""
+    lib = gptrs_b200.lib()
+    for rows in (4, 100, 300):
+        assert lib.gptrs_cuda_vocab_scores(ctypes.byref(_scores(rows=rows)), None) not in (OK, REFUSED)
+        assert b"registers" in lib.gptrs_cuda_last_error()
+
+
 def test_python_checks_its_tensors():
     ints = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
     table = torch.zeros((2, 4), dtype=torch.int32)
