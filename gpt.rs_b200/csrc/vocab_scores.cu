@@ -406,15 +406,17 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                     for (int i = 0; i < 32; ++i) mx[i & 1] = fmaxf(mx[i & 1], z[i]);
                     const float top = fmaxf(mx[0], mx[1]);
                     if constexpr (kSample) {
-                        // g <= -log v: a bound of one logarithm on the special function unit, with room for its error, keeps all but a few tokens (as many as a running maximum
-                        // has steps, about) from the noise in full. Sixteen at a time, so that the best of the ones in front counts.
+                        // g <= -log v: a bound of one logarithm on the special function unit keeps all but a few tokens (as many as a running maximum has steps, about) from the
+                        // noise in full. Sixteen at a time, so that the best of the ones in front counts. Room for the bound's errors: the logarithm's, and five roundings of
+                        // numbers as large as z / T, which the value and the best are too wherever a token comes near the best, so that theirs is the size that counts.
 #pragma unroll
                         for (int d = 0; d < 32; d += 16) {
                             uint32_t may = 0;
+                            const float near = a.best - fmaf(fabsf(a.best), 0x1p-21f, 1e-3f);
 #pragma unroll
                             for (int i = 0; i < 16; ++i) {
                                 const float low = __uint_as_float((draw(seed, row, n_c + d + i) >> 9) | 0x3f800000u) - 1.f;   // v from below
-                                if (fmaf(lg2(low), -kLn2, z[d + i] * p.inv_t) + 1e-3f > a.best) may |= 1u << i;
+                                if (fmaf(lg2(low), -kLn2, z[d + i] * p.inv_t) > near) may |= 1u << i;
                             }
                             if (some_c - d < 16) may &= (1u << max(some_c - d, 0)) - 1u;
                             while (may) {

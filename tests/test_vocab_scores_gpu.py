@@ -255,6 +255,19 @@ def test_tokens_that_are_nearly_certain_keep_their_digits(cuda, rows, temperatur
     assert (got.pick.cpu().numpy() == sure).mean() > 0.9
 
 
+@pytest.mark.parametrize("temperature,logit", [(0.3, 21.25), (1.3e-3, 21.25), (1.7e-6, 17.625), (1.1e-6, 21.25), (7e-7, 17.625), (1e-12, 3.296875)])
+def test_draws_do_not_depend_on_how_many_rows_a_call_has(cuda, temperature, logit):
+    """Logits without an error, most of them equal. At a small temperature z / T is so large that the noise is worth a few steps of f32: the value z / T + g is rounded alike whichever way a call
+    goes, and the first of the largest is taken."""
+    x, w = torch.zeros((300, 16), device=cuda).bfloat16(), torch.zeros((60000, 16), device=cuda).bfloat16()
+    x[:, 0] = 1
+    w[:, 0] = logit
+    w[::9, 0] = -5.5
+    for seed in range(60):
+        few, some, many = (ops.vocab_scores(x[:rows], w, temperature=temperature, seed=seed).pick[:16] for rows in (16, 100, 300))
+        assert few.equal(some) and few.equal(many)
+
+
 @pytest.mark.parametrize("rows,vocab", [(2, 30), (17, 33), (128, 4096), (129, 100), (700, 12345), (1300, 64), (2500, 999)])
 def test_however_it_is_cut(cuda, rows, vocab):
     rng, x, w = _inputs(cuda, rows, 80, vocab, seed=rows)
