@@ -65,7 +65,7 @@ struct ScoreParams {
     int row_tiles, stretches, tiles, cols;   // a stretch is `tiles` tiles of `cols` tokens
     int x_rows;                   // of a copy of x
     int row_parts, stages;
-    float cap, inv_t;             // inv_t 0: greedy
+    float cap, inv_t;             // cap 0: none, negative: see capped(); inv_t 0: greedy
     uint32_t seed, wait_limit;
     int starve;
 };
@@ -87,7 +87,9 @@ __device__ __forceinline__ float lg2(float x) {
 }
 // (h + 1/2 rounds to 2^32 for the last 128 of h: below 1, so that no token's value is -inf for its noise)
 __device__ __forceinline__ float gumbel(uint32_t h) { return -logf(-log1pf(-fminf(((float)h + 0.5f) * (1.f / 4294967296.f), 1.f - 0x1p-24f))); }
-__device__ __noinline__ float capped(float z, float cap) { return cap * tanhf(z / cap); }
+// cap tanh(z / cap), the same for -cap, which says that there is a bias: a token that it leaves out stays out, where the cap would make -cap of it. (A call's place is a call and no more:
+// asked for at the loop of logits, 416 draws took 438 us instead of 423 without a cap.)
+__device__ __noinline__ float capped(float z, float cap) { return cap < 0.f && z == -INFINITY ? z : cap * tanhf(z / cap); }
 __device__ __forceinline__ void join(Part& a, const Part& b) {
     const float m = fmaxf(a.m, b.m);
     const float ref = m == -INFINITY ? 0.f : m;   // (a sum that is NaN stays one)
@@ -298,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                         if (at >= p.cols || token >= unit.end) continue;
                         float z = s_z[row][at];
                         if (p.bias) z += __ldg(p.bias + token);
-                        if (p.cap > 0.f) z = capped(z, p.cap);
+                        if (p.cap != 0.f) z = capped(z, p.cap);
                         if (token == target[r]) a[r].given = z;
                         float value = z;
                         if constexpr (kSample) value = fmaf(z, p.inv_t, gumbel(draw(seed, row, token)));
@@ -387,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_scores_kernel(const __grid_
                         for (int i = 0; i < 32; ++i)
                             if (i < some_c) z[i] += __ldg(p.bias + n_c + i);
                     }
-                    if (p.cap > 0.f) {
+                    if (p.cap != 0.f) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) z[i] = capped(z[i], p.cap);
                     }
@@ -588,7 +590,7 @@ int gptrs_cuda_vocab_scores(const gptrs_vocab_scores* s, void* stream) {
     p.parts = static_cast<Part*>(s->d_scratch);
     p.pick = s->d_pick; p.pick_logprob = s->d_pick_logprob; p.logprob = s->d_logprob; p.lse = s->d_lse; p.status = s->d_status;
     p.rows = (int)s->rows; p.dim = (int)s->dim; p.vocab = (int)s->vocab;
-    p.cap = s->soft_cap; p.inv_t = s->temperature > 0.f ? 1.f / s->temperature : 0.f; p.seed = s->seed;
+    p.cap = s->d_bias ? -s->soft_cap : s->soft_cap; p.inv_t = s->temperature > 0.f ? 1.f / s->temperature : 0.f; p.seed = s->seed;
     prefill_tc_fault(&p.starve, &p.wait_limit);
     static PerDeviceOnce attr_once;
     if (attr_once.first_time())

@@ -76,7 +76,7 @@ def logits(hidden, weight, bias=None, cap=0.0):
     if bias is not None:
         z = z + np.asarray(bias, np.float64)
     if cap:
-        z = cap * np.tanh(z / cap)
+        z = np.where(np.isneginf(z), z, cap * np.tanh(z / cap))   # what a bias leaves out stays out
     return z, np.abs(x) @ np.abs(w).T
 
 

@@ -268,6 +268,21 @@ def test_draws_do_not_depend_on_how_many_rows_a_call_has(cuda, temperature, logi
         assert few.equal(some) and few.equal(many)
 
 
+@pytest.mark.parametrize("temperature", [0.0, 0.7])
+@pytest.mark.parametrize("rows", [3, 100, 300])
+def test_tokens_that_a_bias_leaves_out_stay_out_under_a_cap(cuda, rows, temperature):
+    rng, x, w = _inputs(cuda, rows, 64, 700, seed=rows)
+    bias = rng.normal(0, 1, 700)
+    bias[rng.permutation(700)[:650]] = -np.inf
+    target = rng.integers(0, 700, rows)
+    bias, t = torch.tensor(bias, dtype=torch.float32, device=cuda), torch.tensor(target, dtype=torch.int32, device=cuda)
+    got = ops.vocab_scores(x, w, target=t, bias=bias, soft_cap=3.0, temperature=temperature, seed=8)
+    _check(got, x, w, target, bias=bias, cap=3.0, temperature=temperature, seed=8)
+    assert torch.isfinite(bias[got.pick.long()]).all() and (got.logprob == -math.inf).equal(bias[t.long()] == -math.inf)
+    got = ops.vocab_scores(x, w, target=t, bias=torch.full_like(bias, -math.inf), soft_cap=3.0, temperature=temperature)
+    assert (got.lse == -math.inf).all() and (got.pick == 0).all() and got.logprob.isnan().all()
+
+
 @pytest.mark.parametrize("rows,vocab", [(2, 30), (17, 33), (128, 4096), (129, 100), (700, 12345), (1300, 64), (2500, 999)])
 def test_however_it_is_cut(cuda, rows, vocab):
     rng, x, w = _inputs(cuda, rows, 80, vocab, seed=rows)
