@@ -283,6 +283,33 @@ def test_tokens_that_a_bias_leaves_out_stay_out_under_a_cap(cuda, rows, temperat
     assert (got.lse == -math.inf).all() and (got.pick == 0).all() and got.logprob.isnan().all()
 
 
+@pytest.mark.parametrize("rows,dim,vocab", [(129, 520, 700), (140, 1024, 3001), (300, 1032, 700), (257, 2048, 999), (300, 2368, 2000), (140, 3080, 500), (300, 4104, 1500), (520, 5120, 600),
+                                            (129, 8192, 300), (100, 4104, 1500), (17, 8192, 300), (16, 5120, 600)])
+@pytest.mark.parametrize("temperature", [0.0, 0.7])
+def test_several_accumulators_to_a_tile(cuda, rows, dim, vocab, temperature):
+    """More of dim than an accumulator adds up, with a remainder and without, and the longer accumulators that draws have at a tile's beginning."""
+    rng, x, w = _inputs(cuda, rows, dim, vocab, seed=dim)
+    target = rng.integers(0, vocab, rows)
+    got = ops.vocab_scores(x, w, target=torch.tensor(target, dtype=torch.int32, device=cuda), temperature=temperature, seed=31)
+    _check(got, x, w, target, temperature=temperature, seed=31)
+
+
+def test_many_tiles_of_several_accumulators(cuda):
+    """Several row tiles and tiles of tokens to a pair of CTAs, each of several accumulators. Logits are multiples of 2^-8 that f32 holds, so they are without an error, and lse is off by its own
+    rounding and that of m, 2^-23 lse (below 32), and by the exponentials', 2^-20."""
+    rng, x, w = _inputs(cuda, 530, 2568, 60000, seed=41)
+    x, w = (x * 4).round() / 4, (w * 64).round() / 64                       # products and sums without an error
+    for temperature in (0.0, 0.9):
+        got = ops.vocab_scores(x, w, temperature=temperature, seed=5)
+        z = (x.double() @ w.double().t()).float()
+        assert (got.lse - z.double().logsumexp(-1)).abs().max() < 32 * 2 ** -23 + 2 ** -20
+        few = ops.vocab_scores(x[:16], w, temperature=temperature, seed=5)
+        assert got.pick[:16].equal(few.pick)
+        if temperature == 0:
+            first = torch.where(z == z.amax(-1, keepdim=True), torch.arange(60000, device=cuda), 60000).amin(-1)
+            assert got.pick.equal(first.int())
+
+
 @pytest.mark.parametrize("rows,vocab", [(2, 30), (17, 33), (128, 4096), (129, 100), (700, 12345), (1300, 64), (2500, 999)])
 def test_however_it_is_cut(cuda, rows, vocab):
     rng, x, w = _inputs(cuda, rows, 80, vocab, seed=rows)
