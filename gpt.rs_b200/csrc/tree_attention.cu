@@ -62,8 +62,6 @@ struct Item { int parts, row0, nodes, head, tile, pad[3]; };
 struct AttentionParams {
     CUtensorMap map, q_map;
     DraftTrees t;
-    const __nv_bfloat16* q;
-    long long ldq;
     const unsigned char* pool;
     __nv_bfloat16* out;
     Item* items;                 // [groups tiles], where a second kernel joins the parts; NULL: the warps do
@@ -74,7 +72,7 @@ struct AttentionParams {
     float scale_log2;
     int groups, tiles, row_cap;  // tiles: of a group, 1 or 2
     int tile_nodes;              // of a tile: as many as 128 rows hold
-    int cluster, most_tiles;     // small calls: CTAs of a tile; tiles that a tree may have
+    int cluster;                 // small calls: CTAs of a tile
     uint32_t wait_limit;
     int starve;
 };
@@ -1088,26 +1086,25 @@ int gptrs_cuda_tree_attention(const gptrs_draft_trees* t, const gptrs_tree_atten
     GPTRS_REQUIRE(s && s->d_pool && s->d_status && (t->rows == 0 || (s->d_q && s->d_out)), "null pointer");
     GPTRS_REQUIRE(aligned16(s->d_q) && aligned16(s->d_pool) && aligned16(s->d_out) && aligned16(s->d_scratch), "pointers must be 16-byte aligned");
     const int64_t width = (int64_t)t->q_heads * kTreeDim;
-    p.ldq = s->ldq ? s->ldq : width;
-    GPTRS_REQUIRE(p.ldq >= width && p.ldq % 8 == 0 && p.ldq < ((int64_t)1 << 31), "rows of queries overlap, or do not start at multiples of 16 bytes");
+    const int64_t ldq = s->ldq ? s->ldq : width;
+    GPTRS_REQUIRE(ldq >= width && ldq % 8 == 0 && ldq < ((int64_t)1 << 31), "rows of queries overlap, or do not start at multiples of 16 bytes");
     GPTRS_REQUIRE(t->n_pages * t->kv_heads * 2 * kTreePage < ((int64_t)1 << 31), "the pool has too many pages");
     GPTRS_REQUIRE(t->max_pages * kTreePage / kKeys + 8 < (((int64_t)1 << 31) / ceil_div(t->max_nodes, kRows / (t->q_heads / t->kv_heads)) / t->kv_heads), "the page table is too long for so many rows");
     const size_t scratch = gptrs_cuda_tree_scratch_bytes(t);
     GPTRS_REQUIRE(scratch == 0 || (s->d_scratch && s->scratch_bytes >= scratch), "scratch is too small");
     if (t->rows == 0) return GPTRS_OK;
     const char *q = static_cast<const char*>(s->d_q), *out = static_cast<const char*>(s->d_out);
-    GPTRS_REQUIRE(out >= q + 2 * ((t->rows - 1) * p.ldq + width) || q >= out + 2 * t->rows * width, "the output lies in rows of queries");
+    GPTRS_REQUIRE(out >= q + 2 * ((t->rows - 1) * ldq + width) || q >= out + 2 * t->rows * width, "the output lies in rows of queries");
     static PerDeviceOnce attr_once;
     if (attr_once.first_time()) {
         GPTRS_CUDA_OK(cudaFuncSetAttribute(tree_attention_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
         GPTRS_CUDA_OK(cudaFuncSetAttribute(tree_attention_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
     }
     const Cut c = cut(t);
-    p.cluster = c.cluster; p.groups = c.groups; p.tiles = c.tiles; p.row_cap = c.row_cap; p.tile_nodes = c.tile_nodes; p.most_tiles = c.most_tiles;
+    p.cluster = c.cluster; p.groups = c.groups; p.tiles = c.tiles; p.row_cap = c.row_cap; p.tile_nodes = c.tile_nodes;
     int bad = encode_pool(s->d_pool, p.t, &p.map);
-    if (!bad) bad = encode_queries(s->d_q, p.ldq, p.t, p.tile_nodes, &p.q_map);
+    if (!bad) bad = encode_queries(s->d_q, ldq, p.t, p.tile_nodes, &p.q_map);
     if (bad) return bad;
-    p.q = static_cast<const __nv_bfloat16*>(s->d_q);
     p.pool = static_cast<const unsigned char*>(s->d_pool);
     p.out = static_cast<__nv_bfloat16*>(s->d_out);
     p.status = s->d_status;
