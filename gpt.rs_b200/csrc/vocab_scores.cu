@@ -34,10 +34,11 @@ enum { kFew, kOne, kPairs };
 constexpr int kCols = 256;                      // most tokens of a tile
 constexpr int kMostStages = 16;                 // (as many as fit: narrow tiles have small stages, and need more of them under way)
 constexpr int x_bytes(int mode) { return 128 * (mode == kFew ? 64 : 128); }        // of a stage; products of 64 rows where there are 16 at most
-// Stages that an accumulator adds up. 128 of dim where w's bytes bound the call, 512 where the products do and each handing over takes time from them: relative errors of lse
-// at a dim of 4096 1.0e-7 and 4.0e-7 (f32 sums one by one 5.8e-7), of 4001 rows in 131072 tokens 1.72 ms with 256, 1.54 with 512. 256 up to 16 rows: one row of 50257 x 2048 whose
-// lse is about 15 41.0 us and 2.5e-6 off, with 128 42.1 and 1.3e-6, with 64 44.1 and 0.9e-6 (f32 sums in an order of their own 0.6e-6; a step of f32 is 0.95e-6).
-constexpr int drain_of(int mode) { return mode == kPairs ? 8 : mode == kFew ? 4 : 2; }
+// Stages that an accumulator adds up: 128 of dim where w's bytes bound the call, 512 where the products do and each handing over takes time from them. The cuts go one way: sums of products
+// of one sign come out low by 2.8, 6.4 and 15 times 2^-24 of themselves with 128, 256 and 512 of dim (f32 sums in an order of their own are off by 0.7 either way). Of logits that are not, relative
+// errors of lse at a dim of 4096 are 1.0e-7 and 4.0e-7 with 128 and 512 (f32 sums one by one 5.8e-7); 4001 rows in 131072 tokens take 1.72 ms with 256, 1.54 with 512. One row of
+// 50257 x 2048 whose lse is about 15 takes 41.7 us and is 1.3e-6 off, with 256 40.6 and 2.5e-6, with 64 43.7 and 0.9e-6 (f32 sums 0.6e-6; a step of f32 is 0.95e-6); one of 4000 x 4096 27, 23 and 33 us.
+constexpr int drain_of(int mode) { return mode == kPairs ? 8 : 2; }
 constexpr int kEpilogue = 256, kThreads = kEpilogue + 128;   // two warps of the last four only make their group whole
 // Registers of a thread at launch, and what the groups of four warps make of them: the shares add up to less than the block has, so every request ends.
 constexpr int kLaunchRegs = 168, kEpilogueRegs = 208, kOtherRegs = 80;

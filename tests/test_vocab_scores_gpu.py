@@ -294,6 +294,20 @@ def test_several_accumulators_to_a_tile(cuda, rows, dim, vocab, temperature):
     _check(got, x, w, target, temperature=temperature, seed=31)
 
 
+@pytest.mark.parametrize("rows", [1, 16, 100])
+@pytest.mark.parametrize("dim", [2048, 4096])
+def test_sums_are_read_out_every_128_of_dim(cuda, rows, dim):
+    """Products of one sign, one token, so that lse is its logit. An accumulator cuts each of its eight sums S j / 8 by at most a step of f32, half of one on the average, so 2^-24 (1 + ... + 8) / 8
+    = 4.5 2^-24 of the logit; what is added in f32 is rounded either way. Five standard deviations of the mean on top (a logit's: below 2 2^-24)."""
+    low, n = 0.0, 3200 // rows
+    gen = torch.Generator(device=cuda).manual_seed(rows)
+    for _ in range(n):
+        x, w = (torch.randn((k, dim), device=cuda, generator=gen).abs().bfloat16() for k in (rows, 1))
+        z = (x.double() @ w.double().t())[:, 0]
+        low += float(((z - ops.vocab_scores(x, w).lse.double()) / z).mean()) / n
+    assert abs(low) <= (4.5 + 5 * 2 / (n * rows) ** 0.5) * 2 ** -24
+
+
 def test_many_tiles_of_several_accumulators(cuda):
     """Several row tiles and tiles of tokens to a pair of CTAs, each of several accumulators. Logits are multiples of 2^-8 that f32 holds, so they are without an error, and lse is off by its own
     rounding and that of m, 2^-23 lse (below 32), and by the exponentials', 2^-20."""
