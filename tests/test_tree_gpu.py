@@ -364,6 +364,25 @@ def test_attention_parts_whose_scores_are_all_minus_infinity(cuda, heads, kv, tr
         t.check(got, q)
 
 
+@pytest.mark.parametrize("at", ["first", "root"])
+@pytest.mark.parametrize("heads,kv,trees,nodes,lengths", MINUS_INFINITY)
+def test_attention_a_score_that_is_nan_reaches_its_rows_from_any_part(cuda, heads, kv, trees, nodes, lengths, at):
+    """Beside scores of -inf in its part, and finite ones in others."""
+    rng = np.random.default_rng(nodes)
+    t = Trees(cuda, heads, kv, [(lengths[min(s, 1)], bushy(nodes, rng)) for s in range(trees)], seed=lengths[0])
+    q = t.queries()
+    q[..., 3] = q[..., 3].abs() + 0.5
+    for s, (n, _) in enumerate(t.forest):
+        bad = 0 if at == "first" else n
+        t.kvs[s][0, max(0, bad - 70):bad + 70, ..., 3] = -np.inf
+        t.kvs[s][0, bad, 0, 3] = np.nan                                    # kv head 0
+        t.write(s, np.arange(t.kvs[s].shape[1]), torch.tensor(t.kvs[s], dtype=torch.float32).bfloat16())
+    got = t.attention(q).view(t.rows, kv, -1)
+    assert got[:, 0].isnan().all()
+    if kv > 1 and lengths[1] > 200:
+        assert torch.isfinite(got[:, 1:]).all()
+
+
 @pytest.mark.parametrize("heads,kv,forest", [(8, 2, [(20, 9), (3, 2), (0, 40)]), (32, 8, [(900, 26)]), (8, 8, [(300, 7)] * 30), (4, 1, [(500, 200)] * 2), (2, 1, [(20000, 3)] + [(300, 3)] * 79),
                                              (2, 1, [(30000, 3)])])
 def test_attention_loses_no_more_than_the_rounding_of_its_results(cuda, heads, kv, forest):
