@@ -21,9 +21,10 @@
 // tile), a share of its keys each, and joins through distributed shared memory: nothing has to be added up or looked for in front.
 //
 // What bounds it (times of the kernels in a graph; calls from Python take 2 to 50 us more), 32 / 8 heads: 64 trees of 32 nodes at 512 to 8192 tokens 236 us for the 1.18 GB of the
-// cache (181 at the rate of a copy), two trees at 100003 and 131072 175 us (145): HBM, the wait for the products in front of a stage's reuse, and the joins at the end. Where rows share
-// keys (six trees of 250 nodes at 700 to 4000, 16 / 2 heads, 75 to 80 us) the softmax warps: 64 exponentials a thread and block, four lanes a cycle and scheduler, take 1024 cycles
-// for the two warps that a scheduler has. One tree of 26 nodes at 1500 tokens 13.0 us, a chain of latencies: tree, table, pages, three blocks of the CTA's share, and
+// cache (181 at the rate of a copy), two trees at 100003 and 131072 175 us (145): HBM, the wait for the products in front of a stage's reuse, and the joins at the end. A block takes
+// the softmax warps 1800 to 2100 cycles, of which 64 exponentials a thread, four lanes a cycle and scheduler, are 1024 for the two warps that a scheduler has. Where rows share keys (six trees
+// of 250 nodes at 700 to 4000, 16 / 2 heads, 67 to 80 us) that is half of it: of the 82 to 114 thousand cycles of a CTA 43 to 57 are the softmax of 22 to 28 blocks, 9 to 13 waits for
+// scores, 8 to 49 the ends of its pieces, where parts are joined; some CTAs have nothing, where the second tile of a pair is one too many. One tree of 26 nodes at 1500 tokens 13.0 us, a chain of latencies: tree, table, pages, three blocks of the CTA's share, and
 // the cluster's join. Two threads to a row took 284 us where one took 207 (a barrier every block).
 // Every wait is bounded: on a timeout code 3 goes to the status word, the roles leave their loops, tensor memory is freed.
 #include "draft_tree.cuh"

@@ -37,7 +37,8 @@ struct AppendParams {
 // A CTA per node. A thread takes two chunks of eight channels of a head: a pair that rotates together (c, c + half / 8), or two that stay. Rows, parents and the page are asked for
 // together, in front of the walk up the tree (shared reads, where global ones would wait for each other): what bounds a small call is the two trips to memory, tree and row.
 // 64 trees of 20 to 64 nodes, 32 / 8 heads: 14.3 us, 10 at the rate of a copy (256 threads, two tasks in front 16.2; with the rows behind
-// the walk 17.5; 64 threads 14.3); one tree of 26 nodes 2.7, a launch (64 threads 3.7).
+// the walk 17.5; 64 threads 14.3); one tree of 26 nodes 2.7, a launch (64 threads 3.7). 40 / 8, 64 / 8 and 12 / 12 heads 16.6, 21.5 and 12.4: tasks beyond three a thread, 48 heads, are
+// loaded behind the walk. (Kernels in a graph; a call from Python by itself takes 2 us more.)
 constexpr int kAppendThreads = 128, kAhead = 3;   // tasks of a thread that are asked for in front
 __global__ void __launch_bounds__(kAppendThreads) tree_append_kernel(const AppendParams p) {
     __shared__ int up[kMostNodes];
@@ -123,7 +124,7 @@ struct AcceptParams {
 
 // A CTA per (layer, tree); each walks the tree by itself. The k-th node of the path comes from a place behind k (numbers grow along a path), so a thread that moves one column
 // of chunks in the order of k never reads what it has written. What bounds it is latency: loads of the walk, table, pool. 64 trees with nine nodes accepted, 26 layers, 8 kv heads 14.7
-// us (7.3 at the rate of a copy); one tree 3.9. Several layers to a CTA, so that fewer walk, 21.3.
+// us (7.3 at the rate of a copy); one tree 3.9 (kernels in a graph; a call from Python by itself takes 2 us more). Several layers to a CTA, so that fewer walk, 21.3.
 __global__ void __launch_bounds__(kThreads, 8) tree_accept_kernel(const AcceptParams p) {
     __shared__ int pick[kMostNodes], follow[kMostNodes], path[kMostNodes];
     __shared__ long long from[kMostNodes], to[kMostNodes];

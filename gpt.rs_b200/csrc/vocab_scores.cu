@@ -13,9 +13,11 @@
 // Units go row tile first, so that the CTAs that run at one time share stretches of w through L2. A second kernel joins the parts of a row; it compares tokens where
 // values are equal, so results do not depend on an order.
 //
-// What bounds it: up to 128 rows w's bytes (one row of 50257 x 2048 42 us, 31.5 at the rate of a copy; 16 rows of 131072 x 4096 165 us, 164). Above, the products: 4001 rows of
-// 131072 x 2048 1.39 to 1.55 ms as the power cap allows, the tensor pipe busy in 98 % of the cycles (1.26 at the rate of short products). 416 drawn rows of 131072 x 4096 405 to 420
-// us: they are two tiles of 256 (262 us for 416 rows, 322 for 512), and a draw costs a hash a logit.
+// What bounds it (times of the kernels in a graph; calls from Python by themselves take 2 to 60 us more): up to 128 rows w's bytes (one row of 50257 x 2048 42 us, 31.5 at the rate of a copy;
+// of 131072 x 4096 16 rows 164 us, 64 rows 184, drawn 234, 128 rows 192, drawn 250; 164). Above, the products: 4001 rows of 131072 x 2048 1.37 to 1.58 ms as the power cap allows, the tensor pipe
+// busy in 96 to 98 % of the cycles (1.26 at the rate of short products). 416 drawn rows of 131072 x 4096 415 to 440 us: they are two tiles of 256 (262 us for 416 rows, 322 for 512), and a
+// draw costs a hash a logit. Below a dim of some hundred, and with a cap, the epilogue: 2048 rows of 50257 x 320 96 us (39), 64 rows of 131072 x 2048 108 us, with a bias 121, with a
+// cap, which is a call and a tanhf a logit, 218 (82); 2048 rows 0.81, 0.97 and 1.50 ms (0.65). One row of 4000 x 4096 26 us (5): dim is walked over in order, by 125 CTAs of 32 tokens.
 // Every wait is bounded: on a timeout code 3 goes to the status word, the roles leave their loops, tensor memory is freed.
 #include <algorithm>
 

@@ -886,7 +886,8 @@ int gptrs_cuda_tree_accept(const gptrs_draft_trees* t, const gptrs_tree_accept_s
  *     logprob      z[target] - lse, the target's log-probability (the cross entropy with its sign turned); a negative target: 0; one behind the vocabulary: NaN and 2 in *d_status
  *     pick         the largest z (the first of equals), or with temperature > 0 the largest z / temperature + g, a draw from softmax(z / temperature):
  *                  (temperature 1e-20 .. 1e20) g = -log(-log(1 - v)), v = (h + 1/2) / 2^32 in f32 (1 - 2^-24 at most), h = mix(seed ^ mix(token + 0x9e3779b9 (row + 1))) with the 32-bit mix
- *                  x ^= x >> 16, x *= 0x7feb352d, x ^= x >> 15, x *= 0x846ca68b, x ^= x >> 16
+ *                  x ^= x >> 16, x *= 0x7feb352d, x ^= x >> 15, x *= 0x846ca68b, x ^= x >> 16. (gptrs_cuda_sample_rows draws from the same distribution with the same h, but takes
+ *                  g = -log(-log u), u from its upper 24 bits, which grows with h where this g falls: one seed gives other tokens there)
  *     pick_logprob z[pick] - lse
  * Every result is left out where its pointer is null. bf16 operands, products summed in f32. A bias is finite, or -inf: such a token has no probability, with a cap either (where no
  * token has one: lse -inf, pick 0, log-probabilities NaN). NaN in a row's hidden state makes its lse and log-probabilities NaN, and its pick a token of the vocabulary. dim and both strides are multiples of 8, hidden and weight 16-byte aligned. Waits inside the kernel are bounded (3
